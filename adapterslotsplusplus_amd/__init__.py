@@ -5,6 +5,6 @@ the compute runs in libwarppipe_mi355x.so (hand-written HIP kernels, C ABI in
 include/warppipe_mi355x.h).
 """
 from .config import WarpPipeConfig
-from .engine import WarpPipeEngine
+from .engine import TokenLogprobs, WarpPipeEngine
 
-__all__ = ["WarpPipeConfig", "WarpPipeEngine"]
+__all__ = ["TokenLogprobs", "WarpPipeConfig", "WarpPipeEngine"]

@@ -25,6 +25,10 @@ WP_ERR_STATE = -6
 
 WP_DTYPE_F16 = 0
 WP_DTYPE_BF16 = 1
+WP_DTYPE_F32 = 2  # token_logprobs only
+
+# enum wp_activation.
+ACTIVATIONS = {"none": 0, None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 # Bits of the device error word (wp_types.h DeviceError).
 DEVICE_ERR_ID_RANGE = 1
@@ -44,6 +48,7 @@ EXPORTED = (
     "wp_shrink_expand_slices", "wp_linear_lora", "wp_read_probe",
     "wp_set_max_adapters", "wp_read_static_errors", "wp_poll_device_errors", "wp_lora_shrink", "wp_lora_expand",
     "wp_add_bias", "wp_handoff_probe", "wp_barrier_probe", "wp_shrink_new",
+    "wp_linear", "wp_packed_attention", "wp_token_logprobs",
 )
 
 
@@ -120,6 +125,10 @@ def load():
                            ctypes.c_int),
         "wp_add_bias": ([p, p, i64, i32, p, p, p, p, i32, i64, i32, p], ctypes.c_int),
         "wp_handoff_probe": ([p, i64, p, i64, p, i64, p, p, i32, i32, i32, p], ctypes.c_int),
+        "wp_linear": ([p, p, i64, p, i64, p, i64, p, p, i64, i32, i32, i32, i32, i64, i32, p], ctypes.c_int),
+        "wp_packed_attention": ([p, p, p, p, p, p, p, p, p, p, p, p, i32, i64, i64, i32, i32, i32, f32, i32, i32, i32, p],
+                                ctypes.c_int),
+        "wp_token_logprobs": ([p, p, p, p, p, p, p, i64, p, i32, i64, i32, i32, i32, p], ctypes.c_int),
         "wp_barrier_probe": ([p, i32, i32, i32, p, p], ctypes.c_int),
     }
     for name, (args, res) in sig.items():

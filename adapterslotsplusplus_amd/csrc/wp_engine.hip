@@ -34,6 +34,7 @@
 
 #include "../../include/warppipe_mi355x.h"
 #include "wp_apply.h"
+#include "wp_model.h"
 
 using namespace wp;
 
@@ -239,6 +240,8 @@ struct wp_engine {
   uint32_t* retired = nullptr;  // [num_staging_slots] highest released generation per slot
   uint32_t* lin_cnt = nullptr;  // [kLinCounters] column-tile counters of linear_lora (zero between calls)
   uint32_t* lin_flag = nullptr; // [2][block_cap] H flags and their reader counts (zero between calls)
+  uint32_t* model_cnt = nullptr;  // [kModelCounters] tile counters of linear / packed_attention / token_logprobs (zero between calls)
+  float* mpart = nullptr;       // [kModelPartBytes] their fp32 partials (no invariant)
   Entry* dtable = nullptr;      // [table_cap] id-indexed adapter table of build_seg_bounds plans
   Entry* bentries = nullptr;    // [block_cap] a build_seg_bounds plan's copy of each block's table entry
   // The second table of build_seg_bounds plans over more than kSmallPlanTokens
@@ -790,6 +793,7 @@ int wp_create(const wp_config* cfg_in, wp_engine** out) {
   const size_t o_pub = carve(sizeof(SlotPub) * std::max(cfg.num_staging_slots, 1));
   const size_t o_ret = carve(sizeof(uint32_t) * std::max(cfg.num_staging_slots, 1));
   const size_t o_lin = carve(sizeof(uint32_t) * (kLinCounters + 2 * static_cast<size_t>(e->block_cap)));
+  const size_t o_mcnt = carve(sizeof(uint32_t) * kModelCounters);
   const size_t o_tab = carve(sizeof(Entry) * std::max(e->table_cap, 1));
   const size_t o_bent = carve(sizeof(Entry) * e->block_cap);
   const size_t o_fblk = carve(sizeof(Block) * e->block_cap);
@@ -799,6 +803,7 @@ int wp_create(const wp_config* cfg_in, wp_engine** out) {
   const size_t o_spart = carve(sizeof(float) * kMaxChunks * static_cast<size_t>(e->tok_cap) * kMaxRank);
   const size_t hbuf_bytes = sizeof(uint16_t) * static_cast<size_t>(e->tok_cap) * kMaxSlices * kMaxRank;
   const size_t o_hbuf = carve(hbuf_bytes);
+  const size_t o_mpart = carve(kModelPartBytes);
   if (hipMalloc(reinterpret_cast<void**>(&e->ws), off) != hipSuccess)
     return bail(fail(WP_ERR_HIP, "wp_create: workspace allocation (%zu bytes) failed", off));
   e->header = reinterpret_cast<uint32_t*>(e->ws + o_hdr);
@@ -812,6 +817,8 @@ int wp_create(const wp_config* cfg_in, wp_engine** out) {
   e->retired = reinterpret_cast<uint32_t*>(e->ws + o_ret);
   e->lin_cnt = reinterpret_cast<uint32_t*>(e->ws + o_lin);
   e->lin_flag = e->lin_cnt + kLinCounters;
+  e->model_cnt = reinterpret_cast<uint32_t*>(e->ws + o_mcnt);
+  e->mpart = reinterpret_cast<float*>(e->ws + o_mpart);
   e->dtable = reinterpret_cast<Entry*>(e->ws + o_tab);
   e->bentries = reinterpret_cast<Entry*>(e->ws + o_bent);
   e->fblocks = reinterpret_cast<Block*>(e->ws + o_fblk);
@@ -822,7 +829,8 @@ int wp_create(const wp_config* cfg_in, wp_engine** out) {
   e->part = reinterpret_cast<float*>(e->ws + o_part);
   // Everything before the partials starts at zero, the partials at
   // kPartialEmpty, the publications' ids at -1 (nothing published); the d-range
-  // partials of shrink() and the H rows behind them need no state.  Filled by
+  // partials of shrink(), the H rows behind them and the partials of the
+  // operators around the apply need no state.  Filled by
   // kernels, then waited for.
   if (launch_fill_u32(reinterpret_cast<uint32_t*>(e->ws), 0u, o_part / 4, nullptr) != hipSuccess ||
       launch_fill_u32(reinterpret_cast<uint32_t*>(e->part), kPartialEmpty, e->part_words, nullptr) != hipSuccess)
@@ -2445,6 +2453,156 @@ int wp_read_probe(wp_engine* e, const void* buffer, int64_t bytes, void* sink, v
 int wp_set_spin_limit(wp_engine* e, uint32_t polls) {
   if (!e) return fail(WP_ERR_INVALID, "set_spin_limit: engine is NULL");
   e->spin_limit = polls == 0xFFFFFFFFu ? kDefaultSpinLimit : polls;
+  return WP_OK;
+}
+
+}  // extern "C"
+
+// ============================================================================
+// The operators around the apply: projections with their epilogue, packed
+// attention, token log probabilities.  No segment table is involved; partials
+// and counters are the engine's, so calls of one engine stay ordered by the
+// caller as everywhere else.
+// ============================================================================
+
+extern "C" {
+
+int wp_linear(wp_engine* e, void* y, int64_t y_row_stride, const void* x, int64_t x_row_stride, const void* w,
+              int64_t w_row_stride, const void* bias, const void* residual, int64_t residual_row_stride,
+              int32_t activation, int32_t gated, int32_t d_in, int32_t d_out, int64_t T, int32_t dtype, void* stream) {
+  const char* who = "linear";
+  if (!e) return fail(WP_ERR_INVALID, "%s: engine is NULL", who);
+  if (dtype != WP_DTYPE_F16 && dtype != WP_DTYPE_BF16) return fail(WP_ERR_INVALID, "%s: dtype must be fp16 or bf16", who);
+  if (activation < kActNone || activation > kActSilu) return fail(WP_ERR_INVALID, "%s: unknown activation %d", who, activation);
+  if (T < 0 || d_in < 0 || d_out < 1 || d_in > (1 << 24) || d_out > (1 << 28) || T > (int64_t(1) << 31))
+    return fail(WP_ERR_INVALID, "%s: bad sizes (tokens %lld, d_in %d, d_out %d)", who, (long long)T, d_in, d_out);
+  if (T == 0) return WP_OK;
+  if (!y || (d_in > 0 && (!x || !w))) return fail(WP_ERR_INVALID, "%s: null x, weight or y", who);
+  if (!aligned(x, 2) || !aligned(w, 2) || !aligned(y, 2) || !aligned(bias, 2) || !aligned(residual, 2))
+    return fail(WP_ERR_INVALID, "%s: tensors must be 2-byte aligned", who);
+  if (y_row_stride < d_out) return fail(WP_ERR_INVALID, "%s: y row stride %lld < d_out", who, (long long)y_row_stride);
+  if (w_row_stride < 0 || x_row_stride < 0 || (residual && residual_row_stride < 0))
+    return fail(WP_ERR_INVALID, "%s: negative row stride", who);
+  if (w_row_stride > (1 << 22) || x_row_stride > (1 << 22))
+    return fail(WP_ERR_INVALID, "%s: x and weight rows must be at most 4194304 elements apart", who);
+  ProjArgs a{};
+  a.x = x;
+  a.w = w;
+  a.bias = bias;
+  a.residual = residual;
+  a.y = y;
+  a.ldx = x_row_stride;
+  a.ldw = w_row_stride;
+  a.ldr = residual_row_stride;
+  a.ldy = y_row_stride;
+  a.tokens = T;
+  a.d_in = d_in;
+  a.n_out = d_out;
+  a.act = activation;
+  a.gated = gated ? 1 : 0;
+  a.part = e->mpart;
+  a.part_bytes = kModelPartBytes;
+  a.tile_cnt = e->model_cnt;
+  a.n_cnt = kModelCounters;
+  DeviceGuard g(e->device);
+  WP_HIP(launch_proj(dtype == WP_DTYPE_BF16, a, e->n_cu, static_cast<hipStream_t>(stream)));
+  return WP_OK;
+}
+
+int wp_packed_attention(wp_engine* e, void* out, const int64_t* out_strides, float* lse, const void* q,
+                        const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, const int32_t* cu_q, const int32_t* cu_k, int32_t n_seq,
+                        int64_t tokens, int64_t keys, int32_t heads, int32_t kv_heads, int32_t head_dim, float scale,
+                        int32_t causal, int32_t window, int32_t dtype, void* stream) {
+  const char* who = "packed_attention";
+  if (!e) return fail(WP_ERR_INVALID, "%s: engine is NULL", who);
+  if (dtype != WP_DTYPE_F16 && dtype != WP_DTYPE_BF16) return fail(WP_ERR_INVALID, "%s: dtype must be fp16 or bf16", who);
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || heads > 65535)
+    return fail(WP_ERR_INVALID, "%s: %d query heads do not share %d key heads evenly", who, heads, kv_heads);
+  if (head_dim < 8 || head_dim > kMaxHeadDim || head_dim % 8 != 0)
+    return fail(WP_ERR_INVALID, "%s: head size %d (a multiple of 8 up to %d)", who, head_dim, kMaxHeadDim);
+  if (tokens < 0 || keys < 0 || n_seq < 0 || tokens > 0x7FFFFFFF || keys > 0x7FFFFFFF)
+    return fail(WP_ERR_INVALID, "%s: bad sizes (tokens %lld, keys %lld, sequences %d)", who, (long long)tokens,
+                (long long)keys, n_seq);
+  if (window < 0 || (window > 0 && !causal)) return fail(WP_ERR_INVALID, "%s: a window must be positive, and causal", who);
+  if (!out_strides || !q_strides || !k_strides || !v_strides) return fail(WP_ERR_INVALID, "%s: null strides", who);
+  if (tokens == 0) return WP_OK;
+  if (!out || !q || (keys > 0 && (!k || !v)) || (n_seq > 0 && (!cu_q || !cu_k)))
+    return fail(WP_ERR_INVALID, "%s: null tensor", who);
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || !aligned(lse, 4) ||
+      !aligned(cu_q, 4) || !aligned(cu_k, 4))
+    return fail(WP_ERR_INVALID, "%s: q, k, v and out must be 16-byte aligned", who);
+  for (int i = 0; i < 2; ++i)
+    for (const int64_t* s : {q_strides, k_strides, v_strides, out_strides})
+      if (s[i] < 0 || s[i] % 8 != 0 || s[i] > (int64_t(1) << 22))
+        return fail(WP_ERR_INVALID, "%s: token and head strides must be multiples of 8 elements (got %lld)", who,
+                    (long long)s[i]);
+  AttnArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.lse = lse;
+  a.cu_q = cu_q;
+  a.cu_k = cu_k;
+  a.q_tok = q_strides[0];
+  a.q_head = q_strides[1];
+  a.k_tok = k_strides[0];
+  a.k_head = k_strides[1];
+  a.v_tok = v_strides[0];
+  a.v_head = v_strides[1];
+  a.o_tok = out_strides[0];
+  a.o_head = out_strides[1];
+  a.tokens = tokens;
+  a.keys = keys;
+  a.n_seq = n_seq;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.dim = head_dim;
+  a.scale = scale;
+  a.causal = causal ? 1 : 0;
+  a.window = window;
+  DeviceGuard g(e->device);
+  WP_HIP(launch_attention(dtype == WP_DTYPE_BF16, a, e->n_cu, static_cast<hipStream_t>(stream)));
+  return WP_OK;
+}
+
+int wp_token_logprobs(wp_engine* e, float* logprobs, float* entropy, int32_t* ranks, float* top_logprobs,
+                      int32_t* top_ids, const void* logits, int64_t logits_row_stride, const void* token_ids,
+                      int32_t ids_are_int64, int64_t rows, int32_t vocab, int32_t top, int32_t dtype, void* stream) {
+  const char* who = "token_logprobs";
+  if (!e) return fail(WP_ERR_INVALID, "%s: engine is NULL", who);
+  if (dtype != WP_DTYPE_F16 && dtype != WP_DTYPE_BF16 && dtype != WP_DTYPE_F32)
+    return fail(WP_ERR_INVALID, "%s: dtype must be fp16, bf16 or fp32", who);
+  if (rows < 0 || rows > 0x7FFFFFFF || vocab < 1) return fail(WP_ERR_INVALID, "%s: bad sizes (rows %lld, vocabulary %d)", who,
+                                                              (long long)rows, vocab);
+  if (top < 0 || top > kMaxTop || top > vocab)
+    return fail(WP_ERR_INVALID, "%s: %d alternatives (0 to %d, and at most the vocabulary)", who, top, kMaxTop);
+  if (logits_row_stride < 0) return fail(WP_ERR_INVALID, "%s: negative row stride", who);
+  if (rows == 0) return WP_OK;
+  if (!logprobs || !entropy || !ranks || !logits || !token_ids || (top > 0 && (!top_logprobs || !top_ids)))
+    return fail(WP_ERR_INVALID, "%s: null tensor", who);
+  if (!aligned(logits, dtype == WP_DTYPE_F32 ? 4 : 2) || !aligned(token_ids, ids_are_int64 ? 8 : 4) ||
+      !aligned(logprobs, 4) || !aligned(entropy, 4) || !aligned(ranks, 4) || !aligned(top_logprobs, 4) ||
+      !aligned(top_ids, 4))
+    return fail(WP_ERR_INVALID, "%s: tensors must be aligned to their elements", who);
+  LogprobArgs a{};
+  a.logits = logits;
+  a.ids = token_ids;
+  a.ids64 = ids_are_int64 ? 1 : 0;
+  a.dtype = dtype;
+  a.rows = rows;
+  a.ld = logits_row_stride;
+  a.vocab = vocab;
+  a.top = top;
+  a.logprobs = logprobs;
+  a.entropy = entropy;
+  a.ranks = ranks;
+  a.top_lp = top_logprobs;
+  a.top_ids = top_ids;
+  a.header = e->header;
+  DeviceGuard g(e->device);
+  WP_HIP(launch_logprobs(a, e->n_cu, static_cast<hipStream_t>(stream)));
   return WP_OK;
 }
 

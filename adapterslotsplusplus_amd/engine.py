@@ -28,7 +28,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
-from typing import List, Optional, Sequence, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -67,6 +67,15 @@ def _i64s(v) -> bytes:
 
 def _i32s(v) -> bytes:
     return struct.pack(f"{len(v)}I", *[k & 0xFFFFFFFF for k in v])
+
+
+class TokenLogprobs(NamedTuple):
+    """What token_logprobs returns, per row of the logits."""
+    logprobs: torch.Tensor      # [rows] fp32: log softmax at the given token
+    entropy: torch.Tensor       # [rows] fp32, in nats
+    ranks: torch.Tensor         # [rows] int32: 1 + how many logits are greater than the token's
+    top_logprobs: torch.Tensor  # [rows, top] fp32, the largest first
+    top_ids: torch.Tensor       # [rows, top] int32
 
 
 class _Ext:
@@ -719,6 +728,161 @@ class WarpPipeEngine:
                                       bias_strides, L, rank, T, 1 if add_inputs else 0, dt,
                                       _raw_stream(self._dev_index))
         return _lib.check(rc, "lora_expand") == _lib.WP_OK
+
+    # ---------------------------------------- operators around the apply --
+    # What a model computes between its LoRA deltas (not in the reference,
+    # whose models run them in vLLM or torch).  They need no segment table.
+
+    def linear(self, x, weight, bias=None, residual=None, activation="none", gated=False, out=None):
+        """y = rn(act(x . W^T + bias) + residual), accumulated in fp32 and rounded
+        once.  x [..., in] and weight [out, in] (unit column stride); bias
+        [out]; residual [..., out]; activation "none", "relu", "gelu" (by the
+        error function), "gelu_tanh" or "silu".  gated: weight [2 * out, in]
+        holds the gate's rows and then the up projection's (bias [2 * out]
+        likewise), and y = rn(act(gate) * up + residual).  Returns y
+        [..., out], new unless `out` ([tokens, out], rows any distance apart)
+        is given; residual may be out."""
+        dev = self._dev_index
+        for t, nm in ((x, "x"), (weight, "weight"), (bias, "bias"), (residual, "residual"), (out, "out")):
+            if t is not None and t.get_device() != dev:
+                self._on_device(t, nm)
+        dtype = x.dtype
+        dt = _DTYPES.get(dtype)
+        if dt is None:
+            dt = _dtype_code(x, "x")
+        act = _lib.ACTIVATIONS.get(activation)
+        if act is None:
+            raise RuntimeError(f"linear: unknown activation {activation!r}")
+        if weight.dtype != dtype or (bias is not None and bias.dtype != dtype) or (
+                residual is not None and residual.dtype != dtype):
+            raise RuntimeError("linear: x, weight, bias and residual must share one dtype")
+        rows, d_in = weight.shape if weight.dim() == 2 else (0, -1)
+        if x.dim() < 1 or x.size(-1) != d_in:
+            raise RuntimeError(f"linear: weight {tuple(weight.shape)} must be [out, in] with x's width, x is "
+                               f"{tuple(x.shape)}")
+        if gated and rows % 2:
+            raise RuntimeError("linear: a gated weight holds as many gate rows as up rows")
+        n = rows // 2 if gated else rows
+        if n < 1:
+            raise RuntimeError("linear: weight has no rows")
+        if d_in > 1 and weight.stride(1) != 1:
+            raise RuntimeError("linear: weight must have unit column stride")
+        x2 = x if x.dim() == 2 else x.reshape(-1, d_in)
+        if d_in > 1 and x2.stride(1) != 1:
+            x2 = x2.contiguous()
+        T = x2.size(0)
+        if bias is not None and (bias.dim() != 1 or bias.size(0) != rows or (rows > 1 and bias.stride(0) != 1)):
+            raise RuntimeError(f"linear: bias must be a contiguous [{rows}] tensor")
+        ldr = 0
+        if residual is not None:
+            if residual.shape[-1:] != (n,) or residual.numel() != T * n:
+                raise RuntimeError(f"linear: residual {tuple(residual.shape)} does not match the output [{T}, {n}]")
+            if residual.dim() != 2:
+                residual = residual.reshape(-1, n)
+            if n > 1 and residual.stride(1) != 1:
+                residual = residual.contiguous()
+            ldr = residual.stride(0)
+        y = torch.empty(T, n, dtype=dtype, device=x.device) if out is None else out
+        if out is not None and (out.dim() != 2 or out.shape != (T, n) or out.dtype != dtype
+                                or (n > 1 and out.stride(1) != 1) or (T > 1 and out.stride(0) < n)):
+            raise RuntimeError(f"linear: out must be a [{T}, {n}] tensor of x's dtype with unit column stride")
+        rc = self._lib.wp_linear(self._handle, y.data_ptr(), max(y.stride(0), n), x2.data_ptr(), x2.stride(0),
+                                 weight.data_ptr(), weight.stride(0), None if bias is None else bias.data_ptr(),
+                                 None if residual is None else residual.data_ptr(), ldr, act, 1 if gated else 0, d_in, n,
+                                 T, dt, _raw_stream(dev))
+        _lib.check(rc, "linear")
+        return y if x.dim() == 2 or out is not None else y.view(*x.shape[:-1], n)
+
+    def packed_attention(self, q, k, v, cu_seqlens_q, cu_seqlens_k=None, scale=None, causal=True, window=0, out=None,
+                         return_lse=False):
+        """softmax(scale * q . k) . v over packed sequences of different lengths.
+        q [tokens, heads, dim]; k and v [keys, kv_heads, dim] (heads a multiple
+        of kv_heads, dim a multiple of 8 up to 128); views with other token
+        and head strides (a packed q/k/v projection, a cache) are read as they
+        are.  cu_seqlens_q, cu_seqlens_k: int32 [n + 1] bounds on the device;
+        sequence b has queries [cu_seqlens_q[b], cu_seqlens_q[b + 1]) and keys
+        [cu_seqlens_k[b], cu_seqlens_k[b + 1]) (None: the same bounds), its
+        last query at its last key.  causal: a query sees keys up to its own
+        position, with window > 0 only the last `window` of them.  scale:
+        dim ** -0.5 unless given.  Returns out [tokens, heads, dim], or (out,
+        lse [tokens, heads] fp32) with return_lse; queries that see no key, and
+        rows past the last bound, get 0 and -inf."""
+        dev = self._dev_index
+        if cu_seqlens_k is None:
+            cu_seqlens_k = cu_seqlens_q
+        for t, nm in ((q, "q"), (k, "k"), (v, "v"), (cu_seqlens_q, "cu_seqlens_q"), (cu_seqlens_k, "cu_seqlens_k")):
+            if t.get_device() != dev:
+                self._on_device(t, nm)
+        dtype = q.dtype
+        dt = _DTYPES.get(dtype)
+        if dt is None:
+            dt = _dtype_code(q, "q")
+        if k.dtype != dtype or v.dtype != dtype:
+            raise RuntimeError("packed_attention: q, k and v must share one dtype")
+        if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.size(2) != q.size(2):
+            raise RuntimeError(f"packed_attention: q must be [tokens, heads, dim], k and v [keys, kv_heads, dim]; got "
+                               f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+        T, heads, dim = q.shape
+        S, kv_heads = k.size(0), k.size(1)
+        n = cu_seqlens_q.numel() - 1
+        for cu in (cu_seqlens_q, cu_seqlens_k):
+            if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() != n + 1 or n < 0 or not cu.is_contiguous():
+                raise RuntimeError("packed_attention: cu_seqlens must be contiguous int32 [n + 1] tensors of one length")
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
+        if dim > 1 and (qs[2] != 1 or ks[2] != 1 or vs[2] != 1):
+            raise RuntimeError("packed_attention: a head's elements must be contiguous")
+        if out is None:
+            out = torch.empty(T, heads, dim, dtype=dtype, device=q.device)
+        else:
+            self._on_device(out, "out")
+            if out.shape != q.shape or out.dtype != dtype or out.stride(2) != 1:
+                raise RuntimeError("packed_attention: out must have q's shape and dtype, each head contiguous")
+        lse = torch.empty(T, heads, dtype=torch.float32, device=q.device) if return_lse else None
+        rc = self._lib.wp_packed_attention(
+            self._handle, out.data_ptr(), _i64s(out.stride()[:2]), None if lse is None else lse.data_ptr(),
+            q.data_ptr(), _i64s(qs[:2]), k.data_ptr(), _i64s(ks[:2]), v.data_ptr(), _i64s(vs[:2]),
+            cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), n, T, S, heads, kv_heads, dim,
+            dim ** -0.5 if scale is None else float(scale), 1 if causal else 0, int(window or 0), dt, _raw_stream(dev))
+        _lib.check(rc, "packed_attention")
+        return out if lse is None else (out, lse)
+
+    def token_logprobs(self, logits, token_ids, top=0) -> TokenLogprobs:
+        """What a model's logits say of given tokens, in one pass over them: per
+        row of logits [rows, vocab] (fp16, bf16 or fp32) the log softmax at
+        token_ids[row] (int32 or int64), the softmax's entropy, the token's rank
+        (1 + how many logits are greater), and the `top` (0 to 64) largest
+        logits' ids and log probabilities, equal ones by the lower id.  A token
+        id below 0 names no token (log probability and rank 0); one past the
+        vocabulary counts as none and sets device error 1.  A row that is all
+        -inf, or holds NaN or +inf, gives NaN."""
+        dev = self._dev_index
+        if logits.get_device() != dev or token_ids.get_device() != dev:
+            self._on_device(logits, "logits")
+            self._on_device(token_ids, "token_ids")
+        dt = _lib.WP_DTYPE_F32 if logits.dtype == torch.float32 else _DTYPES.get(logits.dtype)
+        if dt is None:
+            raise RuntimeError(f"logits must be fp16, bf16 or fp32, got {logits.dtype}")
+        if logits.dim() != 2 or (logits.size(1) > 1 and logits.stride(1) != 1):
+            raise RuntimeError("token_logprobs: logits must be [rows, vocab] with unit column stride")
+        rows, vocab = logits.shape
+        if token_ids.dtype not in (torch.int64, torch.int32) or token_ids.shape != (rows,) or not token_ids.is_contiguous():
+            raise RuntimeError(f"token_logprobs: token_ids must be a contiguous int32 or int64 [{rows}] tensor")
+        top = int(top)
+        if top < 0:
+            raise RuntimeError("token_logprobs: top must not be negative")
+        d = logits.device
+        got = TokenLogprobs(torch.empty(rows, dtype=torch.float32, device=d),
+                            torch.empty(rows, dtype=torch.float32, device=d),
+                            torch.empty(rows, dtype=torch.int32, device=d),
+                            torch.empty(rows, top, dtype=torch.float32, device=d),
+                            torch.empty(rows, top, dtype=torch.int32, device=d))
+        rc = self._lib.wp_token_logprobs(self._handle, got.logprobs.data_ptr(), got.entropy.data_ptr(),
+                                         got.ranks.data_ptr(), got.top_logprobs.data_ptr(), got.top_ids.data_ptr(),
+                                         logits.data_ptr(), logits.stride(0), token_ids.data_ptr(),
+                                         1 if token_ids.dtype == torch.int64 else 0, rows, vocab, top, dt,
+                                         _raw_stream(dev))
+        _lib.check(rc, "token_logprobs")
+        return got
 
     # ------------------------------------------------------------- staging --
     def prefetch_adapter(self, adapter_id, layer=None) -> int:

@@ -43,7 +43,11 @@ enum wp_status {
   WP_ERR_STATE = -6             /* call not valid in the engine's current state */
 };
 
-enum wp_dtype { WP_DTYPE_F16 = 0, WP_DTYPE_BF16 = 1 };
+enum wp_dtype { WP_DTYPE_F16 = 0, WP_DTYPE_BF16 = 1, WP_DTYPE_F32 = 2 /* wp_token_logprobs only */ };
+
+/* Activations of wp_linear: gelu by the error function, gelu_tanh by its tanh
+ * approximation, silu = v / (1 + exp(-v)). */
+enum wp_activation { WP_ACT_NONE = 0, WP_ACT_RELU = 1, WP_ACT_GELU = 2, WP_ACT_GELU_TANH = 3, WP_ACT_SILU = 4 };
 
 typedef struct wp_engine wp_engine;
 
@@ -341,6 +345,53 @@ int wp_lora_expand(wp_engine* e, void* y, int64_t y_row_stride, const void* h, i
 int wp_add_bias(wp_engine* e, void* y, int64_t y_row_stride, int32_t n_slices, const void* const* bias,
                 const int64_t* bias_stride0, const int32_t* out_features, const int32_t* y_col_offsets,
                 int32_t num_loras, int64_t T, int32_t dtype, void* stream);
+
+/* ---- operators around the apply ------------------------------------------
+ * What a model computes between its LoRA deltas (no reference counterpart).  They
+ * use no segment table; scratch is the engine's, so the one-call-at-a-time
+ * rule of an engine holds for them too.  They allocate nothing, and can be
+ * captured. */
+
+/* y[t, n] = rn(act(x[t] . w[n] + bias[n]) + residual[t, n]) for n < d_out, or, gated (w has
+ * 2 * d_out rows, bias as many elements),
+ * y[t, n] = rn(act(x[t] . w[n] + bias[n]) * (x[t] . w[d_out + n] + bias[d_out + n]) + residual[t, n]),
+ * accumulated in fp32 and rounded once.  bias and residual may be NULL; residual
+ * may be y.  Any d_in, d_out and row strides in elements (x and w rows with
+ * unit column stride; 16-byte aligned rows and d_in a multiple of 8 run the
+ * faster loads). */
+int wp_linear(wp_engine* e, void* y, int64_t y_row_stride, const void* x, int64_t x_row_stride, const void* w,
+              int64_t w_row_stride, const void* bias, const void* residual, int64_t residual_row_stride,
+              int32_t activation, int32_t gated, int32_t d_in, int32_t d_out, int64_t T, int32_t dtype, void* stream);
+
+/* Attention over n_seq packed sequences: sequence b has the queries
+ * [cu_q[b], cu_q[b + 1]) (rows of q and out) and the keys [cu_k[b], cu_k[b + 1])
+ * (rows of k and v); cu_q and cu_k are n_seq + 1 int32 on the device.  A
+ * sequence's last query stands at its last key.  causal: a query sees the keys
+ * up to its own position, with window > 0 only the last `window` of them;
+ * else every key of its sequence.  Query head h reads key head
+ * h / (heads / kv_heads).  out = softmax(scale * q . k) . v, lse (fp32 [tokens, heads], or NULL)
+ * the natural logarithm of the sum of exponentials; queries that see no key, and rows of no sequence,
+ * get 0 and -inf.  strides[0] between tokens, strides[1] between heads, in elements, multiples of 8;
+ * a head's head_dim elements (a multiple of 8, up to 128) are contiguous and 16-byte
+ * aligned.  Softmax statistics and sums are fp32; the exponentials are rounded to the
+ * tensors' type for the product with v. */
+int wp_packed_attention(wp_engine* e, void* out, const int64_t* out_strides, float* lse, const void* q,
+                        const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, const int32_t* cu_q, const int32_t* cu_k, int32_t n_seq,
+                        int64_t tokens, int64_t keys, int32_t heads, int32_t kv_heads, int32_t head_dim, float scale,
+                        int32_t causal, int32_t window, int32_t dtype, void* stream);
+
+/* For every row of logits [rows, vocab] (fp16, bf16 or fp32, unit column
+ * stride): logprobs = log softmax at token_ids[row], entropy = the softmax's
+ * entropy (nats), ranks = 1 + how many logits are greater than the token's, and
+ * the `top` (up to 64) largest logits in order, equal ones by the lower id, as
+ * top_ids and top_logprobs [rows, top].  NaN counts as the largest value.  A
+ * token id of -1 (or below) names no token: logprob and rank 0; so does one
+ * past the vocabulary, which is flagged (device error 1).  A row whose logits are all
+ * -inf, or which holds NaN or +inf, has no distribution: NaN. */
+int wp_token_logprobs(wp_engine* e, float* logprobs, float* entropy, int32_t* ranks, float* top_logprobs,
+                      int32_t* top_ids, const void* logits, int64_t logits_row_stride, const void* token_ids,
+                      int32_t ids_are_int64, int64_t rows, int32_t vocab, int32_t top, int32_t dtype, void* stream);
 
 /* ---- staging / prefetch ---------------------------------------------------- */
 
