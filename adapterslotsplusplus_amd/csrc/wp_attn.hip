@@ -1,8 +1,31 @@
 // wp_attn.hip -- attention over packed sequences of different lengths
 // (gfx950): causal, grouped heads, optional window, fp32 softmax statistics.
+//
+// For every query row i of a key head (the rows of one key head are its
+// sequence's tokens times the query heads that share it):
+//   out_i = sum_j 2^(c s_ij - m_i) v_j / l_i,   l_i = sum_j 2^(c s_ij - m_i),
+// with s = q . k, c = scale * log2(e) and m_i a running bound of c s_ij, in one
+// pass over the keys.
+//
+// The scores are computed transposed, S^T = K . Q^T (32x32x16): a lane then
+// holds 16 keys of one query per tile, so maximum and sum are sums over its
+// own registers (and one other lane's), and the exponentials, packed in
+// register order, already are the right operand of O^T = V^T . P^T, whose
+// contraction index may run over the keys in any order.  V^T's fragments come
+// out of LDS by the transposing read, four keys of a column at a time, in that
+// same order.
+//
+// Two roles share the launch.  Sequences with more than 32 rows per key head
+// run on row tiles: a workgroup's waves take 32 rows each and stage 64 keys
+// and values at a time in LDS for all of them.  Shorter ones (single tokens,
+// drafted tokens) run on key chunks: the waves hold the same 32 rows and each
+// streams keys of its own.  Either role splits a long key range over
+// workgroups where there are too few of them, and the last one of a row tile
+// to finish joins the partial results.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "wp_device.h"
 #include "wp_model.h"
@@ -10,90 +33,790 @@
 namespace wp {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
 
-// The sequence of packed row t by its bounds cu[0..n]: b with cu[b] <= t <
-// cu[b + 1], or -1.
-__device__ __forceinline__ int sequence_of(const int32_t* cu, int n, int64_t t) {
-  int lo = 0, hi = n;  // the first bound past t is in (lo, hi + 1]
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cu[mid] <= t) lo = mid; else hi = mid - 1;
-  }
-  return lo < n && cu[lo] <= t && t < cu[lo + 1] ? lo : -1;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.69314718055994531f;
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kWaveRows = 32;
+constexpr int kTileRows = kWaveRows * kWaves;  // query rows of a row tile
+constexpr int kTileKeys = 64;                  // keys staged at a time for a row tile
+constexpr int kChunkKeys = 32;                 // keys a wave stages at a time for a key chunk
+// A running bound is raised (and O and l scaled) only once a score exceeds it
+// by 2^8: exponentials then stay within 2^8, far inside fp16, and most tiles
+// scale nothing.
+constexpr float kSlack = 8.f;
+constexpr int kOutside = 0x7FFFFF00;  // a buffer offset past every range: the load gives zeros
+
+__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
+
+template <typename T>
+__device__ __forceinline__ typename VecOf<T>::v8 negate8(typename VecOf<T>::v8 v) {
+  const u32x4 u = __builtin_bit_cast(u32x4, v);
+  return __builtin_bit_cast(typename VecOf<T>::v8, u ^ 0x80008000u);
 }
 
-// One wave per query row and head: a lane scores one key of 64, then the
-// lanes share out the head's columns for the weighted sum.
+// Which of two 16-bit values are infinite or NaN are cleared.
 template <typename T>
-__global__ __launch_bounds__(64) void row_kernel(AttnArgs p) {
-  __shared__ float sq[256];
-  __shared__ float sp[64];
-  const int lane = static_cast<int>(threadIdx.x);
-  const int64_t t = blockIdx.x;
-  const int h = static_cast<int>(blockIdx.y);
-  const int hk = h / (p.heads / p.kv_heads);
-  const int b = sequence_of(p.cu_q, p.n_seq, t);
-  int64_t first = 0, k0 = 0, end = 0;
-  if (b >= 0) {
-    k0 = std::clamp<int64_t>(p.cu_k[b], 0, p.keys);
-    const int64_t n_k = std::clamp<int64_t>(p.cu_k[b + 1], k0, p.keys) - k0;
-    const int64_t pos = t - p.cu_q[b] + n_k - (p.cu_q[b + 1] - p.cu_q[b]);
-    end = p.causal ? std::clamp<int64_t>(pos + 1, 0, n_k) : n_k;
-    first = p.causal && p.window > 0 ? std::max<int64_t>(0, pos - p.window + 1) : 0;
+__device__ __forceinline__ bool finite16(uint32_t half) {
+  constexpr uint32_t e = sizeof(T) == 2 && __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;
+  return (half & e) != e;
+}
+template <typename T>
+__device__ __forceinline__ i16x4 finite_only(i16x4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = finite16<T>(static_cast<uint16_t>(v[i])) ? v[i] : static_cast<short>(0);
+  return v;
+}
+
+// Head columns computed (DP, a multiple of 32) and how a row of K or V lies in
+// LDS: 128 or 256 bytes in 16-byte chunks, columns past the head zero.
+//   K row r keeps chunk c at c ^ key_swizzle(r): the rows that a fragment load touches at one c
+//   fall on different banks.
+//   V row r keeps chunk c at c ^ value_swizzle(r): the transposing read takes 64
+//   bytes of each of eight rows, which so fall on different banks too.
+template <int DP>
+struct Head {
+  static constexpr int kRow = DP <= 64 ? 128 : 256;
+  static constexpr int kChunks = kRow / 16;
+  static constexpr int kRowsPerLoad = 1024 / kRow;  // rows a wave's 16-byte-per-lane load fills
+  static constexpr int kSteps = DP / 16;            // contraction steps of S
+  static constexpr int kCols = DP / 32;             // 32-column tiles of O
+  static __device__ __forceinline__ int key_swizzle(int r) { return kRow == 256 ? r & 15 : (r >> 1) & 7; }
+  static __device__ __forceinline__ int value_swizzle(int r) { return kRow == 256 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
+};
+
+// One work item.
+struct Item {
+  int seq;       // -1: none
+  int head;      // key head
+  int tile;      // row tile of the sequence
+  int chunk;     // key chunk
+  int slot;      // the item's place among the partials
+  int counter;   // its row tile's counter
+  int stride;    // between the slots of a row tile's chunks
+  int64_t q0, k0;
+  int n_q, n_k;
+};
+
+struct Span {
+  int64_t q0, k0;
+  int n_q, n_k;
+};
+__device__ __forceinline__ Span span_of(const AttnArgs& p, int b) {
+  Span s;
+  const int64_t q0 = p.cu_q[b], q1 = p.cu_q[b + 1], k0 = p.cu_k[b], k1 = p.cu_k[b + 1];
+  s.q0 = std::clamp<int64_t>(q0, 0, p.tokens);
+  s.n_q = static_cast<int>(std::clamp<int64_t>(q1, s.q0, p.tokens) - s.q0);
+  s.k0 = std::clamp<int64_t>(k0, 0, p.keys);
+  s.n_k = static_cast<int>(std::clamp<int64_t>(k1, s.k0, p.keys) - s.k0);
+  return s;
+}
+
+// Keys that rows [row, row + rows) of a sequence see: [first, end).
+struct Range {
+  int first, end;
+};
+__device__ __forceinline__ Range keys_of(const AttnArgs& p, int n_q, int n_k, int group, int row, int rows) {
+  Range r{0, n_k};
+  if (!p.causal) return r;
+  const int t0 = row / group, t1 = std::min(n_q - 1, (row + rows - 1) / group);
+  r.end = std::clamp(t1 + n_k - n_q + 1, 0, n_k);
+  if (p.window > 0) r.first = std::clamp(t0 + n_k - n_q - p.window + 1, 0, r.end);
+  return r;
+}
+
+// Key chunks over a whole sequence's keys for a given role.
+__device__ __forceinline__ int chunks_of(int keys, int shift) {
+  return std::max(1, static_cast<int>((static_cast<int64_t>(keys) + (1ll << shift) - 1) >> shift));
+}
+__device__ __forceinline__ int items_of(const AttnArgs& p, const Span& s, int group, bool rows_role, int* tiles) {
+  const int rows = s.n_q * group;
+  *tiles = 0;
+  if (rows == 0 || (rows > kWaveRows) != rows_role) return 0;
+  const Range r = keys_of(p, s.n_q, s.n_k, group, 0, rows);
+  const int unit = rows_role ? kTileKeys : kChunkKeys;
+  const int chunks = chunks_of(r.end - r.first / unit * unit, rows_role ? p.tile_shift : p.chunk_shift);
+  *tiles = rows_role ? (rows + kTileRows - 1) / kTileRows : 1;
+  return *tiles * chunks;
+}
+
+// The item of this workgroup: every wave counts through the sequences, 64 at
+// a time, a lane each.
+__device__ __forceinline__ Item find_item(const AttnArgs& p, int group, bool rows_role, int id) {
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  Item it;
+  it.seq = -1;
+  it.head = id % p.kv_heads;
+  const int want = id / p.kv_heads;
+  int base = 0, tile_base = 0;
+  for (int b0 = 0; b0 < p.n_seq; b0 += 64) {
+    const int b = b0 + lane;
+    int tiles = 0, items = 0;
+    Span s{0, 0, 0, 0};
+    if (b < p.n_seq) {
+      s = span_of(p, b);
+      items = items_of(p, s, group, rows_role, &tiles);
+    }
+    int sum = items, tile_sum = tiles;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) {
+      const int u = __shfl_up(sum, x), v = __shfl_up(tile_sum, x);
+      sum += lane >= x ? u : 0;
+      tile_sum += lane >= x ? v : 0;
+    }
+    const unsigned long long past = __ballot(base + sum > want);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      it.seq = b0 + at;
+      const int local = want - base - (__shfl(sum, at) - __shfl(items, at));
+      const int n_tiles = __shfl(tiles, at);
+      const int first_tile = tile_base + __shfl(tile_sum, at) - n_tiles;
+      // Later row tiles see more keys: they go first.
+      it.tile = n_tiles - 1 - local % n_tiles;
+      it.chunk = local / n_tiles;
+      it.slot = id;
+      it.counter = (first_tile + it.tile) * p.kv_heads + it.head;
+      it.stride = __builtin_amdgcn_readfirstlane(n_tiles * p.kv_heads);
+      it.seq = __builtin_amdgcn_readfirstlane(it.seq);
+      it.tile = __builtin_amdgcn_readfirstlane(it.tile);
+      it.chunk = __builtin_amdgcn_readfirstlane(it.chunk);
+      it.counter = __builtin_amdgcn_readfirstlane(it.counter);
+      const Span f = span_of(p, it.seq);
+      it.q0 = f.q0;
+      it.k0 = f.k0;
+      it.n_q = f.n_q;
+      it.n_k = f.n_k;
+      return it;
+    }
+    base += __shfl(sum, 63);
+    tile_base += __shfl(tile_sum, 63);
   }
-  const T* q = static_cast<const T*>(p.q) + t * p.q_tok + h * p.q_head;
-  for (int d = lane; d < p.dim; d += 64) sq[d] = static_cast<float>(q[d]);
+  return it;
+}
+
+// A wave's 32 query rows and their running state.
+template <typename T, int DP>
+struct Rows {
+  using H = Head<DP>;
+  using V8 = typename VecOf<T>::v8;
+  V8 q[H::kSteps];
+  f32x16 o[H::kCols];
+  float m;      // running bound, in units of c * s
+  float l;      // this lane's keys' sum
+  int pos;      // key position of the lane's query (causal), else the last key
+  int low;      // first key it sees
+
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int i = 0; i < H::kCols; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+    m = -INFINITY;
+    l = 0.f;
+  }
+
+  // Raises the bound where a score exceeds it by the slack (tops: the lane's
+  // largest score of the tile).
+  __device__ __forceinline__ void raise(float tops, float c) {
+    const float t = tops * c;
+    if (__any(t > m + kSlack)) {
+      const float top = fmaxf(fmaxf(t, __shfl_xor(t, 32)), m);
+      const float fade = top == -INFINITY ? 1.f : exp2_fast(m - top);
+      m = top;
+      l *= fade;
+#pragma unroll
+      for (int i = 0; i < H::kCols; ++i) o[i] *= fade;
+    }
+  }
+
+  // Scores of keys [at, at + 32) that the lane's query does not see become -inf.
+  __device__ __forceinline__ void mask(f32x16& s, int at) {
+    const int first = at + ((static_cast<int>(threadIdx.x) & 63) >> 5) * 4;
+    const int up = pos - first, down = low - first;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int key = (e >> 2) * 8 + (e & 3);
+      s[e] = key <= up && key >= down ? s[e] : -INFINITY;
+    }
+  }
+};
+
+__device__ __forceinline__ float top_of(const f32x16& s) {
+  float t = fmaxf(s[0], s[1]);
+#pragma unroll
+  for (int e = 2; e < 16; e += 2) t = fmaxf(fmaxf(t, s[e]), s[e + 1]);
+  return t;
+}
+
+// K fragment of step `step`: keys row0 .. row0 + 31 of a staged tile.
+template <typename T, int DP>
+__device__ __forceinline__ typename VecOf<T>::v8 key_fragment(const char* keys, int row0, int step) {
+  using H = Head<DP>;
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  const int r = lane & 31, c = step * 2 + (lane >> 5);
+  return *reinterpret_cast<const typename VecOf<T>::v8*>(keys + (row0 + r) * H::kRow + ((c ^ H::key_swizzle(r)) << 4));
+}
+
+// V^T fragment of columns col * 32 .. + 31 and the 16 keys from key0, in the
+// order of the packed exponentials: lane half h has keys 4h .. 4h + 3 and
+// 8 + 4h .. 8 + 4h + 3.
+template <typename T, int DP, bool kCareful>
+__device__ __forceinline__ typename VecOf<T>::v8 value_fragment(const char* values, int key0, int col) {
+  using H = Head<DP>;
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  const int i = lane & 15, g = lane >> 4;
+  const int r = 4 * (g >> 1) + (i >> 2);
+  const int c = col * 4 + (g & 1) * 2 + ((i & 3) >> 1);
+  const char* at = values + (key0 + r) * H::kRow + ((c ^ H::value_swizzle(r)) << 4) + (i & 1) * 8;
+  using L = __attribute__((address_space(3))) i16x4;
+  i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(at));
+  i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(at + 8 * H::kRow));
+  if (kCareful) {
+    lo = finite_only<T>(lo);
+    hi = finite_only<T>(hi);
+  }
+  union {
+    i16x4 h[2];
+    typename VecOf<T>::v8 v;
+  } u;
+  u.h[0] = lo;
+  u.h[1] = hi;
+  return u.v;
+}
+
+// Adds the infinite and NaN values of keys [at, at + n) that a query sees,
+// which value_fragment<careful> left out.
+template <typename T, int DP>
+__device__ __forceinline__ void add_nonfinite(Rows<T, DP>& w, const char* values, int at, int n) {
+  using H = Head<DP>;
+  const int lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
+  for (int r = 0; r < n; ++r) {
+    const char* row = values + r * H::kRow;
+    bool odd = false;
+    if (lane < H::kRow / 4) {
+      const uint32_t u = *reinterpret_cast<const uint32_t*>(row + lane * 4);
+      odd = !finite16<T>(u & 0xFFFFu) || !finite16<T>(u >> 16);
+    }
+    if (!__any(odd)) continue;
+    const bool sees = at + r <= w.pos && at + r >= w.low;
+#pragma unroll
+    for (int i = 0; i < H::kCols; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int d = i * 32 + (e >> 2) * 8 + half * 4 + (e & 3);
+        const int c = (d >> 3) ^ H::value_swizzle(r);
+        const uint16_t u = *reinterpret_cast<const uint16_t*>(row + c * 16 + (d & 7) * 2);
+        if (sees && !finite16<T>(u)) w.o[i][e] += static_cast<float>(__builtin_bit_cast(T, u));
+      }
+  }
+}
+
+// Stages rows [0, rows) of 1024 / kRow * loads rows from `src` (rows `stride`
+// bytes apart) at `dst`: load i of this wave fills rows (first + i) *
+// kRowsPerLoad on, 16 bytes a lane, straight to LDS; rows past `rows` and
+// columns past the head are zero.
+template <int DP, bool kValues, int kLoads>
+__device__ __forceinline__ void stage(const void* src, uint32_t stride, int dim, int rows, char* dst, int first) {
+  using H = Head<DP>;
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(src), 0, 0x7FFFFF00, 0x00020000);
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = (first + i) * H::kRowsPerLoad + lane / H::kChunks;
+    const int c = (lane % H::kChunks) ^ (kValues ? H::value_swizzle(r) : H::key_swizzle(r));
+    const int off = r < rows && c * 8 < dim ? static_cast<int>(r * stride) + c * 16 : kOutside;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        rsrc, (__attribute__((address_space(3))) void*)(dst + (first + i) * 1024), 16, off, 0, 0, 0);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ const T* head_row(const void* base, int64_t tok, int64_t tok_stride, int64_t head_offset) {
+  return static_cast<const T*>(base) + tok * tok_stride + head_offset;
+}
+
+// Exponentials of a 32-key tile, added to the lane's sum and packed: the two
+// right operands of its two 16-key steps.
+template <typename T, int DP>
+__device__ __forceinline__ void weigh(Rows<T, DP>& w, const f32x16& s, float c, typename VecOf<T>::v8 (&out)[2]) {
+  const float base = w.m == -INFINITY ? 0.f : w.m;
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = exp2_fast(fmaf(s[b * 8 + e], c, -base));
+      w.l += x;
+      out[b][e] = static_cast<T>(x);
+    }
+}
+
+// Scores of 32 staged keys from row0 on.
+template <typename T, int DP>
+__device__ __forceinline__ f32x16 scores(const Rows<T, DP>& w, const char* keys, int row0) {
+  f32x16 s{};
+#pragma unroll
+  for (int x = 0; x < Head<DP>::kSteps; ++x) s = mfma32(key_fragment<T, DP>(keys, row0, x), w.q[x], s);
+  return s;
+}
+
+// Adds 32 staged keys' weighted values to O.
+template <typename T, int DP, bool kCareful>
+__device__ __forceinline__ void accumulate(Rows<T, DP>& w, const char* values, int row0,
+                                           const typename VecOf<T>::v8 (&e)[2]) {
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int x = 0; x < Head<DP>::kCols; ++x)
+      w.o[x] = mfma32(value_fragment<T, DP, kCareful>(values, row0 + b * 16, x), e[b], w.o[x]);
+}
+
+// LDS of a workgroup.  Each buffer is an array of its own: the compiler then
+// sees that a load into one leaves reads of the others alone, and does not wait
+// for it.
+template <int DP>
+struct Staged {
+  static constexpr int kBytes = kTileKeys * Head<DP>::kRow;
+};
+#define WP_STAGED char (&sk0)[Staged<DP>::kBytes], char (&sk1)[Staged<DP>::kBytes], char (&sv0)[Staged<DP>::kBytes], \
+                  char (&sv1)[Staged<DP>::kBytes]
+
+// Row tile: the keys [first, end) for the workgroup's rows, 64 at a time.
+// While tile j is weighed and added, the scores of tile j + 1 are computed
+// (they need nothing of it, so the matrix cores work beside the exponentials), and tiles j + 2
+// of K and j + 1 of V are on their way.
+template <typename T, int DP>
+__device__ __forceinline__ void run_tile(const AttnArgs& p, const Item& it, Rows<T, DP>& w, float c, int first, int end,
+                                         int wave_low, int wave_pos, int wave, WP_STAGED) {
+  using H = Head<DP>;
+  using V8 = typename VecOf<T>::v8;
+  constexpr int kLoads = kTileKeys * H::kRow / 1024 / kWaves;
+  const T* k = head_row<T>(p.k, it.k0, p.k_tok, it.head * p.k_head);
+  const T* v = head_row<T>(p.v, it.k0, p.v_tok, it.head * p.v_head);
+  const int64_t k_tok = p.k_tok, v_tok = p.v_tok;
+  const int n_k = it.n_k, dim = p.dim;
+  auto load_k = [&](int at, char* to) {
+    if (at < end) stage<DP, false, kLoads>(k + at * k_tok, static_cast<uint32_t>(k_tok) * 2, dim, n_k - at, to, wave * kLoads);
+  };
+  auto load_v = [&](int at, char* to) {
+    if (at < end) stage<DP, true, kLoads>(v + at * v_tok, static_cast<uint32_t>(v_tok) * 2, dim, n_k - at, to, wave * kLoads);
+  };
+  w.reset();
+  if (first >= end) return;
+  load_k(first, sk0);
   __syncthreads();
-  float m = -INFINITY, l = 0.f, o[4] = {};
-  for (int64_t at = first; at < end; at += 64) {
-    const int64_t j = at + lane;
-    float s = -INFINITY;
-    if (j < end) {
-      const T* k = static_cast<const T*>(p.k) + (k0 + j) * p.k_tok + hk * p.k_head;
-      s = 0.f;
-      for (int d = 0; d < p.dim; ++d) s += sq[d] * static_cast<float>(k[d]);
-      s *= p.scale;
+  load_k(first + kTileKeys, sk1);
+  load_v(first, sv0);
+  f32x16 s0 = scores(w, sk0, 0), s1 = scores(w, sk0, 32);
+  auto step = [&](int at, auto more, char* kfree, const char* knext, const char* vnow, char* vnext) {
+    __syncthreads();
+    load_k(at + 2 * kTileKeys, kfree);
+    load_v(at + kTileKeys, vnext);
+    // wave_low, wave_pos: the keys that every row of the wave sees.
+    if (at < wave_low || at + kTileKeys - 1 > wave_pos) {
+      w.mask(s0, at);
+      w.mask(s1, at + 32);
     }
-    float top = s;
-    for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-    top = fmaxf(top, m);
-    const float base = top == -INFINITY ? 0.f : top;
-    const float e = exp2f((s - base) * kLog2e);
-    const float fade = exp2f((m - base) * kLog2e);
-    float sum = e;
-    for (int x = 32; x > 0; x >>= 1) sum += __shfl_xor(sum, x);
-    l = l * fade + sum;
-    m = top;
+    w.raise(fmaxf(top_of(s0), top_of(s1)), c);
+    // In two halves of 32 keys, which keeps the registers of three score
+    // tiles, not four, in use.
+    V8 e[2];
+    f32x16 n;
+    if (more) n = scores(w, knext, 0);
+    weigh(w, s0, c, e);
+    accumulate<T, DP, false>(w, vnow, 0, e);
+    if (more) s0 = n;
+    __builtin_amdgcn_sched_barrier(0);
+    if (more) n = scores(w, knext, 32);
+    weigh(w, s1, c, e);
+    accumulate<T, DP, false>(w, vnow, 32, e);
+    if (more) s1 = n;
+  };
+  int at = first;
+  constexpr std::integral_constant<bool, true> yes{};
+  constexpr std::integral_constant<bool, false> no{};
+  for (; at + 2 * kTileKeys < end; at += 2 * kTileKeys) {
+    step(at, yes, sk0, sk1, sv0, sv1);
+    step(at + kTileKeys, yes, sk1, sk0, sv1, sv0);
+  }
+  if (at + kTileKeys < end) {
+    step(at, yes, sk0, sk1, sv0, sv1);
+    step(at + kTileKeys, no, sk1, sk0, sv1, sv0);
+  } else {
+    step(at, no, sk0, sk1, sv0, sv1);
+  }
+}
+
+// run_tile, one tile after the other, with infinite and NaN values left out of
+// the product and added to the rows that see them: the same sums otherwise.
+template <typename T, int DP>
+__device__ __forceinline__ void run_tile_careful(const AttnArgs& p, const Item& it, Rows<T, DP>& w, float c, int first,
+                                                 int end, int wave_low, int wave_pos, int wave, char* sk, char* sv) {
+  using H = Head<DP>;
+  constexpr int kLoads = kTileKeys * H::kRow / 1024 / kWaves;
+  const T* k = head_row<T>(p.k, it.k0, p.k_tok, it.head * p.k_head);
+  const T* v = head_row<T>(p.v, it.k0, p.v_tok, it.head * p.v_head);
+  w.reset();
+  for (int at = first; at < end; at += kTileKeys) {
     __syncthreads();
-    sp[lane] = e;
+    stage<DP, false, kLoads>(k + at * p.k_tok, static_cast<uint32_t>(p.k_tok) * 2, p.dim, it.n_k - at, sk, wave * kLoads);
+    stage<DP, true, kLoads>(v + at * p.v_tok, static_cast<uint32_t>(p.v_tok) * 2, p.dim, it.n_k - at, sv, wave * kLoads);
     __syncthreads();
-    const int n = static_cast<int>(std::min<int64_t>(64, end - at));
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 64 * i;
-      if (d >= p.dim) break;
-      float w = o[i] * fade;
-      for (int x = 0; x < n; ++x)
-        w += sp[x] * static_cast<float>(static_cast<const T*>(p.v)[(k0 + at + x) * p.v_tok + hk * p.v_head + d]);
-      o[i] = w;
+    f32x16 s0 = scores(w, sk, 0), s1 = scores(w, sk, 32);
+    if (at < wave_low || at + kTileKeys - 1 > wave_pos) {
+      w.mask(s0, at);
+      w.mask(s1, at + 32);
+    }
+    w.raise(fmaxf(top_of(s0), top_of(s1)), c);
+    typename VecOf<T>::v8 e0[2], e1[2];
+    weigh(w, s0, c, e0);
+    weigh(w, s1, c, e1);
+    accumulate<T, DP, true>(w, sv, 0, e0);
+    accumulate<T, DP, true>(w, sv, 32, e1);
+    add_nonfinite(w, sv, at, kTileKeys);
+  }
+}
+
+// Key chunk: keys [first, end), the waves taking 32 of them in turn.
+template <typename T, int DP, bool kCareful>
+__device__ __forceinline__ void run_chunk(const AttnArgs& p, const Item& it, Rows<T, DP>& w, float c, int first, int end,
+                                          int wave_low, int wave_pos, int wave, char* sk, char* sv) {
+  using H = Head<DP>;
+  constexpr int kLoads = kChunkKeys * H::kRow / 1024;
+  const T* k = head_row<T>(p.k, it.k0, p.k_tok, it.head * p.k_head);
+  const T* v = head_row<T>(p.v, it.k0, p.v_tok, it.head * p.v_head);
+  auto load_k = [&](int at) {
+    stage<DP, false, kLoads>(k + at * p.k_tok, static_cast<uint32_t>(p.k_tok) * 2, p.dim, it.n_k - at, sk, 0);
+  };
+  auto load_v = [&](int at) {
+    stage<DP, true, kLoads>(v + at * p.v_tok, static_cast<uint32_t>(p.v_tok) * 2, p.dim, it.n_k - at, sv, 0);
+  };
+  w.reset();
+  int at = first + wave * kChunkKeys;
+  if (at < end) {
+    load_k(at);
+    load_v(at);
+  }
+  for (; at < end; at += kChunkKeys * kWaves) {
+    const int next = at + kChunkKeys * kWaves;
+    wait_vm();
+    f32x16 s = scores(w, sk, 0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (next < end) load_k(next);
+    if (!(at >= wave_low && at + kChunkKeys - 1 <= wave_pos)) w.mask(s, at);
+    w.raise(top_of(s), c);
+    typename VecOf<T>::v8 e[2];
+    weigh(w, s, c, e);
+    accumulate<T, DP, kCareful>(w, sv, 0, e);
+    if (kCareful) add_nonfinite(w, sv, at, kChunkKeys);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (next < end) load_v(next);
+  }
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ bool has_nonfinite(const Rows<T, DP>& w) {
+  float z = 0.f;
+#pragma unroll
+  for (int i = 0; i < Head<DP>::kCols; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) z = fmaf(w.o[i][e], 0.f, z);
+  return z != 0.f;  // NaN: an infinity or NaN times zero
+}
+
+// Writes four columns of a finished row (and with the first of them its lse).
+template <typename T>
+__device__ __forceinline__ void finish_row(const AttnArgs& p, const Item& it, int group, int row, int d, f32x4 v, float m,
+                                           float l) {
+  const int tok = row / group, h = it.head * group + row % group;
+  const int pos = p.causal ? std::min(tok + it.n_k - it.n_q, it.n_k - 1) : it.n_k - 1;
+  const bool sees = pos >= 0;
+  if (d < p.dim)
+    store4(static_cast<T*>(p.out) + (it.q0 + tok) * p.o_tok + h * p.o_head + d, sees ? v * (1.f / l) : f32x4{0.f, 0.f, 0.f, 0.f});
+  if (p.lse && d == 0) p.lse[(it.q0 + tok) * p.heads + h] = sees ? fmaf(m, kLn2, logf(l)) : -INFINITY;
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs p) {
+  using H = Head<DP>;
+  __shared__ __align__(1024) char sk0[Staged<DP>::kBytes];
+  __shared__ __align__(1024) char sk1[Staged<DP>::kBytes];
+  __shared__ __align__(1024) char sv0[Staged<DP>::kBytes];
+  __shared__ __align__(1024) char sv1[Staged<DP>::kBytes];
+  __shared__ float s_m[kWaves][kWaveRows];
+  __shared__ float s_l[kWaves][kWaveRows];
+  __shared__ uint32_t s_last;
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = lane >> 5;
+  const int group = p.heads / p.kv_heads;
+
+  // Rows of no sequence: before the first bound and from the last one on.
+  {
+    const int64_t head_rows = p.n_seq > 0 ? std::clamp<int64_t>(p.cu_q[0], 0, p.tokens) : p.tokens;
+    const int64_t tail = p.n_seq > 0 ? std::clamp<int64_t>(p.cu_q[p.n_seq], head_rows, p.tokens) : p.tokens;
+    const int64_t n = (head_rows + p.tokens - tail) * p.heads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kWaves + wave; i < n; i += static_cast<int64_t>(gridDim.x) * kWaves) {
+      int64_t t = i / p.heads;
+      const int h = static_cast<int>(i % p.heads);
+      if (t >= head_rows) t += tail - head_rows;
+      T* out = static_cast<T*>(p.out) + t * p.o_tok + h * p.o_head;
+      for (int d = lane; d < p.dim; d += 64) out[d] = static_cast<T>(0.f);
+      if (p.lse && lane == 0) p.lse[t * p.heads + h] = -INFINITY;
     }
   }
-  T* out = static_cast<T*>(p.out) + t * p.o_tok + h * p.o_head;
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < p.dim) out[lane + 64 * i] = static_cast<T>(end > first ? o[i] / l : 0.f);
-  if (p.lse && lane == 0) p.lse[t * p.heads + h] = end > first ? m + logf(l) : -INFINITY;
+
+  const bool rows_role = static_cast<int>(blockIdx.x) < p.tile_items;
+  const int id = rows_role ? static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x) - p.tile_items;
+  const Item it = find_item(p, group, rows_role, id);
+  // Bounds that do not rise could name more row tiles than there are counters.
+  if (it.seq < 0 || it.counter >= (rows_role ? p.tile_counters : p.seq_counters)) return;
+  const int n_rows = it.n_q * group;
+  const int block_rows = rows_role ? kTileRows : kWaveRows;
+  const int row0 = it.tile * block_rows;             // the workgroup's first row
+  const int my_rows = std::min(block_rows, n_rows - row0);
+  const Range range = keys_of(p, it.n_q, it.n_k, group, row0, my_rows);
+  const int shift = rows_role ? p.tile_shift : p.chunk_shift;
+  const int unit = rows_role ? kTileKeys : kChunkKeys;
+  const int base = range.first / unit * unit;        // tiles start at whole ones
+  const int chunks = chunks_of(range.end - base, shift);
+  if (it.chunk >= chunks) return;
+  const int first = static_cast<int>(base + (static_cast<int64_t>(it.chunk) << shift));
+  const int end = static_cast<int>(std::min<int64_t>(range.end, first + (1ll << shift)));
+
+  // This lane's query row.
+  const int wave_row0 = row0 + (rows_role ? wave * kWaveRows : 0);
+  const int row = wave_row0 + (lane & 31);
+  const bool real = row < n_rows;
+  const int tok = real ? row / group : 0, sub = real ? row % group : 0;
+  const float c = p.scale == 0.f ? 1.f : fabsf(p.scale) * kLog2e;
+  Rows<T, DP> w;
+  {
+    const T* q = head_row<T>(p.q, it.q0 + tok, p.q_tok, (it.head * group + sub) * p.q_head);
+#pragma unroll
+    for (int x = 0; x < H::kSteps; ++x) {
+      const int d = x * 16 + half * 8;
+      w.q[x] = real && d < p.dim && p.scale != 0.f ? load8(q + d) : zero8<T>();
+      if (p.scale < 0.f) w.q[x] = negate8<T>(w.q[x]);
+    }
+  }
+  const int lag = it.n_k - it.n_q;
+  w.pos = real ? (p.causal ? std::min(tok + lag, it.n_k - 1) : it.n_k - 1) : -1;
+  w.low = p.causal && p.window > 0 ? std::max(0, tok + lag - p.window + 1) : 0;
+  // The keys that all of the wave's rows see.
+  int wave_pos = it.n_k - 1, wave_low = 0;
+  if (p.causal) {
+    const int t0 = wave_row0 / group, t1 = std::min(it.n_q - 1, (wave_row0 + kWaveRows - 1) / group);
+    wave_pos = wave_row0 < n_rows ? t0 + lag : -1;
+    if (p.window > 0) wave_low = std::max(0, t1 + lag - p.window + 1);
+  }
+
+  if (rows_role) {
+    run_tile<T, DP>(p, it, w, c, first, end, wave_low, wave_pos, wave, sk0, sk1, sv0, sv1);
+    // Infinite or NaN values reach every row of a tile through the product, as
+    // zero times them: where there are any, the pass is made again with care.
+    if (__syncthreads_or(has_nonfinite(w)))
+      run_tile_careful<T, DP>(p, it, w, c, first, end, wave_low, wave_pos, wave, sk0, sv0);
+  } else {
+    // A wave's 32 keys and values: half of an array each.
+    char* k = (wave < 2 ? sk0 : sk1) + (wave & 1) * (Staged<DP>::kBytes / 2);
+    char* v = (wave < 2 ? sv0 : sv1) + (wave & 1) * (Staged<DP>::kBytes / 2);
+    run_chunk<T, DP, false>(p, it, w, c, first, end, wave_low, wave_pos, wave, k, v);
+    if (__any(has_nonfinite(w))) run_chunk<T, DP, true>(p, it, w, c, first, end, wave_low, wave_pos, wave, k, v);
+  }
+  w.l += __shfl_xor(w.l, 32);
+
+  const bool split = chunks > 1;
+  const bool sees = real && w.pos >= w.low;
+  const int rows_cap = block_rows;
+  // The item's partials: [rows][bound, sum], then [rows][DP] of O.
+  float* part = p.part + (rows_role ? 0 : p.chunk_part) + static_cast<uint64_t>(it.slot) * rows_cap * (DP + 2);
+  const __amdgpu_buffer_rsrc_t mine = coherent_buffer(part, static_cast<uint32_t>(rows_cap) * (DP + 2) * 4u);
+
+  if (rows_role) {
+    const float inv = 1.f / w.l;
+    if (!split) {
+      if (!real) return;
+      T* out = static_cast<T*>(p.out) + (it.q0 + tok) * p.o_tok + (it.head * group + sub) * p.o_head;
+#pragma unroll
+      for (int i = 0; i < H::kCols; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = i * 32 + e * 8 + half * 4;
+          if (d >= p.dim) continue;
+          const f32x4 v{w.o[i][e * 4], w.o[i][e * 4 + 1], w.o[i][e * 4 + 2], w.o[i][e * 4 + 3]};
+          store4(out + d, sees ? v * inv : f32x4{0.f, 0.f, 0.f, 0.f});
+        }
+      if (p.lse && half == 0)
+        p.lse[(it.q0 + tok) * p.heads + it.head * group + sub] = sees ? fmaf(w.m, kLn2, logf(w.l)) : -INFINITY;
+      return;
+    }
+    const int r = wave * kWaveRows + (lane & 31);
+    if (real) {
+      if (half == 0) {
+        coherent_store8(part + 2 * r, __builtin_bit_cast(unsigned long long, f32x2{w.m, w.l}));
+      }
+#pragma unroll
+      for (int i = 0; i < H::kCols; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          coherent_store16(mine, (2u * rows_cap + r * DP + i * 32 + e * 8 + half * 4) * 4u,
+                           f32x4{w.o[i][e * 4], w.o[i][e * 4 + 1], w.o[i][e * 4 + 2], w.o[i][e * 4 + 3]});
+    }
+  } else {
+    // The waves' shares joined: each scales its O to the common bound and
+    // leaves it in LDS, [row][DP] in an array of its own.
+    if (half == 0) {
+      s_m[wave][lane] = w.m;
+      s_l[wave][lane] = w.l;
+    }
+    __syncthreads();
+    float m = s_m[0][lane & 31];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) m = fmaxf(m, s_m[i][lane & 31]);
+    const float fade = m == -INFINITY ? 1.f : exp2_fast(w.m - m);
+    char* o32 = wave == 0 ? sk0 : wave == 1 ? sk1 : wave == 2 ? sv0 : sv1;
+    if (real)
+#pragma unroll
+      for (int i = 0; i < H::kCols; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<f32x4*>(o32 + ((lane & 31) * DP + i * 32 + e * 8 + half * 4) * 4) =
+              f32x4{w.o[i][e * 4], w.o[i][e * 4 + 1], w.o[i][e * 4 + 2], w.o[i][e * 4 + 3]} * fade;
+    __syncthreads();
+    for (int u = tid; u < my_rows * (DP / 4); u += kThreads) {
+      const int r = u / (DP / 4), d = u % (DP / 4) * 4;
+      float top = s_m[0][r], l = 0.f;
+#pragma unroll
+      for (int i = 1; i < kWaves; ++i) top = fmaxf(top, s_m[i][r]);
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) l += s_l[i][r] * (top == -INFINITY ? 1.f : exp2_fast(s_m[i][r] - top));
+      f32x4 v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i)
+        v += *reinterpret_cast<const f32x4*>((i == 0 ? sk0 : i == 1 ? sk1 : i == 2 ? sv0 : sv1) + (r * DP + d) * 4);
+      if (split) {
+        coherent_store16(mine, (2u * rows_cap + r * DP + d) * 4u, v);
+        if (d == 0) coherent_store8(part + 2 * r, __builtin_bit_cast(unsigned long long, f32x2{top, l}));
+      } else {
+        finish_row<T>(p, it, group, row0 + r, d, v, top, l);
+      }
+    }
+    if (!split) return;
+  }
+
+  // The last of the row tile's chunks to arrive joins them, in chunk order.
+  wait_vm();
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t* cnt = p.counters + (rows_role ? 0 : p.chunk_counters) + it.counter;
+    const bool last = atomic_add_u(cnt, 1u) == static_cast<unsigned>(chunks - 1);
+    if (last) atomic_store_u(cnt, 0u);
+    s_last = last ? 1u : 0u;
+  }
+  __syncthreads();
+  if (s_last == 0u) return;
+  const int64_t step = static_cast<int64_t>(it.stride) * rows_cap * (DP + 2);  // floats between chunks' partials
+  const float* part0 = part - it.chunk * step;
+  for (int u = tid; u < my_rows * (DP / 4); u += kThreads) {
+    const int r = u / (DP / 4), d = u % (DP / 4) * 4;
+    float top = -INFINITY, l = 0.f;
+    f32x4 v{0.f, 0.f, 0.f, 0.f};
+    constexpr int kBatch = 4;
+    for (int i0 = 0; i0 < chunks; i0 += kBatch) {
+      f32x2 ml[kBatch];
+      f32x4 o[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const float* at = part0 + std::min(i0 + i, chunks - 1) * step;
+        ml[i] = __builtin_bit_cast(f32x2, coherent_load8(at + 2 * r));
+        o[i] = coherent_load_f4(at + 2 * rows_cap + r * DP + d);
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (i0 + i >= chunks) break;
+        const float m = fmaxf(top, ml[i][0]);
+        const float old = m == -INFINITY ? 1.f : exp2_fast(top - m), now = m == -INFINITY ? 1.f : exp2_fast(ml[i][0] - m);
+        v = v * old + o[i] * now;
+        l = l * old + ml[i][1] * now;
+        top = m;
+      }
+    }
+    finish_row<T>(p, it, group, row0 + r, d, v, top, l);
+  }
+}
+
+template <typename T, int DP>
+hipError_t launch(const AttnArgs& a, hipStream_t stream) {
+  const int grid = std::max(1, a.tile_items + a.chunk_items);
+  hipLaunchKernelGGL((attention_kernel<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_head(const AttnArgs& a, int dp, hipStream_t stream) {
+  return dp == 64 ? launch<T, 64>(a, stream) : dp == 96 ? launch<T, 96>(a, stream) : launch<T, 128>(a, stream);
 }
 
 }  // namespace
 
 hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t stream) {
-  (void)n_cu;
-  const dim3 grid(static_cast<uint32_t>(a.tokens), static_cast<uint32_t>(a.heads));
-  if (dtype_bf16)
-    hipLaunchKernelGGL(row_kernel<__bf16>, grid, dim3(64), 0, stream, a);
-  else
-    hipLaunchKernelGGL(row_kernel<_Float16>, grid, dim3(64), 0, stream, a);
-  return hipGetLastError();
+  const int dp = a.dim <= 64 ? 64 : a.dim <= 96 ? 96 : 128;
+  const int64_t group = a.heads / a.kv_heads, rows = a.tokens * group;
+  const int64_t kNever = 31;  // a shift past every length: no split
+  // Bounds on the work items, from the sizes the host knows: a sequence of
+  // more than 32 rows has at most rows / 128 + 1 row tiles, and one of fewer
+  // at most keys / chunk + 2 key chunks.
+  const int64_t tile_seqs = std::min<int64_t>(a.n_seq, rows / (kWaveRows + 1));
+  const int64_t tiles = tile_seqs > 0 ? rows / kTileRows + tile_seqs : 0;
+  const int64_t chunk_seqs = std::min<int64_t>(a.n_seq, a.tokens);
+  // Row tiles: enough of them for the device (two workgroups a compute unit)
+  // run whole; fewer are split into ranges of at least 512 keys.
+  int64_t tile_shift = kNever;
+  if (tiles > 0 && std::max<int64_t>(1, rows / kTileRows) * a.kv_heads < n_cu)
+    for (tile_shift = 9; tile_shift < kNever; ++tile_shift)
+      if (tiles * ((a.keys >> tile_shift) + 2) * a.kv_heads <= 4 * n_cu) break;
+  int64_t tile_items = tiles * (tile_shift == kNever ? 1 : (a.keys >> tile_shift) + 2) * a.kv_heads;
+  uint64_t tile_floats = tile_shift == kNever ? 0 : static_cast<uint64_t>(tile_items) * kTileRows * (dp + 2);
+  int64_t tile_counters = tile_shift == kNever ? 0 : tiles * a.kv_heads;
+  if (tile_floats * 4 > a.part_bytes / 2 || tile_counters > a.n_counters / 2) {
+    tile_shift = kNever;
+    tile_items = tiles * a.kv_heads;
+    tile_floats = 0;
+    tile_counters = 0;
+  }
+  // Key chunks: about six workgroups a compute unit, of at least 128 keys (32
+  // for each wave).
+  int64_t chunk_shift = 7;
+  while (chunk_shift < kNever && (a.keys >> chunk_shift) * a.kv_heads > 6 * n_cu) ++chunk_shift;
+  int64_t chunk_items = chunk_seqs * a.kv_heads;
+  uint64_t chunk_floats = 0;
+  if (chunk_seqs > 0) {
+    chunk_items = ((a.keys >> chunk_shift) + 2 * chunk_seqs) * a.kv_heads;
+    chunk_floats = static_cast<uint64_t>(chunk_items) * kWaveRows * (dp + 2);
+    if ((tile_floats + chunk_floats) * 4 > a.part_bytes || tile_counters + chunk_seqs * a.kv_heads > a.n_counters) {
+      chunk_shift = kNever;
+      chunk_items = chunk_seqs * a.kv_heads;
+    }
+  }
+  if (tile_items + chunk_items > 0x7FFFFFFF) return hipErrorInvalidValue;
+  a.tile_items = static_cast<int32_t>(tile_items);
+  a.chunk_items = static_cast<int32_t>(chunk_items);
+  a.tile_shift = static_cast<int32_t>(tile_shift);
+  a.chunk_shift = static_cast<int32_t>(chunk_shift);
+  a.chunk_part = tile_floats;
+  a.tile_counters = tile_shift == kNever ? 0x7FFFFFFF : static_cast<int32_t>(tile_counters);
+  a.seq_counters = chunk_shift == kNever ? 0x7FFFFFFF : a.n_counters - static_cast<int32_t>(tile_counters);
+  a.chunk_counters = static_cast<int32_t>(tile_counters);
+  return dtype_bf16 ? launch_head<__bf16>(a, dp, stream) : launch_head<_Float16>(a, dp, stream);
 }
 
 }  // namespace wp

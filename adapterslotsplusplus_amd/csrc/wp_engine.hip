@@ -2562,6 +2562,10 @@ int wp_packed_attention(wp_engine* e, void* out, const int64_t* out_strides, flo
   a.scale = scale;
   a.causal = causal ? 1 : 0;
   a.window = window;
+  a.part = e->mpart;
+  a.part_bytes = kModelPartBytes;
+  a.counters = e->model_cnt;
+  a.n_counters = kModelCounters;
   DeviceGuard g(e->device);
   WP_HIP(launch_attention(dtype == WP_DTYPE_BF16, a, e->n_cu, static_cast<hipStream_t>(stream)));
   return WP_OK;

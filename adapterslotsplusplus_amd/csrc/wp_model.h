@@ -9,8 +9,8 @@
 namespace wp {
 
 // The engine's scratch for these operators: fp32 partials and tile counters.
-constexpr uint64_t kModelPartBytes = 64ull << 20;
-constexpr int kModelCounters = 8192;
+constexpr uint64_t kModelPartBytes = 128ull << 20;
+constexpr int kModelCounters = 65536;
 
 // Activations of wp_linear, in the order of enum wp_activation.
 enum Activation : int32_t { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
@@ -62,6 +62,18 @@ struct AttnArgs {
   int32_t n_seq, heads, kv_heads, dim;
   float scale;
   int32_t causal, window;  // window 0: none
+  float* part;             // partials of split key ranges
+  uint64_t part_bytes;
+  uint32_t* counters;      // zero between calls
+  int32_t n_counters;
+  // Filled by launch_attention: work items of either role (upper bounds; the
+  // workgroups past the last one leave), the keys per split as a power of
+  // two, and where the second role's partials and counters start.
+  int32_t tile_items, chunk_items;
+  int32_t tile_shift, chunk_shift;
+  int32_t chunk_counters;
+  int32_t tile_counters, seq_counters;  // how many either role has
+  uint64_t chunk_part;
 };
 hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t stream);
 
