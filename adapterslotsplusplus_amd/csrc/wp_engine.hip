@@ -2605,6 +2605,10 @@ int wp_token_logprobs(wp_engine* e, float* logprobs, float* entropy, int32_t* ra
   a.top_lp = top_logprobs;
   a.top_ids = top_ids;
   a.header = e->header;
+  a.part = reinterpret_cast<char*>(e->mpart);
+  a.part_bytes = kModelPartBytes;
+  a.counters = e->model_cnt;
+  a.n_counters = kModelCounters;
   DeviceGuard g(e->device);
   WP_HIP(launch_logprobs(a, e->n_cu, static_cast<hipStream_t>(stream)));
   return WP_OK;

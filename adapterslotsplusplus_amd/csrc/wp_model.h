@@ -96,7 +96,12 @@ struct LogprobArgs {
   float* top_lp;      // [rows, top]
   int32_t* top_ids;   // [rows, top]
   uint32_t* header;   // the plan header, whose error word is flagged
+  char* part;         // shares of rows that several workgroups read
+  uint64_t part_bytes;
+  uint32_t* counters; // zero between calls
+  int32_t n_counters;
+  int32_t parts;      // workgroups per row; filled by launch_logprobs
 };
-hipError_t launch_logprobs(const LogprobArgs& a, int n_cu, hipStream_t stream);
+hipError_t launch_logprobs(LogprobArgs& a, int n_cu, hipStream_t stream);
 
 }  // namespace wp
