@@ -31,7 +31,6 @@ constexpr int kListTrim = 128;      // cut the list down past this many beyond `
 constexpr int kMaxParts = 64;       // workgroups that share a row
 constexpr int kPartBytes = 16 + 8 * kMaxTop;
 static_assert(kMaxTop + kListTrim <= kRowThreads, "a thread each for the candidates kept");
-static_assert(kVecs == 4, "tops[] is indexed by hand");
 static_assert(kMaxParts * kMaxTop <= kListCap, "the joined parts' candidates fit the list");
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -217,6 +216,10 @@ __global__ __launch_bounds__(kRowThreads, 4) void logprobs_kernel(LogprobArgs p)
         st.w = fmaf(z, fmaxf(y, -200.f), st.w);  // 0 times -inf is not taken
         above += __builtin_popcountll(__ballot(v > given));
       }
+    // The sums as finished here: left open, they were taken further down,
+    // with every term held in a register until then.
+    above = __builtin_amdgcn_readfirstlane(above);
+    asm volatile("" : "+v"(st.s), "+v"(st.w), "+s"(above));
 
     if (kTop) {
       if (at == v0) {
@@ -250,28 +253,28 @@ __global__ __launch_bounds__(kRowThreads, 4) void logprobs_kernel(LogprobArgs p)
       for (;;) {
         const uint64_t tau = sh.tau;
         const float floor = tau == 0 ? -INFINITY : key_value(tau);
-        for (int i = 0; i < kVecs; ++i) {
-          // The few vectors that may hold a candidate are read again.
-          const float t = i == 0 ? tops[0] : i == 1 ? tops[1] : i == 2 ? tops[2] : tops[3];
-          const int v = at + i * kRowThreads + tid;
-          if (t < floor && !odd) continue;
-          int k0 = head + v * kN, k1 = k0 + kN;
-          if (at < v0) {
-            k0 = edge;
-            k1 = i == 0 && edge >= 0 ? edge + 1 : edge;
-          } else if (v >= v1) {
-            break;
-          }
-#pragma unroll 1
-          for (int k = k0; k < k1; ++k) {
-            const uint64_t key = order_key(static_cast<float>(x[k]), k);
-            if (key < tau) continue;
-            const int to = atomicAdd(&sh.count, 1);
-            if (to < kListCap) sh.list[to] = key;
+        if (__any(!(most < floor) || odd)) {
+#pragma unroll
+          for (int i = 0; i < kVecs; ++i) {
+            if (!__any(!(tops[i] < floor) || odd)) continue;
+            // The vector as new values, so that nothing of what follows is
+            // computed ahead of the test (and held in registers) for all.
+            int v = at + i * kRowThreads + tid;
+            asm volatile("" : "+v"(cur[i]), "+v"(v));
+#pragma unroll
+            for (int e = 0; e < kN; ++e) {
+              const float u = element<T>(cur[i], e);
+              if (u < floor) continue;
+              const bool real = at >= v0 ? v < v1 : edge >= 0 && i == 0 && e == 0;
+              const uint64_t key = order_key(u, at >= v0 ? head + v * kN + e : edge);
+              if (!real || key < tau) continue;
+              const int to = atomicAdd(&sh.count, 1);
+              if (to < kListCap) sh.list[to] = key;
+            }
           }
         }
         __syncthreads();
-        const int n = sh.count;
+        const int n = __builtin_amdgcn_readfirstlane(sh.count);
         __syncthreads();
         if (n <= kListCap) {
           held = n;
@@ -356,7 +359,7 @@ __global__ __launch_bounds__(kRowThreads, 4) void logprobs_kernel(LogprobArgs p)
         if (key != 0 && key >= least) sh.list[atomicAdd(&sh.count, 1)] = key;
       }
       __syncthreads();
-      held = sh.count;
+      held = __builtin_amdgcn_readfirstlane(sh.count);
       __syncthreads();
       held = cut_list(sh, held, p.top, tid);
     }
