@@ -48,7 +48,6 @@ constexpr int kChunkKeys = 32;                 // keys a wave stages at a time f
 // by 2^8: exponentials then stay within 2^8, far inside fp16, and most tiles
 // scale nothing.
 constexpr float kSlack = 8.f;
-constexpr int kOutside = 0x7FFFFF00;  // a buffer offset past every range: the load gives zeros
 
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -328,14 +327,12 @@ template <int DP, bool kValues, int kLoads>
 __device__ __forceinline__ void stage(const void* src, uint32_t stride, int dim, int rows, char* dst, int first) {
   using H = Head<DP>;
   const int lane = static_cast<int>(threadIdx.x) & 63;
-  const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(src), 0, 0x7FFFFF00, 0x00020000);
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
     const int r = (first + i) * H::kRowsPerLoad + lane / H::kChunks;
     const int c = (lane % H::kChunks) ^ (kValues ? H::value_swizzle(r) : H::key_swizzle(r));
     const int off = r < rows && c * 8 < dim ? static_cast<int>(r * stride) + c * 16 : kOutside;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        rsrc, (__attribute__((address_space(3))) void*)(dst + (first + i) * 1024), 16, off, 0, 0, 0);
+    load_to_lds(src, dst + (first + i) * 1024, off, 0);
   }
 }
 

@@ -10,6 +10,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "wp_device.h"
 #include "wp_model.h"
@@ -50,133 +51,474 @@ __device__ __forceinline__ u32x4 load_ragged(const T* p, int n) {
   return r;
 }
 
+constexpr int kRowsPerLoad = 8;       // staged rows that a wave's 16-byte-per-lane load fills
+
 // Tile of BT tokens x BN weight rows, WT x WN waves.  A gated tile's weight rows
 // are, per wave, half gate rows and half the up rows of the same outputs, so
 // that both factors of an output end in the same lane.
 //
 // LDS: a staged row is 64 columns, eight 16-byte chunks; row r keeps its
 // chunk c at place c ^ ((r >> 1) & 7), so the 16 rows a fragment load touches
-// at one c fall into all banks once.
-template <typename T, int BT, int BN, int WT, int WN>
+// at one c fall into all banks once.  Two buffers: a K-step's columns are
+// loaded while the step before is multiplied.
+//
+// A K-step is two halves of 32 columns.  A half's fragments are read from LDS
+// while the half before is multiplied, so that the matrix cores need not wait
+// for LDS after the step's one barrier.
+template <int BT, int BN, int WT, int WN>
 struct Tile {
   static constexpr int kWaves = WT * WN;
   static constexpr int kThreads = 64 * kWaves;
-  static constexpr int kT = BT / WT;       // tokens per wave
-  static constexpr int kN = BN / WN;       // weight rows per wave
-  static constexpr int kFT = kT / 16;      // token fragments
-  static constexpr int kFN = kN / 16;      // weight fragments
-  static constexpr int kLoadsX = BT * 8 / kThreads;  // 16-byte chunks per thread and K-step
-  static constexpr int kLoadsW = BN * 8 / kThreads;
+  static constexpr int kT = BT / WT;   // tokens per wave
+  static constexpr int kN = BN / WN;   // weight rows per wave
+  static constexpr int kFT = kT / 16;  // token fragments
+  static constexpr int kFN = kN / 16;  // weight fragments
+  static constexpr int kLoadsX = BT / kRowsPerLoad / kWaves;  // loads per wave and K-step
+  static constexpr int kLoadsW = BN / kRowsPerLoad / kWaves;
+  static_assert(kLoadsX >= 1 && kLoadsW >= 1, "every wave stages rows of both");
+  static_assert(kFN % 2 == 0, "a wave holds both factors of a gate");
 };
 
-template <typename T, int BT, int BN, int WT, int WN>
-__global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
-  using C = Tile<T, BT, BN, WT, WN>;
-  using V8 = typename VecOf<T>::v8;
-  __shared__ u32x4 sx[BT * 8];
-  __shared__ u32x4 sw[BN * 8];
-  const int tid = static_cast<int>(threadIdx.x);
-  const int lane = tid & 63;
-  const int wave = tid >> 6;
-  const int wt = wave % WT, wn = wave / WT;
-  const int tile = static_cast<int>(blockIdx.x);
-  const int tile_t = tile % p.tiles_t;
-  const int tile_n = tile / p.tiles_t;
-  const int64_t t0 = static_cast<int64_t>(tile_t) * BT;
-  const int gated = p.gated;
-  const int outs = gated ? BN / 2 : BN;  // outputs of the tile
-  const int n0 = tile_n * outs;
+// Weight row of row r of the tile that starts at output n0; past the weight
+// where `ok` is false.
+template <int kN>
+__device__ __forceinline__ int64_t weight_row(const ProjArgs& p, int n0, int r, bool* ok) {
+  if (!p.gated) {
+    *ok = n0 + r < p.n_out;
+    return n0 + r;
+  }
+  const int n = n0 + r / kN * (kN / 2) + r % (kN / 2);
+  *ok = n < p.n_out;
+  return n + (r % kN < kN / 2 ? 0 : static_cast<int64_t>(p.n_out));
+}
 
-  // Weight row of the tile's row r, or -1 past the weight.
-  auto weight_row = [&](int r) -> int64_t {
-    if (!gated) return n0 + r < p.n_out ? n0 + r : -1;
-    const int w = r / C::kN, i = r % C::kN;
-    const int n = n0 + w * (C::kN / 2) + i % (C::kN / 2);
-    return n < p.n_out ? n + (i < C::kN / 2 ? 0 : static_cast<int64_t>(p.n_out)) : -1;
+// Four consecutive outputs of one token: bias, activation, gate, residual, one
+// rounding.
+template <typename T>
+__device__ __forceinline__ void finish(const ProjArgs& p, int64_t t, int n, f32x4 a, f32x4 up) {
+  const T* bias = static_cast<const T*>(p.bias);
+  const T* res = static_cast<const T*>(p.residual);
+  T* y = static_cast<T*>(p.y) + t * p.ldy + n;
+  if (p.rows_vec && n + 4 <= p.n_out) {
+    if (bias) {
+      a += unpack4f<T>(*reinterpret_cast<const u32x2*>(bias + n));
+      if (p.gated) up += unpack4f<T>(*reinterpret_cast<const u32x2*>(bias + p.n_out + n));
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] = activate(a[e], p.act);
+    if (p.gated) a *= up;
+    if (res) a += unpack4f<T>(*reinterpret_cast<const u32x2*>(res + t * p.ldr + n));
+    store4(y, a);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (n + e >= p.n_out) break;
+    float v = activate(a[e] + (bias ? static_cast<float>(bias[n + e]) : 0.f), p.act);
+    if (p.gated) v *= up[e] + (bias ? static_cast<float>(bias[p.n_out + n + e]) : 0.f);
+    if (res) v += static_cast<float>(res[t * p.ldr + n + e]);
+    y[e] = static_cast<T>(v);
+  }
+}
+
+// The last of a tile's K-ranges to arrive: true in all of its threads, with the
+// counter cleared for the next call.  Every partial stored before is then visible.
+__device__ __forceinline__ bool last_split(uint32_t* cnt, int splits, uint32_t* flag) {
+  wait_vm();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const bool last = atomic_add_u(cnt, 1u) == static_cast<unsigned>(splits - 1);
+    if (last) atomic_store_u(cnt, 0u);
+    *flag = last ? 1u : 0u;
+  }
+  __syncthreads();
+  return *flag != 0u;
+}
+
+// kAligned: rows of x and w are 16-byte aligned and whole 16-byte vectors;
+// they go to LDS directly.  Else they pass through registers, read as their
+// alignment allows.
+template <typename T, int BT, int BN, int WT, int WN, bool kAligned>
+__global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
+  using C = Tile<BT, BN, WT, WN>;
+  using V8 = typename VecOf<T>::v8;
+  // An array per buffer: the compiler then knows that a load into one leaves
+  // reads of the others alone.
+  __shared__ __align__(1024) char sx0[BT * 128];
+  __shared__ __align__(1024) char sx1[BT * 128];
+  __shared__ __align__(1024) char sw0[BN * 128];
+  __shared__ __align__(1024) char sw1[BN * 128];
+  __shared__ uint32_t s_last;
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wt = wave % WT, wn = wave / WT;
+  int tile = static_cast<int>(blockIdx.x) / p.splits;
+  const int split = static_cast<int>(blockIdx.x) % p.splits;
+  const int n_tiles = p.tiles_t * p.tiles_n;
+  // Workgroups go to the eight XCDs in turn, and each XCD has an L2 of its
+  // own: an XCD takes a contiguous eighth of the tiles, which run through
+  // bands of eight token tiles, so that the tiles its compute units hold
+  // at a time share their rows of x and of w.
+  if (p.splits == 1) tile = tile % 8 * (n_tiles / 8) + std::min(tile % 8, n_tiles % 8) + tile / 8;
+  constexpr int kBand = 8;
+  const int band = tile / (kBand * p.tiles_n);
+  const int band_rows = std::min(kBand, p.tiles_t - band * kBand);
+  const int in_band = tile - band * kBand * p.tiles_n;
+  const int tile_t = band * kBand + in_band % band_rows, tile_n = in_band / band_rows;
+  const int64_t t0 = static_cast<int64_t>(tile_t) * BT;
+  const int n0 = tile_n * (p.gated ? BN / 2 : BN);
+  const int k_begin = split * p.k_range, k_end = std::min(p.d_in, k_begin + p.k_range);
+
+  // Fragment reads: lane's row and chunk; a second half's chunk is 4 further,
+  // which the swizzle turns into a flipped bit.
+  const int frag_row = lane & 15;
+  const int frag_off = frag_row * 128 + (((lane >> 4) ^ ((frag_row >> 1) & 7)) << 4);
+  auto fragment = [&](const char* rows, int row0, int half) {
+    return *reinterpret_cast<const V8*>(rows + row0 * 128 + (frag_off ^ (half * 64)));
+  };
+  f32x4 acc[C::kFN][C::kFT];
+#pragma unroll
+  for (int i = 0; i < C::kFN; ++i)
+#pragma unroll
+    for (int j = 0; j < C::kFT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  V8 aw[C::kFN], ax[C::kFT], bw[C::kFN], bx[C::kFT];
+  auto read = [&](const char* sx, const char* sw, int half, V8 (&fw)[C::kFN], V8 (&fx)[C::kFT]) {
+#pragma unroll
+    for (int i = 0; i < C::kFN; ++i) fw[i] = fragment(sw, wn * C::kN + i * 16, half);
+#pragma unroll
+    for (int j = 0; j < C::kFT; ++j) fx[j] = fragment(sx, wt * C::kT + j * 16, half);
+  };
+  auto multiply = [&](V8 (&fw)[C::kFN], V8 (&fx)[C::kFT]) {
+#pragma unroll
+    for (int j = 0; j < C::kFT; ++j)
+#pragma unroll
+      for (int i = 0; i < C::kFN; ++i) acc[i][j] = mfma16(fw[i], fx[j], acc[i][j]);
   };
 
-  f32x4 acc[C::kFN][C::kFT] = {};
-  const T* x = static_cast<const T*>(p.x);
-  const T* w = static_cast<const T*>(p.w);
-  for (int k0 = 0; k0 < p.d_in; k0 += kStepK) {
-    __syncthreads();
+  // Staging: lane l of load i fills chunk l % 8 of row (wave * loads + i) * 8
+  // + l / 8, and so takes the row's column chunk (l % 8) ^ ((row >> 1) & 7).
+  const int sub = lane >> 3;
+  if constexpr (kAligned) {
+    int col[2];  // by the parity of the row's group of eight
+#pragma unroll
+    for (int i = 0; i < 2; ++i) col[i] = ((lane & 7) ^ (i * 4 + (sub >> 1))) * 8;
+    int off_x[C::kLoadsX], off_w[C::kLoadsW];
+    const T* src_x[C::kLoadsX];
+    const T* src_w[C::kLoadsW];
+#pragma unroll
     for (int i = 0; i < C::kLoadsX; ++i) {
-      const int at = i * C::kThreads + tid, r = at >> 3, c = at & 7;
-      const int64_t t = t0 + r;
-      const int n = t < p.tokens ? p.d_in - k0 - c * 8 : 0;
-      sx[r * 8 + (c ^ ((r >> 1) & 7))] = load_ragged(x + t * p.ldx + k0 + c * 8, n);
+      const int g = wave * C::kLoadsX + i;
+      const int64_t t = t0 + g * kRowsPerLoad;
+      src_x[i] = static_cast<const T*>(p.x) + t * p.ldx;
+      off_x[i] = t + sub < p.tokens ? (sub * static_cast<int>(p.ldx) + col[g & 1]) * 2 : kOutside;
     }
+#pragma unroll
     for (int i = 0; i < C::kLoadsW; ++i) {
-      const int at = i * C::kThreads + tid, r = at >> 3, c = at & 7;
-      const int64_t row = weight_row(r);
-      const int n = row >= 0 ? p.d_in - k0 - c * 8 : 0;
-      sw[r * 8 + (c ^ ((r >> 1) & 7))] = load_ragged(w + row * p.ldw + k0 + c * 8, n);
+      const int g = wave * C::kLoadsW + i;
+      bool ok, first_ok;
+      const int64_t row = weight_row<C::kN>(p, n0, g * kRowsPerLoad, &first_ok);
+      (void)weight_row<C::kN>(p, n0, g * kRowsPerLoad + sub, &ok);
+      src_w[i] = static_cast<const T*>(p.w) + row * p.ldw;
+      off_w[i] = ok ? (sub * static_cast<int>(p.ldw) + col[g & 1]) * 2 : kOutside;
     }
-    __syncthreads();
+    auto stage = [&](int k, char* sx, char* sw) {
+      const bool in[2] = {k + col[0] < k_end, k + col[1] < k_end};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      V8 fw[C::kFN], fx[C::kFT];
-      const int c = h * 4 + (lane >> 4);
-#pragma unroll
-      for (int i = 0; i < C::kFN; ++i) {
-        const int r = wn * C::kN + i * 16 + (lane & 15);
-        fw[i] = __builtin_bit_cast(V8, sw[r * 8 + (c ^ ((r >> 1) & 7))]);
+      for (int i = 0; i < C::kLoadsX; ++i) {
+        const int g = wave * C::kLoadsX + i;
+        load_to_lds(src_x[i], sx + g * 1024, in[(C::kLoadsX % 2 ? g : i) & 1] ? off_x[i] : kOutside, k * 2);
       }
 #pragma unroll
-      for (int i = 0; i < C::kFT; ++i) {
-        const int r = wt * C::kT + i * 16 + (lane & 15);
-        fx[i] = __builtin_bit_cast(V8, sx[r * 8 + (c ^ ((r >> 1) & 7))]);
+      for (int i = 0; i < C::kLoadsW; ++i) {
+        const int g = wave * C::kLoadsW + i;
+        load_to_lds(src_w[i], sw + g * 1024, in[(C::kLoadsW % 2 ? g : i) & 1] ? off_w[i] : kOutside, k * 2);
+      }
+    };
+    auto step = [&](int k, char* sx, char* sw, const char* next_x, const char* next_w) {
+      read(sx, sw, 1, bw, bx);
+      multiply(aw, ax);
+      __syncthreads();
+      if (k + 2 * kStepK < k_end) stage(k + 2 * kStepK, sx, sw);
+      if (k + kStepK < k_end) read(next_x, next_w, 0, aw, ax);
+      multiply(bw, bx);
+    };
+    if (k_begin < k_end) {
+      stage(k_begin, sx0, sw0);
+      __syncthreads();
+      if (k_begin + kStepK < k_end) stage(k_begin + kStepK, sx1, sw1);
+      read(sx0, sw0, 0, aw, ax);
+      for (int k = k_begin; k < k_end; k += 2 * kStepK) {
+        step(k, sx0, sw0, sx1, sw1);
+        if (k + kStepK < k_end) step(k + kStepK, sx1, sw1, sx0, sw0);
+      }
+    }
+  } else {
+    u32x4 rx[C::kLoadsX], rw[C::kLoadsW];
+    auto gather = [&](int k) {
+#pragma unroll
+      for (int i = 0; i < C::kLoadsX; ++i) {
+        const int r = (wave * C::kLoadsX + i) * kRowsPerLoad + sub, c = (lane & 7) ^ ((r >> 1) & 7);
+        const int64_t t = t0 + r;
+        rx[i] = load_ragged(static_cast<const T*>(p.x) + t * p.ldx + k + c * 8, t < p.tokens ? k_end - k - c * 8 : 0);
       }
 #pragma unroll
-      for (int i = 0; i < C::kFN; ++i)
+      for (int i = 0; i < C::kLoadsW; ++i) {
+        const int r = (wave * C::kLoadsW + i) * kRowsPerLoad + sub, c = (lane & 7) ^ ((r >> 1) & 7);
+        bool ok;
+        const int64_t row = weight_row<C::kN>(p, n0, r, &ok);
+        rw[i] = load_ragged(static_cast<const T*>(p.w) + row * p.ldw + k + c * 8, ok ? k_end - k - c * 8 : 0);
+      }
+    };
+    gather(k_begin);
+    for (int k = k_begin; k < k_end; k += kStepK) {
+      __syncthreads();
 #pragma unroll
-        for (int j = 0; j < C::kFT; ++j) acc[i][j] = mfma16(fw[i], fx[j], acc[i][j]);
+      for (int i = 0; i < C::kLoadsX; ++i)
+        *reinterpret_cast<u32x4*>(sx0 + (wave * C::kLoadsX + i) * 1024 + lane * 16) = rx[i];
+#pragma unroll
+      for (int i = 0; i < C::kLoadsW; ++i)
+        *reinterpret_cast<u32x4*>(sw0 + (wave * C::kLoadsW + i) * 1024 + lane * 16) = rw[i];
+      __syncthreads();
+      gather(k + kStepK);
+      read(sx0, sw0, 0, aw, ax);
+      multiply(aw, ax);
+      read(sx0, sw0, 1, bw, bx);
+      multiply(bw, bx);
     }
   }
 
-  // Lane: token lane & 15 of a fragment, features (lane >> 4) * 4 + e.
-  const T* bias = static_cast<const T*>(p.bias);
-  const T* res = static_cast<const T*>(p.residual);
-  T* y = static_cast<T*>(p.y);
-  const int n_frags = gated ? C::kFN / 2 : C::kFN;
-  const int wave_n = n0 + wn * (gated ? C::kN / 2 : C::kN);
+  if (p.splits > 1) {
+    // Partial tiles in the lanes' own order, added in the order of the
+    // K-ranges by the last to arrive.
+    constexpr uint32_t kTileBytes = BT * BN * 4;
+    char* parts = reinterpret_cast<char*>(p.part) + static_cast<uint64_t>(tile) * p.splits * kTileBytes;
+    const uint32_t at = static_cast<uint32_t>(wave * C::kFN * C::kFT * 64 + lane) * 16;
+    const __amdgpu_buffer_rsrc_t mine = coherent_buffer(parts + static_cast<uint64_t>(split) * kTileBytes, kTileBytes);
 #pragma unroll
-  for (int i = 0; i < C::kFN; ++i) {
-    if (i >= n_frags) break;
-    const int n = wave_n + i * 16 + (lane >> 4) * 4;
+    for (int i = 0; i < C::kFN; ++i)
 #pragma unroll
-    for (int j = 0; j < C::kFT; ++j) {
-      const int64_t t = t0 + wt * C::kT + j * 16 + (lane & 15);
-      if (t >= p.tokens) continue;
+      for (int j = 0; j < C::kFT; ++j) coherent_store16(mine, at + (i * C::kFT + j) * 1024, acc[i][j]);
+    if (!last_split(p.tile_cnt + tile, p.splits, &s_last)) return;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (n + e >= p.n_out) break;
-        float v = acc[i][j][e] + (bias ? static_cast<float>(bias[n + e]) : 0.f);
-        v = activate(v, p.act);
-        if (gated)
-          v *= acc[(i + C::kFN / 2) % C::kFN][j][e] + (bias ? static_cast<float>(bias[p.n_out + n + e]) : 0.f);
-        if (res) v += static_cast<float>(res[t * p.ldr + n + e]);
-        y[t * p.ldy + n + e] = static_cast<T>(v);
+    for (int i = 0; i < C::kFN; ++i)
+#pragma unroll
+      for (int j = 0; j < C::kFT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < p.splits; ++s) {
+      const __amdgpu_buffer_rsrc_t one = coherent_buffer(parts + static_cast<uint64_t>(s) * kTileBytes, kTileBytes);
+#pragma unroll
+      for (int i = 0; i < C::kFN; ++i)
+#pragma unroll
+        for (int j = 0; j < C::kFT; ++j) acc[i][j] += coherent_load16(one, at + (i * C::kFT + j) * 1024);
+    }
+  }
+
+  // Epilogue, through LDS: a wave writes its sums as rows of kN features of a
+  // token (16-byte chunk c of token t's row at c ^ (t % chunks), so that
+  // neither side's 16 lanes share a bank) and takes them back with the lanes
+  // along a row, which makes residual reads and stores whole lines.  A lane
+  // holds token lane & 15 of a fragment, four features from (lane >> 4) * 4.
+  constexpr int kChunks = C::kN / 4;
+  constexpr int kPassFrags = std::min(C::kFT, 4);
+  constexpr int kWaveBytes = kPassFrags * 16 * C::kN * 4;
+  constexpr int kPerArray = C::kWaves / 4;
+  static_assert(C::kWaves % 4 == 0 && kPerArray * kWaveBytes <= BT * 128 && kPerArray * kWaveBytes <= BN * 128 &&
+                    C::kFT % kPassFrags == 0,
+                "a wave's rows of a pass fit its share of an array");
+  const int array = wave / kPerArray;
+  char* rows = (array == 0 ? sx0 : array == 1 ? sx1 : array == 2 ? sw0 : sw1) + wave % kPerArray * kWaveBytes;
+  const int outs = p.gated ? C::kN / 2 : C::kN;  // a row's outputs
+  const int wave_n = n0 + wn * outs;
+  const int lanes = outs / 4;  // along a row
+  const int c = lane % lanes;
+  __syncthreads();
+#pragma unroll
+  for (int pass = 0; pass < C::kFT / kPassFrags; ++pass) {
+#pragma unroll
+    for (int j = 0; j < kPassFrags; ++j)
+#pragma unroll
+      for (int i = 0; i < C::kFN; ++i) {
+        const int t = j * 16 + (lane & 15), q = i * 4 + (lane >> 4);
+        *reinterpret_cast<f32x4*>(rows + t * (C::kN * 4) + ((q ^ (t & (kChunks - 1))) << 4)) =
+            acc[i][pass * kPassFrags + j];
       }
+    for (int r = lane / lanes; r < kPassFrags * 16; r += 64 / lanes) {
+      const int64_t t = t0 + wt * C::kT + pass * kPassFrags * 16 + r;
+      const int n = wave_n + c * 4;
+      if (t >= p.tokens) break;
+      if (n >= p.n_out) continue;
+      const char* row = rows + r * (C::kN * 4);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(row + ((c ^ (r & (kChunks - 1))) << 4));
+      f32x4 up = v;
+      if (p.gated) up = *reinterpret_cast<const f32x4*>(row + (((c + kChunks / 2) ^ (r & (kChunks - 1))) << 4));
+      finish<T>(p, t, n, v, up);
     }
   }
 }
 
-template <typename T, int BT, int BN, int WT, int WN>
-hipError_t launch_tile(ProjArgs& a, hipStream_t stream) {
+// Few tokens: a workgroup takes 16 outputs (16 gate and 16 up rows) for all
+// of them and its eight waves share out the columns, 64 (a row's 128 bytes) at
+// a time; every weight goes from memory to a register once and is used there.
+// Bound by the weight's bytes.
+constexpr int kRowWaves = 8;
+constexpr int kRowThreads = 64 * kRowWaves;
+constexpr int kRowDepth = 4;  // 64-column blocks in flight per wave
+
+template <typename T, int kFT, bool kAligned>
+__global__ __launch_bounds__(kRowThreads) void proj_rows_kernel(ProjArgs p) {
+  using V8 = typename VecOf<T>::v8;
+  __shared__ f32x4 s_acc[kRowWaves][2][kFT][64];
+  __shared__ uint32_t s_last;
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tile = static_cast<int>(blockIdx.x) / p.splits, split = static_cast<int>(blockIdx.x) % p.splits;
+  const int n0 = tile * 16;
+  const int k_begin = split * p.k_range, k_end = std::min(p.d_in, k_begin + p.k_range);
+  const int n = n0 + (lane & 15);
+  const bool row_ok = n < p.n_out;
+  const int kc = (lane >> 4) * 8;
+  const T* w0 = static_cast<const T*>(p.w) + static_cast<int64_t>(n) * p.ldw + kc;
+  const T* w1 = w0 + static_cast<int64_t>(p.n_out) * p.ldw;
+  const T* x[kFT];
+  bool tok_ok[kFT];
+#pragma unroll
+  for (int j = 0; j < kFT; ++j) {
+    const int64_t t = j * 16 + (lane & 15);
+    tok_ok[j] = t < p.tokens;
+    x[j] = static_cast<const T*>(p.x) + t * p.ldx + kc;
+  }
+  auto get = [&](const T* row, bool ok, int k) -> V8 {
+    if constexpr (kAligned) return ok && k + kc < k_end ? load8(row + k) : zero8<T>();
+    return __builtin_bit_cast(V8, load_ragged(row + k, ok ? k_end - k - kc : 0));
+  };
+  f32x4 acc[2][kFT];
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+#pragma unroll
+    for (int j = 0; j < kFT; ++j) acc[g][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto run = [&](auto gated) {
+    constexpr int kG = decltype(gated)::value ? 2 : 1;
+    constexpr int kDepth = kRowDepth / kG;
+    for (int k = k_begin + wave * kStepK; k < k_end; k += kRowWaves * kStepK * kDepth) {
+      V8 fw[kDepth][2][kG], fx[kDepth][2][kFT];
+#pragma unroll
+      for (int b = 0; b < kDepth; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int at = k + b * kRowWaves * kStepK + h * 32;
+          fw[b][h][0] = get(w0, row_ok, at);
+          if constexpr (kG == 2) fw[b][h][1] = get(w1, row_ok, at);
+#pragma unroll
+          for (int j = 0; j < kFT; ++j) fx[b][h][j] = get(x[j], tok_ok[j], at);
+        }
+#pragma unroll
+      for (int b = 0; b < kDepth; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int g = 0; g < kG; ++g)
+#pragma unroll
+            for (int j = 0; j < kFT; ++j) acc[g][j] = mfma16(fw[b][h][g], fx[b][h][j], acc[g][j]);
+    }
+  };
+  if (p.gated)
+    run(std::integral_constant<bool, true>{});
+  else
+    run(std::integral_constant<bool, false>{});
+
+  const int kG = p.gated ? 2 : 1;
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+    if (g < kG)
+#pragma unroll
+      for (int j = 0; j < kFT; ++j) s_acc[wave][g][j][lane] = acc[g][j];
+  __syncthreads();
+  // Wave j joins token fragment j.
+  f32x4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  if (wave < kFT)
+    for (int g = 0; g < kG; ++g)
+#pragma unroll
+      for (int i = 0; i < kRowWaves; ++i) sum[g] += s_acc[i][g][wave][lane];
+  if (p.splits > 1) {
+    constexpr uint32_t kTileBytes = 2 * kFT * 1024;
+    char* parts = reinterpret_cast<char*>(p.part) + static_cast<uint64_t>(tile) * p.splits * kTileBytes;
+    const uint32_t at = static_cast<uint32_t>(wave * 64 + lane) * 16;
+    if (wave < kFT) {
+      const __amdgpu_buffer_rsrc_t mine = coherent_buffer(parts + static_cast<uint64_t>(split) * kTileBytes, kTileBytes);
+      for (int g = 0; g < kG; ++g) coherent_store16(mine, at + g * kFT * 1024, sum[g]);
+    }
+    if (!last_split(p.tile_cnt + tile, p.splits, &s_last)) return;
+    if (wave < kFT) {
+      sum[0] = sum[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < p.splits; ++s) {
+        const __amdgpu_buffer_rsrc_t one = coherent_buffer(parts + static_cast<uint64_t>(s) * kTileBytes, kTileBytes);
+        for (int g = 0; g < kG; ++g) sum[g] += coherent_load16(one, at + g * kFT * 1024);
+      }
+    }
+  }
+  const int64_t t = wave * 16 + (lane & 15);
+  const int out = n0 + (lane >> 4) * 4;
+  if (wave < kFT && t < p.tokens && out < p.n_out) finish<T>(p, t, out, sum[0], sum[1]);
+}
+
+// K-ranges of a launch of `tiles` workgroups: as many as bring it to `want`
+// of them, each of at least `least` columns, within the scratch.
+void split_columns(ProjArgs& a, int64_t tiles, int64_t want, int least, uint64_t tile_bytes) {
+  int64_t splits = tiles >= want ? 1 : want / tiles;
+  splits = std::max<int64_t>(1, std::min<int64_t>(splits, a.d_in / least));
+  while (splits > 1 && static_cast<uint64_t>(tiles * splits) * tile_bytes > a.part_bytes) --splits;
+  if (tiles > a.n_cnt) splits = 1;
+  const int64_t steps = std::max<int64_t>(1, (a.d_in + kStepK - 1) / kStepK);
+  a.k_range = static_cast<int32_t>((steps + splits - 1) / splits * kStepK);
+  a.splits = static_cast<int32_t>(std::max<int64_t>(1, (static_cast<int64_t>(a.d_in) + a.k_range - 1) / a.k_range));
+}
+
+template <typename T, int BT, int BN, int WT, int WN, bool kAligned>
+hipError_t launch_tiles(ProjArgs& a, int64_t want, hipStream_t stream) {
   const int outs = a.gated ? BN / 2 : BN;
   a.tiles_t = static_cast<int32_t>((a.tokens + BT - 1) / BT);
   a.tiles_n = (a.n_out + outs - 1) / outs;
-  hipLaunchKernelGGL((proj_kernel<T, BT, BN, WT, WN>), dim3(static_cast<uint32_t>(a.tiles_t) * a.tiles_n),
+  const int64_t tiles = static_cast<int64_t>(a.tiles_t) * a.tiles_n;
+  split_columns(a, tiles, want, 4 * kStepK, static_cast<uint64_t>(BT) * BN * 4);
+  if (tiles * a.splits > 0x7FFFFFFF) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((proj_kernel<T, BT, BN, WT, WN, kAligned>), dim3(static_cast<uint32_t>(tiles * a.splits)),
                      dim3(64 * WT * WN), 0, stream, a);
   return hipGetLastError();
+}
+
+template <typename T, int kFT, bool kAligned>
+hipError_t launch_rows(ProjArgs& a, int64_t want, hipStream_t stream) {
+  a.tiles_t = 1;
+  a.tiles_n = (a.n_out + 15) / 16;
+  split_columns(a, a.tiles_n, want, kRowWaves * kStepK, 2 * kFT * 1024);
+  if (static_cast<int64_t>(a.tiles_n) * a.splits > 0x7FFFFFFF) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((proj_rows_kernel<T, kFT, kAligned>), dim3(static_cast<uint32_t>(a.tiles_n) * a.splits),
+                     dim3(kRowThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+template <typename T, bool kAligned>
+hipError_t launch(ProjArgs& a, int n_cu, hipStream_t stream) {
+  if (a.tokens <= 16) return launch_rows<T, 1, kAligned>(a, n_cu, stream);
+  if (a.tokens <= 32) return launch_rows<T, 2, kAligned>(a, n_cu, stream);
+  const int64_t rows = static_cast<int64_t>(a.n_out) * (a.gated ? 2 : 1);
+  auto tiles = [&](int64_t bt, int64_t bn) { return (a.tokens + bt - 1) / bt * ((rows + bn - 1) / bn); };
+  if constexpr (kAligned) {
+    if (tiles(256, 256) >= n_cu * 3 / 4) return launch_tiles<T, 256, 256, 2, 4, kAligned>(a, 1, stream);
+  }
+  if (tiles(128, 128) >= n_cu) return launch_tiles<T, 128, 128, 2, 2, kAligned>(a, 1, stream);
+  return launch_tiles<T, 64, 64, 2, 2, kAligned>(a, 2 * n_cu, stream);
 }
 
 }  // namespace
 
 hipError_t launch_proj(int dtype_bf16, ProjArgs& a, int n_cu, hipStream_t stream) {
-  (void)n_cu;
-  return dtype_bf16 ? launch_tile<__bf16, 128, 128, 2, 2>(a, stream) : launch_tile<_Float16, 128, 128, 2, 2>(a, stream);
+  auto whole = [](const void* p, int64_t ld, int bytes) {
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld % (bytes / 2) == 0;
+  };
+  a.rows_vec = whole(a.y, a.ldy, 8) && whole(a.residual, a.ldr, 8) && whole(a.bias, a.gated ? a.n_out : 0, 8);
+  const bool aligned = a.d_in % 8 == 0 && whole(a.x, a.ldx, 16) && whole(a.w, a.ldw, 16);
+  if (dtype_bf16) return aligned ? launch<__bf16, true>(a, n_cu, stream) : launch<__bf16, false>(a, n_cu, stream);
+  return aligned ? launch<_Float16, true>(a, n_cu, stream) : launch<_Float16, false>(a, n_cu, stream);
 }
 
 }  // namespace wp
