@@ -234,18 +234,41 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
         load_to_lds(src_w[i], sw + g * 1024, in[(C::kLoadsW % 2 ? g : i) & 1] ? off_w[i] : kOutside, k * 2);
       }
     };
+    // One K-step.  Past k_end stage() loads zeros (without memory traffic) and
+    // read() what nobody uses, so that a step is free of branches and its
+    // reads, loads and products can be put in order: each read or load between two products, so
+    // that issuing them leaves no gap in the matrix cores' work.
+    constexpr int kReads = C::kFN + C::kFT, kProducts = C::kFN * C::kFT, kLoads = C::kLoadsX + C::kLoadsW;
     auto step = [&](int k, char* sx, char* sw, const char* next_x, const char* next_w) {
       read(sx, sw, 1, bw, bx);
       multiply(aw, ax);
+#pragma unroll
+      for (int i = 0; i < kReads; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // product
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, kProducts > kReads ? kProducts - kReads : 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
       __syncthreads();
-      if (k + 2 * kStepK < k_end) stage(k + 2 * kStepK, sx, sw);
-      if (k + kStepK < k_end) read(next_x, next_w, 0, aw, ax);
+      stage(k + 2 * kStepK, sx, sw);
+      read(next_x, next_w, 0, aw, ax);
       multiply(bw, bx);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);  // load
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kReads; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     };
     if (k_begin < k_end) {
       stage(k_begin, sx0, sw0);
       __syncthreads();
-      if (k_begin + kStepK < k_end) stage(k_begin + kStepK, sx1, sw1);
+      stage(k_begin + kStepK, sx1, sw1);
       read(sx0, sw0, 0, aw, ax);
       for (int k = k_begin; k < k_end; k += 2 * kStepK) {
         step(k, sx0, sw0, sx1, sw1);
