@@ -20,16 +20,24 @@ namespace {
 
 constexpr int kStepK = 64;  // columns of x and W staged per K-step: 128 bytes of a row
 
-__device__ __forceinline__ float activate(float v, int act) {
-  switch (act) {
+// 1 / (1 + exp(-v)) by the hardware's exponential and reciprocal (an ulp each;
+// an IEEE division would take as long as the rest of an epilogue).
+__device__ __forceinline__ float sigmoid(float v) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+}
+
+template <int kAct>
+__device__ __forceinline__ float activate(float v) {
+  switch (kAct) {
     case kActRelu:
       return v < 0.f ? 0.f : v;  // NaN stays
     case kActGelu:
       return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
     case kActGeluTanh:
-      return 0.5f * v * (1.f + tanhf(0.79788456080286536f * (v + 0.044715f * v * v * v)));
+      // 0.5 v (1 + tanh u) = v sigmoid(2 u)
+      return v * sigmoid(1.5957691216057308f * (v + 0.044715f * v * v * v));
     case kActSilu:
-      return v / (1.f + __expf(-v));
+      return v * sigmoid(v);
     default:
       return v;
   }
@@ -93,31 +101,43 @@ __device__ __forceinline__ int64_t weight_row(const ProjArgs& p, int n0, int r, 
 }
 
 // Four consecutive outputs of one token: bias, activation, gate, residual, one
-// rounding.
-template <typename T>
+// rounding.  kWhole: all four exist, and every tensor takes 8-byte accesses.
+template <typename T, int kAct, bool kWhole>
 __device__ __forceinline__ void finish(const ProjArgs& p, int64_t t, int n, f32x4 a, f32x4 up) {
   const T* bias = static_cast<const T*>(p.bias);
   const T* res = static_cast<const T*>(p.residual);
   T* y = static_cast<T*>(p.y) + t * p.ldy + n;
-  if (p.rows_vec && n + 4 <= p.n_out) {
+  if constexpr (kWhole) {
     if (bias) {
       a += unpack4f<T>(*reinterpret_cast<const u32x2*>(bias + n));
       if (p.gated) up += unpack4f<T>(*reinterpret_cast<const u32x2*>(bias + p.n_out + n));
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) a[e] = activate(a[e], p.act);
+    for (int e = 0; e < 4; ++e) a[e] = activate<kAct>(a[e]);
     if (p.gated) a *= up;
     if (res) a += unpack4f<T>(*reinterpret_cast<const u32x2*>(res + t * p.ldr + n));
     store4(y, a);
-    return;
-  }
+  } else {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if (n + e >= p.n_out) break;
-    float v = activate(a[e] + (bias ? static_cast<float>(bias[n + e]) : 0.f), p.act);
-    if (p.gated) v *= up[e] + (bias ? static_cast<float>(bias[p.n_out + n + e]) : 0.f);
-    if (res) v += static_cast<float>(res[t * p.ldr + n + e]);
-    y[e] = static_cast<T>(v);
+    for (int e = 0; e < 4; ++e) {
+      if (n + e >= p.n_out) break;
+      float v = activate<kAct>(a[e] + (bias ? static_cast<float>(bias[n + e]) : 0.f));
+      if (p.gated) v *= up[e] + (bias ? static_cast<float>(bias[p.n_out + n + e]) : 0.f);
+      if (res) v += static_cast<float>(res[t * p.ldr + n + e]);
+      y[e] = static_cast<T>(v);
+    }
+  }
+}
+
+// Calls f with the activation as a constant: one test for a whole epilogue.
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F f) {
+  switch (act) {
+    case kActRelu: return f(std::integral_constant<int, kActRelu>{});
+    case kActGelu: return f(std::integral_constant<int, kActGelu>{});
+    case kActGeluTanh: return f(std::integral_constant<int, kActGeluTanh>{});
+    case kActSilu: return f(std::integral_constant<int, kActSilu>{});
+    default: return f(std::integral_constant<int, kActNone>{});
   }
 }
 
@@ -351,8 +371,10 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
   char* rows = (array == 0 ? sx0 : array == 1 ? sx1 : array == 2 ? sw0 : sw1) + wave % kPerArray * kWaveBytes;
   const int outs = p.gated ? C::kN / 2 : C::kN;  // a row's outputs
   const int wave_n = n0 + wn * outs;
+  const int64_t wave_t = t0 + wt * C::kT;
   const int lanes = outs / 4;  // along a row
-  const int c = lane % lanes;
+  const int c = lane % lanes, row0 = lane / lanes, row_step = 64 / lanes;
+  const bool whole = p.rows_vec && wave_t + C::kT <= p.tokens && wave_n + outs <= p.n_out;
   __syncthreads();
 #pragma unroll
   for (int pass = 0; pass < C::kFT / kPassFrags; ++pass) {
@@ -364,17 +386,23 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
         *reinterpret_cast<f32x4*>(rows + t * (C::kN * 4) + ((q ^ (t & (kChunks - 1))) << 4)) =
             acc[i][pass * kPassFrags + j];
       }
-    for (int r = lane / lanes; r < kPassFrags * 16; r += 64 / lanes) {
-      const int64_t t = t0 + wt * C::kT + pass * kPassFrags * 16 + r;
-      const int n = wave_n + c * 4;
-      if (t >= p.tokens) break;
-      if (n >= p.n_out) continue;
-      const char* row = rows + r * (C::kN * 4);
-      const f32x4 v = *reinterpret_cast<const f32x4*>(row + ((c ^ (r & (kChunks - 1))) << 4));
-      f32x4 up = v;
-      if (p.gated) up = *reinterpret_cast<const f32x4*>(row + (((c + kChunks / 2) ^ (r & (kChunks - 1))) << 4));
-      finish<T>(p, t, n, v, up);
-    }
+    auto sum_of = [&](int r, int chunk) {
+      return *reinterpret_cast<const f32x4*>(rows + r * (C::kN * 4) + ((chunk ^ (r & (kChunks - 1))) << 4));
+    };
+    const int64_t pass_t = wave_t + pass * kPassFrags * 16;
+    const int n = wave_n + c * 4;
+    with_activation(p.act, [&](auto act) {
+      constexpr int kAct = decltype(act)::value;
+      if (whole) {
+#pragma unroll 4
+        for (int r = row0; r < kPassFrags * 16; r += row_step)
+          finish<T, kAct, true>(p, pass_t + r, n, sum_of(r, c), sum_of(r, c + (p.gated ? kChunks / 2 : 0)));
+      } else {
+        for (int r = row0; r < kPassFrags * 16; r += row_step)
+          if (pass_t + r < p.tokens && n < p.n_out)
+            finish<T, kAct, false>(p, pass_t + r, n, sum_of(r, c), sum_of(r, c + (p.gated ? kChunks / 2 : 0)));
+      }
+    });
   }
 }
 
@@ -480,7 +508,13 @@ __global__ __launch_bounds__(kRowThreads) void proj_rows_kernel(ProjArgs p) {
   }
   const int64_t t = wave * 16 + (lane & 15);
   const int out = n0 + (lane >> 4) * 4;
-  if (wave < kFT && t < p.tokens && out < p.n_out) finish<T>(p, t, out, sum[0], sum[1]);
+  if (wave < kFT && t < p.tokens && out < p.n_out)
+    with_activation(p.act, [&](auto act) {
+      if (p.rows_vec && out + 4 <= p.n_out)
+        finish<T, decltype(act)::value, true>(p, t, out, sum[0], sum[1]);
+      else
+        finish<T, decltype(act)::value, false>(p, t, out, sum[0], sum[1]);
+    });
 }
 
 // K-ranges of a launch of `tiles` workgroups: as many as bring it to `want`
