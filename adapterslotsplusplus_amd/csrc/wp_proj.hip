@@ -141,6 +141,23 @@ __device__ __forceinline__ void with_activation(int act, F f) {
   }
 }
 
+// Waits until at most kLeft of this wave's loads are on their way and its LDS
+// reads are done, then for the workgroup.  By the builtins, whose counts the
+// compiler sees: it then adds no wait of its own to the reads behind them.
+template <int kLeft>
+__device__ __forceinline__ void staged_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((kLeft & 15) | (kLeft >> 4) << 14 | 7 << 4);  // vmcnt(kLeft) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Four bytes a lane from anywhere to LDS, for the line they bring into L2.
+__device__ __forceinline__ void touch_line(const void* src, char* dst) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                   (__attribute__((address_space(3))) void*)dst, 4, 0, 0);
+}
+
 // The last of a tile's K-ranges to arrive: true in all of its threads, with the
 // counter cleared for the next call.  Every partial stored before is then visible.
 __device__ __forceinline__ bool last_split(uint32_t* cnt, int splits, uint32_t* flag) {
@@ -169,6 +186,14 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
   __shared__ __align__(1024) char sw0[BN * 128];
   __shared__ __align__(1024) char sw1[BN * 128];
   __shared__ uint32_t s_last;
+  // The largest tile leaves a compute unit to one workgroup, whose loads have
+  // one K-step (about 1 us) to arrive: enough from L2, not always from behind
+  // it.  So each step also touches lines of a step four further on.  The rows of
+  // x are shared by the tiles beside this one that the XCD's 32 compute units hold at the same
+  // time, those of w by the band's: each tile touches its share.
+  // (8192 x 5120 x 27648: 1785 us without, 1719 with.)
+  constexpr bool kTouch = kAligned && BT * BN >= 256 * 256;
+  __shared__ char s_touch[kTouch ? 256 : 4];
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wt = wave % WT, wn = wave / WT;
@@ -254,6 +279,24 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
         load_to_lds(src_w[i], sw + g * 1024, in[(C::kLoadsW % 2 ? g : i) & 1] ? off_w[i] : kOutside, k * 2);
       }
     };
+    const T* line = nullptr;
+    if constexpr (kTouch) {
+      const int beside = std::max(1, 32 / band_rows);
+      const int n_x = (BT + beside - 1) / beside, n_w = (BN + band_rows - 1) / band_rows;
+      int at = lane * C::kWaves + wave;  // of the tile's n_x + n_w lines; lanes past them repeat the first
+      if (at >= n_x + n_w) at = 0;
+      bool ok;
+      const int r = at < n_x ? tile_n % beside * n_x + at : tile_t % band_rows * n_w + at - n_x;
+      if (at < n_x) {
+        const int64_t t = std::min(t0 + r, p.tokens - 1);
+        line = static_cast<const T*>(p.x) + t * p.ldx;
+      } else {
+        const int64_t row = weight_row<C::kN>(p, n0, std::min(r, BN - 1), &ok);
+        line = static_cast<const T*>(p.w) + (ok ? row : 0) * p.ldw;
+      }
+    }
+    constexpr int kAhead = 6 * kStepK;  // from the step that is multiplied
+    constexpr int kTouches = kTouch ? 1 : 0;
     // One K-step.  Past k_end stage() loads zeros (without memory traffic) and
     // read() what nobody uses, so that a step is free of branches and its
     // reads, loads and products can be put in order: each read or load between two products, so
@@ -269,12 +312,13 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
       }
       __builtin_amdgcn_sched_group_barrier(0x008, kProducts > kReads ? kProducts - kReads : 0, 0);
       __builtin_amdgcn_sched_barrier(0);
-      __syncthreads();
+      staged_barrier<kTouches>();
       stage(k + 2 * kStepK, sx, sw);
+      if constexpr (kTouch) touch_line(line + std::min(k + kAhead, k_end - 8), s_touch);
       read(next_x, next_w, 0, aw, ax);
       multiply(bw, bx);
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
+      for (int i = 0; i < kLoads + kTouches; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);  // load
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       }
@@ -287,8 +331,9 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
     };
     if (k_begin < k_end) {
       stage(k_begin, sx0, sw0);
-      __syncthreads();
+      staged_barrier<0>();
       stage(k_begin + kStepK, sx1, sw1);
+      if constexpr (kTouch) touch_line(line + std::min(k_begin + 2 * kStepK, k_end - 8), s_touch);
       read(sx0, sw0, 0, aw, ax);
       for (int k = k_begin; k < k_end; k += 2 * kStepK) {
         step(k, sx0, sw0, sx1, sw1);
@@ -375,6 +420,7 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
   const int lanes = outs / 4;  // along a row
   const int c = lane % lanes, row0 = lane / lanes, row_step = 64 / lanes;
   const bool whole = p.rows_vec && wave_t + C::kT <= p.tokens && wave_n + outs <= p.n_out;
+  wait_vm();  // loads past the last column write LDS too
   __syncthreads();
 #pragma unroll
   for (int pass = 0; pass < C::kFT / kPassFrags; ++pass) {
