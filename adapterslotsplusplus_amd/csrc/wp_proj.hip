@@ -65,15 +65,17 @@ constexpr int kRowsPerLoad = 8;       // staged rows that a wave's 16-byte-per-l
 // are, per wave, half gate rows and half the up rows of the same outputs, so
 // that both factors of an output end in the same lane.
 //
-// LDS: a staged row is 64 columns, eight 16-byte chunks; row r keeps its
-// chunk c at place c ^ ((r >> 1) & 7), so the 16 rows a fragment load touches
-// at one c fall into all banks once.  Two buffers: a K-step's columns are
-// loaded while the step before is multiplied.
-//
-// A K-step is two halves of 32 columns.  A half's fragments are read from LDS
+// LDS is a ring of R slots, one K-step's 64 columns of the tile's rows each;
+// a step is two halves of 32 columns.  A half's fragments are read from LDS
 // while the half before is multiplied, so that the matrix cores need not wait
-// for LDS after the step's one barrier.
-template <int BT, int BN, int WT, int WN>
+// for LDS after the step's one barrier.  Past that barrier every wave has read
+// the slot that is refilled then, and every wave's loads of the slot that
+// is read next have landed: they had R - 1 steps for it.
+//
+// A staged row is eight 16-byte chunks; row r keeps its chunk c at place
+// c ^ ((r >> 1) & 7), so the 16 rows a fragment read touches at one c fall into
+// all banks once.
+template <int BT, int BN, int WT, int WN, int R>
 struct Tile {
   static constexpr int kWaves = WT * WN;
   static constexpr int kThreads = 64 * kWaves;
@@ -83,8 +85,12 @@ struct Tile {
   static constexpr int kFN = kN / 16;  // weight fragments
   static constexpr int kLoadsX = BT / kRowsPerLoad / kWaves;  // loads per wave and K-step
   static constexpr int kLoadsW = BN / kRowsPerLoad / kWaves;
+  static constexpr int kLoads = kLoadsX + kLoadsW;
+  static constexpr int kXBytes = BT * kStepK * 2;  // of a slot
+  static constexpr int kWBytes = BN * kStepK * 2;
   static_assert(kLoadsX >= 1 && kLoadsW >= 1, "every wave stages rows of both");
   static_assert(kFN % 2 == 0, "a wave holds both factors of a gate");
+  static_assert(R == 2 || R == 4, "the steps of a round are written out");
 };
 
 // Weight row of row r of the tile that starts at output n0; past the weight
@@ -175,17 +181,23 @@ __device__ __forceinline__ bool last_split(uint32_t* cnt, int splits, uint32_t* 
 // kAligned: rows of x and w are 16-byte aligned and whole 16-byte vectors;
 // they go to LDS directly.  Else they pass through registers, read as their
 // alignment allows.
-template <typename T, int BT, int BN, int WT, int WN, bool kAligned>
-__global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
-  using C = Tile<BT, BN, WT, WN>;
+template <typename T, int BT, int BN, int WT, int WN, int R, bool kAligned>
+__global__ __launch_bounds__(64 * WT * WN, 2) void proj_kernel(ProjArgs p) {
+  using C = Tile<BT, BN, WT, WN, R>;
   using V8 = typename VecOf<T>::v8;
-  // An array per buffer: the compiler then knows that a load into one leaves
-  // reads of the others alone.
-  __shared__ __align__(1024) char sx0[BT * 128];
-  __shared__ __align__(1024) char sx1[BT * 128];
-  __shared__ __align__(1024) char sw0[BN * 128];
-  __shared__ __align__(1024) char sw1[BN * 128];
-  __shared__ uint32_t s_last;
+  // An array per slot, or for two slots one for its x and one for its w rows:
+  // the compiler then knows that a load into one leaves reads of the others alone.
+  constexpr int kArray = R == 2 ? std::max(C::kXBytes, C::kWBytes) : C::kXBytes + C::kWBytes;
+  __shared__ __align__(1024) char mem0[kArray];
+  __shared__ __align__(1024) char mem1[kArray];
+  __shared__ __align__(1024) char mem2[kArray];
+  __shared__ __align__(1024) char mem3[kArray];
+  struct Slot {
+    char* x;
+    char* w;
+  };
+  const Slot slot0{mem0, R == 2 ? mem2 : mem0 + C::kXBytes}, slot1{mem1, R == 2 ? mem3 : mem1 + C::kXBytes};
+  const Slot slot2{mem2, mem2 + C::kXBytes}, slot3{mem3, mem3 + C::kXBytes};  // R == 4
   // The largest tile leaves a compute unit to one workgroup, whose loads have
   // one K-step (about 1 us) to arrive: enough from L2, not always from behind
   // it.  So each step also touches lines of a step four further on.  The rows of
@@ -197,14 +209,13 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wt = wave % WT, wn = wave / WT;
-  int tile = static_cast<int>(blockIdx.x) / p.splits;
-  const int split = static_cast<int>(blockIdx.x) % p.splits;
+  int tile = static_cast<int>(blockIdx.x);
   const int n_tiles = p.tiles_t * p.tiles_n;
   // Workgroups go to the eight XCDs in turn, and each XCD has an L2 of its
   // own: an XCD takes a contiguous eighth of the tiles, which run through
   // bands of eight token tiles, so that the tiles its compute units hold
   // at a time share their rows of x and of w.
-  if (p.splits == 1) tile = tile % 8 * (n_tiles / 8) + std::min(tile % 8, n_tiles % 8) + tile / 8;
+  tile = tile % 8 * (n_tiles / 8) + std::min(tile % 8, n_tiles % 8) + tile / 8;
   constexpr int kBand = 8;
   const int band = tile / (kBand * p.tiles_n);
   const int band_rows = std::min(kBand, p.tiles_t - band * kBand);
@@ -212,7 +223,7 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
   const int tile_t = band * kBand + in_band % band_rows, tile_n = in_band / band_rows;
   const int64_t t0 = static_cast<int64_t>(tile_t) * BT;
   const int n0 = tile_n * (p.gated ? BN / 2 : BN);
-  const int k_begin = split * p.k_range, k_end = std::min(p.d_in, k_begin + p.k_range);
+  const int k_end = p.d_in;
 
   // Fragment reads: lane's row and chunk; a second half's chunk is 4 further,
   // which the swizzle turns into a flipped bit.
@@ -227,11 +238,11 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
 #pragma unroll
     for (int j = 0; j < C::kFT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   V8 aw[C::kFN], ax[C::kFT], bw[C::kFN], bx[C::kFT];
-  auto read = [&](const char* sx, const char* sw, int half, V8 (&fw)[C::kFN], V8 (&fx)[C::kFT]) {
+  auto read = [&](const Slot& slot, int half, V8 (&fw)[C::kFN], V8 (&fx)[C::kFT]) {
 #pragma unroll
-    for (int i = 0; i < C::kFN; ++i) fw[i] = fragment(sw, wn * C::kN + i * 16, half);
+    for (int i = 0; i < C::kFN; ++i) fw[i] = fragment(slot.w, wn * C::kN + i * 16, half);
 #pragma unroll
-    for (int j = 0; j < C::kFT; ++j) fx[j] = fragment(sx, wt * C::kT + j * 16, half);
+    for (int j = 0; j < C::kFT; ++j) fx[j] = fragment(slot.x, wt * C::kT + j * 16, half);
   };
   auto multiply = [&](V8 (&fw)[C::kFN], V8 (&fx)[C::kFT]) {
 #pragma unroll
@@ -266,17 +277,17 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
       src_w[i] = static_cast<const T*>(p.w) + row * p.ldw;
       off_w[i] = ok ? (sub * static_cast<int>(p.ldw) + col[g & 1]) * 2 : kOutside;
     }
-    auto stage = [&](int k, char* sx, char* sw) {
+    auto stage = [&](int k, const Slot& slot) {
       const bool in[2] = {k + col[0] < k_end, k + col[1] < k_end};
 #pragma unroll
       for (int i = 0; i < C::kLoadsX; ++i) {
         const int g = wave * C::kLoadsX + i;
-        load_to_lds(src_x[i], sx + g * 1024, in[(C::kLoadsX % 2 ? g : i) & 1] ? off_x[i] : kOutside, k * 2);
+        load_to_lds(src_x[i], slot.x + g * 1024, in[(C::kLoadsX % 2 ? g : i) & 1] ? off_x[i] : kOutside, k * 2);
       }
 #pragma unroll
       for (int i = 0; i < C::kLoadsW; ++i) {
         const int g = wave * C::kLoadsW + i;
-        load_to_lds(src_w[i], sw + g * 1024, in[(C::kLoadsW % 2 ? g : i) & 1] ? off_w[i] : kOutside, k * 2);
+        load_to_lds(src_w[i], slot.w + g * 1024, in[(C::kLoadsW % 2 ? g : i) & 1] ? off_w[i] : kOutside, k * 2);
       }
     };
     const T* line = nullptr;
@@ -301,9 +312,9 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
     // read() what nobody uses, so that a step is free of branches and its
     // reads, loads and products can be put in order: each read or load between two products, so
     // that issuing them leaves no gap in the matrix cores' work.
-    constexpr int kReads = C::kFN + C::kFT, kProducts = C::kFN * C::kFT, kLoads = C::kLoadsX + C::kLoadsW;
-    auto step = [&](int k, char* sx, char* sw, const char* next_x, const char* next_w) {
-      read(sx, sw, 1, bw, bx);
+    constexpr int kReads = C::kFN + C::kFT, kProducts = C::kFN * C::kFT;
+    auto step = [&](int k, const Slot& now, const Slot& next) {
+      read(now, 1, bw, bx);
       multiply(aw, ax);
 #pragma unroll
       for (int i = 0; i < kReads; ++i) {
@@ -312,13 +323,13 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
       }
       __builtin_amdgcn_sched_group_barrier(0x008, kProducts > kReads ? kProducts - kReads : 0, 0);
       __builtin_amdgcn_sched_barrier(0);
-      staged_barrier<kTouches>();
-      stage(k + 2 * kStepK, sx, sw);
+      staged_barrier<C::kLoads*(R - 2) + kTouches>();
+      stage(k + R * kStepK, now);
       if constexpr (kTouch) touch_line(line + std::min(k + kAhead, k_end - 8), s_touch);
-      read(next_x, next_w, 0, aw, ax);
+      read(next, 0, aw, ax);
       multiply(bw, bx);
 #pragma unroll
-      for (int i = 0; i < kLoads + kTouches; ++i) {
+      for (int i = 0; i < C::kLoads + kTouches; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);  // load
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       }
@@ -329,15 +340,35 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
       }
       __builtin_amdgcn_sched_barrier(0);
     };
-    if (k_begin < k_end) {
-      stage(k_begin, sx0, sw0);
-      staged_barrier<0>();
-      stage(k_begin + kStepK, sx1, sw1);
-      if constexpr (kTouch) touch_line(line + std::min(k_begin + 2 * kStepK, k_end - 8), s_touch);
-      read(sx0, sw0, 0, aw, ax);
-      for (int k = k_begin; k < k_end; k += 2 * kStepK) {
-        step(k, sx0, sw0, sx1, sw1);
-        if (k + kStepK < k_end) step(k + kStepK, sx1, sw1, sx0, sw0);
+    if (k_end > 0) {
+      stage(0, slot0);
+      stage(kStepK, slot1);
+      if constexpr (R == 4) {
+        stage(2 * kStepK, slot2);
+        stage(3 * kStepK, slot3);
+      }
+      if constexpr (kTouch) touch_line(line + std::min(2 * kStepK, k_end - 8), s_touch);
+      staged_barrier<C::kLoads*(R - 1) + kTouches>();
+      read(slot0, 0, aw, ax);
+      // Whole rounds of the ring, then the steps left (with a way out of a
+      // round the compiler would wait for every load at its top).
+      const int round_end = k_end / (R * kStepK) * (R * kStepK);
+      int k = 0;
+      for (; k < round_end; k += R * kStepK) {
+        step(k, slot0, slot1);
+        step(k + kStepK, slot1, R == 2 ? slot0 : slot2);
+        if constexpr (R == 4) {
+          step(k + 2 * kStepK, slot2, slot3);
+          step(k + 3 * kStepK, slot3, slot0);
+        }
+      }
+      if (k < k_end) step(k, slot0, slot1);
+      if constexpr (R == 4) {
+        if (k + kStepK < k_end) step(k + kStepK, slot1, slot2);
+        if (k + 2 * kStepK < k_end) step(k + 2 * kStepK, slot2, slot3);
+        if (k + 3 * kStepK < k_end) step(k + 3 * kStepK, slot3, slot0);
+      } else {
+        if (k + kStepK < k_end) step(k + kStepK, slot1, slot0);
       }
     }
   } else {
@@ -357,46 +388,21 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
         rw[i] = load_ragged(static_cast<const T*>(p.w) + row * p.ldw + k + c * 8, ok ? k_end - k - c * 8 : 0);
       }
     };
-    gather(k_begin);
-    for (int k = k_begin; k < k_end; k += kStepK) {
+    gather(0);
+    for (int k = 0; k < k_end; k += kStepK) {
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < C::kLoadsX; ++i)
-        *reinterpret_cast<u32x4*>(sx0 + (wave * C::kLoadsX + i) * 1024 + lane * 16) = rx[i];
+        *reinterpret_cast<u32x4*>(slot0.x + (wave * C::kLoadsX + i) * 1024 + lane * 16) = rx[i];
 #pragma unroll
       for (int i = 0; i < C::kLoadsW; ++i)
-        *reinterpret_cast<u32x4*>(sw0 + (wave * C::kLoadsW + i) * 1024 + lane * 16) = rw[i];
+        *reinterpret_cast<u32x4*>(slot0.w + (wave * C::kLoadsW + i) * 1024 + lane * 16) = rw[i];
       __syncthreads();
       gather(k + kStepK);
-      read(sx0, sw0, 0, aw, ax);
+      read(slot0, 0, aw, ax);
       multiply(aw, ax);
-      read(sx0, sw0, 1, bw, bx);
+      read(slot0, 1, bw, bx);
       multiply(bw, bx);
-    }
-  }
-
-  if (p.splits > 1) {
-    // Partial tiles in the lanes' own order, added in the order of the
-    // K-ranges by the last to arrive.
-    constexpr uint32_t kTileBytes = BT * BN * 4;
-    char* parts = reinterpret_cast<char*>(p.part) + static_cast<uint64_t>(tile) * p.splits * kTileBytes;
-    const uint32_t at = static_cast<uint32_t>(wave * C::kFN * C::kFT * 64 + lane) * 16;
-    const __amdgpu_buffer_rsrc_t mine = coherent_buffer(parts + static_cast<uint64_t>(split) * kTileBytes, kTileBytes);
-#pragma unroll
-    for (int i = 0; i < C::kFN; ++i)
-#pragma unroll
-      for (int j = 0; j < C::kFT; ++j) coherent_store16(mine, at + (i * C::kFT + j) * 1024, acc[i][j]);
-    if (!last_split(p.tile_cnt + tile, p.splits, &s_last)) return;
-#pragma unroll
-    for (int i = 0; i < C::kFN; ++i)
-#pragma unroll
-      for (int j = 0; j < C::kFT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.splits; ++s) {
-      const __amdgpu_buffer_rsrc_t one = coherent_buffer(parts + static_cast<uint64_t>(s) * kTileBytes, kTileBytes);
-#pragma unroll
-      for (int i = 0; i < C::kFN; ++i)
-#pragma unroll
-        for (int j = 0; j < C::kFT; ++j) acc[i][j] += coherent_load16(one, at + (i * C::kFT + j) * 1024);
     }
   }
 
@@ -408,12 +414,10 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
   constexpr int kChunks = C::kN / 4;
   constexpr int kPassFrags = std::min(C::kFT, 4);
   constexpr int kWaveBytes = kPassFrags * 16 * C::kN * 4;
-  constexpr int kPerArray = C::kWaves / 4;
-  static_assert(C::kWaves % 4 == 0 && kPerArray * kWaveBytes <= BT * 128 && kPerArray * kWaveBytes <= BN * 128 &&
-                    C::kFT % kPassFrags == 0,
-                "a wave's rows of a pass fit its share of an array");
+  constexpr int kPerArray = (C::kWaves + 3) / 4;
+  static_assert(kPerArray * kWaveBytes <= kArray && C::kFT % kPassFrags == 0, "a wave's rows of a pass fit its share of an array");
   const int array = wave / kPerArray;
-  char* rows = (array == 0 ? sx0 : array == 1 ? sx1 : array == 2 ? sw0 : sw1) + wave % kPerArray * kWaveBytes;
+  char* rows = (array == 0 ? mem0 : array == 1 ? mem1 : array == 2 ? mem2 : mem3) + wave % kPerArray * kWaveBytes;
   const int outs = p.gated ? C::kN / 2 : C::kN;  // a row's outputs
   const int wave_n = n0 + wn * outs;
   const int64_t wave_t = t0 + wt * C::kT;
@@ -452,115 +456,151 @@ __global__ __launch_bounds__(64 * WT * WN) void proj_kernel(ProjArgs p) {
   }
 }
 
-// Few tokens: a workgroup takes 16 outputs (16 gate and 16 up rows) for all
-// of them and its eight waves share out the columns, 64 (a row's 128 bytes) at
-// a time; every weight goes from memory to a register once and is used there.
-// Bound by the weight's bytes.
-constexpr int kRowWaves = 8;
-constexpr int kRowThreads = 64 * kRowWaves;
-constexpr int kRowDepth = 4;  // 64-column blocks in flight per wave
+// Small products: a workgroup's eight waves share out the columns of one tile,
+// 64 (128 bytes of a row) at a time, and fragments go from memory to registers
+// and into the product there: no LDS, no barrier until the waves' sums are
+// joined, and the loads of several blocks in flight per wave.  What bounds it is the first loads'
+// latency and the tile's bytes, or (few tokens) the weight's bytes.
+// kFT x kFN fragments; gated: half of the kFN are gate rows, half the same
+// outputs' up rows.
+constexpr int kColWaves = 8;
+constexpr int kColThreads = 64 * kColWaves;
+constexpr int kColBlock = 64;
 
-template <typename T, int kFT, bool kAligned>
-__global__ __launch_bounds__(kRowThreads) void proj_rows_kernel(ProjArgs p) {
+template <int kFT, int kFN>
+struct ColTile {
+  static constexpr int kFrags = kFT * kFN;
+  // Blocks in flight: about 128 registers of fragments where the sums leave
+  // them, 96 beside the largest tile's.
+  static constexpr int kDepth = kFrags >= 16 ? 2 : kFrags >= 4 ? 4 : 16 / (2 * (kFT + kFN));
+};
+
+template <typename T, int kFT, int kFN, bool kGated, bool kAligned>
+__global__ __launch_bounds__(kColThreads) void proj_cols_kernel(ProjArgs p) {
   using V8 = typename VecOf<T>::v8;
-  __shared__ f32x4 s_acc[kRowWaves][2][kFT][64];
+  constexpr int kFrags = kFT * kFN, kDepth = ColTile<kFT, kFN>::kDepth;
+  constexpr int kOutFrags = kGated ? kFN / 2 : kFN;  // fragments of outputs per token fragment
+  static_assert(!kGated || kFN % 2 == 0, "both factors of a gate");
+  __shared__ f32x4 s_acc[kColWaves][kFrags][64];
   __shared__ uint32_t s_last;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int tile = static_cast<int>(blockIdx.x) / p.splits, split = static_cast<int>(blockIdx.x) % p.splits;
-  const int n0 = tile * 16;
+  const int tile_t = tile % p.tiles_t, tile_n = tile / p.tiles_t;
+  const int64_t t0 = static_cast<int64_t>(tile_t) * (kFT * 16);
+  const int n0 = tile_n * (kOutFrags * 16);
   const int k_begin = split * p.k_range, k_end = std::min(p.d_in, k_begin + p.k_range);
-  const int n = n0 + (lane & 15);
-  const bool row_ok = n < p.n_out;
   const int kc = (lane >> 4) * 8;
-  const T* w0 = static_cast<const T*>(p.w) + static_cast<int64_t>(n) * p.ldw + kc;
-  const T* w1 = w0 + static_cast<int64_t>(p.n_out) * p.ldw;
+  const T* w[kFN];
   const T* x[kFT];
-  bool tok_ok[kFT];
+  bool w_ok[kFN], x_ok[kFT];
+#pragma unroll
+  for (int i = 0; i < kFN; ++i) {
+    const int n = n0 + i % kOutFrags * 16 + (lane & 15);
+    w_ok[i] = n < p.n_out;
+    w[i] = static_cast<const T*>(p.w) + (n + (i < kOutFrags ? 0 : static_cast<int64_t>(p.n_out))) * p.ldw + kc;
+  }
 #pragma unroll
   for (int j = 0; j < kFT; ++j) {
-    const int64_t t = j * 16 + (lane & 15);
-    tok_ok[j] = t < p.tokens;
+    const int64_t t = t0 + j * 16 + (lane & 15);
+    x_ok[j] = t < p.tokens;
     x[j] = static_cast<const T*>(p.x) + t * p.ldx + kc;
   }
   auto get = [&](const T* row, bool ok, int k) -> V8 {
     if constexpr (kAligned) return ok && k + kc < k_end ? load8(row + k) : zero8<T>();
     return __builtin_bit_cast(V8, load_ragged(row + k, ok ? k_end - k - kc : 0));
   };
-  f32x4 acc[2][kFT];
+  f32x4 acc[kFN][kFT];
 #pragma unroll
-  for (int g = 0; g < 2; ++g)
+  for (int i = 0; i < kFN; ++i)
 #pragma unroll
-    for (int j = 0; j < kFT; ++j) acc[g][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto run = [&](auto gated) {
-    constexpr int kG = decltype(gated)::value ? 2 : 1;
-    constexpr int kDepth = kRowDepth / kG;
-    for (int k = k_begin + wave * kStepK; k < k_end; k += kRowWaves * kStepK * kDepth) {
-      V8 fw[kDepth][2][kG], fx[kDepth][2][kFT];
+    for (int j = 0; j < kFT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  V8 fw[kDepth][2][kFN], fx[kDepth][2][kFT];
+  auto load = [&](int b, int k) {
 #pragma unroll
-      for (int b = 0; b < kDepth; ++b)
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int at = k + b * kRowWaves * kStepK + h * 32;
-          fw[b][h][0] = get(w0, row_ok, at);
-          if constexpr (kG == 2) fw[b][h][1] = get(w1, row_ok, at);
+      for (int i = 0; i < kFN; ++i) fw[b][h][i] = get(w[i], w_ok[i], k + h * 32);
 #pragma unroll
-          for (int j = 0; j < kFT; ++j) fx[b][h][j] = get(x[j], tok_ok[j], at);
-        }
-#pragma unroll
-      for (int b = 0; b < kDepth; ++b)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int g = 0; g < kG; ++g)
-#pragma unroll
-            for (int j = 0; j < kFT; ++j) acc[g][j] = mfma16(fw[b][h][g], fx[b][h][j], acc[g][j]);
+      for (int j = 0; j < kFT; ++j) fx[b][h][j] = get(x[j], x_ok[j], k + h * 32);
     }
   };
-  if (p.gated)
-    run(std::integral_constant<bool, true>{});
-  else
-    run(std::integral_constant<bool, false>{});
+  constexpr int kStride = kColWaves * kColBlock;
+  const int k0 = k_begin + wave * kColBlock;
+#pragma unroll
+  for (int b = 0; b < kDepth; ++b) load(b, k0 + b * kStride);
+  for (int k = k0; k < k_end; k += kDepth * kStride) {
+#pragma unroll
+    for (int b = 0; b < kDepth; ++b) {
+      if (k + b * kStride >= k_end) break;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < kFN; ++i)
+#pragma unroll
+          for (int j = 0; j < kFT; ++j) acc[i][j] = mfma16(fw[b][h][i], fx[b][h][j], acc[i][j]);
+      if (k + (kDepth + b) * kStride < k_end) load(b, k + (kDepth + b) * kStride);
+    }
+  }
 
-  const int kG = p.gated ? 2 : 1;
 #pragma unroll
-  for (int g = 0; g < 2; ++g)
-    if (g < kG)
+  for (int i = 0; i < kFN; ++i)
 #pragma unroll
-      for (int j = 0; j < kFT; ++j) s_acc[wave][g][j][lane] = acc[g][j];
+    for (int j = 0; j < kFT; ++j) s_acc[wave][i * kFT + j][lane] = acc[i][j];
   __syncthreads();
-  // Wave j joins token fragment j.
-  f32x4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  if (wave < kFT)
-    for (int g = 0; g < kG; ++g)
+  // Each wave joins, and finishes, output fragments wave, wave + 8, ...
+  constexpr int kOuts = kOutFrags * kFT;
+  constexpr int kMine = (kOuts + kColWaves - 1) / kColWaves;
+  constexpr uint32_t kTileBytes = kFrags * 1024;
+  char* parts = reinterpret_cast<char*>(p.part) + static_cast<uint64_t>(tile) * p.splits * kTileBytes;
+  f32x4 sum[kMine][2];
 #pragma unroll
-      for (int i = 0; i < kRowWaves; ++i) sum[g] += s_acc[i][g][wave][lane];
+  for (int m = 0; m < kMine; ++m) {
+    const int o = wave + m * kColWaves;
+    sum[m][0] = sum[m][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (o < kOuts)
+#pragma unroll
+      for (int i = 0; i < kColWaves; ++i) {
+        sum[m][0] += s_acc[i][o][lane];
+        if constexpr (kGated) sum[m][1] += s_acc[i][kOuts + o][lane];
+      }
+  }
   if (p.splits > 1) {
-    constexpr uint32_t kTileBytes = 2 * kFT * 1024;
-    char* parts = reinterpret_cast<char*>(p.part) + static_cast<uint64_t>(tile) * p.splits * kTileBytes;
-    const uint32_t at = static_cast<uint32_t>(wave * 64 + lane) * 16;
-    if (wave < kFT) {
-      const __amdgpu_buffer_rsrc_t mine = coherent_buffer(parts + static_cast<uint64_t>(split) * kTileBytes, kTileBytes);
-      for (int g = 0; g < kG; ++g) coherent_store16(mine, at + g * kFT * 1024, sum[g]);
+    const __amdgpu_buffer_rsrc_t mine = coherent_buffer(parts + static_cast<uint64_t>(split) * kTileBytes, kTileBytes);
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      const int o = wave + m * kColWaves;
+      if (o >= kOuts) break;
+      coherent_store16(mine, static_cast<uint32_t>(o * 64 + lane) * 16, sum[m][0]);
+      if constexpr (kGated) coherent_store16(mine, static_cast<uint32_t>((kOuts + o) * 64 + lane) * 16, sum[m][1]);
     }
     if (!last_split(p.tile_cnt + tile, p.splits, &s_last)) return;
-    if (wave < kFT) {
-      sum[0] = sum[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      const int o = wave + m * kColWaves;
+      if (o >= kOuts) break;
+      sum[m][0] = sum[m][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
       for (int s = 0; s < p.splits; ++s) {
         const __amdgpu_buffer_rsrc_t one = coherent_buffer(parts + static_cast<uint64_t>(s) * kTileBytes, kTileBytes);
-        for (int g = 0; g < kG; ++g) sum[g] += coherent_load16(one, at + g * kFT * 1024);
+        sum[m][0] += coherent_load16(one, static_cast<uint32_t>(o * 64 + lane) * 16);
+        if constexpr (kGated) sum[m][1] += coherent_load16(one, static_cast<uint32_t>((kOuts + o) * 64 + lane) * 16);
       }
     }
   }
-  const int64_t t = wave * 16 + (lane & 15);
-  const int out = n0 + (lane >> 4) * 4;
-  if (wave < kFT && t < p.tokens && out < p.n_out)
-    with_activation(p.act, [&](auto act) {
-      if (p.rows_vec && out + 4 <= p.n_out)
-        finish<T, decltype(act)::value, true>(p, t, out, sum[0], sum[1]);
+  with_activation(p.act, [&](auto act) {
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      const int o = wave + m * kColWaves;
+      const int64_t t = t0 + o % kFT * 16 + (lane & 15);
+      const int n = n0 + o / kFT * 16 + (lane >> 4) * 4;
+      if (o >= kOuts || t >= p.tokens || n >= p.n_out) continue;
+      if (p.rows_vec && n + 4 <= p.n_out)
+        finish<T, decltype(act)::value, true>(p, t, n, sum[m][0], sum[m][1]);
       else
-        finish<T, decltype(act)::value, false>(p, t, out, sum[0], sum[1]);
-    });
+        finish<T, decltype(act)::value, false>(p, t, n, sum[m][0], sum[m][1]);
+    }
+  });
 }
 
 // K-ranges of a launch of `tiles` workgroups: as many as bring it to `want`
@@ -575,41 +615,63 @@ void split_columns(ProjArgs& a, int64_t tiles, int64_t want, int least, uint64_t
   a.splits = static_cast<int32_t>(std::max<int64_t>(1, (static_cast<int64_t>(a.d_in) + a.k_range - 1) / a.k_range));
 }
 
-template <typename T, int BT, int BN, int WT, int WN, bool kAligned>
-hipError_t launch_tiles(ProjArgs& a, int64_t want, hipStream_t stream) {
+template <typename T, int BT, int BN, int WT, int WN, int R, bool kAligned>
+hipError_t launch_tiles(ProjArgs& a, hipStream_t stream) {
   const int outs = a.gated ? BN / 2 : BN;
   a.tiles_t = static_cast<int32_t>((a.tokens + BT - 1) / BT);
   a.tiles_n = (a.n_out + outs - 1) / outs;
   const int64_t tiles = static_cast<int64_t>(a.tiles_t) * a.tiles_n;
-  split_columns(a, tiles, want, 4 * kStepK, static_cast<uint64_t>(BT) * BN * 4);
-  if (tiles * a.splits > 0x7FFFFFFF) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((proj_kernel<T, BT, BN, WT, WN, kAligned>), dim3(static_cast<uint32_t>(tiles * a.splits)),
-                     dim3(64 * WT * WN), 0, stream, a);
+  if (tiles > 0x7FFFFFFF) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((proj_kernel<T, BT, BN, WT, WN, R, kAligned>), dim3(static_cast<uint32_t>(tiles)), dim3(64 * WT * WN), 0,
+                     stream, a);
   return hipGetLastError();
 }
 
-template <typename T, int kFT, bool kAligned>
-hipError_t launch_rows(ProjArgs& a, int64_t want, hipStream_t stream) {
-  a.tiles_t = 1;
-  a.tiles_n = (a.n_out + 15) / 16;
-  split_columns(a, a.tiles_n, want, kRowWaves * kStepK, 2 * kFT * 1024);
-  if (static_cast<int64_t>(a.tiles_n) * a.splits > 0x7FFFFFFF) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((proj_rows_kernel<T, kFT, kAligned>), dim3(static_cast<uint32_t>(a.tiles_n) * a.splits),
-                     dim3(kRowThreads), 0, stream, a);
+template <typename T, int kFT, int kFN, bool kAligned>
+hipError_t launch_cols(ProjArgs& a, int n_cu, hipStream_t stream) {
+  const int outs = kFN * 16 / (a.gated ? 2 : 1);
+  a.tiles_t = static_cast<int32_t>((a.tokens + kFT * 16 - 1) / (kFT * 16));
+  a.tiles_n = (a.n_out + outs - 1) / outs;
+  const int64_t tiles = static_cast<int64_t>(a.tiles_t) * a.tiles_n;
+  // A tile's columns are split over workgroups only where tiles leave half of
+  // the device idle: joining costs about 5 us.
+  split_columns(a, tiles, n_cu, 4 * kColWaves * kColBlock, kFT * kFN * 1024);
+  if (tiles * a.splits > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const dim3 grid(static_cast<uint32_t>(tiles * a.splits));
+  if (a.gated) {
+    if constexpr (kFN % 2 == 0)
+      hipLaunchKernelGGL((proj_cols_kernel<T, kFT, kFN, true, kAligned>), grid, dim3(kColThreads), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((proj_cols_kernel<T, kFT, kFN, false, kAligned>), grid, dim3(kColThreads), 0, stream, a);
+  }
   return hipGetLastError();
 }
 
 template <typename T, bool kAligned>
 hipError_t launch(ProjArgs& a, int n_cu, hipStream_t stream) {
-  if (a.tokens <= 16) return launch_rows<T, 1, kAligned>(a, n_cu, stream);
-  if (a.tokens <= 32) return launch_rows<T, 2, kAligned>(a, n_cu, stream);
-  const int64_t rows = static_cast<int64_t>(a.n_out) * (a.gated ? 2 : 1);
-  auto tiles = [&](int64_t bt, int64_t bn) { return (a.tokens + bt - 1) / bt * ((rows + bn - 1) / bn); };
-  if constexpr (kAligned) {
-    if (tiles(256, 256) >= n_cu * 3 / 4) return launch_tiles<T, 256, 256, 2, 4, kAligned>(a, 1, stream);
+  if (a.tokens <= 16) {
+    if (a.gated) return launch_cols<T, 1, 2, kAligned>(a, n_cu, stream);
+    return launch_cols<T, 1, 1, kAligned>(a, n_cu, stream);
   }
-  if (tiles(128, 128) >= n_cu) return launch_tiles<T, 128, 128, 2, 2, kAligned>(a, 1, stream);
-  return launch_tiles<T, 64, 64, 2, 2, kAligned>(a, 2 * n_cu, stream);
+  const int64_t rows = static_cast<int64_t>(a.n_out) * (a.gated ? 2 : 1);
+  auto tiles = [&](int64_t b) { return (a.tokens + b - 1) / b * ((rows + b - 1) / b); };
+  // (32 x 4096 x 4096: 11.8 us, 14.2 on 64-row tiles; 128 x 8192 x 1024, 32 of
+  // those tiles: 19.9 and 24.6; 128 x 2048 x 2048, 64 of them: 9.9 and 8.9.)
+  if (a.tokens <= 32 || tiles(64) < n_cu / 4) return launch_cols<T, 2, 2, kAligned>(a, n_cu, stream);
+  // The tile whose rounds over the device cost least.  A K-step of a round
+  // takes 1.5 us with the 256-row tile (one workgroup a compute unit), 0.72
+  // with the 128-row one, 0.4 with two 64-row ones a compute unit and 0.22
+  // with one.  (512 x 5120 x 27648: 124, 195 and 274 us; 2048 x 2048 x 2048: 49,
+  // 20.9 and 26.7; 1000 x 2048 x 2048: 51, 17.4 and 15.0.)
+  auto rounds = [&](int64_t n, int64_t at_once) { return static_cast<double>((n + at_once - 1) / at_once); };
+  const double cost64 = tiles(64) <= n_cu ? 0.22 : 0.4 * rounds(tiles(64), 2 * n_cu);
+  const double cost128 = 0.72 * rounds(tiles(128), n_cu);
+  if constexpr (kAligned) {
+    if (1.5 * rounds(tiles(256), n_cu) <= std::min(cost64, cost128))
+      return launch_tiles<T, 256, 256, 2, 4, 2, kAligned>(a, stream);
+  }
+  if (cost128 <= cost64) return launch_tiles<T, 128, 128, 4, 2, 4, kAligned>(a, stream);
+  return launch_tiles<T, 64, 64, 2, 2, 4, kAligned>(a, stream);
 }
 
 }  // namespace
