@@ -31,8 +31,17 @@ __device__ __forceinline__ float activate(float v) {
   switch (kAct) {
     case kActRelu:
       return v < 0.f ? 0.f : v;  // NaN stays
-    case kActGelu:
-      return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+    case kActGelu: {
+      // 0.5 v (1 + erf u), u = v / sqrt 2, with erf |u| = 1 - p(t) t exp(-u^2),
+      // t = 1 / (1 + 0.3275911 |u|) (Abramowitz and Stegun 7.1.26, within
+      // 1.5e-7); for negative v the 1 cancels and the tail keeps its precision.
+      const float u = fabsf(v) * 0.70710678118654752f;
+      const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, u, 1.f));
+      const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f),
+                               0.254829592f);
+      const float tail = 0.5f * v * q * __builtin_amdgcn_exp2f(-1.4426950408889634f * u * u);
+      return v < 0.f ? tail : v - tail;
+    }
     case kActGeluTanh:
       // 0.5 v (1 + tanh u) = v sigmoid(2 u)
       return v * sigmoid(1.5957691216057308f * (v + 0.044715f * v * v * v));
@@ -106,32 +115,52 @@ __device__ __forceinline__ int64_t weight_row(const ProjArgs& p, int n0, int r, 
   return n + (r % kN < kN / 2 ? 0 : static_cast<int64_t>(p.n_out));
 }
 
-// Four consecutive outputs of one token: bias, activation, gate, residual, one
-// rounding.  kWhole: all four exist, and every tensor takes 8-byte accesses.
-template <typename T, int kAct, bool kWhole>
-__device__ __forceinline__ void finish(const ProjArgs& p, int64_t t, int n, f32x4 a, f32x4 up) {
+// The biases of four consecutive outputs and, gated, of their up rows.
+struct Biases {
+  f32x4 gate, up;
+};
+template <typename T>
+__device__ __forceinline__ Biases biases(const ProjArgs& p, int n) {
+  Biases b{{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
   const T* bias = static_cast<const T*>(p.bias);
-  const T* res = static_cast<const T*>(p.residual);
-  T* y = static_cast<T*>(p.y) + t * p.ldy + n;
-  if constexpr (kWhole) {
-    if (bias) {
-      a += unpack4f<T>(*reinterpret_cast<const u32x2*>(bias + n));
-      if (p.gated) up += unpack4f<T>(*reinterpret_cast<const u32x2*>(bias + p.n_out + n));
-    }
+  if (bias == nullptr) return b;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) a[e] = activate<kAct>(a[e]);
-    if (p.gated) a *= up;
-    if (res) a += unpack4f<T>(*reinterpret_cast<const u32x2*>(res + t * p.ldr + n));
+  for (int e = 0; e < 4; ++e) {
+    if (n + e >= p.n_out) break;
+    b.gate[e] = static_cast<float>(bias[n + e]);
+    if (p.gated) b.up[e] = static_cast<float>(bias[p.n_out + n + e]);
+  }
+  return b;
+}
+
+// Four consecutive outputs of one token: bias, activation, gate, residual, one
+// rounding.  kWhole: all four exist, and y and the residual take 8-byte
+// accesses; else the first `count` of them are written one by one.
+template <typename T, int kAct, bool kWhole>
+__device__ __forceinline__ void finish(const ProjArgs& p, int64_t t, int n, int count, f32x4 a, f32x4 up, const Biases& b) {
+  const T* res = static_cast<const T*>(p.residual) + t * p.ldr + n;
+  T* y = static_cast<T*>(p.y) + t * p.ldy + n;
+  f32x4 r{0.f, 0.f, 0.f, 0.f};
+  if (p.residual) {
+    if constexpr (kWhole) {
+      r = unpack4f<T>(*reinterpret_cast<const u32x2*>(res));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < count) r[e] = static_cast<float>(res[e]);
+    }
+  }
+  a += b.gate;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) a[e] = activate<kAct>(a[e]);
+  if (p.gated) a *= up + b.up;
+  a += r;
+  if constexpr (kWhole) {
     store4(y, a);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (n + e >= p.n_out) break;
-      float v = activate<kAct>(a[e] + (bias ? static_cast<float>(bias[n + e]) : 0.f));
-      if (p.gated) v *= up[e] + (bias ? static_cast<float>(bias[p.n_out + n + e]) : 0.f);
-      if (res) v += static_cast<float>(res[t * p.ldr + n + e]);
-      y[e] = static_cast<T>(v);
-    }
+    for (int e = 0; e < 4; ++e)
+      if (e < count) y[e] = static_cast<T>(a[e]);
   }
 }
 
@@ -423,7 +452,9 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void proj_kernel(ProjArgs p) {
   const int64_t wave_t = t0 + wt * C::kT;
   const int lanes = outs / 4;  // along a row
   const int c = lane % lanes, row0 = lane / lanes, row_step = 64 / lanes;
+  const int n = wave_n + c * 4;
   const bool whole = p.rows_vec && wave_t + C::kT <= p.tokens && wave_n + outs <= p.n_out;
+  const Biases bias = biases<T>(p, n);
   wait_vm();  // loads past the last column write LDS too
   __syncthreads();
 #pragma unroll
@@ -440,17 +471,17 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void proj_kernel(ProjArgs p) {
       return *reinterpret_cast<const f32x4*>(rows + r * (C::kN * 4) + ((chunk ^ (r & (kChunks - 1))) << 4));
     };
     const int64_t pass_t = wave_t + pass * kPassFrags * 16;
-    const int n = wave_n + c * 4;
     with_activation(p.act, [&](auto act) {
       constexpr int kAct = decltype(act)::value;
       if (whole) {
 #pragma unroll 4
         for (int r = row0; r < kPassFrags * 16; r += row_step)
-          finish<T, kAct, true>(p, pass_t + r, n, sum_of(r, c), sum_of(r, c + (p.gated ? kChunks / 2 : 0)));
+          finish<T, kAct, true>(p, pass_t + r, n, 4, sum_of(r, c), sum_of(r, c + (p.gated ? kChunks / 2 : 0)), bias);
       } else {
+#pragma unroll 2
         for (int r = row0; r < kPassFrags * 16; r += row_step)
-          if (pass_t + r < p.tokens && n < p.n_out)
-            finish<T, kAct, false>(p, pass_t + r, n, sum_of(r, c), sum_of(r, c + (p.gated ? kChunks / 2 : 0)));
+          finish<T, kAct, false>(p, pass_t + r, n, pass_t + r < p.tokens ? p.n_out - n : 0, sum_of(r, c),
+                                 sum_of(r, c + (p.gated ? kChunks / 2 : 0)), bias);
       }
     });
   }
@@ -595,10 +626,11 @@ __global__ __launch_bounds__(kColThreads) void proj_cols_kernel(ProjArgs p) {
       const int64_t t = t0 + o % kFT * 16 + (lane & 15);
       const int n = n0 + o / kFT * 16 + (lane >> 4) * 4;
       if (o >= kOuts || t >= p.tokens || n >= p.n_out) continue;
+      const Biases bias = biases<T>(p, n);
       if (p.rows_vec && n + 4 <= p.n_out)
-        finish<T, decltype(act)::value, true>(p, t, n, sum[m][0], sum[m][1]);
+        finish<T, decltype(act)::value, true>(p, t, n, 4, sum[m][0], sum[m][1], bias);
       else
-        finish<T, decltype(act)::value, false>(p, t, n, sum[m][0], sum[m][1]);
+        finish<T, decltype(act)::value, false>(p, t, n, p.n_out - n, sum[m][0], sum[m][1], bias);
     }
   });
 }
@@ -680,7 +712,7 @@ hipError_t launch_proj(int dtype_bf16, ProjArgs& a, int n_cu, hipStream_t stream
   auto whole = [](const void* p, int64_t ld, int bytes) {
     return reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld % (bytes / 2) == 0;
   };
-  a.rows_vec = whole(a.y, a.ldy, 8) && whole(a.residual, a.ldr, 8) && whole(a.bias, a.gated ? a.n_out : 0, 8);
+  a.rows_vec = whole(a.y, a.ldy, 8) && whole(a.residual, a.ldr, 8);
   const bool aligned = a.d_in % 8 == 0 && whole(a.x, a.ldx, 16) && whole(a.w, a.ldw, 16);
   if (dtype_bf16) return aligned ? launch<__bf16, true>(a, n_cu, stream) : launch<__bf16, false>(a, n_cu, stream);
   return aligned ? launch<_Float16, true>(a, n_cu, stream) : launch<_Float16, false>(a, n_cu, stream);
