@@ -15,11 +15,11 @@
 // out of LDS by the transposing read, four keys of a column at a time, in that
 // same order.
 //
-// Two roles share the launch.  Sequences with more than 32 rows per key head
+// Two roles share the launch.  Sequences with more than 128 rows per key head
 // run on row tiles: a workgroup's waves take 32 rows each and stage 64 keys
 // and values at a time in LDS for all of them.  Shorter ones (single tokens,
-// drafted tokens) run on key chunks: the waves hold the same 32 rows and each
-// streams keys of its own.  Either role splits a long key range over
+// drafted tokens) run on key chunks: the waves share out the keys, 32 at a
+// time, and (past 32 rows) the rows, and each streams keys of its own.  Either role splits a long key range over
 // workgroups where there are too few of them, and the last one of a row tile
 // to finish joins the partial results.
 #include <hip/hip_runtime.h>
@@ -43,6 +43,7 @@ constexpr int kThreads = 64 * kWaves;
 constexpr int kWaveRows = 32;
 constexpr int kTileRows = kWaveRows * kWaves;  // query rows of a row tile
 constexpr int kTileKeys = 64;                  // keys staged at a time for a row tile
+constexpr int kChunkRows = kTileRows;           // most query rows of a sequence that runs on key chunks
 constexpr int kChunkKeys = 32;                 // keys a wave stages at a time for a key chunk
 // A running bound is raised (and O and l scaled) only once a score exceeds it
 // by 2^8: exponentials then stay within 2^8, far inside fp16, and most tiles
@@ -140,7 +141,7 @@ __device__ __forceinline__ int chunks_of(int keys, int shift) {
 __device__ __forceinline__ int items_of(const AttnArgs& p, const Span& s, int group, bool rows_role, int* tiles) {
   const int rows = s.n_q * group;
   *tiles = 0;
-  if (rows == 0 || (rows > kWaveRows) != rows_role) return 0;
+  if (rows == 0 || (rows > kChunkRows) != rows_role) return 0;
   const Range r = keys_of(p, s.n_q, s.n_k, group, 0, rows);
   const int unit = rows_role ? kTileKeys : kChunkKeys;
   const int chunks = chunks_of(r.end - r.first / unit * unit, rows_role ? p.tile_shift : p.chunk_shift);
@@ -392,7 +393,7 @@ struct Staged {
 // of K and j + 1 of V are on their way.
 template <typename T, int DP>
 __device__ __forceinline__ void run_tile(const AttnArgs& p, const Item& it, Rows<T, DP>& w, float c, int first, int end,
-                                         int wave_low, int wave_pos, int wave, WP_STAGED) {
+                                         int wave_low, int wave_pos, int wave_last, int wave, WP_STAGED) {
   using H = Head<DP>;
   using V8 = typename VecOf<T>::v8;
   constexpr int kLoads = kTileKeys * H::kRow / 1024 / kWaves;
@@ -406,6 +407,7 @@ __device__ __forceinline__ void run_tile(const AttnArgs& p, const Item& it, Rows
   auto load_v = [&](int at, char* to) {
     if (at < end) stage<DP, true, kLoads>(v + at * v_tok, static_cast<uint32_t>(v_tok) * 2, dim, n_k - at, to, wave * kLoads);
   };
+  const int live_end = std::min(end, wave_last + 1);
   w.reset();
   if (first >= end) return;
   load_k(first, sk0);
@@ -413,18 +415,17 @@ __device__ __forceinline__ void run_tile(const AttnArgs& p, const Item& it, Rows
   load_k(first + kTileKeys, sk1);
   load_v(first, sv0);
   f32x16 s0 = scores(w, sk0, 0), s1 = scores(w, sk0, 32);
-  auto step = [&](int at, auto more, char* kfree, const char* knext, const char* vnow, char* vnext) {
-    __syncthreads();
-    load_k(at + 2 * kTileKeys, kfree);
-    load_v(at + kTileKeys, vnext);
+  constexpr std::integral_constant<bool, true> yes{};
+  constexpr std::integral_constant<bool, false> no{};
+  // In two halves of 32 keys, which keeps the registers of three score tiles,
+  // not four, in use.
+  auto body = [&](int at, auto more, const char* knext, const char* vnow) {
     // wave_low, wave_pos: the keys that every row of the wave sees.
     if (at < wave_low || at + kTileKeys - 1 > wave_pos) {
       w.mask(s0, at);
       w.mask(s1, at + 32);
     }
     w.raise(fmaxf(top_of(s0), top_of(s1)), c);
-    // In two halves of 32 keys, which keeps the registers of three score
-    // tiles, not four, in use.
     V8 e[2];
     f32x16 n;
     if (more) n = scores(w, knext, 0);
@@ -437,18 +438,20 @@ __device__ __forceinline__ void run_tile(const AttnArgs& p, const Item& it, Rows
     accumulate<T, DP, false>(w, vnow, 32, e);
     if (more) s1 = n;
   };
-  int at = first;
-  constexpr std::integral_constant<bool, true> yes{};
-  constexpr std::integral_constant<bool, false> no{};
-  for (; at + 2 * kTileKeys < end; at += 2 * kTileKeys) {
-    step(at, yes, sk0, sk1, sv0, sv1);
-    step(at + kTileKeys, yes, sk1, sk0, sv1, sv0);
-  }
-  if (at + kTileKeys < end) {
-    step(at, yes, sk0, sk1, sv0, sv1);
-    step(at + kTileKeys, no, sk1, sk0, sv1, sv0);
-  } else {
-    step(at, no, sk0, sk1, sv0, sv1);
+  auto step = [&](int at, char* kfree, const char* knext, const char* vnow, char* vnext) {
+    __syncthreads();
+    load_k(at + 2 * kTileKeys, kfree);
+    load_v(at + kTileKeys, vnext);
+    // Keys past the last one that any of the wave's rows sees are not its
+    // work; the compute unit's other workgroup has the matrix cores then.
+    if (at + kTileKeys < live_end)
+      body(at, yes, knext, vnow);
+    else if (at < live_end)
+      body(at, no, knext, vnow);
+  };
+  for (int at = first; at < end; at += 2 * kTileKeys) {
+    step(at, sk0, sk1, sv0, sv1);
+    if (at + kTileKeys < end) step(at + kTileKeys, sk1, sk0, sv1, sv0);
   }
 }
 
@@ -482,10 +485,10 @@ __device__ __forceinline__ void run_tile_careful(const AttnArgs& p, const Item& 
   }
 }
 
-// Key chunk: keys [first, end), the waves taking 32 of them in turn.
+// Key chunk: keys [first, end), this wave taking every share-th 32 of them.
 template <typename T, int DP, bool kCareful>
 __device__ __forceinline__ void run_chunk(const AttnArgs& p, const Item& it, Rows<T, DP>& w, float c, int first, int end,
-                                          int wave_low, int wave_pos, int wave, char* sk, char* sv) {
+                                          int wave_low, int wave_pos, int phase, int share, char* sk, char* sv) {
   using H = Head<DP>;
   constexpr int kLoads = kChunkKeys * H::kRow / 1024;
   const T* k = head_row<T>(p.k, it.k0, p.k_tok, it.head * p.k_head);
@@ -497,13 +500,13 @@ __device__ __forceinline__ void run_chunk(const AttnArgs& p, const Item& it, Row
     stage<DP, true, kLoads>(v + at * p.v_tok, static_cast<uint32_t>(p.v_tok) * 2, p.dim, it.n_k - at, sv, 0);
   };
   w.reset();
-  int at = first + wave * kChunkKeys;
+  int at = first + phase * kChunkKeys;
   if (at < end) {
     load_k(at);
     load_v(at);
   }
-  for (; at < end; at += kChunkKeys * kWaves) {
-    const int next = at + kChunkKeys * kWaves;
+  for (; at < end; at += kChunkKeys * share) {
+    const int next = at + kChunkKeys * share;
     wait_vm();
     f32x16 s = scores(w, sk, 0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -577,7 +580,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs p) {
   // Bounds that do not rise could name more row tiles than there are counters.
   if (it.seq < 0 || it.counter >= (rows_role ? p.tile_counters : p.seq_counters)) return;
   const int n_rows = it.n_q * group;
-  const int block_rows = rows_role ? kTileRows : kWaveRows;
+  const int block_rows = kTileRows;
   const int row0 = it.tile * block_rows;             // the workgroup's first row
   const int my_rows = std::min(block_rows, n_rows - row0);
   const Range range = keys_of(p, it.n_q, it.n_k, group, row0, my_rows);
@@ -590,7 +593,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs p) {
   const int end = static_cast<int>(std::min<int64_t>(range.end, first + (1ll << shift)));
 
   // This lane's query row.
-  const int wave_row0 = row0 + (rows_role ? wave * kWaveRows : 0);
+  // On key chunks, `share` waves take each 32 rows, every share-th 32 keys.
+  const int row_waves = rows_role || my_rows > 2 * kWaveRows ? kWaves : my_rows > kWaveRows ? 2 : 1;
+  const int share = kWaves / row_waves;
+  const int wave_row0 = row0 + wave % row_waves * kWaveRows;
   const int row = wave_row0 + (lane & 31);
   const bool real = row < n_rows;
   const int tok = real ? row / group : 0, sub = real ? row % group : 0;
@@ -609,15 +615,17 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs p) {
   w.pos = real ? (p.causal ? std::min(tok + lag, it.n_k - 1) : it.n_k - 1) : -1;
   w.low = p.causal && p.window > 0 ? std::max(0, tok + lag - p.window + 1) : 0;
   // The keys that all of the wave's rows see.
-  int wave_pos = it.n_k - 1, wave_low = 0;
+  // wave_last: the last key that any of them sees.
+  int wave_pos = it.n_k - 1, wave_low = 0, wave_last = wave_row0 < n_rows ? it.n_k - 1 : -1;
   if (p.causal) {
     const int t0 = wave_row0 / group, t1 = std::min(it.n_q - 1, (wave_row0 + kWaveRows - 1) / group);
     wave_pos = wave_row0 < n_rows ? t0 + lag : -1;
+    wave_last = wave_row0 < n_rows ? t1 + lag : -1;
     if (p.window > 0) wave_low = std::max(0, t1 + lag - p.window + 1);
   }
 
   if (rows_role) {
-    run_tile<T, DP>(p, it, w, c, first, end, wave_low, wave_pos, wave, sk0, sk1, sv0, sv1);
+    run_tile<T, DP>(p, it, w, c, first, end, wave_low, wave_pos, wave_last, wave, sk0, sk1, sv0, sv1);
     // Infinite or NaN values reach every row of a tile through the product, as
     // zero times them: where there are any, the pass is made again with care.
     if (__syncthreads_or(has_nonfinite(w)))
@@ -626,8 +634,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs p) {
     // A wave's 32 keys and values: half of an array each.
     char* k = (wave < 2 ? sk0 : sk1) + (wave & 1) * (Staged<DP>::kBytes / 2);
     char* v = (wave < 2 ? sv0 : sv1) + (wave & 1) * (Staged<DP>::kBytes / 2);
-    run_chunk<T, DP, false>(p, it, w, c, first, end, wave_low, wave_pos, wave, k, v);
-    if (__any(has_nonfinite(w))) run_chunk<T, DP, true>(p, it, w, c, first, end, wave_low, wave_pos, wave, k, v);
+    run_chunk<T, DP, false>(p, it, w, c, first, end, wave_low, wave_pos, wave / row_waves, share, k, v);
+    if (__any(has_nonfinite(w))) run_chunk<T, DP, true>(p, it, w, c, first, end, wave_low, wave_pos, wave / row_waves, share, k, v);
   }
   w.l += __shfl_xor(w.l, 32);
 
@@ -676,9 +684,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs p) {
       s_l[wave][lane] = w.l;
     }
     __syncthreads();
-    float m = s_m[0][lane & 31];
-#pragma unroll
-    for (int i = 1; i < kWaves; ++i) m = fmaxf(m, s_m[i][lane & 31]);
+    float m = w.m;
+    for (int i = 1; i < share; ++i) m = fmaxf(m, s_m[(wave + i * row_waves) % kWaves][lane & 31]);
     const float fade = m == -INFINITY ? 1.f : exp2_fast(w.m - m);
     char* o32 = wave == 0 ? sk0 : wave == 1 ? sk1 : wave == 2 ? sv0 : sv1;
     if (real)
@@ -691,15 +698,15 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs p) {
     __syncthreads();
     for (int u = tid; u < my_rows * (DP / 4); u += kThreads) {
       const int r = u / (DP / 4), d = u % (DP / 4) * 4;
-      float top = s_m[0][r], l = 0.f;
-#pragma unroll
-      for (int i = 1; i < kWaves; ++i) top = fmaxf(top, s_m[i][r]);
-#pragma unroll
-      for (int i = 0; i < kWaves; ++i) l += s_l[i][r] * (top == -INFINITY ? 1.f : exp2_fast(s_m[i][r] - top));
+      const int w0 = r / kWaveRows, q = r % kWaveRows;
+      float top = s_m[w0][q], l = 0.f;
+      for (int i = 1; i < share; ++i) top = fmaxf(top, s_m[w0 + i * row_waves][q]);
       f32x4 v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < kWaves; ++i)
-        v += *reinterpret_cast<const f32x4*>((i == 0 ? sk0 : i == 1 ? sk1 : i == 2 ? sv0 : sv1) + (r * DP + d) * 4);
+      for (int i = 0; i < share; ++i) {
+        const int x = w0 + i * row_waves;
+        l += s_l[x][q] * (top == -INFINITY ? 1.f : exp2_fast(s_m[x][q] - top));
+        v += *reinterpret_cast<const f32x4*>((x == 0 ? sk0 : x == 1 ? sk1 : x == 2 ? sv0 : sv1) + (q * DP + d) * 4);
+      }
       if (split) {
         coherent_store16(mine, (2u * rows_cap + r * DP + d) * 4u, v);
         if (d == 0) coherent_store8(part + 2 * r, __builtin_bit_cast(unsigned long long, f32x2{top, l}));
@@ -770,9 +777,9 @@ hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t s
   const int64_t group = a.heads / a.kv_heads, rows = a.tokens * group;
   const int64_t kNever = 31;  // a shift past every length: no split
   // Bounds on the work items, from the sizes the host knows: a sequence of
-  // more than 32 rows has at most rows / 128 + 1 row tiles, and one of fewer
+  // more than 128 rows has at most rows / 128 + 1 row tiles, and one of fewer
   // at most keys / chunk + 2 key chunks.
-  const int64_t tile_seqs = std::min<int64_t>(a.n_seq, rows / (kWaveRows + 1));
+  const int64_t tile_seqs = std::min<int64_t>(a.n_seq, rows / (kChunkRows + 1));
   const int64_t tiles = tile_seqs > 0 ? rows / kTileRows + tile_seqs : 0;
   const int64_t chunk_seqs = std::min<int64_t>(a.n_seq, a.tokens);
   // Row tiles: enough of them for the device (two workgroups a compute unit)
@@ -798,7 +805,7 @@ hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t s
   uint64_t chunk_floats = 0;
   if (chunk_seqs > 0) {
     chunk_items = ((a.keys >> chunk_shift) + 2 * chunk_seqs) * a.kv_heads;
-    chunk_floats = static_cast<uint64_t>(chunk_items) * kWaveRows * (dp + 2);
+    chunk_floats = static_cast<uint64_t>(chunk_items) * kChunkRows * (dp + 2);
     if ((tile_floats + chunk_floats) * 4 > a.part_bytes || tile_counters + chunk_seqs * a.kv_heads > a.n_counters) {
       chunk_shift = kNever;
       chunk_items = chunk_seqs * a.kv_heads;

@@ -9,7 +9,7 @@
 namespace wp {
 
 // The engine's scratch for these operators: fp32 partials and tile counters.
-constexpr uint64_t kModelPartBytes = 128ull << 20;
+constexpr uint64_t kModelPartBytes = 256ull << 20;
 constexpr int kModelCounters = 65536;
 
 // Activations of wp_linear, in the order of enum wp_activation.
