@@ -417,26 +417,87 @@ __device__ __forceinline__ void run_tile(const AttnArgs& p, const Item& it, Rows
   f32x16 s0 = scores(w, sk0, 0), s1 = scores(w, sk0, 32);
   constexpr std::integral_constant<bool, true> yes{};
   constexpr std::integral_constant<bool, false> no{};
-  // In two halves of 32 keys, which keeps the registers of three score tiles,
-  // not four, in use.
+  // The order of a tile's work is pinned so that products and vector work run
+  // side by side throughout (two waves a SIMD in the same phase would else wait
+  // for the one unit together and leave the other idle):
+  //   the first half's exponentials between three quarters of the next tile's scores,
+  //   the second half's between the rest of them and the first half's products with V,
+  //   the next scores' maximum between the second half's products with V.
+  // LDS reads go two products ahead.
+  float tops = fmaxf(top_of(s0), top_of(s1));
+  constexpr int kScores = 2 * H::kSteps, kFirst = kScores * 3 / 4, kValues = 2 * H::kCols;
   auto body = [&](int at, auto more, const char* knext, const char* vnow) {
     // wave_low, wave_pos: the keys that every row of the wave sees.
     if (at < wave_low || at + kTileKeys - 1 > wave_pos) {
       w.mask(s0, at);
       w.mask(s1, at + 32);
+      tops = fmaxf(top_of(s0), top_of(s1));
     }
-    w.raise(fmaxf(top_of(s0), top_of(s1)), c);
-    V8 e[2];
-    f32x16 n;
-    if (more) n = scores(w, knext, 0);
-    weigh(w, s0, c, e);
-    accumulate<T, DP, false>(w, vnow, 0, e);
-    if (more) s0 = n;
-    __builtin_amdgcn_sched_barrier(0);
-    if (more) n = scores(w, knext, 32);
-    weigh(w, s1, c, e);
-    accumulate<T, DP, false>(w, vnow, 32, e);
-    if (more) s1 = n;
+    w.raise(tops, c);
+    const float base = w.m == -INFINITY ? 0.f : w.m;
+    auto weigh = [&](f32x16& s, int from, int to) {
+#pragma unroll
+      for (int i = from; i < to; ++i) {
+        s[i] = exp2_fast(fmaf(s[i], c, -base));
+        w.l += s[i];
+      }
+    };
+    auto key = [&](int i) { return key_fragment<T, DP>(knext, i / H::kSteps * 32, i % H::kSteps); };
+    auto value = [&](int i) { return value_fragment<T, DP, false>(vnow, i / H::kCols * 16, i % H::kCols); };
+    f32x16 n[2] = {};
+    V8 kf[3], vf[3], e[4];
+    if (more) {
+      kf[0] = key(0);
+      kf[1] = key(1);
+    }
+    auto score = [&](int i) {
+      n[i / H::kSteps] = mfma32(kf[i % 3], w.q[i % H::kSteps], n[i / H::kSteps]);
+      if (i + 2 < kScores) kf[(i + 2) % 3] = key(i + 2);
+    };
+    auto add = [&](int i) {
+      f32x16& o = w.o[i % H::kCols];
+      o = mfma32(vf[i % 3], e[i / H::kCols], o);
+      if (i + 2 < 2 * kValues) vf[(i + 2) % 3] = value(i + 2);
+    };
+    auto pack = [&](const f32x16& s, int to) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) e[to + i / 8][i % 8] = static_cast<T>(s[i]);
+    };
+#pragma unroll
+    for (int i = 0; i < kFirst; ++i) {
+      if (more) score(i);
+      weigh(s0, i * 16 / kFirst, (i + 1) * 16 / kFirst);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    pack(s0, 0);
+    vf[0] = value(0);
+    vf[1] = value(1);
+    constexpr int kSecond = kScores - kFirst + kValues;
+#pragma unroll
+    for (int i = 0; i < kSecond; ++i) {
+      if (i < kScores - kFirst) {
+        if (more) score(kFirst + i);
+      } else {
+        add(i - (kScores - kFirst));
+      }
+      weigh(s1, i * 16 / kSecond, (i + 1) * 16 / kSecond);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    pack(s1, 2);
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) {
+      add(kValues + i);
+      if (more) {
+#pragma unroll
+        for (int x = i * 16 / kValues; x < (i + 1) * 16 / kValues; ++x)
+          tops = x == 0 ? fmaxf(n[0][0], n[1][0]) : fmaxf(fmaxf(tops, n[0][x]), n[1][x]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (more) {
+      s0 = n[0];
+      s1 = n[1];
+    }
   };
   auto step = [&](int at, char* kfree, const char* knext, const char* vnow, char* vnext) {
     __syncthreads();
