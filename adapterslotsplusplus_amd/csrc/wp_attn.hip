@@ -38,17 +38,16 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
 constexpr int kWaveRows = 32;
-constexpr int kTileRows = kWaveRows * kWaves;  // query rows of a row tile
 constexpr int kTileKeys = 64;                  // keys staged at a time for a row tile
-constexpr int kChunkRows = kTileRows;           // most query rows of a sequence that runs on key chunks
+constexpr int kChunkWaves = 4;
+constexpr int kChunkRows = kWaveRows * kChunkWaves;  // most query rows of a sequence that runs on key chunks
 constexpr int kChunkKeys = 32;                 // keys a wave stages at a time for a key chunk
 // A running bound is raised (and O and l scaled) only once a score exceeds it
 // by 2^8: exponentials then stay within 2^8, far inside fp16, and most tiles
 // scale nothing.
 constexpr float kSlack = 8.f;
+constexpr int kNoSplit = 31;  // keys per split as a power of two: past every length
 
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -138,69 +137,117 @@ __device__ __forceinline__ Range keys_of(const AttnArgs& p, int n_q, int n_k, in
 __device__ __forceinline__ int chunks_of(int keys, int shift) {
   return std::max(1, static_cast<int>((static_cast<int64_t>(keys) + (1ll << shift) - 1) >> shift));
 }
-__device__ __forceinline__ int items_of(const AttnArgs& p, const Span& s, int group, bool rows_role, int* tiles) {
+__device__ __forceinline__ int items_of(const AttnArgs& p, const Span& s, int group, bool rows_role, int tile_rows, int* tiles) {
   const int rows = s.n_q * group;
   *tiles = 0;
   if (rows == 0 || (rows > kChunkRows) != rows_role) return 0;
   const Range r = keys_of(p, s.n_q, s.n_k, group, 0, rows);
   const int unit = rows_role ? kTileKeys : kChunkKeys;
   const int chunks = chunks_of(r.end - r.first / unit * unit, rows_role ? p.tile_shift : p.chunk_shift);
-  *tiles = rows_role ? (rows + kTileRows - 1) / kTileRows : 1;
+  *tiles = rows_role ? (rows + tile_rows - 1) / tile_rows : 1;
   return *tiles * chunks;
+}
+
+// The sum of v over the lanes up to this one, by lane moves within the vector
+// unit (a shuffle goes through LDS and takes some ten times as long).
+__device__ __forceinline__ int sum_up(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // from 1 lane down, in rows of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);  // 2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);  // 4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);  // 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true);  // the row before's last lane
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true);  // the first half's last lane
+  return v;
+}
+__device__ __forceinline__ int total_of(int v) { return __builtin_amdgcn_readlane(sum_up(v), 63); }
+
+__device__ __forceinline__ Item item_of(const AttnArgs& p, int head, int id, int seq, int tile, int chunk, int n_tiles,
+                                        int first_tile) {
+  Item it;
+  it.head = head;
+  it.slot = id;
+  it.seq = __builtin_amdgcn_readfirstlane(seq);
+  it.tile = __builtin_amdgcn_readfirstlane(tile);
+  it.chunk = __builtin_amdgcn_readfirstlane(chunk);
+  it.counter = __builtin_amdgcn_readfirstlane((first_tile + tile) * p.kv_heads + head);
+  it.stride = __builtin_amdgcn_readfirstlane(n_tiles * p.kv_heads);
+  const Span f = span_of(p, it.seq);
+  it.q0 = f.q0;
+  it.k0 = f.k0;
+  it.n_q = f.n_q;
+  it.n_k = f.n_k;
+  return it;
+}
+
+// Row tiles that run whole, of up to 64 sequences (a lane each): the tiles
+// with the most keys first, so that none of the long ones starts last.  The
+// tiles of a sequence that see at least w keys are its last ones; a search over
+// w finds the item's, and its place among the tiles that see exactly as many.
+// (16 prompts of 111 to 2501 tokens, 32 heads: 159 us in the sequences' order.)
+__device__ __forceinline__ Item find_by_weight(const AttnArgs& p, int group, int tile_rows, int id) {
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  int tiles = 0;
+  Span s{0, 0, 0, 0};
+  if (lane < p.n_seq) {
+    s = span_of(p, lane);
+    (void)items_of(p, s, group, true, tile_rows, &tiles);
+  }
+  const int lag = s.n_k - s.n_q;
+  // Tiles whose last row sees at least 64 u keys.
+  auto at_least = [&](int u) {
+    const int w = u * kTileKeys;
+    if (w > s.n_k) return 0;
+    if (!p.causal) return tiles;
+    const int64_t row = static_cast<int64_t>(w - lag - 1) * group;  // the first that sees w keys
+    const int64_t below = row <= 0 ? 0 : row / tile_rows;           // tiles before that row's
+    return below >= tiles ? 0 : static_cast<int>(tiles - below);
+  };
+  Item it;
+  it.seq = -1;
+  const int want = id / p.kv_heads;
+  if (want >= total_of(tiles)) return it;
+  int lo = -1, hi = static_cast<int>(p.keys / kTileKeys) + 1;  // more than `want` tiles see 64 lo keys, not 64 hi
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    if (total_of(at_least(mid)) > want) lo = mid; else hi = mid;
+  }
+  const int above = at_least(lo + 1), here = (lo < 0 ? tiles : at_least(lo)) - above;
+  const int rest = want - total_of(above);
+  const int upto = sum_up(here);
+  const int at = __builtin_ctzll(__ballot(upto > rest));
+  const int from = __builtin_amdgcn_readlane(above, at) + rest -
+                   (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(here, at));  // from the sequence's last tile
+  const int n_tiles = __builtin_amdgcn_readlane(tiles, at);
+  return item_of(p, id % p.kv_heads, id, at, n_tiles - 1 - from, 0, n_tiles, 0);
 }
 
 // The item of this workgroup: every wave counts through the sequences, 64 at
 // a time, a lane each.
-__device__ __forceinline__ Item find_item(const AttnArgs& p, int group, bool rows_role, int id) {
+__device__ __forceinline__ Item find_item(const AttnArgs& p, int group, bool rows_role, int tile_rows, int id) {
   const int lane = static_cast<int>(threadIdx.x) & 63;
-  Item it;
-  it.seq = -1;
-  it.head = id % p.kv_heads;
+  if (rows_role && p.tile_shift == kNoSplit && p.n_seq <= 64) return find_by_weight(p, group, tile_rows, id);
+  Item none;
+  none.seq = -1;
   const int want = id / p.kv_heads;
   int base = 0, tile_base = 0;
   for (int b0 = 0; b0 < p.n_seq; b0 += 64) {
     const int b = b0 + lane;
     int tiles = 0, items = 0;
-    Span s{0, 0, 0, 0};
-    if (b < p.n_seq) {
-      s = span_of(p, b);
-      items = items_of(p, s, group, rows_role, &tiles);
-    }
-    int sum = items, tile_sum = tiles;
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) {
-      const int u = __shfl_up(sum, x), v = __shfl_up(tile_sum, x);
-      sum += lane >= x ? u : 0;
-      tile_sum += lane >= x ? v : 0;
-    }
+    if (b < p.n_seq) items = items_of(p, span_of(p, b), group, rows_role, tile_rows, &tiles);
+    const int sum = sum_up(items), tile_sum = sum_up(tiles);
     const unsigned long long past = __ballot(base + sum > want);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
-      it.seq = b0 + at;
-      const int local = want - base - (__shfl(sum, at) - __shfl(items, at));
-      const int n_tiles = __shfl(tiles, at);
-      const int first_tile = tile_base + __shfl(tile_sum, at) - n_tiles;
+      const int local = want - base - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(items, at));
+      const int n_tiles = __builtin_amdgcn_readlane(tiles, at);
       // Later row tiles see more keys: they go first.
-      it.tile = n_tiles - 1 - local % n_tiles;
-      it.chunk = local / n_tiles;
-      it.slot = id;
-      it.counter = (first_tile + it.tile) * p.kv_heads + it.head;
-      it.stride = __builtin_amdgcn_readfirstlane(n_tiles * p.kv_heads);
-      it.seq = __builtin_amdgcn_readfirstlane(it.seq);
-      it.tile = __builtin_amdgcn_readfirstlane(it.tile);
-      it.chunk = __builtin_amdgcn_readfirstlane(it.chunk);
-      it.counter = __builtin_amdgcn_readfirstlane(it.counter);
-      const Span f = span_of(p, it.seq);
-      it.q0 = f.q0;
-      it.k0 = f.k0;
-      it.n_q = f.n_q;
-      it.n_k = f.n_k;
-      return it;
+      return item_of(p, id % p.kv_heads, id, b0 + at, n_tiles - 1 - local % n_tiles, local / n_tiles, n_tiles,
+                     tile_base + __builtin_amdgcn_readlane(tile_sum, at) - n_tiles);
     }
-    base += __shfl(sum, 63);
-    tile_base += __shfl(tile_sum, 63);
+    base += __builtin_amdgcn_readlane(sum, 63);
+    tile_base += __builtin_amdgcn_readlane(tile_sum, 63);
   }
-  return it;
+  return none;
 }
 
 // A wave's 32 query rows and their running state.
@@ -391,7 +438,7 @@ struct Staged {
 // While tile j is weighed and added, the scores of tile j + 1 are computed
 // (they need nothing of it, so the matrix cores work beside the exponentials), and tiles j + 2
 // of K and j + 1 of V are on their way.
-template <typename T, int DP>
+template <typename T, int DP, int kWaves>
 __device__ __forceinline__ void run_tile(const AttnArgs& p, const Item& it, Rows<T, DP>& w, float c, int first, int end,
                                          int wave_low, int wave_pos, int wave_last, int wave, WP_STAGED) {
   using H = Head<DP>;
@@ -518,7 +565,7 @@ __device__ __forceinline__ void run_tile(const AttnArgs& p, const Item& it, Rows
 
 // run_tile, one tile after the other, with infinite and NaN values left out of
 // the product and added to the rows that see them: the same sums otherwise.
-template <typename T, int DP>
+template <typename T, int DP, int kWaves>
 __device__ __forceinline__ void run_tile_careful(const AttnArgs& p, const Item& it, Rows<T, DP>& w, float c, int first,
                                                  int end, int wave_low, int wave_pos, int wave, char* sk, char* sv) {
   using H = Head<DP>;
@@ -605,9 +652,11 @@ __device__ __forceinline__ void finish_row(const AttnArgs& p, const Item& it, in
   if (p.lse && d == 0) p.lse[(it.q0 + tok) * p.heads + h] = sees ? fmaf(m, kLn2, logf(l)) : -INFINITY;
 }
 
-template <typename T, int DP>
-__global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs p) {
+// kWaves: of a row tile's workgroup; key chunks run with four.
+template <typename T, int DP, int kWaves>
+__global__ __launch_bounds__(64 * kWaves, 2) void attention_kernel(AttnArgs p) {
   using H = Head<DP>;
+  constexpr int kThreads = 64 * kWaves, kTileRows = kWaveRows * kWaves;
   __shared__ __align__(1024) char sk0[Staged<DP>::kBytes];
   __shared__ __align__(1024) char sk1[Staged<DP>::kBytes];
   __shared__ __align__(1024) char sv0[Staged<DP>::kBytes];
@@ -635,9 +684,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs p) {
     }
   }
 
-  const bool rows_role = static_cast<int>(blockIdx.x) < p.tile_items;
+  const bool rows_role = kWaves != kChunkWaves || static_cast<int>(blockIdx.x) < p.tile_items;
   const int id = rows_role ? static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x) - p.tile_items;
-  const Item it = find_item(p, group, rows_role, id);
+  const Item it = find_item(p, group, rows_role, kTileRows, id);
   // Bounds that do not rise could name more row tiles than there are counters.
   if (it.seq < 0 || it.counter >= (rows_role ? p.tile_counters : p.seq_counters)) return;
   const int n_rows = it.n_q * group;
@@ -686,12 +735,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs p) {
   }
 
   if (rows_role) {
-    run_tile<T, DP>(p, it, w, c, first, end, wave_low, wave_pos, wave_last, wave, sk0, sk1, sv0, sv1);
+    run_tile<T, DP, kWaves>(p, it, w, c, first, end, wave_low, wave_pos, wave_last, wave, sk0, sk1, sv0, sv1);
     // Infinite or NaN values reach every row of a tile through the product, as
     // zero times them: where there are any, the pass is made again with care.
     if (__syncthreads_or(has_nonfinite(w)))
-      run_tile_careful<T, DP>(p, it, w, c, first, end, wave_low, wave_pos, wave, sk0, sv0);
-  } else {
+      run_tile_careful<T, DP, kWaves>(p, it, w, c, first, end, wave_low, wave_pos, wave, sk0, sv0);
+  } else if constexpr (kWaves == kChunkWaves) {
     // A wave's 32 keys and values: half of an array each.
     char* k = (wave < 2 ? sk0 : sk1) + (wave & 1) * (Staged<DP>::kBytes / 2);
     char* v = (wave < 2 ? sv0 : sv1) + (wave & 1) * (Staged<DP>::kBytes / 2);
@@ -737,7 +786,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs p) {
           coherent_store16(mine, (2u * rows_cap + r * DP + i * 32 + e * 8 + half * 4) * 4u,
                            f32x4{w.o[i][e * 4], w.o[i][e * 4 + 1], w.o[i][e * 4 + 2], w.o[i][e * 4 + 3]});
     }
-  } else {
+  } else if constexpr (kWaves == kChunkWaves) {
     // The waves' shares joined: each scales its O to the common bound and
     // leaves it in LDS, [row][DP] in an array of its own.
     if (half == 0) {
@@ -819,16 +868,30 @@ __global__ __launch_bounds__(kThreads, 2) void attention_kernel(AttnArgs p) {
   }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int kWaves>
 hipError_t launch(const AttnArgs& a, hipStream_t stream) {
   const int grid = std::max(1, a.tile_items + a.chunk_items);
-  hipLaunchKernelGGL((attention_kernel<T, DP>), dim3(static_cast<uint32_t>(grid)), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((attention_kernel<T, DP, kWaves>), dim3(static_cast<uint32_t>(grid)), dim3(64 * kWaves), 0, stream, a);
   return hipGetLastError();
 }
 
+template <typename T, int DP>
+hipError_t launch_tiles(const AttnArgs& a, int tile_waves, hipStream_t stream) {
+  if (tile_waves == kChunkWaves) return launch<T, DP, kChunkWaves>(a, stream);
+  AttnArgs one = a;
+  one.chunk_items = 0;
+  const hipError_t rc = launch<T, DP, 8>(one, stream);
+  if (rc != hipSuccess || a.chunk_items == 0) return rc;
+  one = a;
+  one.tile_items = 0;
+  return launch<T, DP, kChunkWaves>(one, stream);
+}
+
 template <typename T>
-hipError_t launch_head(const AttnArgs& a, int dp, hipStream_t stream) {
-  return dp == 64 ? launch<T, 64>(a, stream) : dp == 96 ? launch<T, 96>(a, stream) : launch<T, 128>(a, stream);
+hipError_t launch_head(const AttnArgs& a, int dp, int tile_waves, hipStream_t stream) {
+  return dp == 64   ? launch_tiles<T, 64>(a, tile_waves, stream)
+         : dp == 96 ? launch_tiles<T, 96>(a, tile_waves, stream)
+                    : launch_tiles<T, 128>(a, tile_waves, stream);
 }
 
 }  // namespace
@@ -836,24 +899,26 @@ hipError_t launch_head(const AttnArgs& a, int dp, hipStream_t stream) {
 hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t stream) {
   const int dp = a.dim <= 64 ? 64 : a.dim <= 96 ? 96 : 128;
   const int64_t group = a.heads / a.kv_heads, rows = a.tokens * group;
-  const int64_t kNever = 31;  // a shift past every length: no split
   // Bounds on the work items, from the sizes the host knows: a sequence of
   // more than 128 rows has at most rows / 128 + 1 row tiles, and one of fewer
   // at most keys / chunk + 2 key chunks.
   const int64_t tile_seqs = std::min<int64_t>(a.n_seq, rows / (kChunkRows + 1));
-  const int64_t tiles = tile_seqs > 0 ? rows / kTileRows + tile_seqs : 0;
+  // Row tiles of 256 rows read K and V half as often as those of 128.
+  const int tile_waves = rows / 256 * a.kv_heads >= 2 * n_cu && rows >= 1024 * std::max(1, a.n_seq) ? 8 : 4;
+  const int64_t tile_rows = kWaveRows * tile_waves;
+  const int64_t tiles = tile_seqs > 0 ? rows / tile_rows + tile_seqs : 0;
   const int64_t chunk_seqs = std::min<int64_t>(a.n_seq, a.tokens);
   // Row tiles: enough of them for the device (two workgroups a compute unit)
   // run whole; fewer are split into ranges of at least 512 keys.
-  int64_t tile_shift = kNever;
-  if (tiles > 0 && std::max<int64_t>(1, rows / kTileRows) * a.kv_heads < n_cu)
-    for (tile_shift = 9; tile_shift < kNever; ++tile_shift)
+  int64_t tile_shift = kNoSplit;
+  if (tiles > 0 && std::max<int64_t>(1, rows / tile_rows) * a.kv_heads < n_cu)
+    for (tile_shift = 9; tile_shift < kNoSplit; ++tile_shift)
       if (tiles * ((a.keys >> tile_shift) + 2) * a.kv_heads <= 4 * n_cu) break;
-  int64_t tile_items = tiles * (tile_shift == kNever ? 1 : (a.keys >> tile_shift) + 2) * a.kv_heads;
-  uint64_t tile_floats = tile_shift == kNever ? 0 : static_cast<uint64_t>(tile_items) * kTileRows * (dp + 2);
-  int64_t tile_counters = tile_shift == kNever ? 0 : tiles * a.kv_heads;
+  int64_t tile_items = tiles * (tile_shift == kNoSplit ? 1 : (a.keys >> tile_shift) + 2) * a.kv_heads;
+  uint64_t tile_floats = tile_shift == kNoSplit ? 0 : static_cast<uint64_t>(tile_items) * tile_rows * (dp + 2);
+  int64_t tile_counters = tile_shift == kNoSplit ? 0 : tiles * a.kv_heads;
   if (tile_floats * 4 > a.part_bytes / 2 || tile_counters > a.n_counters / 2) {
-    tile_shift = kNever;
+    tile_shift = kNoSplit;
     tile_items = tiles * a.kv_heads;
     tile_floats = 0;
     tile_counters = 0;
@@ -861,14 +926,14 @@ hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t s
   // Key chunks: about six workgroups a compute unit, of at least 128 keys (32
   // for each wave).
   int64_t chunk_shift = 7;
-  while (chunk_shift < kNever && (a.keys >> chunk_shift) * a.kv_heads > 6 * n_cu) ++chunk_shift;
+  while (chunk_shift < kNoSplit && (a.keys >> chunk_shift) * a.kv_heads > 6 * n_cu) ++chunk_shift;
   int64_t chunk_items = chunk_seqs * a.kv_heads;
   uint64_t chunk_floats = 0;
   if (chunk_seqs > 0) {
     chunk_items = ((a.keys >> chunk_shift) + 2 * chunk_seqs) * a.kv_heads;
     chunk_floats = static_cast<uint64_t>(chunk_items) * kChunkRows * (dp + 2);
     if ((tile_floats + chunk_floats) * 4 > a.part_bytes || tile_counters + chunk_seqs * a.kv_heads > a.n_counters) {
-      chunk_shift = kNever;
+      chunk_shift = kNoSplit;
       chunk_items = chunk_seqs * a.kv_heads;
     }
   }
@@ -878,10 +943,10 @@ hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t s
   a.tile_shift = static_cast<int32_t>(tile_shift);
   a.chunk_shift = static_cast<int32_t>(chunk_shift);
   a.chunk_part = tile_floats;
-  a.tile_counters = tile_shift == kNever ? 0x7FFFFFFF : static_cast<int32_t>(tile_counters);
-  a.seq_counters = chunk_shift == kNever ? 0x7FFFFFFF : a.n_counters - static_cast<int32_t>(tile_counters);
+  a.tile_counters = tile_shift == kNoSplit ? 0x7FFFFFFF : static_cast<int32_t>(tile_counters);
+  a.seq_counters = chunk_shift == kNoSplit ? 0x7FFFFFFF : a.n_counters - static_cast<int32_t>(tile_counters);
   a.chunk_counters = static_cast<int32_t>(tile_counters);
-  return dtype_bf16 ? launch_head<__bf16>(a, dp, stream) : launch_head<_Float16>(a, dp, stream);
+  return dtype_bf16 ? launch_head<__bf16>(a, dp, tile_waves, stream) : launch_head<_Float16>(a, dp, tile_waves, stream);
 }
 
 }  // namespace wp
