@@ -323,10 +323,10 @@ __device__ __forceinline__ typename VecOf<T>::v8 value_fragment(const char* valu
   const int i = lane & 15, g = lane >> 4;
   const int r = 4 * (g >> 1) + (i >> 2);
   const int c = col * 4 + (g & 1) * 2 + ((i & 3) >> 1);
-  const char* at = values + (key0 + r) * H::kRow + ((c ^ H::value_swizzle(r)) << 4) + (i & 1) * 8;
+  const int at = (key0 + r) * H::kRow + ((c ^ H::value_swizzle(r)) << 4) + (i & 1) * 8;
   using L = __attribute__((address_space(3))) i16x4;
-  i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(at));
-  i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(at + 8 * H::kRow));
+  i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(values + at));
+  i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(values + (at + 8 * H::kRow)));
   if (kCareful) {
     lo = finite_only<T>(lo);
     hi = finite_only<T>(hi);
@@ -458,6 +458,7 @@ __device__ __forceinline__ void run_tile(const AttnArgs& p, const Item& it, Rows
   w.reset();
   if (first >= end) return;
   load_k(first, sk0);
+  wait_vm();
   __syncthreads();
   load_k(first + kTileKeys, sk1);
   load_v(first, sv0);
@@ -547,6 +548,7 @@ __device__ __forceinline__ void run_tile(const AttnArgs& p, const Item& it, Rows
     }
   };
   auto step = [&](int at, char* kfree, const char* knext, const char* vnow, char* vnext) {
+    wait_vm();
     __syncthreads();
     load_k(at + 2 * kTileKeys, kfree);
     load_v(at + kTileKeys, vnext);
@@ -577,6 +579,7 @@ __device__ __forceinline__ void run_tile_careful(const AttnArgs& p, const Item& 
     __syncthreads();
     stage<DP, false, kLoads>(k + at * p.k_tok, static_cast<uint32_t>(p.k_tok) * 2, p.dim, it.n_k - at, sk, wave * kLoads);
     stage<DP, true, kLoads>(v + at * p.v_tok, static_cast<uint32_t>(p.v_tok) * 2, p.dim, it.n_k - at, sv, wave * kLoads);
+    wait_vm();
     __syncthreads();
     f32x16 s0 = scores(w, sk, 0), s1 = scores(w, sk, 32);
     if (at < wave_low || at + kTileKeys - 1 > wave_pos) {
@@ -602,32 +605,36 @@ __device__ __forceinline__ void run_chunk(const AttnArgs& p, const Item& it, Row
   const T* k = head_row<T>(p.k, it.k0, p.k_tok, it.head * p.k_head);
   const T* v = head_row<T>(p.v, it.k0, p.v_tok, it.head * p.v_head);
   auto load_k = [&](int at) {
-    stage<DP, false, kLoads>(k + at * p.k_tok, static_cast<uint32_t>(p.k_tok) * 2, p.dim, it.n_k - at, sk, 0);
+    stage<DP, false, kLoads>(k + at * p.k_tok, static_cast<uint32_t>(p.k_tok) * 2, p.dim, end - at, sk, 0);
   };
   auto load_v = [&](int at) {
-    stage<DP, true, kLoads>(v + at * p.v_tok, static_cast<uint32_t>(p.v_tok) * 2, p.dim, it.n_k - at, sv, 0);
+    stage<DP, true, kLoads>(v + at * p.v_tok, static_cast<uint32_t>(p.v_tok) * 2, p.dim, end - at, sv, 0);
   };
   w.reset();
+  // K and V take turns in flight: while one is read the other's next keys are
+  // on their way, so each wait leaves the younger one's loads (a load past the
+  // end touches no memory and leaves zeros).
   int at = first + phase * kChunkKeys;
-  if (at < end) {
-    load_k(at);
-    load_v(at);
-  }
+  if (at >= end) return;
+  load_k(at);
+  load_v(at);
   for (; at < end; at += kChunkKeys * share) {
     const int next = at + kChunkKeys * share;
-    wait_vm();
+    wait_vm_but<kLoads>();
     f32x16 s = scores(w, sk, 0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (next < end) load_k(next);
+    load_k(next);
     if (!(at >= wave_low && at + kChunkKeys - 1 <= wave_pos)) w.mask(s, at);
     w.raise(top_of(s), c);
     typename VecOf<T>::v8 e[2];
     weigh(w, s, c, e);
+    wait_vm_but<kLoads>();
     accumulate<T, DP, kCareful>(w, sv, 0, e);
     if (kCareful) add_nonfinite(w, sv, at, kChunkKeys);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (next < end) load_v(next);
+    load_v(next);
   }
+  wait_vm();
 }
 
 template <typename T, int DP>

@@ -135,6 +135,9 @@ __device__ __forceinline__ void atomic_store_u(uint32_t* p, unsigned v) {
 // Waits until this wave's outstanding global loads, stores and atomics are
 // acknowledged, which for sc1 stores means they are device-visible.
 __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Waits for all vector-memory operations but the N youngest.
+template <int N>
+__device__ __forceinline__ void wait_vm_but() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void flag_error(uint32_t* header, uint32_t bits) { atomicOr(&header[kHdrErrors], bits); }
 
