@@ -15,11 +15,12 @@
 // out of LDS by the transposing read, four keys of a column at a time, in that
 // same order.
 //
-// Two roles share the launch.  Sequences with more than 128 rows per key head
-// run on row tiles: a workgroup's waves take 32 rows each and stage 64 keys
-// and values at a time in LDS for all of them.  Shorter ones (single tokens,
-// drafted tokens) run on key chunks: the waves share out the keys, 32 at a
-// time, and (past 32 rows) the rows, and each streams keys of its own.  Either role splits a long key range over
+// Two roles.  Sequences with many rows per key head run on row tiles: a
+// workgroup's waves take 32 rows each and stage 64 keys and values at a time
+// in LDS for all of them.  Short ones (single tokens, drafted tokens) run on
+// key chunks: the waves share out the keys, 32 at a time, and (past 32 rows)
+// the rows, and each streams keys of its own.  A launch has one role where the
+// host can tell, else both.  Either role splits a long key range over
 // workgroups where there are too few of them, and the last one of a row tile
 // to finish joins the partial results.
 #include <hip/hip_runtime.h>
@@ -47,6 +48,7 @@ constexpr int kChunkKeys = 32;                 // keys a wave stages at a time f
 // by 2^8: exponentials then stay within 2^8, far inside fp16, and most tiles
 // scale nothing.
 constexpr float kSlack = 8.f;
+constexpr int kTiles = 1, kChunks = 2;  // the roles of a launch
 constexpr int kNoSplit = 31;  // keys per split as a power of two: past every length
 
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
@@ -107,16 +109,20 @@ struct Item {
 };
 
 struct Span {
-  int64_t q0, k0;
-  int n_q, n_k;
+  int q0, k0, n_q, n_k;
 };
+// n / d, exactly for n < 2^31: the product is under 2^63.
+__device__ __forceinline__ int over(int n, const Divisor& d) {
+  return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * d.magic) >> d.shift);
+}
 __device__ __forceinline__ Span span_of(const AttnArgs& p, int b) {
   Span s;
-  const int64_t q0 = p.cu_q[b], q1 = p.cu_q[b + 1], k0 = p.cu_k[b], k1 = p.cu_k[b + 1];
-  s.q0 = std::clamp<int64_t>(q0, 0, p.tokens);
-  s.n_q = static_cast<int>(std::clamp<int64_t>(q1, s.q0, p.tokens) - s.q0);
-  s.k0 = std::clamp<int64_t>(k0, 0, p.keys);
-  s.n_k = static_cast<int>(std::clamp<int64_t>(k1, s.k0, p.keys) - s.k0);
+  const int q0 = p.cu_q[b], q1 = p.cu_q[b + 1], k0 = p.cu_k[b], k1 = p.cu_k[b + 1];
+  const int tokens = static_cast<int>(p.tokens), keys = static_cast<int>(p.keys);
+  s.q0 = std::clamp(q0, 0, tokens);
+  s.n_q = std::clamp(q1, s.q0, tokens) - s.q0;
+  s.k0 = std::clamp(k0, 0, keys);
+  s.n_k = std::clamp(k1, s.k0, keys) - s.k0;
   return s;
 }
 
@@ -124,10 +130,10 @@ __device__ __forceinline__ Span span_of(const AttnArgs& p, int b) {
 struct Range {
   int first, end;
 };
-__device__ __forceinline__ Range keys_of(const AttnArgs& p, int n_q, int n_k, int group, int row, int rows) {
+__device__ __forceinline__ Range keys_of(const AttnArgs& p, int n_q, int n_k, int row, int rows) {
   Range r{0, n_k};
   if (!p.causal) return r;
-  const int t0 = row / group, t1 = std::min(n_q - 1, (row + rows - 1) / group);
+  const int t0 = over(row, p.by_group), t1 = std::min(n_q - 1, over(row + rows - 1, p.by_group));
   r.end = std::clamp(t1 + n_k - n_q + 1, 0, n_k);
   if (p.window > 0) r.first = std::clamp(t0 + n_k - n_q - p.window + 1, 0, r.end);
   return r;
@@ -137,14 +143,17 @@ __device__ __forceinline__ Range keys_of(const AttnArgs& p, int n_q, int n_k, in
 __device__ __forceinline__ int chunks_of(int keys, int shift) {
   return std::max(1, static_cast<int>((static_cast<int64_t>(keys) + (1ll << shift) - 1) >> shift));
 }
-__device__ __forceinline__ int items_of(const AttnArgs& p, const Span& s, int group, bool rows_role, int tile_rows, int* tiles) {
-  const int rows = s.n_q * group;
+__device__ __forceinline__ int shift_of(const AttnArgs& p, int rows, bool rows_role) {
+  return rows_role ? p.tile_shift : rows > kChunkRows && !p.chunk_wide ? kNoSplit : p.chunk_shift;
+}
+__device__ __forceinline__ int items_of(const AttnArgs& p, const Span& s, bool rows_role, int tile_rows, int* tiles) {
+  const int rows = s.n_q * p.group;
   *tiles = 0;
-  if (rows == 0 || (rows > kChunkRows) != rows_role) return 0;
-  const Range r = keys_of(p, s.n_q, s.n_k, group, 0, rows);
+  if (rows == 0 || (rows > p.chunk_rows) != rows_role) return 0;
+  const Range r = keys_of(p, s.n_q, s.n_k, 0, rows);
   const int unit = rows_role ? kTileKeys : kChunkKeys;
-  const int chunks = chunks_of(r.end - r.first / unit * unit, rows_role ? p.tile_shift : p.chunk_shift);
-  *tiles = rows_role ? (rows + tile_rows - 1) / tile_rows : 1;
+  const int chunks = chunks_of(r.end - r.first / unit * unit, shift_of(p, rows, rows_role));
+  *tiles = (rows + tile_rows - 1) / tile_rows;
   return *tiles * chunks;
 }
 
@@ -161,7 +170,7 @@ __device__ __forceinline__ int sum_up(int v) {
 }
 __device__ __forceinline__ int total_of(int v) { return __builtin_amdgcn_readlane(sum_up(v), 63); }
 
-__device__ __forceinline__ Item item_of(const AttnArgs& p, int head, int id, int seq, int tile, int chunk, int n_tiles,
+__device__ __forceinline__ Item item_of(const AttnArgs& p, const Span& s, int lane, int head, int id, int seq, int tile, int chunk, int n_tiles,
                                         int first_tile) {
   Item it;
   it.head = head;
@@ -171,11 +180,10 @@ __device__ __forceinline__ Item item_of(const AttnArgs& p, int head, int id, int
   it.chunk = __builtin_amdgcn_readfirstlane(chunk);
   it.counter = __builtin_amdgcn_readfirstlane((first_tile + tile) * p.kv_heads + head);
   it.stride = __builtin_amdgcn_readfirstlane(n_tiles * p.kv_heads);
-  const Span f = span_of(p, it.seq);
-  it.q0 = f.q0;
-  it.k0 = f.k0;
-  it.n_q = f.n_q;
-  it.n_k = f.n_k;
+  it.q0 = __builtin_amdgcn_readlane(s.q0, lane);
+  it.k0 = __builtin_amdgcn_readlane(s.k0, lane);
+  it.n_q = __builtin_amdgcn_readlane(s.n_q, lane);
+  it.n_k = __builtin_amdgcn_readlane(s.n_k, lane);
   return it;
 }
 
@@ -184,13 +192,13 @@ __device__ __forceinline__ Item item_of(const AttnArgs& p, int head, int id, int
 // tiles of a sequence that see at least w keys are its last ones; a search over
 // w finds the item's, and its place among the tiles that see exactly as many.
 // (16 prompts of 111 to 2501 tokens, 32 heads: 159 us in the sequences' order.)
-__device__ __forceinline__ Item find_by_weight(const AttnArgs& p, int group, int tile_rows, int id) {
+__device__ __forceinline__ Item find_by_weight(const AttnArgs& p, int tile_rows, int id) {
   const int lane = static_cast<int>(threadIdx.x) & 63;
   int tiles = 0;
   Span s{0, 0, 0, 0};
   if (lane < p.n_seq) {
     s = span_of(p, lane);
-    (void)items_of(p, s, group, true, tile_rows, &tiles);
+    (void)items_of(p, s, true, tile_rows, &tiles);
   }
   const int lag = s.n_k - s.n_q;
   // Tiles whose last row sees at least 64 u keys.
@@ -198,13 +206,13 @@ __device__ __forceinline__ Item find_by_weight(const AttnArgs& p, int group, int
     const int w = u * kTileKeys;
     if (w > s.n_k) return 0;
     if (!p.causal) return tiles;
-    const int64_t row = static_cast<int64_t>(w - lag - 1) * group;  // the first that sees w keys
+    const int64_t row = static_cast<int64_t>(w - lag - 1) * p.group;  // the first that sees w keys
     const int64_t below = row <= 0 ? 0 : row / tile_rows;           // tiles before that row's
     return below >= tiles ? 0 : static_cast<int>(tiles - below);
   };
   Item it;
   it.seq = -1;
-  const int want = id / p.kv_heads;
+  const int want = over(id, p.by_heads);
   if (want >= total_of(tiles)) return it;
   int lo = -1, hi = static_cast<int>(p.keys / kTileKeys) + 1;  // more than `want` tiles see 64 lo keys, not 64 hi
   while (hi - lo > 1) {
@@ -218,22 +226,26 @@ __device__ __forceinline__ Item find_by_weight(const AttnArgs& p, int group, int
   const int from = __builtin_amdgcn_readlane(above, at) + rest -
                    (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(here, at));  // from the sequence's last tile
   const int n_tiles = __builtin_amdgcn_readlane(tiles, at);
-  return item_of(p, id % p.kv_heads, id, at, n_tiles - 1 - from, 0, n_tiles, 0);
+  return item_of(p, s, at, id - want * p.kv_heads, id, at, n_tiles - 1 - from, 0, n_tiles, 0);
 }
 
 // The item of this workgroup: every wave counts through the sequences, 64 at
 // a time, a lane each.
-__device__ __forceinline__ Item find_item(const AttnArgs& p, int group, bool rows_role, int tile_rows, int id) {
+__device__ __forceinline__ Item find_item(const AttnArgs& p, bool rows_role, int tile_rows, int id) {
   const int lane = static_cast<int>(threadIdx.x) & 63;
-  if (rows_role && p.tile_shift == kNoSplit && p.n_seq <= 64) return find_by_weight(p, group, tile_rows, id);
+  if (rows_role && p.tile_shift == kNoSplit && p.n_seq <= 64) return find_by_weight(p, tile_rows, id);
   Item none;
   none.seq = -1;
-  const int want = id / p.kv_heads;
+  const int want = over(id, p.by_heads);
   int base = 0, tile_base = 0;
   for (int b0 = 0; b0 < p.n_seq; b0 += 64) {
     const int b = b0 + lane;
     int tiles = 0, items = 0;
-    if (b < p.n_seq) items = items_of(p, span_of(p, b), group, rows_role, tile_rows, &tiles);
+    Span s{0, 0, 0, 0};
+    if (b < p.n_seq) {
+      s = span_of(p, b);
+      items = items_of(p, s, rows_role, tile_rows, &tiles);
+    }
     const int sum = sum_up(items), tile_sum = sum_up(tiles);
     const unsigned long long past = __ballot(base + sum > want);
     if (past != 0) {
@@ -241,7 +253,7 @@ __device__ __forceinline__ Item find_item(const AttnArgs& p, int group, bool row
       const int local = want - base - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(items, at));
       const int n_tiles = __builtin_amdgcn_readlane(tiles, at);
       // Later row tiles see more keys: they go first.
-      return item_of(p, id % p.kv_heads, id, b0 + at, n_tiles - 1 - local % n_tiles, local / n_tiles, n_tiles,
+      return item_of(p, s, at, id - want * p.kv_heads, id, b0 + at, n_tiles - 1 - local % n_tiles, local / n_tiles, n_tiles,
                      tile_base + __builtin_amdgcn_readlane(tile_sum, at) - n_tiles);
     }
     base += __builtin_amdgcn_readlane(sum, 63);
@@ -367,22 +379,33 @@ __device__ __forceinline__ void add_nonfinite(Rows<T, DP>& w, const char* values
   }
 }
 
-// Stages rows [0, rows) of 1024 / kRow * loads rows from `src` (rows `stride`
-// bytes apart) at `dst`: load i of this wave fills rows (first + i) *
-// kRowsPerLoad on, 16 bytes a lane, straight to LDS; rows past `rows` and
-// columns past the head are zero.
+// Staging: load i of a wave fills rows (first + i) * kRowsPerLoad on of a tile
+// straight in LDS, 16 bytes a lane.  A lane's offsets from the tile's first row
+// are the same for every tile; the rows past the tile's last one and the
+// columns past the head lie outside its bytes and are zero.
 template <int DP, bool kValues, int kLoads>
-__device__ __forceinline__ void stage(const void* src, uint32_t stride, int dim, int rows, char* dst, int first) {
+struct Loads {
   using H = Head<DP>;
-  const int lane = static_cast<int>(threadIdx.x) & 63;
+  int off[kLoads];
+  int stride, row_bytes, first;
+
+  __device__ __forceinline__ Loads(int64_t tok_stride, int dim, int first_load)
+      : stride(static_cast<int>(tok_stride) * 2), row_bytes(dim * 2), first(first_load) {
+    const int lane = static_cast<int>(threadIdx.x) & 63;
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int r = (first + i) * H::kRowsPerLoad + lane / H::kChunks;
-    const int c = (lane % H::kChunks) ^ (kValues ? H::value_swizzle(r) : H::key_swizzle(r));
-    const int off = r < rows && c * 8 < dim ? static_cast<int>(r * stride) + c * 16 : kOutside;
-    load_to_lds(src, dst + (first + i) * 1024, off, 0);
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = (first + i) * H::kRowsPerLoad + lane / H::kChunks;
+      const int c = (lane % H::kChunks) ^ (kValues ? H::value_swizzle(r) : H::key_swizzle(r));
+      off[i] = c * 8 < dim ? r * stride + c * 16 : kOutside;
+    }
   }
-}
+  // The first `rows` rows (at most the tile's) at src to dst.
+  __device__ __forceinline__ void stage(const void* src, int rows, char* dst) const {
+    const int size = rows <= 0 ? 0 : (std::min(rows, kTileKeys) - 1) * stride + row_bytes;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) load_to_lds(src, dst + (first + i) * 1024, off[i], 0, size);
+  }
+};
 
 template <typename T>
 __device__ __forceinline__ const T* head_row(const void* base, int64_t tok, int64_t tok_stride, int64_t head_offset) {
@@ -404,12 +427,21 @@ __device__ __forceinline__ void weigh(Rows<T, DP>& w, const f32x16& s, float c, 
     }
 }
 
-// Scores of 32 staged keys from row0 on.
+// Scores of 32 staged keys from row0 on; LDS reads go four products ahead.
 template <typename T, int DP>
 __device__ __forceinline__ f32x16 scores(const Rows<T, DP>& w, const char* keys, int row0) {
+  constexpr int kSteps = Head<DP>::kSteps;
+  typename VecOf<T>::v8 kf[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) kf[x] = key_fragment<T, DP>(keys, row0, x);
+  __builtin_amdgcn_sched_barrier(0);
   f32x16 s{};
 #pragma unroll
-  for (int x = 0; x < Head<DP>::kSteps; ++x) s = mfma32(key_fragment<T, DP>(keys, row0, x), w.q[x], s);
+  for (int x = 0; x < kSteps; ++x) {
+    s = mfma32(kf[x % 4], w.q[x], s);
+    if (x + 4 < kSteps) kf[x % 4] = key_fragment<T, DP>(keys, row0, x + 4);
+    __builtin_amdgcn_sched_barrier(0);
+  }
   return s;
 }
 
@@ -417,11 +449,18 @@ __device__ __forceinline__ f32x16 scores(const Rows<T, DP>& w, const char* keys,
 template <typename T, int DP, bool kCareful>
 __device__ __forceinline__ void accumulate(Rows<T, DP>& w, const char* values, int row0,
                                            const typename VecOf<T>::v8 (&e)[2]) {
+  constexpr int kCols = Head<DP>::kCols, kAhead = kCols < 4 ? kCols : 4;
+  auto value = [&](int i) { return value_fragment<T, DP, kCareful>(values, row0 + i / kCols * 16, i % kCols); };
+  typename VecOf<T>::v8 vf[kAhead];
 #pragma unroll
-  for (int b = 0; b < 2; ++b)
+  for (int i = 0; i < kAhead; ++i) vf[i] = value(i);
+  if (!kCareful) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int x = 0; x < Head<DP>::kCols; ++x)
-      w.o[x] = mfma32(value_fragment<T, DP, kCareful>(values, row0 + b * 16, x), e[b], w.o[x]);
+  for (int i = 0; i < 2 * kCols; ++i) {
+    w.o[i % kCols] = mfma32(vf[i % kAhead], e[i / kCols], w.o[i % kCols]);
+    if (i + kAhead < 2 * kCols) vf[i % kAhead] = value(i + kAhead);
+    if (!kCareful) __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 // LDS of a workgroup.  Each buffer is an array of its own: the compiler then
@@ -447,12 +486,14 @@ __device__ __forceinline__ void run_tile(const AttnArgs& p, const Item& it, Rows
   const T* k = head_row<T>(p.k, it.k0, p.k_tok, it.head * p.k_head);
   const T* v = head_row<T>(p.v, it.k0, p.v_tok, it.head * p.v_head);
   const int64_t k_tok = p.k_tok, v_tok = p.v_tok;
-  const int n_k = it.n_k, dim = p.dim;
+  const int n_k = it.n_k;
+  const Loads<DP, false, kLoads> loads_k(k_tok, p.dim, wave * kLoads);
+  const Loads<DP, true, kLoads> loads_v(v_tok, p.dim, wave * kLoads);
   auto load_k = [&](int at, char* to) {
-    if (at < end) stage<DP, false, kLoads>(k + at * k_tok, static_cast<uint32_t>(k_tok) * 2, dim, n_k - at, to, wave * kLoads);
+    if (at < end) loads_k.stage(k + at * k_tok, n_k - at, to);
   };
   auto load_v = [&](int at, char* to) {
-    if (at < end) stage<DP, true, kLoads>(v + at * v_tok, static_cast<uint32_t>(v_tok) * 2, dim, n_k - at, to, wave * kLoads);
+    if (at < end) loads_v.stage(v + at * v_tok, n_k - at, to);
   };
   const int live_end = std::min(end, wave_last + 1);
   w.reset();
@@ -574,11 +615,13 @@ __device__ __forceinline__ void run_tile_careful(const AttnArgs& p, const Item& 
   constexpr int kLoads = kTileKeys * H::kRow / 1024 / kWaves;
   const T* k = head_row<T>(p.k, it.k0, p.k_tok, it.head * p.k_head);
   const T* v = head_row<T>(p.v, it.k0, p.v_tok, it.head * p.v_head);
+  const Loads<DP, false, kLoads> loads_k(p.k_tok, p.dim, wave * kLoads);
+  const Loads<DP, true, kLoads> loads_v(p.v_tok, p.dim, wave * kLoads);
   w.reset();
   for (int at = first; at < end; at += kTileKeys) {
     __syncthreads();
-    stage<DP, false, kLoads>(k + at * p.k_tok, static_cast<uint32_t>(p.k_tok) * 2, p.dim, it.n_k - at, sk, wave * kLoads);
-    stage<DP, true, kLoads>(v + at * p.v_tok, static_cast<uint32_t>(p.v_tok) * 2, p.dim, it.n_k - at, sv, wave * kLoads);
+    loads_k.stage(k + at * p.k_tok, it.n_k - at, sk);
+    loads_v.stage(v + at * p.v_tok, it.n_k - at, sv);
     wait_vm();
     __syncthreads();
     f32x16 s0 = scores(w, sk, 0), s1 = scores(w, sk, 32);
@@ -596,43 +639,48 @@ __device__ __forceinline__ void run_tile_careful(const AttnArgs& p, const Item& 
   }
 }
 
-// Key chunk: keys [first, end), this wave taking every share-th 32 of them.
+// Key chunk: a wave's keys from `at` on, 32 at a time and `step` apart.
+template <typename T, int DP>
+struct ChunkLoads {
+  static constexpr int kLoads = kChunkKeys * Head<DP>::kRow / 1024;
+  const T* k;
+  const T* v;
+  int64_t k_tok, v_tok;
+  Loads<DP, false, kLoads> loads_k;
+  Loads<DP, true, kLoads> loads_v;
+  char* sk;
+  char* sv;
+  int end;
+  __device__ __forceinline__ ChunkLoads(const AttnArgs& p, const Item& it, int end_, char* sk_, char* sv_)
+      : k(head_row<T>(p.k, it.k0, p.k_tok, it.head * p.k_head)), v(head_row<T>(p.v, it.k0, p.v_tok, it.head * p.v_head)),
+        k_tok(p.k_tok), v_tok(p.v_tok), loads_k(p.k_tok, p.dim, 0), loads_v(p.v_tok, p.dim, 0), sk(sk_), sv(sv_), end(end_) {}
+  __device__ __forceinline__ void load_k(int at) const { loads_k.stage(k + at * k_tok, end - at, sk); }
+  __device__ __forceinline__ void load_v(int at) const { loads_v.stage(v + at * v_tok, end - at, sv); }
+};
+
+// The first keys and values are on their way.  K and V take turns in flight:
+// while one is read the other's next keys are coming, so each wait leaves the
+// younger one's loads (a load past the end touches no memory and leaves zeros).
 template <typename T, int DP, bool kCareful>
-__device__ __forceinline__ void run_chunk(const AttnArgs& p, const Item& it, Rows<T, DP>& w, float c, int first, int end,
-                                          int wave_low, int wave_pos, int phase, int share, char* sk, char* sv) {
-  using H = Head<DP>;
-  constexpr int kLoads = kChunkKeys * H::kRow / 1024;
-  const T* k = head_row<T>(p.k, it.k0, p.k_tok, it.head * p.k_head);
-  const T* v = head_row<T>(p.v, it.k0, p.v_tok, it.head * p.v_head);
-  auto load_k = [&](int at) {
-    stage<DP, false, kLoads>(k + at * p.k_tok, static_cast<uint32_t>(p.k_tok) * 2, p.dim, end - at, sk, 0);
-  };
-  auto load_v = [&](int at) {
-    stage<DP, true, kLoads>(v + at * p.v_tok, static_cast<uint32_t>(p.v_tok) * 2, p.dim, end - at, sv, 0);
-  };
+__device__ __forceinline__ void run_chunk(const ChunkLoads<T, DP>& in, Rows<T, DP>& w, float c, int at, int step,
+                                          int wave_low, int wave_pos) {
+  constexpr int kLoads = ChunkLoads<T, DP>::kLoads;
   w.reset();
-  // K and V take turns in flight: while one is read the other's next keys are
-  // on their way, so each wait leaves the younger one's loads (a load past the
-  // end touches no memory and leaves zeros).
-  int at = first + phase * kChunkKeys;
-  if (at >= end) return;
-  load_k(at);
-  load_v(at);
-  for (; at < end; at += kChunkKeys * share) {
-    const int next = at + kChunkKeys * share;
+  for (; at < in.end; at += step) {
+    const int next = at + step;
     wait_vm_but<kLoads>();
-    f32x16 s = scores(w, sk, 0);
+    f32x16 s = scores(w, in.sk, 0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    load_k(next);
+    in.load_k(next);
     if (!(at >= wave_low && at + kChunkKeys - 1 <= wave_pos)) w.mask(s, at);
     w.raise(top_of(s), c);
     typename VecOf<T>::v8 e[2];
     weigh(w, s, c, e);
     wait_vm_but<kLoads>();
-    accumulate<T, DP, kCareful>(w, sv, 0, e);
-    if (kCareful) add_nonfinite(w, sv, at, kChunkKeys);
+    accumulate<T, DP, kCareful>(w, in.sv, 0, e);
+    if (kCareful) add_nonfinite(w, in.sv, at, kChunkKeys);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    load_v(next);
+    in.load_v(next);
   }
   wait_vm();
 }
@@ -649,9 +697,9 @@ __device__ __forceinline__ bool has_nonfinite(const Rows<T, DP>& w) {
 
 // Writes four columns of a finished row (and with the first of them its lse).
 template <typename T>
-__device__ __forceinline__ void finish_row(const AttnArgs& p, const Item& it, int group, int row, int d, f32x4 v, float m,
+__device__ __forceinline__ void finish_row(const AttnArgs& p, const Item& it, int row, int d, f32x4 v, float m,
                                            float l) {
-  const int tok = row / group, h = it.head * group + row % group;
+  const int tok = over(row, p.by_group), h = it.head * p.group + row - tok * p.group;
   const int pos = p.causal ? std::min(tok + it.n_k - it.n_q, it.n_k - 1) : it.n_k - 1;
   const bool sees = pos >= 0;
   if (d < p.dim)
@@ -659,64 +707,46 @@ __device__ __forceinline__ void finish_row(const AttnArgs& p, const Item& it, in
   if (p.lse && d == 0) p.lse[(it.q0 + tok) * p.heads + h] = sees ? fmaf(m, kLn2, logf(l)) : -INFINITY;
 }
 
-// kWaves: of a row tile's workgroup; key chunks run with four.
-template <typename T, int DP, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, 2) void attention_kernel(AttnArgs p) {
+// Where a workgroup's waves meet.
+template <int kWaves>
+struct Shared {
+  float m[kWaves][kWaveRows];
+  float l[kWaves][kWaveRows];
+  uint32_t last;
+};
+
+// One work item.  sk0 to sv1: LDS, Staged<DP>::kBytes each; my_k, my_v: this
+// wave's halves of them on key chunks.
+template <typename T, int DP, int kWaves, int kRole>
+__device__ __forceinline__ void run_item(const AttnArgs& p, const Item& it, Shared<kWaves>& sh, WP_STAGED, char* my_k,
+                                         char* my_v) {
   using H = Head<DP>;
-  constexpr int kThreads = 64 * kWaves, kTileRows = kWaveRows * kWaves;
-  __shared__ __align__(1024) char sk0[Staged<DP>::kBytes];
-  __shared__ __align__(1024) char sk1[Staged<DP>::kBytes];
-  __shared__ __align__(1024) char sv0[Staged<DP>::kBytes];
-  __shared__ __align__(1024) char sv1[Staged<DP>::kBytes];
-  __shared__ float s_m[kWaves][kWaveRows];
-  __shared__ float s_l[kWaves][kWaveRows];
-  __shared__ uint32_t s_last;
+  auto area = [&](int i) -> char* { return i == 0 ? sk0 : i == 1 ? sk1 : i == 2 ? sv0 : sv1; };
+  constexpr bool kTile = kRole == kTiles;
+  constexpr int kThreads = 64 * kWaves, kRows = kWaveRows * kWaves;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int half = lane >> 5;
-  const int group = p.heads / p.kv_heads;
-
-  // Rows of no sequence: before the first bound and from the last one on.
-  {
-    const int64_t head_rows = p.n_seq > 0 ? std::clamp<int64_t>(p.cu_q[0], 0, p.tokens) : p.tokens;
-    const int64_t tail = p.n_seq > 0 ? std::clamp<int64_t>(p.cu_q[p.n_seq], head_rows, p.tokens) : p.tokens;
-    const int64_t n = (head_rows + p.tokens - tail) * p.heads;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kWaves + wave; i < n; i += static_cast<int64_t>(gridDim.x) * kWaves) {
-      int64_t t = i / p.heads;
-      const int h = static_cast<int>(i % p.heads);
-      if (t >= head_rows) t += tail - head_rows;
-      T* out = static_cast<T*>(p.out) + t * p.o_tok + h * p.o_head;
-      for (int d = lane; d < p.dim; d += 64) out[d] = static_cast<T>(0.f);
-      if (p.lse && lane == 0) p.lse[t * p.heads + h] = -INFINITY;
-    }
-  }
-
-  const bool rows_role = kWaves != kChunkWaves || static_cast<int>(blockIdx.x) < p.tile_items;
-  const int id = rows_role ? static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x) - p.tile_items;
-  const Item it = find_item(p, group, rows_role, kTileRows, id);
-  // Bounds that do not rise could name more row tiles than there are counters.
-  if (it.seq < 0 || it.counter >= (rows_role ? p.tile_counters : p.seq_counters)) return;
+  const int group = p.group;
   const int n_rows = it.n_q * group;
-  const int block_rows = kTileRows;
-  const int row0 = it.tile * block_rows;             // the workgroup's first row
-  const int my_rows = std::min(block_rows, n_rows - row0);
-  const Range range = keys_of(p, it.n_q, it.n_k, group, row0, my_rows);
-  const int shift = rows_role ? p.tile_shift : p.chunk_shift;
-  const int unit = rows_role ? kTileKeys : kChunkKeys;
+  const int row0 = it.tile * kRows;                  // the workgroup's first row
+  const int my_rows = std::min(kRows, n_rows - row0);
+  const Range range = keys_of(p, it.n_q, it.n_k, row0, my_rows);
+  const int shift = shift_of(p, n_rows, kTile);
+  constexpr int unit = kTile ? kTileKeys : kChunkKeys;
   const int base = range.first / unit * unit;        // tiles start at whole ones
   const int chunks = chunks_of(range.end - base, shift);
   if (it.chunk >= chunks) return;
   const int first = static_cast<int>(base + (static_cast<int64_t>(it.chunk) << shift));
   const int end = static_cast<int>(std::min<int64_t>(range.end, first + (1ll << shift)));
 
-  // This lane's query row.
   // On key chunks, `share` waves take each 32 rows, every share-th 32 keys.
-  const int row_waves = rows_role || my_rows > 2 * kWaveRows ? kWaves : my_rows > kWaveRows ? 2 : 1;
-  const int share = kWaves / row_waves;
-  const int wave_row0 = row0 + wave % row_waves * kWaveRows;
+  const int row_log = kTile || my_rows > 2 * kWaveRows ? (kWaves == 8 ? 3 : 2) : my_rows > kWaveRows ? 1 : 0;
+  const int row_waves = 1 << row_log, share = kWaves >> row_log;
+  const int wave_row0 = row0 + (wave & (row_waves - 1)) * kWaveRows;
   const int row = wave_row0 + (lane & 31);
   const bool real = row < n_rows;
-  const int tok = real ? row / group : 0, sub = real ? row % group : 0;
+  const int tok = real ? over(row, p.by_group) : 0, sub = real ? row - tok * group : 0;
   const float c = p.scale == 0.f ? 1.f : fabsf(p.scale) * kLog2e;
   Rows<T, DP> w;
   {
@@ -725,45 +755,55 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kernel(AttnArgs p) {
     for (int x = 0; x < H::kSteps; ++x) {
       const int d = x * 16 + half * 8;
       w.q[x] = real && d < p.dim && p.scale != 0.f ? load8(q + d) : zero8<T>();
-      if (p.scale < 0.f) w.q[x] = negate8<T>(w.q[x]);
     }
+  }
+  // A key chunk's first loads go out before the rest is worked out.
+  const int at0 = first + (wave >> row_log) * kChunkKeys, step_keys = kChunkKeys * share;
+  const ChunkLoads<T, DP> in(p, it, end, my_k, my_v);
+  auto start = [&] {
+    in.load_k(at0);
+    in.load_v(at0);
+  };
+  if (!kTile) start();
+  if (p.scale < 0.f) {
+#pragma unroll
+    for (int x = 0; x < H::kSteps; ++x) w.q[x] = negate8<T>(w.q[x]);
   }
   const int lag = it.n_k - it.n_q;
   w.pos = real ? (p.causal ? std::min(tok + lag, it.n_k - 1) : it.n_k - 1) : -1;
   w.low = p.causal && p.window > 0 ? std::max(0, tok + lag - p.window + 1) : 0;
-  // The keys that all of the wave's rows see.
-  // wave_last: the last key that any of them sees.
+  // wave_low, wave_pos: the keys that all of the wave's rows see; wave_last: the
+  // last one that any of them sees.
   int wave_pos = it.n_k - 1, wave_low = 0, wave_last = wave_row0 < n_rows ? it.n_k - 1 : -1;
   if (p.causal) {
-    const int t0 = wave_row0 / group, t1 = std::min(it.n_q - 1, (wave_row0 + kWaveRows - 1) / group);
+    const int t0 = over(wave_row0, p.by_group), t1 = std::min(it.n_q - 1, over(wave_row0 + kWaveRows - 1, p.by_group));
     wave_pos = wave_row0 < n_rows ? t0 + lag : -1;
     wave_last = wave_row0 < n_rows ? t1 + lag : -1;
     if (p.window > 0) wave_low = std::max(0, t1 + lag - p.window + 1);
   }
 
-  if (rows_role) {
+  if constexpr (kTile) {
     run_tile<T, DP, kWaves>(p, it, w, c, first, end, wave_low, wave_pos, wave_last, wave, sk0, sk1, sv0, sv1);
     // Infinite or NaN values reach every row of a tile through the product, as
     // zero times them: where there are any, the pass is made again with care.
     if (__syncthreads_or(has_nonfinite(w)))
       run_tile_careful<T, DP, kWaves>(p, it, w, c, first, end, wave_low, wave_pos, wave, sk0, sv0);
-  } else if constexpr (kWaves == kChunkWaves) {
-    // A wave's 32 keys and values: half of an array each.
-    char* k = (wave < 2 ? sk0 : sk1) + (wave & 1) * (Staged<DP>::kBytes / 2);
-    char* v = (wave < 2 ? sv0 : sv1) + (wave & 1) * (Staged<DP>::kBytes / 2);
-    run_chunk<T, DP, false>(p, it, w, c, first, end, wave_low, wave_pos, wave / row_waves, share, k, v);
-    if (__any(has_nonfinite(w))) run_chunk<T, DP, true>(p, it, w, c, first, end, wave_low, wave_pos, wave / row_waves, share, k, v);
+  } else {
+    run_chunk<T, DP, false>(in, w, c, at0, step_keys, wave_low, wave_pos);
+    if (__any(has_nonfinite(w))) {
+      start();
+      run_chunk<T, DP, true>(in, w, c, at0, step_keys, wave_low, wave_pos);
+    }
   }
   w.l += __shfl_xor(w.l, 32);
 
   const bool split = chunks > 1;
   const bool sees = real && w.pos >= w.low;
-  const int rows_cap = block_rows;
   // The item's partials: [rows][bound, sum], then [rows][DP] of O.
-  float* part = p.part + (rows_role ? 0 : p.chunk_part) + static_cast<uint64_t>(it.slot) * rows_cap * (DP + 2);
-  const __amdgpu_buffer_rsrc_t mine = coherent_buffer(part, static_cast<uint32_t>(rows_cap) * (DP + 2) * 4u);
+  float* part = p.part + (kTile ? 0 : p.chunk_part) + static_cast<uint64_t>(it.slot) * kRows * (DP + 2);
+  const __amdgpu_buffer_rsrc_t mine = coherent_buffer(part, static_cast<uint32_t>(kRows) * (DP + 2) * 4u);
 
-  if (rows_role) {
+  if (kTile || share == 1) {
     const float inv = 1.f / w.l;
     if (!split) {
       if (!real) return;
@@ -790,21 +830,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kernel(AttnArgs p) {
       for (int i = 0; i < H::kCols; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          coherent_store16(mine, (2u * rows_cap + r * DP + i * 32 + e * 8 + half * 4) * 4u,
+          coherent_store16(mine, (2u * kRows + r * DP + i * 32 + e * 8 + half * 4) * 4u,
                            f32x4{w.o[i][e * 4], w.o[i][e * 4 + 1], w.o[i][e * 4 + 2], w.o[i][e * 4 + 3]});
     }
-  } else if constexpr (kWaves == kChunkWaves) {
+  } else {
     // The waves' shares joined: each scales its O to the common bound and
     // leaves it in LDS, [row][DP] in an array of its own.
     if (half == 0) {
-      s_m[wave][lane] = w.m;
-      s_l[wave][lane] = w.l;
+      sh.m[wave][lane] = w.m;
+      sh.l[wave][lane] = w.l;
     }
     __syncthreads();
     float m = w.m;
-    for (int i = 1; i < share; ++i) m = fmaxf(m, s_m[(wave + i * row_waves) % kWaves][lane & 31]);
+    for (int i = 1; i < share; ++i) m = fmaxf(m, sh.m[(wave + i * row_waves) & (kWaves - 1)][lane & 31]);
     const float fade = m == -INFINITY ? 1.f : exp2_fast(w.m - m);
-    char* o32 = wave == 0 ? sk0 : wave == 1 ? sk1 : wave == 2 ? sv0 : sv1;
+    char* o32 = area(wave);
     if (real)
 #pragma unroll
       for (int i = 0; i < H::kCols; ++i)
@@ -816,19 +856,26 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kernel(AttnArgs p) {
     for (int u = tid; u < my_rows * (DP / 4); u += kThreads) {
       const int r = u / (DP / 4), d = u % (DP / 4) * 4;
       const int w0 = r / kWaveRows, q = r % kWaveRows;
-      float top = s_m[w0][q], l = 0.f;
-      for (int i = 1; i < share; ++i) top = fmaxf(top, s_m[w0 + i * row_waves][q]);
+      float ms[kWaves], ls[kWaves];
       f32x4 v{0.f, 0.f, 0.f, 0.f};
-      for (int i = 0; i < share; ++i) {
-        const int x = w0 + i * row_waves;
-        l += s_l[x][q] * (top == -INFINITY ? 1.f : exp2_fast(s_m[x][q] - top));
-        v += *reinterpret_cast<const f32x4*>((x == 0 ? sk0 : x == 1 ? sk1 : x == 2 ? sv0 : sv1) + (q * DP + d) * 4);
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) {
+        const int x = w0 + (i < share ? i : 0) * row_waves;
+        const f32x4 o = *reinterpret_cast<const f32x4*>(area(x) + (q * DP + d) * 4);
+        ms[i] = sh.m[x][q];
+        ls[i] = i < share ? sh.l[x][q] : 0.f;
+        if (i < share) v += o;
       }
+      float top = ms[0], l = 0.f;
+#pragma unroll
+      for (int i = 1; i < kWaves; ++i) top = fmaxf(top, ms[i]);
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) l += ls[i] * (top == -INFINITY ? 1.f : exp2_fast(ms[i] - top));
       if (split) {
-        coherent_store16(mine, (2u * rows_cap + r * DP + d) * 4u, v);
+        coherent_store16(mine, (2u * kRows + r * DP + d) * 4u, v);
         if (d == 0) coherent_store8(part + 2 * r, __builtin_bit_cast(unsigned long long, f32x2{top, l}));
       } else {
-        finish_row<T>(p, it, group, row0 + r, d, v, top, l);
+        finish_row<T>(p, it, row0 + r, d, v, top, l);
       }
     }
     if (!split) return;
@@ -838,14 +885,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kernel(AttnArgs p) {
   wait_vm();
   __syncthreads();
   if (tid == 0) {
-    uint32_t* cnt = p.counters + (rows_role ? 0 : p.chunk_counters) + it.counter;
+    uint32_t* cnt = p.counters + (kTile ? 0 : p.chunk_counters) + it.counter;
     const bool last = atomic_add_u(cnt, 1u) == static_cast<unsigned>(chunks - 1);
     if (last) atomic_store_u(cnt, 0u);
-    s_last = last ? 1u : 0u;
+    sh.last = last ? 1u : 0u;
   }
   __syncthreads();
-  if (s_last == 0u) return;
-  const int64_t step = static_cast<int64_t>(it.stride) * rows_cap * (DP + 2);  // floats between chunks' partials
+  if (sh.last == 0u) return;
+  const int64_t step = static_cast<int64_t>(it.stride) * kRows * (DP + 2);  // floats between chunks' partials
   const float* part0 = part - it.chunk * step;
   for (int u = tid; u < my_rows * (DP / 4); u += kThreads) {
     const int r = u / (DP / 4), d = u % (DP / 4) * 4;
@@ -859,7 +906,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kernel(AttnArgs p) {
       for (int i = 0; i < kBatch; ++i) {
         const float* at = part0 + std::min(i0 + i, chunks - 1) * step;
         ml[i] = __builtin_bit_cast(f32x2, coherent_load8(at + 2 * r));
-        o[i] = coherent_load_f4(at + 2 * rows_cap + r * DP + d);
+        o[i] = coherent_load_f4(at + 2 * kRows + r * DP + d);
       }
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
@@ -871,50 +918,133 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_kernel(AttnArgs p) {
         top = m;
       }
     }
-    finish_row<T>(p, it, group, row0 + r, d, v, top, l);
+    finish_row<T>(p, it, row0 + r, d, v, top, l);
   }
 }
 
-template <typename T, int DP, int kWaves>
-hipError_t launch(const AttnArgs& a, hipStream_t stream) {
-  const int grid = std::max(1, a.tile_items + a.chunk_items);
-  hipLaunchKernelGGL((attention_kernel<T, DP, kWaves>), dim3(static_cast<uint32_t>(grid)), dim3(64 * kWaves), 0, stream, a);
+// Clears the rows of no sequence: before the first bound and from the last one on.
+template <typename T, int kWaves>
+__device__ __forceinline__ void clear_rest(const AttnArgs& p, int bound0, int bound1) {
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int64_t head_rows = p.n_seq > 0 ? std::clamp<int64_t>(bound0, 0, p.tokens) : p.tokens;
+  const int64_t tail = p.n_seq > 0 ? std::clamp<int64_t>(bound1, head_rows, p.tokens) : p.tokens;
+  const int64_t n = (head_rows + p.tokens - tail) * p.heads;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kWaves + wave; i < n; i += static_cast<int64_t>(gridDim.x) * kWaves) {
+    int64_t t = i / p.heads;
+    const int h = static_cast<int>(i % p.heads);
+    if (t >= head_rows) t += tail - head_rows;
+    T* out = static_cast<T*>(p.out) + t * p.o_tok + h * p.o_head;
+    for (int d = lane; d < p.dim; d += 64) out[d] = static_cast<T>(0.f);
+    if (p.lse && lane == 0) p.lse[t * p.heads + h] = -INFINITY;
+  }
+}
+
+// Key chunks by themselves: as many workgroups a compute unit as LDS holds
+// or the registers hold (three at heads of up to 64, else two).
+template <int DP, int kRoles>
+constexpr int kOccupancy = kRoles != kChunks || DP > 64 ? 2 : 3;
+
+template <typename T, int DP, int kWaves, int kRoles>
+__global__ __launch_bounds__(64 * kWaves, (kOccupancy<DP, kRoles>)) void attention_kernel(AttnArgs p) {
+  constexpr int kRows = kWaveRows * kWaves, kHalf = Staged<DP>::kBytes / 2;
+  __shared__ Shared<kWaves> sh;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+
+  // Read beside the first item's bounds; used once that is found.
+  const int bound0 = p.n_seq > 0 ? p.cu_q[0] : 0, bound1 = p.n_seq > 0 ? p.cu_q[p.n_seq] : 0;
+  if constexpr (kRoles == kChunks) {
+    __shared__ __align__(1024) char sk[2][Staged<DP>::kBytes];
+    __shared__ __align__(1024) char sv[2][Staged<DP>::kBytes];
+    // The grid covers the items that there usually are, the loop the most that there can be.
+    int id = static_cast<int>(blockIdx.x);
+    Item it = find_item(p, false, kRows, id);
+    clear_rest<T, kWaves>(p, bound0, bound1);
+    // Bounds that do not rise could name more row tiles than there are counters.
+    while (id < p.chunk_items && it.seq >= 0 && it.counter < p.seq_counters) {
+      run_item<T, DP, kWaves, kChunks>(p, it, sh, sk[0], sk[1], sv[0], sv[1], &sk[0][0] + wave * kHalf, &sv[0][0] + wave * kHalf);
+      id += static_cast<int>(gridDim.x);
+      if (id >= p.chunk_items) return;
+      __syncthreads();
+      it = find_item(p, false, kRows, id);
+    }
+  } else {
+    __shared__ __align__(1024) char sk0[Staged<DP>::kBytes];
+    __shared__ __align__(1024) char sk1[Staged<DP>::kBytes];
+    __shared__ __align__(1024) char sv0[Staged<DP>::kBytes];
+    __shared__ __align__(1024) char sv1[Staged<DP>::kBytes];
+    const int block = static_cast<int>(blockIdx.x);
+    const bool rows_role = (kRoles & kChunks) == 0 || block < p.tile_items;
+    const Item it = find_item(p, rows_role, kRows, rows_role ? block : block - p.tile_items);
+    clear_rest<T, kWaves>(p, bound0, bound1);
+    if (it.seq < 0 || it.counter >= (rows_role ? p.tile_counters : p.seq_counters)) return;
+    if (rows_role) {
+      run_item<T, DP, kWaves, kTiles>(p, it, sh, sk0, sk1, sv0, sv1, nullptr, nullptr);
+    } else if constexpr ((kRoles & kChunks) != 0) {
+      run_item<T, DP, kWaves, kChunks>(p, it, sh, sk0, sk1, sv0, sv1, (wave < 2 ? sk0 : sk1) + (wave & 1) * kHalf,
+                                       (wave < 2 ? sv0 : sv1) + (wave & 1) * kHalf);
+    }
+  }
+}
+
+template <typename T, int DP, int kWaves, int kRoles>
+hipError_t launch(const AttnArgs& a, int grid, hipStream_t stream) {
+  hipLaunchKernelGGL((attention_kernel<T, DP, kWaves, kRoles>), dim3(static_cast<uint32_t>(std::max(1, grid))),
+                     dim3(64 * kWaves), 0, stream, a);
   return hipGetLastError();
 }
 
 template <typename T, int DP>
-hipError_t launch_tiles(const AttnArgs& a, int tile_waves, hipStream_t stream) {
-  if (tile_waves == kChunkWaves) return launch<T, DP, kChunkWaves>(a, stream);
-  AttnArgs one = a;
-  one.chunk_items = 0;
-  const hipError_t rc = launch<T, DP, 8>(one, stream);
-  if (rc != hipSuccess || a.chunk_items == 0) return rc;
-  one = a;
-  one.tile_items = 0;
-  return launch<T, DP, kChunkWaves>(one, stream);
+hipError_t launch_roles(const AttnArgs& a, int tile_waves, int chunk_grid, hipStream_t stream) {
+  if (a.tile_items == 0) return launch<T, DP, kChunkWaves, kChunks>(a, chunk_grid, stream);
+  if (tile_waves == kChunkWaves)
+    return a.chunk_items == 0 ? launch<T, DP, kChunkWaves, kTiles>(a, a.tile_items, stream)
+                              : launch<T, DP, kChunkWaves, kTiles | kChunks>(a, a.tile_items + a.chunk_items, stream);
+  const hipError_t rc = launch<T, DP, 8, kTiles>(a, a.tile_items, stream);
+  return rc != hipSuccess || a.chunk_items == 0 ? rc : launch<T, DP, kChunkWaves, kChunks>(a, chunk_grid, stream);
 }
 
 template <typename T>
-hipError_t launch_head(const AttnArgs& a, int dp, int tile_waves, hipStream_t stream) {
-  return dp == 64   ? launch_tiles<T, 64>(a, tile_waves, stream)
-         : dp == 96 ? launch_tiles<T, 96>(a, tile_waves, stream)
-                    : launch_tiles<T, 128>(a, tile_waves, stream);
+hipError_t launch_head(const AttnArgs& a, int dp, int tile_waves, int chunk_grid, hipStream_t stream) {
+  return dp == 64   ? launch_roles<T, 64>(a, tile_waves, chunk_grid, stream)
+         : dp == 96 ? launch_roles<T, 96>(a, tile_waves, chunk_grid, stream)
+                    : launch_roles<T, 128>(a, tile_waves, chunk_grid, stream);
 }
 
 }  // namespace
 
+// Exact for every dividend under 2^31: the quotient's error is under
+// dividend / 2^shift * d < 1 / d of a step.
+static Divisor divisor_of(int d) {
+  Divisor r{0, 31};
+  while ((1ll << (r.shift - 31)) < d) ++r.shift;
+  r.magic = static_cast<uint32_t>(((1ull << r.shift) + static_cast<uint64_t>(d) - 1) / static_cast<uint64_t>(d));
+  return r;
+}
+
 hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t stream) {
   const int dp = a.dim <= 64 ? 64 : a.dim <= 96 ? 96 : 128;
-  const int64_t group = a.heads / a.kv_heads, rows = a.tokens * group;
+  a.group = a.heads / a.kv_heads;
+  a.by_group = divisor_of(a.group);
+  a.by_heads = divisor_of(a.kv_heads);
+  const int64_t group = a.group, rows = a.tokens * group;
   // Bounds on the work items, from the sizes the host knows: a sequence of
   // more than 128 rows has at most rows / 128 + 1 row tiles, and one of fewer
   // at most keys / chunk + 2 key chunks.
-  const int64_t tile_seqs = std::min<int64_t>(a.n_seq, rows / (kChunkRows + 1));
+  const int64_t seqs = std::max(1, a.n_seq);
+  // One sequence has one role.  Many of a few rows each (drafted tokens; their
+  // mean at most 64 and none of more than 1024 if all have a token) run on key
+  // chunks alone, in a kernel of half the registers.  Others share a launch,
+  // where sequences run on key chunks up to 128 rows, or up to 32 next to longer ones.
+  const int64_t longest = (std::max<int64_t>(0, a.tokens - seqs) + 1) * group;
+  const bool few = a.n_seq <= 1 ? rows <= kChunkRows : rows <= 64 * seqs && longest <= 1024;
+  a.chunk_rows = few ? 0x7FFFFFFF : a.n_seq <= 1 ? 0 : rows >= kChunkRows * seqs ? kWaveRows : kChunkRows;
+  const int64_t tile_seqs = few ? 0 : std::min<int64_t>(a.n_seq, rows / (a.chunk_rows + 1));
   // Row tiles of 256 rows read K and V half as often as those of 128.
   const int tile_waves = rows / 256 * a.kv_heads >= 2 * n_cu && rows >= 1024 * std::max(1, a.n_seq) ? 8 : 4;
   const int64_t tile_rows = kWaveRows * tile_waves;
   const int64_t tiles = tile_seqs > 0 ? rows / tile_rows + tile_seqs : 0;
-  const int64_t chunk_seqs = std::min<int64_t>(a.n_seq, a.tokens);
+  const int64_t chunk_seqs = a.chunk_rows == 0 ? 0 : std::min<int64_t>(a.n_seq, a.tokens);
   // Row tiles: enough of them for the device (two workgroups a compute unit)
   // run whole; fewer are split into ranges of at least 512 keys.
   int64_t tile_shift = kNoSplit;
@@ -934,14 +1064,22 @@ hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t s
   // for each wave).
   int64_t chunk_shift = 7;
   while (chunk_shift < kNoSplit && (a.keys >> chunk_shift) * a.kv_heads > 6 * n_cu) ++chunk_shift;
-  int64_t chunk_items = chunk_seqs * a.kv_heads;
-  uint64_t chunk_floats = 0;
+  // Blocks of 128 rows: where sequences of more than 128 run on key chunks, the
+  // longest could have them all.
+  const int64_t blocks = few ? std::max<int64_t>(1, (rows + kChunkRows - 1) / kChunkRows) : 1;
+  const int64_t usual = ((a.keys >> chunk_shift) + 2 * chunk_seqs) * a.kv_heads;
+  int64_t chunk_items = 0, chunk_grid = 0;
   if (chunk_seqs > 0) {
-    chunk_items = ((a.keys >> chunk_shift) + 2 * chunk_seqs) * a.kv_heads;
-    chunk_floats = static_cast<uint64_t>(chunk_items) * kChunkRows * (dp + 2);
-    if ((tile_floats + chunk_floats) * 4 > a.part_bytes || tile_counters + chunk_seqs * a.kv_heads > a.n_counters) {
+    const int64_t counters = tile_counters + (chunk_seqs + blocks) * a.kv_heads;
+    auto fits = [&](int64_t items) {
+      return (tile_floats + static_cast<uint64_t>(items) * kChunkRows * (dp + 2)) * 4 <= a.part_bytes && counters <= a.n_counters;
+    };
+    a.chunk_wide = fits(usual * blocks);
+    chunk_items = a.chunk_wide ? usual * blocks : usual + blocks * a.kv_heads;
+    chunk_grid = usual;
+    if (!fits(chunk_items)) {
       chunk_shift = kNoSplit;
-      chunk_items = chunk_seqs * a.kv_heads;
+      chunk_items = chunk_grid = (chunk_seqs + blocks) * a.kv_heads;
     }
   }
   if (tile_items + chunk_items > 0x7FFFFFFF) return hipErrorInvalidValue;
@@ -953,7 +1091,8 @@ hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t s
   a.tile_counters = tile_shift == kNoSplit ? 0x7FFFFFFF : static_cast<int32_t>(tile_counters);
   a.seq_counters = chunk_shift == kNoSplit ? 0x7FFFFFFF : a.n_counters - static_cast<int32_t>(tile_counters);
   a.chunk_counters = static_cast<int32_t>(tile_counters);
-  return dtype_bf16 ? launch_head<__bf16>(a, dp, tile_waves, stream) : launch_head<_Float16>(a, dp, tile_waves, stream);
+  return dtype_bf16 ? launch_head<__bf16>(a, dp, tile_waves, static_cast<int>(chunk_grid), stream)
+                    : launch_head<_Float16>(a, dp, tile_waves, static_cast<int>(chunk_grid), stream);
 }
 
 }  // namespace wp

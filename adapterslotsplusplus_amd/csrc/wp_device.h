@@ -57,10 +57,11 @@ __device__ __forceinline__ u32x4 load16_global(const void* p) {
   return *reinterpret_cast<const __attribute__((address_space(1))) u32x4*>(reinterpret_cast<uintptr_t>(p));
 }
 // 16 bytes a lane from `src` + its `off` + `more` (uniform) straight to LDS:
-// lane l's at dst + 16 l.  off = kOutside: zeros.  Offsets stay under 2 GiB.
+// lane l's at dst + 16 l.  off >= size (kOutside always is): zeros.  Offsets
+// stay under 2 GiB.
 constexpr int kOutside = 0x7FFFFF00;
-__device__ __forceinline__ void load_to_lds(const void* src, char* dst, int off, int more) {
-  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(src), 0, kOutside, 0x00020000);
+__device__ __forceinline__ void load_to_lds(const void* src, char* dst, int off, int more, int size = kOutside) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(src), 0, size, 0x00020000);
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst, 16, off, more, 0, 0);
 }
 template <typename T>

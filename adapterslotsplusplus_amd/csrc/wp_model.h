@@ -49,6 +49,11 @@ hipError_t launch_proj(int dtype_bf16, ProjArgs& a, int n_cu, hipStream_t stream
 // are 0 and -inf for a query that sees no key and for rows of no sequence.
 // Strides in elements; head rows are contiguous.
 constexpr int kMaxHeadDim = 128;
+// Division by a number that the host knows: (n * magic) >> shift.
+struct Divisor {
+  uint32_t magic;
+  int32_t shift;
+};
 struct AttnArgs {
   const void* q;
   const void* k;
@@ -69,8 +74,12 @@ struct AttnArgs {
   // Filled by launch_attention: work items of either role (upper bounds; the
   // workgroups past the last one leave), the keys per split as a power of
   // two, and where the second role's partials and counters start.
+  int32_t group;  // query heads of a key head
+  Divisor by_group, by_heads;
   int32_t tile_items, chunk_items;
   int32_t tile_shift, chunk_shift;
+  int32_t chunk_rows;  // most rows per key head of a sequence that runs on key chunks
+  int32_t chunk_wide;  // sequences of more rows than a workgroup takes have their keys split there too
   int32_t chunk_counters;
   int32_t tile_counters, seq_counters;  // how many either role has
   uint64_t chunk_part;
