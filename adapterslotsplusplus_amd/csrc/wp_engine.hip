@@ -2524,6 +2524,9 @@ int wp_packed_attention(wp_engine* e, void* out, const int64_t* out_strides, flo
   if (tokens < 0 || keys < 0 || n_seq < 0 || tokens > 0x7FFFFFFF || keys > 0x7FFFFFFF)
     return fail(WP_ERR_INVALID, "%s: bad sizes (tokens %lld, keys %lld, sequences %d)", who, (long long)tokens,
                 (long long)keys, n_seq);
+  if (tokens * (heads / kv_heads) > 0x7FFF0000)
+    return fail(WP_ERR_INVALID, "%s: %lld tokens of %d query heads a key head (up to 2^31 rows)", who, (long long)tokens,
+                heads / kv_heads);
   if (window < 0 || (window > 0 && !causal)) return fail(WP_ERR_INVALID, "%s: a window must be positive, and causal", who);
   if (!out_strides || !q_strides || !k_strides || !v_strides) return fail(WP_ERR_INVALID, "%s: null strides", who);
   if (tokens == 0) return WP_OK;

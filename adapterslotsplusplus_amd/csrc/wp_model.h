@@ -32,7 +32,7 @@ struct ProjArgs {
   // Filled by launch_proj.
   int32_t tiles_t, tiles_n;  // tiles over tokens and over outputs
   int32_t splits, k_range;   // K-ranges of k_range columns (a multiple of 64)
-  int32_t rows_vec;          // y, residual and bias take 8-byte accesses
+  int32_t rows_vec;          // y and residual take 8-byte accesses
   float* part;               // [tile][split] fp32 partial tiles
   uint64_t part_bytes;
   uint32_t* tile_cnt;        // one counter per tile (zero between calls)
@@ -49,11 +49,13 @@ hipError_t launch_proj(int dtype_bf16, ProjArgs& a, int n_cu, hipStream_t stream
 // are 0 and -inf for a query that sees no key and for rows of no sequence.
 // Strides in elements; head rows are contiguous.
 constexpr int kMaxHeadDim = 128;
+
 // Division by a number that the host knows: (n * magic) >> shift.
 struct Divisor {
   uint32_t magic;
   int32_t shift;
 };
+
 struct AttnArgs {
   const void* q;
   const void* k;
