@@ -253,6 +253,24 @@ def test_attention_head_sizes(engine, dim):
     attention_case(engine, [1, 2], [300, 70], 4, 2, dim, torch.float16, seed=dim)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(1, 1, 64), (4, 1, 128)], ids=str)
+@pytest.mark.parametrize("window", [0, 40])
+def test_attention_one_longer_among_single_tokens(engine, heads, kv_heads, dim, window):
+    # One sequence of several 128-row blocks next to many of a row or two.
+    n = 40
+    lens_q = [1 + b % 2 for b in range(n)]
+    lens_k = [3 * b + 2 for b in range(n)]
+    lens_q[7], lens_k[7] = 200, 700
+    attention_case(engine, lens_q, lens_k, heads, kv_heads, dim, torch.bfloat16, window=window)
+
+
+def test_attention_longer_one_among_many_heads(engine):
+    # As above with more partial results than the scratch holds: its keys are not split.
+    lens_q, lens_k = [1] * 100, [b % 13 + 1 for b in range(100)]
+    lens_q[50], lens_k[50] = 40, 700
+    attention_case(engine, lens_q, lens_k, 32, 8, 128, torch.float16)
+
+
 def test_attention_packed_views(engine):
     lens = [60, 1, 90, 130]
     for heads, kv_heads, dim, dtype in ((4, 2, 128, torch.bfloat16), (2, 2, 64, torch.float16), (6, 1, 40, torch.bfloat16)):
