@@ -36,6 +36,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "wp_apply.h"
 #include "wp_device.h"
 #include "wp_model.h"
 
@@ -856,13 +857,15 @@ __device__ __forceinline__ void run_item(const AttnArgs& p, const Item& it, Shar
     float m = w.m;
     for (int i = 1; i < share; ++i) m = fmaxf(m, sh.m[(wave + i * row_waves) & (kWaves - 1)][lane & 31]);
     const float fade = m == -INFINITY ? 1.f : exp2_fast(w.m - m);
+    // (Columns swizzled by the row: whole rows apart, lanes would share banks.)
+    auto place = [](int r, int d) { return (r * (DP / 4) + ((d / 4) ^ (r & (DP == 96 ? 7 : 15)))) * 16; };
     char* o32 = area(wave);
     if (real)
 #pragma unroll
       for (int i = 0; i < H::kCols; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          *reinterpret_cast<f32x4*>(o32 + ((lane & 31) * DP + i * 32 + e * 8 + half * 4) * 4) =
+          *reinterpret_cast<f32x4*>(o32 + place(lane & 31, i * 32 + e * 8 + half * 4)) =
               f32x4{w.o[i][e * 4], w.o[i][e * 4 + 1], w.o[i][e * 4 + 2], w.o[i][e * 4 + 3]} * fade;
     __syncthreads();
     for (int u = tid; u < my_rows * (DP / 4); u += kThreads) {
@@ -873,7 +876,7 @@ __device__ __forceinline__ void run_item(const AttnArgs& p, const Item& it, Shar
 #pragma unroll
       for (int i = 0; i < kWaves; ++i) {
         const int x = w0 + (i < share ? i : 0) * row_waves;
-        const f32x4 o = *reinterpret_cast<const f32x4*>(area(x) + (q * DP + d) * 4);
+        const f32x4 o = *reinterpret_cast<const f32x4*>(area(x) + place(q, d));
         ms[i] = sh.m[x][q];
         ls[i] = i < share ? sh.l[x][q] : 0.f;
         if (i < share) v += o;
@@ -910,7 +913,7 @@ __device__ __forceinline__ void run_item(const AttnArgs& p, const Item& it, Shar
     const int r = u / (DP / 4), d = u % (DP / 4) * 4;
     float top = -INFINITY, l = 0.f;
     f32x4 v{0.f, 0.f, 0.f, 0.f};
-    constexpr int kBatch = 4;
+    constexpr int kBatch = 8;
     for (int i0 = 0; i0 < chunks; i0 += kBatch) {
       f32x2 ml[kBatch];
       f32x4 o[kBatch];
@@ -963,15 +966,18 @@ __global__ __launch_bounds__(64 * kWaves, (kOccupancy<DP, kRoles>)) void attenti
   __shared__ Shared<kWaves> sh;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
 
-  // Read beside the first item's bounds; used once that is found.
-  const int bound0 = p.n_seq > 0 ? p.cu_q[0] : 0, bound1 = p.n_seq > 0 ? p.cu_q[p.n_seq] : 0;
+  touch_kernel_args<static_cast<int>(sizeof(AttnArgs))>();
+  // The outer bounds (lanes 0 and 1): a vector load, on its way together with
+  // the first item's bounds and used once that is found.
+  int outer = 0;
+  if (p.n_seq > 0) outer = p.cu_q[threadIdx.x & 1 ? p.n_seq : 0];
   if constexpr (kRoles == kChunks) {
     __shared__ __align__(1024) char sk[2][Staged<DP>::kBytes];
     __shared__ __align__(1024) char sv[2][Staged<DP>::kBytes];
     // The grid covers the items that there usually are, the loop the most that there can be.
     int id = static_cast<int>(blockIdx.x);
     Item it = find_item(p, false, kRows, id);
-    clear_rest<T, kWaves>(p, bound0, bound1);
+    clear_rest<T, kWaves>(p, __builtin_amdgcn_readlane(outer, 0), __builtin_amdgcn_readlane(outer, 1));
     // Bounds that do not rise could name more row tiles than there are counters.
     while (id < p.chunk_items && it.seq >= 0 && it.counter < p.seq_counters) {
       run_item<T, DP, kWaves, kChunks>(p, it, sh, sk[0], sk[1], sv[0], sv[1], &sk[0][0] + wave * kHalf, &sv[0][0] + wave * kHalf);
@@ -988,7 +994,7 @@ __global__ __launch_bounds__(64 * kWaves, (kOccupancy<DP, kRoles>)) void attenti
     const int block = static_cast<int>(blockIdx.x);
     const bool rows_role = (kRoles & kChunks) == 0 || block < p.tile_items;
     const Item it = find_item(p, rows_role, kRows, rows_role ? block : block - p.tile_items);
-    clear_rest<T, kWaves>(p, bound0, bound1);
+    clear_rest<T, kWaves>(p, __builtin_amdgcn_readlane(outer, 0), __builtin_amdgcn_readlane(outer, 1));
     if (it.seq < 0 || it.counter >= (rows_role ? p.tile_counters : p.seq_counters)) return;
     if (rows_role) {
       run_item<T, DP, kWaves, kTiles>(p, it, sh, sk0, sk1, sv0, sv1, nullptr, nullptr);
