@@ -29,8 +29,8 @@
 // step of 32 rows takes 1024 cycles of products and about 900 of exponentials, sums
 // and roundings).  Decoding over long caches: HBM (64 sequences of up to 8192
 // keys, 8 key heads: 79.5 us, 4.4 TB/s).  Few and short sequences: the chain of
-// latencies from the bounds over K to the join (one token over 777 keys: 11.4 us,
-// of them 2.7 to find the item, 3.5 to the last product, 4 to join).
+// latencies from the bounds over K to the join (one token over 777 keys: 11.3 us,
+// of them 2.2 to find the item, 3.4 to the last product, 4 to join).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -1052,13 +1052,17 @@ hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t s
   const int64_t seqs = std::max(1, a.n_seq);
   // One sequence has one role.  Many of a few rows each (drafted tokens; their
   // mean at most 64 and none of more than 1024 if all have a token) run on key
-  // chunks alone, in a kernel of half the registers.  Others share a launch,
-  // where sequences run on key chunks up to 128 rows, or up to 32 next to longer ones.
+  // chunks alone: a kernel without the row tiles' search and empty workgroups
+  // (32 sequences of up to 40 rows: 21.9 us, 24.1 with both roles).  Others share
+  // a launch, where sequences run on key chunks up to 128 rows, or up to 32 next
+  // to longer ones (32 heads of their own keys: a prompt of 128 rows takes 12.7 us
+  // on key chunks, one of 129 takes 11.0 on a row tile).
   const int64_t longest = (std::max<int64_t>(0, a.tokens - seqs) + 1) * group;
   const bool few = a.n_seq <= 1 ? rows <= kChunkRows : rows <= 64 * seqs && longest <= 1024;
   a.chunk_rows = few ? 0x7FFFFFFF : a.n_seq <= 1 ? 0 : rows >= kChunkRows * seqs ? kWaveRows : kChunkRows;
   const int64_t tile_seqs = few ? 0 : std::min<int64_t>(a.n_seq, rows / (a.chunk_rows + 1));
-  // Row tiles of 256 rows read K and V half as often as those of 128.
+  // Row tiles of 256 rows read K and V half as often as those of 128 (a prompt of
+  // 16384 tokens: 1998 us, 2060 on those), where they leave none idle.
   const int tile_waves = rows / 256 * a.kv_heads >= 2 * n_cu && rows >= 1024 * std::max(1, a.n_seq) ? 8 : 4;
   const int64_t tile_rows = kWaveRows * tile_waves;
   const int64_t tiles = tile_seqs > 0 ? rows / tile_rows + tile_seqs : 0;
