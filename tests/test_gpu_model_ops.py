@@ -444,6 +444,13 @@ def test_attention_refusals(engine):
             bad()
 
 
+def test_attention_refuses_rows_past_31_bits(engine):
+    row = torch.zeros(1, 1, 8, dtype=torch.bfloat16, device="cuda")
+    q = row.expand(65536, 65535, 8)
+    with pytest.raises(RuntimeError, match="2.31 rows"):
+        engine.packed_attention(q, row, row, bounds([4]), bounds([1]), out=q)
+
+
 # ----------------------------------------------------------------- logprobs --
 
 def logprobs_tol(x, top_value):
