@@ -11,11 +11,10 @@
 // chunk (about top elements reach it) and rises when the list is cut down, so
 // nearly every 16-byte vector is dismissed by one comparison of its maximum.
 //
-// What bounds it: 2 to 4 bytes an element from HBM against some ten vector
-// instructions (one of them an exponential at a quarter of the rate), and five
-// more for the alternatives.  4096 rows of 128000, bf16: 210 us without
-// alternatives (5.0 TB/s), 252 with one, 278 with 20, where the vector unit is
-// busy for 85% of the time.
+// What bounds it: 2 to 4 bytes an element from HBM against some eleven vector
+// instructions (one of them an exponential), and six more for the alternatives.
+// 4096 rows of 128000, bf16: 210 to 230 us without alternatives (up to 5.0 TB/s),
+// 250 with 20, where the vector unit is never idle.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -28,11 +27,14 @@ namespace {
 
 constexpr int kRowThreads = 512;
 constexpr int kRowWaves = kRowThreads / 64;
-constexpr int kVecs = 4;            // 16-byte vectors of a chunk per thread
+// Elements of a chunk per thread: 16, of any type.  (4096 rows of 128000, top 20:
+// 16-bit 251 us, with 32 elements 279, whose registers leave two workgroups a
+// compute unit for four; fp32 326 us, with eight 350, for twice the barriers.)
+constexpr int kThreadElements = 16;
 constexpr int kListCap = 4096;      // candidates held; at least kMaxParts * kMaxTop
 // The list is cut down past this many beyond `top`: the threshold then rises
 // with nearly every chunk, and fewer vectors hold a candidate (4096 rows of
-// 128000 logits, top 20: 306 us at 128, 282 at 48, 279 at 16).
+// 128000 logits, top 20, in chunks twice as long: 306 us at 128, 282 at 48, 279 at 16).
 constexpr int kListTrim = 16;
 constexpr int kMaxParts = 64;       // workgroups that share a row
 constexpr int kPartBytes = 16 + 8 * kMaxTop;
@@ -145,6 +147,7 @@ __device__ __forceinline__ int cut_list(Shared& sh, int n, int top, int tid) {
 template <typename T, bool kTop>
 __global__ __launch_bounds__(kRowThreads, 4) void logprobs_kernel(LogprobArgs p) {
   constexpr int kN = Vec<T>::kN;
+  constexpr int kVecs = kThreadElements / kN;
   constexpr int kChunk = kRowThreads * kVecs;  // vectors
   __shared__ Shared sh;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
@@ -419,7 +422,8 @@ hipError_t launch_logprobs(LogprobArgs& a, int n_cu, hipStream_t stream) {
   // Rows enough for four workgroups a compute unit take one each; fewer are
   // shared by workgroups of at least one whole chunk.
   const int64_t n = a.dtype == 2 ? 4 : 8;
-  const int64_t chunks = ((a.vocab + 2 * n - 2) / n + kRowThreads * kVecs - 1) / (kRowThreads * kVecs);
+  const int64_t vecs = kRowThreads * kThreadElements / n;  // of a chunk
+  const int64_t chunks = ((a.vocab + 2 * n - 2) / n + vecs - 1) / vecs;
   a.parts = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>({chunks, (4 * n_cu + a.rows - 1) / a.rows, kMaxParts})));
   if (a.rows > a.n_counters || static_cast<uint64_t>(a.rows) * a.parts * kPartBytes > a.part_bytes) a.parts = 1;
   if (a.rows * a.parts > 0x7FFFFFFF) return hipErrorInvalidValue;
