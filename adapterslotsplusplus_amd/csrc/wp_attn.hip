@@ -750,6 +750,10 @@ __device__ __forceinline__ void run_item(const AttnArgs& p, const Item& it, Shar
   const int base = range.first / unit * unit;        // tiles start at whole ones
   const int chunks = chunks_of(range.end - base, shift);
   if (it.chunk >= chunks) return;
+  // Bounds that fall can name more items than a launch has: a row tile then runs
+  // only if all of its chunks are among them, so that its counter comes back to
+  // zero and the calls after this one join what they should.
+  if (it.slot + static_cast<int64_t>(chunks - 1 - it.chunk) * it.stride >= (kTile ? p.tile_items : p.chunk_items)) return;
   const int first = static_cast<int>(base + (static_cast<int64_t>(it.chunk) << shift));
   const int end = static_cast<int>(std::min<int64_t>(range.end, first + (1ll << shift)));
 

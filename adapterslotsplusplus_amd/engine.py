@@ -802,7 +802,8 @@ class WarpPipeEngine:
         are.  cu_seqlens_q, cu_seqlens_k: int32 [n + 1] bounds on the device;
         sequence b has queries [cu_seqlens_q[b], cu_seqlens_q[b + 1]) and keys
         [cu_seqlens_k[b], cu_seqlens_k[b + 1]) (None: the same bounds), its
-        last query at its last key.  causal: a query sees keys up to its own
+        last query at its last key; bounds must not fall (rows of such a call
+        are unspecified).  causal: a query sees keys up to its own
         position, with window > 0 only the last `window` of them.  scale:
         dim ** -0.5 unless given.  Returns out [tokens, heads, dim], or (out,
         lse [tokens, heads] fp32) with return_lse; queries that see no key, and

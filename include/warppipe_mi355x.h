@@ -366,8 +366,9 @@ int wp_linear(wp_engine* e, void* y, int64_t y_row_stride, const void* x, int64_
 /* Attention over n_seq packed sequences: sequence b has the queries
  * [cu_q[b], cu_q[b + 1]) (rows of q and out) and the keys [cu_k[b], cu_k[b + 1])
  * (rows of k and v); cu_q and cu_k are n_seq + 1 int32 on the device.  A
- * sequence's last query stands at its last key.  causal: a query sees the keys
- * up to its own position, with window > 0 only the last `window` of them;
+ * sequence's last query stands at its last key.  Bounds past the tensors' rows are cut
+ * to them; bounds that fall leave rows of that call unspecified (no later call's).
+ * causal: a query sees the keys up to its own position, with window > 0 only the last `window` of them;
  * else every key of its sequence.  Query head h reads key head
  * h / (heads / kv_heads).  out = softmax(scale * q . k) . v, lse (fp32 [tokens, heads], or NULL)
  * the natural logarithm of the sum of exponentials; queries that see no key, and rows of no sequence,
