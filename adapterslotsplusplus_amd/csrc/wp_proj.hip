@@ -39,7 +39,8 @@ __device__ __forceinline__ float activate(float v) {
       const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, u, 1.f));
       const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f),
                                0.254829592f);
-      const float tail = 0.5f * v * q * __builtin_amdgcn_exp2f(-1.4426950408889634f * u * u);
+      // (Past 64 the tail is zero, and an infinity must not meet it.)
+      const float tail = 0.5f * fminf(v, 64.f) * q * __builtin_amdgcn_exp2f(-1.4426950408889634f * u * u);
       return v < 0.f ? tail : v - tail;
     }
     case kActGeluTanh:
