@@ -32,13 +32,19 @@ __device__ __forceinline__ float activate(float v) {
     case kActRelu:
       return v < 0.f ? 0.f : v;  // NaN stays
     case kActGelu: {
-      // 0.5 v (1 + erf u), u = v / sqrt 2, with erf |u| = 1 - p(t) t exp(-u^2),
-      // t = 1 / (1 + 0.3275911 |u|) (Abramowitz and Stegun 7.1.26, within
-      // 1.5e-7); for negative v the 1 cancels and the tail keeps its precision.
+      // 0.5 v (1 + erf u), u = v / sqrt 2, with 1 - erf |u| = t P(t) exp(-u^2),
+      // t = 1 / (1 + 0.36 |u|): a polynomial fitted here for the least error of
+      // both sides, within 4e-6 of the tail itself up to |u| = 9.3 (fp32 ends
+      // there) and 5e-8 of one.  For negative v the result is the tail, whose
+      // relative error is that and the exponent's rounding (4e-5 at v = -13).
       const float u = fabsf(v) * 0.70710678118654752f;
-      const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, u, 1.f));
-      const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f),
-                               0.254829592f);
+      const float t = __builtin_amdgcn_rcpf(fmaf(0.36f, u, 1.f));
+      float q = fmaf(t, -0.162926913f, 0.561451978f);
+      q = fmaf(t, q, -0.351465345f);
+      q = fmaf(t, q, 0.425491667f);
+      q = fmaf(t, q, 0.108845922f);
+      q = fmaf(t, q, 0.216382673f);
+      q = t * fmaf(t, q, 0.202220065f);
       // (Past 64 the tail is zero, and an infinity must not meet it.)
       const float tail = 0.5f * fminf(v, 64.f) * q * __builtin_amdgcn_exp2f(-1.4426950408889634f * u * u);
       return v < 0.f ? tail : v - tail;

@@ -40,3 +40,24 @@ def test_infinity_and_the_largest_values(engine, act, T, n):
         got, x = through(engine, values, act, dtype, T, n)
         want = mo.activate(x.double(), act).expand(T, n)
         assert torch.equal(got.double().nan_to_num(7e38), want.to(dtype).double().nan_to_num(7e38))
+
+
+@pytest.mark.parametrize("T", [2, 20, 160])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_gelu_in_the_tail(engine, T, dtype):
+    """gelu of every 16-bit value between -13 and 8, within its own size: half
+    a unit of the type, 2^-17 of the polynomial and the hardware's functions,
+    and six roundings (of v / sqrt 2 twice, squared, of the square, of log2 e and
+    its product) of the exponent v^2 / 2."""
+    u, least = (2.0 ** -8, 2.0 ** -126) if dtype == torch.bfloat16 else (2.0 ** -11, 2.0 ** -25)
+    all16 = torch.arange(-(1 << 15), 1 << 15, dtype=torch.int32).to(torch.int16).view(dtype)
+    values = all16[torch.isfinite(all16) & (all16 >= -13) & (all16 <= 8)]
+    announce(f"linear gelu of {len(values)} values T={T} {dtype}")
+    x, w = torch.zeros(T, 8, dtype=dtype), torch.zeros(len(values), 8, dtype=dtype)
+    x[:, 0], w[:, 0] = 1, values
+    got = engine.linear(x.cuda(), w.cuda(), activation="gelu").cpu()
+    assert torch.equal(got, got[:1].expand_as(got))
+    v = values.double()
+    want = 0.5 * v * torch.special.erfc(-v / math.sqrt(2))  # erfc keeps the tail's digits
+    bad = (got[0].double() - want).abs() > want.abs() * (u + 2.0 ** -17 + 6 * 2.0 ** -24 * v.square() / 2) + least
+    assert not bad.any(), f"gelu({v[bad][0].item()}): {got[0][bad][0].item()}, not {want[bad][0].item()}"
