@@ -135,6 +135,12 @@ __device__ __forceinline__ Span span_of(const AttnArgs& p, int b) {
   return s;
 }
 
+// The first key that a query at key position `pos` sees: with the windows the
+// host takes, up to 2^31 - 1, pos - window + 1 need not fit 32 bits.
+__device__ __forceinline__ int window_start(int pos, int window) {
+  return window > 0 ? std::max(0, std::max(0, pos + 1) - window) : 0;
+}
+
 // Keys that rows [row, row + rows) of a sequence see: [first, end).
 struct Range {
   int first, end;
@@ -144,7 +150,7 @@ __device__ __forceinline__ Range keys_of(const AttnArgs& p, int n_q, int n_k, in
   if (!p.causal) return r;
   const int t0 = over(row, p.by_group), t1 = std::min(n_q - 1, over(row + rows - 1, p.by_group));
   r.end = std::clamp(t1 + n_k - n_q + 1, 0, n_k);
-  if (p.window > 0) r.first = std::clamp(t0 + n_k - n_q - p.window + 1, 0, r.end);
+  r.first = std::min(window_start(t0 + n_k - n_q, p.window), r.end);
   return r;
 }
 
@@ -788,7 +794,7 @@ __device__ __forceinline__ void run_item(const AttnArgs& p, const Item& it, Shar
   }
   const int lag = it.n_k - it.n_q;
   w.pos = real ? (p.causal ? std::min(tok + lag, it.n_k - 1) : it.n_k - 1) : -1;
-  w.low = p.causal && p.window > 0 ? std::max(0, tok + lag - p.window + 1) : 0;
+  w.low = p.causal ? window_start(tok + lag, p.window) : 0;
   // wave_low, wave_pos: the keys that all of the wave's rows see; wave_last: the
   // last one that any of them sees.
   int wave_pos = it.n_k - 1, wave_low = 0, wave_last = wave_row0 < n_rows ? it.n_k - 1 : -1;
@@ -796,7 +802,7 @@ __device__ __forceinline__ void run_item(const AttnArgs& p, const Item& it, Shar
     const int t0 = over(wave_row0, p.by_group), t1 = std::min(it.n_q - 1, over(wave_row0 + kWaveRows - 1, p.by_group));
     wave_pos = wave_row0 < n_rows ? t0 + lag : -1;
     wave_last = wave_row0 < n_rows ? t1 + lag : -1;
-    if (p.window > 0) wave_low = std::max(0, t1 + lag - p.window + 1);
+    wave_low = window_start(t1 + lag, p.window);
   }
 
   if constexpr (kTile) {

@@ -65,6 +65,11 @@ def _i64s(v) -> bytes:
     return struct.pack(f"{len(v)}q", *v)
 
 
+def _i32(v) -> int:
+    """v, or the 32-bit number nearest to it (ctypes would take its low bits)."""
+    return max(-0x80000000, min(int(v), 0x7FFFFFFF))
+
+
 def _i32s(v) -> bytes:
     return struct.pack(f"{len(v)}I", *[k & 0xFFFFFFFF for k in v])
 
@@ -843,7 +848,7 @@ class WarpPipeEngine:
             self._handle, out.data_ptr(), _i64s(out.stride()[:2]), None if lse is None else lse.data_ptr(),
             q.data_ptr(), _i64s(qs[:2]), k.data_ptr(), _i64s(ks[:2]), v.data_ptr(), _i64s(vs[:2]),
             cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), n, T, S, heads, kv_heads, dim,
-            dim ** -0.5 if scale is None else float(scale), 1 if causal else 0, int(window or 0), dt, _raw_stream(dev))
+            dim ** -0.5 if scale is None else float(scale), 1 if causal else 0, _i32(window or 0), dt, _raw_stream(dev))
         _lib.check(rc, "packed_attention")
         return out if lse is None else (out, lse)
 

@@ -1,5 +1,5 @@
-"""GPU: packed_attention's bounds: a call whose bounds fall leaves the engine's
-counters as they were, so that the calls after it answer as on a new engine."""
+"""GPU: packed_attention at the ends of its ranges: bounds that fall (the calls
+after such a one answer as on a new engine), windows past 31 bits."""
 import pytest
 import torch
 
@@ -39,3 +39,17 @@ def test_falling_bounds_leave_the_counters_at_zero(cu_q, cu_k, next_q, next_k, h
         engine.packed_attention(q, k, v, ints(cu_q), ints(cu_k))
         for got, t in zip(valid(engine), want):
             assert torch.equal(got, t)
+
+
+@pytest.mark.parametrize("n_q,n_k", [(1000, 500), (5, 900), (300, 300)], ids=str)
+def test_windows_wider_than_the_keys(n_q, n_k):
+    """As no window, up to and past the largest 32-bit number."""
+    engine = WarpPipeEngine()
+    q, k = randn((n_q, 2, 64), 0, torch.bfloat16).cuda(), randn((n_k, 2, 64), 1, torch.bfloat16).cuda()
+    cu_q, cu_k = ints([0, n_q]), ints([0, n_k])
+    want = engine.packed_attention(q, k, k, cu_q, cu_k)
+    for window in (n_k, 2 ** 31 - 1 - n_q, 2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 70):
+        announce(f"attention q={n_q} k={n_k} window={window}")
+        assert torch.equal(engine.packed_attention(q, k, k, cu_q, cu_k, window=window), want), window
+    with pytest.raises(RuntimeError, match="window"):
+        engine.packed_attention(q, k, k, cu_q, cu_k, window=-(2 ** 32))
