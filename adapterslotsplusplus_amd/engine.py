@@ -770,6 +770,8 @@ class WarpPipeEngine:
         n = rows // 2 if gated else rows
         if n < 1:
             raise RuntimeError("linear: weight has no rows")
+        if rows > 0x7FFFFFFF or d_in > 0x7FFFFFFF:
+            raise RuntimeError(f"linear: weight {tuple(weight.shape)} passes 31 bits")
         if d_in > 1 and weight.stride(1) != 1:
             raise RuntimeError("linear: weight must have unit column stride")
         x2 = x if x.dim() == 2 else x.reshape(-1, d_in)
@@ -876,6 +878,8 @@ class WarpPipeEngine:
         top = int(top)
         if top < 0:
             raise RuntimeError("token_logprobs: top must not be negative")
+        if vocab > 0x7FFFFFFF or top > 64:
+            raise RuntimeError(f"token_logprobs: {top} alternatives of a vocabulary of {vocab} (up to 64, and 31 bits)")
         d = logits.device
         got = TokenLogprobs(torch.empty(rows, dtype=torch.float32, device=d),
                             torch.empty(rows, dtype=torch.float32, device=d),
