@@ -2535,11 +2535,23 @@ int wp_packed_attention(wp_engine* e, void* out, const int64_t* out_strides, flo
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || !aligned(lse, 4) ||
       !aligned(cu_q, 4) || !aligned(cu_k, 4))
     return fail(WP_ERR_INVALID, "%s: q, k, v and out must be 16-byte aligned", who);
-  for (int i = 0; i < 2; ++i)
-    for (const int64_t* s : {q_strides, k_strides, v_strides, out_strides})
-      if (s[i] < 0 || s[i] % 8 != 0 || s[i] > (int64_t(1) << 22))
+  // Strides between tokens and heads; one of a dimension of one entry does not matter.
+  const int64_t* given[4] = {q_strides, k_strides, v_strides, out_strides};
+  int64_t strides[4][2];
+  for (int t = 0; t < 4; ++t) {
+    const bool is_kv = t == 1 || t == 2;
+    const int64_t sizes[2] = {is_kv ? keys : tokens, is_kv ? kv_heads : heads};
+    for (int i = 0; i < 2; ++i) {
+      const int64_t s = strides[t][i] = sizes[i] > 1 ? given[t][i] : 0;
+      if (s < 0 || s % 8 != 0)
         return fail(WP_ERR_INVALID, "%s: token and head strides must be multiples of 8 elements (got %lld)", who,
-                    (long long)s[i]);
+                    (long long)s);
+    }
+    // 64 keys are staged by 32-bit byte offsets from the first.
+    if (is_kv && strides[t][0] > kMaxKeyStride)
+      return fail(WP_ERR_INVALID, "%s: keys and values must be at most %lld elements apart (got %lld)", who,
+                  (long long)kMaxKeyStride, (long long)strides[t][0]);
+  }
   AttnArgs a{};
   a.q = q;
   a.k = k;
@@ -2548,14 +2560,14 @@ int wp_packed_attention(wp_engine* e, void* out, const int64_t* out_strides, flo
   a.lse = lse;
   a.cu_q = cu_q;
   a.cu_k = cu_k;
-  a.q_tok = q_strides[0];
-  a.q_head = q_strides[1];
-  a.k_tok = k_strides[0];
-  a.k_head = k_strides[1];
-  a.v_tok = v_strides[0];
-  a.v_head = v_strides[1];
-  a.o_tok = out_strides[0];
-  a.o_head = out_strides[1];
+  a.q_tok = strides[0][0];
+  a.q_head = strides[0][1];
+  a.k_tok = strides[1][0];
+  a.k_head = strides[1][1];
+  a.v_tok = strides[2][0];
+  a.v_head = strides[2][1];
+  a.o_tok = strides[3][0];
+  a.o_head = strides[3][1];
   a.tokens = tokens;
   a.keys = keys;
   a.n_seq = n_seq;

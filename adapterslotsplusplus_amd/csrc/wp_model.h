@@ -49,6 +49,7 @@ hipError_t launch_proj(int dtype_bf16, ProjArgs& a, int n_cu, hipStream_t stream
 // are 0 and -inf for a query that sees no key and for rows of no sequence.
 // Strides in elements; head rows are contiguous.
 constexpr int kMaxHeadDim = 128;
+constexpr int64_t kMaxKeyStride = 1 << 24;  // elements between two keys: 63 of them and a row stay under 2 GiB
 
 // Division by a number that the host knows: (n * magic) >> shift.
 struct Divisor {

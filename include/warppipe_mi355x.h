@@ -372,7 +372,8 @@ int wp_linear(wp_engine* e, void* y, int64_t y_row_stride, const void* x, int64_
  * else every key of its sequence.  Query head h reads key head
  * h / (heads / kv_heads).  out = softmax(scale * q . k) . v, lse (fp32 [tokens, heads], or NULL)
  * the natural logarithm of the sum of exponentials; queries that see no key, and rows of no sequence,
- * get 0 and -inf.  strides[0] between tokens, strides[1] between heads, in elements, multiples of 8;
+ * get 0 and -inf.  strides[0] between tokens, strides[1] between heads, in elements, multiples of 8
+ * (any where there is one token or head; k and v tokens at most 2^24 elements apart);
  * a head's head_dim elements (a multiple of 8, up to 128) are contiguous and 16-byte
  * aligned.  Softmax statistics and sums are fp32; the exponentials are rounded to the
  * tensors' type for the product with v. */

@@ -28,3 +28,57 @@ def test_sizes_past_31_bits_are_refused(engine):
             engine.token_logprobs(x[:1], ids, top=top)
     with pytest.raises(RuntimeError, match="31 bits"):
         engine.token_logprobs(torch.empty(1, far, dtype=torch.float16, device="cuda"), ids)
+
+
+def ints(*v):
+    return torch.tensor(v, dtype=torch.int32).cuda()
+
+
+def test_attention_over_a_head_major_cache(engine):
+    """[kv_heads, keys, dim]: heads lie more than 2^22 elements apart."""
+    n = 40000
+    q = randn((3, 4, 128), 0, torch.bfloat16).cuda()
+    k, v = (randn((2, n, 128), i, torch.bfloat16).cuda().permute(1, 0, 2) for i in (1, 2))
+    announce(f"attention, head strides {q.stride(1)} {k.stride(1)}")
+    got = engine.packed_attention(q, k, v, ints(0, 3), ints(0, n))
+    assert torch.equal(got, engine.packed_attention(q, k.contiguous(), v.contiguous(), ints(0, 3), ints(0, n)))
+    # Queries and outputs head by head too.
+    wide = torch.zeros(4, 40000, 128, dtype=torch.bfloat16, device="cuda").permute(1, 0, 2)
+    wide[:3] = q
+    out = torch.zeros_like(wide)
+    assert out.stride(1) > 1 << 22
+    engine.packed_attention(wide[:3], k, v, ints(0, 3), ints(0, n), out=out[:3])
+    assert torch.equal(out[:3], got) and not out[3:].any()
+
+
+def test_attention_keys_far_apart(engine):
+    """As far as is taken, and the message past that."""
+    far, n = 1 << 24, 70
+    store = torch.zeros(n * (far + 8), dtype=torch.bfloat16, device="cuda")
+    small = randn((n, 2, 1, 64), 0, torch.bfloat16).cuda()
+    q = randn((5, 4, 64), 1, torch.bfloat16).cuda()
+    want = engine.packed_attention(q, small[:, 0], small[:, 1], ints(0, 5), ints(0, n))
+    for heads in (4, 128):  # key chunks, a row tile
+        qh = q[:, :1].expand(5, heads, 64)
+        view = store[:n * far].view(n, far)[:, :128].view(n, 2, 1, 64)
+        view.copy_(small)
+        announce(f"attention, keys {view.stride(0)} apart, {heads} heads")
+        assert torch.equal(engine.packed_attention(qh, view[:, 0], view[:, 1], ints(0, 5), ints(0, n)),
+                           engine.packed_attention(qh, small[:, 0], small[:, 1], ints(0, 5), ints(0, n)))
+    far_q = store[:5 * (far + 8)].view(5, far + 8)[:, :256].view(5, 4, 64)
+    far_q.copy_(q)
+    assert torch.equal(engine.packed_attention(far_q, small[:, 0], small[:, 1], ints(0, 5), ints(0, n)), want)
+    past = store.view(n, far + 8)[:, :64].unsqueeze(1)
+    with pytest.raises(RuntimeError, match="16777216 elements apart"):
+        engine.packed_attention(q, past, past, ints(0, 5), ints(0, n))
+
+
+def test_attention_strides_of_one_entry_do_not_matter(engine):
+    q, k = randn((1, 2, 64), 0, torch.bfloat16).cuda(), randn((9, 1, 64), 1, torch.bfloat16).cuda()
+    want = engine.packed_attention(q, k, k, ints(0, 1), ints(0, 9))
+    announce("attention, strides of size-one dimensions")
+    odd_q, odd_k = q.as_strided(q.shape, (3, 64, 1)), k.as_strided(k.shape, (64, 1 << 40, 1))
+    out = torch.empty_like(q).as_strided(q.shape, (5, 64, 1))
+    assert torch.equal(engine.packed_attention(odd_q, odd_k, odd_k, ints(0, 1), ints(0, 9), out=out), want)
+    one = k[:1].as_strided((1, 1, 64), (1, 1, 1))
+    assert torch.equal(engine.packed_attention(odd_q, one, one, ints(0, 1), ints(0, 1)), k[:1].expand(1, 2, 64))
