@@ -2483,18 +2483,17 @@ int wp_linear(wp_engine* e, void* y, int64_t y_row_stride, const void* x, int64_
   if (y_row_stride < d_out) return fail(WP_ERR_INVALID, "%s: y row stride %lld < d_out", who, (long long)y_row_stride);
   if (w_row_stride < 0 || x_row_stride < 0 || (residual && residual_row_stride < 0))
     return fail(WP_ERR_INVALID, "%s: negative row stride", who);
-  if (w_row_stride > (1 << 22) || x_row_stride > (1 << 22))
-    return fail(WP_ERR_INVALID, "%s: x and weight rows must be at most 4194304 elements apart", who);
   ProjArgs a{};
   a.x = x;
   a.w = w;
   a.bias = bias;
   a.residual = residual;
   a.y = y;
-  a.ldx = x_row_stride;
-  a.ldw = w_row_stride;
-  a.ldr = residual_row_stride;
-  a.ldy = y_row_stride;
+  // (The stride of a single row does not matter.)
+  a.ldx = T > 1 ? x_row_stride : 0;
+  a.ldw = d_out > 1 || gated ? w_row_stride : 0;
+  a.ldr = T > 1 ? residual_row_stride : 0;
+  a.ldy = T > 1 ? y_row_stride : 0;
   a.tokens = T;
   a.d_in = d_in;
   a.n_out = d_out;

@@ -76,6 +76,7 @@ __device__ __forceinline__ u32x4 load_ragged(const T* p, int n) {
 }
 
 constexpr int kRowsPerLoad = 8;       // staged rows that a wave's 16-byte-per-lane load fills
+constexpr int64_t kFarRows = 1 << 27; // elements between rows: seven of them and the columns stay under 2 GiB
 
 // Tile of BT tokens x BN weight rows, WT x WN waves.  A gated tile's weight rows
 // are, per wave, half gate rows and half the up rows of the same outputs, so
@@ -720,7 +721,8 @@ hipError_t launch_proj(int dtype_bf16, ProjArgs& a, int n_cu, hipStream_t stream
     return reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld % (bytes / 2) == 0;
   };
   a.rows_vec = whole(a.y, a.ldy, 8) && whole(a.residual, a.ldr, 8);
-  const bool aligned = a.d_in % 8 == 0 && whole(a.x, a.ldx, 16) && whole(a.w, a.ldw, 16);
+  // Rows further apart than kFarRows take the register path, which has no 32-bit offsets.
+  const bool aligned = a.d_in % 8 == 0 && whole(a.x, a.ldx, 16) && whole(a.w, a.ldw, 16) && a.ldx <= kFarRows && a.ldw <= kFarRows;
   if (dtype_bf16) return aligned ? launch<__bf16, true>(a, n_cu, stream) : launch<__bf16, false>(a, n_cu, stream);
   return aligned ? launch<_Float16, true>(a, n_cu, stream) : launch<_Float16, false>(a, n_cu, stream);
 }

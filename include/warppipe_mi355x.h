@@ -357,8 +357,8 @@ int wp_add_bias(wp_engine* e, void* y, int64_t y_row_stride, int32_t n_slices, c
  * y[t, n] = rn(act(x[t] . w[n] + bias[n]) * (x[t] . w[d_out + n] + bias[d_out + n]) + residual[t, n]),
  * accumulated in fp32 and rounded once.  bias and residual may be NULL; residual
  * may be y.  Any d_in, d_out and row strides in elements (x and w rows with
- * unit column stride; 16-byte aligned rows and d_in a multiple of 8 run the
- * faster loads). */
+ * unit column stride; 16-byte aligned rows at most 2^27 elements apart and d_in
+ * a multiple of 8 run the faster loads). */
 int wp_linear(wp_engine* e, void* y, int64_t y_row_stride, const void* x, int64_t x_row_stride, const void* w,
               int64_t w_row_stride, const void* bias, const void* residual, int64_t residual_row_stride,
               int32_t activation, int32_t gated, int32_t d_in, int32_t d_out, int64_t T, int32_t dtype, void* stream);

@@ -82,3 +82,32 @@ def test_attention_strides_of_one_entry_do_not_matter(engine):
     assert torch.equal(engine.packed_attention(odd_q, odd_k, odd_k, ints(0, 1), ints(0, 9), out=out), want)
     one = k[:1].as_strided((1, 1, 64), (1, 1, 1))
     assert torch.equal(engine.packed_attention(odd_q, one, one, ints(0, 1), ints(0, 1)), k[:1].expand(1, 2, 64))
+
+
+@pytest.mark.parametrize("far", [1 << 23, (1 << 27) + 8], ids=["2^23", "past 2^27"])
+@pytest.mark.parametrize("T,n", [(2, 40), (20, 72), (70, 2048)], ids=str)
+def test_linear_rows_far_apart(engine, far, T, n):
+    """The last position of each of several sequences: [:, -1] of [T, 2048, 4096] lies 2^23 elements apart."""
+    store = torch.empty(T * far, dtype=torch.bfloat16, device="cuda")
+    x, w = randn((T, 136), 0, torch.bfloat16).cuda(), randn((n, 136), 1, torch.bfloat16).cuda()
+    r = randn((T, n), 2, torch.bfloat16).cuda()
+    view = store.view(T, far)[:, -136:] if far % 136 else store.view(T, far)[:, :136]
+    view.copy_(x)
+    res = store.view(T, far)[:, :n]
+    res.copy_(r)
+    announce(f"linear T={T} n={n}, rows {view.stride(0)} apart")
+    want = engine.linear(x, w, residual=r)
+    assert torch.equal(engine.linear(view, w, residual=res), want)
+    assert torch.equal(engine.linear(view, w, residual=res, out=res), want) and torch.equal(view, x)
+    if n < 100 and T * far < 1 << 29:  # weight rows as far
+        far_w = torch.empty(n * far, dtype=torch.bfloat16, device="cuda").view(n, far)[:, :136]
+        far_w.copy_(w)
+        assert torch.equal(engine.linear(view, far_w, residual=r), want)
+
+
+def test_linear_strides_of_one_row_do_not_matter(engine):
+    x, w = randn((1, 64), 0, torch.bfloat16).cuda(), randn((1, 64), 1, torch.bfloat16).cuda()
+    announce("linear, strides of single rows")
+    want = engine.linear(x, w, residual=x[:, :1])
+    far = [t.as_strided(t.shape, (s, 1)) for t, s in ((x, 1 << 40), (w, 3), (x[:, :1], 1 << 50))]
+    assert torch.equal(engine.linear(*far[:2], residual=far[2]), want)
