@@ -70,6 +70,13 @@ class PackedCache:
         self.cu = torch.tensor(ends, dtype=torch.int32, device=device)
         self.lens = [had + more for had, more in zip(self.lens, lens)]
 
+    def state(self):
+        """What restore() goes back to: grow() and add() put new tensors in their places and write none."""
+        return list(self.lens), list(self.k), list(self.v), self.old, self.new, self.cu
+
+    def restore(self, state) -> None:
+        self.lens, self.k, self.v, self.old, self.new, self.cu = state
+
     def add(self, layer: int, k: torch.Tensor, v: torch.Tensor):
         if self.k[layer] is None:  # nothing kept: the new rows are the cache
             self.k[layer], self.v[layer] = k, v
@@ -130,8 +137,15 @@ class TenantDecoder:
         return self.verify(ids, cu_seqlens, tenants, lens, cache, top), cache
 
     def verify(self, ids, cu_seqlens, tenants, lens: Sequence[int], cache: PackedCache, top: int = 0) -> TokenLogprobs:
-        """score() for tokens that follow what the cache holds; it keeps theirs too."""
-        cache.grow(lens, ids.device)
-        after = torch.roll(ids, -1)
-        after[cu_seqlens[1:].long() - 1] = -1  # an empty sequence names its neighbour's last token, which ends too
-        return self.engine.token_logprobs(self.engine.linear(self.hidden(ids, cu_seqlens, tenants, cache), self.head), after, top)
+        """score() for tokens that follow what the cache holds; it keeps theirs
+        too (a step that raises leaves it as it was)."""
+        kept = cache.state()
+        try:
+            cache.grow(lens, ids.device)
+            logits = self.engine.linear(self.hidden(ids, cu_seqlens, tenants, cache), self.head)
+            after = torch.roll(ids, -1)
+            after[cu_seqlens[1:].long() - 1] = -1  # an empty sequence names its neighbour's last token, which ends too
+            return self.engine.token_logprobs(logits, after, top)
+        except BaseException:
+            cache.restore(kept)
+            raise
