@@ -139,13 +139,20 @@ class TenantDecoder:
     def verify(self, ids, cu_seqlens, tenants, lens: Sequence[int], cache: PackedCache, top: int = 0) -> TokenLogprobs:
         """score() for tokens that follow what the cache holds; it keeps theirs
         too (a step that raises leaves it as it was)."""
+        n = ids.numel()
+        if sum(lens) != n or tenants.numel() != n or cu_seqlens.numel() != len(lens) + 1:
+            raise RuntimeError(f"TenantDecoder: {n} tokens, {tenants.numel()} tenants, {cu_seqlens.numel()} bounds and "
+                               f"lengths {list(lens)} do not go together")
+        # The token after each one: none at a sequence's end.  (An empty
+        # sequence names its neighbour's last token, which ends too.)
+        after = torch.roll(ids, -1)
+        if n > 0:
+            after[torch.tensor(lens).cumsum(0).sub(1).to(ids.device)] = -1
         kept = cache.state()
         try:
             cache.grow(lens, ids.device)
-            logits = self.engine.linear(self.hidden(ids, cu_seqlens, tenants, cache), self.head)
-            after = torch.roll(ids, -1)
-            after[cu_seqlens[1:].long() - 1] = -1  # an empty sequence names its neighbour's last token, which ends too
-            return self.engine.token_logprobs(logits, after, top)
+            hidden = self.hidden(ids, cu_seqlens, tenants, cache) if n > 0 else self.embed[:0]
+            return self.engine.token_logprobs(self.engine.linear(hidden, self.head), after, top)
         except BaseException:
             cache.restore(kept)
             raise

@@ -93,3 +93,24 @@ def test_a_batch_of_another_size_leaves_the_cache():
     with pytest.raises(RuntimeError, match="1 sequences"):
         step(model, parts(2, 1), cache)
     assert cache.lens == [3, 2] and all(len(t) == 5 for t in cache.k + cache.v)
+
+
+def test_steps_of_no_tokens():
+    """On a new cache and between steps that have some; they change nothing."""
+    model = decoder(HostEngine())
+    got, cache = step(model, parts(0, 0, 0))
+    assert got.logprobs.shape == (0,) and cache.lens == [0, 0]
+    first, more = parts(1, 0, 4), parts(2, 2, 3)
+    step(model, first, cache)
+    assert step(model, parts(0, 0, 0), cache).logprobs.shape == (0,)
+    got = step(model, more, cache)
+    want = step(model, more, step(model, first)[1])
+    assert torch.equal(got.logprobs, want.logprobs) and cache.lens == [2, 7]
+
+
+def test_lengths_must_cover_the_tokens():
+    model = decoder(HostEngine())
+    ids, cu, who = torch.arange(5), torch.tensor([0, 2, 5], dtype=torch.int32), torch.zeros(5, dtype=torch.int64)
+    for bad in ((ids, cu, who, [2, 4]), (ids, cu, who, [5]), (ids, cu, who[:4], [2, 3]), (ids[:4], cu, who[:4], [2, 3])):
+        with pytest.raises(RuntimeError, match="do not go together"):
+            model.score(*bad)
