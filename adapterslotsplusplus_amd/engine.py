@@ -27,6 +27,7 @@ Additions (each a superset of the reference behaviour):
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 from typing import List, NamedTuple, Optional, Sequence, Tuple
 
@@ -774,7 +775,7 @@ class WarpPipeEngine:
             raise RuntimeError(f"linear: weight {tuple(weight.shape)} passes 31 bits")
         if d_in > 1 and weight.stride(1) != 1:
             raise RuntimeError("linear: weight must have unit column stride")
-        x2 = x if x.dim() == 2 else x.reshape(-1, d_in)
+        x2 = x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), d_in)
         if d_in > 1 and x2.stride(1) != 1:
             x2 = x2.contiguous()
         T = x2.size(0)

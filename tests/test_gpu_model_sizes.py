@@ -111,3 +111,11 @@ def test_linear_strides_of_one_row_do_not_matter(engine):
     want = engine.linear(x, w, residual=x[:, :1])
     far = [t.as_strided(t.shape, (s, 1)) for t, s in ((x, 1 << 40), (w, 3), (x[:, :1], 1 << 50))]
     assert torch.equal(engine.linear(*far[:2], residual=far[2]), want)
+
+
+@pytest.mark.parametrize("shape", [(0,), (2, 3, 0), (2, 0, 0), (1, 1, 1, 0)], ids=str)
+def test_linear_of_no_columns_in_any_shape(engine, shape):
+    announce(f"linear of {shape}")
+    x, w = torch.zeros(shape, dtype=torch.float16, device="cuda"), torch.zeros(12, 0, dtype=torch.float16, device="cuda")
+    b = randn((12,), 0, torch.float16).cuda()
+    assert torch.equal(engine.linear(x, w, bias=b), b.expand(*shape[:-1], 12))
