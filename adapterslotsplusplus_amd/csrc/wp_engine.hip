@@ -241,7 +241,7 @@ struct wp_engine {
   uint32_t* lin_cnt = nullptr;  // [kLinCounters] column-tile counters of linear_lora (zero between calls)
   uint32_t* lin_flag = nullptr; // [2][block_cap] H flags and their reader counts (zero between calls)
   uint32_t* model_cnt = nullptr;  // [kModelCounters] tile counters of linear / packed_attention / token_logprobs (zero between calls)
-  float* mpart = nullptr;       // [kModelPartBytes] their fp32 partials (no invariant)
+  float* mpart = nullptr;       // [kModelPartBytes] their fp32 partials (no invariant), allocated by their first call
   Entry* dtable = nullptr;      // [table_cap] id-indexed adapter table of build_seg_bounds plans
   Entry* bentries = nullptr;    // [block_cap] a build_seg_bounds plan's copy of each block's table entry
   // The second table of build_seg_bounds plans over more than kSmallPlanTokens
@@ -803,7 +803,6 @@ int wp_create(const wp_config* cfg_in, wp_engine** out) {
   const size_t o_spart = carve(sizeof(float) * kMaxChunks * static_cast<size_t>(e->tok_cap) * kMaxRank);
   const size_t hbuf_bytes = sizeof(uint16_t) * static_cast<size_t>(e->tok_cap) * kMaxSlices * kMaxRank;
   const size_t o_hbuf = carve(hbuf_bytes);
-  const size_t o_mpart = carve(kModelPartBytes);
   if (hipMalloc(reinterpret_cast<void**>(&e->ws), off) != hipSuccess)
     return bail(fail(WP_ERR_HIP, "wp_create: workspace allocation (%zu bytes) failed", off));
   e->header = reinterpret_cast<uint32_t*>(e->ws + o_hdr);
@@ -818,7 +817,6 @@ int wp_create(const wp_config* cfg_in, wp_engine** out) {
   e->lin_cnt = reinterpret_cast<uint32_t*>(e->ws + o_lin);
   e->lin_flag = e->lin_cnt + kLinCounters;
   e->model_cnt = reinterpret_cast<uint32_t*>(e->ws + o_mcnt);
-  e->mpart = reinterpret_cast<float*>(e->ws + o_mpart);
   e->dtable = reinterpret_cast<Entry*>(e->ws + o_tab);
   e->bentries = reinterpret_cast<Entry*>(e->ws + o_bent);
   e->fblocks = reinterpret_cast<Block*>(e->ws + o_fblk);
@@ -829,8 +827,7 @@ int wp_create(const wp_config* cfg_in, wp_engine** out) {
   e->part = reinterpret_cast<float*>(e->ws + o_part);
   // Everything before the partials starts at zero, the partials at
   // kPartialEmpty, the publications' ids at -1 (nothing published); the d-range
-  // partials of shrink(), the H rows behind them and the partials of the
-  // operators around the apply need no state.  Filled by
+  // partials of shrink() and the H rows behind them need no state.  Filled by
   // kernels, then waited for.
   if (launch_fill_u32(reinterpret_cast<uint32_t*>(e->ws), 0u, o_part / 4, nullptr) != hipSuccess ||
       launch_fill_u32(reinterpret_cast<uint32_t*>(e->part), kPartialEmpty, e->part_words, nullptr) != hipSuccess)
@@ -904,6 +901,7 @@ int wp_destroy(wp_engine* e) {
     if (s.ready) (void)hipEventDestroy(s.ready);
   }
   if (e->ws) (void)hipFree(e->ws);
+  if (e->mpart) (void)hipFree(e->mpart);
   for (int i = 0; i < kUploadRing; ++i) {
     if (e->pinned[i]) (void)hipHostFree(e->pinned[i]);
     if (e->upload_done[i]) (void)hipEventDestroy(e->upload_done[i]);
@@ -2465,6 +2463,28 @@ int wp_set_spin_limit(wp_engine* e, uint32_t polls) {
 // caller as everywhere else.
 // ============================================================================
 
+namespace {
+
+// Their scratch, allocated by the first call: an engine that runs none of them
+// keeps no memory for them.  A capture may make that call (memory is allocated
+// beside it, not by the graph).
+int model_scratch(wp_engine* e, const char* who) {
+  if (e->mpart != nullptr) return WP_OK;
+  hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+  WP_HIP(hipThreadExchangeStreamCaptureMode(&mode));
+  void* p = nullptr;
+  const hipError_t rc = hipMalloc(&p, kModelPartBytes);
+  (void)hipThreadExchangeStreamCaptureMode(&mode);
+  if (rc != hipSuccess) {
+    (void)hipGetLastError();
+    return fail(WP_ERR_HIP, "%s: scratch allocation (%llu bytes) failed", who, (unsigned long long)kModelPartBytes);
+  }
+  e->mpart = static_cast<float*>(p);
+  return WP_OK;
+}
+
+}  // namespace
+
 extern "C" {
 
 int wp_linear(wp_engine* e, void* y, int64_t y_row_stride, const void* x, int64_t x_row_stride, const void* w,
@@ -2483,6 +2503,8 @@ int wp_linear(wp_engine* e, void* y, int64_t y_row_stride, const void* x, int64_
   if (y_row_stride < d_out) return fail(WP_ERR_INVALID, "%s: y row stride %lld < d_out", who, (long long)y_row_stride);
   if (w_row_stride < 0 || x_row_stride < 0 || (residual && residual_row_stride < 0))
     return fail(WP_ERR_INVALID, "%s: negative row stride", who);
+  DeviceGuard g(e->device);
+  if (const int rc = model_scratch(e, who); rc != WP_OK) return rc;
   ProjArgs a{};
   a.x = x;
   a.w = w;
@@ -2503,7 +2525,6 @@ int wp_linear(wp_engine* e, void* y, int64_t y_row_stride, const void* x, int64_
   a.part_bytes = kModelPartBytes;
   a.tile_cnt = e->model_cnt;
   a.n_cnt = kModelCounters;
-  DeviceGuard g(e->device);
   WP_HIP(launch_proj(dtype == WP_DTYPE_BF16, a, e->n_cu, static_cast<hipStream_t>(stream)));
   return WP_OK;
 }
@@ -2551,6 +2572,8 @@ int wp_packed_attention(wp_engine* e, void* out, const int64_t* out_strides, flo
       return fail(WP_ERR_INVALID, "%s: keys and values must be at most %lld elements apart (got %lld)", who,
                   (long long)kMaxKeyStride, (long long)strides[t][0]);
   }
+  DeviceGuard g(e->device);
+  if (const int rc = model_scratch(e, who); rc != WP_OK) return rc;
   AttnArgs a{};
   a.q = q;
   a.k = k;
@@ -2580,7 +2603,6 @@ int wp_packed_attention(wp_engine* e, void* out, const int64_t* out_strides, flo
   a.part_bytes = kModelPartBytes;
   a.counters = e->model_cnt;
   a.n_counters = kModelCounters;
-  DeviceGuard g(e->device);
   WP_HIP(launch_attention(dtype == WP_DTYPE_BF16, a, e->n_cu, static_cast<hipStream_t>(stream)));
   return WP_OK;
 }
@@ -2604,6 +2626,8 @@ int wp_token_logprobs(wp_engine* e, float* logprobs, float* entropy, int32_t* ra
       !aligned(logprobs, 4) || !aligned(entropy, 4) || !aligned(ranks, 4) || !aligned(top_logprobs, 4) ||
       !aligned(top_ids, 4))
     return fail(WP_ERR_INVALID, "%s: tensors must be aligned to their elements", who);
+  DeviceGuard g(e->device);
+  if (const int rc = model_scratch(e, who); rc != WP_OK) return rc;
   LogprobArgs a{};
   a.logits = logits;
   a.ids = token_ids;
@@ -2623,7 +2647,6 @@ int wp_token_logprobs(wp_engine* e, float* logprobs, float* entropy, int32_t* ra
   a.part_bytes = kModelPartBytes;
   a.counters = e->model_cnt;
   a.n_counters = kModelCounters;
-  DeviceGuard g(e->device);
   WP_HIP(launch_logprobs(a, e->n_cu, static_cast<hipStream_t>(stream)));
   return WP_OK;
 }

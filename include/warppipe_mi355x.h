@@ -349,8 +349,8 @@ int wp_add_bias(wp_engine* e, void* y, int64_t y_row_stride, int32_t n_slices, c
 /* ---- operators around the apply ------------------------------------------
  * What a model computes between its LoRA deltas (no reference counterpart).  They
  * use no segment table; scratch is the engine's, so the one-call-at-a-time
- * rule of an engine holds for them too.  They allocate nothing, and can be
- * captured. */
+ * rule of an engine holds for them too.  It is allocated by the first of their
+ * calls (256 MiB), which may be a captured one; the others allocate nothing. */
 
 /* y[t, n] = rn(act(x[t] . w[n] + bias[n]) + residual[t, n]) for n < d_out, or, gated (w has
  * 2 * d_out rows, bias as many elements),
