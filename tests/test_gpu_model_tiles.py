@@ -1,0 +1,183 @@
+"""GPU: sizes that reach the kernels which the sizes of test_gpu_model_ops.py do
+not: linear's tiles on rows that are not whole 16-byte vectors, its largest
+tiles in each type and gated, attention's row tiles of 256 rows.  Against 64
+bits on the device, with that file's tolerances."""
+import math
+
+import pytest
+import torch
+
+from adapterslotsplusplus_amd import WarpPipeEngine
+from oracle import model_ops as mo
+from tests.helpers import announce, randn
+from tests.test_gpu_model_ops import attention_tol, bounds, check, linear_tol, logprobs_tol
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+
+
+@pytest.fixture(scope="module")
+def engine():
+    return WarpPipeEngine()
+
+
+# ------------------------------------------------------------------- linear --
+
+def linear_case(engine, T, d_in, n, dtype, act="none", gated=False, bias=False, residual=False, shift=0, pad=0):
+    """shift: elements before x's and the weight's first; pad: between their rows."""
+    announce(f"linear T={T} d_in={d_in} n={n} {dtype} {act} gated={gated} bias={bias} residual={residual} shift={shift} pad={pad}")
+    rows = 2 * n if gated else n
+
+    def place(t):
+        buf = torch.full((t.size(0) * (d_in + pad) + 16,), float("nan"), dtype=dtype, device="cuda")
+        view = buf[shift:shift + t.size(0) * (d_in + pad)].view(t.size(0), d_in + pad)[:, :d_in]
+        view.copy_(t)
+        return view
+
+    x, w = place(randn((T, d_in), T, dtype)), place(randn((rows, d_in), n, dtype, d_in ** -0.5))
+    b = randn((rows,), 2, dtype).cuda() if bias else None
+    r = randn((T, n), 3, dtype).cuda() if residual else None
+    want, size = mo.linear(x, w, b, r, act, gated)
+    tol = linear_tol(want, size, d_in, dtype)
+    got = engine.linear(x, w, bias=b, residual=r, activation=act, gated=gated)
+    check(got, want.cpu(), tol.cpu(), "linear")
+
+
+# d_in odd, even and a multiple of 4; less than a K-step, whole ones, one column past them.
+@DTYPES
+@pytest.mark.parametrize("T,d_in,n", [(700, 1001, 1101), (300, 1028, 1000), (65, 4097, 2100), (257, 62, 900), (700, 129, 1200)], ids=str)
+def test_rows_of_no_whole_vectors_on_small_tiles(engine, T, d_in, n, dtype):
+    linear_case(engine, T, d_in, n, dtype, "silu", bias=True, residual=True)
+    linear_case(engine, T, d_in, (n + 1) // 2, dtype, "gelu", gated=True, residual=True)
+
+
+@DTYPES
+@pytest.mark.parametrize("T,d_in,n", [(1500, 257, 1500), (1537, 1001, 1411), (1900, 63, 1900), (1500, 3, 1500), (2500, 650, 2500)], ids=str)
+def test_rows_of_no_whole_vectors_on_large_tiles(engine, T, d_in, n, dtype):
+    linear_case(engine, T, d_in, n, dtype, "gelu_tanh", bias=True, residual=True)
+    linear_case(engine, T, d_in, (n + 1) // 2, dtype, "silu", gated=True, bias=True)
+
+
+@DTYPES
+@pytest.mark.parametrize("shift,pad", [(1, 0), (0, 1), (4, 4), (3, 7), (8, 8)], ids=str)
+def test_rows_that_start_anywhere(engine, shift, pad, dtype):
+    """Whole vectors of columns, rows that start between them; NaN around."""
+    for T, d_in, n in ((1000, 520, 700), (1500, 2056, 1600), (90, 264, 4000)):
+        linear_case(engine, T, d_in, n, dtype, shift=shift, pad=pad)
+
+
+# Columns: a multiple of the K-step, of 8 only, less than one step, one step, of eight.
+@DTYPES
+@pytest.mark.parametrize("T,d_in,n", [(4100, 576, 2304), (4133, 584, 2311), (4100, 72, 2304), (4100, 64, 2310), (4100, 8, 2304), (4100, 1096, 2304)],
+                         ids=str)
+def test_largest_tiles(engine, T, d_in, n, dtype):
+    linear_case(engine, T, d_in, n, dtype, "gelu", bias=True, residual=True)
+    linear_case(engine, T, d_in, (n + 1) // 2, dtype, "silu", gated=True, bias=True, residual=True)
+
+
+@pytest.mark.parametrize("T,d_in,n", [(700, 1001, 1101), (1500, 257, 1500), (4100, 576, 2304)], ids=str)
+def test_linear_tiles_repeat_bit_for_bit(engine, T, d_in, n):
+    x, w = randn((T, d_in), 0, torch.bfloat16).cuda(), randn((n, d_in), 1, torch.bfloat16).cuda()
+    first = engine.linear(x, w)
+    for _ in range(5):
+        assert torch.equal(engine.linear(x, w), first)
+
+
+# ---------------------------------------------------------------- attention --
+# 256-row tiles: at least 512 of them over the key heads, sequences of 1024 rows on average.
+
+def attention_case(engine, lens_q, lens_k, heads, kv_heads, dim, dtype, causal=True, window=0):
+    announce(f"attention q={lens_q} k={lens_k} {heads}/{kv_heads}x{dim} {dtype} causal={causal} window={window}")
+    q = randn((sum(lens_q), heads, dim), 0, dtype).cuda()
+    k, v = (randn((sum(lens_k), kv_heads, dim), i, dtype).cuda() for i in (1, 2))
+    got, got_lse = engine.packed_attention(q, k, v, bounds(lens_q), bounds(lens_k), causal=causal, window=window, return_lse=True)
+    a = b = 0
+    for n_q, n_k in zip(lens_q, lens_k):
+        pos = torch.arange(n_q, device="cuda")[:, None] + n_k - n_q
+        at = torch.arange(n_k, device="cuda")[None]
+        hide = at > pos if causal else torch.zeros(n_q, n_k, dtype=torch.bool, device="cuda")
+        if window:
+            hide |= at <= pos - window
+        for h in range(heads):
+            qh = q[a:a + n_q, h].double()
+            kh, vh = (t[b:b + n_k, h * kv_heads // heads].double() for t in (k, v))
+            s = (qh @ kh.t().contiguous()) * dim ** -0.5
+            s = s.masked_fill(hide, -math.inf)
+            p, lse = torch.softmax(s, 1).nan_to_num(0.0), torch.logsumexp(s, 1)  # rows that see nothing: 0
+            reach = (qh.abs() @ kh.abs().t().contiguous()).amax(1) * dim ** -0.5
+            tol, lse_tol = attention_tol(p @ vh, lse, p @ vh.abs(), reach, dim, [n_k], float(vh.abs().max()), dtype)
+            check(got[a:a + n_q, h], (p @ vh).cpu(), tol.cpu(), f"out of head {h}")
+            check(got_lse[a:a + n_q, h], lse.cpu(), lse_tol.cpu(), f"lse of head {h}")
+        a, b = a + n_q, b + n_k
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(64, 64, 128, torch.bfloat16), (64, 64, 64, torch.float16), (64, 64, 96, torch.bfloat16),
+                                                      (48, 16, 128, torch.float16), (64, 64, 40, torch.bfloat16)], ids=str)
+def test_long_prompts_of_many_heads(engine, heads, kv_heads, dim, dtype):
+    n = 2100 if heads == kv_heads else 2800
+    attention_case(engine, [n], [n], heads, kv_heads, dim, dtype)
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, torch.float16), (64, torch.bfloat16)], ids=str)
+def test_long_prompts_windows_and_no_mask(engine, dim, dtype):
+    for window in (1, 100, 700):
+        attention_case(engine, [2100], [2100], 64, 64, dim, dtype, window=window)
+    attention_case(engine, [2100], [2100], 64, 64, dim, dtype, causal=False)
+    attention_case(engine, [2100], [900], 64, 64, dim, dtype, causal=False)
+    attention_case(engine, [2100], [900], 64, 64, dim, dtype)  # rows that see nothing
+    attention_case(engine, [2100], [4000], 64, 64, dim, dtype, window=1000)
+
+
+@pytest.mark.parametrize("lens_q,lens_k", [([2090, 10], [2090, 10]), ([10, 1, 3000, 1100], [900, 70, 3000, 2000])], ids=str)
+def test_long_prompts_beside_short_sequences(engine, lens_q, lens_k):
+    attention_case(engine, lens_q, lens_k, 64, 64, 128, torch.bfloat16)
+    attention_case(engine, lens_q, lens_k, 64, 64, 64, torch.float16, window=50)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_prompts_unseen_keys_do_not_matter(engine, dim):
+    """NaN and infinity in keys and values: rows that do not see them stay bit for bit."""
+    T, heads = 2100, 64
+    q, k, v = (randn((T, heads, dim), i, torch.bfloat16).cuda() for i in range(3))
+    cu = bounds([T])
+    for window in (0, 300):
+        clean = engine.packed_attention(q, k, v, cu, window=window)
+        for at in (0, 1023, 1200, 2099):
+            announce(f"attention, odd values at key {at}, window {window}, {dim} columns")
+            seen = torch.zeros(T, dtype=torch.bool)
+            seen[at:at + window if window else T] = True
+            for value in (math.nan, math.inf, -math.inf):
+                v2 = v.clone()
+                v2[at] = value
+                got = engine.packed_attention(q, k, v2, cu, window=window)
+                assert torch.equal(got[~seen], clean[~seen]) and not torch.isfinite(got[seen]).any()
+            k2 = k.clone()
+            k2[at] = math.nan
+            got = engine.packed_attention(q, k2, v, cu, window=window)
+            assert torch.equal(got[~seen], clean[~seen]) and torch.isnan(got[seen]).all()
+
+
+def test_long_prompts_repeat_bit_for_bit(engine):
+    q, k, v = (randn((2100, 64, 128), i, torch.bfloat16).cuda() for i in range(3))
+    first = engine.packed_attention(q, k, v, bounds([2090, 10]))
+    for _ in range(5):
+        assert torch.equal(engine.packed_attention(q, k, v, bounds([2090, 10])), first)
+
+
+# ----------------------------------------------------------------- logprobs --
+
+@pytest.mark.parametrize("vocab", [1000, 30000, 128000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+def test_rows_of_the_lowest_value(engine, vocab, dtype):
+    """Every logit the type's lowest: the uniform distribution; one above them: that one."""
+    announce(f"logprobs of the lowest values, vocab {vocab} {dtype}")
+    x = torch.full((3, vocab), torch.finfo(dtype).min, dtype=dtype, device="cuda")
+    x[1, 7], x[2, vocab - 1] = 0.0, torch.finfo(dtype).max
+    got = engine.token_logprobs(x, torch.tensor([3, 7, vocab - 1]).cuda(), top=4)
+    tol = logprobs_tol(x, 0.0)
+    assert abs(float(got.logprobs[0]) + math.log(vocab)) <= tol + 2.0 ** -23 * math.log(vocab)
+    assert abs(float(got.entropy[0]) - math.log(vocab)) <= tol * (2 + math.log(vocab))
+    assert got.top_ids.tolist() == [[0, 1, 2, 3], [7, 0, 1, 2], [vocab - 1, 0, 1, 2]] and got.ranks.tolist() == [1, 1, 1]
+    assert got.logprobs[1:].tolist() == [0, 0] and got.entropy[1:].tolist() == [0, 0]
+    assert (got.top_logprobs[0] - got.logprobs[0]).abs().max() == 0 and got.top_logprobs[1:, 0].tolist() == [0, 0]
