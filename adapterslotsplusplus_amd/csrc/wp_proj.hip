@@ -59,14 +59,46 @@ __device__ __forceinline__ float activate(float v) {
   }
 }
 
-// 16 bytes of a row that need not be 16-byte aligned, `n` elements of it
-// inside the row (n <= 0: none); the rest are zero.
+// How a product's rows lie: each is whole 16-byte vectors, starts on a 4-byte
+// word, or on any element.
+enum RowKind { kVectors, kWords, kElements };
+
+// 16 bytes from any element on.
 template <typename T>
-__device__ __forceinline__ u32x4 load_ragged(const T* p, int n) {
+__device__ __forceinline__ u32x4 load_any(const T* p) {
   struct __attribute__((packed, aligned(2))) Loose {
     u32x4 v;
   };
-  if (n >= 8) return reinterpret_cast<const Loose*>(p)->v;
+  return reinterpret_cast<const Loose*>(p)->v;
+}
+// The same as the words that hold them.  Where a wave's neighbouring lanes read
+// different rows, the memory pipeline takes some four cycles a lane for 16
+// bytes that start inside a word (128 x 8191 -> 1000: 59 us, and as words 32).
+struct Words {
+  u32x4 v;
+  uint32_t next;  // the word after them, if the first starts before p
+};
+template <typename T>
+__device__ __forceinline__ uint32_t inside_word(const T* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 2);
+}
+template <typename T>
+__device__ __forceinline__ Words load_words(const T* p) {
+  struct __attribute__((packed, aligned(4))) Loose {
+    u32x4 v;
+  };
+  const uint32_t* q = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(3));
+  return Words{reinterpret_cast<const Loose*>(q)->v, q[3 + inside_word(p) / 2]};
+}
+__device__ __forceinline__ u32x4 settle(const Words& w, uint32_t inside) {
+  const uint32_t w0 = w.v[0], w1 = w.v[1], w2 = w.v[2], w3 = w.v[3];
+  return u32x4{__builtin_amdgcn_alignbyte(w1, w0, inside), __builtin_amdgcn_alignbyte(w2, w1, inside),
+               __builtin_amdgcn_alignbyte(w3, w2, inside), __builtin_amdgcn_alignbyte(w.next, w3, inside)};
+}
+// The first `n` elements from p on, 8 at most (n <= 0: none); the rest are zero.
+template <typename T>
+__device__ __forceinline__ u32x4 load_first(const T* p, int n) {
+  if (n >= 8) return load_any(p);
   u32x4 r{0u, 0u, 0u, 0u};
   const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
@@ -409,37 +441,80 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void proj_kernel(ProjArgs p) {
       }
     }
   } else {
-    u32x4 rx[C::kLoadsX], rw[C::kLoadsW];
-    auto gather = [&](int k) {
+    // Rows of any alignment: whole K-steps go through registers, kAhead of them
+    // on their way, to two slots in turn; the columns left then to a third.
+    // (100 x 8191 -> 8000, one step ahead: 112 us, four: 55.)
+    constexpr int kAhead = 4;
+    static_assert(R == 4, "three slots");
+    // Rows past the last read another one: their sums are written nowhere.
+    const T* src_x[C::kLoadsX];
+    const T* src_w[C::kLoadsW];
+    int col_x[C::kLoadsX], col_w[C::kLoadsW];
+    auto column = [&](int r) { return ((lane & 7) ^ ((r >> 1) & 7)) * 8; };
 #pragma unroll
-      for (int i = 0; i < C::kLoadsX; ++i) {
-        const int r = (wave * C::kLoadsX + i) * kRowsPerLoad + sub, c = (lane & 7) ^ ((r >> 1) & 7);
-        const int64_t t = t0 + r;
-        rx[i] = load_ragged(static_cast<const T*>(p.x) + t * p.ldx + k + c * 8, t < p.tokens ? k_end - k - c * 8 : 0);
-      }
+    for (int i = 0; i < C::kLoadsX; ++i) {
+      const int r = (wave * C::kLoadsX + i) * kRowsPerLoad + sub;
+      col_x[i] = column(r);
+      src_x[i] = static_cast<const T*>(p.x) + (t0 + r < p.tokens ? t0 + r : t0) * p.ldx + col_x[i];
+    }
 #pragma unroll
-      for (int i = 0; i < C::kLoadsW; ++i) {
-        const int r = (wave * C::kLoadsW + i) * kRowsPerLoad + sub, c = (lane & 7) ^ ((r >> 1) & 7);
-        bool ok;
-        const int64_t row = weight_row<C::kN>(p, n0, r, &ok);
-        rw[i] = load_ragged(static_cast<const T*>(p.w) + row * p.ldw + k + c * 8, ok ? k_end - k - c * 8 : 0);
-      }
+    for (int i = 0; i < C::kLoadsW; ++i) {
+      const int r = (wave * C::kLoadsW + i) * kRowsPerLoad + sub;
+      bool ok;
+      const int64_t row = weight_row<C::kN>(p, n0, r, &ok);
+      col_w[i] = column(r);
+      src_w[i] = static_cast<const T*>(p.w) + (ok ? row : 0) * p.ldw + col_w[i];
+    }
+    u32x4 rx[kAhead][C::kLoadsX], rw[kAhead][C::kLoadsW];
+    auto place = [&](char* rows, int load, const u32x4& v) {
+      *reinterpret_cast<u32x4*>(rows + load * 1024 + lane * 16) = v;
     };
-    gather(0);
-    for (int k = 0; k < k_end; k += kStepK) {
-      __syncthreads();
+    auto products = [&](const Slot& slot) {
+      read(slot, 0, aw, ax);
+      read(slot, 1, bw, bx);
+      multiply(aw, ax);
+      multiply(bw, bx);
+    };
+    const int full = k_end / kStepK * kStepK;
+    auto gather = [&](int b, int k) {  // past the last whole step: that one again
+      k = std::min(k, full - kStepK);
+#pragma unroll
+      for (int i = 0; i < C::kLoadsX; ++i) rx[b][i] = load_any(src_x[i] + k);
+#pragma unroll
+      for (int i = 0; i < C::kLoadsW; ++i) rw[b][i] = load_any(src_w[i] + k);
+    };
+    if (full > 0) {
+#pragma unroll
+      for (int b = 0; b < kAhead; ++b) gather(b, b * kStepK);
+      auto step = [&](int k, int b) {
+        const Slot& slot = b & 1 ? slot1 : slot0;
+#pragma unroll
+        for (int i = 0; i < C::kLoadsX; ++i) place(slot.x, wave * C::kLoadsX + i, rx[b][i]);
+#pragma unroll
+        for (int i = 0; i < C::kLoadsW; ++i) place(slot.w, wave * C::kLoadsW + i, rw[b][i]);
+        staged_barrier<63>();
+        gather(b, k + kAhead * kStepK);
+        products(slot);
+      };
+      // Whole rounds, then the steps left (as above).
+      const int round_end = full / (kAhead * kStepK) * (kAhead * kStepK);
+      int k = 0;
+      for (; k < round_end; k += kAhead * kStepK)
+#pragma unroll
+        for (int b = 0; b < kAhead; ++b) step(k + b * kStepK, b);
+      if (k < full) step(k, 0);
+      if (k + kStepK < full) step(k + kStepK, 1);
+      if (k + 2 * kStepK < full) step(k + 2 * kStepK, 2);
+    }
+    if (full < k_end) {
 #pragma unroll
       for (int i = 0; i < C::kLoadsX; ++i)
-        *reinterpret_cast<u32x4*>(slot0.x + (wave * C::kLoadsX + i) * 1024 + lane * 16) = rx[i];
+        place(slot2.x, wave * C::kLoadsX + i, load_first(src_x[i] + full, k_end - full - col_x[i]));
 #pragma unroll
       for (int i = 0; i < C::kLoadsW; ++i)
-        *reinterpret_cast<u32x4*>(slot0.w + (wave * C::kLoadsW + i) * 1024 + lane * 16) = rw[i];
-      __syncthreads();
-      gather(k + kStepK);
-      read(slot0, 0, aw, ax);
-      multiply(aw, ax);
-      read(slot0, 1, bw, bx);
-      multiply(bw, bx);
+        place(slot2.w, wave * C::kLoadsW + i, load_first(src_w[i] + full, k_end - full - col_w[i]));
+      staged_barrier<63>();
+      products(slot2);
     }
   }
 
@@ -514,9 +589,10 @@ struct ColTile {
   static constexpr int kDepth = kFrags >= 16 ? 2 : kFrags >= 4 ? 4 : 16 / (2 * (kFT + kFN));
 };
 
-template <typename T, int kFT, int kFN, bool kGated, bool kAligned>
+template <typename T, int kFT, int kFN, bool kGated, RowKind kRows>
 __global__ __launch_bounds__(kColThreads) void proj_cols_kernel(ProjArgs p) {
   using V8 = typename VecOf<T>::v8;
+  constexpr bool kAligned = kRows == kVectors;
   constexpr int kFrags = kFT * kFN, kDepth = ColTile<kFT, kFN>::kDepth;
   constexpr int kOutFrags = kGated ? kFN / 2 : kFN;  // fragments of outputs per token fragment
   static_assert(!kGated || kFN % 2 == 0, "both factors of a gate");
@@ -533,28 +609,41 @@ __global__ __launch_bounds__(kColThreads) void proj_cols_kernel(ProjArgs p) {
   const T* w[kFN];
   const T* x[kFT];
   bool w_ok[kFN], x_ok[kFT];
+  // (Rows past the last read another one where their loads are not held back:
+  // their sums are written nowhere.)
 #pragma unroll
   for (int i = 0; i < kFN; ++i) {
     const int n = n0 + i % kOutFrags * 16 + (lane & 15);
     w_ok[i] = n < p.n_out;
-    w[i] = static_cast<const T*>(p.w) + (n + (i < kOutFrags ? 0 : static_cast<int64_t>(p.n_out))) * p.ldw + kc;
+    w[i] = static_cast<const T*>(p.w) + ((w_ok[i] ? n : 0) + (i < kOutFrags ? 0 : static_cast<int64_t>(p.n_out))) * p.ldw + kc;
   }
 #pragma unroll
   for (int j = 0; j < kFT; ++j) {
     const int64_t t = t0 + j * 16 + (lane & 15);
     x_ok[j] = t < p.tokens;
-    x[j] = static_cast<const T*>(p.x) + t * p.ldx + kc;
+    x[j] = static_cast<const T*>(p.x) + (x_ok[j] ? t : t0) * p.ldx + kc;
   }
-  auto get = [&](const T* row, bool ok, int k) -> V8 {
-    if constexpr (kAligned) return ok && k + kc < k_end ? load8(row + k) : zero8<T>();
-    return __builtin_bit_cast(V8, load_ragged(row + k, ok ? k_end - k - kc : 0));
-  };
   f32x4 acc[kFN][kFT];
 #pragma unroll
   for (int i = 0; i < kFN; ++i)
 #pragma unroll
     for (int j = 0; j < kFT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  V8 fw[kDepth][2][kFN], fx[kDepth][2][kFT];
+  using Held = std::conditional_t<kRows == kElements, Words, V8>;  // eight elements on their way
+  auto get = [&](const T* row, bool ok, int k) -> Held {
+    if constexpr (kRows == kVectors)
+      return ok && k + kc < k_end ? load8(row + k) : zero8<T>();
+    else if constexpr (kRows == kWords)
+      return __builtin_bit_cast(V8, load_any(row + k));
+    else
+      return load_words(row + k);
+  };
+  auto fragment = [&](const Held& v, const T* row) -> V8 {
+    if constexpr (kRows == kElements)
+      return __builtin_bit_cast(V8, settle(v, inside_word(row)));
+    else
+      return v;
+  };
+  Held fw[kDepth][2][kFN], fx[kDepth][2][kFT];
   auto load = [&](int b, int k) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -564,21 +653,46 @@ __global__ __launch_bounds__(kColThreads) void proj_cols_kernel(ProjArgs p) {
       for (int j = 0; j < kFT; ++j) fx[b][h][j] = get(x[j], x_ok[j], k + h * 32);
     }
   };
+  auto multiply = [&](const V8 (&vw)[kFN], const V8 (&vx)[kFT]) {
+#pragma unroll
+    for (int i = 0; i < kFN; ++i)
+#pragma unroll
+      for (int j = 0; j < kFT; ++j) acc[i][j] = mfma16(vw[i], vx[j], acc[i][j]);
+  };
   constexpr int kStride = kColWaves * kColBlock;
   const int k0 = k_begin + wave * kColBlock;
+  // Rows that are not whole vectors: the whole blocks, whose loads need no tests,
+  // then the columns left, which are one wave's.
+  const int blocks_end = kAligned ? k_end : k_begin + (k_end - k_begin) / kColBlock * kColBlock;
 #pragma unroll
-  for (int b = 0; b < kDepth; ++b) load(b, k0 + b * kStride);
-  for (int k = k0; k < k_end; k += kDepth * kStride) {
+  for (int b = 0; b < kDepth; ++b)
+    if (kAligned || k0 + b * kStride < blocks_end) load(b, k0 + b * kStride);
+  for (int k = k0; k < blocks_end; k += kDepth * kStride) {
 #pragma unroll
     for (int b = 0; b < kDepth; ++b) {
-      if (k + b * kStride >= k_end) break;
+      if (k + b * kStride >= blocks_end) break;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        V8 vw[kFN], vx[kFT];
 #pragma unroll
-        for (int i = 0; i < kFN; ++i)
+        for (int i = 0; i < kFN; ++i) vw[i] = fragment(fw[b][h][i], w[i]);
 #pragma unroll
-          for (int j = 0; j < kFT; ++j) acc[i][j] = mfma16(fw[b][h][i], fx[b][h][j], acc[i][j]);
-      if (k + (kDepth + b) * kStride < k_end) load(b, k + (kDepth + b) * kStride);
+        for (int j = 0; j < kFT; ++j) vx[j] = fragment(fx[b][h][j], x[j]);
+        multiply(vw, vx);
+      }
+      if (k + (kDepth + b) * kStride < blocks_end) load(b, k + (kDepth + b) * kStride);
+    }
+  }
+  if (blocks_end < k_end && (blocks_end - k_begin) / kColBlock % kColWaves == wave) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = blocks_end + h * 32;
+      V8 vw[kFN], vx[kFT];
+#pragma unroll
+      for (int i = 0; i < kFN; ++i) vw[i] = __builtin_bit_cast(V8, load_first(w[i] + k, k_end - k - kc));
+#pragma unroll
+      for (int j = 0; j < kFT; ++j) vx[j] = __builtin_bit_cast(V8, load_first(x[j] + k, k_end - k - kc));
+      multiply(vw, vx);
     }
   }
 
@@ -667,7 +781,7 @@ hipError_t launch_tiles(ProjArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename T, int kFT, int kFN, bool kAligned>
+template <typename T, int kFT, int kFN, RowKind kRows>
 hipError_t launch_cols(ProjArgs& a, int n_cu, hipStream_t stream) {
   const int outs = kFN * 16 / (a.gated ? 2 : 1);
   a.tiles_t = static_cast<int32_t>((a.tokens + kFT * 16 - 1) / (kFT * 16));
@@ -680,31 +794,36 @@ hipError_t launch_cols(ProjArgs& a, int n_cu, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(tiles * a.splits));
   if (a.gated) {
     if constexpr (kFN % 2 == 0)
-      hipLaunchKernelGGL((proj_cols_kernel<T, kFT, kFN, true, kAligned>), grid, dim3(kColThreads), 0, stream, a);
+      hipLaunchKernelGGL((proj_cols_kernel<T, kFT, kFN, true, kRows>), grid, dim3(kColThreads), 0, stream, a);
   } else {
-    hipLaunchKernelGGL((proj_cols_kernel<T, kFT, kFN, false, kAligned>), grid, dim3(kColThreads), 0, stream, a);
+    hipLaunchKernelGGL((proj_cols_kernel<T, kFT, kFN, false, kRows>), grid, dim3(kColThreads), 0, stream, a);
   }
   return hipGetLastError();
 }
 
-template <typename T, bool kAligned>
+template <typename T, RowKind kRows>
 hipError_t launch(ProjArgs& a, int n_cu, hipStream_t stream) {
+  constexpr bool kAligned = kRows == kVectors;
   if (a.tokens <= 16) {
-    if (a.gated) return launch_cols<T, 1, 2, kAligned>(a, n_cu, stream);
-    return launch_cols<T, 1, 1, kAligned>(a, n_cu, stream);
+    if (a.gated) return launch_cols<T, 1, 2, kRows>(a, n_cu, stream);
+    return launch_cols<T, 1, 1, kRows>(a, n_cu, stream);
   }
   const int64_t rows = static_cast<int64_t>(a.n_out) * (a.gated ? 2 : 1);
   auto tiles = [&](int64_t b) { return (a.tokens + b - 1) / b * ((rows + b - 1) / b); };
   // (32 x 4096 x 4096: 11.8 us, 14.2 on 64-row tiles; 128 x 8192 x 1024, 32 of
   // those tiles: 19.9 and 24.6; 128 x 2048 x 2048, 64 of them: 9.9 and 8.9.)
-  if (a.tokens <= 32 || tiles(64) < n_cu / 4) return launch_cols<T, 2, 2, kAligned>(a, n_cu, stream);
+  if (a.tokens <= 32 || tiles(64) < n_cu / 4) return launch_cols<T, 2, 2, kRows>(a, n_cu, stream);
   // The tile whose rounds over the device cost least.  A K-step of a round
   // takes 1.5 us with the 256-row tile (one workgroup a compute unit), 0.72
   // with the 128-row one, 0.4 with two 64-row ones a compute unit and 0.22
   // with one.  (512 x 5120 x 27648: 124, 195 and 274 us; 2048 x 2048 x 2048: 49,
   // 20.9 and 26.7; 1000 x 2048 x 2048: 51, 17.4 and 15.0.)
   auto rounds = [&](int64_t n, int64_t at_once) { return static_cast<double>((n + at_once - 1) / at_once); };
-  const double cost64 = tiles(64) <= n_cu ? 0.22 : 0.4 * rounds(tiles(64), 2 * n_cu);
+  // Rows that are not whole vectors: 0.66 and 0.36 on the 64-row tiles, as long
+  // as the others on the 128-row one.  (300 x 8191 x 14336: 166 us on 128 rows, 195
+  // on 64; 400 x 4097 x 8000: 50 and 84; 500 x 8191 x 4096: 88 and 85; 1000 x 1001 x
+  // 1101: 17.8 and 15.7.)
+  const double cost64 = tiles(64) <= n_cu ? (kAligned ? 0.22 : 0.36) : (kAligned ? 0.4 : 0.66) * rounds(tiles(64), 2 * n_cu);
   const double cost128 = 0.72 * rounds(tiles(128), n_cu);
   if constexpr (kAligned) {
     if (1.5 * rounds(tiles(256), n_cu) <= std::min(cost64, cost128))
@@ -721,10 +840,14 @@ hipError_t launch_proj(int dtype_bf16, ProjArgs& a, int n_cu, hipStream_t stream
     return reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld % (bytes / 2) == 0;
   };
   a.rows_vec = whole(a.y, a.ldy, 8) && whole(a.residual, a.ldr, 8);
-  // Rows further apart than kFarRows take the register path, which has no 32-bit offsets.
-  const bool aligned = a.d_in % 8 == 0 && whole(a.x, a.ldx, 16) && whole(a.w, a.ldw, 16) && a.ldx <= kFarRows && a.ldw <= kFarRows;
-  if (dtype_bf16) return aligned ? launch<__bf16, true>(a, n_cu, stream) : launch<__bf16, false>(a, n_cu, stream);
-  return aligned ? launch<_Float16, true>(a, n_cu, stream) : launch<_Float16, false>(a, n_cu, stream);
+  // Rows further apart than kFarRows take the register paths, which have no 32-bit offsets.
+  const bool vectors = a.d_in % 8 == 0 && whole(a.x, a.ldx, 16) && whole(a.w, a.ldw, 16) && a.ldx <= kFarRows && a.ldw <= kFarRows;
+  const bool words = whole(a.x, a.ldx, 4) && whole(a.w, a.ldw, 4);
+  auto run = [&](auto t) {
+    using T = decltype(t);
+    return vectors ? launch<T, kVectors>(a, n_cu, stream) : words ? launch<T, kWords>(a, n_cu, stream) : launch<T, kElements>(a, n_cu, stream);
+  };
+  return dtype_bf16 ? run(__bf16{}) : run(_Float16{});
 }
 
 }  // namespace wp

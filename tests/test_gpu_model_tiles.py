@@ -67,6 +67,42 @@ def test_rows_that_start_anywhere(engine, shift, pad, dtype):
         linear_case(engine, T, d_in, n, dtype, shift=shift, pad=pad)
 
 
+# Few tokens, whose rows go straight to registers: on 4-byte words and on any
+# element, less than a block of 64 columns, several rounds of them, split.
+@DTYPES
+@pytest.mark.parametrize("T,n", [(1, 70), (9, 200), (16, 33), (24, 100), (100, 300)], ids=str)
+@pytest.mark.parametrize("d_in", [2, 62, 63, 129, 1026, 4099, 8190, 8191])
+def test_rows_of_no_whole_vectors_of_few_tokens(engine, T, n, d_in, dtype):
+    linear_case(engine, T, d_in, n, dtype, "silu", bias=True, residual=True)
+    linear_case(engine, T, d_in, n, dtype, "relu", gated=True)
+    for shift, pad in ((1, 1), (1, 2), (2, 2)):
+        linear_case(engine, T, d_in, n, dtype, shift=shift, pad=pad)
+
+
+def test_rows_of_no_whole_vectors_beat_a_plain_product(engine):
+    """33 x 8191 -> 4200 as one call and as a product in 32 bits that casts its
+    operands: half the time, and not more than all of it."""
+    x, w = randn((33, 8191), 0, torch.bfloat16).cuda(), randn((4200, 8191), 1, torch.bfloat16).cuda()
+    announce("linear 33 x 8191 -> 4200, timed")
+
+    def time(f):
+        for _ in range(5):
+            f()
+        took = []
+        for _ in range(15):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(10):
+                f()
+            b.record()
+            b.synchronize()
+            took.append(a.elapsed_time(b) * 100)
+        return sorted(took)[7]
+
+    one, plain = time(lambda: engine.linear(x, w)), time(lambda: (x.float() @ w.float().t()).to(x.dtype))
+    assert one < plain, f"{one:.1f} us, {plain:.1f} as a plain product"
+
+
 # Columns: a multiple of the K-step, of 8 only, less than one step, one step, of eight.
 @DTYPES
 @pytest.mark.parametrize("T,d_in,n", [(4100, 576, 2304), (4133, 584, 2311), (4100, 72, 2304), (4100, 64, 2310), (4100, 8, 2304), (4100, 1096, 2304)],
