@@ -159,7 +159,7 @@ __device__ __forceinline__ int chunks_of(int keys, int shift) {
   return std::max(1, static_cast<int>((static_cast<int64_t>(keys) + (1ll << shift) - 1) >> shift));
 }
 __device__ __forceinline__ int shift_of(const AttnArgs& p, int rows, bool rows_role) {
-  return rows_role ? p.tile_shift : rows > kChunkRows && !p.chunk_wide ? kNoSplit : p.chunk_shift;
+  return rows_role ? p.tile_shift : rows > p.split_rows ? kNoSplit : p.chunk_shift;
 }
 __device__ __forceinline__ int items_of(const AttnArgs& p, const Span& s, bool rows_role, int tile_rows, int* tiles) {
   const int rows = s.n_q * p.group;
@@ -822,9 +822,10 @@ __device__ __forceinline__ void run_item(const AttnArgs& p, const Item& it, Shar
 
   const bool split = chunks > 1;
   const bool sees = real && w.pos >= w.low;
-  // The item's partials: [rows][bound, sum], then [rows][DP] of O.
-  float* part = p.part + (kTile ? 0 : p.chunk_part) + static_cast<uint64_t>(it.slot) * kRows * (DP + 2);
-  const __amdgpu_buffer_rsrc_t mine = coherent_buffer(part, static_cast<uint32_t>(kRows) * (DP + 2) * 4u);
+  // The item's partials: [rows][DP] of O, then [rows][bound, sum].
+  const uint32_t slot_rows = kTile ? kRows : p.slot_rows;
+  float* part = p.part + (kTile ? 0 : p.chunk_part) + static_cast<uint64_t>(it.slot) * slot_rows * (DP + 2);
+  const __amdgpu_buffer_rsrc_t mine = coherent_buffer(part, slot_rows * (DP + 2) * 4u);
 
   if (kTile || share == 1) {
     const float inv = 1.f / w.l;
@@ -847,13 +848,13 @@ __device__ __forceinline__ void run_item(const AttnArgs& p, const Item& it, Shar
     const int r = wave * kWaveRows + (lane & 31);
     if (real) {
       if (half == 0) {
-        coherent_store8(part + 2 * r, __builtin_bit_cast(unsigned long long, f32x2{w.m, w.l}));
+        coherent_store8(part + slot_rows * DP + 2 * r, __builtin_bit_cast(unsigned long long, f32x2{w.m, w.l}));
       }
 #pragma unroll
       for (int i = 0; i < H::kCols; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          coherent_store16(mine, (2u * kRows + r * DP + i * 32 + e * 8 + half * 4) * 4u,
+          coherent_store16(mine, (r * DP + i * 32 + e * 8 + half * 4) * 4u,
                            f32x4{w.o[i][e * 4], w.o[i][e * 4 + 1], w.o[i][e * 4 + 2], w.o[i][e * 4 + 3]});
     }
   } else {
@@ -897,8 +898,8 @@ __device__ __forceinline__ void run_item(const AttnArgs& p, const Item& it, Shar
 #pragma unroll
       for (int i = 0; i < kWaves; ++i) l += ls[i] * (top == -INFINITY ? 1.f : exp2_fast(ms[i] - top));
       if (split) {
-        coherent_store16(mine, (2u * kRows + r * DP + d) * 4u, v);
-        if (d == 0) coherent_store8(part + 2 * r, __builtin_bit_cast(unsigned long long, f32x2{top, l}));
+        coherent_store16(mine, (r * DP + d) * 4u, v);
+        if (d == 0) coherent_store8(part + slot_rows * DP + 2 * r, __builtin_bit_cast(unsigned long long, f32x2{top, l}));
       } else {
         finish_row<T>(p, it, row0 + r, d, v, top, l);
       }
@@ -917,7 +918,7 @@ __device__ __forceinline__ void run_item(const AttnArgs& p, const Item& it, Shar
   }
   __syncthreads();
   if (sh.last == 0u) return;
-  const int64_t step = static_cast<int64_t>(it.stride) * kRows * (DP + 2);  // floats between chunks' partials
+  const int64_t step = static_cast<int64_t>(it.stride) * slot_rows * (DP + 2);  // floats between chunks' partials
   const float* part0 = part - it.chunk * step;
   for (int u = tid; u < my_rows * (DP / 4); u += kThreads) {
     const int r = u / (DP / 4), d = u % (DP / 4) * 4;
@@ -930,8 +931,8 @@ __device__ __forceinline__ void run_item(const AttnArgs& p, const Item& it, Shar
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const float* at = part0 + std::min(i0 + i, chunks - 1) * step;
-        ml[i] = __builtin_bit_cast(f32x2, coherent_load8(at + 2 * r));
-        o[i] = coherent_load_f4(at + 2 * kRows + r * DP + d);
+        ml[i] = __builtin_bit_cast(f32x2, coherent_load8(at + slot_rows * DP + 2 * r));
+        o[i] = coherent_load_f4(at + r * DP + d);
       }
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
@@ -1058,7 +1059,7 @@ hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t s
   const int64_t group = a.group, rows = a.tokens * group;
   // Bounds on the work items, from the sizes the host knows: a sequence of
   // more than 128 rows has at most rows / 128 + 1 row tiles, and one of fewer
-  // at most keys / chunk + 2 key chunks.
+  // at most keys / chunk + 1 key chunks.
   const int64_t seqs = std::max(1, a.n_seq);
   // One sequence has one role.  Many of a few rows each (drafted tokens; their
   // mean at most 64 and none of more than 1024 if all have a token) run on key
@@ -1099,20 +1100,29 @@ hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t s
   // Blocks of 128 rows: where sequences of more than 128 run on key chunks, the
   // longest could have them all.
   const int64_t blocks = few ? std::max<int64_t>(1, (rows + kChunkRows - 1) / kChunkRows) : 1;
-  const int64_t usual = ((a.keys >> chunk_shift) + 2 * chunk_seqs) * a.kv_heads;
+  const int64_t usual = ((a.keys >> chunk_shift) + chunk_seqs) * a.kv_heads;
   int64_t chunk_items = 0, chunk_grid = 0;
   if (chunk_seqs > 0) {
     const int64_t counters = tile_counters + (chunk_seqs + blocks) * a.kv_heads;
-    auto fits = [&](int64_t items) {
-      return (tile_floats + static_cast<uint64_t>(items) * kChunkRows * (dp + 2)) * 4 <= a.part_bytes && counters <= a.n_counters;
+    auto fits = [&](int64_t items, int64_t slot) {
+      return (tile_floats + static_cast<uint64_t>(items) * slot * (dp + 2)) * 4 <= a.part_bytes && counters <= a.n_counters;
     };
-    a.chunk_wide = fits(usual * blocks);
-    chunk_items = a.chunk_wide ? usual * blocks : usual + blocks * a.kv_heads;
+    // A chunk has room for the partial results of 128 rows or, where the scratch
+    // does not hold that many, of half as many or fewer, down to a token's;
+    // sequences of more rows then have their keys run in one go.  (512 single tokens,
+    // 32 heads over 8 of 128, one cache of 32768 keys among others of 100: 131 us
+    // with room for 64 rows, 443 if no keys are split; all of 2000 keys: 692 either way.)
+    int64_t slot = kChunkRows;
+    const bool wide = fits(usual * blocks, slot);
+    chunk_items = wide ? usual * blocks : usual + blocks * a.kv_heads;
     chunk_grid = usual;
-    if (!fits(chunk_items)) {
+    while (!wide && slot >= a.group && !fits(chunk_items, slot)) slot /= 2;
+    if (slot < a.group && !wide) {
       chunk_shift = kNoSplit;
       chunk_items = chunk_grid = (chunk_seqs + blocks) * a.kv_heads;
     }
+    a.slot_rows = static_cast<int32_t>(slot);
+    a.split_rows = wide ? 0x7FFFFFFF : static_cast<int32_t>(slot);
   }
   if (tile_items + chunk_items > 0x7FFFFFFF) return hipErrorInvalidValue;
   a.tile_items = static_cast<int32_t>(tile_items);

@@ -82,7 +82,8 @@ struct AttnArgs {
   int32_t tile_items, chunk_items;
   int32_t tile_shift, chunk_shift;
   int32_t chunk_rows;  // most rows per key head of a sequence that runs on key chunks
-  int32_t chunk_wide;  // sequences of more rows than a workgroup takes have their keys split there too
+  int32_t split_rows;  // and of one whose keys are split there
+  int32_t slot_rows;   // rows that a key chunk has room for among the partials
   int32_t chunk_counters;
   int32_t tile_counters, seq_counters;  // how many either role has
   uint64_t chunk_part;
