@@ -113,6 +113,7 @@ struct Item {
   int slot;      // the item's place among the partials
   int counter;   // its row tile's counter
   int stride;    // between the slots of a row tile's chunks
+  int end;       // no item's id reaches this
   int64_t q0, k0;
   int n_q, n_k;
 };
@@ -269,8 +270,10 @@ __device__ __forceinline__ Item find_item(const AttnArgs& p, bool rows_role, int
       const int local = want - base - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(items, at));
       const int n_tiles = __builtin_amdgcn_readlane(tiles, at);
       // Later row tiles see more keys: they go first.
-      return item_of(p, s, at, id - want * p.kv_heads, id, b0 + at, n_tiles - 1 - local % n_tiles, local / n_tiles, n_tiles,
-                     tile_base + __builtin_amdgcn_readlane(tile_sum, at) - n_tiles);
+      Item it = item_of(p, s, at, id - want * p.kv_heads, id, b0 + at, n_tiles - 1 - local % n_tiles, local / n_tiles, n_tiles,
+                        tile_base + __builtin_amdgcn_readlane(tile_sum, at) - n_tiles);
+      it.end = b0 + 64 < p.n_seq ? p.chunk_items : (base + __builtin_amdgcn_readlane(sum, 63)) * p.kv_heads;
+      return it;
     }
     base += __builtin_amdgcn_readlane(sum, 63);
     tile_base += __builtin_amdgcn_readlane(tile_sum, 63);
@@ -993,7 +996,7 @@ __global__ __launch_bounds__(64 * kWaves, (kOccupancy<DP, kRoles>)) void attenti
     while (id < p.chunk_items && it.seq >= 0 && it.counter < p.seq_counters) {
       run_item<T, DP, kWaves, kChunks>(p, it, sh, sk[0], sk[1], sv[0], sv[1], &sk[0][0] + wave * kHalf, &sv[0][0] + wave * kHalf);
       id += static_cast<int>(gridDim.x);
-      if (id >= p.chunk_items) return;
+      if (id >= p.chunk_items || id >= it.end) return;
       __syncthreads();
       it = find_item(p, false, kRows, id);
     }
