@@ -1064,15 +1064,19 @@ hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t s
   // more than 128 rows has at most rows / 128 + 1 row tiles, and one of fewer
   // at most keys / chunk + 1 key chunks.
   const int64_t seqs = std::max(1, a.n_seq);
-  // One sequence has one role.  Many of a few rows each (drafted tokens; their
-  // mean at most 64 and none of more than 1024 if all have a token) run on key
-  // chunks alone: a kernel without the row tiles' search and empty workgroups
-  // (32 sequences of up to 40 rows: 21.9 us, 24.1 with both roles).  Others share
-  // a launch, where sequences run on key chunks up to 128 rows, or up to 32 next
+  // One sequence has one role.  Many of a few rows each (their mean at most 64,
+  // and none of more than 128 if all have a token: single tokens, mostly) run on
+  // key chunks alone, in a kernel without the row tiles' search and empty workgroups
+  // (64 single tokens over up to 8192 keys: 79.6 us, 81.4 with both roles; 256: 193
+  // and 196).  Where one could be longer the roles share a launch: drafted tokens
+  // take the same either way (32 of up to 5, 8 heads a key head: 20.4 and 20.3;
+  // 200 of up to 8, heads of their own keys: 50.2 and 51.9), but a prompt of 130
+  // tokens among 19 single ones 35.2 us on key chunks and 26.0 on row tiles.
+  // There, sequences run on key chunks up to 128 rows, or up to 32 next
   // to longer ones (32 heads of their own keys: a prompt of 128 rows takes 12.7 us
   // on key chunks, one of 129 takes 11.0 on a row tile).
   const int64_t longest = (std::max<int64_t>(0, a.tokens - seqs) + 1) * group;
-  const bool few = a.n_seq <= 1 ? rows <= kChunkRows : rows <= 64 * seqs && longest <= 1024;
+  const bool few = a.n_seq <= 1 ? rows <= kChunkRows : rows <= 64 * seqs && longest <= kChunkRows;
   a.chunk_rows = few ? 0x7FFFFFFF : a.n_seq <= 1 ? 0 : rows >= kChunkRows * seqs ? kWaveRows : kChunkRows;
   const int64_t tile_seqs = few ? 0 : std::min<int64_t>(a.n_seq, rows / (a.chunk_rows + 1));
   // Row tiles of 256 rows read K and V half as often as those of 128 (a prompt of
