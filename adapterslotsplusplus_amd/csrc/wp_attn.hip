@@ -25,11 +25,11 @@
 // to finish joins the partial results.
 //
 // What bounds it.  Long prompts: the matrix and the vector unit take turns at
-// nearly equal work (16384 tokens, 32 heads of 128: 1950 us, 1.13 PF/s; a 64-key
+// nearly equal work (16384 tokens, 32 heads of 128: 2000 us, 1.10 PF/s; a 64-key
 // step of 32 rows takes 1024 cycles of products and about 900 of exponentials, sums
 // and roundings).  Decoding over long caches: HBM (64 sequences of up to 8192
-// keys, 8 key heads: 79.5 us, 4.4 TB/s).  Few and short sequences: the chain of
-// latencies from the bounds over K to the join (one token over 777 keys: 11.3 us,
+// keys, 8 key heads: 79.7 us, 4.4 TB/s).  Few and short sequences: the chain of
+// latencies from the bounds over K to the join (one token over 777 keys: 11.5 us,
 // of them 2.2 to find the item, 3.4 to the last product, 4 to join).
 #include <hip/hip_runtime.h>
 

@@ -816,8 +816,9 @@ hipError_t launch(ProjArgs& a, int n_cu, hipStream_t stream) {
   // The tile whose rounds over the device cost least.  A K-step of a round
   // takes 1.5 us with the 256-row tile (one workgroup a compute unit), 0.72
   // with the 128-row one, 0.4 with two 64-row ones a compute unit and 0.22
-  // with one.  (512 x 5120 x 27648: 124, 195 and 274 us; 2048 x 2048 x 2048: 49,
-  // 20.9 and 26.7; 1000 x 2048 x 2048: 51, 17.4 and 15.0.)
+  // with one.  (512 x 5120 x 27648: 130, 202 and 279 us; 2048 x 2048 x 2048: 49,
+  // 20.2 and 26.3; 1000 x 2048 x 2048: 52, 17.5 and 14.9; on operands of one
+  // magnitude: the first takes 129 with constant ones and 141 with normal ones.)
   auto rounds = [&](int64_t n, int64_t at_once) { return static_cast<double>((n + at_once - 1) / at_once); };
   // Rows that are not whole vectors: 0.66 and 0.36 on the 64-row tiles, as long
   // as the others on the 128-row one.  (300 x 8191 x 14336: 166 us on 128 rows, 195

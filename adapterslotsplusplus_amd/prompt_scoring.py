@@ -14,8 +14,8 @@ once by `engine.token_logprobs`.  The adapters' deltas are
   * `verify(ids, cu_seqlens, tenants, cache)`: the same for tokens drafted after
     what the cache holds, all in one pass; the cache grows by them.
 
-Nothing here waits for the device except the cache's growth, whose new size
-the host must know (it is given by the lengths the caller passes).
+Nothing here waits for the device; the lengths that the caller passes, and
+where the cache's rows go, are uploaded from host memory at each step.
 """
 from __future__ import annotations
 

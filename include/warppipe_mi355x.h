@@ -387,8 +387,8 @@ int wp_packed_attention(wp_engine* e, void* out, const int64_t* out_strides, flo
  * stride): logprobs = log softmax at token_ids[row], entropy = the softmax's
  * entropy (nats), ranks = 1 + how many logits are greater than the token's, and
  * the `top` (up to 64) largest logits in order, equal ones by the lower id, as
- * top_ids and top_logprobs [rows, top].  NaN counts as the largest value.  A
- * token id of -1 (or below) names no token: logprob and rank 0; so does one
+ * top_ids and top_logprobs [rows, top].  NaN comes first among these, and is
+ * greater than none in a rank.  A token id of -1 (or below) names no token: logprob and rank 0; so does one
  * past the vocabulary, which is flagged (device error 1).  A row whose logits are all
  * -inf, or which holds NaN or +inf, has no distribution: NaN. */
 int wp_token_logprobs(wp_engine* e, float* logprobs, float* entropy, int32_t* ranks, float* top_logprobs,
