@@ -84,7 +84,7 @@ def test_attention_strides_of_one_entry_do_not_matter(engine):
     assert torch.equal(engine.packed_attention(odd_q, one, one, ints(0, 1), ints(0, 1)), k[:1].expand(1, 2, 64))
 
 
-@pytest.mark.parametrize("far", [1 << 23, (1 << 27) + 8], ids=["2^23", "past 2^27"])
+@pytest.mark.parametrize("far", [1 << 23, 1 << 27, (1 << 27) + 8], ids=["2^23", "2^27", "past 2^27"])
 @pytest.mark.parametrize("T,n", [(2, 40), (20, 72), (70, 2048)], ids=str)
 def test_linear_rows_far_apart(engine, far, T, n):
     """The last position of each of several sequences: [:, -1] of [T, 2048, 4096] lies 2^23 elements apart."""
