@@ -49,6 +49,7 @@ EXPORTED = (
     "wp_set_max_adapters", "wp_read_static_errors", "wp_poll_device_errors", "wp_lora_shrink", "wp_lora_expand",
     "wp_add_bias", "wp_handoff_probe", "wp_barrier_probe", "wp_shrink_new",
     "wp_linear", "wp_packed_attention", "wp_token_logprobs",
+    "wp_rotate_heads", "wp_rotate_into_cache", "wp_write_cache", "wp_read_cache",
 )
 
 
@@ -129,6 +130,10 @@ def load():
         "wp_packed_attention": ([p, p, p, p, p, p, p, p, p, p, p, p, i32, i64, i64, i32, i32, i32, f32, i32, i32, i32, p],
                                 ctypes.c_int),
         "wp_token_logprobs": ([p, p, p, p, p, p, p, i64, p, i32, i64, i32, i32, i32, p], ctypes.c_int),
+        "wp_rotate_heads": ([p, p, p, p, p, p, p, p, p, p, p, f32, p, i64, i32, i32, i32, i32, p], ctypes.c_int),
+        "wp_rotate_into_cache": ([p, p, p, p, p, p, p, p, p, p, p, f32, p, p, p, i32, i64, i32, i32, p], ctypes.c_int),
+        "wp_write_cache": ([p, p, p, p, p, p, p, i32, i64, i32, p], ctypes.c_int),
+        "wp_read_cache": ([p, p, p, p, p, p, p, i32, i64, i32, p], ctypes.c_int),
         "wp_barrier_probe": ([p, i32, i32, i32, p, p], ctypes.c_int),
     }
     for name, (args, res) in sig.items():

@@ -1045,15 +1045,6 @@ hipError_t launch_head(const AttnArgs& a, int dp, int tile_waves, int chunk_grid
 
 }  // namespace
 
-// Exact for every dividend under 2^31: the quotient's error is under
-// dividend / 2^shift * d < 1 / d of a step.
-static Divisor divisor_of(int d) {
-  Divisor r{0, 31};
-  while ((1ll << (r.shift - 31)) < d) ++r.shift;
-  r.magic = static_cast<uint32_t>(((1ull << r.shift) + static_cast<uint64_t>(d) - 1) / static_cast<uint64_t>(d));
-  return r;
-}
-
 hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t stream) {
   const int dp = a.dim <= 64 ? 64 : a.dim <= 96 ? 96 : 128;
   a.group = a.heads / a.kv_heads;

@@ -35,6 +35,7 @@
 #include "../../include/warppipe_mi355x.h"
 #include "wp_apply.h"
 #include "wp_model.h"
+#include "wp_paged.h"
 
 using namespace wp;
 
@@ -2649,6 +2650,248 @@ int wp_token_logprobs(wp_engine* e, float* logprobs, float* entropy, int32_t* ra
   a.n_counters = kModelCounters;
   WP_HIP(launch_logprobs(a, e->n_cu, static_cast<hipStream_t>(stream)));
   return WP_OK;
+}
+
+}  // extern "C"
+
+// ------------------------------------------------- heads and a paged cache --
+
+namespace {
+
+int check_dtype(const char* who, int32_t dtype) {
+  if (dtype != WP_DTYPE_F16 && dtype != WP_DTYPE_BF16) return fail(WP_ERR_INVALID, "%s: dtype must be fp16 or bf16", who);
+  return WP_OK;
+}
+
+// Strides between tokens and heads of a [tokens, heads, dim] tensor; one of a
+// dimension of one entry does not matter.  apart: rows must not overlap.
+int head_strides(const char* who, const char* what, const void* p, const int64_t* given, int64_t tokens, int32_t heads,
+                 int32_t dim, bool apart, int64_t (&s)[2]) {
+  if (!p || !given) return fail(WP_ERR_INVALID, "%s: null %s", who, what);
+  if (!aligned(p, 16)) return fail(WP_ERR_INVALID, "%s: %s must be 16-byte aligned", who, what);
+  const int64_t sizes[2] = {tokens, heads};
+  for (int i = 0; i < 2; ++i) {
+    s[i] = sizes[i] > 1 ? given[i] : 0;
+    if (s[i] < 0 || s[i] % 8 != 0)
+      return fail(WP_ERR_INVALID, "%s: strides of %s must be multiples of 8 elements (got %lld)", who, what, (long long)s[i]);
+    if (apart && sizes[i] > 1 && s[i] < dim)
+      return fail(WP_ERR_INVALID, "%s: rows of %s overlap (stride %lld, head size %d)", who, what, (long long)s[i], dim);
+  }
+  return WP_OK;
+}
+
+int check_pages(const char* who, const wp_pages* c, int32_t most_dim) {
+  if (!c) return fail(WP_ERR_INVALID, "%s: null cache", who);
+  const int unit = c->e4m3 ? 16 : 8;
+  if (c->pages < 0 || c->pages > 0x7FFFFFFF) return fail(WP_ERR_INVALID, "%s: %lld pages", who, (long long)c->pages);
+  if (c->page_size < kMinPage || c->page_size > (1 << 24) || (c->page_size & (c->page_size - 1)) != 0)
+    return fail(WP_ERR_INVALID, "%s: pages of %d tokens (a power of two from %d on)", who, c->page_size, kMinPage);
+  if (c->kv_heads < 1 || c->kv_heads > 65535) return fail(WP_ERR_INVALID, "%s: %d key heads", who, c->kv_heads);
+  if (c->head_dim < unit || c->head_dim > most_dim || c->head_dim % unit != 0)
+    return fail(WP_ERR_INVALID, "%s: head size %d (a multiple of %d up to %d)", who, c->head_dim, unit, most_dim);
+  if (c->pages == 0) return WP_OK;
+  if (!c->k || !c->v || (c->e4m3 && (!c->k_scales || !c->v_scales))) return fail(WP_ERR_INVALID, "%s: null pages or scales", who);
+  if (!aligned(c->k, 16) || !aligned(c->v, 16)) return fail(WP_ERR_INVALID, "%s: pages must be 16-byte aligned", who);
+  const int64_t sizes[3] = {c->pages, c->page_size, c->kv_heads};
+  for (const int64_t* s : {c->k_strides, c->v_strides})
+    for (int i = 0; i < 3; ++i)
+      if (sizes[i] > 1 && (s[i] < c->head_dim || s[i] % unit != 0))
+        return fail(WP_ERR_INVALID, "%s: strides of pages must be multiples of %d elements, a head or more (got %lld)", who, unit,
+                    (long long)s[i]);
+  for (const int64_t* s : {c->k_strides, c->v_strides})
+    if (s[1] > kMaxKeyStride)
+      return fail(WP_ERR_INVALID, "%s: tokens of a page must be at most %lld elements apart", who, (long long)kMaxKeyStride);
+  if (c->e4m3)
+    for (const int64_t* s : {c->k_scale_strides, c->v_scale_strides})
+      for (int i = 0; i < 3; ++i)
+        if (sizes[i] > 1 && s[i] < 1) return fail(WP_ERR_INVALID, "%s: scales overlap (stride %lld)", who, (long long)s[i]);
+  return WP_OK;
+}
+
+int check_rotation(const char* who, const wp_rotation* r, int32_t head_dim, HeadArgs& a) {
+  if (!r) return WP_OK;
+  if (r->dim < 2 || r->dim % 2 != 0 || r->dim > head_dim)
+    return fail(WP_ERR_INVALID, "%s: %d of a head's %d elements rotate (an even number)", who, r->dim, head_dim);
+  if (!r->turns || !r->positions) return fail(WP_ERR_INVALID, "%s: null turns or positions", who);
+  if (!aligned(r->turns, 8) || !aligned(r->positions, r->positions_are_int64 ? 8 : 4))
+    return fail(WP_ERR_INVALID, "%s: turns and positions must be aligned to their elements", who);
+  a.positions = r->positions;
+  a.positions64 = r->positions_are_int64 ? 1 : 0;
+  a.turns = r->turns;
+  a.rot = r->dim;
+  a.interleaved = r->interleaved ? 1 : 0;
+  a.factor = r->factor;
+  return WP_OK;
+}
+
+// Rows of a kind: heads of `x`, and where they go (y, or, null, the cache).
+int head_part(const char* who, const char* what, HeadPart& h, const void* x, const int64_t* x_strides, const void* norm,
+              void* y, const int64_t* y_strides, bool rotate, int64_t tokens, int32_t heads, int32_t dim) {
+  int64_t s[2];
+  if (const int rc = head_strides(who, what, x, x_strides, tokens, heads, dim, false, s); rc != WP_OK) return rc;
+  if (!aligned(norm, 16)) return fail(WP_ERR_INVALID, "%s: norm weights must be 16-byte aligned", who);
+  h.x = x;
+  h.x_tok = s[0];
+  h.x_head = s[1];
+  h.norm = norm;
+  h.rotate = rotate ? 1 : 0;
+  h.heads = heads;
+  if (y_strides) {
+    if (const int rc = head_strides(who, "an output", y, y_strides, tokens, heads, dim, true, s); rc != WP_OK) return rc;
+    h.y = y;
+    h.y_tok = s[0];
+    h.y_head = s[1];
+  }
+  return WP_OK;
+}
+
+// Part i of a launch goes to (or comes from) the cache's keys (1) or values (2).
+void cached_part(HeadArgs& a, int i, const wp_pages& c) {
+  HeadPart& h = a.part[i];
+  const int64_t* s = i == 1 ? c.k_strides : c.v_strides;
+  const int64_t* z = i == 1 ? c.k_scale_strides : c.v_scale_strides;
+  h.cached = 1;
+  h.y = i == 1 ? c.k : c.v;
+  h.scales = i == 1 ? c.k_scales : c.v_scales;
+  h.y_page = c.pages > 1 ? s[0] : 0;
+  h.y_tok = s[1];
+  h.y_head = c.kv_heads > 1 ? s[2] : 0;
+  h.s_page = c.pages > 1 ? z[0] : 0;
+  h.s_tok = z[1];
+  h.s_head = c.kv_heads > 1 ? z[2] : 0;
+}
+
+void cache_args(HeadArgs& a, const wp_pages& c, const void* slots, int32_t slots64) {
+  a.slots = slots;
+  a.slots64 = slots64 ? 1 : 0;
+  a.n_slots = c.pages * c.page_size;
+  a.e4m3 = c.e4m3 ? 1 : 0;
+  a.page_shift = __builtin_ctz(static_cast<unsigned>(c.page_size));
+}
+
+int check_rows(const char* who, wp_engine* e, int32_t dtype, int64_t tokens) {
+  if (!e) return fail(WP_ERR_INVALID, "%s: engine is NULL", who);
+  if (const int rc = check_dtype(who, dtype); rc != WP_OK) return rc;
+  if (tokens < 0 || tokens > 0x7FFFFFFF) return fail(WP_ERR_INVALID, "%s: %lld tokens", who, (long long)tokens);
+  return WP_OK;
+}
+
+int check_slots(const char* who, const void* slots, int32_t slots64) {
+  if (!slots) return fail(WP_ERR_INVALID, "%s: null slots", who);
+  if (!aligned(slots, slots64 ? 8 : 4)) return fail(WP_ERR_INVALID, "%s: slots must be aligned to their elements", who);
+  return WP_OK;
+}
+
+int run_rows(const char* who, wp_engine* e, HeadArgs& a, int64_t tokens, int32_t head_dim, float eps, int32_t dtype,
+             void* stream, bool read = false) {
+  // A launch numbers its waves in 31 bits; none takes less than a token's head.
+  const int64_t heads = static_cast<int64_t>(a.part[0].heads) + a.part[1].heads + a.part[2].heads;
+  if (tokens * heads > 0x7FFFFFFF) return fail(WP_ERR_INVALID, "%s: %lld heads of all tokens (up to 2^31)", who, (long long)(tokens * heads));
+  a.header = e->header;
+  a.tokens = tokens;
+  a.dim = head_dim;
+  a.eps = eps;
+  DeviceGuard g(e->device);
+  WP_HIP((read ? launch_read_rows : launch_head_rows)(dtype == WP_DTYPE_BF16, a, e->n_cu, static_cast<hipStream_t>(stream)));
+  return WP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int wp_rotate_heads(wp_engine* e, void* q_out, const int64_t* q_out_strides, const void* q, const int64_t* q_strides,
+                    void* k_out, const int64_t* k_out_strides, const void* k, const int64_t* k_strides,
+                    const void* q_norm, const void* k_norm, float eps, const wp_rotation* rotation, int64_t tokens,
+                    int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype, void* stream) {
+  const char* who = "rotate_heads";
+  if (const int rc = check_rows(who, e, dtype, tokens); rc != WP_OK) return rc;
+  if (heads < 0 || heads > 65535 || kv_heads < 0 || kv_heads > 65535)
+    return fail(WP_ERR_INVALID, "%s: %d query and %d key heads", who, heads, kv_heads);
+  if (head_dim < 8 || head_dim > kMaxRowDim || head_dim % 8 != 0)
+    return fail(WP_ERR_INVALID, "%s: head size %d (a multiple of 8 up to %d)", who, head_dim, kMaxRowDim);
+  if (tokens == 0 || heads + kv_heads == 0) return WP_OK;
+  HeadArgs a{};
+  if (const int rc = check_rotation(who, rotation, head_dim, a); rc != WP_OK) return rc;
+  if ((heads > 0 && !q_out_strides) || (kv_heads > 0 && !k_out_strides)) return fail(WP_ERR_INVALID, "%s: null strides", who);
+  if (heads > 0)
+    if (const int rc = head_part(who, "q", a.part[0], q, q_strides, q_norm, q_out, q_out_strides, rotation != nullptr, tokens, heads, head_dim);
+        rc != WP_OK)
+      return rc;
+  if (kv_heads > 0)
+    if (const int rc = head_part(who, "k", a.part[1], k, k_strides, k_norm, k_out, k_out_strides, rotation != nullptr, tokens, kv_heads, head_dim);
+        rc != WP_OK)
+      return rc;
+  return run_rows(who, e, a, tokens, head_dim, eps, dtype, stream);
+}
+
+int wp_rotate_into_cache(wp_engine* e, void* q_out, const int64_t* q_out_strides, const void* q,
+                         const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                         const int64_t* v_strides, const void* q_norm, const void* k_norm, float eps,
+                         const wp_rotation* rotation, const wp_pages* cache, const void* slots,
+                         int32_t slots_are_int64, int64_t tokens, int32_t heads, int32_t dtype, void* stream) {
+  const char* who = heads == 0 && !rotation && !k_norm ? "write_cache" : "rotate_into_cache";
+  if (const int rc = check_rows(who, e, dtype, tokens); rc != WP_OK) return rc;
+  if (heads < 0 || heads > 65535) return fail(WP_ERR_INVALID, "%s: %d query heads", who, heads);
+  if (const int rc = check_pages(who, cache, kMaxRowDim); rc != WP_OK) return rc;
+  if (tokens == 0) return WP_OK;
+  if (const int rc = check_slots(who, slots, slots_are_int64); rc != WP_OK) return rc;
+  const int32_t dim = cache->head_dim;
+  HeadArgs a{};
+  if (const int rc = check_rotation(who, rotation, dim, a); rc != WP_OK) return rc;
+  if (heads > 0) {
+    if (!q_out_strides) return fail(WP_ERR_INVALID, "%s: null strides", who);
+    if (const int rc = head_part(who, "q", a.part[0], q, q_strides, q_norm, q_out, q_out_strides, rotation != nullptr, tokens, heads, dim);
+        rc != WP_OK)
+      return rc;
+  }
+  if (const int rc = head_part(who, "k", a.part[1], k, k_strides, k_norm, nullptr, nullptr, rotation != nullptr, tokens, cache->kv_heads, dim);
+      rc != WP_OK)
+    return rc;
+  if (const int rc = head_part(who, "v", a.part[2], v, v_strides, nullptr, nullptr, nullptr, false, tokens, cache->kv_heads, dim);
+      rc != WP_OK)
+    return rc;
+  cached_part(a, 1, *cache);
+  cached_part(a, 2, *cache);
+  cache_args(a, *cache, slots, slots_are_int64);
+  return run_rows(who, e, a, tokens, dim, eps, dtype, stream);
+}
+
+int wp_write_cache(wp_engine* e, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                   const wp_pages* cache, const void* slots, int32_t slots_are_int64, int64_t tokens, int32_t dtype,
+                   void* stream) {
+  return wp_rotate_into_cache(e, nullptr, nullptr, nullptr, nullptr, k, k_strides, v, v_strides, nullptr, nullptr, 0.f,
+                              nullptr, cache, slots, slots_are_int64, tokens, 0, dtype, stream);
+}
+
+int wp_read_cache(wp_engine* e, void* k_out, const int64_t* k_out_strides, void* v_out, const int64_t* v_out_strides,
+                  const wp_pages* cache, const void* slots, int32_t slots_are_int64, int64_t tokens, int32_t dtype,
+                  void* stream) {
+  const char* who = "read_cache";
+  if (const int rc = check_rows(who, e, dtype, tokens); rc != WP_OK) return rc;
+  if (const int rc = check_pages(who, cache, kMaxRowDim); rc != WP_OK) return rc;
+  if (tokens == 0) return WP_OK;
+  if (const int rc = check_slots(who, slots, slots_are_int64); rc != WP_OK) return rc;
+  HeadArgs a{};
+  for (int i = 1; i < 3; ++i) {
+    int64_t s[2];
+    void* out = i == 1 ? k_out : v_out;
+    if (const int rc = head_strides(who, "an output", out, i == 1 ? k_out_strides : v_out_strides, tokens, cache->kv_heads, cache->head_dim,
+                                    true, s);
+        rc != WP_OK)
+      return rc;
+    cached_part(a, i, *cache);
+    HeadPart& h = a.part[i];
+    h.x = h.y;
+    h.x_tok = h.y_tok;
+    h.x_head = h.y_head;
+    h.y = out;
+    h.y_tok = s[0];
+    h.y_head = s[1];
+    h.heads = cache->kv_heads;
+  }
+  cache_args(a, *cache, slots, slots_are_int64);
+  return run_rows(who, e, a, tokens, cache->head_dim, 0.f, dtype, stream, true);
 }
 
 }  // extern "C"

@@ -1,0 +1,432 @@
+// wp_heads.hip -- rows of heads between a projection and a paged cache (gfx950):
+// norms of queries and keys, rotation by position, rows into the cache's pages
+// (in the tensors' type or e4m3) and back.
+//
+// For a row x of a head at position p, with norm weights w:
+//   n = x * w / sqrt(mean x^2 + eps)                      (x itself without)
+//   y_a = n_a cos(p f_i) - n_b sin(p f_i),  y_b = n_b cos(p f_i) + n_a sin(p f_i)
+// for the pair i of elements (a, b), all in fp32, rounded once: to the tensors'
+// type, or, into an 8-bit cache, to e4m3 of y / s, s the smallest power of two
+// that brings the row's largest magnitude to at most 448.  (A power of two costs
+// e4m3 nothing of its 4 significant bits and makes y / s and its way back exact.)
+//
+// Angles are 64-bit fractions of a turn: p * f modulo 2^64 is exact, its top 32
+// bits are the angle within 2^-32 turns, and an eighth of a turn either way is left to
+// polynomials (the Taylor series of sine to t^9 and of cosine to t^10: off by
+// at most 2e-9 there).
+//
+// What bounds it.  Prompts: HBM, each element read and written once.  Few
+// tokens: launch and the chain position, angle, row, store.  A wave takes one
+// token's heads of one kind (so that every choice by kind is its own branch),
+// 16 bytes a lane, several rows of loads at once; it computes the sines of its
+// 8 columns once for all of them.  A row stays within a wave, which has read all
+// of it before it writes: results may replace their inputs.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "wp_apply.h"
+#include "wp_device.h"
+#include "wp_paged.h"
+
+namespace wp {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kBatch = 4;  // rows of loads of a wave that are on their way together
+
+__device__ __forceinline__ uint32_t over(uint32_t n, const Divisor& d) {
+  return static_cast<uint32_t>((static_cast<uint64_t>(n) * d.magic) >> d.shift);
+}
+
+// Sum (or maximum) over the L lanes of a row, in every one of them.
+template <int L, typename F>
+__device__ __forceinline__ float over_row(float v, F f) {
+  auto moved = [](float x, auto ctrl) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xF, 0xF, true));
+  };
+  v = f(v, moved(v, std::integral_constant<int, 0xB1>{}));   // its neighbour's
+  v = f(v, moved(v, std::integral_constant<int, 0x4E>{}));   // the other two of four
+  v = f(v, moved(v, std::integral_constant<int, 0x141>{}));  // the other four of eight, reversed
+  if constexpr (L >= 16) v = f(v, moved(v, std::integral_constant<int, 0x140>{}));
+  if constexpr (L >= 32) v = f(v, __shfl_xor(v, 16));
+  return v;
+}
+
+// Cosine and sine of p * turns, times `factor`.
+__device__ __forceinline__ void turn(uint64_t p, uint64_t turns, float factor, float& c, float& s) {
+  const int32_t phase = static_cast<int32_t>(static_cast<uint32_t>((p * turns) >> 32));
+  const uint32_t quarter = (static_cast<uint32_t>(phase) + 0x20000000u) >> 30;
+  const int32_t rest = static_cast<int32_t>(static_cast<uint32_t>(phase) - (quarter << 30));  // an eighth either way
+  const float t = static_cast<float>(rest) * 1.4629180792671596e-9f;  // 2 pi / 2^32
+  const float u = t * t;
+  const float sn = fmaf(t * u, fmaf(u, fmaf(u, fmaf(u, 2.7557319e-6f, -1.9841270e-4f), 8.3333333e-3f), -1.6666667e-1f), t);
+  const float cs =
+      fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, -2.7557319e-7f, 2.4801587e-5f), -1.3888889e-3f), 4.1666667e-2f), -0.5f), 1.f);
+  const float x = quarter & 1u ? sn : cs, y = quarter & 1u ? cs : sn;
+  c = (quarter + 1u) & 2u ? -factor * x : factor * x;  // quarters 1 and 2
+  s = quarter & 2u ? -factor * y : factor * y;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack8(u32x4 q, float (&v)[8]) {
+  const auto h = __builtin_bit_cast(typename VecOf<T>::v8, q);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(h[e]);
+}
+template <typename T>
+__device__ __forceinline__ u32x4 pack8(const float (&v)[8]) {
+  typename VecOf<T>::v8 h;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) h[e] = static_cast<T>(v[e]);
+  return __builtin_bit_cast(u32x4, h);
+}
+
+// A lane's 8 elements of a row in e4m3: its bytes, and the row's scale code in
+// every lane.  The scale goes by the finite elements; infinities and magnitudes
+// that the tensors' type rounds to them become NaN, as e4m3 has none.  Where the largest magnitude would come
+// back beyond the type's range (fp16's 65504 is 256 * 2^8 in 4 significant
+// bits), it becomes the value below.
+template <typename T, int L>
+__device__ __forceinline__ u32x2 quantise(const float (&y)[8], uint32_t& code) {
+  constexpr bool kHalf = __is_same(T, _Float16);
+  constexpr float kPast = kHalf ? 65520.f : 0x1.FFp127f;  // rounds to infinity
+  constexpr int kTopScale = kHalf ? 8 : 120;              // 2^this * 256 is past the type's range
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = fabsf(y[e]) < kPast ? fmaxf(top, fabsf(y[e])) : top;
+  top = over_row<L>(top, [](float a, float b) { return fmaxf(a, b); });
+  const uint32_t bits = __builtin_bit_cast(uint32_t, top);
+  // 448 = 1.75 * 2^8.
+  int x = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  x = std::clamp(x, -126, 127);
+  code = static_cast<uint32_t>(x + 127);
+  const float most = x >= kTopScale ? 240.f : 448.f;
+  float z[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float s = __builtin_ldexpf(y[e], -x);
+    z[e] = fabsf(y[e]) < kPast ? std::clamp(s, -most, most) : __builtin_nanf("");
+  }
+  u32x2 r{0u, 0u};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * h], z[4 * h + 1], 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * h + 2], z[4 * h + 3], w, true);
+    r[h] = static_cast<uint32_t>(w);
+  }
+  return r;
+}
+
+// The unit of this wave.
+struct Unit {
+  int64_t tok;
+  int kind, head0;
+};
+template <int kRows>
+__device__ __forceinline__ bool unit_of(const HeadArgs& p, Unit& u) {
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const uint32_t id = blockIdx.x * kWaves + wave;
+  if (id >= p.n_units) return false;
+  const uint32_t tok = over(id, p.by_units);
+  int at = static_cast<int>(id - tok * static_cast<uint32_t>(p.units_tok));
+  u.tok = tok;
+  u.kind = at < p.units[0] ? 0 : at < p.units[0] + p.units[1] ? 1 : 2;
+  at -= u.kind == 0 ? 0 : u.kind == 1 ? p.units[0] : p.units[0] + p.units[1];
+  u.head0 = at * p.steps * kRows;
+  return true;
+}
+
+// Entry i of int64 or int32 numbers.
+__device__ __forceinline__ int64_t number(const void* p, int wide, int64_t i) {
+  return wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+}
+
+template <typename T, int L>
+__global__ __launch_bounds__(64 * kWaves) void head_rows_kernel(HeadArgs p) {
+  constexpr int kRows = 64 / L;
+  touch_kernel_args<static_cast<int>(sizeof(HeadArgs))>();
+  Unit u;
+  if (!unit_of<kRows>(p, u)) return;
+  // (Selected field by field: a pointer to an argument would move them all to memory.)
+  auto mine = [&](auto f) { return u.kind == 0 ? f(p.part[0]) : u.kind == 1 ? f(p.part[1]) : f(p.part[2]); };
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  const int d0 = lane % L * 8, dim = p.dim, heads = mine([](const HeadPart& h) { return h.heads; });
+  const bool holds = d0 < dim;
+  const T* x = static_cast<const T*>(mine([](const HeadPart& h) { return h.x; })) +
+               u.tok * mine([](const HeadPart& h) { return h.x_tok; });
+  const int64_t x_head = mine([](const HeadPart& h) { return h.x_head; });
+  const T* w = static_cast<const T*>(mine([](const HeadPart& h) { return h.norm; }));
+  const bool cached = mine([](const HeadPart& h) { return h.cached; }) != 0;
+  const bool rotates = mine([](const HeadPart& h) { return h.rotate; }) != 0;
+
+  // Where results go.
+  char* y = static_cast<char*>(mine([](const HeadPart& h) { return h.y; }));
+  uint8_t* scales = mine([](const HeadPart& h) { return h.scales; });
+  const int64_t y_tok = mine([](const HeadPart& h) { return h.y_tok; }), y_head = mine([](const HeadPart& h) { return h.y_head; });
+  const int64_t s_head = mine([](const HeadPart& h) { return h.s_head; });
+  const bool small = cached && p.e4m3 != 0;
+  if (cached) {
+    const int64_t slot = number(p.slots, p.slots64, u.tok);
+    if (slot < 0) return;
+    if (slot >= p.n_slots) {
+      if (lane == 0 && u.head0 == 0) flag_error(p.header, kErrIdRange);
+      return;
+    }
+    const int64_t page = slot >> p.page_shift, at = slot & ((1ll << p.page_shift) - 1);
+    y += (page * mine([](const HeadPart& h) { return h.y_page; }) + at * y_tok) * (small ? 1 : 2);
+    if (small) scales += page * mine([](const HeadPart& h) { return h.s_page; }) + at * mine([](const HeadPart& h) { return h.s_tok; });
+  } else {
+    y += u.tok * y_tok * 2;
+  }
+
+  // The lane's columns: sines, and where each one's partner is.
+  const int rot = rotates ? p.rot : 0, half = rot >> 1;
+  const bool apart = rot > 0 && p.interleaved == 0;  // the partner is half a rotation away
+  const bool vectors = (half & 7) == 0;              // ... in one 16-byte vector
+  const int partner = d0 < half ? d0 + half : d0 - half;
+  float cs[8], sn[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    cs[e] = 1.f;
+    sn[e] = 0.f;
+  }
+  if (rot > 0 && d0 < rot) {
+    const uint64_t pos = static_cast<uint64_t>(number(p.positions, p.positions64, u.tok));
+    if (apart) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int d = d0 + e;
+        if (d >= rot) continue;
+        float c, s;
+        turn(pos, static_cast<uint64_t>(p.turns[d < half ? d : d - half]), p.factor, c, s);
+        cs[e] = c;
+        sn[e] = d < half ? -s : s;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        if (d0 + e >= rot) continue;
+        float c, s;
+        turn(pos, static_cast<uint64_t>(p.turns[(d0 + e) >> 1]), p.factor, c, s);
+        cs[e] = cs[e + 1] = c;
+        sn[e] = -s;
+        sn[e + 1] = s;
+      }
+    }
+  }
+  // The partners of eight columns, zero where there are none.
+  auto partners = [&](const T* row, float (&v)[8]) {
+    if (vectors) {
+      unpack8<T>(d0 < rot ? load16_global(row + partner) : u32x4{0u, 0u, 0u, 0u}, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int d = d0 + e;
+        v[e] = d < rot ? static_cast<float>(row[d < half ? d + half : d - half]) : 0.f;
+      }
+    }
+  };
+  float wn[8], wo[8];
+  if (w != nullptr) {
+    unpack8<T>(holds ? load16_global(w + d0) : u32x4{0u, 0u, 0u, 0u}, wn);
+    if (apart) partners(w, wo);
+  }
+
+  const int row = lane / L;
+  const float inv_dim = 1.f / static_cast<float>(dim);
+  for (int step = 0; step < p.steps && u.head0 + step * kRows < heads; step += kBatch) {
+    u32x4 in[kBatch];
+    float other[kBatch][8];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int h = u.head0 + (step + i) * kRows + row;
+      const bool live = holds && h < heads && step + i < p.steps;
+      in[i] = live ? load16_global(x + h * x_head + d0) : u32x4{0u, 0u, 0u, 0u};
+    }
+    if (apart) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int h = u.head0 + (step + i) * kRows + row;
+        const bool live = holds && h < heads && step + i < p.steps;
+        if (live) {
+          partners(x + h * x_head, other[i]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) other[i][e] = 0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int h = u.head0 + (step + i) * kRows + row;
+      const bool live = holds && h < heads && step + i < p.steps;
+      float v[8];
+      unpack8<T>(in[i], v);
+      if (w != nullptr) {
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
+        sum = over_row<L>(sum, [](float a, float b) { return a + b; });
+        const float r = 1.f / sqrtf(fmaf(sum, inv_dim, p.eps));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = v[e] * r * wn[e];
+        if (apart) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) other[i][e] = other[i][e] * r * wo[e];
+        }
+      }
+      if (rot > 0) {
+        float z[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float o = apart ? other[i][e] : d0 + e < rot ? v[e ^ 1] : 0.f;
+          z[e] = fmaf(v[e], cs[e], o * sn[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = z[e];
+      }
+      if (small) {
+        uint32_t code;
+        const u32x2 q = quantise<T, L>(v, code);
+        if (live) {
+          *reinterpret_cast<u32x2*>(y + h * y_head + d0) = q;
+          if (d0 == 0) scales[h * s_head] = static_cast<uint8_t>(code);
+        }
+      } else if (live) {
+        *reinterpret_cast<u32x4*>(y + (h * y_head + d0) * 2) = pack8<T>(v);
+      }
+    }
+  }
+}
+
+// Rows of the cache, as the tensors' type: a factor outside fp32's normal
+// numbers (codes 0 and 255, which nothing here writes) gives zero and NaN.
+template <typename T, int L, bool kSmall>
+__global__ __launch_bounds__(64 * kWaves) void read_rows_kernel(HeadArgs p) {
+  constexpr int kRows = 64 / L;
+  touch_kernel_args<static_cast<int>(sizeof(HeadArgs))>();
+  Unit u;
+  if (!unit_of<kRows>(p, u)) return;
+  auto mine = [&](auto f) { return u.kind == 0 ? f(p.part[0]) : u.kind == 1 ? f(p.part[1]) : f(p.part[2]); };
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  const int d0 = lane % L * 8, heads = mine([](const HeadPart& h) { return h.heads; });
+  const bool holds = d0 < p.dim;
+  const int64_t slot = number(p.slots, p.slots64, u.tok);
+  const bool there = slot >= 0 && slot < p.n_slots;
+  if (slot >= p.n_slots && lane == 0 && u.head0 == 0) flag_error(p.header, kErrIdRange);
+  const int64_t page = there ? slot >> p.page_shift : 0, at = there ? slot & ((1ll << p.page_shift) - 1) : 0;
+  constexpr int kSize = kSmall ? 1 : 2;
+  const char* x = static_cast<const char*>(mine([](const HeadPart& h) { return h.x; })) +
+                  (page * mine([](const HeadPart& h) { return h.y_page; }) + at * mine([](const HeadPart& h) { return h.x_tok; })) * kSize;
+  const uint8_t* scales = mine([](const HeadPart& h) { return h.scales; });
+  if (kSmall) scales += page * mine([](const HeadPart& h) { return h.s_page; }) + at * mine([](const HeadPart& h) { return h.s_tok; });
+  const int64_t x_head = mine([](const HeadPart& h) { return h.x_head; }), s_head = mine([](const HeadPart& h) { return h.s_head; });
+  T* y = static_cast<T*>(mine([](const HeadPart& h) { return h.y; })) + u.tok * mine([](const HeadPart& h) { return h.y_tok; });
+  const int64_t y_head = mine([](const HeadPart& h) { return h.y_head; });
+  const int row = lane / L;
+  for (int step = 0; step < p.steps && u.head0 + step * kRows < heads; step += kBatch) {
+    u32x4 in[kBatch];
+    uint32_t code[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int h = u.head0 + (step + i) * kRows + row;
+      const bool live = there && holds && h < heads && step + i < p.steps;
+      in[i] = u32x4{0u, 0u, 0u, 0u};
+      code[i] = 1u;
+      if (live) {
+        if constexpr (kSmall) {
+          const u32x2 q = *reinterpret_cast<const u32x2*>(x + h * x_head + d0);
+          in[i][0] = q[0];
+          in[i][1] = q[1];
+          code[i] = scales[h * s_head];
+        } else {
+          in[i] = load16_global(x + (h * x_head + d0) * 2);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int h = u.head0 + (step + i) * kRows + row;
+      if (!(holds && h < heads && step + i < p.steps)) continue;
+      if constexpr (kSmall) {
+        const float s = __builtin_bit_cast(float, code[i] << 23);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(in[i][e / 4]), false);
+          const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(in[i][e / 4]), true);
+          v[e] = a[0] * s;
+          v[e + 1] = a[1] * s;
+          v[e + 2] = b[0] * s;
+          v[e + 3] = b[1] * s;
+        }
+        *reinterpret_cast<u32x4*>(y + h * y_head + d0) = pack8<T>(v);
+      } else {
+        *reinterpret_cast<u32x4*>(y + h * y_head + d0) = in[i];
+      }
+    }
+  }
+}
+
+// Splits each token's heads of each kind into units of `steps` wave-wide rows:
+// one unit if there are tokens enough, else as many as keep the device's
+// waves busy.
+bool plan_units(HeadArgs& a, int lanes, int n_cu) {
+  const int rows = 64 / lanes;
+  int most = 1;
+  for (const HeadPart& h : a.part) most = std::max(most, (h.heads + rows - 1) / rows);
+  int64_t steps = most;
+  // At least eight waves a compute unit, in units of one batch or more.
+  while (steps > kBatch && a.tokens * ((most + steps - 1) / steps) < 8ll * n_cu) steps = std::max<int64_t>(kBatch, steps / 2);
+  a.steps = static_cast<int32_t>(steps);
+  a.units_tok = 0;
+  for (int i = 0; i < 3; ++i) {
+    a.units[i] = static_cast<int32_t>((a.part[i].heads + steps * rows - 1) / (steps * rows));
+    a.units_tok += a.units[i];
+  }
+  const int64_t n = a.tokens * a.units_tok;
+  if (n > 0x7FFFFFFF) return false;
+  a.n_units = static_cast<uint32_t>(n);
+  a.by_units = divisor_of(a.units_tok);
+  return true;
+}
+
+}  // namespace
+
+hipError_t launch_head_rows(int dtype_bf16, HeadArgs& a, int n_cu, hipStream_t stream) {
+  const int lanes = a.dim <= 64 ? 8 : a.dim <= 128 ? 16 : 32;
+  if (!plan_units(a, lanes, n_cu)) return hipErrorInvalidValue;
+  const dim3 grid((a.n_units + kWaves - 1) / kWaves), block(64 * kWaves);
+  auto go = [&](auto* kernel) {
+    hipLaunchKernelGGL(kernel, grid, block, 0, stream, a);
+    return hipGetLastError();
+  };
+  if (dtype_bf16)
+    return lanes == 8 ? go(head_rows_kernel<__bf16, 8>) : lanes == 16 ? go(head_rows_kernel<__bf16, 16>) : go(head_rows_kernel<__bf16, 32>);
+  return lanes == 8 ? go(head_rows_kernel<_Float16, 8>) : lanes == 16 ? go(head_rows_kernel<_Float16, 16>) : go(head_rows_kernel<_Float16, 32>);
+}
+
+namespace {
+template <typename T, bool kSmall>
+hipError_t read_rows(const HeadArgs& a, int lanes, hipStream_t stream) {
+  const dim3 grid((a.n_units + kWaves - 1) / kWaves), block(64 * kWaves);
+  if (lanes == 8)
+    hipLaunchKernelGGL((read_rows_kernel<T, 8, kSmall>), grid, block, 0, stream, a);
+  else if (lanes == 16)
+    hipLaunchKernelGGL((read_rows_kernel<T, 16, kSmall>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((read_rows_kernel<T, 32, kSmall>), grid, block, 0, stream, a);
+  return hipGetLastError();
+}
+}  // namespace
+
+hipError_t launch_read_rows(int dtype_bf16, HeadArgs& a, int n_cu, hipStream_t stream) {
+  const int lanes = a.dim <= 64 ? 8 : a.dim <= 128 ? 16 : 32;
+  if (!plan_units(a, lanes, n_cu)) return hipErrorInvalidValue;
+  if (dtype_bf16) return a.e4m3 ? read_rows<__bf16, true>(a, lanes, stream) : read_rows<__bf16, false>(a, lanes, stream);
+  return a.e4m3 ? read_rows<_Float16, true>(a, lanes, stream) : read_rows<_Float16, false>(a, lanes, stream);
+}
+
+}  // namespace wp

@@ -56,6 +56,14 @@ struct Divisor {
   uint32_t magic;
   int32_t shift;
 };
+// Exact for every dividend under 2^31: the quotient's error is under
+// dividend / 2^shift * d < 1 / d of a step.
+inline Divisor divisor_of(int d) {
+  Divisor r{0, 31};
+  while ((1ll << (r.shift - 31)) < d) ++r.shift;
+  r.magic = static_cast<uint32_t>(((1ull << r.shift) + static_cast<uint64_t>(d) - 1) / static_cast<uint64_t>(d));
+  return r;
+}
 
 struct AttnArgs {
   const void* q;

@@ -895,6 +895,210 @@ class WarpPipeEngine:
         _lib.check(rc, "token_logprobs")
         return got
 
+    # ------------------------------------------- heads and a paged cache --
+    # What lies between a decoder's qkv projection and its attention over a
+    # cache in pages (not in the reference, whose models run it in vLLM).
+
+    def _heads_of(self, t, what: str, op: str, dtype, dim: int):
+        """Checks of a [tokens, heads, dim] tensor."""
+        if t.get_device() != self._dev_index:
+            self._on_device(t, what)
+        if t.dtype != dtype:
+            raise RuntimeError(f"{op}: {what} must be {dtype}, got {t.dtype}")
+        if t.dim() != 3 or t.size(2) != dim:
+            raise RuntimeError(f"{op}: {what} must be [tokens, heads, {dim}], got {tuple(t.shape)}")
+        if dim > 1 and t.stride(2) != 1:
+            raise RuntimeError(f"{op}: a head's elements of {what} must be contiguous")
+
+    def _head_norm(self, w, what: str, op: str, dtype, dim: int):
+        if w is None:
+            return None
+        if w.get_device() != self._dev_index:
+            self._on_device(w, what)
+        if w.dtype != dtype or w.shape != (dim,) or (dim > 1 and w.stride(0) != 1):
+            raise RuntimeError(f"{op}: {what} must be a contiguous [{dim}] tensor of {dtype}")
+        return w.data_ptr()
+
+    def _rotation(self, rotary, positions, tokens: int, op: str):
+        """The C struct wp_rotation as bytes, or None."""
+        if rotary is None:
+            return None
+        turns = rotary.turns
+        if turns.get_device() != self._dev_index:
+            self._on_device(turns, "rotary")
+        if positions is None:
+            raise RuntimeError(f"{op}: rotating needs positions")
+        if positions.get_device() != self._dev_index:
+            self._on_device(positions, "positions")
+        if positions.dtype not in (torch.int64, torch.int32) or positions.shape != (tokens,) or (
+                tokens > 1 and positions.stride(0) != 1):
+            raise RuntimeError(f"{op}: positions must be a contiguous int32 or int64 [{tokens}] tensor")
+        return struct.pack("2Q3if", turns.data_ptr(), positions.data_ptr(), 1 if positions.dtype == torch.int64 else 0,
+                           rotary.dim, 1 if rotary.interleaved else 0, rotary.factor)
+
+    def _pages(self, k_pages, v_pages, k_scales, v_scales, dtype, op: str):
+        """The C struct wp_pages as bytes."""
+        kept = k_pages.dtype
+        if k_pages.get_device() != self._dev_index or v_pages.get_device() != self._dev_index:
+            self._on_device(k_pages, "k_pages")
+            self._on_device(v_pages, "v_pages")
+        if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != kept:
+            raise RuntimeError(f"{op}: k_pages and v_pages must be [pages, page_size, kv_heads, dim] tensors of one dtype; "
+                               f"got {tuple(k_pages.shape)} {kept}, {tuple(v_pages.shape)} {v_pages.dtype}")
+        small = kept == torch.float8_e4m3fn
+        if not small and kept != dtype:
+            raise RuntimeError(f"{op}: pages must be {dtype} or float8_e4m3fn, got {kept}")
+        pages, size, heads, dim = k_pages.shape
+        ks, vs = k_pages.stride(), v_pages.stride()
+        if dim > 1 and (ks[3] != 1 or vs[3] != 1):
+            raise RuntimeError(f"{op}: a head's elements of the pages must be contiguous")
+        if not small:
+            if k_scales is not None or v_scales is not None:
+                raise RuntimeError(f"{op}: scales belong to float8_e4m3fn pages")
+            return struct.pack("4Q13q4i", k_pages.data_ptr(), v_pages.data_ptr(), 0, 0, *ks[:3], *vs[:3], 0, 0, 0, 0, 0, 0,
+                               pages, size, heads, dim, 0)
+        for t, nm in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+            if t is None:
+                raise RuntimeError(f"{op}: float8_e4m3fn pages need {nm}")
+            if t.get_device() != self._dev_index:
+                self._on_device(t, nm)
+            if t.dtype != torch.uint8 or t.shape != k_pages.shape[:3]:
+                raise RuntimeError(f"{op}: {nm} must be a uint8 {tuple(k_pages.shape[:3])} tensor")
+        return struct.pack("4Q13q4i", k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+                           *ks[:3], *vs[:3], *k_scales.stride(), *v_scales.stride(), pages, size, heads, dim, 1)
+
+    def _slots(self, slots, tokens: int, op: str) -> int:
+        if slots.get_device() != self._dev_index:
+            self._on_device(slots, "slots")
+        if slots.dtype not in (torch.int64, torch.int32) or slots.shape != (tokens,) or (tokens > 1 and slots.stride(0) != 1):
+            raise RuntimeError(f"{op}: slots must be a contiguous int32 or int64 [{tokens}] tensor")
+        return 1 if slots.dtype == torch.int64 else 0
+
+    def rotate_heads(self, q, k, positions, rotary, q_norm=None, k_norm=None, eps=1e-6, q_out=None, k_out=None):
+        """Every head of q [tokens, heads, dim] and k [tokens, kv_heads, dim] (or
+        None) divided by its root mean square and times q_norm / k_norm [dim]
+        where those are given, then turned by its token's position as `rotary`
+        (rotary.Rotary; None: not at all) says; one launch, in fp32, rounded
+        once.  dim: a multiple of 8 up to 256; q and k may be views with other
+        token and head strides (multiples of 8).  positions [tokens] int32 or
+        int64, any values.  Returns (q_out, k_out), new unless given; either may
+        be its input."""
+        op = "rotate_heads"
+        dtype = q.dtype
+        dt = _DTYPES.get(dtype)
+        if dt is None:
+            dt = _dtype_code(q, "q")
+        dim = q.size(-1) if q.dim() == 3 else 0
+        self._heads_of(q, "q", op, dtype, dim)
+        T, heads = q.size(0), q.size(1)
+        q_out = self._head_out(q_out, q, "q_out", op)
+        kv_heads = 0
+        kp = ko = ks = kos = None
+        if k is not None:
+            self._heads_of(k, "k", op, dtype, dim)
+            if k.size(0) != T:
+                raise RuntimeError(f"{op}: q has {T} tokens, k has {k.size(0)}")
+            kv_heads = k.size(1)
+            k_out = self._head_out(k_out, k, "k_out", op)
+            kp, ko, ks, kos = k.data_ptr(), k_out.data_ptr(), _i64s(k.stride()[:2]), _i64s(k_out.stride()[:2])
+        rc = self._lib.wp_rotate_heads(
+            self._handle, q_out.data_ptr(), _i64s(q_out.stride()[:2]), q.data_ptr(), _i64s(q.stride()[:2]), ko, kos, kp, ks,
+            self._head_norm(q_norm, "q_norm", op, dtype, dim), self._head_norm(k_norm, "k_norm", op, dtype, dim), eps,
+            self._rotation(rotary, positions, T, op), T, heads, kv_heads, dim, dt, _raw_stream(self._dev_index))
+        _lib.check(rc, op)
+        return q_out, (None if k is None else k_out)
+
+    def _head_out(self, out, like, what: str, op: str):
+        if out is None:
+            return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        self._heads_of(out, what, op, like.dtype, like.size(2))
+        if out.shape != like.shape:
+            raise RuntimeError(f"{op}: {what} must be {tuple(like.shape)}, got {tuple(out.shape)}")
+        return out
+
+    def rotate_into_cache(self, q, k, v, positions, rotary, k_pages, v_pages, slots, k_scales=None, v_scales=None,
+                          q_norm=None, k_norm=None, eps=1e-6, q_out=None):
+        """rotate_heads(q, k) and write_cache(k, v) in one launch: the turned keys
+        and the values go to slots[token] of the cache (see write_cache), the
+        turned queries are returned (q_out, new unless given; it may be q).  q
+        may be None.  Keys go into a float8_e4m3fn cache without being rounded
+        to their own type first."""
+        op = "rotate_into_cache"
+        dtype = k.dtype
+        dt = _DTYPES.get(dtype)
+        if dt is None:
+            dt = _dtype_code(k, "k")
+        cache = self._pages(k_pages, v_pages, k_scales, v_scales, dtype, op)
+        kv_heads, dim = k_pages.size(2), k_pages.size(3)
+        T = self._kv_rows(k, v, kv_heads, dim, dtype, op)
+        heads = 0
+        qp = qo = qs = qos = None
+        if q is not None:
+            self._heads_of(q, "q", op, dtype, dim)
+            if q.size(0) != T:
+                raise RuntimeError(f"{op}: q has {q.size(0)} tokens, k has {T}")
+            heads = q.size(1)
+            q_out = self._head_out(q_out, q, "q_out", op)
+            qp, qo, qs, qos = q.data_ptr(), q_out.data_ptr(), _i64s(q.stride()[:2]), _i64s(q_out.stride()[:2])
+        rc = self._lib.wp_rotate_into_cache(
+            self._handle, qo, qos, qp, qs, k.data_ptr(), _i64s(k.stride()[:2]), v.data_ptr(), _i64s(v.stride()[:2]),
+            self._head_norm(q_norm, "q_norm", op, dtype, dim), self._head_norm(k_norm, "k_norm", op, dtype, dim), eps,
+            self._rotation(rotary, positions, T, op), cache, slots.data_ptr(), self._slots(slots, T, op), T, heads, dt,
+            _raw_stream(self._dev_index))
+        _lib.check(rc, op)
+        return None if q is None else q_out
+
+    def _kv_rows(self, k, v, kv_heads: int, dim: int, dtype, op: str) -> int:
+        self._heads_of(k, "k", op, dtype, dim)
+        self._heads_of(v, "v", op, dtype, dim)
+        if k.size(1) != kv_heads or v.shape != k.shape:
+            raise RuntimeError(f"{op}: k and v must be [tokens, {kv_heads}, {dim}], got {tuple(k.shape)} and {tuple(v.shape)}")
+        return k.size(0)
+
+    def write_cache(self, k, v, k_pages, v_pages, slots, k_scales=None, v_scales=None) -> None:
+        """Rows k and v [tokens, kv_heads, dim] to slots[token] (int32 or int64) of
+        the cache, which is k_pages and v_pages [pages, page_size, kv_heads, dim]
+        (page_size a power of two from 16 on; any page, token and head strides:
+        pages may lie head by head); slot s is token s % page_size of page s //
+        page_size.  Pages have the rows' type, or are float8_e4m3fn with k_scales
+        and v_scales [pages, page_size, kv_heads] uint8: a row's elements are then
+        e4m3 * 2^(byte - 127), the smallest such power that brings the row's largest
+        magnitude to at most 448.  A negative slot keeps no row; one past the
+        cache is skipped and sets device error 1.  Slots of a call must differ."""
+        op = "write_cache"
+        dtype = k.dtype
+        dt = _DTYPES.get(dtype)
+        if dt is None:
+            dt = _dtype_code(k, "k")
+        cache = self._pages(k_pages, v_pages, k_scales, v_scales, dtype, op)
+        T = self._kv_rows(k, v, k_pages.size(2), k_pages.size(3), dtype, op)
+        rc = self._lib.wp_write_cache(self._handle, k.data_ptr(), _i64s(k.stride()[:2]), v.data_ptr(),
+                                      _i64s(v.stride()[:2]), cache, slots.data_ptr(), self._slots(slots, T, op), T, dt,
+                                      _raw_stream(self._dev_index))
+        _lib.check(rc, op)
+
+    def read_cache(self, k_pages, v_pages, slots, k_scales=None, v_scales=None, dtype=None):
+        """The cache's rows of slots [tokens]: (k, v), each [tokens, kv_heads, dim],
+        in the pages' type, or of float8_e4m3fn pages as what they stand for, in
+        dtype (bf16 unless given).  Rows of a negative slot are zero, and so are
+        those of one past the cache, which sets device error 1."""
+        op = "read_cache"
+        kept = k_pages.dtype
+        if dtype is None:
+            dtype = torch.bfloat16 if kept == torch.float8_e4m3fn else kept
+        dt = _DTYPES.get(dtype)
+        if dt is None:
+            raise RuntimeError(f"{op}: rows are read as fp16 or bf16, not {dtype}")
+        cache = self._pages(k_pages, v_pages, k_scales, v_scales, dtype, op)
+        T = slots.numel()
+        k = torch.empty((T,) + k_pages.shape[2:], dtype=dtype, device=k_pages.device)
+        v = torch.empty_like(k)
+        rc = self._lib.wp_read_cache(self._handle, k.data_ptr(), _i64s(k.stride()[:2]), v.data_ptr(), _i64s(v.stride()[:2]),
+                                     cache, slots.data_ptr(), self._slots(slots, T, op), T, dt,
+                                     _raw_stream(self._dev_index))
+        _lib.check(rc, op)
+        return k, v
+
     # ------------------------------------------------------------- staging --
     def prefetch_adapter(self, adapter_id, layer=None) -> int:
         """Stages the adapter's A/B in a slot on the prefetch stream; returns the

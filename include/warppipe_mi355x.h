@@ -395,6 +395,77 @@ int wp_token_logprobs(wp_engine* e, float* logprobs, float* entropy, int32_t* ra
                       int32_t* top_ids, const void* logits, int64_t logits_row_stride, const void* token_ids,
                       int32_t ids_are_int64, int64_t rows, int32_t vocab, int32_t top, int32_t dtype, void* stream);
 
+/* ---- heads and a paged cache ---------------------------------------------
+ * What lies between a decoder's qkv projection and its attention over a cache
+ * in pages (no reference counterpart).  Tensors are fp16 or bf16, a head's
+ * elements contiguous and 16-byte aligned; strides in elements, multiples of 8
+ * and not negative (any where there is one token or head). */
+
+/* How a head's first `dim` elements (even, up to the head) turn: by
+ * positions[token] * turns[i] / 2^64 turns for the pair i, (i, i + dim / 2) or,
+ * interleaved, (2 i, 2 i + 1); cosine and sine times factor.  Products are
+ * modulo 2^64, so every position, negative ones too, has its exact angle. */
+typedef struct wp_rotation {
+  const int64_t* turns;        /* [dim / 2], device */
+  const void* positions;       /* [tokens], device */
+  int32_t positions_are_int64; /* else int32 */
+  int32_t dim;
+  int32_t interleaved;
+  float factor;
+} wp_rotation;
+
+/* A cache of `pages` pages of page_size tokens (a power of two from 16 on): the
+ * row of head h of slot s is at k + (s / page_size) * strides[0] + (s % page_size)
+ * * strides[1] + h * strides[2], head_dim contiguous elements of the calls'
+ * dtype or, with e4m3, bytes (strides then multiples of 16, as head_dim), with
+ * a byte b in the scales for each row: its elements are e4m3 * 2^(b - 127). */
+typedef struct wp_pages {
+  void* k;
+  void* v;
+  uint8_t* k_scales; /* e4m3 only */
+  uint8_t* v_scales;
+  int64_t k_strides[3], v_strides[3];             /* page, token, head */
+  int64_t k_scale_strides[3], v_scale_strides[3]; /* any but negative */
+  int64_t pages;
+  int32_t page_size, kv_heads, head_dim, e4m3;
+} wp_pages;
+
+/* q_out and k_out: every head of q [tokens, heads] and k [tokens, kv_heads]
+ * divided by its root mean square (of mean + eps) times q_norm / k_norm
+ * [head_dim] where that is given, then turned by `rotation` where that is
+ * given; in fp32, rounded once.  head_dim: a multiple of 8 up to 256.  Either
+ * kind may have no heads.  An output may be its input, else they must not overlap. */
+int wp_rotate_heads(wp_engine* e, void* q_out, const int64_t* q_out_strides, const void* q, const int64_t* q_strides,
+                    void* k_out, const int64_t* k_out_strides, const void* k, const int64_t* k_strides,
+                    const void* q_norm, const void* k_norm, float eps, const wp_rotation* rotation, int64_t tokens,
+                    int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype, void* stream);
+
+/* The same in one launch with the keys going to slots[token] of the cache, and
+ * the values v as they are.  Into an e4m3 cache a row (keys unrounded) is divided
+ * by the smallest power of two s >= 2^-126 that brings its largest magnitude to
+ * at most 448 and rounded to nearest even; magnitudes that would come back past
+ * the dtype's range take the largest that does not, infinities and NaN become NaN.  A
+ * negative slot keeps no row; one past the cache is skipped and flagged (device
+ * error 1).  Slots of one call must differ (else either row, or parts of both,
+ * remain).  heads may be 0. */
+int wp_rotate_into_cache(wp_engine* e, void* q_out, const int64_t* q_out_strides, const void* q,
+                         const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                         const int64_t* v_strides, const void* q_norm, const void* k_norm, float eps,
+                         const wp_rotation* rotation, const wp_pages* cache, const void* slots,
+                         int32_t slots_are_int64, int64_t tokens, int32_t heads, int32_t dtype, void* stream);
+
+/* Keys and values as they are to slots[token] of the cache. */
+int wp_write_cache(wp_engine* e, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                   const wp_pages* cache, const void* slots, int32_t slots_are_int64, int64_t tokens, int32_t dtype,
+                   void* stream);
+
+/* The rows of slots[token], in dtype (e4m3 times its factor, rounded once): k_out
+ * and v_out [tokens, kv_heads, head_dim].  Rows of a negative slot are zero, and
+ * so are those of one past the cache, which is flagged (device error 1). */
+int wp_read_cache(wp_engine* e, void* k_out, const int64_t* k_out_strides, void* v_out, const int64_t* v_out_strides,
+                  const wp_pages* cache, const void* slots, int32_t slots_are_int64, int64_t tokens, int32_t dtype,
+                  void* stream);
+
 /* ---- staging / prefetch ---------------------------------------------------- */
 
 /* Replaces WarpPipeExtension::prefetch_adapter (bindings:46-57): copies the
