@@ -37,72 +37,18 @@
 #include <type_traits>
 
 #include "wp_apply.h"
+#include "wp_attn_core.h"
 #include "wp_device.h"
 #include "wp_model.h"
 
 namespace wp {
 namespace {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef short i16x4 __attribute__((ext_vector_type(4)));
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.69314718055994531f;
-constexpr int kWaveRows = 32;
-constexpr int kTileKeys = 64;                  // keys staged at a time for a row tile
 constexpr int kChunkWaves = 4;
 constexpr int kChunkRows = kWaveRows * kChunkWaves;  // most query rows of a sequence that runs on key chunks
 constexpr int kChunkKeys = 32;                 // keys a wave stages at a time for a key chunk
-// A running bound is raised (and O and l scaled) only once a score exceeds it
-// by 2^8: exponentials then stay within 2^8, far inside fp16, and most tiles
-// scale nothing.
-constexpr float kSlack = 8.f;
 constexpr int kTiles = 1, kChunks = 2;  // the roles of a launch
 constexpr int kNoSplit = 31;  // keys per split as a power of two: past every length
-
-__device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
-
-template <typename T>
-__device__ __forceinline__ typename VecOf<T>::v8 negate8(typename VecOf<T>::v8 v) {
-  const u32x4 u = __builtin_bit_cast(u32x4, v);
-  return __builtin_bit_cast(typename VecOf<T>::v8, u ^ 0x80008000u);
-}
-
-// Which of two 16-bit values are infinite or NaN are cleared.
-template <typename T>
-__device__ __forceinline__ bool finite16(uint32_t half) {
-  constexpr uint32_t e = sizeof(T) == 2 && __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;
-  return (half & e) != e;
-}
-template <typename T>
-__device__ __forceinline__ i16x4 finite_only(i16x4 v) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = finite16<T>(static_cast<uint16_t>(v[i])) ? v[i] : static_cast<short>(0);
-  return v;
-}
-
-// Head columns computed (DP, a multiple of 32) and how a row of K or V lies in
-// LDS: 128 or 256 bytes in 16-byte chunks, columns past the head zero.
-//   K row r keeps chunk c at c ^ key_swizzle(r): the rows that a fragment load touches at one c
-//   fall on different banks.
-//   V row r keeps chunk c at c ^ value_swizzle(r): the transposing read takes 64
-//   bytes of each of eight rows, which so fall on different banks too.
-template <int DP>
-struct Head {
-  static constexpr int kRow = DP <= 64 ? 128 : 256;
-  static constexpr int kChunks = kRow / 16;
-  static constexpr int kRowsPerLoad = 1024 / kRow;  // rows a wave's 16-byte-per-lane load fills
-  static constexpr int kSteps = DP / 16;            // contraction steps of S
-  static constexpr int kCols = DP / 32;             // 32-column tiles of O
-  static __device__ __forceinline__ int key_swizzle(int r) { return kRow == 256 ? r & 15 : (r >> 1) & 7; }
-  static __device__ __forceinline__ int value_swizzle(int r) { return kRow == 256 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
-};
 
 // One work item.
 struct Item {
@@ -121,10 +67,6 @@ struct Item {
 struct Span {
   int q0, k0, n_q, n_k;
 };
-// n / d, exactly for n < 2^31: the product is under 2^63.
-__device__ __forceinline__ int over(int n, const Divisor& d) {
-  return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * d.magic) >> d.shift);
-}
 __device__ __forceinline__ Span span_of(const AttnArgs& p, int b) {
   Span s;
   const int q0 = p.cu_q[b], q1 = p.cu_q[b + 1], k0 = p.cu_k[b], k1 = p.cu_k[b + 1];
@@ -134,12 +76,6 @@ __device__ __forceinline__ Span span_of(const AttnArgs& p, int b) {
   s.k0 = std::clamp(k0, 0, keys);
   s.n_k = std::clamp(k1, s.k0, keys) - s.k0;
   return s;
-}
-
-// The first key that a query at key position `pos` sees: with the windows the
-// host takes, up to 2^31 - 1, pos - window + 1 need not fit 32 bits.
-__device__ __forceinline__ int window_start(int pos, int window) {
-  return window > 0 ? std::max(0, std::max(0, pos + 1) - window) : 0;
 }
 
 // Keys that rows [row, row + rows) of a sequence see: [first, end).
@@ -172,19 +108,6 @@ __device__ __forceinline__ int items_of(const AttnArgs& p, const Span& s, bool r
   *tiles = (rows + tile_rows - 1) / tile_rows;
   return *tiles * chunks;
 }
-
-// The sum of v over the lanes up to this one, by lane moves within the vector
-// unit (a shuffle goes through LDS and takes some ten times as long).
-__device__ __forceinline__ int sum_up(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // from 1 lane down, in rows of 16
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);  // 2
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);  // 4
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);  // 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true);  // the row before's last lane
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true);  // the first half's last lane
-  return v;
-}
-__device__ __forceinline__ int total_of(int v) { return __builtin_amdgcn_readlane(sum_up(v), 63); }
 
 __device__ __forceinline__ Item item_of(const AttnArgs& p, const Span& s, int lane, int head, int id, int seq, int tile, int chunk, int n_tiles,
                                         int first_tile) {
@@ -281,123 +204,6 @@ __device__ __forceinline__ Item find_item(const AttnArgs& p, bool rows_role, int
   return none;
 }
 
-// A wave's 32 query rows and their running state.
-template <typename T, int DP>
-struct Rows {
-  using H = Head<DP>;
-  using V8 = typename VecOf<T>::v8;
-  V8 q[H::kSteps];
-  f32x16 o[H::kCols];
-  float m;      // running bound, in units of c * s
-  float l;      // this lane's keys' sum
-  int pos;      // key position of the lane's query (causal), else the last key
-  int low;      // first key it sees
-
-  __device__ __forceinline__ void reset() {
-#pragma unroll
-    for (int i = 0; i < H::kCols; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
-    m = -INFINITY;
-    l = 0.f;
-  }
-
-  // Raises the bound where a score exceeds it by the slack (tops: the lane's
-  // largest score of the tile).
-  __device__ __forceinline__ void raise(float tops, float c) {
-    const float t = tops * c;
-    if (__any(t > m + kSlack)) {
-      const float top = fmaxf(fmaxf(t, __shfl_xor(t, 32)), m);
-      const float fade = top == -INFINITY ? 1.f : exp2_fast(m - top);
-      m = top;
-      l *= fade;
-#pragma unroll
-      for (int i = 0; i < H::kCols; ++i) o[i] *= fade;
-    }
-  }
-
-  // Scores of keys [at, at + 32) that the lane's query does not see become -inf.
-  __device__ __forceinline__ void mask(f32x16& s, int at) {
-    const int first = at + ((static_cast<int>(threadIdx.x) & 63) >> 5) * 4;
-    const int up = pos - first, down = low - first;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int key = (e >> 2) * 8 + (e & 3);
-      s[e] = key <= up && key >= down ? s[e] : -INFINITY;
-    }
-  }
-};
-
-__device__ __forceinline__ float top_of(const f32x16& s) {
-  float t = fmaxf(s[0], s[1]);
-#pragma unroll
-  for (int e = 2; e < 16; e += 2) t = fmaxf(fmaxf(t, s[e]), s[e + 1]);
-  return t;
-}
-
-// K fragment of step `step`: keys row0 .. row0 + 31 of a staged tile.
-template <typename T, int DP>
-__device__ __forceinline__ typename VecOf<T>::v8 key_fragment(const char* keys, int row0, int step) {
-  using H = Head<DP>;
-  const int lane = static_cast<int>(threadIdx.x) & 63;
-  const int r = lane & 31, c = step * 2 + (lane >> 5);
-  return *reinterpret_cast<const typename VecOf<T>::v8*>(keys + (row0 + r) * H::kRow + ((c ^ H::key_swizzle(r)) << 4));
-}
-
-// V^T fragment of columns col * 32 .. + 31 and the 16 keys from key0, in the
-// order of the packed exponentials: lane half h has keys 4h .. 4h + 3 and
-// 8 + 4h .. 8 + 4h + 3.
-template <typename T, int DP, bool kCareful>
-__device__ __forceinline__ typename VecOf<T>::v8 value_fragment(const char* values, int key0, int col) {
-  using H = Head<DP>;
-  const int lane = static_cast<int>(threadIdx.x) & 63;
-  const int i = lane & 15, g = lane >> 4;
-  const int r = 4 * (g >> 1) + (i >> 2);
-  const int c = col * 4 + (g & 1) * 2 + ((i & 3) >> 1);
-  const int at = (key0 + r) * H::kRow + ((c ^ H::value_swizzle(r)) << 4) + (i & 1) * 8;
-  using L = __attribute__((address_space(3))) i16x4;
-  i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(values + at));
-  i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(values + (at + 8 * H::kRow)));
-  if (kCareful) {
-    lo = finite_only<T>(lo);
-    hi = finite_only<T>(hi);
-  }
-  union {
-    i16x4 h[2];
-    typename VecOf<T>::v8 v;
-  } u;
-  u.h[0] = lo;
-  u.h[1] = hi;
-  return u.v;
-}
-
-// Adds the infinite and NaN values of keys [at, at + n) that a query sees,
-// which value_fragment<careful> left out.
-template <typename T, int DP>
-__device__ __forceinline__ void add_nonfinite(Rows<T, DP>& w, const char* values, int at, int n) {
-  using H = Head<DP>;
-  const int lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
-  for (int r = 0; r < n; ++r) {
-    const char* row = values + r * H::kRow;
-    bool odd = false;
-    if (lane < H::kRow / 4) {
-      const uint32_t u = *reinterpret_cast<const uint32_t*>(row + lane * 4);
-      odd = !finite16<T>(u & 0xFFFFu) || !finite16<T>(u >> 16);
-    }
-    if (!__any(odd)) continue;
-    const bool sees = at + r <= w.pos && at + r >= w.low;
-#pragma unroll
-    for (int i = 0; i < H::kCols; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int d = i * 32 + (e >> 2) * 8 + half * 4 + (e & 3);
-        const int c = (d >> 3) ^ H::value_swizzle(r);
-        const uint16_t u = *reinterpret_cast<const uint16_t*>(row + c * 16 + (d & 7) * 2);
-        if (sees && !finite16<T>(u)) w.o[i][e] += static_cast<float>(__builtin_bit_cast(T, u));
-      }
-  }
-}
-
 // Staging: load i of a wave fills rows (first + i) * kRowsPerLoad on of a tile
 // straight in LDS, 16 bytes a lane.  A lane's offsets from the tile's first row
 // are the same for every tile; the rows past the tile's last one and the
@@ -426,75 +232,6 @@ struct Loads {
   }
 };
 
-template <typename T>
-__device__ __forceinline__ const T* head_row(const void* base, int64_t tok, int64_t tok_stride, int64_t head_offset) {
-  return static_cast<const T*>(base) + tok * tok_stride + head_offset;
-}
-
-// Exponentials of a 32-key tile, added to the lane's sum in fp32 and packed: the
-// two right operands of its two 16-key steps.  The matrix cores take 16-bit
-// operands: each weight is rounded to the tensors' type, once, so that O is off
-// by at most half a unit of that type of sum p |v| -- what rounding the values
-// themselves did.
-template <typename T, int DP>
-__device__ __forceinline__ void weigh(Rows<T, DP>& w, const f32x16& s, float c, typename VecOf<T>::v8 (&out)[2]) {
-  const float base = w.m == -INFINITY ? 0.f : w.m;
-#pragma unroll
-  for (int b = 0; b < 2; ++b)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float x = exp2_fast(fmaf(s[b * 8 + e], c, -base));
-      w.l += x;
-      out[b][e] = static_cast<T>(x);
-    }
-}
-
-// Scores of 32 staged keys from row0 on; LDS reads go four products ahead.
-template <typename T, int DP>
-__device__ __forceinline__ f32x16 scores(const Rows<T, DP>& w, const char* keys, int row0) {
-  constexpr int kSteps = Head<DP>::kSteps;
-  typename VecOf<T>::v8 kf[4];
-#pragma unroll
-  for (int x = 0; x < 4; ++x) kf[x] = key_fragment<T, DP>(keys, row0, x);
-  __builtin_amdgcn_sched_barrier(0);
-  f32x16 s{};
-#pragma unroll
-  for (int x = 0; x < kSteps; ++x) {
-    s = mfma32(kf[x % 4], w.q[x], s);
-    if (x + 4 < kSteps) kf[x % 4] = key_fragment<T, DP>(keys, row0, x + 4);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  return s;
-}
-
-// Adds 32 staged keys' weighted values to O.
-template <typename T, int DP, bool kCareful>
-__device__ __forceinline__ void accumulate(Rows<T, DP>& w, const char* values, int row0,
-                                           const typename VecOf<T>::v8 (&e)[2]) {
-  constexpr int kCols = Head<DP>::kCols, kAhead = kCols < 4 ? kCols : 4;
-  auto value = [&](int i) { return value_fragment<T, DP, kCareful>(values, row0 + i / kCols * 16, i % kCols); };
-  typename VecOf<T>::v8 vf[kAhead];
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) vf[i] = value(i);
-  if (!kCareful) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-  for (int i = 0; i < 2 * kCols; ++i) {
-    w.o[i % kCols] = mfma32(vf[i % kAhead], e[i / kCols], w.o[i % kCols]);
-    if (i + kAhead < 2 * kCols) vf[i % kAhead] = value(i + kAhead);
-    if (!kCareful) __builtin_amdgcn_sched_barrier(0);
-  }
-}
-
-// LDS of a workgroup.  Each buffer is an array of its own: the compiler then
-// sees that a load into one leaves reads of the others alone, and does not wait
-// for it.
-template <int DP>
-struct Staged {
-  static constexpr int kBytes = kTileKeys * Head<DP>::kRow;
-};
-#define WP_STAGED char (&sk0)[Staged<DP>::kBytes], char (&sk1)[Staged<DP>::kBytes], char (&sv0)[Staged<DP>::kBytes], \
-                  char (&sv1)[Staged<DP>::kBytes]
-
 // Row tile: the keys [first, end) for the workgroup's rows, 64 at a time.
 // While tile j is weighed and added, the scores of tile j + 1 are computed
 // (they need nothing of it, so the matrix cores work beside the exponentials), and tiles j + 2
@@ -503,7 +240,6 @@ template <typename T, int DP, int kWaves>
 __device__ __forceinline__ void run_tile(const AttnArgs& p, const Item& it, Rows<T, DP>& w, float c, int first, int end,
                                          int wave_low, int wave_pos, int wave_last, int wave, WP_STAGED) {
   using H = Head<DP>;
-  using V8 = typename VecOf<T>::v8;
   constexpr int kLoads = kTileKeys * H::kRow / 1024 / kWaves;
   const T* k = head_row<T>(p.k, it.k0, p.k_tok, it.head * p.k_head);
   const T* v = head_row<T>(p.v, it.k0, p.v_tok, it.head * p.v_head);
@@ -528,15 +264,7 @@ __device__ __forceinline__ void run_tile(const AttnArgs& p, const Item& it, Rows
   f32x16 s0 = scores(w, sk0, 0), s1 = scores(w, sk0, 32);
   constexpr std::integral_constant<bool, true> yes{};
   constexpr std::integral_constant<bool, false> no{};
-  // The order of a tile's work is pinned so that products and vector work run
-  // side by side throughout (two waves a SIMD in the same phase would else wait
-  // for the one unit together and leave the other idle):
-  //   the first half's exponentials between three quarters of the next tile's scores,
-  //   the second half's between the rest of them and the first half's products with V,
-  //   the next scores' maximum between the second half's products with V.
-  // LDS reads go two products ahead.
   float tops = fmaxf(top_of(s0), top_of(s1));
-  constexpr int kScores = 2 * H::kSteps, kFirst = kScores * 3 / 4, kValues = 2 * H::kCols;
   auto body = [&](int at, auto more, const char* knext, const char* vnow) {
     // wave_low, wave_pos: the keys that every row of the wave sees.
     if (at < wave_low || at + kTileKeys - 1 > wave_pos) {
@@ -544,71 +272,7 @@ __device__ __forceinline__ void run_tile(const AttnArgs& p, const Item& it, Rows
       w.mask(s1, at + 32);
       tops = fmaxf(top_of(s0), top_of(s1));
     }
-    w.raise(tops, c);
-    const float base = w.m == -INFINITY ? 0.f : w.m;
-    auto weigh = [&](f32x16& s, int from, int to) {
-#pragma unroll
-      for (int i = from; i < to; ++i) {
-        s[i] = exp2_fast(fmaf(s[i], c, -base));
-        w.l += s[i];
-      }
-    };
-    auto key = [&](int i) { return key_fragment<T, DP>(knext, i / H::kSteps * 32, i % H::kSteps); };
-    auto value = [&](int i) { return value_fragment<T, DP, false>(vnow, i / H::kCols * 16, i % H::kCols); };
-    f32x16 n[2] = {};
-    V8 kf[3], vf[3], e[4];
-    if (more) {
-      kf[0] = key(0);
-      kf[1] = key(1);
-    }
-    auto score = [&](int i) {
-      n[i / H::kSteps] = mfma32(kf[i % 3], w.q[i % H::kSteps], n[i / H::kSteps]);
-      if (i + 2 < kScores) kf[(i + 2) % 3] = key(i + 2);
-    };
-    auto add = [&](int i) {
-      f32x16& o = w.o[i % H::kCols];
-      o = mfma32(vf[i % 3], e[i / H::kCols], o);
-      if (i + 2 < 2 * kValues) vf[(i + 2) % 3] = value(i + 2);
-    };
-    auto pack = [&](const f32x16& s, int to) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) e[to + i / 8][i % 8] = static_cast<T>(s[i]);
-    };
-#pragma unroll
-    for (int i = 0; i < kFirst; ++i) {
-      if (more) score(i);
-      weigh(s0, i * 16 / kFirst, (i + 1) * 16 / kFirst);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    pack(s0, 0);
-    vf[0] = value(0);
-    vf[1] = value(1);
-    constexpr int kSecond = kScores - kFirst + kValues;
-#pragma unroll
-    for (int i = 0; i < kSecond; ++i) {
-      if (i < kScores - kFirst) {
-        if (more) score(kFirst + i);
-      } else {
-        add(i - (kScores - kFirst));
-      }
-      weigh(s1, i * 16 / kSecond, (i + 1) * 16 / kSecond);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    pack(s1, 2);
-#pragma unroll
-    for (int i = 0; i < kValues; ++i) {
-      add(kValues + i);
-      if (more) {
-#pragma unroll
-        for (int x = i * 16 / kValues; x < (i + 1) * 16 / kValues; ++x)
-          tops = x == 0 ? fmaxf(n[0][0], n[1][0]) : fmaxf(fmaxf(tops, n[0][x]), n[1][x]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if (more) {
-      s0 = n[0];
-      s1 = n[1];
-    }
+    tile_body(w, s0, s1, tops, c, more, knext, vnow);
   };
   auto step = [&](int at, char* kfree, const char* knext, const char* vnow, char* vnext) {
     wait_vm();
@@ -657,7 +321,7 @@ __device__ __forceinline__ void run_tile_careful(const AttnArgs& p, const Item& 
     weigh(w, s1, c, e1);
     accumulate<T, DP, true>(w, sv, 0, e0);
     accumulate<T, DP, true>(w, sv, 32, e1);
-    add_nonfinite(w, sv, at, kTileKeys);
+    add_nonfinite(w, sv, kTileKeys, [&](int r) { return at + r <= w.pos && at + r >= w.low; });
   }
 }
 
@@ -700,21 +364,11 @@ __device__ __forceinline__ void run_chunk(const ChunkLoads<T, DP>& in, Rows<T, D
     weigh(w, s, c, e);
     wait_vm_but<kLoads>();
     accumulate<T, DP, kCareful>(w, in.sv, 0, e);
-    if (kCareful) add_nonfinite(w, in.sv, at, kChunkKeys);
+    if (kCareful) add_nonfinite(w, in.sv, kChunkKeys, [&](int r) { return at + r <= w.pos && at + r >= w.low; });
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     in.load_v(next);
   }
   wait_vm();
-}
-
-template <typename T, int DP>
-__device__ __forceinline__ bool has_nonfinite(const Rows<T, DP>& w) {
-  float z = 0.f;
-#pragma unroll
-  for (int i = 0; i < Head<DP>::kCols; ++i)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) z = fmaf(w.o[i][e], 0.f, z);
-  return z != 0.f;  // NaN: an infinity or NaN times zero
 }
 
 // Writes four columns of a finished row (and with the first of them its lse).
