@@ -50,6 +50,7 @@ EXPORTED = (
     "wp_add_bias", "wp_handoff_probe", "wp_barrier_probe", "wp_shrink_new",
     "wp_linear", "wp_packed_attention", "wp_token_logprobs",
     "wp_rotate_heads", "wp_rotate_into_cache", "wp_write_cache", "wp_read_cache",
+    "wp_paged_attention",
 )
 
 
@@ -134,6 +135,7 @@ def load():
         "wp_rotate_into_cache": ([p, p, p, p, p, p, p, p, p, p, p, f32, p, p, p, i32, i64, i32, i32, p], ctypes.c_int),
         "wp_write_cache": ([p, p, p, p, p, p, p, i32, i64, i32, p], ctypes.c_int),
         "wp_read_cache": ([p, p, p, p, p, p, p, i32, i64, i32, p], ctypes.c_int),
+        "wp_paged_attention": ([p, p, p, p, p, p, p, p, i64, i32, p, p, i32, i64, i32, f32, i32, i32, i32, p], ctypes.c_int),
         "wp_barrier_probe": ([p, i32, i32, i32, p, p], ctypes.c_int),
     }
     for name, (args, res) in sig.items():

@@ -19,7 +19,7 @@ OBJ_DIR = os.path.join(CSRC, "_build")
 LIB_NAME = "libwarppipe_mi355x.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 SOURCES = ["wp_plan.hip", "wp_apply.hip", "wp_aux.hip", "wp_proj.hip", "wp_attn.hip",
-           "wp_logprobs.hip", "wp_heads.hip", "wp_engine.hip"]
+           "wp_logprobs.hip", "wp_heads.hip", "wp_paged.hip", "wp_engine.hip"]
 ARCH = os.environ.get("WP_OFFLOAD_ARCH", "gfx950")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

@@ -92,9 +92,21 @@ __device__ __forceinline__ int sum_up(int v) {
 }
 __device__ __forceinline__ int total_of(int v) { return __builtin_amdgcn_readlane(sum_up(v), 63); }
 
+// The lane that a wave's work goes by: the thread's own number or (kHeld) one
+// that a kernel keeps, in a form that the compiler takes for a number of that moment alone.
+template <bool kHeld>
+struct Lane {
+  __device__ __forceinline__ int lane() const { return static_cast<int>(threadIdx.x) & 63; }
+};
+template <>
+struct Lane<true> {
+  int held;
+  __device__ __forceinline__ int lane() const { return held; }
+};
+
 // A wave's 32 query rows and their running state.
-template <typename T, int DP>
-struct Rows {
+template <typename T, int DP, bool kHeld = false>
+struct Rows : Lane<kHeld> {
   using H = Head<DP>;
   using V8 = typename VecOf<T>::v8;
   V8 q[H::kSteps];
@@ -129,7 +141,7 @@ struct Rows {
 
   // Scores of keys [at, at + 32) that the lane's query does not see become -inf.
   __device__ __forceinline__ void mask(f32x16& s, int at) {
-    const int first = at + ((static_cast<int>(threadIdx.x) & 63) >> 5) * 4;
+    const int first = at + (this->lane() >> 5) * 4;
     const int up = pos - first, down = low - first;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
@@ -148,9 +160,8 @@ __device__ __forceinline__ float top_of(const f32x16& s) {
 
 // K fragment of step `step`: keys row0 .. row0 + 31 of a staged tile.
 template <typename T, int DP>
-__device__ __forceinline__ typename VecOf<T>::v8 key_fragment(const char* keys, int row0, int step) {
+__device__ __forceinline__ typename VecOf<T>::v8 key_fragment(const char* keys, int row0, int step, int lane) {
   using H = Head<DP>;
-  const int lane = static_cast<int>(threadIdx.x) & 63;
   const int r = lane & 31, c = step * 2 + (lane >> 5);
   return *reinterpret_cast<const typename VecOf<T>::v8*>(keys + (row0 + r) * H::kRow + ((c ^ H::key_swizzle(r)) << 4));
 }
@@ -159,9 +170,8 @@ __device__ __forceinline__ typename VecOf<T>::v8 key_fragment(const char* keys, 
 // order of the packed exponentials: lane half h has keys 4h .. 4h + 3 and
 // 8 + 4h .. 8 + 4h + 3.
 template <typename T, int DP, bool kCareful>
-__device__ __forceinline__ typename VecOf<T>::v8 value_fragment(const char* values, int key0, int col) {
+__device__ __forceinline__ typename VecOf<T>::v8 value_fragment(const char* values, int key0, int col, int lane) {
   using H = Head<DP>;
-  const int lane = static_cast<int>(threadIdx.x) & 63;
   const int i = lane & 15, g = lane >> 4;
   const int r = 4 * (g >> 1) + (i >> 2);
   const int c = col * 4 + (g & 1) * 2 + ((i & 3) >> 1);
@@ -184,10 +194,10 @@ __device__ __forceinline__ typename VecOf<T>::v8 value_fragment(const char* valu
 
 // Adds the infinite and NaN values of n staged keys that a query sees (sees(r):
 // the lane's of key r), which value_fragment<careful> left out.
-template <typename T, int DP, typename Sees>
-__device__ __forceinline__ void add_nonfinite(Rows<T, DP>& w, const char* values, int n, Sees sees_key) {
+template <typename T, int DP, bool kHeld, typename Sees>
+__device__ __forceinline__ void add_nonfinite(Rows<T, DP, kHeld>& w, const char* values, int n, Sees sees_key) {
   using H = Head<DP>;
-  const int lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
+  const int lane = w.lane(), half = lane >> 5;
   for (int r = 0; r < n; ++r) {
     const char* row = values + r * H::kRow;
     bool odd = false;
@@ -219,8 +229,8 @@ __device__ __forceinline__ const T* head_row(const void* base, int64_t tok, int6
 // operands: each weight is rounded to the tensors' type, once, so that O is off
 // by at most half a unit of that type of sum p |v| -- what rounding the values
 // themselves did.
-template <typename T, int DP>
-__device__ __forceinline__ void weigh(Rows<T, DP>& w, const f32x16& s, float c, typename VecOf<T>::v8 (&out)[2]) {
+template <typename T, int DP, bool kHeld>
+__device__ __forceinline__ void weigh(Rows<T, DP, kHeld>& w, const f32x16& s, float c, typename VecOf<T>::v8 (&out)[2]) {
   const float base = w.m == -INFINITY ? 0.f : w.m;
 #pragma unroll
   for (int b = 0; b < 2; ++b)
@@ -233,29 +243,29 @@ __device__ __forceinline__ void weigh(Rows<T, DP>& w, const f32x16& s, float c, 
 }
 
 // Scores of 32 staged keys from row0 on; LDS reads go four products ahead.
-template <typename T, int DP>
-__device__ __forceinline__ f32x16 scores(const Rows<T, DP>& w, const char* keys, int row0) {
+template <typename T, int DP, bool kHeld>
+__device__ __forceinline__ f32x16 scores(const Rows<T, DP, kHeld>& w, const char* keys, int row0) {
   constexpr int kSteps = Head<DP>::kSteps;
   typename VecOf<T>::v8 kf[4];
 #pragma unroll
-  for (int x = 0; x < 4; ++x) kf[x] = key_fragment<T, DP>(keys, row0, x);
+  for (int x = 0; x < 4; ++x) kf[x] = key_fragment<T, DP>(keys, row0, x, w.lane());
   __builtin_amdgcn_sched_barrier(0);
   f32x16 s{};
 #pragma unroll
   for (int x = 0; x < kSteps; ++x) {
     s = mfma32(kf[x % 4], w.q[x], s);
-    if (x + 4 < kSteps) kf[x % 4] = key_fragment<T, DP>(keys, row0, x + 4);
+    if (x + 4 < kSteps) kf[x % 4] = key_fragment<T, DP>(keys, row0, x + 4, w.lane());
     __builtin_amdgcn_sched_barrier(0);
   }
   return s;
 }
 
 // Adds 32 staged keys' weighted values to O.
-template <typename T, int DP, bool kCareful>
-__device__ __forceinline__ void accumulate(Rows<T, DP>& w, const char* values, int row0,
+template <typename T, int DP, bool kCareful, bool kHeld>
+__device__ __forceinline__ void accumulate(Rows<T, DP, kHeld>& w, const char* values, int row0,
                                            const typename VecOf<T>::v8 (&e)[2]) {
   constexpr int kCols = Head<DP>::kCols, kAhead = kCols < 4 ? kCols : 4;
-  auto value = [&](int i) { return value_fragment<T, DP, kCareful>(values, row0 + i / kCols * 16, i % kCols); };
+  auto value = [&](int i) { return value_fragment<T, DP, kCareful>(values, row0 + i / kCols * 16, i % kCols, w.lane()); };
   typename VecOf<T>::v8 vf[kAhead];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) vf[i] = value(i);
@@ -278,8 +288,8 @@ __device__ __forceinline__ void accumulate(Rows<T, DP>& w, const char* values, i
 //
 // Weighs and adds the 64 staged keys whose masked scores are s0 and s1 (tops: the
 // lane's largest of them) and, with `more`, computes the next tile's into their place.
-template <typename T, int DP, typename More>
-__device__ __forceinline__ void tile_body(Rows<T, DP>& w, f32x16& s0, f32x16& s1, float& tops, float c, More more,
+template <typename T, int DP, bool kHeld, typename More>
+__device__ __forceinline__ void tile_body(Rows<T, DP, kHeld>& w, f32x16& s0, f32x16& s1, float& tops, float c, More more,
                                           const char* knext, const char* vnow) {
   using H = Head<DP>;
   using V8 = typename VecOf<T>::v8;
@@ -293,8 +303,8 @@ __device__ __forceinline__ void tile_body(Rows<T, DP>& w, f32x16& s0, f32x16& s1
       w.l += s[i];
     }
   };
-  auto key = [&](int i) { return key_fragment<T, DP>(knext, i / H::kSteps * 32, i % H::kSteps); };
-  auto value = [&](int i) { return value_fragment<T, DP, false>(vnow, i / H::kCols * 16, i % H::kCols); };
+  auto key = [&](int i) { return key_fragment<T, DP>(knext, i / H::kSteps * 32, i % H::kSteps, w.lane()); };
+  auto value = [&](int i) { return value_fragment<T, DP, false>(vnow, i / H::kCols * 16, i % H::kCols, w.lane()); };
   f32x16 n[2] = {};
   V8 kf[3], vf[3], e[4];
   if (more) {
@@ -361,8 +371,8 @@ struct Staged {
 #define WP_STAGED char (&sk0)[Staged<DP>::kBytes], char (&sk1)[Staged<DP>::kBytes], char (&sv0)[Staged<DP>::kBytes], \
                   char (&sv1)[Staged<DP>::kBytes]
 
-template <typename T, int DP>
-__device__ __forceinline__ bool has_nonfinite(const Rows<T, DP>& w) {
+template <typename T, int DP, bool kHeld>
+__device__ __forceinline__ bool has_nonfinite(const Rows<T, DP, kHeld>& w) {
   float z = 0.f;
 #pragma unroll
   for (int i = 0; i < Head<DP>::kCols; ++i)

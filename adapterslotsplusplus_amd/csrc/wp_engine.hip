@@ -2704,7 +2704,9 @@ int check_pages(const char* who, const wp_pages* c, int32_t most_dim) {
   if (c->e4m3)
     for (const int64_t* s : {c->k_scale_strides, c->v_scale_strides})
       for (int i = 0; i < 3; ++i)
-        if (sizes[i] > 1 && s[i] < 1) return fail(WP_ERR_INVALID, "%s: scales overlap (stride %lld)", who, (long long)s[i]);
+        if (sizes[i] > 1 && (s[i] < 1 || (i == 1 && s[i] > kMaxKeyStride)))
+          return fail(WP_ERR_INVALID, "%s: scales overlap, or a page's are more than %lld apart (stride %lld)", who, (long long)kMaxKeyStride,
+                      (long long)s[i]);
   return WP_OK;
 }
 
@@ -2892,6 +2894,90 @@ int wp_read_cache(wp_engine* e, void* k_out, const int64_t* k_out_strides, void*
   }
   cache_args(a, *cache, slots, slots_are_int64);
   return run_rows(who, e, a, tokens, cache->head_dim, 0.f, dtype, stream, true);
+}
+
+int wp_paged_attention(wp_engine* e, void* out, const int64_t* out_strides, float* lse, const void* q,
+                       const int64_t* q_strides, const wp_pages* cache, const int32_t* block_table,
+                       int64_t table_row_stride, int32_t columns, const int32_t* cu_q, const int32_t* kv_lens,
+                       int32_t n_seq, int64_t tokens, int32_t heads, float scale, int32_t window, int32_t sinks,
+                       int32_t dtype, void* stream) {
+  const char* who = "paged_attention";
+  if (const int rc = check_rows(who, e, dtype, tokens); rc != WP_OK) return rc;
+  if (const int rc = check_pages(who, cache, kMaxHeadDim); rc != WP_OK) return rc;
+  const int32_t kv_heads = cache->kv_heads, dim = cache->head_dim;
+  if (heads < 1 || heads > 65535 || heads % kv_heads != 0)
+    return fail(WP_ERR_INVALID, "%s: %d query heads do not share %d key heads evenly", who, heads, kv_heads);
+  const int group = heads / kv_heads;
+  if (n_seq < 0 || columns < 0) return fail(WP_ERR_INVALID, "%s: bad sizes (sequences %d, columns %d)", who, n_seq, columns);
+  if (tokens * group > 0x7FFF0000)
+    return fail(WP_ERR_INVALID, "%s: %lld tokens of %d query heads a key head (up to 2^31 rows)", who, (long long)tokens, group);
+  if (window < 0 || sinks < 0 || (sinks > 0 && window == 0))
+    return fail(WP_ERR_INVALID, "%s: a window must be positive, and only with one have first keys to stay in sight", who);
+  if (tokens == 0) return WP_OK;
+  int64_t qs[2], os[2];
+  if (const int rc = head_strides(who, "q", q, q_strides, tokens, heads, dim, false, qs); rc != WP_OK) return rc;
+  if (const int rc = head_strides(who, "out", out, out_strides, tokens, heads, dim, true, os); rc != WP_OK) return rc;
+  if (n_seq > 0 && (!cu_q || !kv_lens || (columns > 0 && !block_table))) return fail(WP_ERR_INVALID, "%s: null tensor", who);
+  if (!aligned(lse, 4) || !aligned(cu_q, 4) || !aligned(kv_lens, 4) || !aligned(block_table, 4))
+    return fail(WP_ERR_INVALID, "%s: bounds, lengths and block_table must be 4-byte aligned", who);
+  if (n_seq > 1 && table_row_stride < 0) return fail(WP_ERR_INVALID, "%s: negative table row stride", who);
+  DeviceGuard g(e->device);
+  if (const int rc = model_scratch(e, who); rc != WP_OK) return rc;
+  PagedArgs a{};
+  const int size = cache->e4m3 ? 1 : 2;
+  const bool many = cache->pages > 1, more = kv_heads > 1;
+  a.q = q;
+  a.out = out;
+  a.lse = lse;
+  a.k = static_cast<const char*>(cache->k);
+  a.v = static_cast<const char*>(cache->v);
+  a.table = block_table;
+  a.cu_q = cu_q;
+  a.kv_lens = kv_lens;
+  a.q_tok = qs[0];
+  a.q_head = qs[1];
+  a.o_tok = os[0];
+  a.o_head = os[1];
+  a.k_page = many ? cache->k_strides[0] * size : 0;
+  a.v_page = many ? cache->v_strides[0] * size : 0;
+  a.k_tok = static_cast<int32_t>(cache->k_strides[1] * size);
+  a.v_tok = static_cast<int32_t>(cache->v_strides[1] * size);
+  a.k_head = more ? cache->k_strides[2] * size : 0;
+  a.v_head = more ? cache->v_strides[2] * size : 0;
+  if (cache->e4m3) {
+    a.k_scales = cache->k_scales;
+    a.v_scales = cache->v_scales;
+    a.ks_page = many ? cache->k_scale_strides[0] : 0;
+    a.vs_page = many ? cache->v_scale_strides[0] : 0;
+    a.ks_tok = static_cast<int32_t>(cache->k_scale_strides[1]);
+    a.vs_tok = static_cast<int32_t>(cache->v_scale_strides[1]);
+    a.ks_head = more ? cache->k_scale_strides[2] : 0;
+    a.vs_head = more ? cache->v_scale_strides[2] : 0;
+  }
+  a.tokens = tokens;
+  a.table_row = n_seq > 1 ? table_row_stride : 0;
+  a.n_pages = static_cast<int32_t>(cache->pages);
+  a.page_shift = __builtin_ctz(static_cast<unsigned>(cache->page_size));
+  a.capacity = static_cast<int32_t>(std::min<int64_t>(static_cast<int64_t>(columns) << a.page_shift, 0x7FFFFF00));
+  a.n_seq = n_seq;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.dim = dim;
+  a.e4m3 = cache->e4m3 ? 1 : 0;
+  a.scale = scale;
+  a.window = window;
+  a.sinks = sinks;
+  a.part = e->mpart;
+  a.part_bytes = kModelPartBytes;
+  a.counters = e->model_cnt;
+  a.n_counters = kModelCounters;
+  a.header = e->header;
+  const hipError_t rc = launch_paged_attention(dtype == WP_DTYPE_BF16, a, e->n_cu, static_cast<hipStream_t>(stream));
+  if (rc == hipErrorInvalidValue)
+    return fail(WP_ERR_INVALID, "%s: %lld tokens of %d heads over tables for %d keys are too large for one call", who, (long long)tokens, heads,
+                a.capacity);
+  WP_HIP(rc);
+  return WP_OK;
 }
 
 }  // extern "C"

@@ -50,4 +50,43 @@ hipError_t launch_head_rows(int dtype_bf16, HeadArgs& a, int n_cu, hipStream_t s
 // cache's strides between pages; y by token and head.
 hipError_t launch_read_rows(int dtype_bf16, HeadArgs& a, int n_cu, hipStream_t stream);
 
+// Attention of new tokens over the cache: sequence b's queries are rows
+// [cu_q[b], cu_q[b + 1]) of q, its keys the first kv_lens[b] tokens of the pages
+// table[b * table_row ..]; its last query stands at its last key.  A query sees the
+// keys up to its own position and, with a window, only the last `window` of
+// them and the first `sinks` of all.  out and lse as packed attention's.
+struct PagedArgs {
+  const void* q;
+  void* out;
+  float* lse;  // or null
+  const char* k;
+  const char* v;
+  const uint8_t* k_scales;
+  const uint8_t* v_scales;
+  const int32_t* table;
+  const int32_t* cu_q;
+  const int32_t* kv_lens;
+  int64_t q_tok, q_head, o_tok, o_head;
+  int64_t k_page, k_head, v_page, v_head;      // bytes
+  int64_t ks_page, ks_head, vs_page, vs_head;
+  int64_t tokens, table_row;
+  int32_t k_tok, v_tok, ks_tok, vs_tok;        // bytes
+  int32_t n_pages, page_shift, capacity;       // capacity: most keys of a sequence
+  int32_t n_seq, heads, kv_heads, dim, e4m3;
+  float scale;
+  int32_t window, sinks;
+  float* part;         // partials of sequences that several workgroups share
+  uint64_t part_bytes;
+  uint32_t* counters;  // zero between calls
+  int32_t n_counters;
+  uint32_t* header;    // the plan header, whose error word is flagged
+  // Filled by launch_paged_attention.
+  int32_t group;       // query heads of a key head
+  Divisor by_group;
+  int32_t chunk_rows;  // most rows per key head of a sequence that runs on key chunks
+  int32_t n_wg;
+  double per_wg;       // 1 / n_wg
+};
+hipError_t launch_paged_attention(int dtype_bf16, PagedArgs& a, int n_cu, hipStream_t stream);
+
 }  // namespace wp

@@ -1,0 +1,965 @@
+// wp_paged.hip -- attention of new tokens over a paged cache (gfx950): grouped
+// heads, causal, optional window with the first keys kept in sight, keys and
+// values in 16 bits or e4m3 with a power of two per row, fp32 statistics.
+//
+//   out_i = sum_j 2^(c s_ij - m_i) v_j / l_i,   l_i = sum_j 2^(c s_ij - m_i)
+// over the keys j that row i sees, s = q . k, c = scale * log2(e), m_i a running
+// bound of c s_ij: one pass over the keys, by the tiles of wp_attn_core.h.
+//
+// Lengths are known on the device alone, and a table has room for far more keys
+// than there are.  So a launch has two workgroups for each compute unit, and
+// each works out its share by itself: the cost of every row tile (32 or 128 rows
+// of a key head) in keys is a linear function of the tile, cut off below and at
+// the window, whose sum over a sequence has a closed form; the line of all tiles'
+// costs is cut into equal shares, wherever that is.  A tile that several workgroups
+// share is joined by the last of them to finish (by a counter of steps done), so
+// each key is read once, by one workgroup, and all end at about the same time.
+//
+// Two roles.  Tiles of 128 rows: four waves of 32 rows, 64 keys and values at a
+// time staged in LDS for all of them.  Up to 32 rows (single tokens, drafted
+// tokens): the waves share out the keys, 32 at a time.  Keys and values go from
+// their pages straight to LDS; in 8 bits they pass through registers, one tile
+// ahead, and become the queries' type on their way to LDS (a power of two and 4
+// significant bits are exact in both).
+//
+// 16 keys are the unit of loads: a page holds whole ones, so that a wave's load
+// has one base address, out of a list of pages in LDS.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "wp_apply.h"
+#include "wp_attn_core.h"
+#include "wp_device.h"
+#include "wp_paged.h"
+
+namespace wp {
+namespace {
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kTiles = 1, kChunks = 2;  // the roles of a launch
+constexpr int kGranule = 16;            // keys of one load address
+constexpr int kListed = 1024;           // granules whose pages are listed at a time
+constexpr int kMostWorkgroups = kListed;
+constexpr int kChunkKeys = 32;          // keys of a wave's step on key chunks
+static_assert(kGranule == kMinPage, "a granule lies in one page");
+
+template <bool kTile>
+constexpr int kStep = kTile ? kTileKeys : kChunkKeys * kWaves;  // keys of a workgroup's step
+template <bool kTile>
+constexpr int kTileRows = kTile ? kWaveRows * kWaves : kWaveRows;
+
+// ------------------------------------------------------------ the schedule --
+
+struct Shape {
+  int q0, n_q, n_k;
+};
+__device__ __forceinline__ Shape shape_of(const PagedArgs& p, int b) {
+  const int tokens = static_cast<int>(p.tokens);
+  Shape s;
+  const int q0 = p.cu_q[b], q1 = p.cu_q[b + 1];
+  s.n_k = std::clamp(p.kv_lens[b], 0, p.capacity);
+  s.q0 = std::clamp(q0, 0, tokens);
+  s.n_q = std::clamp(q1, s.q0, tokens) - s.q0;
+  return s;
+}
+
+// Costs of a sequence's row tiles, in keys times the group: tile t sees about
+// lag + (t + 1) * rows / group keys, at least 128 count, and no more than the
+// window, its own tokens and the first keys.
+struct Cost {
+  long long lag, least, most;
+  int tiles, log_rows;
+  // A tile's start and end cost about as much as 64 keys.
+  __device__ __forceinline__ long long extra(const PagedArgs& p) const { return 64ll * p.group; }
+  __device__ __forceinline__ long long of(const PagedArgs& p, int t) const {
+    const long long keys = lag + (static_cast<long long>(t + 1) << log_rows);
+    return (keys < least ? least : keys > most ? most : keys) + extra(p);
+  }
+  // Sum over the tiles before t.
+  __device__ __forceinline__ long long before(const PagedArgs& p, int t) const {
+    // Tiles whose line is at most `least`, and those below `most`.
+    const long long low = (least - lag) >> log_rows, high = (most - lag - 1) >> log_rows;
+    const long long a = low < 0 ? 0 : low > t ? t : low, b = high < a ? a : high > t ? t : high;
+    const long long line = (b - a) * lag + (((b * (b + 1) - a * (a + 1)) >> 1) << log_rows);
+    return a * least + line + (t - b) * most + t * extra(p);
+  }
+};
+__device__ __forceinline__ Cost cost_of(const PagedArgs& p, const Shape& s) {
+  const int rows = s.n_q * p.group;
+  Cost c;
+  c.log_rows = rows > p.chunk_rows ? 7 : 5;
+  c.tiles = static_cast<int>((static_cast<long long>(rows) + (1ll << c.log_rows) - 1) >> c.log_rows);
+  c.lag = static_cast<long long>(p.group) * (s.n_k - s.n_q);
+  c.least = 128ll * p.group;
+  c.most = p.window > 0 ? (static_cast<long long>(p.window) + p.sinks + 128) * p.group + (1ll << c.log_rows) : (1ll << 60);
+  return c;
+}
+
+// a / b for 0 <= a < 2^52, 0 < b.
+__device__ __forceinline__ long long divide(long long a, long long b) {
+  long long q = static_cast<long long>(static_cast<double>(a) / static_cast<double>(b));
+  if (q * b > a) --q;
+  if ((q + 1) * b <= a) ++q;
+  return q;
+}
+
+// The tile at cost y from the sequence's start: 64 places a round.
+__device__ __forceinline__ int tile_at(const PagedArgs& p, const Cost& c, long long y) {
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  int lo = 0, n = c.tiles;  // the tile is in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 63) / 64;
+    const bool upto = lane * static_cast<long long>(step) < n && c.before(p, lo + lane * step) <= y;
+    const int k = __builtin_popcountll(__ballot(upto)) - 1;
+    lo += k * step;
+    n = std::min(step, n - k * step);
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// Sum of v over the lanes up to this one.
+__device__ __forceinline__ long long sum_up64(long long v) {
+  auto add = [&](auto ctrl, auto rows) {
+    const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ctrl)::value, decltype(rows)::value, 0xF, true));
+    const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), decltype(ctrl)::value, decltype(rows)::value, 0xF, true));
+    v += static_cast<long long>((static_cast<unsigned long long>(hi) << 32) | lo);
+  };
+  add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});  // as sum_up's moves
+  add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
+  return v;
+}
+__device__ __forceinline__ long long lane_of(long long v, int lane) {
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane));
+  return static_cast<long long>((static_cast<unsigned long long>(hi) << 32) | lo);
+}
+
+// One row tile of a key head, and what of it this workgroup does.
+struct Item {
+  int seq, head, tile;
+  Shape s;
+  int row0, rows;         // of the sequence's rows of this key head
+  int end;                // no row sees a key from here on
+  int base, sink_steps;   // step i: keys from i * kStep for the first sink_steps, then from base on
+  int steps, from, to;    // all of its steps, and the workgroup's
+
+  template <int kKeys>
+  __device__ __forceinline__ int key_of(int i) const {
+    return i < sink_steps ? i * kKeys : base + (i - sink_steps) * kKeys;
+  }
+};
+
+// Where an item is on the line of all costs, and how the line is shared out.
+struct Place {
+  long long start, cost;
+  long long total, share;
+  int id;  // this workgroup's
+  // The item's step at which the line's point x cuts it.  Cuts near its ends are moved there.
+  __device__ __forceinline__ int cut(long long x, int steps) const {
+    const long long off = x - start, rest = cost - off, near = share >> 3;
+    if (off <= 0) return 0;
+    if (rest <= 0) return steps;
+    if (off < near || rest < near) return off <= rest ? 0 : steps;
+    return static_cast<int>(static_cast<double>(off) * static_cast<double>(steps) / static_cast<double>(cost));
+  }
+  __device__ __forceinline__ long long from() const { return id * share; }
+  __device__ __forceinline__ long long to() const { return std::min(total, (id + 1) * share); }
+};
+
+// What the workgroup shares.  The item and its place are kept here, not in registers,
+// while its keys are worked through.
+struct Shared {
+  float m[kWaves][kWaveRows];
+  float l[kWaves][kWaveRows];
+  Place at;
+  Item item;
+  long long sums[kWaves];
+  int count;
+  uint32_t last;
+};
+
+// The thread's number, anew to the compiler: what goes by it is worked out where
+// it is needed, and not kept in registers from item to item or past the keys.
+__device__ __forceinline__ int thread_number() {
+  int t = static_cast<int>(threadIdx.x);
+  asm volatile("" : "+v"(t));
+  return t;
+}
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ Item item_of(const Shared& sh) {
+  const Item& i = sh.item;
+  return Item{uniform(i.seq), uniform(i.head), uniform(i.tile), Shape{uniform(i.s.q0), uniform(i.s.n_q), uniform(i.s.n_k)},
+              uniform(i.row0), uniform(i.rows), uniform(i.end), uniform(i.base), uniform(i.sink_steps), uniform(i.steps),
+              uniform(i.from), uniform(i.to)};
+}
+
+template <bool kTile>
+__device__ __forceinline__ void range_of(const PagedArgs& p, Item& it) {
+  constexpr int kKeys = kStep<kTile>;
+  const int all = it.s.n_q * p.group;
+  it.row0 = it.tile * kTileRows<kTile>;
+  it.rows = std::min(kTileRows<kTile>, all - it.row0);
+  const int lag = it.s.n_k - it.s.n_q;
+  const int t0 = over(it.row0, p.by_group), t1 = over(it.row0 + it.rows - 1, p.by_group);
+  it.end = std::clamp(t1 + lag + 1, 0, it.s.n_k);
+  const int low = std::min(window_start(t0 + lag, p.window), it.end);
+  it.base = low / kKeys * kKeys;
+  const int sinks = std::min(p.sinks, it.end);
+  it.sink_steps = std::min((sinks + kKeys - 1) / kKeys, it.base / kKeys);
+  it.steps = std::max(1, it.sink_steps + (it.end - it.base + kKeys - 1) / kKeys);
+}
+
+// ---------------------------------------------------------- keys and values --
+
+// Loads of one granule of keys or values.  16 bits: load i fills rows i *
+// kRowsPerLoad on straight in LDS.  8 bits: rows to registers, 16 elements a
+// lane, and from there, in the queries' type, to LDS.  Offsets from the
+// granule's first row are the same for every granule; rows past the last key and columns past
+// the head lie outside its bytes and are zero.
+template <typename T, int DP, bool kValues, bool kSmall>
+struct Granule {
+  using H = Head<DP>;
+  static constexpr int kLanes = kSmall ? (DP <= 64 ? 4 : 8) : H::kChunks;  // of a row
+  static constexpr int kRowsPerLoad = 64 / kLanes;
+  static constexpr int kLoads = kGranule / kRowsPerLoad;
+  struct Held {
+    u32x4 q[kLoads];
+    uint32_t code[kLoads];
+  };
+  int off[kLoads];
+  int stride, scale_stride, row_bytes, lane;
+
+  static __device__ __forceinline__ int swizzle(int r) { return kValues ? H::value_swizzle(r) : H::key_swizzle(r); }
+
+  __device__ __forceinline__ Granule(int stride_, int scale_stride_, int dim, int lane_)
+      : stride(stride_), scale_stride(scale_stride_), row_bytes(kSmall ? dim : 2 * dim), lane(lane_) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = i * kRowsPerLoad + lane / kLanes;
+      const int c = kSmall ? lane % kLanes : (lane % kLanes) ^ swizzle(r);
+      off[i] = c * 16 < row_bytes ? r * stride + c * 16 : kOutside;
+    }
+  }
+  __device__ __forceinline__ int bytes(int rows) const { return rows <= 0 ? 0 : (std::min(rows, kGranule) - 1) * stride + row_bytes; }
+
+  __device__ __forceinline__ void stage(const char* src, int rows, char* dst) const {
+    const int size = bytes(rows);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) load_to_lds(src, dst + i * 1024, off[i], 0, size);
+  }
+
+  __device__ __forceinline__ void fetch(const char* src, const uint8_t* scales, int rows, Held& h) const {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(src), 0, bytes(rows), 0x00020000);
+    const int scale_size = rows <= 0 ? 0 : (std::min(rows, kGranule) - 1) * scale_stride + 1;
+    const __amdgpu_buffer_rsrc_t s = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(scales), 0, scale_size, 0x00020000);
+    const int row = lane / kLanes;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      h.q[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off[i], 0, 0));
+      h.code[i] = __builtin_amdgcn_raw_buffer_load_b8(s, (i * kRowsPerLoad + row) * scale_stride, 0, 0);
+    }
+  }
+
+  static __device__ __forceinline__ uint32_t two(uint32_t q, float scale, std::integral_constant<bool, false>) {
+    if constexpr (__is_same(T, __bf16))
+      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q, scale, false));
+    else
+      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q, scale, false));
+  }
+  static __device__ __forceinline__ uint32_t two(uint32_t q, float scale, std::integral_constant<bool, true>) {
+    if constexpr (__is_same(T, __bf16))
+      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q, scale, true));
+    else
+      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q, scale, true));
+  }
+  __device__ __forceinline__ void put(const Held& h, char* dst) const {
+    constexpr std::integral_constant<bool, false> low{};
+    constexpr std::integral_constant<bool, true> high{};
+    const int c = lane % kLanes * 2;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = i * kRowsPerLoad + lane / kLanes;
+      const float s = __builtin_bit_cast(float, h.code[i] << 23);
+      char* row = dst + r * H::kRow;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t a = h.q[i][2 * e], b = h.q[i][2 * e + 1];
+        *reinterpret_cast<u32x4*>(row + (((c + e) ^ swizzle(r)) << 4)) = u32x4{two(a, s, low), two(a, s, high), two(b, s, low), two(b, s, high)};
+      }
+    }
+  }
+};
+
+// A workgroup's keys and values: addresses of an item's granules by the listed pages.
+template <typename T, int DP, bool kSmall>
+struct Source {
+  using K = Granule<T, DP, false, kSmall>;
+  using V = Granule<T, DP, true, kSmall>;
+  const char* k;
+  const char* v;
+  const uint8_t* ks;
+  const uint8_t* vs;
+  int64_t k_page, v_page, ks_page, vs_page;
+  int ks_tok, vs_tok, in_page, end;
+  const int* list;
+  K keys;
+  V values;
+
+  __device__ __forceinline__ Source(const PagedArgs& p, const Item& it, const int* list_, int lane)
+      : k(p.k + it.head * p.k_head), v(p.v + it.head * p.v_head),
+        ks(kSmall ? p.k_scales + it.head * p.ks_head : nullptr), vs(kSmall ? p.v_scales + it.head * p.vs_head : nullptr),
+        k_page(p.k_page), v_page(p.v_page), ks_page(p.ks_page), vs_page(p.vs_page), ks_tok(p.ks_tok), vs_tok(p.vs_tok),
+        in_page((1 << p.page_shift) - 1), end(it.end), list(list_), keys(p.k_tok, p.ks_tok, p.dim, lane),
+        values(p.v_tok, p.vs_tok, p.dim, lane) {}
+
+  // Rows of the granule at `key`, 0 if its page is none.
+  __device__ __forceinline__ int page(int at) const { return __builtin_amdgcn_readfirstlane(list[at]); }
+  __device__ __forceinline__ void stage_k(int at, bool there, int key, char* to) const {
+    const int pg = there ? page(at) : -1;
+    keys.stage(k + std::max(pg, 0) * k_page + static_cast<int64_t>(key & in_page) * keys.stride, pg < 0 ? 0 : end - key, to);
+  }
+  __device__ __forceinline__ void stage_v(int at, bool there, int key, char* to) const {
+    const int pg = there ? page(at) : -1;
+    values.stage(v + std::max(pg, 0) * v_page + static_cast<int64_t>(key & in_page) * values.stride, pg < 0 ? 0 : end - key, to);
+  }
+  __device__ __forceinline__ void fetch_k(int at, bool there, int key, typename K::Held& h) const {
+    const int pg = there ? page(at) : -1;
+    const int64_t i = std::max(pg, 0), j = key & in_page;
+    keys.fetch(k + i * k_page + j * keys.stride, ks + i * ks_page + j * ks_tok, pg < 0 ? 0 : end - key, h);
+  }
+  __device__ __forceinline__ void fetch_v(int at, bool there, int key, typename V::Held& h) const {
+    const int pg = there ? page(at) : -1;
+    const int64_t i = std::max(pg, 0), j = key & in_page;
+    values.fetch(v + i * v_page + j * values.stride, vs + i * vs_page + j * vs_tok, pg < 0 ? 0 : end - key, h);
+  }
+};
+
+// Lists the pages of the item's steps [from, to), a granule each; -1: a page
+// outside the cache (flagged: its keys and values are taken as zero) or no key.
+template <bool kTile>
+__device__ __forceinline__ void list_pages(const PagedArgs& p, const Shared& sh, int from, int to, int* list) {
+  const Item it = item_of(sh);
+  const int tid = thread_number();
+  constexpr int kEach = kStep<kTile> / kGranule;
+  const int n = (to - from) * kEach;
+  const int32_t* row = p.table + static_cast<int64_t>(it.seq) * p.table_row;
+  for (int g = tid; g < n; g += kThreads) {
+    const int key = it.key_of<kStep<kTile>>(from + g / kEach) + g % kEach * kGranule;
+    int page = -1;
+    if (key < it.end) {
+      page = row[key >> p.page_shift];
+      if (page < 0 || page >= p.n_pages) {
+        flag_error(p.header, kErrIdRange);
+        page = -1;
+      }
+    }
+    list[g] = page;
+  }
+}
+
+// Scores of keys [at, at + 32) that the lane's query does not see become -inf.
+template <typename T, int DP>
+__device__ __forceinline__ void mask_seen(const Rows<T, DP, true>& w, f32x16& s, int at, int sinks) {
+  const int first = at + (w.lane() >> 5) * 4;
+  const int up = w.pos - first, down = w.low - first, kept = sinks - first;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int key = (e >> 2) * 8 + (e & 3);
+    s[e] = key <= up && (key >= down || key < kept) ? s[e] : -INFINITY;
+  }
+}
+
+// What all rows of a wave see: every key of [low, pos], and of the first `sinks`; none past `last`.
+struct Sight {
+  int low, pos, last, sinks;
+  __device__ __forceinline__ bool whole(int at, int n) const { return at + n - 1 <= pos && (at >= low || at + n <= sinks); }
+};
+
+// --------------------------------------------------------------------- roles --
+
+// Key chunks: this wave's 32 keys of each of the item's steps [from, to), whose
+// pages are listed.
+template <typename T, int DP, bool kSmall, bool kCareful>
+__device__ __forceinline__ void run_chunk(const Source<T, DP, kSmall>& in, const Item& it, Rows<T, DP, true>& w, float c,
+                                          const Sight& see, int from, int to, int wave, char* sk, char* sv) {
+  using Src = Source<T, DP, kSmall>;
+  constexpr int kRow = Head<DP>::kRow, kKeys = kStep<false>, kEach = kKeys / kGranule;
+  auto key_of = [&](int i) { return it.key_of<kKeys>(i) + wave * kChunkKeys; };
+  auto place = [&](int i) { return (i - from) * kEach + wave * 2; };
+  auto weigh_in = [&](f32x16& s, int at, typename VecOf<T>::v8 (&e)[2]) {
+    if (!see.whole(at, kChunkKeys)) mask_seen(w, s, at, see.sinks);
+    w.raise(top_of(s), c);
+    weigh(w, s, c, e);
+  };
+  auto add = [&](int at, const typename VecOf<T>::v8 (&e)[2]) {
+    accumulate<T, DP, kCareful>(w, sv, 0, e);
+    if (kCareful)
+      add_nonfinite(w, sv, kChunkKeys, [&](int r) { return at + r <= w.pos && (at + r >= w.low || at + r < see.sinks); });
+  };
+  if constexpr (kSmall) {
+    typename Src::K::Held hk[2];
+    typename Src::V::Held hv[2];
+    auto fetch_k = [&](int i) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) in.fetch_k(place(i) + g, i < to, key_of(i) + g * kGranule, hk[g]);
+    };
+    auto fetch_v = [&](int i) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) in.fetch_v(place(i) + g, i < to, key_of(i) + g * kGranule, hv[g]);
+    };
+    fetch_k(from);
+    fetch_v(from);
+    for (int i = from; i < to; ++i) {
+      const int at = key_of(i);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) in.keys.put(hk[g], sk + g * kGranule * kRow);
+      fetch_k(i + 1);
+      f32x16 s = scores(w, sk, 0);
+      typename VecOf<T>::v8 e[2];
+      weigh_in(s, at, e);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) in.values.put(hv[g], sv + g * kGranule * kRow);
+      fetch_v(i + 1);
+      add(at, e);
+    }
+  } else {
+    // K and V take turns in flight: while one is read the other's next keys are
+    // coming, so each wait leaves the younger one's loads (a load of no rows
+    // touches no memory and leaves zeros).
+    constexpr int kLoads = 2 * Src::K::kLoads;
+    auto load_k = [&](int i) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) in.stage_k(place(i) + g, i < to, key_of(i) + g * kGranule, sk + g * kGranule * kRow);
+    };
+    auto load_v = [&](int i) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g) in.stage_v(place(i) + g, i < to, key_of(i) + g * kGranule, sv + g * kGranule * kRow);
+    };
+    load_k(from);
+    load_v(from);
+    for (int i = from; i < to; ++i) {
+      const int at = key_of(i);
+      wait_vm_but<kLoads>();
+      f32x16 s = scores(w, sk, 0);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      load_k(i + 1);
+      typename VecOf<T>::v8 e[2];
+      weigh_in(s, at, e);
+      wait_vm_but<kLoads>();
+      add(at, e);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      load_v(i + 1);
+    }
+    wait_vm();
+  }
+}
+
+// Row tile: the item's steps [from, to), whose pages are listed, for the
+// workgroup's rows.  While step i is weighed and added, the scores of step i + 1
+// are computed, and steps i + 2 of K and i + 1 of V are on their way; each wave
+// brings in a granule of either.
+template <typename T, int DP, bool kSmall>
+__device__ __forceinline__ void run_tile(const Source<T, DP, kSmall>& in, const Item& it, Rows<T, DP, true>& w, float c,
+                                         const Sight& see, int from, int to, int wave, WP_STAGED) {
+  using Src = Source<T, DP, kSmall>;
+  constexpr int kKeys = kStep<true>, kEach = kKeys / kGranule;
+  const int mine = wave * kGranule * Head<DP>::kRow;
+  // Steps past the last key that any of the wave's rows sees are not its work.
+  const int live = std::min(to, see.last < 0 ? 0 : see.last < it.base ? std::min(it.sink_steps, see.last / kKeys + 1) : it.sink_steps + (see.last - it.base) / kKeys + 1);
+  auto key_of = [&](int i) { return it.key_of<kKeys>(i); };
+  auto place = [&](int i) { return (i - from) * kEach + wave; };
+  typename Src::K::Held hk;
+  typename Src::V::Held hv;
+  auto fetch_k = [&](int i) { in.fetch_k(place(i), i < to, key_of(i) + wave * kGranule, hk); };
+  auto fetch_v = [&](int i) { in.fetch_v(place(i), i < to, key_of(i) + wave * kGranule, hv); };
+  // Steps are asked for in their order.
+  auto load_k = [&](int i, char* buf) {
+    if constexpr (kSmall) {
+      in.keys.put(hk, buf + mine);
+      fetch_k(i + 1);
+    } else if (i < to) {
+      in.stage_k(place(i), true, key_of(i) + wave * kGranule, buf + mine);
+    }
+  };
+  auto load_v = [&](int i, char* buf) {
+    if constexpr (kSmall) {
+      in.values.put(hv, buf + mine);
+      fetch_v(i + 1);
+    } else if (i < to) {
+      in.stage_v(place(i), true, key_of(i) + wave * kGranule, buf + mine);
+    }
+  };
+  auto meet = [&] {
+    if (!kSmall) wait_vm();
+    __syncthreads();
+  };
+  if constexpr (kSmall) {
+    fetch_k(from);
+    fetch_v(from);
+  }
+  load_k(from, sk0);
+  meet();
+  load_k(from + 1, sk1);
+  load_v(from, sv0);
+  f32x16 s0 = scores(w, sk0, 0), s1 = scores(w, sk0, 32);
+  float tops = fmaxf(top_of(s0), top_of(s1));
+  auto step = [&](int i, char* kfree, const char* knext, const char* vnow, char* vnext) {
+    meet();
+    load_k(i + 2, kfree);
+    load_v(i + 1, vnext);
+    if (i >= live) return;
+    const int at = key_of(i);
+    if (!see.whole(at, kKeys)) {
+      mask_seen(w, s0, at, see.sinks);
+      mask_seen(w, s1, at + 32, see.sinks);
+      tops = fmaxf(top_of(s0), top_of(s1));
+    }
+    // (After the last step the next one's scores are of no use, and cost less
+    // than a second copy of this, without them, costs in registers.)
+    tile_body(w, s0, s1, tops, c, std::integral_constant<bool, true>{}, knext, vnow);
+  };
+  for (int i = from; i < to; i += 2) {
+    step(i, sk0, sk1, sv0, sv1);
+    if (i + 1 < to) step(i + 1, sk1, sk0, sv1, sv0);
+  }
+}
+
+// run_tile, one step after the other, with infinite and NaN values left out of
+// the product and added to the rows that see them: the same sums otherwise.
+template <typename T, int DP, bool kSmall>
+__device__ __forceinline__ void run_tile_careful(const Source<T, DP, kSmall>& in, const Item& it, Rows<T, DP, true>& w, float c,
+                                                 const Sight& see, int from, int to, int wave, char* sk, char* sv) {
+  using Src = Source<T, DP, kSmall>;
+  constexpr int kKeys = kStep<true>, kEach = kKeys / kGranule;
+  const int mine = wave * kGranule * Head<DP>::kRow;
+  for (int i = from; i < to; ++i) {
+    const int at = it.key_of<kKeys>(i), key = at + wave * kGranule, place = (i - from) * kEach + wave;
+    __syncthreads();
+    if constexpr (kSmall) {
+      typename Src::K::Held hk;
+      typename Src::V::Held hv;
+      in.fetch_k(place, true, key, hk);
+      in.fetch_v(place, true, key, hv);
+      in.keys.put(hk, sk + mine);
+      in.values.put(hv, sv + mine);
+    } else {
+      in.stage_k(place, true, key, sk + mine);
+      in.stage_v(place, true, key, sv + mine);
+      wait_vm();
+    }
+    __syncthreads();
+    f32x16 s0 = scores(w, sk, 0), s1 = scores(w, sk, 32);
+    if (!see.whole(at, kKeys)) {
+      mask_seen(w, s0, at, see.sinks);
+      mask_seen(w, s1, at + 32, see.sinks);
+    }
+    w.raise(fmaxf(top_of(s0), top_of(s1)), c);
+    typename VecOf<T>::v8 e0[2], e1[2];
+    weigh(w, s0, c, e0);
+    weigh(w, s1, c, e1);
+    accumulate<T, DP, true>(w, sv, 0, e0);
+    accumulate<T, DP, true>(w, sv, 32, e1);
+    add_nonfinite(w, sv, kKeys, [&](int r) { return at + r <= w.pos && (at + r >= w.low || at + r < see.sinks); });
+  }
+}
+
+// Writes four columns of a finished row (and with the first of them its lse).
+template <typename T>
+__device__ __forceinline__ void finish_row(const PagedArgs& p, const Item& it, int row, int d, f32x4 v, float m, float l) {
+  const int tok = over(row, p.by_group), h = it.head * p.group + row - tok * p.group;
+  const bool sees = tok + it.s.n_k - it.s.n_q >= 0;
+  const int64_t at = static_cast<int64_t>(it.s.q0) + tok;
+  if (d < p.dim)
+    store4(static_cast<T*>(p.out) + at * p.o_tok + h * p.o_head + d, sees ? v * (1.f / l) : f32x4{0.f, 0.f, 0.f, 0.f});
+  if (p.lse && d == 0) p.lse[at * p.heads + h] = sees ? fmaf(m, kLn2, logf(l)) : -INFINITY;
+}
+
+// The workgroup's steps of one item.
+template <typename T, int DP, bool kSmall, bool kTile, int kSlotRows>
+__device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, int* list, WP_STAGED) {
+  using H = Head<DP>;
+  constexpr int kBatch = kListed * kGranule / kStep<kTile>;  // steps whose pages are listed at a time
+  int tid = thread_number(), lane = tid & 63, half = lane >> 5;
+  const int wave = uniform(tid >> 6);
+  Item it = item_of(sh);
+  const int group = p.group, lag = it.s.n_k - it.s.n_q;
+  int row, tok, sub;
+  bool real;
+  const int wave_row0 = it.row0 + (kTile ? wave * kWaveRows : 0);
+  auto find_row = [&] {
+    row = it.row0 + (kTile ? wave * kWaveRows : 0) + (lane & 31);
+    real = row < it.row0 + it.rows;
+    tok = real ? over(row, p.by_group) : 0;
+    sub = real ? row - tok * group : 0;
+  };
+  find_row();
+  const float c = p.scale == 0.f ? 1.f : fabsf(p.scale) * kLog2e;
+  Rows<T, DP, true> w;
+  w.held = lane;
+  {
+    const T* q = static_cast<const T*>(p.q) + (static_cast<int64_t>(it.s.q0) + tok) * p.q_tok + (it.head * group + sub) * p.q_head;
+#pragma unroll
+    for (int x = 0; x < H::kSteps; ++x) {
+      const int d = x * 16 + half * 8;
+      w.q[x] = real && d < p.dim && p.scale != 0.f ? load8(q + d) : zero8<T>();
+    }
+  }
+  if (p.scale < 0.f) {
+#pragma unroll
+    for (int x = 0; x < H::kSteps; ++x) w.q[x] = negate8<T>(w.q[x]);
+  }
+  w.pos = real ? tok + lag : -1;
+  w.low = window_start(tok + lag, p.window);
+  Sight see{0, -1, -1, p.sinks};
+  if (wave_row0 < it.row0 + it.rows) {
+    const int t0 = over(wave_row0, p.by_group), t1 = std::min(it.s.n_q - 1, over(wave_row0 + kWaveRows - 1, p.by_group));
+    see.pos = t0 + lag;
+    see.last = t1 + lag;
+    see.low = window_start(t1 + lag, p.window);
+  }
+  const Source<T, DP, kSmall> in(p, it, list, lane);
+  char* my_k = (wave < 2 ? sk0 : sk1) + (wave & 1) * (Staged<DP>::kBytes / 2);
+  char* my_v = (wave < 2 ? sv0 : sv1) + (wave & 1) * (Staged<DP>::kBytes / 2);
+  auto pass = [&](auto careful) {
+    w.reset();
+    for (int i = it.from; i < it.to; i += kBatch) {
+      const int to = std::min(it.to, i + kBatch);
+      __syncthreads();  // the last batch's pages and tiles have been read
+      list_pages<kTile>(p, sh, i, to, list);
+      __syncthreads();
+      if constexpr (!kTile)
+        run_chunk<T, DP, kSmall, decltype(careful)::value>(in, it, w, c, see, i, to, wave, my_k, my_v);
+      else if constexpr (decltype(careful)::value)
+        run_tile_careful(in, it, w, c, see, i, to, wave, sk0, sv0);
+      else
+        run_tile(in, it, w, c, see, i, to, wave, sk0, sk1, sv0, sv1);
+    }
+  };
+  pass(std::integral_constant<bool, false>{});
+  // Infinite or NaN values reach every row of a tile through the product, as
+  // zero times them: where there are any, the pass is made again with care.
+  if (__syncthreads_or(has_nonfinite(w))) pass(std::integral_constant<bool, true>{});
+  w.l += __shfl_xor(w.l, 32);
+
+  it = item_of(sh);
+  tid = thread_number();
+  lane = tid & 63;
+  half = lane >> 5;
+  find_row();
+  const bool split = it.from > 0 || it.to < it.steps;
+  constexpr uint32_t kSlot = kSlotRows * (DP + 2);  // floats: [rows][DP] of O, then [rows][bound, sum]
+  // A workgroup's first item may have begun before it, and its last one may go on after it.
+  float* part = p.part + static_cast<uint64_t>(2 * uniform(sh.at.id) + (it.from == 0 ? 1 : 0)) * kSlot;
+  const __amdgpu_buffer_rsrc_t mine = coherent_buffer(part, kSlot * 4u);
+  if constexpr (kTile) {
+    if (!split) {
+      if (!real) return;
+      const bool sees = tok + it.s.n_k - it.s.n_q >= 0;
+      const float inv = 1.f / w.l;
+      const int64_t at = static_cast<int64_t>(it.s.q0) + tok;
+      T* out = static_cast<T*>(p.out) + at * p.o_tok + (it.head * group + sub) * p.o_head;
+#pragma unroll
+      for (int i = 0; i < H::kCols; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = i * 32 + e * 8 + half * 4;
+          if (d >= p.dim) continue;
+          const f32x4 v{w.o[i][e * 4], w.o[i][e * 4 + 1], w.o[i][e * 4 + 2], w.o[i][e * 4 + 3]};
+          store4(out + d, sees ? v * inv : f32x4{0.f, 0.f, 0.f, 0.f});
+        }
+      if (p.lse && half == 0) p.lse[at * p.heads + it.head * group + sub] = sees ? fmaf(w.m, kLn2, logf(w.l)) : -INFINITY;
+      return;
+    }
+    const int r = wave * kWaveRows + (lane & 31);
+    if (real) {
+      if (half == 0) coherent_store8(part + kSlotRows * DP + 2 * r, __builtin_bit_cast(unsigned long long, f32x2{w.m, w.l}));
+#pragma unroll
+      for (int i = 0; i < H::kCols; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          coherent_store16(mine, (r * DP + i * 32 + e * 8 + half * 4) * 4u,
+                           f32x4{w.o[i][e * 4], w.o[i][e * 4 + 1], w.o[i][e * 4 + 2], w.o[i][e * 4 + 3]});
+    }
+  } else {
+    // The waves' shares joined: each scales its O to the common bound and
+    // leaves it in LDS, [row][DP] in an array of its own.
+    if (half == 0) {
+      sh.m[wave][lane] = w.m;
+      sh.l[wave][lane] = w.l;
+    }
+    __syncthreads();
+    float m = w.m;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) m = fmaxf(m, sh.m[i][lane & 31]);
+    const float fade = m == -INFINITY ? 1.f : exp2_fast(w.m - m);
+    // (Columns swizzled by the row: whole rows apart, lanes would share banks.)
+    auto place = [](int r, int d) { return (r * (DP / 4) + ((d / 4) ^ (r & (DP == 96 ? 7 : 15)))) * 16; };
+    auto area = [&](int i) -> char* { return i == 0 ? sk0 : i == 1 ? sk1 : i == 2 ? sv0 : sv1; };
+    char* o32 = area(wave);
+    if (real)
+#pragma unroll
+      for (int i = 0; i < H::kCols; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<f32x4*>(o32 + place(lane & 31, i * 32 + e * 8 + half * 4)) =
+              f32x4{w.o[i][e * 4], w.o[i][e * 4 + 1], w.o[i][e * 4 + 2], w.o[i][e * 4 + 3]} * fade;
+    __syncthreads();
+    for (int u = tid; u < it.rows * (DP / 4); u += kThreads) {
+      const int r = u / (DP / 4), d = u % (DP / 4) * 4;
+      f32x4 v{0.f, 0.f, 0.f, 0.f};
+      float top = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) {
+        v += *reinterpret_cast<const f32x4*>(area(i) + place(r, d));
+        top = fmaxf(top, sh.m[i][r]);
+      }
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) l += sh.l[i][r] * (top == -INFINITY ? 1.f : exp2_fast(sh.m[i][r] - top));
+      if (!split) {
+        finish_row<T>(p, it, it.row0 + r, d, v, top, l);
+      } else {
+        if (d == 0) coherent_store8(part + kSlotRows * DP + 2 * r, __builtin_bit_cast(unsigned long long, f32x2{top, l}));
+        coherent_store16(mine, (r * DP + d) * 4u, v);
+      }
+    }
+    if (!split) return;
+  }
+
+  // The workgroup that does an item's last step joins its shares.  An item that
+  // several share begins in one that no other shared item begins in: its counter's place.
+  const Place at = sh.at;
+  const int first = uniform(static_cast<int>(divide(at.start, at.share)));
+  const int final = uniform(static_cast<int>(divide(at.start + at.cost - 1, at.share)));
+  wait_vm();
+  __syncthreads();
+  if (tid == 0) {
+    const bool last = atomic_add_u(p.counters + first, static_cast<unsigned>(it.to - it.from)) + static_cast<unsigned>(it.to - it.from) ==
+                      static_cast<unsigned>(it.steps);
+    if (last) atomic_store_u(p.counters + first, 0u);
+    sh.last = last ? 1u : 0u;
+  }
+  __syncthreads();
+  if (sh.last == 0u) return;
+  // Where the shares are (a workgroup may have none).
+  if (wave == 0) {
+    int n = 0;
+    for (int i = first; i <= final; i += 64) {
+      const int id = i + lane;
+      int from = 0, to = 0;
+      if (id <= final) {
+        from = at.cut(std::max(id * at.share, at.start), it.steps);
+        to = at.cut(std::min((id + 1) * at.share, at.start + at.cost), it.steps);
+      }
+      const unsigned long long some = __ballot(to > from);
+      if (to > from) list[n + __builtin_popcountll(some & ((1ull << lane) - 1))] = 2 * id + (from == 0 ? 1 : 0);
+      n += __builtin_popcountll(some);
+    }
+    if (lane == 0) sh.count = n;
+  }
+  __syncthreads();
+  const int count = sh.count;
+  for (int u = tid; u < it.rows * (DP / 4); u += kThreads) {
+    const int r = u / (DP / 4), d = u % (DP / 4) * 4;
+    float top = -INFINITY, l = 0.f;
+    f32x4 v{0.f, 0.f, 0.f, 0.f};
+    constexpr int kAtOnce = 8;
+    for (int i0 = 0; i0 < count; i0 += kAtOnce) {
+      f32x2 ml[kAtOnce];
+      f32x4 o[kAtOnce];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const float* share = p.part + static_cast<uint64_t>(list[std::min(i0 + i, count - 1)]) * kSlot;
+        ml[i] = __builtin_bit_cast(f32x2, coherent_load8(share + kSlotRows * DP + 2 * r));
+        o[i] = coherent_load_f4(share + r * DP + d);
+      }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        if (i0 + i >= count) break;
+        const float m = fmaxf(top, ml[i][0]);
+        const float old = m == -INFINITY ? 1.f : exp2_fast(top - m), now = m == -INFINITY ? 1.f : exp2_fast(ml[i][0] - m);
+        v = v * old + o[i] * now;
+        l = l * old + ml[i][1] * now;
+        top = m;
+      }
+    }
+    finish_row<T>(p, it, it.row0 + r, d, v, top, l);
+  }
+}
+
+// Clears the rows of no sequence: before the first bound and from the last one on.
+template <typename T>
+__device__ __forceinline__ void clear_rest(const PagedArgs& p) {
+  const int lane = static_cast<int>(threadIdx.x) & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int64_t head_rows = p.n_seq > 0 ? std::clamp<int64_t>(p.cu_q[0], 0, p.tokens) : p.tokens;
+  const int64_t tail = p.n_seq > 0 ? std::clamp<int64_t>(p.cu_q[p.n_seq], head_rows, p.tokens) : p.tokens;
+  const int64_t n = (head_rows + p.tokens - tail) * p.heads;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kWaves + wave; i < n; i += static_cast<int64_t>(gridDim.x) * kWaves) {
+    int64_t t = i / p.heads;
+    const int h = static_cast<int>(i % p.heads);
+    if (t >= head_rows) t += tail - head_rows;
+    T* out = static_cast<T*>(p.out) + t * p.o_tok + h * p.o_head;
+    for (int d = lane; d < p.dim; d += 64) out[d] = static_cast<T>(0.f);
+    if (p.lse && lane == 0) p.lse[t * p.heads + h] = -INFINITY;
+  }
+}
+
+template <typename T, int DP, bool kSmall, int kRoles>
+__global__ __launch_bounds__(kThreads, 2) void paged_kernel(PagedArgs p) {
+  constexpr int kSlotRows = (kRoles & kTiles) != 0 ? kTileRows<true> : kTileRows<false>;
+  __shared__ Shared sh;
+  __shared__ int list[kListed];
+  __shared__ __align__(1024) char sk0[Staged<DP>::kBytes];
+  __shared__ __align__(1024) char sk1[Staged<DP>::kBytes];
+  __shared__ __align__(1024) char sv0[Staged<DP>::kBytes];
+  __shared__ __align__(1024) char sv1[Staged<DP>::kBytes];
+  touch_kernel_args<static_cast<int>(sizeof(PagedArgs))>();
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  // A thread for each sequence, and the sum of their costs.
+  auto cost_at = [&](int b) -> long long {
+    if (b >= p.n_seq) return 0;
+    const Cost c = cost_of(p, shape_of(p, b));
+    return c.tiles > 0 ? c.before(p, c.tiles) * p.kv_heads : 0;
+  };
+  const long long mine = cost_at(tid);
+  long long sum = mine;
+  for (int b = tid + kThreads; b < p.n_seq; b += kThreads) sum += cost_at(b);
+  clear_rest<T>(p);
+  sum = lane_of(sum_up64(sum), 63);
+  if (lane == 0) sh.sums[wave] = sum;
+  __syncthreads();
+  const long long total = sh.sums[0] + sh.sums[1] + sh.sums[2] + sh.sums[3];
+  const long long share = static_cast<long long>(static_cast<double>(total) * p.per_wg) + 1;
+  // Neighbours on the line, which read the same keys, on one die.
+  const int block = static_cast<int>(blockIdx.x), dies = p.n_wg % 8 == 0 ? 8 : 1;
+  const int id = block % dies * (p.n_wg / dies) + block / dies;
+  const long long x0 = id * share;
+  if (x0 >= total) return;
+  // The sequence at x0, its start on the line, and from there the tile.
+  if (tid == 0) sh.item.seq = -1;
+  long long run = 0;
+  for (int b0 = 0; b0 < p.n_seq && run <= x0; b0 += kThreads) {
+    const long long v = b0 == 0 ? mine : cost_at(b0 + tid);
+    const long long up = sum_up64(v);
+    __syncthreads();  // the sums have been read
+    if (lane == 63) sh.sums[wave] = up;
+    __syncthreads();
+    long long before = run;
+    for (int i = 0; i < kWaves; ++i) {
+      if (i < wave) before += sh.sums[i];
+      run += sh.sums[i];
+    }
+    if (before + up - v <= x0 && x0 < before + up) {
+      sh.item.seq = b0 + tid;
+      sh.at = Place{before + up - v, 0, total, share, id};
+    }
+  }
+  __syncthreads();
+  int seq = uniform(sh.item.seq), head, tile;
+  if (seq < 0) return;  // (lengths that change under the call)
+  Shape s = shape_of(p, seq);
+  Cost c = cost_of(p, s);
+  long long start = sh.at.start;
+  {
+    const long long per_head = c.before(p, c.tiles);
+    head = uniform(static_cast<int>(divide(x0 - start, per_head)));
+    start += head * per_head;
+    tile = tile_at(p, c, x0 - start);
+    start += c.before(p, tile);
+  }
+  for (;;) {
+    Item it;
+    it.seq = seq;
+    it.head = head;
+    it.tile = tile;
+    it.s = s;
+    const bool tiled = (kRoles & kTiles) != 0 && c.log_rows == 7;
+    if (tiled) range_of<true>(p, it); else range_of<false>(p, it);
+    Place at = sh.at;
+    at.start = start;
+    at.cost = c.of(p, tile);
+    it.from = uniform(at.cut(at.from(), it.steps));
+    it.to = uniform(at.cut(std::min(at.to(), start + at.cost), it.steps));
+    __syncthreads();  // the item before has been read
+    if (tid == 0) {
+      sh.item = it;
+      sh.at = at;
+    }
+    __syncthreads();
+    if (it.to > it.from) {
+      if ((kRoles & kTiles) != 0 && tiled)
+        run_item<T, DP, kSmall, true, kSlotRows>(p, sh, list, sk0, sk1, sv0, sv1);
+      else
+        run_item<T, DP, kSmall, false, kSlotRows>(p, sh, list, sk0, sk1, sv0, sv1);
+    }
+    at = sh.at;
+    start = at.start + at.cost;
+    if (start >= at.to()) return;
+    // The next tile, key head or sequence with rows (there is one, as the line goes on).
+    it = item_of(sh);
+    seq = it.seq;
+    head = it.head;
+    s = it.s;
+    c = cost_of(p, s);
+    tile = it.tile + 1;
+    if (tile < c.tiles) continue;
+    tile = 0;
+    if (++head < p.kv_heads) continue;
+    head = 0;
+    do {
+      if (++seq >= p.n_seq) return;
+      s = shape_of(p, seq);
+      c = cost_of(p, s);
+    } while (c.tiles == 0);
+  }
+}
+
+template <typename T, int DP, bool kSmall>
+hipError_t launch(const PagedArgs& a, bool tiles, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(a.n_wg)), block(kThreads);
+  if (tiles)
+    hipLaunchKernelGGL((paged_kernel<T, DP, kSmall, kTiles | kChunks>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_kernel<T, DP, kSmall, kChunks>), grid, block, 0, stream, a);
+  return hipGetLastError();
+}
+
+template <typename T, bool kSmall>
+hipError_t launch_head(const PagedArgs& a, bool tiles, hipStream_t stream) {
+  return a.dim <= 64   ? launch<T, 64, kSmall>(a, tiles, stream)
+         : a.dim <= 96 ? launch<T, 96, kSmall>(a, tiles, stream)
+                       : launch<T, 128, kSmall>(a, tiles, stream);
+}
+
+}  // namespace
+
+hipError_t launch_paged_attention(int dtype_bf16, PagedArgs& a, int n_cu, hipStream_t stream) {
+  a.group = a.heads / a.kv_heads;
+  a.by_group = divisor_of(a.group);
+  const int64_t rows = a.tokens * a.group;
+  // Sequences of few rows on the whole run on key chunks, in tiles of 32 rows.
+  const bool tiles = rows > static_cast<int64_t>(kWaveRows) * std::max(1, a.n_seq);
+  a.chunk_rows = tiles ? kWaveRows : 0x7FFFFFFF;
+  a.n_wg = std::min(2 * n_cu, kMostWorkgroups);
+  a.per_wg = 1.0 / a.n_wg;
+  const int dp = a.dim <= 64 ? 64 : a.dim <= 96 ? 96 : 128;
+  const uint64_t slots = 2ull * a.n_wg * (tiles ? kTileRows<true> : kTileRows<false>) * (dp + 2) * 4;
+  if (slots > a.part_bytes || a.n_wg > a.n_counters) return hipErrorInvalidValue;
+  // The line of costs stays under 2^50, even where bounds that fall give every
+  // sequence all tokens.
+  const double most = static_cast<double>(a.kv_heads) * std::max(1, a.n_seq) * (static_cast<double>(rows) / kWaveRows + 1) *
+                      (static_cast<double>(a.group) * (static_cast<double>(a.capacity) + 512) + static_cast<double>(rows));
+  if (most > 0x1p50) return hipErrorInvalidValue;
+  if (dtype_bf16) return a.e4m3 ? launch_head<__bf16, true>(a, tiles, stream) : launch_head<__bf16, false>(a, tiles, stream);
+  return a.e4m3 ? launch_head<_Float16, true>(a, tiles, stream) : launch_head<_Float16, false>(a, tiles, stream);
+}
+
+}  // namespace wp

@@ -1099,6 +1099,52 @@ class WarpPipeEngine:
         _lib.check(rc, op)
         return k, v
 
+    def paged_attention(self, q, k_pages, v_pages, block_table, cu_seqlens_q, kv_lens, k_scales=None, v_scales=None,
+                        scale=None, window=0, sinks=0, out=None, return_lse=False):
+        """Attention of new tokens over a cache in pages (see write_cache; dim up to
+        128).  Sequence b has the queries [cu_seqlens_q[b], cu_seqlens_q[b + 1]) of q
+        [tokens, heads, dim] and as keys the first kv_lens[b] tokens of the pages
+        block_table[b]; its last query stands at its last key (the step's own
+        rows are written first).  cu_seqlens_q int32 [n + 1], kv_lens int32 [n] and
+        block_table int32 [n, columns] are on the device.  A query sees the keys
+        up to its own position; with window > 0 only the last `window` of them and
+        the sequence's first `sinks`.  heads a multiple of kv_heads; any token and
+        head strides of q that are multiples of 8.  scale: dim ** -0.5 unless
+        given.  Returns out [tokens, heads, dim], or (out, lse [tokens, heads] fp32)
+        with return_lse; queries that see no key, and rows of no sequence, get 0 and
+        -inf.  Lengths past the table are cut to it; a page outside the cache counts as
+        zeros and sets device error 1; bounds must not fall (rows of such a call
+        are unspecified)."""
+        op = "paged_attention"
+        dev = self._dev_index
+        dtype = q.dtype
+        dt = _DTYPES.get(dtype)
+        if dt is None:
+            dt = _dtype_code(q, "q")
+        cache = self._pages(k_pages, v_pages, k_scales, v_scales, dtype, op)
+        self._heads_of(q, "q", op, dtype, k_pages.size(3))
+        T, heads, dim = q.shape
+        for t, nm in ((block_table, "block_table"), (cu_seqlens_q, "cu_seqlens_q"), (kv_lens, "kv_lens")):
+            if t.get_device() != dev:
+                self._on_device(t, nm)
+            if t.dtype != torch.int32:
+                raise RuntimeError(f"{op}: {nm} must be int32, got {t.dtype}")
+        n = kv_lens.numel()
+        if kv_lens.dim() != 1 or cu_seqlens_q.shape != (n + 1,) or not kv_lens.is_contiguous() or not cu_seqlens_q.is_contiguous():
+            raise RuntimeError(f"{op}: cu_seqlens_q must be a contiguous [n + 1] and kv_lens a contiguous [n] tensor, got "
+                               f"{tuple(cu_seqlens_q.shape)} and {tuple(kv_lens.shape)}")
+        if block_table.dim() != 2 or block_table.size(0) != n or (block_table.size(1) > 1 and block_table.stride(1) != 1):
+            raise RuntimeError(f"{op}: block_table must be [{n}, columns] with unit column stride, got {tuple(block_table.shape)}")
+        out = self._head_out(out, q, "out", op)
+        lse = torch.empty(T, heads, dtype=torch.float32, device=q.device) if return_lse else None
+        rc = self._lib.wp_paged_attention(
+            self._handle, out.data_ptr(), _i64s(out.stride()[:2]), None if lse is None else lse.data_ptr(), q.data_ptr(),
+            _i64s(q.stride()[:2]), cache, block_table.data_ptr(), block_table.stride(0), block_table.size(1),
+            cu_seqlens_q.data_ptr(), kv_lens.data_ptr(), n, T, heads, dim ** -0.5 if scale is None else float(scale),
+            _i32(window or 0), _i32(sinks or 0), dt, _raw_stream(dev))
+        _lib.check(rc, op)
+        return out if lse is None else (out, lse)
+
     # ------------------------------------------------------------- staging --
     def prefetch_adapter(self, adapter_id, layer=None) -> int:
         """Stages the adapter's A/B in a slot on the prefetch stream; returns the

@@ -466,6 +466,24 @@ int wp_read_cache(wp_engine* e, void* k_out, const int64_t* k_out_strides, void*
                   const wp_pages* cache, const void* slots, int32_t slots_are_int64, int64_t tokens, int32_t dtype,
                   void* stream);
 
+/* Attention of new tokens over the cache: sequence b has the queries [cu_q[b],
+ * cu_q[b + 1]) (rows of q and out; cu_q is n_seq + 1 int32, on the device) and as
+ * keys the first kv_lens[b] tokens (int32, device) of the pages block_table[b *
+ * table_row_stride ..] (`columns` int32 a sequence, device); its last query stands at its
+ * last key, so the step's own rows have to be in the cache before.  A query sees the keys up to its own position;
+ * with window > 0 only the last `window` of them, and the first `sinks` of the
+ * sequence.  Grouped heads, out, lse, strides and rounding as wp_packed_attention's; queries that
+ * see no key, and rows of no sequence, get 0 and -inf.  Lengths past the table
+ * are cut to it; bounds that fall leave rows of that call unspecified.  A page outside the
+ * cache counts as keys and values of zero and is flagged (device error 1).  e4m3
+ * elements times their row's factor are taken in dtype, where they are exact if
+ * that can hold them. */
+int wp_paged_attention(wp_engine* e, void* out, const int64_t* out_strides, float* lse, const void* q,
+                       const int64_t* q_strides, const wp_pages* cache, const int32_t* block_table,
+                       int64_t table_row_stride, int32_t columns, const int32_t* cu_q, const int32_t* kv_lens,
+                       int32_t n_seq, int64_t tokens, int32_t heads, float scale, int32_t window, int32_t sinks,
+                       int32_t dtype, void* stream);
+
 /* ---- staging / prefetch ---------------------------------------------------- */
 
 /* Replaces WarpPipeExtension::prefetch_adapter (bindings:46-57): copies the
