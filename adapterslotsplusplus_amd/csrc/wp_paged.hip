@@ -27,6 +27,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "wp_apply.h"
@@ -40,13 +41,16 @@ namespace {
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kTiles = 1, kChunks = 2;  // the roles of a launch
 constexpr int kGranule = 16;            // keys of one load address
-constexpr int kListed = 1024;           // granules whose pages are listed at a time
-constexpr int kMostWorkgroups = kListed;
+constexpr int kListed = 256;            // granules whose places are listed at a time
+constexpr int kMostWorkgroups = 1024;
 constexpr int kChunkKeys = 32;          // keys of a wave's step on key chunks
+constexpr float kLongestLine = 0x1p30f;
 static_assert(kGranule == kMinPage, "a granule lies in one page");
 
 template <bool kTile>
 constexpr int kStep = kTile ? kTileKeys : kChunkKeys * kWaves;  // keys of a workgroup's step
+template <bool kTile>
+constexpr int kSteps = kListed * kGranule / kStep<kTile>;  // steps listed at a time
 template <bool kTile>
 constexpr int kTileRows = kTile ? kWaveRows * kWaves : kWaveRows;
 
@@ -65,79 +69,68 @@ __device__ __forceinline__ Shape shape_of(const PagedArgs& p, int b) {
   return s;
 }
 
-// Costs of a sequence's row tiles, in keys times the group: tile t sees about
-// lag + (t + 1) * rows / group keys, at least 128 count, and no more than the
-// window, its own tokens and the first keys.
+// The line of costs.  Row tile t of a sequence sees about lag + (t + 1) * rows /
+// group keys, and no more than the window, its own tokens and the first keys; it counts
+// for at least 64, and as much again as 128 for its start and end.  Counted in
+// keys times the group, whose sum over tiles has a closed form, and on the line
+// in 2^cost_shift of them (and one for each tile), which keeps it in 31 bits.
 struct Cost {
   long long lag, least, most;
-  int tiles, log_rows;
-  // A tile's start and end cost about as much as 64 keys.
-  __device__ __forceinline__ long long extra(const PagedArgs& p) const { return 64ll * p.group; }
-  __device__ __forceinline__ long long of(const PagedArgs& p, int t) const {
-    const long long keys = lag + (static_cast<long long>(t + 1) << log_rows);
-    return (keys < least ? least : keys > most ? most : keys) + extra(p);
-  }
-  // Sum over the tiles before t.
-  __device__ __forceinline__ long long before(const PagedArgs& p, int t) const {
+  int extra, tiles, log_rows, shift;
+  // Where tile t starts, from the sequence's start.
+  __device__ __forceinline__ int before(int t) const {
+    if (t == 0) return 0;
+    if (t == 1) {
+      const long long keys = lag + (1 << log_rows);
+      return static_cast<int>(((keys < least ? least : keys > most ? most : keys) + extra) >> shift) + 1;
+    }
     // Tiles whose line is at most `least`, and those below `most`.
     const long long low = (least - lag) >> log_rows, high = (most - lag - 1) >> log_rows;
     const long long a = low < 0 ? 0 : low > t ? t : low, b = high < a ? a : high > t ? t : high;
     const long long line = (b - a) * lag + (((b * (b + 1) - a * (a + 1)) >> 1) << log_rows);
-    return a * least + line + (t - b) * most + t * extra(p);
+    return static_cast<int>((a * least + line + (t - b) * most + static_cast<long long>(t) * extra) >> shift) + t;
   }
 };
 __device__ __forceinline__ Cost cost_of(const PagedArgs& p, const Shape& s) {
   const int rows = s.n_q * p.group;
   Cost c;
   c.log_rows = rows > p.chunk_rows ? 7 : 5;
-  c.tiles = static_cast<int>((static_cast<long long>(rows) + (1ll << c.log_rows) - 1) >> c.log_rows);
+  c.tiles = static_cast<int>((static_cast<unsigned>(rows) + (1u << c.log_rows) - 1) >> c.log_rows);
   c.lag = static_cast<long long>(p.group) * (s.n_k - s.n_q);
-  c.least = 128ll * p.group;
-  c.most = p.window > 0 ? (static_cast<long long>(p.window) + p.sinks + 128) * p.group + (1ll << c.log_rows) : (1ll << 60);
+  c.least = 64ll * p.group;
+  c.extra = 128 * p.group;
+  c.most = p.window > 0 ? (static_cast<long long>(p.window) + p.sinks + 128) * p.group + (1 << c.log_rows) : (1ll << 60);
+  c.shift = p.cost_shift;
   return c;
 }
 
-// a / b for 0 <= a < 2^52, 0 < b.
-__device__ __forceinline__ long long divide(long long a, long long b) {
-  long long q = static_cast<long long>(static_cast<double>(a) / static_cast<double>(b));
-  if (q * b > a) --q;
-  if ((q + 1) * b <= a) ++q;
-  return q;
+// Sum over the wave's lanes, in the last one.
+__device__ __forceinline__ float wave_sum(float v) {
+  auto add = [&](auto ctrl, auto rows) {
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, decltype(rows)::value, 0xF, true));
+  };
+  constexpr std::integral_constant<int, 0xF> all{};
+  add(std::integral_constant<int, 0x111>{}, all);  // sum_up's moves
+  add(std::integral_constant<int, 0x112>{}, all);
+  add(std::integral_constant<int, 0x114>{}, all);
+  add(std::integral_constant<int, 0x118>{}, all);
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
+  return v;
 }
 
-// The tile at cost y from the sequence's start: 64 places a round.
-__device__ __forceinline__ int tile_at(const PagedArgs& p, const Cost& c, long long y) {
+// The tile at place y from the sequence's start: 64 places a round.
+__device__ __forceinline__ int tile_at(const Cost& c, int y) {
   const int lane = static_cast<int>(threadIdx.x) & 63;
   int lo = 0, n = c.tiles;  // the tile is in [lo, lo + n)
   while (n > 1) {
     const int step = (n + 63) / 64;
-    const bool upto = lane * static_cast<long long>(step) < n && c.before(p, lo + lane * step) <= y;
+    const bool upto = lane * static_cast<long long>(step) < n && c.before(lo + lane * step) <= y;
     const int k = __builtin_popcountll(__ballot(upto)) - 1;
     lo += k * step;
     n = std::min(step, n - k * step);
   }
   return __builtin_amdgcn_readfirstlane(lo);
-}
-
-// Sum of v over the lanes up to this one.
-__device__ __forceinline__ long long sum_up64(long long v) {
-  auto add = [&](auto ctrl, auto rows) {
-    const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ctrl)::value, decltype(rows)::value, 0xF, true));
-    const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), decltype(ctrl)::value, decltype(rows)::value, 0xF, true));
-    v += static_cast<long long>((static_cast<unsigned long long>(hi) << 32) | lo);
-  };
-  add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});  // as sum_up's moves
-  add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
-  add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
-  add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
-  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
-  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
-  return v;
-}
-__device__ __forceinline__ long long lane_of(long long v, int lane) {
-  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
-  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane));
-  return static_cast<long long>((static_cast<unsigned long long>(hi) << 32) | lo);
 }
 
 // One row tile of a key head, and what of it this workgroup does.
@@ -157,19 +150,19 @@ struct Item {
 
 // Where an item is on the line of all costs, and how the line is shared out.
 struct Place {
-  long long start, cost;
-  long long total, share;
+  int start, cost;
+  int total, share, near;
   int id;  // this workgroup's
-  // The item's step at which the line's point x cuts it.  Cuts near its ends are moved there.
-  __device__ __forceinline__ int cut(long long x, int steps) const {
-    const long long off = x - start, rest = cost - off, near = share >> 3;
+  // The item's step at which the line's point x cuts it.  Cuts near its ends are
+  // moved there: a cut costs the shares' way through memory.
+  __device__ __forceinline__ int cut(int x, int steps) const {
+    const int off = x - start, rest = cost - off;
     if (off <= 0) return 0;
     if (rest <= 0) return steps;
-    if (off < near || rest < near) return off <= rest ? 0 : steps;
-    return static_cast<int>(static_cast<double>(off) * static_cast<double>(steps) / static_cast<double>(cost));
+    if (std::min(off, rest) < near) return off <= rest ? 0 : steps;
+    return std::min(steps, static_cast<int>(static_cast<float>(off) * __builtin_amdgcn_rcpf(static_cast<float>(cost)) * static_cast<float>(steps)));
   }
-  __device__ __forceinline__ long long from() const { return id * share; }
-  __device__ __forceinline__ long long to() const { return std::min(total, (id + 1) * share); }
+  __device__ __forceinline__ int from(int i) const { return static_cast<int>(std::min<long long>(total, static_cast<long long>(i) * share)); }
 };
 
 // What the workgroup shares.  The item and its place are kept here, not in registers,
@@ -179,7 +172,8 @@ struct Shared {
   float l[kWaves][kWaveRows];
   Place at;
   Item item;
-  long long sums[kWaves];
+  int sums[kWaves];
+  float sizes[kWaves];
   int count;
   uint32_t last;
 };
@@ -296,7 +290,17 @@ struct Granule {
   }
 };
 
-// A workgroup's keys and values: addresses of an item's granules by the listed pages.
+// Where a granule's keys, values and their scales are, from their arrays' starts;
+// none: its keys and values are zero.
+struct Listed {
+  long long k, v;
+  static constexpr long long kNone = -1;
+};
+struct ListedScales {
+  long long k, v;
+};
+
+// A workgroup's keys and values: addresses of an item's granules by the list.
 template <typename T, int DP, bool kSmall>
 struct Source {
   using K = Granule<T, DP, false, kSmall>;
@@ -305,61 +309,67 @@ struct Source {
   const char* v;
   const uint8_t* ks;
   const uint8_t* vs;
-  int64_t k_page, v_page, ks_page, vs_page;
-  int ks_tok, vs_tok, in_page, end;
-  const int* list;
+  int end;
+  const Listed* list;
+  const ListedScales* scales;
   K keys;
   V values;
 
-  __device__ __forceinline__ Source(const PagedArgs& p, const Item& it, const int* list_, int lane)
+  __device__ __forceinline__ Source(const PagedArgs& p, const Item& it, const Listed* list_, const ListedScales* scales_, int lane)
       : k(p.k + it.head * p.k_head), v(p.v + it.head * p.v_head),
         ks(kSmall ? p.k_scales + it.head * p.ks_head : nullptr), vs(kSmall ? p.v_scales + it.head * p.vs_head : nullptr),
-        k_page(p.k_page), v_page(p.v_page), ks_page(p.ks_page), vs_page(p.vs_page), ks_tok(p.ks_tok), vs_tok(p.vs_tok),
-        in_page((1 << p.page_shift) - 1), end(it.end), list(list_), keys(p.k_tok, p.ks_tok, p.dim, lane),
-        values(p.v_tok, p.vs_tok, p.dim, lane) {}
+        end(it.end), list(list_), scales(scales_), keys(p.k_tok, p.ks_tok, p.dim, lane), values(p.v_tok, p.vs_tok, p.dim, lane) {}
 
-  // Rows of the granule at `key`, 0 if its page is none.
-  __device__ __forceinline__ int page(int at) const { return __builtin_amdgcn_readfirstlane(list[at]); }
+  static __device__ __forceinline__ long long first(long long v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(v));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32));
+    return static_cast<long long>((static_cast<unsigned long long>(hi) << 32) | lo);
+  }
   __device__ __forceinline__ void stage_k(int at, bool there, int key, char* to) const {
-    const int pg = there ? page(at) : -1;
-    keys.stage(k + std::max(pg, 0) * k_page + static_cast<int64_t>(key & in_page) * keys.stride, pg < 0 ? 0 : end - key, to);
+    const long long off = there ? first(list[at].k) : Listed::kNone;
+    keys.stage(k + off, off < 0 ? 0 : end - key, to);
   }
   __device__ __forceinline__ void stage_v(int at, bool there, int key, char* to) const {
-    const int pg = there ? page(at) : -1;
-    values.stage(v + std::max(pg, 0) * v_page + static_cast<int64_t>(key & in_page) * values.stride, pg < 0 ? 0 : end - key, to);
+    const long long off = there ? first(list[at].v) : Listed::kNone;
+    values.stage(v + off, off < 0 ? 0 : end - key, to);
   }
   __device__ __forceinline__ void fetch_k(int at, bool there, int key, typename K::Held& h) const {
-    const int pg = there ? page(at) : -1;
-    const int64_t i = std::max(pg, 0), j = key & in_page;
-    keys.fetch(k + i * k_page + j * keys.stride, ks + i * ks_page + j * ks_tok, pg < 0 ? 0 : end - key, h);
+    const long long off = there ? first(list[at].k) : Listed::kNone, scale = there ? first(scales[at].k) : 0;
+    keys.fetch(k + off, ks + scale, off < 0 ? 0 : end - key, h);
   }
   __device__ __forceinline__ void fetch_v(int at, bool there, int key, typename V::Held& h) const {
-    const int pg = there ? page(at) : -1;
-    const int64_t i = std::max(pg, 0), j = key & in_page;
-    values.fetch(v + i * v_page + j * values.stride, vs + i * vs_page + j * vs_tok, pg < 0 ? 0 : end - key, h);
+    const long long off = there ? first(list[at].v) : Listed::kNone, scale = there ? first(scales[at].v) : 0;
+    values.fetch(v + off, vs + scale, off < 0 ? 0 : end - key, h);
   }
 };
 
-// Lists the pages of the item's steps [from, to), a granule each; -1: a page
-// outside the cache (flagged: its keys and values are taken as zero) or no key.
-template <bool kTile>
-__device__ __forceinline__ void list_pages(const PagedArgs& p, const Shared& sh, int from, int to, int* list) {
-  const Item it = item_of(sh);
-  const int tid = thread_number();
+// Lists where the item's steps [from, to) are, a granule each.  None: a page outside
+// the cache (flagged), or no key.
+template <bool kTile, bool kSmall>
+__device__ __forceinline__ void list_pages(const PagedArgs& p, const Item& it, int from, int to, int tid, Listed* list, ListedScales* scales) {
   constexpr int kEach = kStep<kTile> / kGranule;
   const int n = (to - from) * kEach;
   const int32_t* row = p.table + static_cast<int64_t>(it.seq) * p.table_row;
   for (int g = tid; g < n; g += kThreads) {
     const int key = it.key_of<kStep<kTile>>(from + g / kEach) + g % kEach * kGranule;
-    int page = -1;
+    Listed l{Listed::kNone, Listed::kNone};
+    ListedScales z{0, 0};
     if (key < it.end) {
-      page = row[key >> p.page_shift];
+      const int page = row[key >> p.page_shift];
       if (page < 0 || page >= p.n_pages) {
         flag_error(p.header, kErrIdRange);
-        page = -1;
+      } else {
+        const int64_t i = page, j = key & ((1 << p.page_shift) - 1);
+        l.k = i * p.k_page + j * p.k_tok;
+        l.v = i * p.v_page + j * p.v_tok;
+        if (kSmall) {
+          z.k = i * p.ks_page + j * p.ks_tok;
+          z.v = i * p.vs_page + j * p.vs_tok;
+        }
       }
     }
-    list[g] = page;
+    list[g] = l;
+    if (kSmall) scales[g] = z;
   }
 }
 
@@ -582,9 +592,9 @@ __device__ __forceinline__ void finish_row(const PagedArgs& p, const Item& it, i
 
 // The workgroup's steps of one item.
 template <typename T, int DP, bool kSmall, bool kTile, int kSlotRows>
-__device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, int* list, WP_STAGED) {
+__device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed* list, ListedScales* scales, WP_STAGED) {
   using H = Head<DP>;
-  constexpr int kBatch = kListed * kGranule / kStep<kTile>;  // steps whose pages are listed at a time
+  constexpr int kBatch = kSteps<kTile>;
   int tid = thread_number(), lane = tid & 63, half = lane >> 5;
   const int wave = uniform(tid >> 6);
   Item it = item_of(sh);
@@ -623,16 +633,19 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, int* li
     see.last = t1 + lag;
     see.low = window_start(t1 + lag, p.window);
   }
-  const Source<T, DP, kSmall> in(p, it, list, lane);
+  const Source<T, DP, kSmall> in(p, it, list, scales, lane);
   char* my_k = (wave < 2 ? sk0 : sk1) + (wave & 1) * (Staged<DP>::kBytes / 2);
   char* my_v = (wave < 2 ? sv0 : sv1) + (wave & 1) * (Staged<DP>::kBytes / 2);
+  // (The first steps are listed.)
   auto pass = [&](auto careful) {
     w.reset();
     for (int i = it.from; i < it.to; i += kBatch) {
       const int to = std::min(it.to, i + kBatch);
-      __syncthreads();  // the last batch's pages and tiles have been read
-      list_pages<kTile>(p, sh, i, to, list);
-      __syncthreads();
+      if (i > it.from || decltype(careful)::value) {
+        __syncthreads();  // the last batch's places and tiles have been read
+        list_pages<kTile, kSmall>(p, item_of(sh), i, to, thread_number(), list, scales);
+        __syncthreads();
+      }
       if constexpr (!kTile)
         run_chunk<T, DP, kSmall, decltype(careful)::value>(in, it, w, c, see, i, to, wave, my_k, my_v);
       else if constexpr (decltype(careful)::value)
@@ -734,61 +747,80 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, int* li
   // The workgroup that does an item's last step joins its shares.  An item that
   // several share begins in one that no other shared item begins in: its counter's place.
   const Place at = sh.at;
-  const int first = uniform(static_cast<int>(divide(at.start, at.share)));
-  const int final = uniform(static_cast<int>(divide(at.start + at.cost - 1, at.share)));
+  const int first = uniform(at.start / at.share), final = uniform((at.start + at.cost - 1) / at.share);
   wait_vm();
   __syncthreads();
   if (tid == 0) {
-    const bool last = atomic_add_u(p.counters + first, static_cast<unsigned>(it.to - it.from)) + static_cast<unsigned>(it.to - it.from) ==
-                      static_cast<unsigned>(it.steps);
+    const unsigned mine = static_cast<unsigned>(it.to - it.from);
+    const bool last = atomic_add_u(p.counters + first, mine) + mine == static_cast<unsigned>(it.steps);
     if (last) atomic_store_u(p.counters + first, 0u);
     sh.last = last ? 1u : 0u;
   }
   __syncthreads();
   if (sh.last == 0u) return;
   // Where the shares are (a workgroup may have none).
+  int* slots = reinterpret_cast<int*>(list);
+  static_assert(kListed * sizeof(Listed) >= kMostWorkgroups * sizeof(int), "the list holds a slot for each workgroup");
   if (wave == 0) {
     int n = 0;
     for (int i = first; i <= final; i += 64) {
       const int id = i + lane;
       int from = 0, to = 0;
       if (id <= final) {
-        from = at.cut(std::max(id * at.share, at.start), it.steps);
-        to = at.cut(std::min((id + 1) * at.share, at.start + at.cost), it.steps);
+        from = at.cut(std::max(at.from(id), at.start), it.steps);
+        to = at.cut(std::min(at.from(id + 1), at.start + at.cost), it.steps);
       }
       const unsigned long long some = __ballot(to > from);
-      if (to > from) list[n + __builtin_popcountll(some & ((1ull << lane) - 1))] = 2 * id + (from == 0 ? 1 : 0);
+      if (to > from) slots[n + __builtin_popcountll(some & ((1ull << lane) - 1))] = 2 * id + (from == 0 ? 1 : 0);
       n += __builtin_popcountll(some);
     }
     if (lane == 0) sh.count = n;
   }
   __syncthreads();
-  const int count = sh.count;
-  for (int u = tid; u < it.rows * (DP / 4); u += kThreads) {
-    const int r = u / (DP / 4), d = u % (DP / 4) * 4;
-    float top = -INFINITY, l = 0.f;
-    f32x4 v{0.f, 0.f, 0.f, 0.f};
-    constexpr int kAtOnce = 8;
-    for (int i0 = 0; i0 < count; i0 += kAtOnce) {
-      f32x2 ml[kAtOnce];
-      f32x4 o[kAtOnce];
+  // Several loads at once: of one place in many shares (few rows), or of
+  // several places in a few (a tile's).
+  const int count = sh.count, places = it.rows * (DP / 4);
+  constexpr int kPlaces = kTile ? 4 : 1, kShares = kTile ? 2 : 16;
+  for (int u0 = tid; u0 < places; u0 += kThreads * kPlaces) {
+    float top[kPlaces], l[kPlaces];
+    f32x4 v[kPlaces];
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) {
-        const float* share = p.part + static_cast<uint64_t>(list[std::min(i0 + i, count - 1)]) * kSlot;
-        ml[i] = __builtin_bit_cast(f32x2, coherent_load8(share + kSlotRows * DP + 2 * r));
-        o[i] = coherent_load_f4(share + r * DP + d);
+    for (int x = 0; x < kPlaces; ++x) {
+      top[x] = -INFINITY;
+      l[x] = 0.f;
+      v[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int i0 = 0; i0 < count; i0 += kShares) {
+      f32x2 ml[kShares][kPlaces];
+      f32x4 o[kShares][kPlaces];
+#pragma unroll
+      for (int i = 0; i < kShares; ++i) {
+        const float* share = p.part + static_cast<uint64_t>(slots[std::min(i0 + i, count - 1)]) * kSlot;
+#pragma unroll
+        for (int x = 0; x < kPlaces; ++x) {
+          const int u = std::min(u0 + x * kThreads, places - 1), r = u / (DP / 4), d = u % (DP / 4) * 4;
+          ml[i][x] = __builtin_bit_cast(f32x2, coherent_load8(share + kSlotRows * DP + 2 * r));
+          o[i][x] = coherent_load_f4(share + r * DP + d);
+        }
       }
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) {
-        if (i0 + i >= count) break;
-        const float m = fmaxf(top, ml[i][0]);
-        const float old = m == -INFINITY ? 1.f : exp2_fast(top - m), now = m == -INFINITY ? 1.f : exp2_fast(ml[i][0] - m);
-        v = v * old + o[i] * now;
-        l = l * old + ml[i][1] * now;
-        top = m;
+      for (int i = 0; i < kShares; ++i) {
+        const bool there = i0 + i < count;
+#pragma unroll
+        for (int x = 0; x < kPlaces; ++x) {
+          const float m = there ? fmaxf(top[x], ml[i][x][0]) : top[x];
+          const float old = m == -INFINITY ? 1.f : exp2_fast(top[x] - m), now = m == -INFINITY ? 1.f : exp2_fast(ml[i][x][0] - m);
+          v[x] = there ? v[x] * old + o[i][x] * now : v[x];
+          l[x] = there ? l[x] * old + ml[i][x][1] * now : l[x];
+          top[x] = m;
+        }
       }
     }
-    finish_row<T>(p, it, it.row0 + r, d, v, top, l);
+#pragma unroll
+    for (int x = 0; x < kPlaces; ++x) {
+      const int u = u0 + x * kThreads, r = u / (DP / 4), d = u % (DP / 4) * 4;
+      if (u < places) finish_row<T>(p, it, it.row0 + r, d, v[x], top[x], l[x]);
+    }
   }
 }
 
@@ -814,7 +846,8 @@ template <typename T, int DP, bool kSmall, int kRoles>
 __global__ __launch_bounds__(kThreads, 2) void paged_kernel(PagedArgs p) {
   constexpr int kSlotRows = (kRoles & kTiles) != 0 ? kTileRows<true> : kTileRows<false>;
   __shared__ Shared sh;
-  __shared__ int list[kListed];
+  __shared__ Listed list[kListed];
+  __shared__ ListedScales scales[kSmall ? kListed : 1];
   __shared__ __align__(1024) char sk0[Staged<DP>::kBytes];
   __shared__ __align__(1024) char sk1[Staged<DP>::kBytes];
   __shared__ __align__(1024) char sv0[Staged<DP>::kBytes];
@@ -824,56 +857,72 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(PagedArgs p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   // A thread for each sequence, and the sum of their costs.
-  auto cost_at = [&](int b) -> long long {
+  auto cost_at = [&](int b, Shape& s) {
     if (b >= p.n_seq) return 0;
-    const Cost c = cost_of(p, shape_of(p, b));
-    return c.tiles > 0 ? c.before(p, c.tiles) * p.kv_heads : 0;
+    s = shape_of(p, b);
+    const Cost c = cost_of(p, s);
+    return c.before(c.tiles) * p.kv_heads;
   };
-  const long long mine = cost_at(tid);
-  long long sum = mine;
-  for (int b = tid + kThreads; b < p.n_seq; b += kThreads) sum += cost_at(b);
+  Shape my_shape{0, 0, 0}, other;
+  const int mine = cost_at(tid, my_shape);
+  int sum = mine;
+  float size = static_cast<float>(mine);
+  for (int b = tid + kThreads; b < p.n_seq; b += kThreads) {
+    const int v = cost_at(b, other);
+    sum += v;
+    size += static_cast<float>(v);
+  }
   clear_rest<T>(p);
-  sum = lane_of(sum_up64(sum), 63);
-  if (lane == 0) sh.sums[wave] = sum;
+  const int up0 = sum_up(sum);
+  size = wave_sum(size);
+  if (lane == 63) {
+    sh.sums[wave] = up0;
+    sh.sizes[wave] = size;
+  }
   __syncthreads();
-  const long long total = sh.sums[0] + sh.sums[1] + sh.sums[2] + sh.sums[3];
-  const long long share = static_cast<long long>(static_cast<double>(total) * p.per_wg) + 1;
-  // Neighbours on the line, which read the same keys, on one die.
-  const int block = static_cast<int>(blockIdx.x), dies = p.n_wg % 8 == 0 ? 8 : 1;
+  // Bounds that fall can give sequences more rows than there are, and a line
+  // past its 31 bits: such a call does nothing.
+  if (sh.sizes[0] + sh.sizes[1] + sh.sizes[2] + sh.sizes[3] > kLongestLine) return;
+  const int total = sh.sums[0] + sh.sums[1] + sh.sums[2] + sh.sums[3];
+  const int share = over(total, p.by_wg) + 1;
+  // Tiles: neighbours on the line, which read the same keys, on one die.  Chunks
+  // read keys of their own, and the dies share out all kinds of items.
+  const int block = static_cast<int>(blockIdx.x), dies = (kRoles & kTiles) != 0 && p.n_wg % 8 == 0 ? 8 : 1;
   const int id = block % dies * (p.n_wg / dies) + block / dies;
-  const long long x0 = id * share;
-  if (x0 >= total) return;
+  const long long x0_wide = static_cast<long long>(id) * share;
+  if (x0_wide >= total) return;
+  const int x0 = static_cast<int>(x0_wide), x1 = static_cast<int>(std::min<long long>(total, x0_wide + share));
   // The sequence at x0, its start on the line, and from there the tile.
   if (tid == 0) sh.item.seq = -1;
-  long long run = 0;
+  int run = 0;
   for (int b0 = 0; b0 < p.n_seq && run <= x0; b0 += kThreads) {
-    const long long v = b0 == 0 ? mine : cost_at(b0 + tid);
-    const long long up = sum_up64(v);
+    const int v = b0 == 0 ? mine : cost_at(b0 + tid, my_shape);
+    const int up = sum_up(v);
     __syncthreads();  // the sums have been read
     if (lane == 63) sh.sums[wave] = up;
     __syncthreads();
-    long long before = run;
+    int before = run;
     for (int i = 0; i < kWaves; ++i) {
       if (i < wave) before += sh.sums[i];
       run += sh.sums[i];
     }
     if (before + up - v <= x0 && x0 < before + up) {
       sh.item.seq = b0 + tid;
-      sh.at = Place{before + up - v, 0, total, share, id};
+      sh.item.s = my_shape;
+      sh.at.start = before + up - v;
     }
   }
   __syncthreads();
-  int seq = uniform(sh.item.seq), head, tile;
+  int seq = uniform(sh.item.seq), head, tile, start = uniform(sh.at.start);
   if (seq < 0) return;  // (lengths that change under the call)
-  Shape s = shape_of(p, seq);
+  Shape s{uniform(sh.item.s.q0), uniform(sh.item.s.n_q), uniform(sh.item.s.n_k)};
   Cost c = cost_of(p, s);
-  long long start = sh.at.start;
   {
-    const long long per_head = c.before(p, c.tiles);
-    head = uniform(static_cast<int>(divide(x0 - start, per_head)));
+    const int per_head = c.before(c.tiles);
+    head = uniform((x0 - start) / per_head);
     start += head * per_head;
-    tile = tile_at(p, c, x0 - start);
-    start += c.before(p, tile);
+    tile = tile_at(c, x0 - start);
+    start = uniform(start + c.before(tile));
   }
   for (;;) {
     Item it;
@@ -883,34 +932,35 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(PagedArgs p) {
     it.s = s;
     const bool tiled = (kRoles & kTiles) != 0 && c.log_rows == 7;
     if (tiled) range_of<true>(p, it); else range_of<false>(p, it);
-    Place at = sh.at;
+    Place at;
     at.start = start;
-    at.cost = c.of(p, tile);
-    it.from = uniform(at.cut(at.from(), it.steps));
-    it.to = uniform(at.cut(std::min(at.to(), start + at.cost), it.steps));
-    __syncthreads();  // the item before has been read
-    if (tid == 0) {
-      sh.item = it;
-      sh.at = at;
-    }
-    __syncthreads();
+    at.cost = c.before(tile + 1) - c.before(tile);
+    at.total = total;
+    at.share = share;
+    at.near = std::min(share >> 3, ((tiled ? 512 : 128) * p.group) >> p.cost_shift);
+    at.id = id;
+    it.from = uniform(at.cut(x0, it.steps));
+    it.to = uniform(at.cut(std::min(x1, start + at.cost), it.steps));
     if (it.to > it.from) {
-      if ((kRoles & kTiles) != 0 && tiled)
-        run_item<T, DP, kSmall, true, kSlotRows>(p, sh, list, sk0, sk1, sv0, sv1);
+      __syncthreads();  // what the item before left in LDS has been read
+      if (tid == 0) {
+        sh.item = it;
+        sh.at = at;
+      }
+      if (tiled)
+        list_pages<true, kSmall>(p, it, it.from, std::min(it.to, it.from + kSteps<true>), thread_number(), list, scales);
       else
-        run_item<T, DP, kSmall, false, kSlotRows>(p, sh, list, sk0, sk1, sv0, sv1);
+        list_pages<false, kSmall>(p, it, it.from, std::min(it.to, it.from + kSteps<false>), thread_number(), list, scales);
+      __syncthreads();
+      if ((kRoles & kTiles) != 0 && tiled)
+        run_item<T, DP, kSmall, true, kSlotRows>(p, sh, list, scales, sk0, sk1, sv0, sv1);
+      else
+        run_item<T, DP, kSmall, false, kSlotRows>(p, sh, list, scales, sk0, sk1, sv0, sv1);
     }
-    at = sh.at;
-    start = at.start + at.cost;
-    if (start >= at.to()) return;
+    start += at.cost;
+    if (start >= x1) return;
     // The next tile, key head or sequence with rows (there is one, as the line goes on).
-    it = item_of(sh);
-    seq = it.seq;
-    head = it.head;
-    s = it.s;
-    c = cost_of(p, s);
-    tile = it.tile + 1;
-    if (tile < c.tiles) continue;
+    if (++tile < c.tiles) continue;
     tile = 0;
     if (++head < p.kv_heads) continue;
     head = 0;
@@ -949,15 +999,17 @@ hipError_t launch_paged_attention(int dtype_bf16, PagedArgs& a, int n_cu, hipStr
   const bool tiles = rows > static_cast<int64_t>(kWaveRows) * std::max(1, a.n_seq);
   a.chunk_rows = tiles ? kWaveRows : 0x7FFFFFFF;
   a.n_wg = std::min(2 * n_cu, kMostWorkgroups);
-  a.per_wg = 1.0 / a.n_wg;
+  a.by_wg = divisor_of(a.n_wg);
   const int dp = a.dim <= 64 ? 64 : a.dim <= 96 ? 96 : 128;
   const uint64_t slots = 2ull * a.n_wg * (tiles ? kTileRows<true> : kTileRows<false>) * (dp + 2) * 4;
   if (slots > a.part_bytes || a.n_wg > a.n_counters) return hipErrorInvalidValue;
-  // The line of costs stays under 2^50, even where bounds that fall give every
-  // sequence all tokens.
-  const double most = static_cast<double>(a.kv_heads) * std::max(1, a.n_seq) * (static_cast<double>(rows) / kWaveRows + 1) *
-                      (static_cast<double>(a.group) * (static_cast<double>(a.capacity) + 512) + static_cast<double>(rows));
-  if (most > 0x1p50) return hipErrorInvalidValue;
+  // The line of costs stays under 2^30: every tile of all rows with a sequence's
+  // most keys, in units that allow it.
+  const double tiles_most = static_cast<double>(rows) / (tiles ? kTileRows<true> : kTileRows<false>) + std::max(1, a.n_seq);
+  const double most = a.kv_heads * tiles_most * (a.group * (static_cast<double>(a.capacity) + 512) + 256.0);
+  a.cost_shift = 0;
+  while (a.cost_shift < 31 && std::ldexp(most, -a.cost_shift) + a.kv_heads * tiles_most > 0x1p30) ++a.cost_shift;
+  if (a.cost_shift == 31) return hipErrorInvalidValue;
   if (dtype_bf16) return a.e4m3 ? launch_head<__bf16, true>(a, tiles, stream) : launch_head<__bf16, false>(a, tiles, stream);
   return a.e4m3 ? launch_head<_Float16, true>(a, tiles, stream) : launch_head<_Float16, false>(a, tiles, stream);
 }
