@@ -38,21 +38,27 @@
 namespace wp {
 namespace {
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves;
+constexpr int kTileWaves = 4;             // waves of a workgroup with row tiles among its items
+constexpr int kChunkWaves = 2;            // and of one with key chunks alone
+constexpr int kMostWaves = 4;
 constexpr int kTiles = 1, kChunks = 2;  // the roles of a launch
 constexpr int kGranule = 16;            // keys of one load address
-constexpr int kListed = 256;            // granules whose places are listed at a time
 constexpr int kMostWorkgroups = 1024;
 constexpr int kChunkKeys = 32;          // keys of a wave's step on key chunks
+// A share of fewer keys costs more at the join than it saves before it.
+constexpr int kLeastShare = 128;
 constexpr float kLongestLine = 0x1p30f;
 static_assert(kGranule == kMinPage, "a granule lies in one page");
 
+// Of a workgroup of kWaves:
+template <bool kTile, int kWaves>
+constexpr int kStep = kTile ? kTileKeys : kChunkKeys * kWaves;  // keys of a step
+template <bool kSmall>
+constexpr int kListed = kSmall ? 128 : 256;  // granules whose places are listed at a time
+template <bool kTile, bool kSmall, int kWaves>
+constexpr int kSteps = kListed<kSmall> * kGranule / kStep<kTile, kWaves>;  // steps listed at a time
 template <bool kTile>
-constexpr int kStep = kTile ? kTileKeys : kChunkKeys * kWaves;  // keys of a workgroup's step
-template <bool kTile>
-constexpr int kSteps = kListed * kGranule / kStep<kTile>;  // steps listed at a time
-template <bool kTile>
-constexpr int kTileRows = kTile ? kWaveRows * kWaves : kWaveRows;
+constexpr int kTileRows = kTile ? kWaveRows * kTileWaves : kWaveRows;
 
 // ------------------------------------------------------------ the schedule --
 
@@ -168,12 +174,10 @@ struct Place {
 // What the workgroup shares.  The item and its place are kept here, not in registers,
 // while its keys are worked through.
 struct Shared {
-  float m[kWaves][kWaveRows];
-  float l[kWaves][kWaveRows];
+  float m[kMostWaves][kWaveRows];
+  float l[kMostWaves][kWaveRows];
   Place at;
   Item item;
-  int sums[kWaves];
-  float sizes[kWaves];
   int count;
   uint32_t last;
 };
@@ -193,9 +197,9 @@ __device__ __forceinline__ Item item_of(const Shared& sh) {
               uniform(i.from), uniform(i.to)};
 }
 
-template <bool kTile>
+template <bool kTile, int kWaves>
 __device__ __forceinline__ void range_of(const PagedArgs& p, Item& it) {
-  constexpr int kKeys = kStep<kTile>;
+  constexpr int kKeys = kStep<kTile, kWaves>;
   const int all = it.s.n_q * p.group;
   it.row0 = it.tile * kTileRows<kTile>;
   it.rows = std::min(kTileRows<kTile>, all - it.row0);
@@ -345,13 +349,13 @@ struct Source {
 
 // Lists where the item's steps [from, to) are, a granule each.  None: a page outside
 // the cache (flagged), or no key.
-template <bool kTile, bool kSmall>
+template <bool kTile, bool kSmall, int kWaves>
 __device__ __forceinline__ void list_pages(const PagedArgs& p, const Item& it, int from, int to, int tid, Listed* list, ListedScales* scales) {
-  constexpr int kEach = kStep<kTile> / kGranule;
+  constexpr int kKeys = kStep<kTile, kWaves>, kEach = kKeys / kGranule;
   const int n = (to - from) * kEach;
   const int32_t* row = p.table + static_cast<int64_t>(it.seq) * p.table_row;
-  for (int g = tid; g < n; g += kThreads) {
-    const int key = it.key_of<kStep<kTile>>(from + g / kEach) + g % kEach * kGranule;
+  for (int g = tid; g < n; g += 64 * kWaves) {
+    const int key = it.key_of<kKeys>(from + g / kEach) + g % kEach * kGranule;
     Listed l{Listed::kNone, Listed::kNone};
     ListedScales z{0, 0};
     if (key < it.end) {
@@ -395,11 +399,11 @@ struct Sight {
 
 // Key chunks: this wave's 32 keys of each of the item's steps [from, to), whose
 // pages are listed.
-template <typename T, int DP, bool kSmall, bool kCareful>
+template <typename T, int DP, bool kSmall, int kWaves, bool kCareful>
 __device__ __forceinline__ void run_chunk(const Source<T, DP, kSmall>& in, const Item& it, Rows<T, DP, true>& w, float c,
                                           const Sight& see, int from, int to, int wave, char* sk, char* sv) {
   using Src = Source<T, DP, kSmall>;
-  constexpr int kRow = Head<DP>::kRow, kKeys = kStep<false>, kEach = kKeys / kGranule;
+  constexpr int kRow = Head<DP>::kRow, kKeys = kStep<false, kWaves>, kEach = kKeys / kGranule;
   auto key_of = [&](int i) { return it.key_of<kKeys>(i) + wave * kChunkKeys; };
   auto place = [&](int i) { return (i - from) * kEach + wave * 2; };
   auto weigh_in = [&](f32x16& s, int at, typename VecOf<T>::v8 (&e)[2]) {
@@ -478,7 +482,7 @@ template <typename T, int DP, bool kSmall>
 __device__ __forceinline__ void run_tile(const Source<T, DP, kSmall>& in, const Item& it, Rows<T, DP, true>& w, float c,
                                          const Sight& see, int from, int to, int wave, WP_STAGED) {
   using Src = Source<T, DP, kSmall>;
-  constexpr int kKeys = kStep<true>, kEach = kKeys / kGranule;
+  constexpr int kKeys = kStep<true, kTileWaves>, kEach = kKeys / kGranule;
   const int mine = wave * kGranule * Head<DP>::kRow;
   // Steps past the last key that any of the wave's rows sees are not its work.
   const int live = std::min(to, see.last < 0 ? 0 : see.last < it.base ? std::min(it.sink_steps, see.last / kKeys + 1) : it.sink_steps + (see.last - it.base) / kKeys + 1);
@@ -546,7 +550,7 @@ template <typename T, int DP, bool kSmall>
 __device__ __forceinline__ void run_tile_careful(const Source<T, DP, kSmall>& in, const Item& it, Rows<T, DP, true>& w, float c,
                                                  const Sight& see, int from, int to, int wave, char* sk, char* sv) {
   using Src = Source<T, DP, kSmall>;
-  constexpr int kKeys = kStep<true>, kEach = kKeys / kGranule;
+  constexpr int kKeys = kStep<true, kTileWaves>, kEach = kKeys / kGranule;
   const int mine = wave * kGranule * Head<DP>::kRow;
   for (int i = from; i < to; ++i) {
     const int at = it.key_of<kKeys>(i), key = at + wave * kGranule, place = (i - from) * kEach + wave;
@@ -591,10 +595,10 @@ __device__ __forceinline__ void finish_row(const PagedArgs& p, const Item& it, i
 }
 
 // The workgroup's steps of one item.
-template <typename T, int DP, bool kSmall, bool kTile, int kSlotRows>
+template <typename T, int DP, bool kSmall, int kWaves, bool kTile, int kSlotRows>
 __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed* list, ListedScales* scales, WP_STAGED) {
   using H = Head<DP>;
-  constexpr int kBatch = kSteps<kTile>;
+  constexpr int kBatch = kSteps<kTile, kSmall, kWaves>, kThreads = 64 * kWaves;
   int tid = thread_number(), lane = tid & 63, half = lane >> 5;
   const int wave = uniform(tid >> 6);
   Item it = item_of(sh);
@@ -634,8 +638,10 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
     see.low = window_start(t1 + lag, p.window);
   }
   const Source<T, DP, kSmall> in(p, it, list, scales, lane);
-  char* my_k = (wave < 2 ? sk0 : sk1) + (wave & 1) * (Staged<DP>::kBytes / 2);
-  char* my_v = (wave < 2 ? sv0 : sv1) + (wave & 1) * (Staged<DP>::kBytes / 2);
+  // Key chunks: a wave's keys and values, and later its share of O.
+  constexpr int kHalf = Staged<DP>::kBytes / 2;
+  char* my_k = (kWaves == 2 || wave < 2 ? sk0 : sk1) + (wave & 1) * kHalf;
+  char* my_v = (kWaves == 2 || wave < 2 ? sv0 : sv1) + (wave & 1) * kHalf;
   // (The first steps are listed.)
   auto pass = [&](auto careful) {
     w.reset();
@@ -643,11 +649,11 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
       const int to = std::min(it.to, i + kBatch);
       if (i > it.from || decltype(careful)::value) {
         __syncthreads();  // the last batch's places and tiles have been read
-        list_pages<kTile, kSmall>(p, item_of(sh), i, to, thread_number(), list, scales);
+        list_pages<kTile, kSmall, kWaves>(p, item_of(sh), i, to, thread_number(), list, scales);
         __syncthreads();
       }
       if constexpr (!kTile)
-        run_chunk<T, DP, kSmall, decltype(careful)::value>(in, it, w, c, see, i, to, wave, my_k, my_v);
+        run_chunk<T, DP, kSmall, kWaves, decltype(careful)::value>(in, it, w, c, see, i, to, wave, my_k, my_v);
       else if constexpr (decltype(careful)::value)
         run_tile_careful(in, it, w, c, see, i, to, wave, sk0, sv0);
       else
@@ -713,7 +719,7 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
     const float fade = m == -INFINITY ? 1.f : exp2_fast(w.m - m);
     // (Columns swizzled by the row: whole rows apart, lanes would share banks.)
     auto place = [](int r, int d) { return (r * (DP / 4) + ((d / 4) ^ (r & (DP == 96 ? 7 : 15)))) * 16; };
-    auto area = [&](int i) -> char* { return i == 0 ? sk0 : i == 1 ? sk1 : i == 2 ? sv0 : sv1; };
+    auto area = [&](int i) -> char* { return i == 0 ? sk0 : i == 1 ? (kWaves == 2 ? sv0 : sk1) : i == 2 ? sv0 : sv1; };
     char* o32 = area(wave);
     if (real)
 #pragma unroll
@@ -759,8 +765,8 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
   __syncthreads();
   if (sh.last == 0u) return;
   // Where the shares are (a workgroup may have none).
-  int* slots = reinterpret_cast<int*>(list);
-  static_assert(kListed * sizeof(Listed) >= kMostWorkgroups * sizeof(int), "the list holds a slot for each workgroup");
+  int* slots = reinterpret_cast<int*>(sk0);
+  static_assert(Staged<DP>::kBytes >= kMostWorkgroups * sizeof(int), "there is room for a slot of each workgroup");
   if (wave == 0) {
     int n = 0;
     for (int i = first; i <= final; i += 64) {
@@ -780,6 +786,7 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
   // Several loads at once: of one place in many shares (few rows), or of
   // several places in a few (a tile's).
   const int count = sh.count, places = it.rows * (DP / 4);
+  const __amdgpu_buffer_rsrc_t shares = coherent_buffer(p.part, static_cast<uint32_t>(p.n_wg) * 2u * (kSlot * 4u));
   constexpr int kPlaces = kTile ? 4 : 1, kShares = kTile ? 2 : 16;
   for (int u0 = tid; u0 < places; u0 += kThreads * kPlaces) {
     float top[kPlaces], l[kPlaces];
@@ -795,12 +802,12 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
       f32x4 o[kShares][kPlaces];
 #pragma unroll
       for (int i = 0; i < kShares; ++i) {
-        const float* share = p.part + static_cast<uint64_t>(slots[std::min(i0 + i, count - 1)]) * kSlot;
+        const uint32_t share = static_cast<uint32_t>(slots[std::min(i0 + i, count - 1)]) * (kSlot * 4u);
 #pragma unroll
         for (int x = 0; x < kPlaces; ++x) {
           const int u = std::min(u0 + x * kThreads, places - 1), r = u / (DP / 4), d = u % (DP / 4) * 4;
-          ml[i][x] = __builtin_bit_cast(f32x2, coherent_load8(share + kSlotRows * DP + 2 * r));
-          o[i][x] = coherent_load_f4(share + r * DP + d);
+          ml[i][x] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(shares, share + (kSlotRows * DP + 2 * r) * 4u, 0, kSc1));
+          o[i][x] = coherent_load16(shares, share + (r * DP + d) * 4u);
         }
       }
 #pragma unroll
@@ -825,7 +832,7 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
 }
 
 // Clears the rows of no sequence: before the first bound and from the last one on.
-template <typename T>
+template <typename T, int kWaves>
 __device__ __forceinline__ void clear_rest(const PagedArgs& p) {
   const int lane = static_cast<int>(threadIdx.x) & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -842,49 +849,46 @@ __device__ __forceinline__ void clear_rest(const PagedArgs& p) {
   }
 }
 
+template <int kRoles>
+constexpr int kWavesOf = (kRoles & kTiles) != 0 ? kTileWaves : kChunkWaves;
+
 template <typename T, int DP, bool kSmall, int kRoles>
-__global__ __launch_bounds__(kThreads, 2) void paged_kernel(PagedArgs p) {
+__global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedArgs p) {
+  constexpr int kWaves = kWavesOf<kRoles>, kThreads = 64 * kWaves;
   constexpr int kSlotRows = (kRoles & kTiles) != 0 ? kTileRows<true> : kTileRows<false>;
   __shared__ Shared sh;
-  __shared__ Listed list[kListed];
-  __shared__ ListedScales scales[kSmall ? kListed : 1];
+  __shared__ Listed list[kListed<kSmall>];
+  __shared__ ListedScales scales[kSmall ? kListed<kSmall> : 1];
   __shared__ __align__(1024) char sk0[Staged<DP>::kBytes];
-  __shared__ __align__(1024) char sk1[Staged<DP>::kBytes];
   __shared__ __align__(1024) char sv0[Staged<DP>::kBytes];
-  __shared__ __align__(1024) char sv1[Staged<DP>::kBytes];
   touch_kernel_args<static_cast<int>(sizeof(PagedArgs))>();
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  // A thread for each sequence, and the sum of their costs.
+  // Every wave by itself: a lane for each sequence, 64 at a time, and the sum of
+  // their costs.
   auto cost_at = [&](int b, Shape& s) {
+    s = Shape{0, 0, 0};
     if (b >= p.n_seq) return 0;
     s = shape_of(p, b);
     const Cost c = cost_of(p, s);
     return c.before(c.tiles) * p.kv_heads;
   };
-  Shape my_shape{0, 0, 0}, other;
-  const int mine = cost_at(tid, my_shape);
+  Shape first, other;
+  const int mine = cost_at(lane, first);
   int sum = mine;
-  float size = static_cast<float>(mine);
-  for (int b = tid + kThreads; b < p.n_seq; b += kThreads) {
+  float length = static_cast<float>(mine);
+  for (int b = lane + 64; b < p.n_seq; b += 64) {
     const int v = cost_at(b, other);
     sum += v;
-    size += static_cast<float>(v);
+    length += static_cast<float>(v);
   }
-  clear_rest<T>(p);
-  const int up0 = sum_up(sum);
-  size = wave_sum(size);
-  if (lane == 63) {
-    sh.sums[wave] = up0;
-    sh.sizes[wave] = size;
-  }
-  __syncthreads();
+  clear_rest<T, kWaves>(p);
+  const int total = total_of(sum);
+  length = wave_sum(length);
   // Bounds that fall can give sequences more rows than there are, and a line
   // past its 31 bits: such a call does nothing.
-  if (sh.sizes[0] + sh.sizes[1] + sh.sizes[2] + sh.sizes[3] > kLongestLine) return;
-  const int total = sh.sums[0] + sh.sums[1] + sh.sums[2] + sh.sums[3];
-  const int share = over(total, p.by_wg) + 1;
+  if (__builtin_amdgcn_readlane(__builtin_bit_cast(int, length), 63) > __builtin_bit_cast(int, kLongestLine)) return;
+  const int share = std::max(over(total, p.by_wg) + 1, p.least_share);
   // Tiles: neighbours on the line, which read the same keys, on one die.  Chunks
   // read keys of their own, and the dies share out all kinds of items.
   const int block = static_cast<int>(blockIdx.x), dies = (kRoles & kTiles) != 0 && p.n_wg % 8 == 0 ? 8 : 1;
@@ -893,29 +897,22 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(PagedArgs p) {
   if (x0_wide >= total) return;
   const int x0 = static_cast<int>(x0_wide), x1 = static_cast<int>(std::min<long long>(total, x0_wide + share));
   // The sequence at x0, its start on the line, and from there the tile.
-  if (tid == 0) sh.item.seq = -1;
-  int run = 0;
-  for (int b0 = 0; b0 < p.n_seq && run <= x0; b0 += kThreads) {
-    const int v = b0 == 0 ? mine : cost_at(b0 + tid, my_shape);
+  int seq = -1, head, tile, start = 0;
+  Shape s{0, 0, 0};
+  for (int b0 = 0; b0 < p.n_seq; b0 += 64) {
+    const int v = b0 == 0 ? mine : cost_at(b0 + lane, first);
     const int up = sum_up(v);
-    __syncthreads();  // the sums have been read
-    if (lane == 63) sh.sums[wave] = up;
-    __syncthreads();
-    int before = run;
-    for (int i = 0; i < kWaves; ++i) {
-      if (i < wave) before += sh.sums[i];
-      run += sh.sums[i];
+    const unsigned long long past = __ballot(start + up > x0);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      seq = b0 + at;
+      start += __builtin_amdgcn_readlane(up, at) - __builtin_amdgcn_readlane(v, at);
+      s = Shape{__builtin_amdgcn_readlane(first.q0, at), __builtin_amdgcn_readlane(first.n_q, at), __builtin_amdgcn_readlane(first.n_k, at)};
+      break;
     }
-    if (before + up - v <= x0 && x0 < before + up) {
-      sh.item.seq = b0 + tid;
-      sh.item.s = my_shape;
-      sh.at.start = before + up - v;
-    }
+    start += __builtin_amdgcn_readlane(up, 63);
   }
-  __syncthreads();
-  int seq = uniform(sh.item.seq), head, tile, start = uniform(sh.at.start);
   if (seq < 0) return;  // (lengths that change under the call)
-  Shape s{uniform(sh.item.s.q0), uniform(sh.item.s.n_q), uniform(sh.item.s.n_k)};
   Cost c = cost_of(p, s);
   {
     const int per_head = c.before(c.tiles);
@@ -931,7 +928,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(PagedArgs p) {
     it.tile = tile;
     it.s = s;
     const bool tiled = (kRoles & kTiles) != 0 && c.log_rows == 7;
-    if (tiled) range_of<true>(p, it); else range_of<false>(p, it);
+    if (tiled) range_of<true, kWaves>(p, it); else range_of<false, kWaves>(p, it);
     Place at;
     at.start = start;
     at.cost = c.before(tile + 1) - c.before(tile);
@@ -948,14 +945,20 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(PagedArgs p) {
         sh.at = at;
       }
       if (tiled)
-        list_pages<true, kSmall>(p, it, it.from, std::min(it.to, it.from + kSteps<true>), thread_number(), list, scales);
+        list_pages<true, kSmall, kWaves>(p, it, it.from, std::min(it.to, it.from + kSteps<true, kSmall, kWaves>), thread_number(), list, scales);
       else
-        list_pages<false, kSmall>(p, it, it.from, std::min(it.to, it.from + kSteps<false>), thread_number(), list, scales);
+        list_pages<false, kSmall, kWaves>(p, it, it.from, std::min(it.to, it.from + kSteps<false, kSmall, kWaves>), thread_number(), list, scales);
       __syncthreads();
-      if ((kRoles & kTiles) != 0 && tiled)
-        run_item<T, DP, kSmall, true, kSlotRows>(p, sh, list, scales, sk0, sk1, sv0, sv1);
-      else
-        run_item<T, DP, kSmall, false, kSlotRows>(p, sh, list, scales, sk0, sk1, sv0, sv1);
+      if constexpr ((kRoles & kTiles) != 0) {
+        __shared__ __align__(1024) char sk1[Staged<DP>::kBytes];
+        __shared__ __align__(1024) char sv1[Staged<DP>::kBytes];
+        if (tiled)
+          run_item<T, DP, kSmall, kWaves, true, kSlotRows>(p, sh, list, scales, sk0, sk1, sv0, sv1);
+        else
+          run_item<T, DP, kSmall, kWaves, false, kSlotRows>(p, sh, list, scales, sk0, sk1, sv0, sv1);
+      } else {
+        run_item<T, DP, kSmall, kWaves, false, kSlotRows>(p, sh, list, scales, sk0, sk0, sv0, sv0);
+      }
     }
     start += at.cost;
     if (start >= x1) return;
@@ -974,7 +977,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_kernel(PagedArgs p) {
 
 template <typename T, int DP, bool kSmall>
 hipError_t launch(const PagedArgs& a, bool tiles, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(a.n_wg)), block(kThreads);
+  const dim3 grid(static_cast<uint32_t>(a.n_wg)), block(64 * (tiles ? kTileWaves : kChunkWaves));
   if (tiles)
     hipLaunchKernelGGL((paged_kernel<T, DP, kSmall, kTiles | kChunks>), grid, block, 0, stream, a);
   else
@@ -998,7 +1001,8 @@ hipError_t launch_paged_attention(int dtype_bf16, PagedArgs& a, int n_cu, hipStr
   // Sequences of few rows on the whole run on key chunks, in tiles of 32 rows.
   const bool tiles = rows > static_cast<int64_t>(kWaveRows) * std::max(1, a.n_seq);
   a.chunk_rows = tiles ? kWaveRows : 0x7FFFFFFF;
-  a.n_wg = std::min(2 * n_cu, kMostWorkgroups);
+  // As many workgroups as the device holds at a time: eight waves a compute unit.
+  a.n_wg = std::min(8 / (tiles ? kTileWaves : kChunkWaves) * n_cu, kMostWorkgroups);
   a.by_wg = divisor_of(a.n_wg);
   const int dp = a.dim <= 64 ? 64 : a.dim <= 96 ? 96 : 128;
   const uint64_t slots = 2ull * a.n_wg * (tiles ? kTileRows<true> : kTileRows<false>) * (dp + 2) * 4;
@@ -1010,6 +1014,7 @@ hipError_t launch_paged_attention(int dtype_bf16, PagedArgs& a, int n_cu, hipStr
   a.cost_shift = 0;
   while (a.cost_shift < 31 && std::ldexp(most, -a.cost_shift) + a.kv_heads * tiles_most > 0x1p30) ++a.cost_shift;
   if (a.cost_shift == 31) return hipErrorInvalidValue;
+  a.least_share = std::max(1, (kLeastShare * a.group) >> a.cost_shift);
   if (dtype_bf16) return a.e4m3 ? launch_head<__bf16, true>(a, tiles, stream) : launch_head<__bf16, false>(a, tiles, stream);
   return a.e4m3 ? launch_head<_Float16, true>(a, tiles, stream) : launch_head<_Float16, false>(a, tiles, stream);
 }
