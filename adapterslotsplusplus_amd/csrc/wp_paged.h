@@ -86,7 +86,7 @@ struct PagedArgs {
   int32_t chunk_rows;  // most rows per key head of a sequence that runs on key chunks
   int32_t n_wg;
   Divisor by_wg;
-  int32_t cost_shift, least_share;
+  int32_t cost_shift;
 };
 hipError_t launch_paged_attention(int dtype_bf16, PagedArgs& a, int n_cu, hipStream_t stream);
 

@@ -45,8 +45,7 @@ constexpr int kTiles = 1, kChunks = 2;  // the roles of a launch
 constexpr int kGranule = 16;            // keys of one load address
 constexpr int kMostWorkgroups = 1024;
 constexpr int kChunkKeys = 32;          // keys of a wave's step on key chunks
-// A share of fewer keys costs more at the join than it saves before it.
-constexpr int kLeastShare = 128;
+constexpr int kMostPieces = 32;  // of a tile: more take longer to join than they save
 constexpr float kLongestLine = 0x1p30f;
 static_assert(kGranule == kMinPage, "a granule lies in one page");
 
@@ -83,8 +82,10 @@ __device__ __forceinline__ Shape shape_of(const PagedArgs& p, int b) {
 struct Cost {
   long long lag, least, most;
   int extra, tiles, log_rows, shift;
+  int pieces;  // of each tile, or 0: the line is one of costs
   // Where tile t starts, from the sequence's start.
   __device__ __forceinline__ int before(int t) const {
+    if (pieces > 0) return t * pieces;
     if (t == 0) return 0;
     if (t == 1) {
       const long long keys = lag + (1 << log_rows);
@@ -107,6 +108,7 @@ __device__ __forceinline__ Cost cost_of(const PagedArgs& p, const Shape& s) {
   c.extra = 128 * p.group;
   c.most = p.window > 0 ? (static_cast<long long>(p.window) + p.sinks + 128) * p.group + (1 << c.log_rows) : (1ll << 60);
   c.shift = p.cost_shift;
+  c.pieces = 0;
   return c;
 }
 
@@ -123,6 +125,13 @@ __device__ __forceinline__ float wave_sum(float v) {
   add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
   add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
   return v;
+}
+
+// The largest of the wave's numbers.
+__device__ __forceinline__ int longest_of(int v) {
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) v = std::max(v, __shfl_xor(v, i));
+  return __builtin_amdgcn_readfirstlane(v);
 }
 
 // The tile at place y from the sequence's start: 64 places a round.
@@ -158,7 +167,8 @@ struct Item {
 struct Place {
   int start, cost;
   int total, share, near;
-  int id;  // this workgroup's
+  int pieces;  // of each tile (Cost)
+  int id;      // this workgroup's
   // The item's step at which the line's point x cuts it.  Cuts near its ends are
   // moved there: a cut costs the shares' way through memory.
   __device__ __forceinline__ int cut(int x, int steps) const {
@@ -166,7 +176,7 @@ struct Place {
     if (off <= 0) return 0;
     if (rest <= 0) return steps;
     if (std::min(off, rest) < near) return off <= rest ? 0 : steps;
-    return std::min(steps, static_cast<int>(static_cast<float>(off) * __builtin_amdgcn_rcpf(static_cast<float>(cost)) * static_cast<float>(steps)));
+    return std::min(steps, static_cast<int>(static_cast<float>(off) * __builtin_amdgcn_rcpf(static_cast<float>(cost)) * static_cast<float>(steps) + 0.01f));
   }
   __device__ __forceinline__ int from(int i) const { return static_cast<int>(std::min<long long>(total, static_cast<long long>(i) * share)); }
 };
@@ -874,7 +884,7 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
     return c.before(c.tiles) * p.kv_heads;
   };
   Shape first, other;
-  const int mine = cost_at(lane, first);
+  int mine = cost_at(lane, first);
   int sum = mine;
   float length = static_cast<float>(mine);
   for (int b = lane + 64; b < p.n_seq; b += 64) {
@@ -883,19 +893,47 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
     length += static_cast<float>(v);
   }
   clear_rest<T, kWaves>(p);
-  const int total = total_of(sum);
+  int total = total_of(sum);
   length = wave_sum(length);
   // Bounds that fall can give sequences more rows than there are, and a line
   // past its 31 bits: such a call does nothing.
   if (__builtin_amdgcn_readlane(__builtin_bit_cast(int, length), 63) > __builtin_bit_cast(int, kLongestLine)) return;
-  const int share = std::max(over(total, p.by_wg) + 1, p.least_share);
+  int share = over(total, p.by_wg) + 1, pieces = 0;
+  if (p.n_seq <= 64) {
+    // A line of pieces, one for each workgroup, where that is as short: a tile's
+    // keys in equal pieces, and no workgroup with an end of one item and a start of another.
+    const Cost c = cost_of(p, first);
+    const int step = c.log_rows == 7 ? kStep<true, kWaves> : kStep<false, kWaves>;
+    const int keys = std::max(1, p.window > 0 ? static_cast<int>(std::min<long long>(first.n_k, static_cast<long long>(p.window) + p.sinks + 128)) : first.n_k);
+    const float tiles = static_cast<float>(c.tiles) * p.kv_heads, all = tiles * keys;
+    auto whole = [&](float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_sum(v)), 63)); };
+    if (whole(tiles) <= p.n_wg) {
+      // The shortest pieces of which there are no more than workgroups (whole tiles are few enough).
+      float size = std::max(64.f, whole(all) / p.n_wg);
+      auto pieces_of = [&](float size) {
+        return std::clamp(static_cast<int>(static_cast<float>(keys) * __builtin_amdgcn_rcpf(size) + 0.99f), 1, kMostPieces);
+      };
+      while (whole(tiles * pieces_of(size)) > p.n_wg) size *= 1.125f;
+      pieces = pieces_of(size);
+      const int longest = longest_of(c.tiles > 0 ? std::max(step, (keys + pieces - 1) / pieces) : 0);
+      const long long slack = (kRoles & kTiles) != 0 ? 768 : 256;
+      if (static_cast<long long>(longest) * p.group > (static_cast<long long>(share) << p.cost_shift) + slack * p.group) pieces = 0;
+      else share = 1;
+    }
+  }
   // Tiles: neighbours on the line, which read the same keys, on one die.  Chunks
   // read keys of their own, and the dies share out all kinds of items.
   const int block = static_cast<int>(blockIdx.x), dies = (kRoles & kTiles) != 0 && p.n_wg % 8 == 0 ? 8 : 1;
-  const int id = block % dies * (p.n_wg / dies) + block / dies;
+  int id = block % dies * (p.n_wg / dies) + block / dies;
+  if (pieces > 0) {
+    Cost c = cost_of(p, first);
+    c.pieces = pieces;
+    mine = c.tiles * pieces * p.kv_heads;
+    total = total_of(mine);
+  }
   const long long x0_wide = static_cast<long long>(id) * share;
   if (x0_wide >= total) return;
-  const int x0 = static_cast<int>(x0_wide), x1 = static_cast<int>(std::min<long long>(total, x0_wide + share));
+  int x0 = static_cast<int>(x0_wide), x1 = static_cast<int>(std::min<long long>(total, x0_wide + share));
   // The sequence at x0, its start on the line, and from there the tile.
   int seq = -1, head, tile, start = 0;
   Shape s{0, 0, 0};
@@ -907,6 +945,7 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
       const int at = __builtin_ctzll(past);
       seq = b0 + at;
       start += __builtin_amdgcn_readlane(up, at) - __builtin_amdgcn_readlane(v, at);
+      pieces = __builtin_amdgcn_readlane(pieces, at);
       s = Shape{__builtin_amdgcn_readlane(first.q0, at), __builtin_amdgcn_readlane(first.n_q, at), __builtin_amdgcn_readlane(first.n_k, at)};
       break;
     }
@@ -914,6 +953,7 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
   }
   if (seq < 0) return;  // (lengths that change under the call)
   Cost c = cost_of(p, s);
+  c.pieces = pieces;
   {
     const int per_head = c.before(c.tiles);
     head = uniform((x0 - start) / per_head);
@@ -922,23 +962,26 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
     start = uniform(start + c.before(tile));
   }
   for (;;) {
-    Item it;
-    it.seq = seq;
-    it.head = head;
-    it.tile = tile;
-    it.s = s;
-    const bool tiled = (kRoles & kTiles) != 0 && c.log_rows == 7;
-    if (tiled) range_of<true, kWaves>(p, it); else range_of<false, kWaves>(p, it);
-    Place at;
-    at.start = start;
-    at.cost = c.before(tile + 1) - c.before(tile);
-    at.total = total;
-    at.share = share;
-    at.near = std::min(share >> 3, ((tiled ? 512 : 128) * p.group) >> p.cost_shift);
-    at.id = id;
-    it.from = uniform(at.cut(x0, it.steps));
-    it.to = uniform(at.cut(std::min(x1, start + at.cost), it.steps));
-    if (it.to > it.from) {
+    {
+      Item it;
+      it.seq = seq;
+      it.head = head;
+      it.tile = tile;
+      it.s = s;
+      Cost c = cost_of(p, s);
+      c.pieces = pieces;
+      const bool tiled = (kRoles & kTiles) != 0 && c.log_rows == 7;
+      if (tiled) range_of<true, kWaves>(p, it); else range_of<false, kWaves>(p, it);
+      Place at;
+      at.start = start;
+      at.cost = c.before(tile + 1) - c.before(tile);
+      at.total = total;
+      at.share = share;
+      at.near = pieces > 0 ? 0 : std::min(share >> 3, ((tiled ? 512 : 128) * p.group) >> p.cost_shift);
+      at.id = id;
+      at.pieces = pieces;
+      it.from = uniform(at.cut(x0, it.steps));
+      it.to = uniform(at.cut(std::min(x1, start + at.cost), it.steps));
       __syncthreads();  // what the item before left in LDS has been read
       if (tid == 0) {
         sh.item = it;
@@ -949,10 +992,12 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
       else
         list_pages<false, kSmall, kWaves>(p, it, it.from, std::min(it.to, it.from + kSteps<false, kSmall, kWaves>), thread_number(), list, scales);
       __syncthreads();
+    }
+    if (uniform(sh.item.to) > uniform(sh.item.from)) {
       if constexpr ((kRoles & kTiles) != 0) {
         __shared__ __align__(1024) char sk1[Staged<DP>::kBytes];
         __shared__ __align__(1024) char sv1[Staged<DP>::kBytes];
-        if (tiled)
+        if (uniform(sh.item.s.n_q) * p.group > p.chunk_rows)
           run_item<T, DP, kSmall, kWaves, true, kSlotRows>(p, sh, list, scales, sk0, sk1, sv0, sv1);
         else
           run_item<T, DP, kSmall, kWaves, false, kSlotRows>(p, sh, list, scales, sk0, sk1, sv0, sv1);
@@ -960,18 +1005,29 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
         run_item<T, DP, kSmall, kWaves, false, kSlotRows>(p, sh, list, scales, sk0, sk0, sv0, sv0);
       }
     }
-    start += at.cost;
+    // The next tile, key head or sequence with rows, if it is before the share's end.
+    const Place at = sh.at;
+    total = uniform(at.total);
+    share = uniform(at.share);
+    pieces = uniform(at.pieces);
+    id = uniform(at.id);
+    x0 = at.from(id);
+    x1 = at.from(id + 1);
+    start = uniform(at.start + at.cost);
     if (start >= x1) return;
-    // The next tile, key head or sequence with rows (there is one, as the line goes on).
-    if (++tile < c.tiles) continue;
+    const Item it = item_of(sh);
+    seq = it.seq;
+    head = it.head;
+    tile = it.tile + 1;
+    s = it.s;
+    if (tile < cost_of(p, s).tiles) continue;
     tile = 0;
     if (++head < p.kv_heads) continue;
     head = 0;
-    do {
+    do {  // (there is one, as the line goes on)
       if (++seq >= p.n_seq) return;
       s = shape_of(p, seq);
-      c = cost_of(p, s);
-    } while (c.tiles == 0);
+    } while (cost_of(p, s).tiles == 0);
   }
 }
 
@@ -1014,7 +1070,6 @@ hipError_t launch_paged_attention(int dtype_bf16, PagedArgs& a, int n_cu, hipStr
   a.cost_shift = 0;
   while (a.cost_shift < 31 && std::ldexp(most, -a.cost_shift) + a.kv_heads * tiles_most > 0x1p30) ++a.cost_shift;
   if (a.cost_shift == 31) return hipErrorInvalidValue;
-  a.least_share = std::max(1, (kLeastShare * a.group) >> a.cost_shift);
   if (dtype_bf16) return a.e4m3 ? launch_head<__bf16, true>(a, tiles, stream) : launch_head<__bf16, false>(a, tiles, stream);
   return a.e4m3 ? launch_head<_Float16, true>(a, tiles, stream) : launch_head<_Float16, false>(a, tiles, stream);
 }
