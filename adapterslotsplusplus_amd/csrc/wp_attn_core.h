@@ -92,16 +92,84 @@ __device__ __forceinline__ int sum_up(int v) {
 }
 __device__ __forceinline__ int total_of(int v) { return __builtin_amdgcn_readlane(sum_up(v), 63); }
 
-// The lane that a wave's work goes by: the thread's own number or (kHeld) one
-// that a kernel keeps, in a form that the compiler takes for a number of that moment alone.
+// K fragment of step `step`: keys row0 .. row0 + 31 of a staged tile.
+template <typename T, int DP>
+__device__ __forceinline__ typename VecOf<T>::v8 key_fragment(const char* keys, int row0, int step, int lane) {
+  using H = Head<DP>;
+  const int r = lane & 31, c = step * 2 + (lane >> 5);
+  return *reinterpret_cast<const typename VecOf<T>::v8*>(keys + (row0 + r) * H::kRow + ((c ^ H::key_swizzle(r)) << 4));
+}
+
+// Four keys of a column at `at`, and the four that are eight rows on.
+template <typename T, int DP, bool kCareful>
+__device__ __forceinline__ typename VecOf<T>::v8 value_at(const char* values, int at) {
+  using H = Head<DP>;
+  using L = __attribute__((address_space(3))) i16x4;
+  i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(values + at));
+  i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(values + (at + 8 * H::kRow)));
+  if (kCareful) {
+    lo = finite_only<T>(lo);
+    hi = finite_only<T>(hi);
+  }
+  union {
+    i16x4 h[2];
+    typename VecOf<T>::v8 v;
+  } u;
+  u.h[0] = lo;
+  u.h[1] = hi;
+  return u.v;
+}
+
+// V^T fragment of columns col * 32 .. + 31 and the 16 keys from key0, in the
+// order of the packed exponentials: lane half h has keys 4h .. 4h + 3 and
+// 8 + 4h .. 8 + 4h + 3.
+template <typename T, int DP, bool kCareful>
+__device__ __forceinline__ typename VecOf<T>::v8 value_fragment(const char* values, int key0, int col, int lane) {
+  using H = Head<DP>;
+  const int i = lane & 15, g = lane >> 4;
+  const int r = 4 * (g >> 1) + (i >> 2);
+  const int c = col * 4 + (g & 1) * 2 + ((i & 3) >> 1);
+  return value_at<T, DP, kCareful>(values, (key0 + r) * H::kRow + ((c ^ H::value_swizzle(r)) << 4) + (i & 1) * 8);
+}
+
+// The lane that a wave's work goes by, and its fragments: the thread's own
+// number or (kHeld) one that a kernel keeps, in a form that the compiler takes for a number of
+// that moment alone.  Then one address of either kind is kept, too: a step or a column on
+// changes bits of it that no row touches.
 template <bool kHeld>
 struct Lane {
   __device__ __forceinline__ int lane() const { return static_cast<int>(threadIdx.x) & 63; }
+  __device__ __forceinline__ void renew() {}
+  template <typename T, int DP>
+  __device__ __forceinline__ typename VecOf<T>::v8 key(const char* keys, int row0, int step) const {
+    return key_fragment<T, DP>(keys, row0, step, lane());
+  }
+  template <typename T, int DP, bool kCareful>
+  __device__ __forceinline__ typename VecOf<T>::v8 value(const char* values, int key0, int col) const {
+    return value_fragment<T, DP, kCareful>(values, key0, col, lane());
+  }
 };
 template <>
 struct Lane<true> {
-  int held;
+  int held, key_place, value_place;
   __device__ __forceinline__ int lane() const { return held; }
+  template <int DP>
+  __device__ __forceinline__ void hold(int lane) {
+    using H = Head<DP>;
+    held = lane;
+    const int k = lane & 31, i = lane & 15, g = lane >> 4, v = 4 * (g >> 1) + (i >> 2);
+    key_place = k * H::kRow + (((lane >> 5) ^ H::key_swizzle(k)) << 4);
+    value_place = v * H::kRow + ((((g & 1) * 2 + ((i & 3) >> 1)) ^ H::value_swizzle(v)) << 4) + (i & 1) * 8;
+  }
+  __device__ __forceinline__ void renew() { asm volatile("" : "+v"(key_place), "+v"(value_place)); }
+  template <typename T, int DP>
+  __device__ __forceinline__ typename VecOf<T>::v8 key(const char* keys, int row0, int step) const {
+    return *reinterpret_cast<const typename VecOf<T>::v8*>(keys + (key_place ^ (step << 5)) + row0 * Head<DP>::kRow);
+  }
+  template <typename T, int DP, bool kCareful>
+  __device__ __forceinline__ typename VecOf<T>::v8 value(const char* values, int key0, int col) const {
+    return value_at<T, DP, kCareful>(values, (value_place ^ (col << 6)) + key0 * Head<DP>::kRow);
+  }
 };
 
 // A wave's 32 query rows and their running state.
@@ -156,40 +224,6 @@ __device__ __forceinline__ float top_of(const f32x16& s) {
 #pragma unroll
   for (int e = 2; e < 16; e += 2) t = fmaxf(fmaxf(t, s[e]), s[e + 1]);
   return t;
-}
-
-// K fragment of step `step`: keys row0 .. row0 + 31 of a staged tile.
-template <typename T, int DP>
-__device__ __forceinline__ typename VecOf<T>::v8 key_fragment(const char* keys, int row0, int step, int lane) {
-  using H = Head<DP>;
-  const int r = lane & 31, c = step * 2 + (lane >> 5);
-  return *reinterpret_cast<const typename VecOf<T>::v8*>(keys + (row0 + r) * H::kRow + ((c ^ H::key_swizzle(r)) << 4));
-}
-
-// V^T fragment of columns col * 32 .. + 31 and the 16 keys from key0, in the
-// order of the packed exponentials: lane half h has keys 4h .. 4h + 3 and
-// 8 + 4h .. 8 + 4h + 3.
-template <typename T, int DP, bool kCareful>
-__device__ __forceinline__ typename VecOf<T>::v8 value_fragment(const char* values, int key0, int col, int lane) {
-  using H = Head<DP>;
-  const int i = lane & 15, g = lane >> 4;
-  const int r = 4 * (g >> 1) + (i >> 2);
-  const int c = col * 4 + (g & 1) * 2 + ((i & 3) >> 1);
-  const int at = (key0 + r) * H::kRow + ((c ^ H::value_swizzle(r)) << 4) + (i & 1) * 8;
-  using L = __attribute__((address_space(3))) i16x4;
-  i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(values + at));
-  i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(values + (at + 8 * H::kRow)));
-  if (kCareful) {
-    lo = finite_only<T>(lo);
-    hi = finite_only<T>(hi);
-  }
-  union {
-    i16x4 h[2];
-    typename VecOf<T>::v8 v;
-  } u;
-  u.h[0] = lo;
-  u.h[1] = hi;
-  return u.v;
 }
 
 // Adds the infinite and NaN values of n staged keys that a query sees (sees(r):
@@ -248,13 +282,13 @@ __device__ __forceinline__ f32x16 scores(const Rows<T, DP, kHeld>& w, const char
   constexpr int kSteps = Head<DP>::kSteps;
   typename VecOf<T>::v8 kf[4];
 #pragma unroll
-  for (int x = 0; x < 4; ++x) kf[x] = key_fragment<T, DP>(keys, row0, x, w.lane());
+  for (int x = 0; x < 4; ++x) kf[x] = w.template key<T, DP>(keys, row0, x);
   __builtin_amdgcn_sched_barrier(0);
   f32x16 s{};
 #pragma unroll
   for (int x = 0; x < kSteps; ++x) {
     s = mfma32(kf[x % 4], w.q[x], s);
-    if (x + 4 < kSteps) kf[x % 4] = key_fragment<T, DP>(keys, row0, x + 4, w.lane());
+    if (x + 4 < kSteps) kf[x % 4] = w.template key<T, DP>(keys, row0, x + 4);
     __builtin_amdgcn_sched_barrier(0);
   }
   return s;
@@ -265,7 +299,7 @@ template <typename T, int DP, bool kCareful, bool kHeld>
 __device__ __forceinline__ void accumulate(Rows<T, DP, kHeld>& w, const char* values, int row0,
                                            const typename VecOf<T>::v8 (&e)[2]) {
   constexpr int kCols = Head<DP>::kCols, kAhead = kCols < 4 ? kCols : 4;
-  auto value = [&](int i) { return value_fragment<T, DP, kCareful>(values, row0 + i / kCols * 16, i % kCols, w.lane()); };
+  auto value = [&](int i) { return w.template value<T, DP, kCareful>(values, row0 + i / kCols * 16, i % kCols); };
   typename VecOf<T>::v8 vf[kAhead];
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) vf[i] = value(i);
@@ -293,6 +327,7 @@ __device__ __forceinline__ void tile_body(Rows<T, DP, kHeld>& w, f32x16& s0, f32
                                           const char* knext, const char* vnow) {
   using H = Head<DP>;
   using V8 = typename VecOf<T>::v8;
+  w.renew();
   constexpr int kScores = 2 * H::kSteps, kFirst = kScores * 3 / 4, kValues = 2 * H::kCols;
   w.raise(tops, c);
   const float base = w.m == -INFINITY ? 0.f : w.m;
@@ -303,8 +338,8 @@ __device__ __forceinline__ void tile_body(Rows<T, DP, kHeld>& w, f32x16& s0, f32
       w.l += s[i];
     }
   };
-  auto key = [&](int i) { return key_fragment<T, DP>(knext, i / H::kSteps * 32, i % H::kSteps, w.lane()); };
-  auto value = [&](int i) { return value_fragment<T, DP, false>(vnow, i / H::kCols * 16, i % H::kCols, w.lane()); };
+  auto key = [&](int i) { return w.template key<T, DP>(knext, i / H::kSteps * 32, i % H::kSteps); };
+  auto value = [&](int i) { return w.template value<T, DP, false>(vnow, i / H::kCols * 16, i % H::kCols); };
   f32x16 n[2] = {};
   V8 kf[3], vf[3], e[4];
   if (more) {

@@ -225,6 +225,14 @@ __device__ __forceinline__ void range_of(const PagedArgs& p, Item& it) {
 
 // ---------------------------------------------------------- keys and values --
 
+// A buffer of `size` bytes.  (Its flags are a new number to the compiler each time: it
+// would else keep the whole descriptor from load to load, in lanes of vector registers.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* src, int size) {
+  int flags = 0x00020000;
+  asm volatile("" : "+s"(flags));
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(src), 0, size, flags);
+}
+
 // Loads of one granule of keys or values.  16 bits: load i fills rows i *
 // kRowsPerLoad on straight in LDS.  8 bits: rows to registers, 16 elements a
 // lane, and from there, in the queries' type, to LDS.  Offsets from the
@@ -257,15 +265,16 @@ struct Granule {
   __device__ __forceinline__ int bytes(int rows) const { return rows <= 0 ? 0 : (std::min(rows, kGranule) - 1) * stride + row_bytes; }
 
   __device__ __forceinline__ void stage(const char* src, int rows, char* dst) const {
-    const int size = bytes(rows);
+    const __amdgpu_buffer_rsrc_t b = buffer_of(src, bytes(rows));
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) load_to_lds(src, dst + i * 1024, off[i], 0, size);
+    for (int i = 0; i < kLoads; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void*)(dst + i * 1024), 16, off[i], 0, 0, 0);
   }
 
   __device__ __forceinline__ void fetch(const char* src, const uint8_t* scales, int rows, Held& h) const {
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(src), 0, bytes(rows), 0x00020000);
+    const __amdgpu_buffer_rsrc_t r = buffer_of(src, bytes(rows));
     const int scale_size = rows <= 0 ? 0 : (std::min(rows, kGranule) - 1) * scale_stride + 1;
-    const __amdgpu_buffer_rsrc_t s = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(scales), 0, scale_size, 0x00020000);
+    const __amdgpu_buffer_rsrc_t s = buffer_of(scales, scale_size);
     const int row = lane / kLanes;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -494,8 +503,6 @@ __device__ __forceinline__ void run_tile(const Source<T, DP, kSmall>& in, const 
   using Src = Source<T, DP, kSmall>;
   constexpr int kKeys = kStep<true, kTileWaves>, kEach = kKeys / kGranule;
   const int mine = wave * kGranule * Head<DP>::kRow;
-  // Steps past the last key that any of the wave's rows sees are not its work.
-  const int live = std::min(to, see.last < 0 ? 0 : see.last < it.base ? std::min(it.sink_steps, see.last / kKeys + 1) : it.sink_steps + (see.last - it.base) / kKeys + 1);
   auto key_of = [&](int i) { return it.key_of<kKeys>(i); };
   auto place = [&](int i) { return (i - from) * kEach + wave; };
   typename Src::K::Held hk;
@@ -531,21 +538,24 @@ __device__ __forceinline__ void run_tile(const Source<T, DP, kSmall>& in, const 
   meet();
   load_k(from + 1, sk1);
   load_v(from, sv0);
-  f32x16 s0 = scores(w, sk0, 0), s1 = scores(w, sk0, 32);
-  float tops = fmaxf(top_of(s0), top_of(s1));
-  auto step = [&](int i, char* kfree, const char* knext, const char* vnow, char* vnext) {
+  auto next = [&](int i, char* kfree, char* vnext) {
     meet();
     load_k(i + 2, kfree);
     load_v(i + 1, vnext);
-    if (i >= live) return;
+  };
+  f32x16 s0 = scores(w, sk0, 0), s1 = scores(w, sk0, 32);
+  float tops = fmaxf(top_of(s0), top_of(s1));
+  auto step = [&](int i, char* kfree, const char* knext, const char* vnow, char* vnext) {
+    next(i, kfree, vnext);
     const int at = key_of(i);
     if (!see.whole(at, kKeys)) {
       mask_seen(w, s0, at, see.sinks);
       mask_seen(w, s1, at + 32, see.sinks);
       tops = fmaxf(top_of(s0), top_of(s1));
     }
-    // (After the last step the next one's scores are of no use, and cost less
-    // than a second copy of this, without them, costs in registers.)
+    // (After the last step the next one's scores are of no use, as are steps past
+    // the last key that the wave's rows see: they cost less than a second copy of this, without
+    // them, costs in registers.)
     tile_body(w, s0, s1, tops, c, std::integral_constant<bool, true>{}, knext, vnow);
   };
   for (int i = from; i < to; i += 2) {
@@ -625,7 +635,7 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
   find_row();
   const float c = p.scale == 0.f ? 1.f : fabsf(p.scale) * kLog2e;
   Rows<T, DP, true> w;
-  w.held = lane;
+  w.template hold<DP>(lane);
   {
     const T* q = static_cast<const T*>(p.q) + (static_cast<int64_t>(it.s.q0) + tok) * p.q_tok + (it.head * group + sub) * p.q_head;
 #pragma unroll
@@ -864,7 +874,7 @@ constexpr int kWavesOf = (kRoles & kTiles) != 0 ? kTileWaves : kChunkWaves;
 
 template <typename T, int DP, bool kSmall, int kRoles>
 __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedArgs p) {
-  constexpr int kWaves = kWavesOf<kRoles>, kThreads = 64 * kWaves;
+  constexpr int kWaves = kWavesOf<kRoles>;
   constexpr int kSlotRows = (kRoles & kTiles) != 0 ? kTileRows<true> : kTileRows<false>;
   __shared__ Shared sh;
   __shared__ Listed list[kListed<kSmall>];
