@@ -52,10 +52,10 @@ static_assert(kGranule == kMinPage, "a granule lies in one page");
 // Of a workgroup of kWaves:
 template <bool kTile, int kWaves>
 constexpr int kStep = kTile ? kTileKeys : kChunkKeys * kWaves;  // keys of a step
-template <bool kSmall>
-constexpr int kListed = kSmall ? 128 : 256;  // granules whose places are listed at a time
+template <bool kSmall, int kWaves>
+constexpr int kListed = 64 * kWaves / (kSmall ? 2 : 1);  // granules whose places are listed at a time: 2 KiB a wave
 template <bool kTile, bool kSmall, int kWaves>
-constexpr int kSteps = kListed<kSmall> * kGranule / kStep<kTile, kWaves>;  // steps listed at a time
+constexpr int kSteps = kListed<kSmall, kWaves> * kGranule / kStep<kTile, kWaves>;  // steps listed at a time
 template <bool kTile>
 constexpr int kTileRows = kTile ? kWaveRows * kTileWaves : kWaveRows;
 
@@ -225,12 +225,25 @@ __device__ __forceinline__ void range_of(const PagedArgs& p, Item& it) {
 
 // ---------------------------------------------------------- keys and values --
 
-// A buffer of `size` bytes.  (Its flags are a new number to the compiler each time: it
-// would else keep the whole descriptor from load to load, in lanes of vector registers.)
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* src, int size) {
+// A granule's place as the list holds it: the first three words of a buffer's
+// description, its address and how many bytes of it there are (none: what is loaded is zero).
+__device__ __forceinline__ u32x4 place_of(const void* at, int bytes) {
+  const unsigned long long a = reinterpret_cast<unsigned long long>(at);
+  return u32x4{static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32), static_cast<uint32_t>(bytes), 0u};
+}
+// The buffer at a place that is the same in every lane.  (Its flags are a new number
+// to the compiler each time: it would else keep the whole description from load to load, in
+// lanes of vector registers.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const u32x4& place) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(place[0]), hi = __builtin_amdgcn_readfirstlane(place[1]);
   int flags = 0x00020000;
   asm volatile("" : "+s"(flags));
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(src), 0, size, flags);
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((static_cast<unsigned long long>(hi) << 32) | lo), 0,
+                                           __builtin_amdgcn_readfirstlane(place[2]), flags);
+}
+// Bytes of `rows` rows, a granule's at most, the last one of `row_bytes`.
+__device__ __forceinline__ int bytes_of(int rows, int stride, int row_bytes) {
+  return rows <= 0 ? 0 : (std::min(rows, kGranule) - 1) * stride + row_bytes;
 }
 
 // Loads of one granule of keys or values.  16 bits: load i fills rows i *
@@ -249,12 +262,12 @@ struct Granule {
     uint32_t code[kLoads];
   };
   int off[kLoads];
-  int stride, scale_stride, row_bytes, lane;
+  int scale_stride, lane;
 
   static __device__ __forceinline__ int swizzle(int r) { return kValues ? H::value_swizzle(r) : H::key_swizzle(r); }
 
-  __device__ __forceinline__ Granule(int stride_, int scale_stride_, int dim, int lane_)
-      : stride(stride_), scale_stride(scale_stride_), row_bytes(kSmall ? dim : 2 * dim), lane(lane_) {
+  __device__ __forceinline__ Granule(int stride, int scale_stride_, int dim, int lane_) : scale_stride(scale_stride_), lane(lane_) {
+    const int row_bytes = kSmall ? dim : 2 * dim;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int r = i * kRowsPerLoad + lane / kLanes;
@@ -262,19 +275,15 @@ struct Granule {
       off[i] = c * 16 < row_bytes ? r * stride + c * 16 : kOutside;
     }
   }
-  __device__ __forceinline__ int bytes(int rows) const { return rows <= 0 ? 0 : (std::min(rows, kGranule) - 1) * stride + row_bytes; }
-
-  __device__ __forceinline__ void stage(const char* src, int rows, char* dst) const {
-    const __amdgpu_buffer_rsrc_t b = buffer_of(src, bytes(rows));
+  __device__ __forceinline__ void stage(const u32x4& place, char* dst) const {
+    const __amdgpu_buffer_rsrc_t b = buffer_at(place);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void*)(dst + i * 1024), 16, off[i], 0, 0, 0);
   }
 
-  __device__ __forceinline__ void fetch(const char* src, const uint8_t* scales, int rows, Held& h) const {
-    const __amdgpu_buffer_rsrc_t r = buffer_of(src, bytes(rows));
-    const int scale_size = rows <= 0 ? 0 : (std::min(rows, kGranule) - 1) * scale_stride + 1;
-    const __amdgpu_buffer_rsrc_t s = buffer_of(scales, scale_size);
+  __device__ __forceinline__ void fetch(const u32x4& place, const u32x4& scales, Held& h) const {
+    const __amdgpu_buffer_rsrc_t r = buffer_at(place), s = buffer_at(scales);
     const int row = lane / kLanes;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -313,86 +322,60 @@ struct Granule {
   }
 };
 
-// Where a granule's keys, values and their scales are, from their arrays' starts;
-// none: its keys and values are zero.
+// The places of a granule's keys, values and their scales.
 struct Listed {
-  long long k, v;
-  static constexpr long long kNone = -1;
-};
-struct ListedScales {
-  long long k, v;
+  u32x4 k, v;
 };
 
-// A workgroup's keys and values: addresses of an item's granules by the list.
+// A workgroup's keys and values, by the list.
 template <typename T, int DP, bool kSmall>
 struct Source {
   using K = Granule<T, DP, false, kSmall>;
   using V = Granule<T, DP, true, kSmall>;
-  const char* k;
-  const char* v;
-  const uint8_t* ks;
-  const uint8_t* vs;
-  int end;
   const Listed* list;
-  const ListedScales* scales;
+  const Listed* scales;
   K keys;
   V values;
 
-  __device__ __forceinline__ Source(const PagedArgs& p, const Item& it, const Listed* list_, const ListedScales* scales_, int lane)
-      : k(p.k + it.head * p.k_head), v(p.v + it.head * p.v_head),
-        ks(kSmall ? p.k_scales + it.head * p.ks_head : nullptr), vs(kSmall ? p.v_scales + it.head * p.vs_head : nullptr),
-        end(it.end), list(list_), scales(scales_), keys(p.k_tok, p.ks_tok, p.dim, lane), values(p.v_tok, p.vs_tok, p.dim, lane) {}
+  __device__ __forceinline__ Source(const PagedArgs& p, const Listed* list_, const Listed* scales_, int lane)
+      : list(list_), scales(scales_), keys(p.k_tok, p.ks_tok, p.dim, lane), values(p.v_tok, p.vs_tok, p.dim, lane) {}
 
-  static __device__ __forceinline__ long long first(long long v) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(v));
-    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32));
-    return static_cast<long long>((static_cast<unsigned long long>(hi) << 32) | lo);
+  // Of granule `at` of the list; past its end (there: it is not) nothing is loaded.
+  __device__ __forceinline__ void stage_k(int at, bool there, char* to) const { keys.stage(there ? list[at].k : u32x4{0u, 0u, 0u, 0u}, to); }
+  __device__ __forceinline__ void stage_v(int at, bool there, char* to) const { values.stage(there ? list[at].v : u32x4{0u, 0u, 0u, 0u}, to); }
+  __device__ __forceinline__ void fetch_k(int at, bool there, typename K::Held& h) const {
+    keys.fetch(there ? list[at].k : u32x4{0u, 0u, 0u, 0u}, there ? scales[at].k : u32x4{0u, 0u, 0u, 0u}, h);
   }
-  __device__ __forceinline__ void stage_k(int at, bool there, int key, char* to) const {
-    const long long off = there ? first(list[at].k) : Listed::kNone;
-    keys.stage(k + off, off < 0 ? 0 : end - key, to);
-  }
-  __device__ __forceinline__ void stage_v(int at, bool there, int key, char* to) const {
-    const long long off = there ? first(list[at].v) : Listed::kNone;
-    values.stage(v + off, off < 0 ? 0 : end - key, to);
-  }
-  __device__ __forceinline__ void fetch_k(int at, bool there, int key, typename K::Held& h) const {
-    const long long off = there ? first(list[at].k) : Listed::kNone, scale = there ? first(scales[at].k) : 0;
-    keys.fetch(k + off, ks + scale, off < 0 ? 0 : end - key, h);
-  }
-  __device__ __forceinline__ void fetch_v(int at, bool there, int key, typename V::Held& h) const {
-    const long long off = there ? first(list[at].v) : Listed::kNone, scale = there ? first(scales[at].v) : 0;
-    values.fetch(v + off, vs + scale, off < 0 ? 0 : end - key, h);
+  __device__ __forceinline__ void fetch_v(int at, bool there, typename V::Held& h) const {
+    values.fetch(there ? list[at].v : u32x4{0u, 0u, 0u, 0u}, there ? scales[at].v : u32x4{0u, 0u, 0u, 0u}, h);
   }
 };
 
-// Lists where the item's steps [from, to) are, a granule each.  None: a page outside
-// the cache (flagged), or no key.
+// Lists the places of the item's steps [from, to), a granule each.  Nothing is
+// there past the last key, and of a page outside the cache (which is flagged).
 template <bool kTile, bool kSmall, int kWaves>
-__device__ __forceinline__ void list_pages(const PagedArgs& p, const Item& it, int from, int to, int tid, Listed* list, ListedScales* scales) {
+__device__ __forceinline__ void list_pages(const PagedArgs& p, const Item& it, int from, int to, int tid, Listed* list, Listed* scales) {
   constexpr int kKeys = kStep<kTile, kWaves>, kEach = kKeys / kGranule;
-  const int n = (to - from) * kEach;
+  const int n = (to - from) * kEach, row_bytes = kSmall ? p.dim : 2 * p.dim;
   const int32_t* row = p.table + static_cast<int64_t>(it.seq) * p.table_row;
   for (int g = tid; g < n; g += 64 * kWaves) {
     const int key = it.key_of<kKeys>(from + g / kEach) + g % kEach * kGranule;
-    Listed l{Listed::kNone, Listed::kNone};
-    ListedScales z{0, 0};
-    if (key < it.end) {
-      const int page = row[key >> p.page_shift];
-      if (page < 0 || page >= p.n_pages) {
+    int rows = it.end - key;
+    int64_t i = 0;
+    if (rows > 0) {
+      i = row[key >> p.page_shift];
+      if (i < 0 || i >= p.n_pages) {
         flag_error(p.header, kErrIdRange);
-      } else {
-        const int64_t i = page, j = key & ((1 << p.page_shift) - 1);
-        l.k = i * p.k_page + j * p.k_tok;
-        l.v = i * p.v_page + j * p.v_tok;
-        if (kSmall) {
-          z.k = i * p.ks_page + j * p.ks_tok;
-          z.v = i * p.vs_page + j * p.vs_tok;
-        }
+        rows = 0;
+        i = 0;
       }
     }
-    list[g] = l;
-    if (kSmall) scales[g] = z;
+    const int64_t j = key & ((1 << p.page_shift) - 1);
+    list[g] = Listed{place_of(p.k + it.head * p.k_head + i * p.k_page + j * p.k_tok, bytes_of(rows, p.k_tok, row_bytes)),
+                     place_of(p.v + it.head * p.v_head + i * p.v_page + j * p.v_tok, bytes_of(rows, p.v_tok, row_bytes))};
+    if (kSmall)
+      scales[g] = Listed{place_of(p.k_scales + it.head * p.ks_head + i * p.ks_page + j * p.ks_tok, bytes_of(rows, p.ks_tok, 1)),
+                         place_of(p.v_scales + it.head * p.vs_head + i * p.vs_page + j * p.vs_tok, bytes_of(rows, p.vs_tok, 1))};
   }
 }
 
@@ -440,11 +423,11 @@ __device__ __forceinline__ void run_chunk(const Source<T, DP, kSmall>& in, const
     typename Src::V::Held hv[2];
     auto fetch_k = [&](int i) {
 #pragma unroll
-      for (int g = 0; g < 2; ++g) in.fetch_k(place(i) + g, i < to, key_of(i) + g * kGranule, hk[g]);
+      for (int g = 0; g < 2; ++g) in.fetch_k(place(i) + g, i < to, hk[g]);
     };
     auto fetch_v = [&](int i) {
 #pragma unroll
-      for (int g = 0; g < 2; ++g) in.fetch_v(place(i) + g, i < to, key_of(i) + g * kGranule, hv[g]);
+      for (int g = 0; g < 2; ++g) in.fetch_v(place(i) + g, i < to, hv[g]);
     };
     fetch_k(from);
     fetch_v(from);
@@ -468,11 +451,11 @@ __device__ __forceinline__ void run_chunk(const Source<T, DP, kSmall>& in, const
     constexpr int kLoads = 2 * Src::K::kLoads;
     auto load_k = [&](int i) {
 #pragma unroll
-      for (int g = 0; g < 2; ++g) in.stage_k(place(i) + g, i < to, key_of(i) + g * kGranule, sk + g * kGranule * kRow);
+      for (int g = 0; g < 2; ++g) in.stage_k(place(i) + g, i < to, sk + g * kGranule * kRow);
     };
     auto load_v = [&](int i) {
 #pragma unroll
-      for (int g = 0; g < 2; ++g) in.stage_v(place(i) + g, i < to, key_of(i) + g * kGranule, sv + g * kGranule * kRow);
+      for (int g = 0; g < 2; ++g) in.stage_v(place(i) + g, i < to, sv + g * kGranule * kRow);
     };
     load_k(from);
     load_v(from);
@@ -507,15 +490,15 @@ __device__ __forceinline__ void run_tile(const Source<T, DP, kSmall>& in, const 
   auto place = [&](int i) { return (i - from) * kEach + wave; };
   typename Src::K::Held hk;
   typename Src::V::Held hv;
-  auto fetch_k = [&](int i) { in.fetch_k(place(i), i < to, key_of(i) + wave * kGranule, hk); };
-  auto fetch_v = [&](int i) { in.fetch_v(place(i), i < to, key_of(i) + wave * kGranule, hv); };
+  auto fetch_k = [&](int i) { in.fetch_k(place(i), i < to, hk); };
+  auto fetch_v = [&](int i) { in.fetch_v(place(i), i < to, hv); };
   // Steps are asked for in their order.
   auto load_k = [&](int i, char* buf) {
     if constexpr (kSmall) {
       in.keys.put(hk, buf + mine);
       fetch_k(i + 1);
     } else if (i < to) {
-      in.stage_k(place(i), true, key_of(i) + wave * kGranule, buf + mine);
+      in.stage_k(place(i), true, buf + mine);
     }
   };
   auto load_v = [&](int i, char* buf) {
@@ -523,7 +506,7 @@ __device__ __forceinline__ void run_tile(const Source<T, DP, kSmall>& in, const 
       in.values.put(hv, buf + mine);
       fetch_v(i + 1);
     } else if (i < to) {
-      in.stage_v(place(i), true, key_of(i) + wave * kGranule, buf + mine);
+      in.stage_v(place(i), true, buf + mine);
     }
   };
   auto meet = [&] {
@@ -573,18 +556,18 @@ __device__ __forceinline__ void run_tile_careful(const Source<T, DP, kSmall>& in
   constexpr int kKeys = kStep<true, kTileWaves>, kEach = kKeys / kGranule;
   const int mine = wave * kGranule * Head<DP>::kRow;
   for (int i = from; i < to; ++i) {
-    const int at = it.key_of<kKeys>(i), key = at + wave * kGranule, place = (i - from) * kEach + wave;
+    const int at = it.key_of<kKeys>(i), place = (i - from) * kEach + wave;
     __syncthreads();
     if constexpr (kSmall) {
       typename Src::K::Held hk;
       typename Src::V::Held hv;
-      in.fetch_k(place, true, key, hk);
-      in.fetch_v(place, true, key, hv);
+      in.fetch_k(place, true, hk);
+      in.fetch_v(place, true, hv);
       in.keys.put(hk, sk + mine);
       in.values.put(hv, sv + mine);
     } else {
-      in.stage_k(place, true, key, sk + mine);
-      in.stage_v(place, true, key, sv + mine);
+      in.stage_k(place, true, sk + mine);
+      in.stage_v(place, true, sv + mine);
       wait_vm();
     }
     __syncthreads();
@@ -616,7 +599,7 @@ __device__ __forceinline__ void finish_row(const PagedArgs& p, const Item& it, i
 
 // The workgroup's steps of one item.
 template <typename T, int DP, bool kSmall, int kWaves, bool kTile, int kSlotRows>
-__device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed* list, ListedScales* scales, WP_STAGED) {
+__device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed* list, Listed* scales, WP_STAGED) {
   using H = Head<DP>;
   constexpr int kBatch = kSteps<kTile, kSmall, kWaves>, kThreads = 64 * kWaves;
   int tid = thread_number(), lane = tid & 63, half = lane >> 5;
@@ -657,7 +640,7 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
     see.last = t1 + lag;
     see.low = window_start(t1 + lag, p.window);
   }
-  const Source<T, DP, kSmall> in(p, it, list, scales, lane);
+  const Source<T, DP, kSmall> in(p, list, scales, lane);
   // Key chunks: a wave's keys and values, and later its share of O.
   constexpr int kHalf = Staged<DP>::kBytes / 2;
   char* my_k = (kWaves == 2 || wave < 2 ? sk0 : sk1) + (wave & 1) * kHalf;
@@ -877,8 +860,8 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
   constexpr int kWaves = kWavesOf<kRoles>;
   constexpr int kSlotRows = (kRoles & kTiles) != 0 ? kTileRows<true> : kTileRows<false>;
   __shared__ Shared sh;
-  __shared__ Listed list[kListed<kSmall>];
-  __shared__ ListedScales scales[kSmall ? kListed<kSmall> : 1];
+  __shared__ Listed list[kListed<kSmall, kWaves>];
+  __shared__ Listed scales[kSmall ? kListed<kSmall, kWaves> : 1];
   __shared__ __align__(1024) char sk0[Staged<DP>::kBytes];
   __shared__ __align__(1024) char sv0[Staged<DP>::kBytes];
   touch_kernel_args<static_cast<int>(sizeof(PagedArgs))>();
