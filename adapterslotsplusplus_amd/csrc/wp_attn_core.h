@@ -132,12 +132,18 @@ __device__ __forceinline__ typename VecOf<T>::v8 value_fragment(const char* valu
   return value_at<T, DP, kCareful>(values, (key0 + r) * H::kRow + ((c ^ H::value_swizzle(r)) << 4) + (i & 1) * 8);
 }
 
-// The lane that a wave's work goes by, and its fragments: the thread's own
-// number or (kHeld) one that a kernel keeps, in a form that the compiler takes for a number of
-// that moment alone.  Then one address of either kind is kept, too: a step or a column on
-// changes bits of it that no row touches.
-template <bool kHeld>
-struct Lane {
+// The lane that a wave's work goes by, and its fragments: the thread's own number
+// (kOwn) or one that a kernel keeps (kHeld), in a form that the compiler takes for
+// a number of that moment alone.  Then one address of either kind is kept, too: a
+// step or a column on changes bits of it that no row touches.  kRenewed: those changes are
+// made anew for each tile and not kept in registers from tile to tile.
+enum LaneKind { kOwn, kHeld, kRenewed };
+template <LaneKind kKind>
+struct KeptLane;
+template <LaneKind kKind>
+struct Lane : KeptLane<kKind> {};
+template <>
+struct Lane<kOwn> {
   __device__ __forceinline__ int lane() const { return static_cast<int>(threadIdx.x) & 63; }
   __device__ __forceinline__ void renew() {}
   template <typename T, int DP>
@@ -149,8 +155,8 @@ struct Lane {
     return value_fragment<T, DP, kCareful>(values, key0, col, lane());
   }
 };
-template <>
-struct Lane<true> {
+template <LaneKind kKind>
+struct KeptLane {
   int held, key_place, value_place;
   __device__ __forceinline__ int lane() const { return held; }
   template <int DP>
@@ -161,7 +167,9 @@ struct Lane<true> {
     key_place = k * H::kRow + (((lane >> 5) ^ H::key_swizzle(k)) << 4);
     value_place = v * H::kRow + ((((g & 1) * 2 + ((i & 3) >> 1)) ^ H::value_swizzle(v)) << 4) + (i & 1) * 8;
   }
-  __device__ __forceinline__ void renew() { asm volatile("" : "+v"(key_place), "+v"(value_place)); }
+  __device__ __forceinline__ void renew() {
+    if (kKind == kRenewed) asm volatile("" : "+v"(key_place), "+v"(value_place));
+  }
   template <typename T, int DP>
   __device__ __forceinline__ typename VecOf<T>::v8 key(const char* keys, int row0, int step) const {
     return *reinterpret_cast<const typename VecOf<T>::v8*>(keys + (key_place ^ (step << 5)) + row0 * Head<DP>::kRow);
@@ -173,8 +181,8 @@ struct Lane<true> {
 };
 
 // A wave's 32 query rows and their running state.
-template <typename T, int DP, bool kHeld = false>
-struct Rows : Lane<kHeld> {
+template <typename T, int DP, LaneKind kKind = kOwn>
+struct Rows : Lane<kKind> {
   using H = Head<DP>;
   using V8 = typename VecOf<T>::v8;
   V8 q[H::kSteps];
@@ -228,8 +236,8 @@ __device__ __forceinline__ float top_of(const f32x16& s) {
 
 // Adds the infinite and NaN values of n staged keys that a query sees (sees(r):
 // the lane's of key r), which value_fragment<careful> left out.
-template <typename T, int DP, bool kHeld, typename Sees>
-__device__ __forceinline__ void add_nonfinite(Rows<T, DP, kHeld>& w, const char* values, int n, Sees sees_key) {
+template <typename T, int DP, LaneKind kKind, typename Sees>
+__device__ __forceinline__ void add_nonfinite(Rows<T, DP, kKind>& w, const char* values, int n, Sees sees_key) {
   using H = Head<DP>;
   const int lane = w.lane(), half = lane >> 5;
   for (int r = 0; r < n; ++r) {
@@ -263,8 +271,8 @@ __device__ __forceinline__ const T* head_row(const void* base, int64_t tok, int6
 // operands: each weight is rounded to the tensors' type, once, so that O is off
 // by at most half a unit of that type of sum p |v| -- what rounding the values
 // themselves did.
-template <typename T, int DP, bool kHeld>
-__device__ __forceinline__ void weigh(Rows<T, DP, kHeld>& w, const f32x16& s, float c, typename VecOf<T>::v8 (&out)[2]) {
+template <typename T, int DP, LaneKind kKind>
+__device__ __forceinline__ void weigh(Rows<T, DP, kKind>& w, const f32x16& s, float c, typename VecOf<T>::v8 (&out)[2]) {
   const float base = w.m == -INFINITY ? 0.f : w.m;
 #pragma unroll
   for (int b = 0; b < 2; ++b)
@@ -277,8 +285,8 @@ __device__ __forceinline__ void weigh(Rows<T, DP, kHeld>& w, const f32x16& s, fl
 }
 
 // Scores of 32 staged keys from row0 on; LDS reads go four products ahead.
-template <typename T, int DP, bool kHeld>
-__device__ __forceinline__ f32x16 scores(const Rows<T, DP, kHeld>& w, const char* keys, int row0) {
+template <typename T, int DP, LaneKind kKind>
+__device__ __forceinline__ f32x16 scores(const Rows<T, DP, kKind>& w, const char* keys, int row0) {
   constexpr int kSteps = Head<DP>::kSteps;
   typename VecOf<T>::v8 kf[4];
 #pragma unroll
@@ -295,8 +303,8 @@ __device__ __forceinline__ f32x16 scores(const Rows<T, DP, kHeld>& w, const char
 }
 
 // Adds 32 staged keys' weighted values to O.
-template <typename T, int DP, bool kCareful, bool kHeld>
-__device__ __forceinline__ void accumulate(Rows<T, DP, kHeld>& w, const char* values, int row0,
+template <typename T, int DP, bool kCareful, LaneKind kKind>
+__device__ __forceinline__ void accumulate(Rows<T, DP, kKind>& w, const char* values, int row0,
                                            const typename VecOf<T>::v8 (&e)[2]) {
   constexpr int kCols = Head<DP>::kCols, kAhead = kCols < 4 ? kCols : 4;
   auto value = [&](int i) { return w.template value<T, DP, kCareful>(values, row0 + i / kCols * 16, i % kCols); };
@@ -322,8 +330,8 @@ __device__ __forceinline__ void accumulate(Rows<T, DP, kHeld>& w, const char* va
 //
 // Weighs and adds the 64 staged keys whose masked scores are s0 and s1 (tops: the
 // lane's largest of them) and, with `more`, computes the next tile's into their place.
-template <typename T, int DP, bool kHeld, typename More>
-__device__ __forceinline__ void tile_body(Rows<T, DP, kHeld>& w, f32x16& s0, f32x16& s1, float& tops, float c, More more,
+template <typename T, int DP, LaneKind kKind, typename More>
+__device__ __forceinline__ void tile_body(Rows<T, DP, kKind>& w, f32x16& s0, f32x16& s1, float& tops, float c, More more,
                                           const char* knext, const char* vnow) {
   using H = Head<DP>;
   using V8 = typename VecOf<T>::v8;
@@ -406,8 +414,8 @@ struct Staged {
 #define WP_STAGED char (&sk0)[Staged<DP>::kBytes], char (&sk1)[Staged<DP>::kBytes], char (&sv0)[Staged<DP>::kBytes], \
                   char (&sv1)[Staged<DP>::kBytes]
 
-template <typename T, int DP, bool kHeld>
-__device__ __forceinline__ bool has_nonfinite(const Rows<T, DP, kHeld>& w) {
+template <typename T, int DP, LaneKind kKind>
+__device__ __forceinline__ bool has_nonfinite(const Rows<T, DP, kKind>& w) {
   float z = 0.f;
 #pragma unroll
   for (int i = 0; i < Head<DP>::kCols; ++i)

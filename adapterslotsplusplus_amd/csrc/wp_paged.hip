@@ -42,6 +42,9 @@ constexpr int kTileWaves = 4;             // waves of a workgroup with row tiles
 constexpr int kChunkWaves = 2;            // and of one with key chunks alone
 constexpr int kMostWaves = 4;
 constexpr int kTiles = 1, kChunks = 2;  // the roles of a launch
+// (Rows that pass through registers leave none for a tile's addresses.)
+template <bool kSmall>
+constexpr LaneKind kLane = kSmall ? kRenewed : kHeld;
 constexpr int kGranule = 16;            // keys of one load address
 constexpr int kMostWorkgroups = 1024;
 constexpr int kChunkKeys = 32;          // keys of a wave's step on key chunks
@@ -351,37 +354,42 @@ struct Source {
   }
 };
 
-// Lists the places of the item's steps [from, to), a granule each.  Nothing is
-// there past the last key, and of a page outside the cache (which is flagged).
+// The page of the granule at `key` (0 past the item's last key).
+__device__ __forceinline__ int page_of(const PagedArgs& p, const Item& it, int key) {
+  return key < it.end ? p.table[static_cast<int64_t>(it.seq) * p.table_row + (key >> p.page_shift)] : 0;
+}
+// Lists the granule at `key`, in `page`.  Nothing is there past the last key, and
+// of a page outside the cache (which is flagged).
+template <bool kSmall>
+__device__ __forceinline__ void list_granule(const PagedArgs& p, const Item& it, int key, int page, Listed& list, Listed& scales) {
+  const int row_bytes = kSmall ? p.dim : 2 * p.dim;
+  int rows = it.end - key;
+  if (page < 0 || page >= p.n_pages) {
+    if (rows > 0) flag_error(p.header, kErrIdRange);
+    rows = 0;
+    page = 0;
+  }
+  const int64_t i = page, j = key & ((1 << p.page_shift) - 1);
+  list = Listed{place_of(p.k + it.head * p.k_head + i * p.k_page + j * p.k_tok, bytes_of(rows, p.k_tok, row_bytes)),
+                place_of(p.v + it.head * p.v_head + i * p.v_page + j * p.v_tok, bytes_of(rows, p.v_tok, row_bytes))};
+  if (kSmall)
+    scales = Listed{place_of(p.k_scales + it.head * p.ks_head + i * p.ks_page + j * p.ks_tok, bytes_of(rows, p.ks_tok, 1)),
+                    place_of(p.v_scales + it.head * p.vs_head + i * p.vs_page + j * p.vs_tok, bytes_of(rows, p.vs_tok, 1))};
+}
+// Lists the item's steps [from, to).
 template <bool kTile, bool kSmall, int kWaves>
 __device__ __forceinline__ void list_pages(const PagedArgs& p, const Item& it, int from, int to, int tid, Listed* list, Listed* scales) {
   constexpr int kKeys = kStep<kTile, kWaves>, kEach = kKeys / kGranule;
-  const int n = (to - from) * kEach, row_bytes = kSmall ? p.dim : 2 * p.dim;
-  const int32_t* row = p.table + static_cast<int64_t>(it.seq) * p.table_row;
+  const int n = (to - from) * kEach;
   for (int g = tid; g < n; g += 64 * kWaves) {
     const int key = it.key_of<kKeys>(from + g / kEach) + g % kEach * kGranule;
-    int rows = it.end - key;
-    int64_t i = 0;
-    if (rows > 0) {
-      i = row[key >> p.page_shift];
-      if (i < 0 || i >= p.n_pages) {
-        flag_error(p.header, kErrIdRange);
-        rows = 0;
-        i = 0;
-      }
-    }
-    const int64_t j = key & ((1 << p.page_shift) - 1);
-    list[g] = Listed{place_of(p.k + it.head * p.k_head + i * p.k_page + j * p.k_tok, bytes_of(rows, p.k_tok, row_bytes)),
-                     place_of(p.v + it.head * p.v_head + i * p.v_page + j * p.v_tok, bytes_of(rows, p.v_tok, row_bytes))};
-    if (kSmall)
-      scales[g] = Listed{place_of(p.k_scales + it.head * p.ks_head + i * p.ks_page + j * p.ks_tok, bytes_of(rows, p.ks_tok, 1)),
-                         place_of(p.v_scales + it.head * p.vs_head + i * p.vs_page + j * p.vs_tok, bytes_of(rows, p.vs_tok, 1))};
+    list_granule<kSmall>(p, it, key, page_of(p, it, key), list[g], scales[kSmall ? g : 0]);
   }
 }
 
 // Scores of keys [at, at + 32) that the lane's query does not see become -inf.
-template <typename T, int DP>
-__device__ __forceinline__ void mask_seen(const Rows<T, DP, true>& w, f32x16& s, int at, int sinks) {
+template <typename T, int DP, LaneKind kKind>
+__device__ __forceinline__ void mask_seen(const Rows<T, DP, kKind>& w, f32x16& s, int at, int sinks) {
   const int first = at + (w.lane() >> 5) * 4;
   const int up = w.pos - first, down = w.low - first, kept = sinks - first;
 #pragma unroll
@@ -402,7 +410,7 @@ struct Sight {
 // Key chunks: this wave's 32 keys of each of the item's steps [from, to), whose
 // pages are listed.
 template <typename T, int DP, bool kSmall, int kWaves, bool kCareful>
-__device__ __forceinline__ void run_chunk(const Source<T, DP, kSmall>& in, const Item& it, Rows<T, DP, true>& w, float c,
+__device__ __forceinline__ void run_chunk(const Source<T, DP, kSmall>& in, const Item& it, Rows<T, DP, kLane<kSmall>>& w, float c,
                                           const Sight& see, int from, int to, int wave, char* sk, char* sv) {
   using Src = Source<T, DP, kSmall>;
   constexpr int kRow = Head<DP>::kRow, kKeys = kStep<false, kWaves>, kEach = kKeys / kGranule;
@@ -481,24 +489,46 @@ __device__ __forceinline__ void run_chunk(const Source<T, DP, kSmall>& in, const
 // are computed, and steps i + 2 of K and i + 1 of V are on their way; each wave
 // brings in a granule of either.
 template <typename T, int DP, bool kSmall>
-__device__ __forceinline__ void run_tile(const Source<T, DP, kSmall>& in, const Item& it, Rows<T, DP, true>& w, float c,
-                                         const Sight& see, int from, int to, int wave, WP_STAGED) {
+__device__ __forceinline__ void run_tile(const PagedArgs& p, const Source<T, DP, kSmall>& in, const Item& it, Rows<T, DP, kLane<kSmall>>& w,
+                                         float c, const Sight& see, int wave, Listed* list, Listed* scales, WP_STAGED) {
   using Src = Source<T, DP, kSmall>;
   constexpr int kKeys = kStep<true, kTileWaves>, kEach = kKeys / kGranule;
+  constexpr int kRing = kListed<kSmall, kTileWaves>, kHalf = kSteps<true, kSmall, kTileWaves> / 2;
+  static_assert((kRing & (kRing - 1)) == 0 && kHalf >= 8 && kHalf * kEach <= 64 * kTileWaves, "half of the list is written in one go, well ahead");
+  const int from = it.from, to = it.to;
   const int mine = wave * kGranule * Head<DP>::kRow;
   auto key_of = [&](int i) { return it.key_of<kKeys>(i); };
-  auto place = [&](int i) { return (i - from) * kEach + wave; };
+  auto place = [&](int i) { return ((i - from) * kEach & (kRing - 1)) + wave; };
+  // The list is a ring: where a half of it has been worked through, the steps after the other
+  // half are listed in its place, their pages read in one step and listed in the next.
+  int page = 0;
+  auto refill = [&](int i) {
+    const int done = (i - from) & (kHalf - 1);
+    if (i - from < kHalf || done > 1) return;
+    const int tid = thread_number(), first = i - done + kHalf;  // the first step to list
+    if (first >= to || tid >= kHalf * kEach) return;
+    const int key = it.key_of<kKeys>(first + tid / kEach) + tid % kEach * kGranule;
+    if (done == 0) {
+      page = page_of(p, it, key);
+    } else {
+      const int at = ((first - from) * kEach & (kRing - 1)) + tid;
+      list_granule<kSmall>(p, it, key, page, list[at], scales[kSmall ? at : 0]);
+    }
+  };
   typename Src::K::Held hk;
   typename Src::V::Held hv;
   auto fetch_k = [&](int i) { in.fetch_k(place(i), i < to, hk); };
   auto fetch_v = [&](int i) { in.fetch_v(place(i), i < to, hv); };
   // Steps are asked for in their order.
+  // (16 bits: a granule's place is read a step before it is used.)
+  u32x4 at_k = in.list[place(from)].k, at_v = in.list[place(from)].v;
   auto load_k = [&](int i, char* buf) {
     if constexpr (kSmall) {
       in.keys.put(hk, buf + mine);
       fetch_k(i + 1);
     } else if (i < to) {
-      in.stage_k(place(i), true, buf + mine);
+      in.keys.stage(at_k, buf + mine);
+      at_k = in.list[place(std::min(i + 1, to - 1))].k;
     }
   };
   auto load_v = [&](int i, char* buf) {
@@ -506,7 +536,8 @@ __device__ __forceinline__ void run_tile(const Source<T, DP, kSmall>& in, const 
       in.values.put(hv, buf + mine);
       fetch_v(i + 1);
     } else if (i < to) {
-      in.stage_v(place(i), true, buf + mine);
+      in.values.stage(at_v, buf + mine);
+      at_v = in.list[place(std::min(i + 1, to - 1))].v;
     }
   };
   auto meet = [&] {
@@ -523,6 +554,7 @@ __device__ __forceinline__ void run_tile(const Source<T, DP, kSmall>& in, const 
   load_v(from, sv0);
   auto next = [&](int i, char* kfree, char* vnext) {
     meet();
+    refill(i);
     load_k(i + 2, kfree);
     load_v(i + 1, vnext);
   };
@@ -550,7 +582,7 @@ __device__ __forceinline__ void run_tile(const Source<T, DP, kSmall>& in, const 
 // run_tile, one step after the other, with infinite and NaN values left out of
 // the product and added to the rows that see them: the same sums otherwise.
 template <typename T, int DP, bool kSmall>
-__device__ __forceinline__ void run_tile_careful(const Source<T, DP, kSmall>& in, const Item& it, Rows<T, DP, true>& w, float c,
+__device__ __forceinline__ void run_tile_careful(const Source<T, DP, kSmall>& in, const Item& it, Rows<T, DP, kLane<kSmall>>& w, float c,
                                                  const Sight& see, int from, int to, int wave, char* sk, char* sv) {
   using Src = Source<T, DP, kSmall>;
   constexpr int kKeys = kStep<true, kTileWaves>, kEach = kKeys / kGranule;
@@ -617,7 +649,7 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
   };
   find_row();
   const float c = p.scale == 0.f ? 1.f : fabsf(p.scale) * kLog2e;
-  Rows<T, DP, true> w;
+  Rows<T, DP, kLane<kSmall>> w;
   w.template hold<DP>(lane);
   {
     const T* q = static_cast<const T*>(p.q) + (static_cast<int64_t>(it.s.q0) + tok) * p.q_tok + (it.head * group + sub) * p.q_head;
@@ -657,13 +689,16 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
       }
       if constexpr (!kTile)
         run_chunk<T, DP, kSmall, kWaves, decltype(careful)::value>(in, it, w, c, see, i, to, wave, my_k, my_v);
-      else if constexpr (decltype(careful)::value)
-        run_tile_careful(in, it, w, c, see, i, to, wave, sk0, sv0);
       else
-        run_tile(in, it, w, c, see, i, to, wave, sk0, sk1, sv0, sv1);
+        run_tile_careful(in, it, w, c, see, i, to, wave, sk0, sv0);
     }
   };
-  pass(std::integral_constant<bool, false>{});
+  if constexpr (kTile) {
+    w.reset();
+    run_tile(p, in, it, w, c, see, wave, list, scales, sk0, sk1, sv0, sv1);
+  } else {
+    pass(std::integral_constant<bool, false>{});
+  }
   // Infinite or NaN values reach every row of a tile through the product, as
   // zero times them: where there are any, the pass is made again with care.
   if (__syncthreads_or(has_nonfinite(w))) pass(std::integral_constant<bool, true>{});

@@ -190,6 +190,43 @@ def test_workgroups_of_several_requests(engine):
     attend(engine, [b % 4 for b in range(150)], lens_k, 8, 4, 64, HF, page=32)
 
 
+def device_want(c, window=0, sinks=0):
+    """The definition in 64 bits on the device, for one request."""
+    (n_q,), (n_k,) = c.lens_q, c.lens_k
+    T, heads, dim = c.q.shape
+    rows = c.rows.cuda()
+    k, v = (t.reshape(-1, *t.shape[2:]).cuda()[rows] for t in c.values)
+    group = heads // k.size(1)
+    j, pos = torch.arange(n_k, device="cuda"), torch.arange(n_q, device="cuda")[:, None] + n_k - n_q
+    hide = j > pos
+    if window:
+        hide |= (j <= pos - window) & (j >= sinks)
+    out, spread = torch.zeros(T, heads, dim, dtype=torch.float64), torch.zeros(T, heads, dim, dtype=torch.float64)
+    lse, reach = torch.zeros(T, heads, dtype=torch.float64), torch.zeros(T, heads, dtype=torch.float64)
+    for h in range(heads):
+        q, kk, vv = c.q[:, h].double().cuda(), k[:, h // group].double(), v[:, h // group].double()
+        s = (q @ kk.t().contiguous() * dim ** -0.5).masked_fill(hide, -math.inf)
+        p = torch.softmax(s, -1)
+        out[:, h], spread[:, h], lse[:, h] = (p @ vv).cpu(), (p @ vv.abs()).cpu(), torch.logsumexp(s, -1).cpu()
+        reach[:, h] = (q.abs() @ kk.abs().t().contiguous() * dim ** -0.5).masked_fill(hide, 0.0).amax(-1).cpu()
+    return out, lse, spread, reach
+
+
+@pytest.mark.parametrize("small", [False, True], ids=["same", "8bit"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (5000, 300)])
+def test_workgroups_that_walk_long_caches(engine, window, sinks, small):
+    """As many row tiles as workgroups, each of more keys than are listed at a
+    time; and single tokens, each of more than a wave's list."""
+    for tokens, heads, kv_heads, dim, keys, dtype in ((700, 128, 64, 64, 9000, HF), (1500, 64, 16, 128, 11000, BF), (1, 1024, 1024, 16, 4500, BF)):
+        announce(f"paged long walks {tokens} tokens {heads}/{kv_heads}x{dim} over {keys} {dtype} small={small} window={window}+{sinks}")
+        c = Case([tokens], [keys], heads, kv_heads, dim, dtype, page=32, small=small)
+        got, lse = c.run(engine, window=window, sinks=sinks)
+        want = device_want(c, window, sinks)
+        tol, lse_tol = c.tolerance(*want)
+        check(got, want[0], tol, "out")
+        check(lse, want[1], lse_tol, "lse")
+
+
 def test_scales(engine):
     for scale in (0.0, 1.0, 4.0, -0.3):
         attend(engine, [100], [300], 2, 2, 64, BF, scale=scale)
