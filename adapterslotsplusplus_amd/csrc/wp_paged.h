@@ -85,7 +85,8 @@ struct PagedArgs {
   Divisor by_group;
   int32_t chunk_rows;  // most rows per key head of a sequence that runs on key chunks
   int32_t n_wg;
-  Divisor by_wg;
+  Divisor by_wg, by_heads;
+  int32_t whole_tiles;  // a workgroup for each row tile, if they may run whole
   int32_t cost_shift;
 };
 hipError_t launch_paged_attention(int dtype_bf16, PagedArgs& a, int n_cu, hipStream_t stream);

@@ -137,6 +137,38 @@ __device__ __forceinline__ int longest_of(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
+// Row tiles that run whole, of up to 64 sequences (a lane each): the `want`-th of
+// those of a key head, the tiles with the most keys first, so that none of the long
+// ones starts last.  The tiles of a sequence that see at least w keys are its last
+// ones; a search over w finds the tile's, and its place among those that see exactly
+// as many.  seq: -1 past the last one.
+__device__ __forceinline__ void tile_by_weight(const PagedArgs& p, const Shape& mine, int want, int& seq, int& tile) {
+  const Cost c = cost_of(p, mine);
+  const int tiles = c.tiles, lag = mine.n_k - mine.n_q;
+  // Tiles whose last row sees at least 64 u keys.
+  auto at_least = [&](int u) {
+    const int w = u * 64;
+    if (w > mine.n_k) return 0;
+    const int64_t row = static_cast<int64_t>(w - lag - 1) * p.group;  // the first that sees w keys
+    const int64_t below = row <= 0 ? 0 : row >> c.log_rows;         // tiles before that row's
+    return below >= tiles ? 0 : static_cast<int>(tiles - below);
+  };
+  seq = -1;
+  if (want >= total_of(tiles)) return;
+  int lo = -1, hi = longest_of(mine.n_k) / 64 + 1;  // more than `want` tiles see 64 lo keys, not 64 hi
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    if (total_of(at_least(mid)) > want) lo = mid; else hi = mid;
+  }
+  const int above = at_least(lo + 1), here = (lo < 0 ? tiles : at_least(lo)) - above;
+  const int rest = want - total_of(above);
+  const int upto = sum_up(here);
+  seq = __builtin_ctzll(__ballot(upto > rest));
+  const int from = __builtin_amdgcn_readlane(above, seq) + rest -
+                   (__builtin_amdgcn_readlane(upto, seq) - __builtin_amdgcn_readlane(here, seq));  // from the sequence's last tile
+  tile = __builtin_amdgcn_readlane(tiles, seq) - 1 - from;
+}
+
 // The tile at place y from the sequence's start: 64 places a round.
 __device__ __forceinline__ int tile_at(const Cost& c, int y) {
   const int lane = static_cast<int>(threadIdx.x) & 63;
@@ -904,12 +936,15 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
 
   // Every wave by itself: a lane for each sequence, 64 at a time, and the sum of
   // their costs.
+  int most_cost = 0;  // of a tile
   auto cost_at = [&](int b, Shape& s) {
     s = Shape{0, 0, 0};
     if (b >= p.n_seq) return 0;
     s = shape_of(p, b);
     const Cost c = cost_of(p, s);
-    return c.before(c.tiles) * p.kv_heads;
+    const int all = c.before(c.tiles);
+    if ((kRoles & kTiles) != 0 && c.tiles > 0) most_cost = std::max(most_cost, all - c.before(c.tiles - 1));
+    return all * p.kv_heads;
   };
   Shape first, other;
   int mine = cost_at(lane, first);
@@ -927,7 +962,12 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
   // past its 31 bits: such a call does nothing.
   if (__builtin_amdgcn_readlane(__builtin_bit_cast(int, length), 63) > __builtin_bit_cast(int, kLongestLine)) return;
   int share = over(total, p.by_wg) + 1, pieces = 0;
-  if (p.n_seq <= 64) {
+  // Many row tiles run whole, one a workgroup, in the order that the device takes
+  // workgroups (the host offers that, see there), if none costs more than a share of the whole: those
+  // of a key head walk its keys together, on one die.
+  const bool whole_tiles = (kRoles & kTiles) != 0 && static_cast<int>(gridDim.x) > p.n_wg && longest_of(most_cost) <= share;
+  if (!whole_tiles && static_cast<int>(blockIdx.x) >= p.n_wg) return;
+  if (p.n_seq <= 64 && !whole_tiles) {
     // A line of pieces, one for each workgroup, where that is as short: a tile's
     // keys in equal pieces, and no workgroup with an end of one item and a start of another.
     const Cost c = cost_of(p, first);
@@ -944,7 +984,7 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
       while (whole(tiles * pieces_of(size)) > p.n_wg) size *= 1.125f;
       pieces = pieces_of(size);
       const int longest = longest_of(c.tiles > 0 ? std::max(step, (keys + pieces - 1) / pieces) : 0);
-      const long long slack = (kRoles & kTiles) != 0 ? 768 : 256;
+      const long long slack = (kRoles & kTiles) != 0 ? 1536 : 256;
       if (static_cast<long long>(longest) * p.group > (static_cast<long long>(share) << p.cost_shift) + slack * p.group) pieces = 0;
       else share = 1;
     }
@@ -960,29 +1000,56 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
     total = total_of(mine);
   }
   const long long x0_wide = static_cast<long long>(id) * share;
-  if (x0_wide >= total) return;
+  if (x0_wide >= total && !whole_tiles) return;
   int x0 = static_cast<int>(x0_wide), x1 = static_cast<int>(std::min<long long>(total, x0_wide + share));
-  // The sequence at x0, its start on the line, and from there the tile.
   int seq = -1, head, tile, start = 0;
   Shape s{0, 0, 0};
-  for (int b0 = 0; b0 < p.n_seq; b0 += 64) {
-    const int v = b0 == 0 ? mine : cost_at(b0 + lane, first);
-    const int up = sum_up(v);
-    const unsigned long long past = __ballot(start + up > x0);
-    if (past != 0) {
-      const int at = __builtin_ctzll(past);
-      seq = b0 + at;
-      start += __builtin_amdgcn_readlane(up, at) - __builtin_amdgcn_readlane(v, at);
-      pieces = __builtin_amdgcn_readlane(pieces, at);
-      s = Shape{__builtin_amdgcn_readlane(first.q0, at), __builtin_amdgcn_readlane(first.n_q, at), __builtin_amdgcn_readlane(first.n_k, at)};
-      break;
+  if (whole_tiles) {
+    const int want = over(block, p.by_heads);
+    head = block - want * p.kv_heads;
+    if (p.n_seq <= 64) {
+      tile_by_weight(p, first, want, seq, tile);
+    } else {
+      int base = 0;
+      for (int b0 = 0; b0 < p.n_seq && seq < 0; b0 += 64) {
+        int tiles = 0;
+        if (b0 + lane < p.n_seq) tiles = cost_of(p, shape_of(p, b0 + lane)).tiles;
+        const int up = sum_up(tiles);
+        const unsigned long long past = __ballot(base + up > want);
+        if (past != 0) {
+          const int at = __builtin_ctzll(past);
+          seq = b0 + at;
+          tile = base + __builtin_amdgcn_readlane(up, at) - 1 - want;  // a sequence's last tiles see the most keys
+        }
+        base += __builtin_amdgcn_readlane(up, 63);
+      }
     }
-    start += __builtin_amdgcn_readlane(up, 63);
-  }
-  if (seq < 0) return;  // (lengths that change under the call)
-  Cost c = cost_of(p, s);
-  c.pieces = pieces;
-  {
+    if (seq < 0) return;
+    s = shape_of(p, seq);
+    s = Shape{uniform(s.q0), uniform(s.n_q), uniform(s.n_k)};
+    // A line of one piece, the workgroup's.
+    pieces = 1;
+    total = share = x1 = 1;
+    x0 = id = 0;
+  } else {
+    // The sequence at x0, its start on the line, and from there the tile.
+    for (int b0 = 0; b0 < p.n_seq; b0 += 64) {
+      const int v = b0 == 0 ? mine : cost_at(b0 + lane, first);
+      const int up = sum_up(v);
+      const unsigned long long past = __ballot(start + up > x0);
+      if (past != 0) {
+        const int at = __builtin_ctzll(past);
+        seq = b0 + at;
+        start += __builtin_amdgcn_readlane(up, at) - __builtin_amdgcn_readlane(v, at);
+        pieces = __builtin_amdgcn_readlane(pieces, at);
+        s = Shape{__builtin_amdgcn_readlane(first.q0, at), __builtin_amdgcn_readlane(first.n_q, at), __builtin_amdgcn_readlane(first.n_k, at)};
+        break;
+      }
+      start += __builtin_amdgcn_readlane(up, 63);
+    }
+    if (seq < 0) return;  // (lengths that change under the call)
+    Cost c = cost_of(p, s);
+    c.pieces = pieces;
     const int per_head = c.before(c.tiles);
     head = uniform((x0 - start) / per_head);
     start += head * per_head;
@@ -1061,7 +1128,7 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
 
 template <typename T, int DP, bool kSmall>
 hipError_t launch(const PagedArgs& a, bool tiles, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(a.n_wg)), block(64 * (tiles ? kTileWaves : kChunkWaves));
+  const dim3 grid(static_cast<uint32_t>(std::max(a.n_wg, a.whole_tiles))), block(64 * (tiles ? kTileWaves : kChunkWaves));
   if (tiles)
     hipLaunchKernelGGL((paged_kernel<T, DP, kSmall, kTiles | kChunks>), grid, block, 0, stream, a);
   else
@@ -1088,6 +1155,11 @@ hipError_t launch_paged_attention(int dtype_bf16, PagedArgs& a, int n_cu, hipStr
   // As many workgroups as the device holds at a time: eight waves a compute unit.
   a.n_wg = std::min(8 / (tiles ? kTileWaves : kChunkWaves) * n_cu, kMostWorkgroups);
   a.by_wg = divisor_of(a.n_wg);
+  a.by_heads = divisor_of(a.kv_heads);
+  // Row tiles that may run whole: where there are some for each workgroup, none of
+  // them is late (one prompt of 16384 tokens, 32 heads over 8: 2250 us in shares).
+  const int64_t all_tiles = (rows / kTileRows<true> + std::max(1, a.n_seq)) * a.kv_heads;
+  a.whole_tiles = tiles && rows / kTileRows<true> * a.kv_heads >= 3ll * a.n_wg && all_tiles <= 0x7FFFFFFF ? static_cast<int32_t>(all_tiles) : 0;
   const int dp = a.dim <= 64 ? 64 : a.dim <= 96 ? 96 : 128;
   const uint64_t slots = 2ull * a.n_wg * (tiles ? kTileRows<true> : kTileRows<false>) * (dp + 2) * 4;
   if (slots > a.part_bytes || a.n_wg > a.n_counters) return hipErrorInvalidValue;
