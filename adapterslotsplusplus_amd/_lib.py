@@ -131,11 +131,11 @@ def load():
         "wp_packed_attention": ([p, p, p, p, p, p, p, p, p, p, p, p, i32, i64, i64, i32, i32, i32, f32, i32, i32, i32, p],
                                 ctypes.c_int),
         "wp_token_logprobs": ([p, p, p, p, p, p, p, i64, p, i32, i64, i32, i32, i32, p], ctypes.c_int),
-        "wp_rotate_heads": ([p, p, p, p, p, p, p, p, p, p, p, f32, p, i64, i32, i32, i32, i32, p], ctypes.c_int),
-        "wp_rotate_into_cache": ([p, p, p, p, p, p, p, p, p, p, p, f32, p, p, p, i32, i64, i32, i32, p], ctypes.c_int),
-        "wp_write_cache": ([p, p, p, p, p, p, p, i32, i64, i32, p], ctypes.c_int),
-        "wp_read_cache": ([p, p, p, p, p, p, p, i32, i64, i32, p], ctypes.c_int),
-        "wp_paged_attention": ([p, p, p, p, p, p, p, p, i64, i32, p, p, i32, i64, i32, f32, i32, i32, i32, p], ctypes.c_int),
+        "wp_rotate_heads": ([p, p, p, f32, p, i64, i32, i32, p], ctypes.c_int),
+        "wp_rotate_into_cache": ([p, p, p, p, f32, p, p, p, i32, i64, i32, p], ctypes.c_int),
+        "wp_write_cache": ([p, p, p, p, p, i32, i64, i32, p], ctypes.c_int),
+        "wp_read_cache": ([p, p, p, p, p, i32, i64, i32, p], ctypes.c_int),
+        "wp_paged_attention": ([p, p, p, p, p, i64, f32, i32, i32, i32, p], ctypes.c_int),
         "wp_barrier_probe": ([p, i32, i32, i32, p, p], ctypes.c_int),
     }
     for name, (args, res) in sig.items():

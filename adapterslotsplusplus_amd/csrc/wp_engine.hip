@@ -2726,24 +2726,31 @@ int check_rotation(const char* who, const wp_rotation* r, int32_t head_dim, Head
   return WP_OK;
 }
 
-// Rows of a kind: heads of `x`, and where they go (y, or, null, the cache).
-int head_part(const char* who, const char* what, HeadPart& h, const void* x, const int64_t* x_strides, const void* norm,
-              void* y, const int64_t* y_strides, bool rotate, int64_t tokens, int32_t heads, int32_t dim) {
+// Rows of a kind, and where they go (to_out; else to the cache).
+int head_part(const char* who, const char* what, HeadPart& h, const wp_head_rows& r, const void* norm, bool rotate, bool to_out,
+              int64_t tokens, int32_t dim) {
   int64_t s[2];
-  if (const int rc = head_strides(who, what, x, x_strides, tokens, heads, dim, false, s); rc != WP_OK) return rc;
+  if (const int rc = head_strides(who, what, r.x, r.strides, tokens, r.heads, dim, false, s); rc != WP_OK) return rc;
   if (!aligned(norm, 16)) return fail(WP_ERR_INVALID, "%s: norm weights must be 16-byte aligned", who);
-  h.x = x;
+  h.x = r.x;
   h.x_tok = s[0];
   h.x_head = s[1];
   h.norm = norm;
   h.rotate = rotate ? 1 : 0;
-  h.heads = heads;
-  if (y_strides) {
-    if (const int rc = head_strides(who, "an output", y, y_strides, tokens, heads, dim, true, s); rc != WP_OK) return rc;
-    h.y = y;
+  h.heads = r.heads;
+  if (to_out) {
+    if (const int rc = head_strides(who, "an output", r.out, r.out_strides, tokens, r.heads, dim, true, s); rc != WP_OK) return rc;
+    h.y = r.out;
     h.y_tok = s[0];
     h.y_head = s[1];
   }
+  return WP_OK;
+}
+
+int check_heads(const char* who, const wp_head_rows* r, const wp_pages* cache) {
+  if (r && (r->heads < 0 || r->heads > 65535)) return fail(WP_ERR_INVALID, "%s: %d heads", who, r->heads);
+  if (cache && (!r || r->heads != cache->kv_heads))
+    return fail(WP_ERR_INVALID, "%s: %d heads of a token, the cache has %d", who, r ? r->heads : 0, cache->kv_heads);
   return WP_OK;
 }
 
@@ -2802,84 +2809,74 @@ int run_rows(const char* who, wp_engine* e, HeadArgs& a, int64_t tokens, int32_t
 
 extern "C" {
 
-int wp_rotate_heads(wp_engine* e, void* q_out, const int64_t* q_out_strides, const void* q, const int64_t* q_strides,
-                    void* k_out, const int64_t* k_out_strides, const void* k, const int64_t* k_strides,
-                    const void* q_norm, const void* k_norm, float eps, const wp_rotation* rotation, int64_t tokens,
-                    int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype, void* stream) {
+int wp_rotate_heads(wp_engine* e, const wp_head_rows* q, const wp_head_rows* k, float eps, const wp_rotation* rotation,
+                    int64_t tokens, int32_t head_dim, int32_t dtype, void* stream) {
   const char* who = "rotate_heads";
   if (const int rc = check_rows(who, e, dtype, tokens); rc != WP_OK) return rc;
-  if (heads < 0 || heads > 65535 || kv_heads < 0 || kv_heads > 65535)
-    return fail(WP_ERR_INVALID, "%s: %d query and %d key heads", who, heads, kv_heads);
+  HeadArgs a{};
+  const wp_head_rows* rows[2] = {q, k};
+  for (const wp_head_rows* r : rows)
+    if (const int rc = check_heads(who, r, nullptr); rc != WP_OK) return rc;
   if (head_dim < 8 || head_dim > kMaxRowDim || head_dim % 8 != 0)
     return fail(WP_ERR_INVALID, "%s: head size %d (a multiple of 8 up to %d)", who, head_dim, kMaxRowDim);
-  if (tokens == 0 || heads + kv_heads == 0) return WP_OK;
-  HeadArgs a{};
+  if (tokens == 0 || ((!q || q->heads == 0) && (!k || k->heads == 0))) return WP_OK;
   if (const int rc = check_rotation(who, rotation, head_dim, a); rc != WP_OK) return rc;
-  if ((heads > 0 && !q_out_strides) || (kv_heads > 0 && !k_out_strides)) return fail(WP_ERR_INVALID, "%s: null strides", who);
-  if (heads > 0)
-    if (const int rc = head_part(who, "q", a.part[0], q, q_strides, q_norm, q_out, q_out_strides, rotation != nullptr, tokens, heads, head_dim);
-        rc != WP_OK)
-      return rc;
-  if (kv_heads > 0)
-    if (const int rc = head_part(who, "k", a.part[1], k, k_strides, k_norm, k_out, k_out_strides, rotation != nullptr, tokens, kv_heads, head_dim);
-        rc != WP_OK)
-      return rc;
+  for (int i = 0; i < 2; ++i)
+    if (rows[i] && rows[i]->heads > 0)
+      if (const int rc = head_part(who, i == 0 ? "q" : "k", a.part[i], *rows[i], rows[i]->norm, rotation != nullptr, true, tokens, head_dim);
+          rc != WP_OK)
+        return rc;
   return run_rows(who, e, a, tokens, head_dim, eps, dtype, stream);
 }
 
-int wp_rotate_into_cache(wp_engine* e, void* q_out, const int64_t* q_out_strides, const void* q,
-                         const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
-                         const int64_t* v_strides, const void* q_norm, const void* k_norm, float eps,
+int wp_rotate_into_cache(wp_engine* e, const wp_head_rows* q, const wp_head_rows* k, const wp_head_rows* v, float eps,
                          const wp_rotation* rotation, const wp_pages* cache, const void* slots,
-                         int32_t slots_are_int64, int64_t tokens, int32_t heads, int32_t dtype, void* stream) {
-  const char* who = heads == 0 && !rotation && !k_norm ? "write_cache" : "rotate_into_cache";
+                         int32_t slots_are_int64, int64_t tokens, int32_t dtype, void* stream) {
+  const char* who = !q && !rotation && k && !k->norm ? "write_cache" : "rotate_into_cache";
   if (const int rc = check_rows(who, e, dtype, tokens); rc != WP_OK) return rc;
-  if (heads < 0 || heads > 65535) return fail(WP_ERR_INVALID, "%s: %d query heads", who, heads);
   if (const int rc = check_pages(who, cache, kMaxRowDim); rc != WP_OK) return rc;
+  if (const int rc = check_heads(who, q, nullptr); rc != WP_OK) return rc;
+  for (const wp_head_rows* r : {k, v})
+    if (const int rc = check_heads(who, r, cache); rc != WP_OK) return rc;
   if (tokens == 0) return WP_OK;
   if (const int rc = check_slots(who, slots, slots_are_int64); rc != WP_OK) return rc;
   const int32_t dim = cache->head_dim;
   HeadArgs a{};
   if (const int rc = check_rotation(who, rotation, dim, a); rc != WP_OK) return rc;
-  if (heads > 0) {
-    if (!q_out_strides) return fail(WP_ERR_INVALID, "%s: null strides", who);
-    if (const int rc = head_part(who, "q", a.part[0], q, q_strides, q_norm, q_out, q_out_strides, rotation != nullptr, tokens, heads, dim);
-        rc != WP_OK)
-      return rc;
-  }
-  if (const int rc = head_part(who, "k", a.part[1], k, k_strides, k_norm, nullptr, nullptr, rotation != nullptr, tokens, cache->kv_heads, dim);
-      rc != WP_OK)
-    return rc;
-  if (const int rc = head_part(who, "v", a.part[2], v, v_strides, nullptr, nullptr, nullptr, false, tokens, cache->kv_heads, dim);
-      rc != WP_OK)
-    return rc;
+  if (q && q->heads > 0)
+    if (const int rc = head_part(who, "q", a.part[0], *q, q->norm, rotation != nullptr, true, tokens, dim); rc != WP_OK) return rc;
+  if (const int rc = head_part(who, "k", a.part[1], *k, k->norm, rotation != nullptr, false, tokens, dim); rc != WP_OK) return rc;
+  if (const int rc = head_part(who, "v", a.part[2], *v, nullptr, false, false, tokens, dim); rc != WP_OK) return rc;
   cached_part(a, 1, *cache);
   cached_part(a, 2, *cache);
   cache_args(a, *cache, slots, slots_are_int64);
   return run_rows(who, e, a, tokens, dim, eps, dtype, stream);
 }
 
-int wp_write_cache(wp_engine* e, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                   const wp_pages* cache, const void* slots, int32_t slots_are_int64, int64_t tokens, int32_t dtype,
-                   void* stream) {
-  return wp_rotate_into_cache(e, nullptr, nullptr, nullptr, nullptr, k, k_strides, v, v_strides, nullptr, nullptr, 0.f,
-                              nullptr, cache, slots, slots_are_int64, tokens, 0, dtype, stream);
+int wp_write_cache(wp_engine* e, const wp_head_rows* k, const wp_head_rows* v, const wp_pages* cache, const void* slots,
+                   int32_t slots_are_int64, int64_t tokens, int32_t dtype, void* stream) {
+  wp_head_rows rows{};
+  if (k) {
+    rows = *k;
+    rows.norm = nullptr;
+  }
+  return wp_rotate_into_cache(e, nullptr, k ? &rows : nullptr, v, 0.f, nullptr, cache, slots, slots_are_int64, tokens, dtype, stream);
 }
 
-int wp_read_cache(wp_engine* e, void* k_out, const int64_t* k_out_strides, void* v_out, const int64_t* v_out_strides,
-                  const wp_pages* cache, const void* slots, int32_t slots_are_int64, int64_t tokens, int32_t dtype,
-                  void* stream) {
+int wp_read_cache(wp_engine* e, const wp_head_rows* k, const wp_head_rows* v, const wp_pages* cache, const void* slots,
+                  int32_t slots_are_int64, int64_t tokens, int32_t dtype, void* stream) {
   const char* who = "read_cache";
   if (const int rc = check_rows(who, e, dtype, tokens); rc != WP_OK) return rc;
   if (const int rc = check_pages(who, cache, kMaxRowDim); rc != WP_OK) return rc;
+  const wp_head_rows* rows[3] = {nullptr, k, v};
+  for (int i = 1; i < 3; ++i)
+    if (const int rc = check_heads(who, rows[i], cache); rc != WP_OK) return rc;
   if (tokens == 0) return WP_OK;
   if (const int rc = check_slots(who, slots, slots_are_int64); rc != WP_OK) return rc;
   HeadArgs a{};
   for (int i = 1; i < 3; ++i) {
     int64_t s[2];
-    void* out = i == 1 ? k_out : v_out;
-    if (const int rc = head_strides(who, "an output", out, i == 1 ? k_out_strides : v_out_strides, tokens, cache->kv_heads, cache->head_dim,
-                                    true, s);
+    if (const int rc = head_strides(who, "an output", rows[i]->out, rows[i]->out_strides, tokens, cache->kv_heads, cache->head_dim, true, s);
         rc != WP_OK)
       return rc;
     cached_part(a, i, *cache);
@@ -2887,7 +2884,7 @@ int wp_read_cache(wp_engine* e, void* k_out, const int64_t* k_out_strides, void*
     h.x = h.y;
     h.x_tok = h.y_tok;
     h.x_head = h.y_head;
-    h.y = out;
+    h.y = rows[i]->out;
     h.y_tok = s[0];
     h.y_head = s[1];
     h.heads = cache->kv_heads;
@@ -2896,15 +2893,14 @@ int wp_read_cache(wp_engine* e, void* k_out, const int64_t* k_out_strides, void*
   return run_rows(who, e, a, tokens, cache->head_dim, 0.f, dtype, stream, true);
 }
 
-int wp_paged_attention(wp_engine* e, void* out, const int64_t* out_strides, float* lse, const void* q,
-                       const int64_t* q_strides, const wp_pages* cache, const int32_t* block_table,
-                       int64_t table_row_stride, int32_t columns, const int32_t* cu_q, const int32_t* kv_lens,
-                       int32_t n_seq, int64_t tokens, int32_t heads, float scale, int32_t window, int32_t sinks,
+int wp_paged_attention(wp_engine* e, const wp_head_rows* q, float* lse, const wp_pages* cache,
+                       const wp_sequences* sequences, int64_t tokens, float scale, int32_t window, int32_t sinks,
                        int32_t dtype, void* stream) {
   const char* who = "paged_attention";
   if (const int rc = check_rows(who, e, dtype, tokens); rc != WP_OK) return rc;
   if (const int rc = check_pages(who, cache, kMaxHeadDim); rc != WP_OK) return rc;
-  const int32_t kv_heads = cache->kv_heads, dim = cache->head_dim;
+  if (!q || !sequences) return fail(WP_ERR_INVALID, "%s: null q or sequences", who);
+  const int32_t kv_heads = cache->kv_heads, dim = cache->head_dim, heads = q->heads, n_seq = sequences->n_seq, columns = sequences->columns;
   if (heads < 1 || heads > 65535 || heads % kv_heads != 0)
     return fail(WP_ERR_INVALID, "%s: %d query heads do not share %d key heads evenly", who, heads, kv_heads);
   const int group = heads / kv_heads;
@@ -2915,25 +2911,26 @@ int wp_paged_attention(wp_engine* e, void* out, const int64_t* out_strides, floa
     return fail(WP_ERR_INVALID, "%s: a window must be positive, and only with one have first keys to stay in sight", who);
   if (tokens == 0) return WP_OK;
   int64_t qs[2], os[2];
-  if (const int rc = head_strides(who, "q", q, q_strides, tokens, heads, dim, false, qs); rc != WP_OK) return rc;
-  if (const int rc = head_strides(who, "out", out, out_strides, tokens, heads, dim, true, os); rc != WP_OK) return rc;
-  if (n_seq > 0 && (!cu_q || !kv_lens || (columns > 0 && !block_table))) return fail(WP_ERR_INVALID, "%s: null tensor", who);
-  if (!aligned(lse, 4) || !aligned(cu_q, 4) || !aligned(kv_lens, 4) || !aligned(block_table, 4))
+  if (const int rc = head_strides(who, "q", q->x, q->strides, tokens, heads, dim, false, qs); rc != WP_OK) return rc;
+  if (const int rc = head_strides(who, "out", q->out, q->out_strides, tokens, heads, dim, true, os); rc != WP_OK) return rc;
+  if (n_seq > 0 && (!sequences->cu_q || !sequences->kv_lens || (columns > 0 && !sequences->block_table)))
+    return fail(WP_ERR_INVALID, "%s: null tensor", who);
+  if (!aligned(lse, 4) || !aligned(sequences->cu_q, 4) || !aligned(sequences->kv_lens, 4) || !aligned(sequences->block_table, 4))
     return fail(WP_ERR_INVALID, "%s: bounds, lengths and block_table must be 4-byte aligned", who);
-  if (n_seq > 1 && table_row_stride < 0) return fail(WP_ERR_INVALID, "%s: negative table row stride", who);
+  if (n_seq > 1 && sequences->row_stride < 0) return fail(WP_ERR_INVALID, "%s: negative table row stride", who);
   DeviceGuard g(e->device);
   if (const int rc = model_scratch(e, who); rc != WP_OK) return rc;
   PagedArgs a{};
   const int size = cache->e4m3 ? 1 : 2;
   const bool many = cache->pages > 1, more = kv_heads > 1;
-  a.q = q;
-  a.out = out;
+  a.q = q->x;
+  a.out = q->out;
   a.lse = lse;
   a.k = static_cast<const char*>(cache->k);
   a.v = static_cast<const char*>(cache->v);
-  a.table = block_table;
-  a.cu_q = cu_q;
-  a.kv_lens = kv_lens;
+  a.table = sequences->block_table;
+  a.cu_q = sequences->cu_q;
+  a.kv_lens = sequences->kv_lens;
   a.q_tok = qs[0];
   a.q_head = qs[1];
   a.o_tok = os[0];
@@ -2955,7 +2952,7 @@ int wp_paged_attention(wp_engine* e, void* out, const int64_t* out_strides, floa
     a.vs_head = more ? cache->v_scale_strides[2] : 0;
   }
   a.tokens = tokens;
-  a.table_row = n_seq > 1 ? table_row_stride : 0;
+  a.table_row = n_seq > 1 ? sequences->row_stride : 0;
   a.n_pages = static_cast<int32_t>(cache->pages);
   a.page_shift = __builtin_ctz(static_cast<unsigned>(cache->page_size));
   a.capacity = static_cast<int32_t>(std::min<int64_t>(static_cast<int64_t>(columns) << a.page_shift, 0x7FFFFF00));

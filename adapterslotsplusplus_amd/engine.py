@@ -75,6 +75,14 @@ def _i32s(v) -> bytes:
     return struct.pack(f"{len(v)}I", *[k & 0xFFFFFFFF for k in v])
 
 
+# The library's argument structs, as bytes.
+_ROWS = struct.Struct("3Q4q2i")        # wp_head_rows
+_PAGES = struct.Struct("4Q13q4i")      # wp_pages
+_ROTATION = struct.Struct("2Q3if")     # wp_rotation
+_SEQUENCES = struct.Struct("3Qq2i")    # wp_sequences
+_INTS = {torch.int32: 0, torch.int64: 1}
+
+
 class TokenLogprobs(NamedTuple):
     """What token_logprobs returns, per row of the logits."""
     logprobs: torch.Tensor      # [rows] fp32: log softmax at the given token
@@ -900,24 +908,50 @@ class WarpPipeEngine:
     # cache in pages (not in the reference, whose models run it in vLLM).
 
     def _heads_of(self, t, what: str, op: str, dtype, dim: int):
-        """Checks of a [tokens, heads, dim] tensor."""
+        """The shape and the strides of a [tokens, heads, dim] tensor, checked."""
         if t.get_device() != self._dev_index:
             self._on_device(t, what)
         if t.dtype != dtype:
             raise RuntimeError(f"{op}: {what} must be {dtype}, got {t.dtype}")
-        if t.dim() != 3 or t.size(2) != dim:
-            raise RuntimeError(f"{op}: {what} must be [tokens, heads, {dim}], got {tuple(t.shape)}")
-        if dim > 1 and t.stride(2) != 1:
+        shape, strides = t.shape, t.stride()
+        if len(strides) != 3 or shape[2] != dim:
+            raise RuntimeError(f"{op}: {what} must be [tokens, heads, {dim}], got {tuple(shape)}")
+        if strides[2] != 1 and dim > 1:
             raise RuntimeError(f"{op}: a head's elements of {what} must be contiguous")
+        return shape, strides
 
-    def _head_norm(self, w, what: str, op: str, dtype, dim: int):
-        if w is None:
-            return None
-        if w.get_device() != self._dev_index:
-            self._on_device(w, what)
-        if w.dtype != dtype or w.shape != (dim,) or (dim > 1 and w.stride(0) != 1):
-            raise RuntimeError(f"{op}: {what} must be a contiguous [{dim}] tensor of {dtype}")
-        return w.data_ptr()
+    def _rows(self, t, shape, strides, norm, norm_name: str, out, out_name: str, op: str):
+        """(the C struct wp_head_rows as bytes, out): new rows unless `out` is given."""
+        w = 0
+        if norm is not None:
+            if norm.get_device() != self._dev_index:
+                self._on_device(norm, norm_name)
+            dim = shape[2]
+            if norm.dtype != t.dtype or norm.shape != (dim,) or (dim > 1 and norm.stride(0) != 1):
+                raise RuntimeError(f"{op}: {norm_name} must be a contiguous [{dim}] tensor of {t.dtype}")
+            w = norm.data_ptr()
+        if out is None:
+            out = torch.empty_like(t, memory_format=torch.contiguous_format)
+            to = (shape[1] * shape[2], shape[2])
+        else:
+            os, to = self._heads_of(out, out_name, op, t.dtype, shape[2])
+            if os != shape:
+                raise RuntimeError(f"{op}: {out_name} must be {tuple(shape)}, got {tuple(os)}")
+        return _ROWS.pack(t.data_ptr(), out.data_ptr(), w, strides[0], strides[1], to[0], to[1], shape[1], 0), out
+
+    def _kept_rows(self, t, what: str, op: str, dtype, heads: int, dim: int, norm=None):
+        """(the C struct wp_head_rows as bytes, tokens) of rows that go to a cache."""
+        shape, strides = self._heads_of(t, what, op, dtype, dim)
+        if shape[1] != heads:
+            raise RuntimeError(f"{op}: k and v must be [tokens, {heads}, {dim}], got {tuple(shape)}")
+        w = 0
+        if norm is not None:
+            if norm.get_device() != self._dev_index:
+                self._on_device(norm, "k_norm")
+            if norm.dtype != dtype or norm.shape != (dim,) or (dim > 1 and norm.stride(0) != 1):
+                raise RuntimeError(f"{op}: k_norm must be a contiguous [{dim}] tensor of {dtype}")
+            w = norm.data_ptr()
+        return _ROWS.pack(t.data_ptr(), 0, w, strides[0], strides[1], 0, 0, heads, 0), shape[0]
 
     def _rotation(self, rotary, positions, tokens: int, op: str):
         """The C struct wp_rotation as bytes, or None."""
@@ -930,49 +964,51 @@ class WarpPipeEngine:
             raise RuntimeError(f"{op}: rotating needs positions")
         if positions.get_device() != self._dev_index:
             self._on_device(positions, "positions")
-        if positions.dtype not in (torch.int64, torch.int32) or positions.shape != (tokens,) or (
-                tokens > 1 and positions.stride(0) != 1):
+        kind = positions.dtype
+        if kind not in _INTS or positions.shape != (tokens,) or (tokens > 1 and positions.stride(0) != 1):
             raise RuntimeError(f"{op}: positions must be a contiguous int32 or int64 [{tokens}] tensor")
-        return struct.pack("2Q3if", turns.data_ptr(), positions.data_ptr(), 1 if positions.dtype == torch.int64 else 0,
-                           rotary.dim, 1 if rotary.interleaved else 0, rotary.factor)
+        return _ROTATION.pack(turns.data_ptr(), positions.data_ptr(), _INTS[kind], rotary.dim, rotary.interleaved, rotary.factor)
 
     def _pages(self, k_pages, v_pages, k_scales, v_scales, dtype, op: str):
-        """The C struct wp_pages as bytes."""
+        """(the C struct wp_pages as bytes, kv_heads, dim)."""
         kept = k_pages.dtype
         if k_pages.get_device() != self._dev_index or v_pages.get_device() != self._dev_index:
             self._on_device(k_pages, "k_pages")
             self._on_device(v_pages, "v_pages")
-        if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != kept:
+        shape = k_pages.shape
+        if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != kept:
             raise RuntimeError(f"{op}: k_pages and v_pages must be [pages, page_size, kv_heads, dim] tensors of one dtype; "
-                               f"got {tuple(k_pages.shape)} {kept}, {tuple(v_pages.shape)} {v_pages.dtype}")
-        small = kept == torch.float8_e4m3fn
-        if not small and kept != dtype:
-            raise RuntimeError(f"{op}: pages must be {dtype} or float8_e4m3fn, got {kept}")
-        pages, size, heads, dim = k_pages.shape
-        ks, vs = k_pages.stride(), v_pages.stride()
-        if dim > 1 and (ks[3] != 1 or vs[3] != 1):
+                               f"got {tuple(shape)} {kept}, {tuple(v_pages.shape)} {v_pages.dtype}")
+        k0, k1, k2, k3 = k_pages.stride()
+        v0, v1, v2, v3 = v_pages.stride()
+        pages, size, heads, dim = shape
+        if dim > 1 and (k3 != 1 or v3 != 1):
             raise RuntimeError(f"{op}: a head's elements of the pages must be contiguous")
-        if not small:
+        if kept != torch.float8_e4m3fn:
+            if kept != dtype:
+                raise RuntimeError(f"{op}: pages must be {dtype} or float8_e4m3fn, got {kept}")
             if k_scales is not None or v_scales is not None:
                 raise RuntimeError(f"{op}: scales belong to float8_e4m3fn pages")
-            return struct.pack("4Q13q4i", k_pages.data_ptr(), v_pages.data_ptr(), 0, 0, *ks[:3], *vs[:3], 0, 0, 0, 0, 0, 0,
-                               pages, size, heads, dim, 0)
+            return _PAGES.pack(k_pages.data_ptr(), v_pages.data_ptr(), 0, 0, k0, k1, k2, v0, v1, v2, 0, 0, 0, 0, 0, 0, pages,
+                               size, heads, dim, 0), heads, dim
         for t, nm in ((k_scales, "k_scales"), (v_scales, "v_scales")):
             if t is None:
                 raise RuntimeError(f"{op}: float8_e4m3fn pages need {nm}")
             if t.get_device() != self._dev_index:
                 self._on_device(t, nm)
-            if t.dtype != torch.uint8 or t.shape != k_pages.shape[:3]:
-                raise RuntimeError(f"{op}: {nm} must be a uint8 {tuple(k_pages.shape[:3])} tensor")
-        return struct.pack("4Q13q4i", k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
-                           *ks[:3], *vs[:3], *k_scales.stride(), *v_scales.stride(), pages, size, heads, dim, 1)
+            if t.dtype != torch.uint8 or t.shape != shape[:3]:
+                raise RuntimeError(f"{op}: {nm} must be a uint8 {tuple(shape[:3])} tensor")
+        return _PAGES.pack(k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), k0, k1, k2, v0, v1,
+                           v2, *k_scales.stride(), *v_scales.stride(), pages, size, heads, dim, 1), heads, dim
 
     def _slots(self, slots, tokens: int, op: str) -> int:
+        """Whether slots are int64, checked."""
         if slots.get_device() != self._dev_index:
             self._on_device(slots, "slots")
-        if slots.dtype not in (torch.int64, torch.int32) or slots.shape != (tokens,) or (tokens > 1 and slots.stride(0) != 1):
+        kind = slots.dtype
+        if kind not in _INTS or slots.shape != (tokens,) or (tokens > 1 and slots.stride(0) != 1):
             raise RuntimeError(f"{op}: slots must be a contiguous int32 or int64 [{tokens}] tensor")
-        return 1 if slots.dtype == torch.int64 else 0
+        return _INTS[kind]
 
     def rotate_heads(self, q, k, positions, rotary, q_norm=None, k_norm=None, eps=1e-6, q_out=None, k_out=None):
         """Every head of q [tokens, heads, dim] and k [tokens, kv_heads, dim] (or
@@ -988,33 +1024,20 @@ class WarpPipeEngine:
         dt = _DTYPES.get(dtype)
         if dt is None:
             dt = _dtype_code(q, "q")
-        dim = q.size(-1) if q.dim() == 3 else 0
-        self._heads_of(q, "q", op, dtype, dim)
-        T, heads = q.size(0), q.size(1)
-        q_out = self._head_out(q_out, q, "q_out", op)
-        kv_heads = 0
-        kp = ko = ks = kos = None
+        shape, strides = self._heads_of(q, "q", op, dtype, q.shape[-1] if q.dim() else 0)
+        T, dim = shape[0], shape[2]
+        q_rows, q_out = self._rows(q, shape, strides, q_norm, "q_norm", q_out, "q_out", op)
+        k_rows = None
         if k is not None:
-            self._heads_of(k, "k", op, dtype, dim)
-            if k.size(0) != T:
-                raise RuntimeError(f"{op}: q has {T} tokens, k has {k.size(0)}")
-            kv_heads = k.size(1)
-            k_out = self._head_out(k_out, k, "k_out", op)
-            kp, ko, ks, kos = k.data_ptr(), k_out.data_ptr(), _i64s(k.stride()[:2]), _i64s(k_out.stride()[:2])
-        rc = self._lib.wp_rotate_heads(
-            self._handle, q_out.data_ptr(), _i64s(q_out.stride()[:2]), q.data_ptr(), _i64s(q.stride()[:2]), ko, kos, kp, ks,
-            self._head_norm(q_norm, "q_norm", op, dtype, dim), self._head_norm(k_norm, "k_norm", op, dtype, dim), eps,
-            self._rotation(rotary, positions, T, op), T, heads, kv_heads, dim, dt, _raw_stream(self._dev_index))
-        _lib.check(rc, op)
+            shape, strides = self._heads_of(k, "k", op, dtype, dim)
+            if shape[0] != T:
+                raise RuntimeError(f"{op}: q has {T} tokens, k has {shape[0]}")
+            k_rows, k_out = self._rows(k, shape, strides, k_norm, "k_norm", k_out, "k_out", op)
+        rc = self._lib.wp_rotate_heads(self._handle, q_rows, k_rows, eps, self._rotation(rotary, positions, T, op), T, dim, dt,
+                                       _raw_stream(self._dev_index))
+        if rc != 0:
+            _lib.check(rc, op)
         return q_out, (None if k is None else k_out)
-
-    def _head_out(self, out, like, what: str, op: str):
-        if out is None:
-            return torch.empty(like.shape, dtype=like.dtype, device=like.device)
-        self._heads_of(out, what, op, like.dtype, like.size(2))
-        if out.shape != like.shape:
-            raise RuntimeError(f"{op}: {what} must be {tuple(like.shape)}, got {tuple(out.shape)}")
-        return out
 
     def rotate_into_cache(self, q, k, v, positions, rotary, k_pages, v_pages, slots, k_scales=None, v_scales=None,
                           q_norm=None, k_norm=None, eps=1e-6, q_out=None):
@@ -1028,32 +1051,23 @@ class WarpPipeEngine:
         dt = _DTYPES.get(dtype)
         if dt is None:
             dt = _dtype_code(k, "k")
-        cache = self._pages(k_pages, v_pages, k_scales, v_scales, dtype, op)
-        kv_heads, dim = k_pages.size(2), k_pages.size(3)
-        T = self._kv_rows(k, v, kv_heads, dim, dtype, op)
-        heads = 0
-        qp = qo = qs = qos = None
+        cache, kv_heads, dim = self._pages(k_pages, v_pages, k_scales, v_scales, dtype, op)
+        k_rows, T = self._kept_rows(k, "k", op, dtype, kv_heads, dim, k_norm)
+        v_rows, n = self._kept_rows(v, "v", op, dtype, kv_heads, dim)
+        if n != T:
+            raise RuntimeError(f"{op}: k and v must be of as many tokens, got {T} and {n}")
+        q_rows = None
         if q is not None:
-            self._heads_of(q, "q", op, dtype, dim)
-            if q.size(0) != T:
-                raise RuntimeError(f"{op}: q has {q.size(0)} tokens, k has {T}")
-            heads = q.size(1)
-            q_out = self._head_out(q_out, q, "q_out", op)
-            qp, qo, qs, qos = q.data_ptr(), q_out.data_ptr(), _i64s(q.stride()[:2]), _i64s(q_out.stride()[:2])
-        rc = self._lib.wp_rotate_into_cache(
-            self._handle, qo, qos, qp, qs, k.data_ptr(), _i64s(k.stride()[:2]), v.data_ptr(), _i64s(v.stride()[:2]),
-            self._head_norm(q_norm, "q_norm", op, dtype, dim), self._head_norm(k_norm, "k_norm", op, dtype, dim), eps,
-            self._rotation(rotary, positions, T, op), cache, slots.data_ptr(), self._slots(slots, T, op), T, heads, dt,
-            _raw_stream(self._dev_index))
-        _lib.check(rc, op)
+            shape, strides = self._heads_of(q, "q", op, dtype, dim)
+            if shape[0] != T:
+                raise RuntimeError(f"{op}: q has {shape[0]} tokens, k has {T}")
+            q_rows, q_out = self._rows(q, shape, strides, q_norm, "q_norm", q_out, "q_out", op)
+        rc = self._lib.wp_rotate_into_cache(self._handle, q_rows, k_rows, v_rows, eps, self._rotation(rotary, positions, T, op),
+                                            cache, slots.data_ptr(), self._slots(slots, T, op), T, dt,
+                                            _raw_stream(self._dev_index))
+        if rc != 0:
+            _lib.check(rc, op)
         return None if q is None else q_out
-
-    def _kv_rows(self, k, v, kv_heads: int, dim: int, dtype, op: str) -> int:
-        self._heads_of(k, "k", op, dtype, dim)
-        self._heads_of(v, "v", op, dtype, dim)
-        if k.size(1) != kv_heads or v.shape != k.shape:
-            raise RuntimeError(f"{op}: k and v must be [tokens, {kv_heads}, {dim}], got {tuple(k.shape)} and {tuple(v.shape)}")
-        return k.size(0)
 
     def write_cache(self, k, v, k_pages, v_pages, slots, k_scales=None, v_scales=None) -> None:
         """Rows k and v [tokens, kv_heads, dim] to slots[token] (int32 or int64) of
@@ -1070,12 +1084,15 @@ class WarpPipeEngine:
         dt = _DTYPES.get(dtype)
         if dt is None:
             dt = _dtype_code(k, "k")
-        cache = self._pages(k_pages, v_pages, k_scales, v_scales, dtype, op)
-        T = self._kv_rows(k, v, k_pages.size(2), k_pages.size(3), dtype, op)
-        rc = self._lib.wp_write_cache(self._handle, k.data_ptr(), _i64s(k.stride()[:2]), v.data_ptr(),
-                                      _i64s(v.stride()[:2]), cache, slots.data_ptr(), self._slots(slots, T, op), T, dt,
+        cache, kv_heads, dim = self._pages(k_pages, v_pages, k_scales, v_scales, dtype, op)
+        k_rows, T = self._kept_rows(k, "k", op, dtype, kv_heads, dim)
+        v_rows, n = self._kept_rows(v, "v", op, dtype, kv_heads, dim)
+        if n != T:
+            raise RuntimeError(f"{op}: k and v must be of as many tokens, got {T} and {n}")
+        rc = self._lib.wp_write_cache(self._handle, k_rows, v_rows, cache, slots.data_ptr(), self._slots(slots, T, op), T, dt,
                                       _raw_stream(self._dev_index))
-        _lib.check(rc, op)
+        if rc != 0:
+            _lib.check(rc, op)
 
     def read_cache(self, k_pages, v_pages, slots, k_scales=None, v_scales=None, dtype=None):
         """The cache's rows of slots [tokens]: (k, v), each [tokens, kv_heads, dim],
@@ -1083,20 +1100,22 @@ class WarpPipeEngine:
         dtype (bf16 unless given).  Rows of a negative slot are zero, and so are
         those of one past the cache, which sets device error 1."""
         op = "read_cache"
-        kept = k_pages.dtype
         if dtype is None:
-            dtype = torch.bfloat16 if kept == torch.float8_e4m3fn else kept
+            dtype = torch.bfloat16 if k_pages.dtype == torch.float8_e4m3fn else k_pages.dtype
         dt = _DTYPES.get(dtype)
         if dt is None:
             raise RuntimeError(f"{op}: rows are read as fp16 or bf16, not {dtype}")
-        cache = self._pages(k_pages, v_pages, k_scales, v_scales, dtype, op)
+        cache, heads, dim = self._pages(k_pages, v_pages, k_scales, v_scales, dtype, op)
         T = slots.numel()
-        k = torch.empty((T,) + k_pages.shape[2:], dtype=dtype, device=k_pages.device)
+        wide = self._slots(slots, T, op)
+        k = torch.empty((T, heads, dim), dtype=dtype, device=k_pages.device)
         v = torch.empty_like(k)
-        rc = self._lib.wp_read_cache(self._handle, k.data_ptr(), _i64s(k.stride()[:2]), v.data_ptr(), _i64s(v.stride()[:2]),
-                                     cache, slots.data_ptr(), self._slots(slots, T, op), T, dt,
+        row = heads * dim
+        rc = self._lib.wp_read_cache(self._handle, _ROWS.pack(0, k.data_ptr(), 0, 0, 0, row, dim, heads, 0),
+                                     _ROWS.pack(0, v.data_ptr(), 0, 0, 0, row, dim, heads, 0), cache, slots.data_ptr(), wide, T, dt,
                                      _raw_stream(self._dev_index))
-        _lib.check(rc, op)
+        if rc != 0:
+            _lib.check(rc, op)
         return k, v
 
     def paged_attention(self, q, k_pages, v_pages, block_table, cu_seqlens_q, kv_lens, k_scales=None, v_scales=None,
@@ -1121,9 +1140,9 @@ class WarpPipeEngine:
         dt = _DTYPES.get(dtype)
         if dt is None:
             dt = _dtype_code(q, "q")
-        cache = self._pages(k_pages, v_pages, k_scales, v_scales, dtype, op)
-        self._heads_of(q, "q", op, dtype, k_pages.size(3))
-        T, heads, dim = q.shape
+        cache, _, dim = self._pages(k_pages, v_pages, k_scales, v_scales, dtype, op)
+        shape, strides = self._heads_of(q, "q", op, dtype, dim)
+        T = shape[0]
         for t, nm in ((block_table, "block_table"), (cu_seqlens_q, "cu_seqlens_q"), (kv_lens, "kv_lens")):
             if t.get_device() != dev:
                 self._on_device(t, nm)
@@ -1133,16 +1152,17 @@ class WarpPipeEngine:
         if kv_lens.dim() != 1 or cu_seqlens_q.shape != (n + 1,) or not kv_lens.is_contiguous() or not cu_seqlens_q.is_contiguous():
             raise RuntimeError(f"{op}: cu_seqlens_q must be a contiguous [n + 1] and kv_lens a contiguous [n] tensor, got "
                                f"{tuple(cu_seqlens_q.shape)} and {tuple(kv_lens.shape)}")
-        if block_table.dim() != 2 or block_table.size(0) != n or (block_table.size(1) > 1 and block_table.stride(1) != 1):
-            raise RuntimeError(f"{op}: block_table must be [{n}, columns] with unit column stride, got {tuple(block_table.shape)}")
-        out = self._head_out(out, q, "out", op)
-        lse = torch.empty(T, heads, dtype=torch.float32, device=q.device) if return_lse else None
+        table = block_table.shape
+        if len(table) != 2 or table[0] != n or (table[1] > 1 and block_table.stride(1) != 1):
+            raise RuntimeError(f"{op}: block_table must be [{n}, columns] with unit column stride, got {tuple(table)}")
+        rows, out = self._rows(q, shape, strides, None, "", out, "out", op)
+        lse = torch.empty(shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
         rc = self._lib.wp_paged_attention(
-            self._handle, out.data_ptr(), _i64s(out.stride()[:2]), None if lse is None else lse.data_ptr(), q.data_ptr(),
-            _i64s(q.stride()[:2]), cache, block_table.data_ptr(), block_table.stride(0), block_table.size(1),
-            cu_seqlens_q.data_ptr(), kv_lens.data_ptr(), n, T, heads, dim ** -0.5 if scale is None else float(scale),
-            _i32(window or 0), _i32(sinks or 0), dt, _raw_stream(dev))
-        _lib.check(rc, op)
+            self._handle, rows, None if lse is None else lse.data_ptr(), cache,
+            _SEQUENCES.pack(block_table.data_ptr(), cu_seqlens_q.data_ptr(), kv_lens.data_ptr(), block_table.stride(0), table[1], n),
+            T, dim ** -0.5 if scale is None else scale, _i32(window or 0), _i32(sinks or 0), dt, _raw_stream(dev))
+        if rc != 0:
+            _lib.check(rc, op)
         return out if lse is None else (out, lse)
 
     # ------------------------------------------------------------- staging --

@@ -401,6 +401,15 @@ int wp_token_logprobs(wp_engine* e, float* logprobs, float* entropy, int32_t* ra
  * elements contiguous and 16-byte aligned; strides in elements, multiples of 8
  * and not negative (any where there is one token or head). */
 
+/* Heads of a [tokens, heads, head_dim] tensor, and where their results go. */
+typedef struct wp_head_rows {
+  const void* x;
+  void* out;
+  const void* norm;                   /* norm weights [head_dim], or NULL */
+  int64_t strides[2], out_strides[2]; /* between tokens, between heads */
+  int32_t heads, reserved;
+} wp_head_rows;
+
 /* How a head's first `dim` elements (even, up to the head) turn: by
  * positions[token] * turns[i] / 2^64 turns for the pair i, (i, i + dim / 2) or,
  * interleaved, (2 i, 2 i + 1); cosine and sine times factor.  Products are
@@ -430,58 +439,58 @@ typedef struct wp_pages {
   int32_t page_size, kv_heads, head_dim, e4m3;
 } wp_pages;
 
-/* q_out and k_out: every head of q [tokens, heads] and k [tokens, kv_heads]
- * divided by its root mean square (of mean + eps) times q_norm / k_norm
- * [head_dim] where that is given, then turned by `rotation` where that is
- * given; in fp32, rounded once.  head_dim: a multiple of 8 up to 256.  Either
- * kind may have no heads.  An output may be its input, else they must not overlap. */
-int wp_rotate_heads(wp_engine* e, void* q_out, const int64_t* q_out_strides, const void* q, const int64_t* q_strides,
-                    void* k_out, const int64_t* k_out_strides, const void* k, const int64_t* k_strides,
-                    const void* q_norm, const void* k_norm, float eps, const wp_rotation* rotation, int64_t tokens,
-                    int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t dtype, void* stream);
+/* Every head of q and of k (either may be NULL or have no heads) divided by its
+ * root mean square (of mean + eps) times its norm weights where those are given, then
+ * turned by `rotation` where that is given; in fp32, rounded once.  head_dim: a
+ * multiple of 8 up to 256.  An out may be its x, else they must not overlap. */
+int wp_rotate_heads(wp_engine* e, const wp_head_rows* q, const wp_head_rows* k, float eps, const wp_rotation* rotation,
+                    int64_t tokens, int32_t head_dim, int32_t dtype, void* stream);
 
 /* The same in one launch with the keys going to slots[token] of the cache, and
- * the values v as they are.  Into an e4m3 cache a row (keys unrounded) is divided
- * by the smallest power of two s >= 2^-126 that brings its largest magnitude to
+ * the values v as they are (out of k and v, and v's norm, are not used).  Into an e4m3 cache a row (keys unrounded) is
+ * divided by the smallest power of two s >= 2^-126 that brings its largest magnitude to
  * at most 448 and rounded to nearest even; magnitudes that would come back past
  * the dtype's range take the largest that does not, infinities and NaN become NaN.  A
  * negative slot keeps no row; one past the cache is skipped and flagged (device
  * error 1).  Slots of one call must differ (else either row, or parts of both,
- * remain).  heads may be 0. */
-int wp_rotate_into_cache(wp_engine* e, void* q_out, const int64_t* q_out_strides, const void* q,
-                         const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
-                         const int64_t* v_strides, const void* q_norm, const void* k_norm, float eps,
+ * remain).  q may be NULL. */
+int wp_rotate_into_cache(wp_engine* e, const wp_head_rows* q, const wp_head_rows* k, const wp_head_rows* v, float eps,
                          const wp_rotation* rotation, const wp_pages* cache, const void* slots,
-                         int32_t slots_are_int64, int64_t tokens, int32_t heads, int32_t dtype, void* stream);
+                         int32_t slots_are_int64, int64_t tokens, int32_t dtype, void* stream);
 
 /* Keys and values as they are to slots[token] of the cache. */
-int wp_write_cache(wp_engine* e, const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                   const wp_pages* cache, const void* slots, int32_t slots_are_int64, int64_t tokens, int32_t dtype,
-                   void* stream);
+int wp_write_cache(wp_engine* e, const wp_head_rows* k, const wp_head_rows* v, const wp_pages* cache, const void* slots,
+                   int32_t slots_are_int64, int64_t tokens, int32_t dtype, void* stream);
 
-/* The rows of slots[token], in dtype (e4m3 times its factor, rounded once): k_out
- * and v_out [tokens, kv_heads, head_dim].  Rows of a negative slot are zero, and
- * so are those of one past the cache, which is flagged (device error 1). */
-int wp_read_cache(wp_engine* e, void* k_out, const int64_t* k_out_strides, void* v_out, const int64_t* v_out_strides,
-                  const wp_pages* cache, const void* slots, int32_t slots_are_int64, int64_t tokens, int32_t dtype,
-                  void* stream);
+/* The rows of slots[token], in dtype (e4m3 times its factor, rounded once), to out
+ * of k and v (their other fields are not used).  Rows of a negative slot are zero, and so are
+ * those of one past the cache, which is flagged (device error 1). */
+int wp_read_cache(wp_engine* e, const wp_head_rows* k, const wp_head_rows* v, const wp_pages* cache, const void* slots,
+                  int32_t slots_are_int64, int64_t tokens, int32_t dtype, void* stream);
 
-/* Attention of new tokens over the cache: sequence b has the queries [cu_q[b],
- * cu_q[b + 1]) (rows of q and out; cu_q is n_seq + 1 int32, on the device) and as
- * keys the first kv_lens[b] tokens (int32, device) of the pages block_table[b *
- * table_row_stride ..] (`columns` int32 a sequence, device); its last query stands at its
- * last key, so the step's own rows have to be in the cache before.  A query sees the keys up to its own position;
- * with window > 0 only the last `window` of them, and the first `sinks` of the
- * sequence.  Grouped heads, out, lse, strides and rounding as wp_packed_attention's; queries that
- * see no key, and rows of no sequence, get 0 and -inf.  Lengths past the table
- * are cut to it; bounds that fall leave rows of that call unspecified.  A page outside the
- * cache counts as keys and values of zero and is flagged (device error 1).  e4m3
- * elements times their row's factor are taken in dtype, where they are exact if
- * that can hold them. */
-int wp_paged_attention(wp_engine* e, void* out, const int64_t* out_strides, float* lse, const void* q,
-                       const int64_t* q_strides, const wp_pages* cache, const int32_t* block_table,
-                       int64_t table_row_stride, int32_t columns, const int32_t* cu_q, const int32_t* kv_lens,
-                       int32_t n_seq, int64_t tokens, int32_t heads, float scale, int32_t window, int32_t sinks,
+/* Where sequences' rows are, all on the device: sequence b has the rows [cu_q[b],
+ * cu_q[b + 1]) of the new tokens, and the first kv_lens[b] tokens of the pages
+ * block_table[b * row_stride ..], `columns` of them. */
+typedef struct wp_sequences {
+  const int32_t* block_table;
+  const int32_t* cu_q;    /* [n_seq + 1] */
+  const int32_t* kv_lens; /* [n_seq] */
+  int64_t row_stride;
+  int32_t columns, n_seq;
+} wp_sequences;
+
+/* Attention of new tokens over the cache: a sequence's queries are its rows of q
+ * [tokens, heads] (q's norm is not used), its keys and values those of its pages;
+ * its last query stands at its last key, so the step's own rows have to be in the
+ * cache before.  A query sees the keys up to its own position; with window > 0
+ * only the last `window` of them, and the first `sinks` of the sequence.  Grouped
+ * heads, out, lse (or NULL) and rounding as wp_packed_attention's; queries that see no
+ * key, and rows of no sequence, get 0 and -inf.  Lengths past the table are cut to
+ * it; bounds that fall leave rows of that call unspecified.  A page outside the cache counts
+ * as keys and values of zero and is flagged (device error 1).  e4m3 elements times
+ * their row's factor are taken in dtype, where they are exact if that can hold them. */
+int wp_paged_attention(wp_engine* e, const wp_head_rows* q, float* lse, const wp_pages* cache,
+                       const wp_sequences* sequences, int64_t tokens, float scale, int32_t window, int32_t sinks,
                        int32_t dtype, void* stream);
 
 /* ---- staging / prefetch ---------------------------------------------------- */
