@@ -48,7 +48,7 @@ __device__ __forceinline__ float over_row(float v, F f) {
   };
   v = f(v, moved(v, std::integral_constant<int, 0xB1>{}));   // its neighbour's
   v = f(v, moved(v, std::integral_constant<int, 0x4E>{}));   // the other two of four
-  v = f(v, moved(v, std::integral_constant<int, 0x141>{}));  // the other four of eight, reversed
+  if constexpr (L >= 8) v = f(v, moved(v, std::integral_constant<int, 0x141>{}));  // the other four of eight, reversed
   if constexpr (L >= 16) v = f(v, moved(v, std::integral_constant<int, 0x140>{}));
   if constexpr (L >= 32) v = f(v, __shfl_xor(v, 16));
   return v;
@@ -83,43 +83,53 @@ __device__ __forceinline__ u32x4 pack8(const float (&v)[8]) {
   return __builtin_bit_cast(u32x4, h);
 }
 
-// A lane's 8 elements of a row in e4m3: its bytes, and the row's scale code in
+// A lane's N elements of a row in e4m3: its bytes, and the row's scale code in
 // every lane.  The scale goes by the finite elements; infinities and magnitudes
-// that the tensors' type rounds to them become NaN, as e4m3 has none.  Where the largest magnitude would come
-// back beyond the type's range (fp16's 65504 is 256 * 2^8 in 4 significant
-// bits), it becomes the value below.
-template <typename T, int L>
-__device__ __forceinline__ u32x2 quantise(const float (&y)[8], uint32_t& code) {
+// that the tensors' type rounds to them become NaN, as e4m3 has none.  Where the
+// largest magnitude would come back beyond the type's range (fp16's 65504 is 256 *
+// 2^8 in 4 significant bits), it becomes the value below.  Such rows are told by their
+// largest magnitude, NaN if there is one, and looked at element by element.
+template <typename T, int L, int N>
+__device__ __forceinline__ void quantise(const float (&y)[N], uint32_t (&q)[N / 4], uint32_t& code) {
   constexpr bool kHalf = __is_same(T, _Float16);
   constexpr float kPast = kHalf ? 65520.f : 0x1.FFp127f;  // rounds to infinity
   constexpr int kTopScale = kHalf ? 8 : 120;              // 2^this * 256 is past the type's range
+  auto most = [](float a, float b) { return __builtin_elementwise_maximum(a, b); };
+  // 448 = 1.75 * 2^8.
+  auto scale_of = [](float top) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, top);
+    return std::clamp(static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0), -126, 127);
+  };
   float top = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) top = fabsf(y[e]) < kPast ? fmaxf(top, fabsf(y[e])) : top;
-  top = over_row<L>(top, [](float a, float b) { return fmaxf(a, b); });
-  const uint32_t bits = __builtin_bit_cast(uint32_t, top);
-  // 448 = 1.75 * 2^8.
-  int x = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-  x = std::clamp(x, -126, 127);
+  for (int e = 0; e < N; ++e) top = most(top, fabsf(y[e]));
+  top = over_row<L>(top, most);
+  const bool plain = top < kPast && scale_of(top) < kTopScale;
+  int x = scale_of(top);
+  float z[N];
+  if (__all(plain)) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) z[e] = __builtin_ldexpf(y[e], -x);
+  } else {
+    top = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) top = fabsf(y[e]) < kPast ? fmaxf(top, fabsf(y[e])) : top;
+    top = over_row<L>(top, most);
+    x = scale_of(top);
+    const float limit = x >= kTopScale ? 240.f : 448.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      z[e] = fabsf(y[e]) < kPast ? std::clamp(__builtin_ldexpf(y[e], -x), -limit, limit) : __builtin_nanf("");
+  }
   code = static_cast<uint32_t>(x + 127);
-  const float most = x >= kTopScale ? 240.f : 448.f;
-  float z[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float s = __builtin_ldexpf(y[e], -x);
-    z[e] = fabsf(y[e]) < kPast ? std::clamp(s, -most, most) : __builtin_nanf("");
-  }
-  u32x2 r{0u, 0u};
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < N / 4; ++h) {
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * h], z[4 * h + 1], 0, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * h + 2], z[4 * h + 3], w, true);
-    r[h] = static_cast<uint32_t>(w);
+    q[h] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(z[4 * h + 2], z[4 * h + 3], w, true));
   }
-  return r;
 }
 
-// The unit of this wave.
+// The unit of this wave: heads of a kind from head0 on, or (p.all) all of a token's.
 struct Unit {
   int64_t tok;
   int kind, head0;
@@ -143,6 +153,167 @@ __device__ __forceinline__ int64_t number(const void* p, int wide, int64_t i) {
   return wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
 }
 
+// Rows whose halves lie in whole 16-byte vectors (and what does not rotate, too):
+// a lane holds both vectors of eight pairs, so that each element is loaded once
+// and each pair's angle computed once a row group.  kAdjacent: the pairs of 16 elements in a row;
+// else elements 8 i .. of the first half and of the second, and past them two vectors that pass.
+//   y1 = r (x1 w1 c - x2 w2 s),  y2 = r (x2 w2 c + x1 w1 s),  r = 1 / sqrt(mean x^2 + eps)
+// with the products of weights and sines computed once for a kind's heads.
+template <typename T, int L, bool kAdjacent>
+__global__ __launch_bounds__(64 * kWaves) void head_pairs_kernel(HeadArgs p) {
+  constexpr int kRows = 64 / L;
+  touch_kernel_args<static_cast<int>(sizeof(HeadArgs))>();
+  Unit u;
+  if (!unit_of<kRows>(p, u)) return;
+  const int lane = static_cast<int>(threadIdx.x) & 63, col = lane % L, row = lane / L;
+  const int dim = p.dim, rot = p.positions != nullptr ? p.rot : 0, half = rot >> 1;
+  const bool holds = col * 16 < dim, turns = col * 16 < rot;
+  // The lane's two vectors.
+  const int past = 2 * (col - half / 8) * 8 + rot;
+  const int d1 = kAdjacent ? col * 16 : turns ? col * 8 : past, d2 = kAdjacent ? d1 + 8 : turns ? d1 + half : past + 8;
+  float c[8], s[8];
+  if (rot > 0) {
+    const uint64_t pos = static_cast<uint64_t>(number(p.positions, p.positions64, u.tok));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      c[e] = 1.f;
+      s[e] = 0.f;
+    }
+    if (turns) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) turn(pos, static_cast<uint64_t>(p.turns[col * 8 + e]), p.factor, c[e], s[e]);
+    }
+  }
+  // A vector's elements as the pairs' first and second ones.
+  auto pairs_of = [&](u32x4 a, u32x4 b, float (&x1)[8], float (&x2)[8]) {
+    float v[8], w[8];
+    unpack8<T>(a, v);
+    unpack8<T>(b, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x1[e] = !kAdjacent ? v[e] : e < 4 ? v[2 * e] : w[2 * e - 8];
+      x2[e] = !kAdjacent ? w[e] : e < 4 ? v[2 * e + 1] : w[2 * e - 7];
+    }
+  };
+  const float inv_dim = 1.f / static_cast<float>(dim);
+  const u32x4 zero{0u, 0u, 0u, 0u};
+  for (int kind = p.all ? 0 : u.kind; kind < (p.all ? 3 : u.kind + 1); ++kind) {
+    // (Selected field by field: a pointer to an argument would move them all to memory.)
+    auto mine = [&](auto f) { return kind == 0 ? f(p.part[0]) : kind == 1 ? f(p.part[1]) : f(p.part[2]); };
+    const int heads = mine([](const HeadPart& h) { return h.heads; });
+    if (heads == 0) continue;
+    const T* x = static_cast<const T*>(mine([](const HeadPart& h) { return h.x; })) +
+                 u.tok * mine([](const HeadPart& h) { return h.x_tok; });
+    const int64_t x_head = mine([](const HeadPart& h) { return h.x_head; });
+    const T* w = static_cast<const T*>(mine([](const HeadPart& h) { return h.norm; }));
+    const bool cached = mine([](const HeadPart& h) { return h.cached; }) != 0;
+    const bool rotates = rot > 0 && mine([](const HeadPart& h) { return h.rotate; }) != 0;
+    char* y = static_cast<char*>(mine([](const HeadPart& h) { return h.y; }));
+    uint8_t* scales = mine([](const HeadPart& h) { return h.scales; });
+    const int64_t y_tok = mine([](const HeadPart& h) { return h.y_tok; }), y_head = mine([](const HeadPart& h) { return h.y_head; });
+    const int64_t s_head = mine([](const HeadPart& h) { return h.s_head; });
+    const bool small = cached && p.e4m3 != 0;
+    if (cached) {
+      const int64_t slot = number(p.slots, p.slots64, u.tok);
+      if (slot < 0) continue;
+      if (slot >= p.n_slots) {
+        if (lane == 0 && u.head0 == 0) flag_error(p.header, kErrIdRange);
+        continue;
+      }
+      const int64_t page = slot >> p.page_shift, at = slot & ((1ll << p.page_shift) - 1);
+      y += (page * mine([](const HeadPart& h) { return h.y_page; }) + at * y_tok) * (small ? 1 : 2);
+      if (small) scales += page * mine([](const HeadPart& h) { return h.s_page; }) + at * mine([](const HeadPart& h) { return h.s_tok; });
+    } else {
+      y += u.tok * y_tok * 2;
+    }
+    const int head0 = p.all ? 0 : u.head0, end = p.all ? heads : std::min(heads, head0 + p.steps * kRows);
+    // Weights times sines.
+    float k11[8], k12[8], k21[8], k22[8];
+    {
+      float w1[8], w2[8];
+      if (w != nullptr) pairs_of(holds ? load16_global(w + d1) : zero, holds ? load16_global(w + d2) : zero, w1, w2);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = w != nullptr ? w1[e] : 1.f, b = w != nullptr ? w2[e] : 1.f;
+        k11[e] = rotates ? a * c[e] : a;
+        k22[e] = rotates ? b * c[e] : b;
+        k12[e] = rotates ? -b * s[e] : 0.f;
+        k21[e] = rotates ? a * s[e] : 0.f;
+      }
+    }
+    // A row of nothing but copies keeps every bit.
+    const bool copies = w == nullptr && !rotates && !small;
+    constexpr int kAtOnce = 2;
+    for (int h0 = head0; h0 < end; h0 += kAtOnce * kRows) {
+      u32x4 in1[kAtOnce], in2[kAtOnce];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int h = h0 + i * kRows + row;
+        const bool live = holds && h < end;
+        in1[i] = live ? load16_global(x + h * x_head + d1) : zero;
+        in2[i] = live ? load16_global(x + h * x_head + d2) : zero;
+      }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int h = h0 + i * kRows + row;
+        const bool live = holds && h < end;
+        if (copies) {
+          if (live) {
+            *reinterpret_cast<u32x4*>(y + (h * y_head + d1) * 2) = in1[i];
+            *reinterpret_cast<u32x4*>(y + (h * y_head + d2) * 2) = in2[i];
+          }
+          continue;
+        }
+        float x1[8], x2[8], z[16];
+        pairs_of(in1[i], in2[i], x1, x2);
+        float r = 1.f;
+        if (w != nullptr) {
+          float sum = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum = fmaf(x1[e], x1[e], fmaf(x2[e], x2[e], sum));
+          sum = over_row<L>(sum, [](float a, float b) { return a + b; });
+          r = 1.f / sqrtf(fmaf(sum, inv_dim, p.eps));
+        }
+        if (rotates) {
+          // (What passes beside rotating elements must not see its neighbour's infinities.)
+          const bool mixes = rot == dim || turns;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float a = mixes ? x2[e] : 0.f, b = mixes ? x1[e] : 0.f;
+            z[kAdjacent ? 2 * e : e] = fmaf(x1[e], k11[e], a * k12[e]) * r;
+            z[kAdjacent ? 2 * e + 1 : 8 + e] = fmaf(x2[e], k22[e], b * k21[e]) * r;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            z[kAdjacent ? 2 * e : e] = x1[e] * k11[e] * r;
+            z[kAdjacent ? 2 * e + 1 : 8 + e] = x2[e] * k22[e] * r;
+          }
+        }
+        if (small) {
+          uint32_t code, q[4];
+          quantise<T, L>(z, q, code);
+          if (live) {
+            *reinterpret_cast<u32x2*>(y + h * y_head + d1) = u32x2{q[0], q[1]};
+            *reinterpret_cast<u32x2*>(y + h * y_head + d2) = u32x2{q[2], q[3]};
+            if (col == 0) scales[h * s_head] = static_cast<uint8_t>(code);
+          }
+        } else if (live) {
+          float a[8], b[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            a[e] = z[e];
+            b[e] = z[8 + e];
+          }
+          *reinterpret_cast<u32x4*>(y + (h * y_head + d1) * 2) = pack8<T>(a);
+          *reinterpret_cast<u32x4*>(y + (h * y_head + d2) * 2) = pack8<T>(b);
+        }
+      }
+    }
+  }
+}
+
+// Any other rows: the lane's eight columns, and their partners' loaded beside them.
 template <typename T, int L>
 __global__ __launch_bounds__(64 * kWaves) void head_rows_kernel(HeadArgs p) {
   constexpr int kRows = 64 / L;
@@ -288,10 +459,10 @@ __global__ __launch_bounds__(64 * kWaves) void head_rows_kernel(HeadArgs p) {
         for (int e = 0; e < 8; ++e) v[e] = z[e];
       }
       if (small) {
-        uint32_t code;
-        const u32x2 q = quantise<T, L>(v, code);
+        uint32_t code, q[2];
+        quantise<T, L>(v, q, code);
         if (live) {
-          *reinterpret_cast<u32x2*>(y + h * y_head + d0) = q;
+          *reinterpret_cast<u32x2*>(y + h * y_head + d0) = u32x2{q[0], q[1]};
           if (d0 == 0) scales[h * s_head] = static_cast<uint8_t>(code);
         }
       } else if (live) {
@@ -373,8 +544,20 @@ __global__ __launch_bounds__(64 * kWaves) void read_rows_kernel(HeadArgs p) {
 // Splits each token's heads of each kind into units of `steps` wave-wide rows:
 // one unit if there are tokens enough, else as many as keep the device's
 // waves busy.
-bool plan_units(HeadArgs& a, int lanes, int n_cu) {
+bool plan_units(HeadArgs& a, int lanes, int n_cu, bool may_join) {
   const int rows = 64 / lanes;
+  // Tokens enough for eight waves a compute unit each take a wave for all of
+  // their heads, whose angles it computes once.
+  a.all = may_join && a.tokens >= 8ll * n_cu ? 1 : 0;
+  if (a.all) {
+    a.units_tok = 1;
+    a.units[0] = 1;
+    a.units[1] = a.units[2] = 0;
+    a.steps = 0;
+    a.n_units = static_cast<uint32_t>(a.tokens);
+    a.by_units = divisor_of(1);
+    return true;
+  }
   int most = 1;
   for (const HeadPart& h : a.part) most = std::max(most, (h.heads + rows - 1) / rows);
   int64_t steps = most;
@@ -395,17 +578,27 @@ bool plan_units(HeadArgs& a, int lanes, int n_cu) {
 
 }  // namespace
 
-hipError_t launch_head_rows(int dtype_bf16, HeadArgs& a, int n_cu, hipStream_t stream) {
-  const int lanes = a.dim <= 64 ? 8 : a.dim <= 128 ? 16 : 32;
-  if (!plan_units(a, lanes, n_cu)) return hipErrorInvalidValue;
+namespace {
+template <typename T>
+hipError_t head_rows(HeadArgs& a, int n_cu, hipStream_t stream) {
+  const bool pairs = a.dim % 16 == 0 && (a.positions == nullptr || a.rot % 16 == 0);
+  const int lanes = pairs ? (a.dim <= 64 ? 4 : a.dim <= 128 ? 8 : 16) : a.dim <= 64 ? 8 : a.dim <= 128 ? 16 : 32;
+  if (!plan_units(a, lanes, n_cu, pairs)) return hipErrorInvalidValue;
   const dim3 grid((a.n_units + kWaves - 1) / kWaves), block(64 * kWaves);
   auto go = [&](auto* kernel) {
     hipLaunchKernelGGL(kernel, grid, block, 0, stream, a);
     return hipGetLastError();
   };
-  if (dtype_bf16)
-    return lanes == 8 ? go(head_rows_kernel<__bf16, 8>) : lanes == 16 ? go(head_rows_kernel<__bf16, 16>) : go(head_rows_kernel<__bf16, 32>);
-  return lanes == 8 ? go(head_rows_kernel<_Float16, 8>) : lanes == 16 ? go(head_rows_kernel<_Float16, 16>) : go(head_rows_kernel<_Float16, 32>);
+  if (!pairs)
+    return lanes == 8 ? go(head_rows_kernel<T, 8>) : lanes == 16 ? go(head_rows_kernel<T, 16>) : go(head_rows_kernel<T, 32>);
+  if (a.interleaved)
+    return lanes == 4 ? go(head_pairs_kernel<T, 4, true>) : lanes == 8 ? go(head_pairs_kernel<T, 8, true>) : go(head_pairs_kernel<T, 16, true>);
+  return lanes == 4 ? go(head_pairs_kernel<T, 4, false>) : lanes == 8 ? go(head_pairs_kernel<T, 8, false>) : go(head_pairs_kernel<T, 16, false>);
+}
+}  // namespace
+
+hipError_t launch_head_rows(int dtype_bf16, HeadArgs& a, int n_cu, hipStream_t stream) {
+  return dtype_bf16 ? head_rows<__bf16>(a, n_cu, stream) : head_rows<_Float16>(a, n_cu, stream);
 }
 
 namespace {
@@ -424,7 +617,7 @@ hipError_t read_rows(const HeadArgs& a, int lanes, hipStream_t stream) {
 
 hipError_t launch_read_rows(int dtype_bf16, HeadArgs& a, int n_cu, hipStream_t stream) {
   const int lanes = a.dim <= 64 ? 8 : a.dim <= 128 ? 16 : 32;
-  if (!plan_units(a, lanes, n_cu)) return hipErrorInvalidValue;
+  if (!plan_units(a, lanes, n_cu, false)) return hipErrorInvalidValue;
   if (dtype_bf16) return a.e4m3 ? read_rows<__bf16, true>(a, lanes, stream) : read_rows<__bf16, false>(a, lanes, stream);
   return a.e4m3 ? read_rows<_Float16, true>(a, lanes, stream) : read_rows<_Float16, false>(a, lanes, stream);
 }

@@ -42,6 +42,7 @@ struct HeadArgs {
   // Filled by the launchers.
   Divisor by_units;  // units of a token
   int32_t units_tok, units[3], steps;
+  int32_t all;  // a unit is all of a token's heads
   uint32_t n_units;
 };
 // What rotate_heads, rotate_into_cache and write_cache run.
