@@ -172,7 +172,8 @@ __global__ __launch_bounds__(64 * kWaves) void head_pairs_kernel(HeadArgs p) {
   const int past = 2 * (col - half / 8) * 8 + rot;
   const int d1 = kAdjacent ? col * 16 : turns ? col * 8 : past, d2 = kAdjacent ? d1 + 8 : turns ? d1 + half : past + 8;
   float c[8], s[8];
-  if (rot > 0) {
+  bool known = rot == 0;  // the angles
+  auto angles = [&] {
     const uint64_t pos = static_cast<uint64_t>(number(p.positions, p.positions64, u.tok));
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -183,7 +184,8 @@ __global__ __launch_bounds__(64 * kWaves) void head_pairs_kernel(HeadArgs p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) turn(pos, static_cast<uint64_t>(p.turns[col * 8 + e]), p.factor, c[e], s[e]);
     }
-  }
+    known = true;
+  };
   // A vector's elements as the pairs' first and second ones.
   auto pairs_of = [&](u32x4 a, u32x4 b, float (&x1)[8], float (&x2)[8]) {
     float v[8], w[8];
@@ -227,6 +229,20 @@ __global__ __launch_bounds__(64 * kWaves) void head_pairs_kernel(HeadArgs p) {
       y += u.tok * y_tok * 2;
     }
     const int head0 = p.all ? 0 : u.head0, end = p.all ? heads : std::min(heads, head0 + p.steps * kRows);
+    // Loads go a batch ahead, the first ones before the angles are worked out.
+    constexpr int kAtOnce = 2;
+    u32x4 in1[kAtOnce], in2[kAtOnce];
+    auto load = [&](int h0) {
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int h = h0 + i * kRows + row;
+        const bool live = holds && h < end;
+        in1[i] = live ? load16_global(x + h * x_head + d1) : zero;
+        in2[i] = live ? load16_global(x + h * x_head + d2) : zero;
+      }
+    };
+    load(head0);
+    if (!known) angles();
     // Weights times sines.
     float k11[8], k12[8], k21[8], k22[8];
     {
@@ -243,29 +259,27 @@ __global__ __launch_bounds__(64 * kWaves) void head_pairs_kernel(HeadArgs p) {
     }
     // A row of nothing but copies keeps every bit.
     const bool copies = w == nullptr && !rotates && !small;
-    constexpr int kAtOnce = 2;
     for (int h0 = head0; h0 < end; h0 += kAtOnce * kRows) {
-      u32x4 in1[kAtOnce], in2[kAtOnce];
+      u32x4 now1[kAtOnce], now2[kAtOnce];
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
-        const int h = h0 + i * kRows + row;
-        const bool live = holds && h < end;
-        in1[i] = live ? load16_global(x + h * x_head + d1) : zero;
-        in2[i] = live ? load16_global(x + h * x_head + d2) : zero;
+        now1[i] = in1[i];
+        now2[i] = in2[i];
       }
+      if (h0 + kAtOnce * kRows < end) load(h0 + kAtOnce * kRows);
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
         const int h = h0 + i * kRows + row;
         const bool live = holds && h < end;
         if (copies) {
           if (live) {
-            *reinterpret_cast<u32x4*>(y + (h * y_head + d1) * 2) = in1[i];
-            *reinterpret_cast<u32x4*>(y + (h * y_head + d2) * 2) = in2[i];
+            *reinterpret_cast<u32x4*>(y + (h * y_head + d1) * 2) = now1[i];
+            *reinterpret_cast<u32x4*>(y + (h * y_head + d2) * 2) = now2[i];
           }
           continue;
         }
         float x1[8], x2[8], z[16];
-        pairs_of(in1[i], in2[i], x1, x2);
+        pairs_of(now1[i], now2[i], x1, x2);
         float r = 1.f;
         if (w != nullptr) {
           float sum = 0.f;
