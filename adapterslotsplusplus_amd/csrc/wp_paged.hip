@@ -86,6 +86,7 @@ struct Cost {
   long long lag, least, most;
   int extra, tiles, log_rows, shift;
   int pieces;  // of each tile, or 0: the line is one of costs
+  int stretches;  // of keys at the start of each tile that are not on the line
   // Where tile t starts, from the sequence's start.
   __device__ __forceinline__ int before(int t) const {
     if (pieces > 0) return t * pieces;
@@ -101,7 +102,9 @@ struct Cost {
     return static_cast<int>((a * least + line + (t - b) * most + static_cast<long long>(t) * extra) >> shift) + t;
   }
 };
-__device__ __forceinline__ Cost cost_of(const PagedArgs& p, const Shape& s) {
+// `stretch`: how many steps of keys such a stretch has (0: there are none).  All
+// tiles of a sequence have as many of them, before the first one's own tokens.
+__device__ __forceinline__ Cost cost_of(const PagedArgs& p, const Shape& s, int stretch = 0) {
   const int rows = s.n_q * p.group;
   Cost c;
   c.log_rows = rows > p.chunk_rows ? 7 : 5;
@@ -112,6 +115,11 @@ __device__ __forceinline__ Cost cost_of(const PagedArgs& p, const Shape& s) {
   c.most = p.window > 0 ? (static_cast<long long>(p.window) + p.sinks + 128) * p.group + (1 << c.log_rows) : (1ll << 60);
   c.shift = p.cost_shift;
   c.pieces = 0;
+  c.stretches = 0;
+  if (stretch > 0 && c.log_rows == 7 && s.n_k > s.n_q) {
+    c.stretches = (s.n_k - s.n_q) / kTileKeys / stretch;
+    c.lag -= static_cast<long long>(c.stretches) * stretch * kTileKeys * p.group;
+  }
   return c;
 }
 
@@ -204,8 +212,16 @@ struct Place {
   int total, share, near;
   int pieces;  // of each tile (Cost)
   int id;      // this workgroup's
-  // The item's step at which the line's point x cuts it.  Cuts near its ends are
-  // moved there: a cut costs the shares' way through memory.
+  int stretch, whole;  // steps of a stretch, and workgroups that do one: the ones before those on the line
+  int stretches;       // of the tile,
+  int tiles, one;      // one workgroup for each, `tiles` apart from `one` on
+  __device__ __forceinline__ int skipped() const { return stretches * stretch; }
+  // Where workgroup i leaves its share of the item, if it is not the whole: two places for each
+  // workgroup.  Its first item may have begun before it, its last one may go on after it,
+  // and what is left of a tile with stretches goes beside the first of those.
+  __device__ __forceinline__ int slot(int i, bool begins) const { return !begins ? 2 * i : stretches > 0 ? 2 * one + 1 : 2 * i + 1; }
+  // Of the steps on the line, the one at which the line's point x cuts the item.  Cuts near its ends
+  // are moved there: a cut costs the shares' way through memory.
   __device__ __forceinline__ int cut(int x, int steps) const {
     const int off = x - start, rest = cost - off;
     if (off <= 0) return 0;
@@ -213,7 +229,7 @@ struct Place {
     if (std::min(off, rest) < near) return off <= rest ? 0 : steps;
     return std::min(steps, static_cast<int>(static_cast<float>(off) * __builtin_amdgcn_rcpf(static_cast<float>(cost)) * static_cast<float>(steps) + 0.01f));
   }
-  __device__ __forceinline__ int from(int i) const { return static_cast<int>(std::min<long long>(total, static_cast<long long>(i) * share)); }
+  __device__ __forceinline__ int from(int i) const { return static_cast<int>(std::min<long long>(total, static_cast<long long>(i - whole) * share)); }
 };
 
 // What the workgroup shares.  The item and its place are kept here, not in registers,
@@ -605,10 +621,19 @@ __device__ __forceinline__ void run_tile(const PagedArgs& p, const Source<T, DP,
     // them, costs in registers.)
     tile_body(w, s0, s1, tops, c, std::integral_constant<bool, true>{}, knext, vnow);
   };
+  // Of two workgroups on a compute unit the older one goes first wherever both can, and the
+  // younger one ends 17% later, alone at the end (4 x 512 tokens over 10636 keys each).  So each
+  // has the right of way half of the time, by the clock: 4% (16384 keys, 2048 tokens: 1%).
+  const uint32_t young = blockIdx.x >= (static_cast<uint32_t>(p.n_wg) >> 1);
   for (int i = from; i < to; i += 2) {
+    if ((((static_cast<uint32_t>(__builtin_readcyclecounter()) >> 13) ^ young) & 1u) != 0)
+      __builtin_amdgcn_s_setprio(1);
+    else
+      __builtin_amdgcn_s_setprio(0);
     step(i, sk0, sk1, sv0, sv1);
     if (i + 1 < to) step(i + 1, sk1, sk0, sv1, sv0);
   }
+  __builtin_amdgcn_s_setprio(0);
 }
 
 // run_tile, one step after the other, with infinite and NaN values left out of
@@ -743,8 +768,7 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
   find_row();
   const bool split = it.from > 0 || it.to < it.steps;
   constexpr uint32_t kSlot = kSlotRows * (DP + 2);  // floats: [rows][DP] of O, then [rows][bound, sum]
-  // A workgroup's first item may have begun before it, and its last one may go on after it.
-  float* part = p.part + static_cast<uint64_t>(2 * uniform(sh.at.id) + (it.from == 0 ? 1 : 0)) * kSlot;
+  float* part = p.part + static_cast<uint64_t>(uniform(sh.at.slot(sh.at.id, it.from == sh.at.skipped()))) * kSlot;
   const __amdgpu_buffer_rsrc_t mine = coherent_buffer(part, kSlot * 4u);
   if constexpr (kTile) {
     if (!split) {
@@ -823,13 +847,14 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
   // The workgroup that does an item's last step joins its shares.  An item that
   // several share begins in one that no other shared item begins in: its counter's place.
   const Place at = sh.at;
-  const int first = uniform(at.start / at.share), final = uniform((at.start + at.cost - 1) / at.share);
+  const int first = uniform(at.whole + at.start / at.share), final = uniform(at.whole + (at.start + at.cost - 1) / at.share);
+  const int counter = uniform(at.stretches > 0 ? at.one : first);
   wait_vm();
   __syncthreads();
   if (tid == 0) {
     const unsigned mine = static_cast<unsigned>(it.to - it.from);
-    const bool last = atomic_add_u(p.counters + first, mine) + mine == static_cast<unsigned>(it.steps);
-    if (last) atomic_store_u(p.counters + first, 0u);
+    const bool last = atomic_add_u(p.counters + counter, mine) + mine == static_cast<unsigned>(it.steps);
+    if (last) atomic_store_u(p.counters + counter, 0u);
     sh.last = last ? 1u : 0u;
   }
   __syncthreads();
@@ -838,16 +863,18 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
   int* slots = reinterpret_cast<int*>(sk0);
   static_assert(Staged<DP>::kBytes >= kMostWorkgroups * sizeof(int), "there is room for a slot of each workgroup");
   if (wave == 0) {
-    int n = 0;
+    int n = uniform(at.stretches);
+    const int left = it.steps - uniform(at.skipped());
+    for (int i = lane; i < n; i += 64) slots[i] = at.slot(at.one + i * at.tiles, false);
     for (int i = first; i <= final; i += 64) {
       const int id = i + lane;
       int from = 0, to = 0;
       if (id <= final) {
-        from = at.cut(std::max(at.from(id), at.start), it.steps);
-        to = at.cut(std::min(at.from(id + 1), at.start + at.cost), it.steps);
+        from = at.cut(std::max(at.from(id), at.start), left);
+        to = at.cut(std::min(at.from(id + 1), at.start + at.cost), left);
       }
       const unsigned long long some = __ballot(to > from);
-      if (to > from) slots[n + __builtin_popcountll(some & ((1ull << lane) - 1))] = 2 * id + (from == 0 ? 1 : 0);
+      if (to > from) slots[n + __builtin_popcountll(some & ((1ull << lane) - 1))] = at.slot(id, from == 0);
       n += __builtin_popcountll(some);
     }
     if (lane == 0) sh.count = n;
@@ -999,10 +1026,35 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
     mine = c.tiles * pieces * p.kv_heads;
     total = total_of(mine);
   }
-  const long long x0_wide = static_cast<long long>(id) * share;
+  // Chunks over caches of different lengths: stretches of keys as long as a share, from
+  // the first key on, go to workgroups of their own, and the line is of what is left.
+  // Those on the line have more ends and starts of items to do, so a stretch is ten steps
+  // longer than a share (4 x 512 tokens over 16384, 9577, 2048 and 14536 keys: 444 us
+  // with all on the line, 430 with stretches of a share, 416; 16 x 128 tokens 504 and
+  // 428).  Below shares of 64 steps there is nothing in it: 168 and 175 us at 55.
+  int stretch = 0, whole = 0, mine_whole = 0;
+  if ((kRoles & kTiles) != 0 && pieces == 0 && !whole_tiles && p.n_seq <= 64 && p.window == 0) {
+    const float steps = ldexpf(static_cast<float>(share), p.cost_shift) * __builtin_amdgcn_rcpf(static_cast<float>(p.group * kTileKeys));
+    stretch = static_cast<int>(std::min(steps + 11.f, 0x1p25f));
+    Cost c;
+    if (steps >= 64.f && __ballot((first.n_k - first.n_q) / kTileKeys >= stretch) != 0) {
+      c = cost_of(p, first, stretch);
+      mine_whole = c.tiles * c.stretches * p.kv_heads;
+      whole = total_of(mine_whole);
+    }
+    if (whole > 0 && whole < p.n_wg) {
+      mine = c.before(c.tiles) * p.kv_heads;
+      total = total_of(mine);
+      share = total / (p.n_wg - whole) + 1;
+    } else {
+      stretch = whole = mine_whole = 0;
+    }
+  }
+  const long long x0_wide = static_cast<long long>(std::max(0, id - whole)) * share;
   if (x0_wide >= total && !whole_tiles) return;
   int x0 = static_cast<int>(x0_wide), x1 = static_cast<int>(std::min<long long>(total, x0_wide + share));
   int seq = -1, head, tile, start = 0;
+  int part = -1, one = 0;  // which stretch, and the workgroup of the sequence's first
   Shape s{0, 0, 0};
   if (whole_tiles) {
     const int want = over(block, p.by_heads);
@@ -1032,28 +1084,39 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
     total = share = x1 = 1;
     x0 = id = 0;
   } else {
-    // The sequence at x0, its start on the line, and from there the tile.
+    // The sequence at x0 (or of the stretch), its start on the line, and from there the tile.
+    const bool stretched = id < whole;
+    const int up_whole = stretch > 0 ? sum_up(mine_whole) : 0;
     for (int b0 = 0; b0 < p.n_seq; b0 += 64) {
       const int v = b0 == 0 ? mine : cost_at(b0 + lane, first);
       const int up = sum_up(v);
-      const unsigned long long past = __ballot(start + up > x0);
+      const unsigned long long past = __ballot(stretched ? up_whole > id : start + up > x0);
       if (past != 0) {
         const int at = __builtin_ctzll(past);
         seq = b0 + at;
         start += __builtin_amdgcn_readlane(up, at) - __builtin_amdgcn_readlane(v, at);
         pieces = __builtin_amdgcn_readlane(pieces, at);
+        one = __builtin_amdgcn_readlane(up_whole, at) - __builtin_amdgcn_readlane(mine_whole, at);
         s = Shape{__builtin_amdgcn_readlane(first.q0, at), __builtin_amdgcn_readlane(first.n_q, at), __builtin_amdgcn_readlane(first.n_k, at)};
         break;
       }
       start += __builtin_amdgcn_readlane(up, 63);
     }
     if (seq < 0) return;  // (lengths that change under the call)
-    Cost c = cost_of(p, s);
+    Cost c = cost_of(p, s, stretch);
     c.pieces = pieces;
     const int per_head = c.before(c.tiles);
-    head = uniform((x0 - start) / per_head);
-    start += head * per_head;
-    tile = tile_at(c, x0 - start);
+    if (stretched) {  // tiles beside one another have stretches of the same keys
+      const int rest = (id - one) / c.tiles;
+      tile = uniform(id - one - rest * c.tiles);
+      head = uniform(rest / c.stretches);
+      part = uniform(rest - head * c.stretches);
+      start += head * per_head;
+    } else {
+      head = uniform((x0 - start) / per_head);
+      start += head * per_head;
+      tile = tile_at(c, x0 - start);
+    }
     start = uniform(start + c.before(tile));
   }
   for (;;) {
@@ -1063,7 +1126,7 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
       it.head = head;
       it.tile = tile;
       it.s = s;
-      Cost c = cost_of(p, s);
+      Cost c = cost_of(p, s, stretch);
       c.pieces = pieces;
       const bool tiled = (kRoles & kTiles) != 0 && c.log_rows == 7;
       if (tiled) range_of<true, kWaves>(p, it); else range_of<false, kWaves>(p, it);
@@ -1075,8 +1138,19 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
       at.near = pieces > 0 ? 0 : std::min(share >> 3, ((tiled ? 512 : 128) * p.group) >> p.cost_shift);
       at.id = id;
       at.pieces = pieces;
-      it.from = uniform(at.cut(x0, it.steps));
-      it.to = uniform(at.cut(std::min(x1, start + at.cost), it.steps));
+      at.stretch = stretch;
+      at.whole = whole;
+      at.stretches = c.stretches;
+      at.tiles = c.tiles;
+      at.one = one + head * c.tiles * c.stretches + tile;
+      if (part >= 0) {
+        it.from = part * stretch;
+        it.to = it.from + stretch;
+      } else {
+        const int skipped = uniform(at.skipped());
+        it.from = skipped + uniform(at.cut(x0, it.steps - skipped));
+        it.to = skipped + uniform(at.cut(std::min(x1, start + at.cost), it.steps - skipped));
+      }
       __syncthreads();  // what the item before left in LDS has been read
       if (tid == 0) {
         sh.item = it;
@@ -1106,6 +1180,11 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
     share = uniform(at.share);
     pieces = uniform(at.pieces);
     id = uniform(at.id);
+    if ((kRoles & kTiles) != 0) {
+      stretch = uniform(at.stretch);
+      whole = uniform(at.whole);
+    }
+    part = -1;  // (those of a stretch end here: they are before the line)
     x0 = at.from(id);
     x1 = at.from(id + 1);
     start = uniform(at.start + at.cost);
@@ -1115,10 +1194,13 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
     head = it.head;
     tile = it.tile + 1;
     s = it.s;
-    if (tile < cost_of(p, s).tiles) continue;
+    const int tiles = uniform(at.tiles), of_head = tiles * uniform(at.stretches);
+    one = uniform(at.one) - head * of_head - it.tile;
+    if (tile < tiles) continue;
     tile = 0;
     if (++head < p.kv_heads) continue;
     head = 0;
+    one += of_head * p.kv_heads;
     do {  // (there is one, as the line goes on)
       if (++seq >= p.n_seq) return;
       s = shape_of(p, seq);

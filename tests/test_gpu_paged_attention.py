@@ -6,6 +6,7 @@ in the same precision.  8-bit rows are compared with the values they stand for,
 which the queries' type holds exactly.
 """
 import math
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -225,6 +226,34 @@ def test_workgroups_that_walk_long_caches(engine, window, sinks, small):
         tol, lse_tol = c.tolerance(*want)
         check(got, want[0], tol, "out")
         check(lse, want[1], lse_tol, "lse")
+
+
+def each_want(c):
+    """device_want of each request."""
+    parts, at_q, at_k = [], 0, 0
+    for n_q, n_k in zip(c.lens_q, c.lens_k):
+        parts.append(device_want(SimpleNamespace(lens_q=[n_q], lens_k=[n_k], q=c.q[at_q:at_q + n_q], rows=c.rows[at_k:at_k + n_k], values=c.values)))
+        at_q, at_k = at_q + n_q, at_k + n_k
+    return [torch.cat(t) for t in zip(*parts)]
+
+
+@pytest.mark.parametrize("small", [False, True], ids=["same", "8bit"])
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(128, 16, 64, BF), (32, 4, 128, HF), (64, 32, 32, BF)], ids=str)
+def test_chunks_of_different_caches(engine, heads, kv_heads, dim, dtype, small):
+    """More row tiles than workgroups over caches of different lengths, some longer
+    than a workgroup's share, one twice as long; a single token among them."""
+    more = 128 // heads  # as many rows of heads in all
+    lens_q, lens_k = [120 * more, 1, 200 * more, 0, 140 * more, 60 * more], [6000, 700, 3100, 50, 2000, 16000]
+    announce(f"paged chunks of different caches {heads}/{kv_heads}x{dim} {dtype} small={small}")
+    c = Case(lens_q, lens_k, heads, kv_heads, dim, dtype, page=32, small=small)
+    got, lse = c.run(engine)
+    want = each_want(c)
+    tol, lse_tol = c.tolerance(*want)
+    check(got, want[0], tol, "out")
+    check(lse, want[1], lse_tol, "lse")
+    again = c.run(engine)
+    assert torch.equal(got, again[0]) and torch.equal(lse, again[1])
+    assert engine.device_errors() == 0
 
 
 def test_scales(engine):
