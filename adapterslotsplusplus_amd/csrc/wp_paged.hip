@@ -7,23 +7,40 @@
 // bound of c s_ij: one pass over the keys, by the tiles of wp_attn_core.h.
 //
 // Lengths are known on the device alone, and a table has room for far more keys
-// than there are.  So a launch has two workgroups for each compute unit, and
-// each works out its share by itself: the cost of every row tile (32 or 128 rows
-// of a key head) in keys is a linear function of the tile, cut off below and at
-// the window, whose sum over a sequence has a closed form; the line of all tiles'
-// costs is cut into equal shares, wherever that is.  A tile that several workgroups
-// share is joined by the last of them to finish (by a counter of steps done), so
-// each key is read once, by one workgroup, and all end at about the same time.
+// than there are.  So a launch has as many workgroups as the device holds, and each
+// wave works out the workgroup's share by itself, a lane for each sequence.  The cost of a row
+// tile (32 or 128 rows of a key head) in keys is a linear function of the tile, cut off
+// below and at the window, whose sum over a sequence has a closed form:
+//   - a line of all tiles' costs, cut into equal shares wherever that is;
+//   - where there are no more tiles than workgroups and it takes no longer, a line of equal
+//     pieces, one for each workgroup, that has no end of one tile and start of another in a
+//     share (one token over 8192 keys: 35.5 -> 20.9 us);
+//   - chunks over long caches: first stretches of whole shares (see there);
+//   - many row tiles: each whole, the ones with the most keys first (see the launcher).
+// A tile that several workgroups share is joined by the last of them to finish (by a
+// counter of steps done), in a fixed order, so each key is read once for a tile, all
+// end at about the same time, and results repeat bit for bit.
 //
 // Two roles.  Tiles of 128 rows: four waves of 32 rows, 64 keys and values at a
 // time staged in LDS for all of them.  Up to 32 rows (single tokens, drafted
-// tokens): the waves share out the keys, 32 at a time.  Keys and values go from
-// their pages straight to LDS; in 8 bits they pass through registers, one tile
-// ahead, and become the queries' type on their way to LDS (a power of two and 4
-// significant bits are exact in both).
+// tokens): the waves share out the keys, 32 at a time.  Launches whose sequences have no
+// more rows than that on the whole have workgroups of two waves, twice as many of them: 64 single
+// tokens over 1 to 8192 keys, 32 heads over 8 of 128, 89 us, and 100 in workgroups of
+// four; 64 of 8 tokens 106 and 117.  (Few requests of 20 to 32 rows each would rather have
+// four, with half as many shares to join: 16 of 8 tokens 64 and 54.)
 //
-// 16 keys are the unit of loads: a page holds whole ones, so that a wave's load
-// has one base address, out of a list of pages in LDS.
+// Keys and values go from their pages straight to LDS; in 8 bits they pass through
+// registers, one tile ahead, and become the queries' type on their way to LDS (a power
+// of two and 4 significant bits are exact in it, in fp16 where its range holds them).  16 keys are the unit of loads: a page holds whole ones, so that a
+// wave's load has one base address.  Places of granules are listed in LDS as the first
+// words of their buffers' descriptions, by lanes side by side, well before they are
+// loaded: the tables' latency and the address arithmetic are off the path.
+//
+// What bounds it (32 heads over 8 of 128, bf16).  Single tokens: HBM, 64 over 8192 keys
+// each at 5.7 TB/s; over 1 to 8192 keys 85 us at 4.1 TB/s; 8-bit rows 5.2 TB/s (208 us),
+// near the conversions' rate.  Few: the chain from launch to join, 14.5 us over 777 keys.
+// Chunks: matrix and vector units as in wp_attn.hip, 2048 tokens over 16384 keys 495 us
+// (1.04 PF/s), in 8 bits 540: converting there takes the wave's own slots.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -1246,10 +1263,13 @@ hipError_t launch_paged_attention(int dtype_bf16, PagedArgs& a, int n_cu, hipStr
   a.n_wg = std::min(8 / (tiles ? kTileWaves : kChunkWaves) * n_cu, kMostWorkgroups);
   a.by_wg = divisor_of(a.n_wg);
   a.by_heads = divisor_of(a.kv_heads);
-  // Row tiles that may run whole: where there are some for each workgroup, none of
-  // them is late (one prompt of 16384 tokens, 32 heads over 8: 2250 us in shares).
+  // Row tiles that may run whole: where there are some for each workgroup, and sequences
+  // are not short ones, whose tiles' starts take the most of it (us, whole and in shares; 32
+  // heads over 8 of 128: a prompt of 16384 tokens 2132 and 2253, 8 of 2048 385 and 441, 16
+  // of 512 98 and 121, 64 of 512 389 and 362, 32 of 400 151 and 138, 64 of 100 74 and 68,
+  // 256 of 60 174 and 123).
   const int64_t all_tiles = (rows / kTileRows<true> + std::max(1, a.n_seq)) * a.kv_heads;
-  a.whole_tiles = tiles && rows / kTileRows<true> * a.kv_heads >= 3ll * a.n_wg && all_tiles <= 0x7FFFFFFF ? static_cast<int32_t>(all_tiles) : 0;
+  a.whole_tiles = tiles && rows / kTileRows<true> * a.kv_heads >= 3ll * a.n_wg && a.tokens >= 448ll * a.n_seq && all_tiles <= 0x7FFFFFFF ? static_cast<int32_t>(all_tiles) : 0;
   const int dp = a.dim <= 64 ? 64 : a.dim <= 96 ? 96 : 128;
   const uint64_t slots = 2ull * a.n_wg * (tiles ? kTileRows<true> : kTileRows<false>) * (dp + 2) * 4;
   if (slots > a.part_bytes || a.n_wg > a.n_counters) return hipErrorInvalidValue;

@@ -256,6 +256,21 @@ def test_chunks_of_different_caches(engine, heads, kv_heads, dim, dtype, small):
     assert engine.device_errors() == 0
 
 
+@pytest.mark.parametrize("lens_q,lens_k,heads", [([900, 450, 600, 500, 800], [900, 700, 600, 1600, 800], 64), ([450, 451] * 35, [450, 480] * 35, 8),
+                                                 ([700] * 5, [700, 700, 700, 700, 30000], 64)], ids=["five", "seventy", "one-long"])
+def test_many_row_tiles(engine, lens_q, lens_k, heads):
+    """Several row tiles for each workgroup, of alike lengths and with one cache far longer."""
+    announce(f"paged many row tiles, {len(lens_q)} requests")
+    c = Case(lens_q, lens_k, heads, heads, 16, HF, page=64)
+    got, lse = c.run(engine)
+    want = each_want(c)
+    tol, lse_tol = c.tolerance(*want)
+    check(got, want[0], tol, "out")
+    check(lse, want[1], lse_tol, "lse")
+    again = c.run(engine)
+    assert torch.equal(got, again[0]) and torch.equal(lse, again[1])
+
+
 def test_scales(engine):
     for scale in (0.0, 1.0, 4.0, -0.3):
         attend(engine, [100], [300], 2, 2, 64, BF, scale=scale)
