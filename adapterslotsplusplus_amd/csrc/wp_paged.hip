@@ -26,15 +26,15 @@
 // tokens): the waves share out the keys, 32 at a time.  Launches whose sequences have no
 // more rows than that on the whole have workgroups of two waves, twice as many of them: 64 single
 // tokens over 1 to 8192 keys, 32 heads over 8 of 128, 89 us, and 100 in workgroups of
-// four; 64 of 8 tokens 106 and 117.  (Few requests of 20 to 32 rows each would rather have
-// four, with half as many shares to join: 16 of 8 tokens 64 and 54.)
+// four; 64 of 8 tokens 106 and 117 (and see the launcher).
 //
 // Keys and values go from their pages straight to LDS; in 8 bits they pass through
 // registers, one tile ahead, and become the queries' type on their way to LDS (a power
-// of two and 4 significant bits are exact in it, in fp16 where its range holds them).  16 keys are the unit of loads: a page holds whole ones, so that a
-// wave's load has one base address.  Places of granules are listed in LDS as the first
-// words of their buffers' descriptions, by lanes side by side, well before they are
-// loaded: the tables' latency and the address arithmetic are off the path.
+// of two and 4 significant bits are exact in it, in fp16 where its range holds them).
+// 16 keys are the unit of loads: a page holds whole ones, so that a wave's load has one
+// base address.  Places of granules are listed in LDS as the first words of their
+// buffers' descriptions, by lanes side by side, well before they are loaded: the tables'
+// latency and the address arithmetic are off the path.
 //
 // What bounds it (32 heads over 8 of 128, bf16).  Single tokens: HBM, 64 over 8192 keys
 // each at 5.7 TB/s; over 1 to 8192 keys 85 us at 4.1 TB/s; 8-bit rows 5.2 TB/s (208 us),
@@ -1257,7 +1257,12 @@ hipError_t launch_paged_attention(int dtype_bf16, PagedArgs& a, int n_cu, hipStr
   a.by_group = divisor_of(a.group);
   const int64_t rows = a.tokens * a.group;
   // Sequences of few rows on the whole run on key chunks, in tiles of 32 rows.
-  const bool tiles = rows > static_cast<int64_t>(kWaveRows) * std::max(1, a.n_seq);
+  // Few sequences of many such rows, though, in workgroups of four waves, as row tiles are: half
+  // as many shares of each to join (us, in four and in two, 32 heads over 8 of 128: 4 of 8
+  // tokens 41 and 48, 16 of 6 59 and 69, 32 of 8 100 and 107; 64 of 8 117 and 106, 16 of 4 58
+  // and 60, 4 of 4 40 and 35; heads of 64, 4 of 4 tokens 29 and 24).
+  const bool few = a.dim > 64 && rows >= 24ll * a.n_seq && static_cast<int64_t>(a.n_seq) * a.kv_heads <= n_cu;
+  const bool tiles = few || rows > static_cast<int64_t>(kWaveRows) * std::max(1, a.n_seq);
   a.chunk_rows = tiles ? kWaveRows : 0x7FFFFFFF;
   // As many workgroups as the device holds at a time: eight waves a compute unit.
   a.n_wg = std::min(8 / (tiles ? kTileWaves : kChunkWaves) * n_cu, kMostWorkgroups);
