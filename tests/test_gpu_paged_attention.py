@@ -349,6 +349,19 @@ def test_lengths_past_the_table_are_cut(engine):
     check(got[2:], want[0][2:], c.tolerance(*want)[0][2:], "out")
 
 
+@pytest.mark.parametrize("small", [False, True], ids=["same", "8bit"])
+def test_requests_that_share_pages(engine, small):
+    """A prefix kept once: several rows of the table name the same pages, and a
+    request may name one twice."""
+    c = Case([1, 40, 3], [300, 300, 300], 8, 2, 128, BF, page=32, small=small)
+    t = c.table.clone()
+    t[1], t[2] = t[0], t[0]
+    t[2, 4] = t[2, 3]
+    got = engine.paged_attention(c.q.cuda(), *c.dev, t.cuda(), c.cu, c.kv, *c.scales)
+    want = co.paged_attention(c.q, *c.values, t, c.lens_q, c.lens_k, 128 ** -0.5)
+    check(got, want[0], c.tolerance(*want)[0], "out")
+
+
 def test_unseen_keys_do_not_matter(engine):
     """NaN and infinity in keys and values that a query does not see leave it as it is."""
     for heads, kv_heads, small in ((2, 2, False), (8, 1, False), (8, 1, True)):
