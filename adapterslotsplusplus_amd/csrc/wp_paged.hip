@@ -213,7 +213,7 @@ struct Item {
   int seq, head, tile;
   Shape s;
   int row0, rows;         // of the sequence's rows of this key head
-  int end;                // no row sees a key from here on
+  int low, end;           // rows see keys from `low` on, before `end`, and the first keys
   int base, sink_steps;   // step i: keys from i * kStep for the first sink_steps, then from base on
   int steps, from, to;    // all of its steps, and the workgroup's
 
@@ -271,7 +271,7 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 __device__ __forceinline__ Item item_of(const Shared& sh) {
   const Item& i = sh.item;
   return Item{uniform(i.seq), uniform(i.head), uniform(i.tile), Shape{uniform(i.s.q0), uniform(i.s.n_q), uniform(i.s.n_k)},
-              uniform(i.row0), uniform(i.rows), uniform(i.end), uniform(i.base), uniform(i.sink_steps), uniform(i.steps),
+              uniform(i.row0), uniform(i.rows), uniform(i.low), uniform(i.end), uniform(i.base), uniform(i.sink_steps), uniform(i.steps),
               uniform(i.from), uniform(i.to)};
 }
 
@@ -284,8 +284,8 @@ __device__ __forceinline__ void range_of(const PagedArgs& p, Item& it) {
   const int lag = it.s.n_k - it.s.n_q;
   const int t0 = over(it.row0, p.by_group), t1 = over(it.row0 + it.rows - 1, p.by_group);
   it.end = std::clamp(t1 + lag + 1, 0, it.s.n_k);
-  const int low = std::min(window_start(t0 + lag, p.window), it.end);
-  it.base = low / kKeys * kKeys;
+  it.low = std::min(window_start(t0 + lag, p.window), it.end);
+  it.base = it.low / kKeys * kKeys;
   const int sinks = std::min(p.sinks, it.end);
   it.sink_steps = std::min((sinks + kKeys - 1) / kKeys, it.base / kKeys);
   it.steps = std::max(1, it.sink_steps + (it.end - it.base + kKeys - 1) / kKeys);
@@ -419,16 +419,22 @@ struct Source {
   }
 };
 
-// The page of the granule at `key` (0 past the item's last key).
-__device__ __forceinline__ int page_of(const PagedArgs& p, const Item& it, int key) {
-  return key < it.end ? p.table[static_cast<int64_t>(it.seq) * p.table_row + (key >> p.page_shift)] : 0;
+// Rows of the granule at `key` up to the item's last key, 0 or less past it and
+// where no row of the item sees any: steps begin before a window and end past the first
+// keys, and pages out of sight need not be there any more.
+__device__ __forceinline__ int rows_at(const PagedArgs& p, const Item& it, int key) {
+  return key + kGranule > it.low || key < p.sinks ? it.end - key : 0;
 }
-// Lists the granule at `key`, in `page`.  Nothing is there past the last key, and
-// of a page outside the cache (which is flagged).
+// The page of the granule at `key` (0 where it has no rows).
+__device__ __forceinline__ int page_of(const PagedArgs& p, const Item& it, int key) {
+  return rows_at(p, it, key) > 0 ? p.table[static_cast<int64_t>(it.seq) * p.table_row + (key >> p.page_shift)] : 0;
+}
+// Lists the granule at `key`, in `page`: its rows, and nothing of a page outside
+// the cache (which is flagged).
 template <bool kSmall>
 __device__ __forceinline__ void list_granule(const PagedArgs& p, const Item& it, int key, int page, Listed& list, Listed& scales) {
   const int row_bytes = kSmall ? p.dim : 2 * p.dim;
-  int rows = it.end - key;
+  int rows = rows_at(p, it, key);
   if (page < 0 || page >= p.n_pages) {
     if (rows > 0) flag_error(p.header, kErrIdRange);
     rows = 0;
