@@ -92,16 +92,16 @@ __device__ __forceinline__ u32x4 pack8(const float (&v)[8]) {
 }
 
 // A lane's N elements of a row in e4m3: its bytes, and the row's scale code in
-// every lane.  The scale goes by the finite elements; infinities and magnitudes
-// that the tensors' type rounds to them become NaN, as e4m3 has none.  Where the
-// largest magnitude would come back beyond the type's range (fp16's 65504 is 256 *
-// 2^8 in 4 significant bits), it becomes the value below.  Such rows are told by their
-// largest magnitude, NaN if there is one, and looked at element by element.
+// every lane.  The scale goes by the finite elements; infinities and NaN become NaN,
+// as e4m3 has no infinity.  Magnitudes past the tensors' type's range count as its
+// largest, so the scale ends where that one's does (fp16's 65504: 2^8), and where a
+// magnitude would come back beyond the range (65504 is 256 * 2^8 in 4 significant
+// bits), it becomes the value below.  Such rows are told by their largest
+// magnitude, NaN if there is one, and looked at element by element.
 template <typename T, int L, int N>
 __device__ __forceinline__ void quantise(const float (&y)[N], uint32_t (&q)[N / 4], uint32_t& code) {
   constexpr bool kHalf = __is_same(T, _Float16);
-  constexpr float kPast = kHalf ? 65520.f : 0x1.FFp127f;  // rounds to infinity
-  constexpr int kTopScale = kHalf ? 8 : 120;              // 2^this * 256 is past the type's range
+  constexpr int kTopScale = kHalf ? 8 : 120;  // of the type's largest; 2^this * 256 is past its range
   auto most = [](float a, float b) { return __builtin_elementwise_maximum(a, b); };
   // 448 = 1.75 * 2^8.
   auto scale_of = [](float top) {
@@ -112,8 +112,8 @@ __device__ __forceinline__ void quantise(const float (&y)[N], uint32_t (&q)[N / 
 #pragma unroll
   for (int e = 0; e < N; ++e) top = most(top, fabsf(y[e]));
   top = over_row<L>(top, most);
-  const bool plain = top < kPast && scale_of(top) < kTopScale;
   int x = scale_of(top);
+  const bool plain = x < kTopScale;  // (an infinity's and NaN's is past it)
   float z[N];
   if (__all(plain)) {
 #pragma unroll
@@ -121,13 +121,13 @@ __device__ __forceinline__ void quantise(const float (&y)[N], uint32_t (&q)[N / 
   } else {
     top = 0.f;
 #pragma unroll
-    for (int e = 0; e < N; ++e) top = fabsf(y[e]) < kPast ? fmaxf(top, fabsf(y[e])) : top;
+    for (int e = 0; e < N; ++e) top = fabsf(y[e]) < INFINITY ? fmaxf(top, fabsf(y[e])) : top;
     top = over_row<L>(top, most);
-    x = scale_of(top);
-    const float limit = x >= kTopScale ? 240.f : 448.f;
+    x = std::min(scale_of(top), kTopScale);
+    const float limit = x == kTopScale ? 240.f : 448.f;
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      z[e] = fabsf(y[e]) < kPast ? std::clamp(__builtin_ldexpf(y[e], -x), -limit, limit) : __builtin_nanf("");
+      z[e] = fabsf(y[e]) < INFINITY ? std::clamp(__builtin_ldexpf(y[e], -x), -limit, limit) : __builtin_nanf("");
   }
   code = static_cast<uint32_t>(x + 127);
 #pragma unroll

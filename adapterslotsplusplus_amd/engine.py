@@ -1045,7 +1045,8 @@ class WarpPipeEngine:
         and the values go to slots[token] of the cache (see write_cache), the
         turned queries are returned (q_out, new unless given; it may be q).  q
         may be None.  Keys go into a float8_e4m3fn cache without being rounded
-        to their own type first."""
+        to their own type first; finite ones past its range (two fp16 elements
+        of 60000 turn into 84852) count as its largest."""
         op = "rotate_into_cache"
         dtype = k.dtype
         dt = _DTYPES.get(dtype)

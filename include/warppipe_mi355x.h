@@ -449,8 +449,10 @@ int wp_rotate_heads(wp_engine* e, const wp_head_rows* q, const wp_head_rows* k, 
 /* The same in one launch with the keys going to slots[token] of the cache, and
  * the values v as they are (out of k and v, and v's norm, are not used).  Into an e4m3 cache a row (keys unrounded) is
  * divided by the smallest power of two s >= 2^-126 that brings its largest magnitude to
- * at most 448 and rounded to nearest even; magnitudes that would come back past
- * the dtype's range take the largest that does not, infinities and NaN become NaN.  A
+ * at most 448 and rounded to nearest even, finite magnitudes past the dtype's largest
+ * counting as that; magnitudes that would come back past
+ * the dtype's range take the largest that does not, infinities (fp32's, of a turned
+ * key) and NaN become NaN.  A
  * negative slot keeps no row; one past the cache is skipped and flagged (device
  * error 1).  Slots of one call must differ (else either row, or parts of both,
  * remain).  q may be NULL. */

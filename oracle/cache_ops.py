@@ -43,9 +43,11 @@ def e4m3(y):
 
 def quantise(rows, largest):
     """(values, scale exponents) of rows [..., dim] whose type's largest finite
-    value is `largest`: what a cache of e4m3 rows holds of them."""
+    value is `largest`: what a cache of e4m3 rows holds of them.  Finite
+    magnitudes past that one count as it."""
     x = rows.double()
     finite = x.isfinite()
+    x = torch.where(finite, x.clamp(-largest, largest), x)
     top = torch.where(finite, x.abs(), 0.0).amax(-1)
     e = torch.full(top.shape, -126, dtype=torch.int64)
     some = top > 0

@@ -53,3 +53,12 @@ def test_paged_attention_is_attention_over_the_gathered_rows():
     keys = rows[0][0][[0, 1] + list(range(13, 18))], rows[1][0][[0, 1] + list(range(13, 18))]
     one = mo.attention(q[:1], keys[0], keys[1], [1], [7], 0.3)
     assert torch.allclose(few[0][0], one[0][0])
+
+
+def test_magnitudes_past_the_range_count_as_its_end():
+    big = 65504.0
+    x = torch.tensor([[70000.0, 3.0], [-1e9, 3.0], [65504.0, 3.0], [math.inf, 57344.0], [-math.inf, 1e5]], dtype=torch.float64)
+    v, e = co.quantise(x, big)
+    assert e.tolist() == [8, 8, 8, 7, 8]
+    assert v[:3].tolist() == [[61440.0, 3.0], [-61440.0, 3.0], [61440.0, 3.0]]
+    assert torch.isnan(v[3:, 0]).all() and v[3:, 1].tolist() == [57344.0, 61440.0]
