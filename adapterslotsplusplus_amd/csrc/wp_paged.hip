@@ -576,8 +576,9 @@ __device__ __forceinline__ void run_tile(const PagedArgs& p, const Source<T, DP,
   auto refill = [&](int i) {
     const int done = (i - from) & (kHalf - 1);
     if (i - from < kHalf || done > 1) return;
+    // (No further than the last step: near 2^31 keys the ones past it have no number.)
     const int tid = thread_number(), first = i - done + kHalf;  // the first step to list
-    if (first >= to || tid >= kHalf * kEach) return;
+    if (tid >= std::min(kHalf, to - first) * kEach) return;
     const int key = it.key_of<kKeys>(first + tid / kEach) + tid % kEach * kGranule;
     if (done == 0) {
       page = page_of(p, it, key);

@@ -1132,7 +1132,7 @@ class WarpPipeEngine:
         head strides of q that are multiples of 8.  scale: dim ** -0.5 unless
         given.  Returns out [tokens, heads, dim], or (out, lse [tokens, heads] fp32)
         with return_lse; queries that see no key, and rows of no sequence, get 0 and
-        -inf.  Lengths past the table are cut to it; a page outside the cache that a
+        -inf.  Lengths past the table are cut to it (and to 2^31 - 256); a page outside the cache that a
         query sees counts as zeros and sets device error 1 (entries of pages that
         none sees, behind the windows, may hold anything); bounds must not fall (rows of such a call
         are unspecified)."""

@@ -488,7 +488,7 @@ typedef struct wp_sequences {
  * only the last `window` of them, and the first `sinks` of the sequence.  Grouped
  * heads, out, lse (or NULL) and rounding as wp_packed_attention's; queries that see no
  * key, and rows of no sequence, get 0 and -inf.  Lengths past the table are cut to
- * it; bounds that fall leave rows of that call unspecified.  A page outside the cache counts
+ * it, and to 2^31 - 256; bounds that fall leave rows of that call unspecified.  A page outside the cache counts
  * as keys and values of zero and is flagged (device error 1), if any query sees one of its
  * keys: entries of pages behind every window need not be valid.  e4m3 elements times
  * their row's factor are taken in dtype, where they are exact if that can hold them. */
