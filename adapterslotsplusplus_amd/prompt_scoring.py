@@ -55,6 +55,13 @@ def _positions(ends: Sequence[int], lens: Sequence[int], device) -> torch.Tensor
     return (torch.cat(parts) if parts else torch.zeros(0, dtype=torch.int64)).to(device)
 
 
+def _check_more(cache: str, had: Sequence[int], lens: Sequence[int]) -> None:
+    if len(lens) != len(had):
+        raise RuntimeError(f"{cache}: {len(lens)} sequences, the cache has {len(had)}")
+    if any(n < 0 for n in lens):
+        raise RuntimeError(f"{cache}: sequences grow by {list(lens)} tokens, none by fewer than 0")
+
+
 class PackedCache:
     """Keys and values of several sequences, packed one after the other: per
     layer [sum(lens), kv_heads, dim]."""
@@ -72,8 +79,7 @@ class PackedCache:
     def grow(self, lens: Sequence[int], device) -> None:
         """Makes room for lens[b] tokens more of sequence b: where the kept and
         the new rows of each layer go."""
-        if len(lens) != len(self.lens):
-            raise RuntimeError(f"PackedCache: {len(lens)} sequences, the cache has {len(self.lens)}")
+        _check_more("PackedCache", self.lens, lens)
         old, new, at, ends = [], [], 0, [0]
         for had, more in zip(self.lens, lens):
             old += range(at, at + had)
@@ -141,8 +147,7 @@ class PagedCache:
 
     def grow(self, lens: Sequence[int], device) -> None:
         """Takes the pages for lens[b] tokens more of sequence b."""
-        if len(lens) != len(self.lens):
-            raise RuntimeError(f"PagedCache: {len(lens)} sequences, the cache has {len(self.lens)}")
+        _check_more("PagedCache", self.lens, lens)
         size = self.page_size
         ends = [had + more for had, more in zip(self.lens, lens)]
         need = [-(-end // size) - len(table) for end, table in zip(ends, self.tables)]
@@ -275,6 +280,7 @@ class TenantDecoder:
         if sum(lens) != n or tenants.numel() != n or cu_seqlens.numel() != len(lens) + 1:
             raise RuntimeError(f"TenantDecoder: {n} tokens, {tenants.numel()} tenants, {cu_seqlens.numel()} bounds and "
                                f"lengths {list(lens)} do not go together")
+        _check_more(type(cache).__name__, cache.lens, lens)
         # The token after each one: none at a sequence's end.  (An empty
         # sequence names its neighbour's last token, which ends too.)
         after = torch.roll(ids, -1)

@@ -3,7 +3,7 @@ over one on an engine that computes on the CPU (no GPU)."""
 import pytest
 import torch
 
-from adapterslotsplusplus_amd.prompt_scoring import DecoderLayer, PagedCache, TenantDecoder
+from adapterslotsplusplus_amd.prompt_scoring import DecoderLayer, PackedCache, PagedCache, TenantDecoder
 from adapterslotsplusplus_amd.rotary import Rotary, frequencies
 from oracle import cache_ops as co
 from tests.test_prompt_scoring_steps_host import DIM, HEADS, KV, VOCAB, HostEngine, parts
@@ -161,3 +161,26 @@ def test_a_step_that_fails_gives_its_pages_back(refuse, message):
     engine.refuse = None
     more = parts(4, 3, 13)
     assert torch.equal(step(model, more, cache).logprobs, step(model, more, other).logprobs)
+
+
+@pytest.mark.parametrize("kind", ["packed", "paged"])
+def test_sequences_do_not_grow_by_fewer_than_no_tokens(kind):
+    """A negative length is refused before anything of the cache changes (its pages
+    would be handed out twice, or lost)."""
+    model = decoder(PagedHostEngine())
+    cache = model.paged_cache(2, pages=6, page_size=SIZE) if kind == "paged" else PackedCache(2, 2)
+    other = model.paged_cache(2, pages=6, page_size=SIZE)
+    for c in (cache, other):
+        step(model, parts(1, 33, 4), c)
+    ids = torch.cat(parts(2, 2))
+    kept = cache.state()
+    for lens in ([-1, 3], [3, -1]):
+        with pytest.raises(RuntimeError, match="none by fewer than 0"):
+            cache.grow(lens, "cpu")
+        with pytest.raises(RuntimeError, match="none by fewer than 0"):
+            model.verify(ids, torch.tensor([0, 2, 2], dtype=torch.int32), torch.tensor([-1, -1]), lens, cache)
+    assert cache.lens == [33, 4]
+    if kind == "paged":
+        assert cache.state()[:3] == kept[:3] and sorted([p for t in cache.tables for p in t] + cache.free) == list(range(6))
+    more = parts(3, 1, 14)
+    assert torch.allclose(step(model, more, cache).logprobs, step(model, more, other).logprobs, atol=1e-5)
