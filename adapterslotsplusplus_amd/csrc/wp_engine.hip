@@ -2793,15 +2793,24 @@ int check_slots(const char* who, const void* slots, int32_t slots64) {
 
 int run_rows(const char* who, wp_engine* e, HeadArgs& a, int64_t tokens, int32_t head_dim, float eps, int32_t dtype,
              void* stream, bool read = false) {
-  // A launch numbers its waves in 31 bits; none takes less than a token's head.
   const int64_t heads = static_cast<int64_t>(a.part[0].heads) + a.part[1].heads + a.part[2].heads;
   if (tokens * heads > 0x7FFFFFFF) return fail(WP_ERR_INVALID, "%s: %lld heads of all tokens (up to 2^31)", who, (long long)(tokens * heads));
   a.header = e->header;
-  a.tokens = tokens;
   a.dim = head_dim;
   a.eps = eps;
   DeviceGuard g(e->device);
-  WP_HIP((read ? launch_read_rows : launch_head_rows)(dtype == WP_DTYPE_BF16, a, e->n_cu, static_cast<hipStream_t>(stream)));
+  auto moved = [](const void* p, int64_t bytes) { return p ? static_cast<const char*>(p) + bytes : nullptr; };
+  for (int64_t done = 0; done < tokens; done += kMostRowTokens) {
+    HeadArgs b = a;
+    b.tokens = std::min(tokens - done, kMostRowTokens);
+    b.positions = moved(a.positions, done * (a.positions64 ? 8 : 4));
+    b.slots = moved(a.slots, done * (a.slots64 ? 8 : 4));
+    for (HeadPart& h : b.part) {
+      if (!read) h.x = moved(h.x, done * h.x_tok * 2);
+      if (read || !h.cached) h.y = const_cast<char*>(static_cast<const char*>(moved(h.y, done * h.y_tok * 2)));
+    }
+    WP_HIP((read ? launch_read_rows : launch_head_rows)(dtype == WP_DTYPE_BF16, b, e->n_cu, static_cast<hipStream_t>(stream)));
+  }
   return WP_OK;
 }
 

@@ -13,6 +13,9 @@
 namespace wp {
 
 constexpr int kMaxRowDim = 256;
+// Tokens of a launch: a grid has fewer than 2^32 threads, and so many tokens take at
+// most three waves each (one for each kind).
+constexpr int64_t kMostRowTokens = 1 << 24;
 constexpr int kMinPage = 16;  // a wave's 16-byte loads of one kind then touch one page each
 
 // The rows of one kind (queries, keys or values) of a launch: heads of each
