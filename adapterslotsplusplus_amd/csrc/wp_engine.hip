@@ -2648,7 +2648,20 @@ int wp_token_logprobs(wp_engine* e, float* logprobs, float* entropy, int32_t* ra
   a.part_bytes = kModelPartBytes;
   a.counters = e->model_cnt;
   a.n_counters = kModelCounters;
-  WP_HIP(launch_logprobs(a, e->n_cu, static_cast<hipStream_t>(stream)));
+  for (int64_t done = 0; done < rows; done += kMostLogprobRows) {
+    LogprobArgs b = a;
+    b.rows = std::min(rows - done, kMostLogprobRows);
+    b.logits = static_cast<const char*>(logits) + done * logits_row_stride * (dtype == WP_DTYPE_F32 ? 4 : 2);
+    b.ids = static_cast<const char*>(token_ids) + done * (ids_are_int64 ? 8 : 4);
+    b.logprobs += done;
+    b.entropy += done;
+    b.ranks += done;
+    if (top > 0) {
+      b.top_lp += done * top;
+      b.top_ids += done * top;
+    }
+    WP_HIP(launch_logprobs(b, e->n_cu, static_cast<hipStream_t>(stream)));
+  }
   return WP_OK;
 }
 

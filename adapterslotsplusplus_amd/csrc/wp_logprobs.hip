@@ -419,6 +419,7 @@ hipError_t launch(const LogprobArgs& a, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_logprobs(LogprobArgs& a, int n_cu, hipStream_t stream) {
+  static_assert(kMostLogprobRows * kRowThreads <= 0xFFFFFFFFll, "a grid has room for a workgroup each");
   // Rows enough for four workgroups a compute unit take one each; fewer are
   // shared by workgroups of at least one whole chunk.
   const int64_t n = a.dtype == 2 ? 4 : 8;
@@ -426,7 +427,7 @@ hipError_t launch_logprobs(LogprobArgs& a, int n_cu, hipStream_t stream) {
   const int64_t chunks = ((a.vocab + 2 * n - 2) / n + vecs - 1) / vecs;
   a.parts = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>({chunks, (4 * n_cu + a.rows - 1) / a.rows, kMaxParts})));
   if (a.rows > a.n_counters || static_cast<uint64_t>(a.rows) * a.parts * kPartBytes > a.part_bytes) a.parts = 1;
-  if (a.rows * a.parts > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (!grid_fits(a.rows * a.parts, kRowThreads)) return hipErrorInvalidValue;
   return a.dtype == 0 ? launch<_Float16>(a, stream) : a.dtype == 1 ? launch<__bf16>(a, stream) : launch<float>(a, stream);
 }
 

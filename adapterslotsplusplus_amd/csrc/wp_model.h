@@ -65,6 +65,9 @@ inline Divisor divisor_of(int d) {
   return r;
 }
 
+// A grid of 2^32 threads or more is cut to its low 32 bits, without an error.
+inline bool grid_fits(int64_t workgroups, int threads) { return workgroups * threads <= 0xFFFFFFFFll; }
+
 struct AttnArgs {
   const void* q;
   const void* k;
@@ -104,6 +107,7 @@ hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t s
 // negative id names no token: log probability and rank 0; an id past the
 // vocabulary counts as none and is flagged (kErrIdRange).  Strides in elements.
 constexpr int kMaxTop = 64;
+constexpr int64_t kMostLogprobRows = 1 << 22;  // of a launch
 struct LogprobArgs {
   const void* logits;
   const void* ids;
