@@ -777,6 +777,10 @@ hipError_t launch_attention(int dtype_bf16, AttnArgs& a, int n_cu, hipStream_t s
     a.split_rows = wide ? 0x7FFFFFFF : static_cast<int32_t>(slot);
   }
   if (tile_items + chunk_items > 0x7FFFFFFF) return hipErrorInvalidValue;
+  // (The roles share a launch if their workgroups are alike.)
+  const bool apart = tile_items == 0 || tile_waves != kChunkWaves;
+  if (!grid_fits(apart ? tile_items : tile_items + chunk_items, 64 * tile_waves) || !grid_fits(apart ? chunk_grid : 0, 64 * kChunkWaves))
+    return hipErrorInvalidValue;
   a.tile_items = static_cast<int32_t>(tile_items);
   a.chunk_items = static_cast<int32_t>(chunk_items);
   a.tile_shift = static_cast<int32_t>(tile_shift);

@@ -2526,7 +2526,9 @@ int wp_linear(wp_engine* e, void* y, int64_t y_row_stride, const void* x, int64_
   a.part_bytes = kModelPartBytes;
   a.tile_cnt = e->model_cnt;
   a.n_cnt = kModelCounters;
-  WP_HIP(launch_proj(dtype == WP_DTYPE_BF16, a, e->n_cu, static_cast<hipStream_t>(stream)));
+  const hipError_t rc = launch_proj(dtype == WP_DTYPE_BF16, a, e->n_cu, static_cast<hipStream_t>(stream));
+  if (rc == hipErrorInvalidValue) return fail(WP_ERR_INVALID, "%s: %lld tokens of %d outputs are too many for one call", who, (long long)T, d_out);
+  WP_HIP(rc);
   return WP_OK;
 }
 
@@ -2604,7 +2606,10 @@ int wp_packed_attention(wp_engine* e, void* out, const int64_t* out_strides, flo
   a.part_bytes = kModelPartBytes;
   a.counters = e->model_cnt;
   a.n_counters = kModelCounters;
-  WP_HIP(launch_attention(dtype == WP_DTYPE_BF16, a, e->n_cu, static_cast<hipStream_t>(stream)));
+  const hipError_t rc = launch_attention(dtype == WP_DTYPE_BF16, a, e->n_cu, static_cast<hipStream_t>(stream));
+  if (rc == hipErrorInvalidValue)
+    return fail(WP_ERR_INVALID, "%s: %lld tokens of %d heads in %d sequences are too many for one call", who, (long long)tokens, heads, n_seq);
+  WP_HIP(rc);
   return WP_OK;
 }
 

@@ -775,7 +775,7 @@ hipError_t launch_tiles(ProjArgs& a, hipStream_t stream) {
   a.tiles_t = static_cast<int32_t>((a.tokens + BT - 1) / BT);
   a.tiles_n = (a.n_out + outs - 1) / outs;
   const int64_t tiles = static_cast<int64_t>(a.tiles_t) * a.tiles_n;
-  if (tiles > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (!grid_fits(tiles, 64 * WT * WN)) return hipErrorInvalidValue;
   hipLaunchKernelGGL((proj_kernel<T, BT, BN, WT, WN, R, kAligned>), dim3(static_cast<uint32_t>(tiles)), dim3(64 * WT * WN), 0,
                      stream, a);
   return hipGetLastError();
@@ -790,7 +790,7 @@ hipError_t launch_cols(ProjArgs& a, int n_cu, hipStream_t stream) {
   // A tile's columns are split over workgroups only where tiles leave half of
   // the device idle: joining costs about 5 us.
   split_columns(a, tiles, n_cu, 4 * kColWaves * kColBlock, kFT * kFN * 1024);
-  if (tiles * a.splits > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (!grid_fits(tiles * a.splits, kColThreads)) return hipErrorInvalidValue;
   const dim3 grid(static_cast<uint32_t>(tiles * a.splits));
   if (a.gated) {
     if constexpr (kFN % 2 == 0)
