@@ -1281,7 +1281,7 @@ hipError_t launch_paged_attention(int dtype_bf16, PagedArgs& a, int n_cu, hipStr
   // of 512 98 and 121, 64 of 512 389 and 362, 32 of 400 151 and 138, 64 of 100 74 and 68,
   // 256 of 60 174 and 123).
   const int64_t all_tiles = (rows / kTileRows<true> + std::max(1, a.n_seq)) * a.kv_heads;
-  a.whole_tiles = tiles && rows / kTileRows<true> * a.kv_heads >= 3ll * a.n_wg && a.tokens >= 448ll * a.n_seq && all_tiles <= 0x7FFFFFFF ? static_cast<int32_t>(all_tiles) : 0;
+  a.whole_tiles = tiles && rows / kTileRows<true> * a.kv_heads >= 3ll * a.n_wg && a.tokens >= 448ll * a.n_seq && grid_fits(all_tiles, 64 * kTileWaves) ? static_cast<int32_t>(all_tiles) : 0;
   const int dp = a.dim <= 64 ? 64 : a.dim <= 96 ? 96 : 128;
   const uint64_t slots = 2ull * a.n_wg * (tiles ? kTileRows<true> : kTileRows<false>) * (dp + 2) * 4;
   if (slots > a.part_bytes || a.n_wg > a.n_counters) return hipErrorInvalidValue;

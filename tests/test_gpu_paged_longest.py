@@ -45,3 +45,20 @@ def test_lengths_up_to_31_bits(engine, tokens, small):
         assert engine.device_errors() == 0
         assert (out == 1).all()
         assert ((lse.double() - math.log(n)).abs() <= 2.0 ** -14).all()
+
+
+def test_more_row_tiles_than_a_grid_holds(engine):
+    """2^20 tokens of 2048 heads, each its own key head's: 2^24 row tiles, which
+    a grid of a workgroup each would not hold.  All but the last 16 tokens stand
+    before the first key."""
+    T, heads, dim = 1 << 20, 2048, 8
+    announce(f"paged {T} tokens of {heads} heads")
+    q = torch.ones(1, heads, dim, dtype=torch.bfloat16, device="cuda").expand(T, heads, dim)
+    k, v = (torch.full((1, 16, heads, dim), x, dtype=torch.bfloat16, device="cuda") for x in (0.0, 1.0))
+    out = torch.full((T, heads, dim), 3.0, dtype=torch.bfloat16, device="cuda")
+    cu, kv = (torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([0, T], [16]))
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    engine.paged_attention(q, k, v, table, cu, kv, out=out)
+    assert (out[-16:] == 1).all()
+    for part in out[:-16].split(1 << 16):
+        assert (part == 0).all()
