@@ -14,13 +14,15 @@ from typing import List, Mapping, Optional, Tuple
 import torch
 
 
-def _number(scaling: Mapping, name: str, kind: str) -> float:
+def _number(scaling: Mapping, name: str, kind: str, default: Optional[float] = None, positive: bool = True) -> float:
     v = scaling.get(name)
+    if v is None:
+        v = default
     if v is None:
         raise RuntimeError(f"Rotary: {kind} scaling needs {name!r}")
     v = float(v)
-    if not (math.isfinite(v) and v > 0):
-        raise RuntimeError(f"Rotary: {name} must be a positive number, got {v}")
+    if not (math.isfinite(v) and (v > 0 or not positive)):
+        raise RuntimeError(f"Rotary: {name} must be a {'positive' if positive else 'finite'} number, got {v}")
     return v
 
 
@@ -64,15 +66,14 @@ def frequencies(dim: int, base: float = 10000.0, scaling: Optional[Mapping] = No
         def pair(turns: float) -> float:  # the (fractional) index that turns so often over the trained length
             return dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-        low = max(math.floor(pair(float(scaling.get("beta_fast", 32.0)))), 0)
-        high = min(math.ceil(pair(float(scaling.get("beta_slow", 1.0)))), dim - 1)
+        low = max(math.floor(pair(_number(scaling, "beta_fast", kind, 32.0))), 0)
+        high = min(math.ceil(pair(_number(scaling, "beta_slow", kind, 1.0))), dim - 1)
         stretch = [min(max((i - low) / max(high - low, 0.001), 0.0), 1.0) for i in range(half)]
-        more = scaling.get("attention_factor")
-        more = float(more) if more is not None else 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+        more = _number(scaling, "attention_factor", kind, 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0, positive=False)
         return [f / factor * s + f * (1.0 - s) for f, s in zip(plain, stretch)], more
     if kind == "bands":
         length = _number(scaling, "original_length", kind)
-        low, high = float(scaling.get("low_freq_factor", 1.0)), float(scaling.get("high_freq_factor", 4.0))
+        low, high = (_number(scaling, n, kind, d, positive=False) for n, d in (("low_freq_factor", 1.0), ("high_freq_factor", 4.0)))
         if not high > low:
             raise RuntimeError("Rotary: high_freq_factor must be above low_freq_factor")
         keep = [min(max((length * f / (2 * math.pi) - low) / (high - low), 0.0), 1.0) for f in plain]

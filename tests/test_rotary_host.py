@@ -58,3 +58,17 @@ def test_turns_are_64_bit_fractions():
 def test_refusals(args):
     with pytest.raises(RuntimeError, match="Rotary"):
         frequencies(**args)
+
+
+@pytest.mark.parametrize("more", [dict(type="yarn", beta_fast=0), dict(type="yarn", beta_slow=-1), dict(type="yarn", beta_fast=math.nan),
+                                  dict(type="yarn", attention_factor=math.nan), dict(type="bands", low_freq_factor=-math.inf),
+                                  dict(type="bands", high_freq_factor=math.inf)], ids=str)
+def test_numbers_that_scale_nothing_are_refused(more):
+    with pytest.raises(RuntimeError, match="Rotary: .* must be a"):
+        frequencies(8, scaling=dict(factor=8.0, original_length=4096, **more))
+
+
+def test_numbers_left_empty_have_their_defaults():
+    for kind, names in (("yarn", ("beta_fast", "beta_slow", "attention_factor")), ("bands", ("low_freq_factor", "high_freq_factor"))):
+        some = dict(type=kind, factor=8.0, original_length=4096)
+        assert frequencies(64, scaling=dict(some, **{n: None for n in names})) == frequencies(64, scaling=some)
