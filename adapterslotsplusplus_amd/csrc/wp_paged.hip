@@ -135,6 +135,11 @@ __device__ __forceinline__ Cost cost_of(const PagedArgs& p, const Shape& s, int 
   c.stretches = 0;
   if (stretch > 0 && c.log_rows == 7 && s.n_k > s.n_q) {
     c.stretches = (s.n_k - s.n_q) / kTileKeys / stretch;
+    // What is left of a tile with stretches is a share of it, and often the one that joins
+    // them: some 20 us, 8 steps' time, 4 of them beyond a whole tile's start and end.  (16 x 128
+    // tokens over caches that leave 1 to 3 steps: 518 us without, as one workgroup had
+    // sixteen of those, 324.)
+    if (c.stretches > 0) c.extra += 256 * p.group;
     c.lag -= static_cast<long long>(c.stretches) * stretch * kTileKeys * p.group;
   }
   return c;
@@ -1061,9 +1066,10 @@ __global__ __launch_bounds__(64 * kWavesOf<kRoles>, 2) void paged_kernel(PagedAr
   // Chunks over caches of different lengths: stretches of keys as long as a share, from
   // the first key on, go to workgroups of their own, and the line is of what is left.
   // Those on the line have more ends and starts of items to do, so a stretch is ten steps
-  // longer than a share (4 x 512 tokens over 16384, 9577, 2048 and 14536 keys: 444 us
-  // with all on the line, 430 with stretches of a share, 416; 16 x 128 tokens 504 and
-  // 428).  Below shares of 64 steps there is nothing in it: 168 and 175 us at 55.
+  // longer than a share (4 x 512 tokens over 16384, 9577, 2048 and 14536 keys: 440 us
+  // with all on the line, 418; 16 x 128 tokens over four of each 492 and 436, over 256 to
+  // 16384 keys at random 359 and 324, 268 and 221, 291 and 250, 213 and 216).  Below shares of 64 steps there
+  // is nothing in it: 168 and 175 us at 55.
   int stretch = 0, whole = 0, mine_whole = 0;
   if ((kRoles & kTiles) != 0 && pieces == 0 && !whole_tiles && p.n_seq <= 64 && p.window == 0) {
     const float steps = ldexpf(static_cast<float>(share), p.cost_shift) * __builtin_amdgcn_rcpf(static_cast<float>(p.group * kTileKeys));
