@@ -69,10 +69,6 @@ struct Head {
   static __device__ __forceinline__ int value_swizzle(int r) { return kRow == 256 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
 };
 
-// n / d, exactly for n < 2^31: the product is under 2^63.
-__device__ __forceinline__ int over(int n, const Divisor& d) {
-  return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * d.magic) >> d.shift);
-}
 // The first key that a query at key position `pos` sees: with the windows the
 // host takes, up to 2^31 - 1, pos - window + 1 need not fit 32 bits.
 __device__ __forceinline__ int window_start(int pos, int window) {

@@ -44,10 +44,6 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kBatch = 4;  // rows of loads of a wave that are on their way together
 
-__device__ __forceinline__ uint32_t over(uint32_t n, const Divisor& d) {
-  return static_cast<uint32_t>((static_cast<uint64_t>(n) * d.magic) >> d.shift);
-}
-
 // Sum (or maximum) over the L lanes of a row, in every one of them.
 template <int L, typename F>
 __device__ __forceinline__ float over_row(float v, F f) {
@@ -147,8 +143,8 @@ __device__ __forceinline__ bool unit_of(const HeadArgs& p, Unit& u) {
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const uint32_t id = blockIdx.x * kWaves + wave;
   if (id >= p.n_units) return false;
-  const uint32_t tok = over(id, p.by_units);
-  int at = static_cast<int>(id - tok * static_cast<uint32_t>(p.units_tok));
+  const int tok = over(static_cast<int>(id), p.by_units);
+  int at = static_cast<int>(id) - tok * p.units_tok;
   u.tok = tok;
   u.kind = at < p.units[0] ? 0 : at < p.units[0] + p.units[1] ? 1 : 2;
   at -= u.kind == 0 ? 0 : u.kind == 1 ? p.units[0] : p.units[0] + p.units[1];
@@ -159,6 +155,27 @@ __device__ __forceinline__ bool unit_of(const HeadArgs& p, Unit& u) {
 // Entry i of int64 or int32 numbers.
 __device__ __forceinline__ int64_t number(const void* p, int wide, int64_t i) {
   return wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+}
+
+// Moves y, and scales with it, to where the token's rows of a kind go (mine: reads a
+// field of it).  False: its slot keeps none.
+template <typename F>
+__device__ __forceinline__ bool find_results(const HeadArgs& p, const Unit& u, int lane, F mine, bool cached, int64_t y_tok, char*& y,
+                                             uint8_t*& scales) {
+  if (!cached) {
+    y += u.tok * y_tok * 2;
+    return true;
+  }
+  const int64_t slot = number(p.slots, p.slots64, u.tok);
+  if (slot < 0) return false;
+  if (slot >= p.n_slots) {
+    if (lane == 0 && u.head0 == 0) flag_error(p.header, kErrIdRange);
+    return false;
+  }
+  const int64_t page = slot >> p.page_shift, at = slot & ((1ll << p.page_shift) - 1);
+  y += (page * mine([](const HeadPart& h) { return h.y_page; }) + at * y_tok) * (p.e4m3 != 0 ? 1 : 2);
+  if (p.e4m3 != 0) scales += page * mine([](const HeadPart& h) { return h.s_page; }) + at * mine([](const HeadPart& h) { return h.s_tok; });
+  return true;
 }
 
 // Rows whose halves lie in whole 16-byte vectors (and what does not rotate, too):
@@ -223,19 +240,7 @@ __global__ __launch_bounds__(64 * kWaves) void head_pairs_kernel(HeadArgs p) {
     const int64_t y_tok = mine([](const HeadPart& h) { return h.y_tok; }), y_head = mine([](const HeadPart& h) { return h.y_head; });
     const int64_t s_head = mine([](const HeadPart& h) { return h.s_head; });
     const bool small = cached && p.e4m3 != 0;
-    if (cached) {
-      const int64_t slot = number(p.slots, p.slots64, u.tok);
-      if (slot < 0) continue;
-      if (slot >= p.n_slots) {
-        if (lane == 0 && u.head0 == 0) flag_error(p.header, kErrIdRange);
-        continue;
-      }
-      const int64_t page = slot >> p.page_shift, at = slot & ((1ll << p.page_shift) - 1);
-      y += (page * mine([](const HeadPart& h) { return h.y_page; }) + at * y_tok) * (small ? 1 : 2);
-      if (small) scales += page * mine([](const HeadPart& h) { return h.s_page; }) + at * mine([](const HeadPart& h) { return h.s_tok; });
-    } else {
-      y += u.tok * y_tok * 2;
-    }
+    if (!find_results(p, u, lane, mine, cached, y_tok, y, scales)) continue;
     const int head0 = p.all ? 0 : u.head0, end = p.all ? heads : std::min(heads, head0 + p.steps * kRows);
     // Loads go a batch ahead, the first ones before the angles are worked out.
     constexpr int kAtOnce = 2;
@@ -360,19 +365,7 @@ __global__ __launch_bounds__(64 * kWaves) void head_rows_kernel(HeadArgs p) {
   const int64_t y_tok = mine([](const HeadPart& h) { return h.y_tok; }), y_head = mine([](const HeadPart& h) { return h.y_head; });
   const int64_t s_head = mine([](const HeadPart& h) { return h.s_head; });
   const bool small = cached && p.e4m3 != 0;
-  if (cached) {
-    const int64_t slot = number(p.slots, p.slots64, u.tok);
-    if (slot < 0) return;
-    if (slot >= p.n_slots) {
-      if (lane == 0 && u.head0 == 0) flag_error(p.header, kErrIdRange);
-      return;
-    }
-    const int64_t page = slot >> p.page_shift, at = slot & ((1ll << p.page_shift) - 1);
-    y += (page * mine([](const HeadPart& h) { return h.y_page; }) + at * y_tok) * (small ? 1 : 2);
-    if (small) scales += page * mine([](const HeadPart& h) { return h.s_page; }) + at * mine([](const HeadPart& h) { return h.s_tok; });
-  } else {
-    y += u.tok * y_tok * 2;
-  }
+  if (!find_results(p, u, lane, mine, cached, y_tok, y, scales)) return;
 
   // The lane's columns: sines, and where each one's partner is.
   const int rot = rotates ? p.rot : 0, half = rot >> 1;
@@ -494,8 +487,8 @@ __global__ __launch_bounds__(64 * kWaves) void head_rows_kernel(HeadArgs p) {
   }
 }
 
-// Rows of the cache, as the tensors' type: a factor outside fp32's normal
-// numbers (codes 0 and 255, which nothing here writes) gives zero and NaN.
+// Rows of the cache, as the tensors' type.  (Codes 0 and 255, which nothing here
+// writes, are no factors of fp32's normal numbers: what such rows give is not defined.)
 template <typename T, int L, bool kSmall>
 __global__ __launch_bounds__(64 * kWaves) void read_rows_kernel(HeadArgs p) {
   constexpr int kRows = 64 / L;

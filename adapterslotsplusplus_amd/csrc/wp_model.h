@@ -65,6 +65,11 @@ inline Divisor divisor_of(int d) {
   return r;
 }
 
+// n / d, exactly for n < 2^31: the product is under 2^63.
+__device__ __forceinline__ int over(int n, const Divisor& d) {
+  return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * d.magic) >> d.shift);
+}
+
 // A grid of 2^32 threads or more is cut to its low 32 bits, without an error.
 inline bool grid_fits(int64_t workgroups, int threads) { return workgroups * threads <= 0xFFFFFFFFll; }
 

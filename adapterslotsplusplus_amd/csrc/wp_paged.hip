@@ -475,9 +475,9 @@ __device__ __forceinline__ void mask_seen(const Rows<T, DP, kKind>& w, f32x16& s
   }
 }
 
-// What all rows of a wave see: every key of [low, pos], and of the first `sinks`; none past `last`.
+// What all rows of a wave see: every key of [low, pos], and of the first `sinks` up to pos.
 struct Sight {
-  int low, pos, last, sinks;
+  int low, pos, sinks;
   __device__ __forceinline__ bool whole(int at, int n) const { return at + n - 1 <= pos && (at >= low || at + n <= sinks); }
 };
 
@@ -751,11 +751,10 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
   }
   w.pos = real ? tok + lag : -1;
   w.low = window_start(tok + lag, p.window);
-  Sight see{0, -1, -1, p.sinks};
+  Sight see{0, -1, p.sinks};
   if (wave_row0 < it.row0 + it.rows) {
     const int t0 = over(wave_row0, p.by_group), t1 = std::min(it.s.n_q - 1, over(wave_row0 + kWaveRows - 1, p.by_group));
     see.pos = t0 + lag;
-    see.last = t1 + lag;
     see.low = window_start(t1 + lag, p.window);
   }
   const Source<T, DP, kSmall> in(p, list, scales, lane);
