@@ -12,11 +12,14 @@
 // tile (32 or 128 rows of a key head) in keys is a linear function of the tile, cut off
 // below and at the window, whose sum over a sequence has a closed form:
 //   - a line of all tiles' costs, cut into equal shares wherever that is;
-//   - where there are no more tiles than workgroups and it takes no longer, a line of equal
-//     pieces, one for each workgroup, that has no end of one tile and start of another in a
-//     share (one token over 8192 keys: 35.5 -> 20.9 us);
-//   - chunks over long caches: first stretches of whole shares (see there);
+//   - up to 64 sequences, where there are no more tiles than workgroups and it takes no
+//     longer, a line of equal pieces, one for each workgroup, that has no end of one tile and
+//     start of another in a share (one token over 8192 keys 20.3 us, 34.1 without);
+//   - up to 64 sequences' chunks over long caches: first stretches of whole shares (see there);
 //   - many row tiles: each whole, the ones with the most keys first (see the launcher).
+// 64 is where a lane holds a sequence; more share the one line (single tokens over 1 to 8192 keys,
+// 4 query heads a key head of 128, 64 and 65 of them: 25.4 and 32.5 us on one key head, 31.8 and
+// 35.8 on 2, 87.8 and 89.0 on 8; four chunks of 512 among 60 and 61 idle ones 403 and 426).
 // A tile that several workgroups share is joined by the last of them to finish (by a
 // counter of steps done), in a fixed order, so each key is read once for a tile, all
 // end at about the same time, and results repeat bit for bit.
@@ -25,8 +28,8 @@
 // time staged in LDS for all of them.  Up to 32 rows (single tokens, drafted
 // tokens): the waves share out the keys, 32 at a time.  Launches whose sequences have no
 // more rows than that on the whole have workgroups of two waves, twice as many of them: 64 single
-// tokens over 1 to 8192 keys, 32 heads over 8 of 128, 89 us, and 100 in workgroups of
-// four; 64 of 8 tokens 106 and 117 (and see the launcher).
+// tokens over 1 to 8192 keys, 32 heads over 8 of 128, 85.5 us, and 98.6 in workgroups of
+// four (and see the launcher).
 //
 // Keys and values go from their pages straight to LDS; in 8 bits they pass through
 // registers, one tile ahead, and become the queries' type on their way to LDS (a power
@@ -36,11 +39,12 @@
 // buffers' descriptions, by lanes side by side, well before they are loaded: the tables'
 // latency and the address arithmetic are off the path.
 //
-// What bounds it (32 heads over 8 of 128, bf16).  Single tokens: HBM, 64 over 8192 keys
-// each at 5.7 TB/s; over 1 to 8192 keys 85 us at 4.1 TB/s; 8-bit rows 5.2 TB/s (208 us),
-// near the conversions' rate.  Few: the chain from launch to join, 14.5 us over 777 keys.
-// Chunks: matrix and vector units as in wp_attn.hip, 2048 tokens over 16384 keys 495 us
-// (1.04 PF/s), in 8 bits 540: converting there takes the wave's own slots.
+// What bounds it (32 heads over 8 of 128, bf16; over several cards).  Single tokens: HBM,
+// 64 over 8192 keys each 381 to 388 us (5.6 TB/s), over 1 to 8192 keys 81 to 87 (4.1 to 4.3);
+// 64 over 8192 keys in 8 bits 207 to 209 (5.2), near the conversions' rate.  Few: the
+// chain from launch to join, 13.6 to 14.5 us over 777 keys.  Chunks: matrix and vector units as in
+// wp_attn.hip, 2048 tokens over 16384 keys 489 to 504 us (1.02 to 1.05 PF/s), in 8 bits 528
+// to 540: converting there takes the wave's own slots.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -652,7 +656,8 @@ __device__ __forceinline__ void run_tile(const PagedArgs& p, const Source<T, DP,
   };
   // Of two workgroups on a compute unit the older one goes first wherever both can, and the
   // younger one ends 17% later, alone at the end (4 x 512 tokens over 10636 keys each).  So each
-  // has the right of way half of the time, by the clock: 4% (16384 keys, 2048 tokens: 1%).
+  // has the right of way half of the time, by the clock (us, with and without: 2048 tokens over
+  // 16384 keys 503 and 507, 4 x 512 over 16384, 9577, 2048 and 14536 418 and 423, over 8192 each 279 and 281).
   const uint32_t young = blockIdx.x >= (static_cast<uint32_t>(p.n_wg) >> 1);
   for (int i = from; i < to; i += 2) {
     if ((((static_cast<uint32_t>(__builtin_readcyclecounter()) >> 13) ^ young) & 1u) != 0)
@@ -958,7 +963,7 @@ __device__ __forceinline__ void run_item(const PagedArgs& p, Shared& sh, Listed*
   };
   if constexpr (kTile)
     join(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
-  else if (places > kThreads)  // 48 requests of up to 5 tokens, 8 heads a key head of 64: 28.5 us by the other form, 23.8
+  else if (places > kThreads)  // 48 requests of up to 5 tokens, 8 heads a key head of 64: 24 us, 28.5 by the other form
     join(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
   else
     join(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
@@ -1270,9 +1275,12 @@ hipError_t launch_paged_attention(int dtype_bf16, PagedArgs& a, int n_cu, hipStr
   const int64_t rows = a.tokens * a.group;
   // Sequences of few rows on the whole run on key chunks, in tiles of 32 rows.
   // Few sequences of many such rows, though, in workgroups of four waves, as row tiles are: half
-  // as many shares of each to join (us, in four and in two, 32 heads over 8 of 128: 4 of 8
-  // tokens 41 and 48, 16 of 6 59 and 69, 32 of 8 100 and 107; 64 of 8 117 and 106, 16 of 4 58
-  // and 60, 4 of 4 40 and 35; heads of 64, 4 of 4 tokens 29 and 24).
+  // as many shares of each to join (us, in four and in two, 32 heads over 8 of 128, caches of
+  // 33 to 8192 keys at random: 4 of 8 tokens 40 and 41, 16 of 6 40 and 58, 32 of 8 72 and 81; 64
+  // of 8 155 and 142, 200 of 3 317 and 289, 64 of 1 140 and 122, 16 of 4 41 and 44, 4 of 4 39 and 30).
+  // Many over caches of one length would gain 1 to 20% by four (64 of 8 over 500, 2048 and 8192
+  // keys 35 and 44, 115 and 125, 373 and 389; 4 of 4 over 2048 30 and 37, heads of 64 18 and 32), but
+  // the lengths are on the device.
   const bool few = a.dim > 64 && rows >= 24ll * a.n_seq && static_cast<int64_t>(a.n_seq) * a.kv_heads <= n_cu;
   const bool tiles = few || rows > static_cast<int64_t>(kWaveRows) * std::max(1, a.n_seq);
   a.chunk_rows = tiles ? kWaveRows : 0x7FFFFFFF;
@@ -1282,9 +1290,9 @@ hipError_t launch_paged_attention(int dtype_bf16, PagedArgs& a, int n_cu, hipStr
   a.by_heads = divisor_of(a.kv_heads);
   // Row tiles that may run whole: where there are some for each workgroup, and sequences
   // are not short ones, whose tiles' starts take the most of it (us, whole and in shares; 32
-  // heads over 8 of 128: a prompt of 16384 tokens 2132 and 2253, 8 of 2048 385 and 441, 16
-  // of 512 98 and 121, 64 of 512 389 and 362, 32 of 400 151 and 138, 64 of 100 74 and 68,
-  // 256 of 60 174 and 123).
+  // heads over 8 of 128: a prompt of 16384 tokens 2095 and 2411, 8 of 2048 372 and 433, 16
+  // of 512 97 and 123, 64 of 512 384 and 357, 32 of 400 151 and 139, 64 of 100 69 and 65,
+  // 256 of 60 165 and 127).
   const int64_t all_tiles = (rows / kTileRows<true> + std::max(1, a.n_seq)) * a.kv_heads;
   a.whole_tiles = tiles && rows / kTileRows<true> * a.kv_heads >= 3ll * a.n_wg && a.tokens >= 448ll * a.n_seq && grid_fits(all_tiles, 64 * kTileWaves) ? static_cast<int32_t>(all_tiles) : 0;
   const int dp = a.dim <= 64 ? 64 : a.dim <= 96 ? 96 : 128;

@@ -1074,7 +1074,8 @@ class WarpPipeEngine:
         """Rows k and v [tokens, kv_heads, dim] to slots[token] (int32 or int64) of
         the cache, which is k_pages and v_pages [pages, page_size, kv_heads, dim]
         (page_size a power of two from 16 on; any page, token and head strides:
-        pages may lie head by head); slot s is token s % page_size of page s //
+        pages may lie head by head; dim up to 256, of which paged_attention
+        reads 128); slot s is token s % page_size of page s //
         page_size.  Pages have the rows' type, or are float8_e4m3fn with k_scales
         and v_scales [pages, page_size, kv_heads] uint8: a row's elements are then
         e4m3 * 2^(byte - 127), the smallest such power that brings the row's largest

@@ -427,7 +427,9 @@ typedef struct wp_rotation {
  * row of head h of slot s is at k + (s / page_size) * strides[0] + (s % page_size)
  * * strides[1] + h * strides[2], head_dim contiguous elements of the calls'
  * dtype or, with e4m3, bytes (strides then multiples of 16, as head_dim), with
- * a byte b in the scales for each row: its elements are e4m3 * 2^(b - 127). */
+ * a byte b of 1 to 254 in the scales for each row: its elements are e4m3 * 2^(b - 127)
+ * (what rows with other bytes give is not defined).  Heads of up to 256 can be
+ * kept, wp_paged_attention reads those of up to 128. */
 typedef struct wp_pages {
   void* k;
   void* v;
